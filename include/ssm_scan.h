@@ -28,7 +28,7 @@
 extern "C" {
 #endif
 
-#define SSM_ABI_VERSION 8
+#define SSM_ABI_VERSION 9
 
 enum { SSM_OK = 0, SSM_EINVAL = 1, SSM_EKEY = 2, SSM_ESPACE = 3, SSM_EHIP = 4 };
 
@@ -378,6 +378,76 @@ typedef struct ssm_norm_args {
   int64_t workspace_bytes;
 } ssm_norm_args;
 
+/* ------------------------------------------------------------------ gated delta rule
+ * No counterpart in the reference: a recurrence with a matrix state, S (Dk, Dv) per batch row and
+ * value head, key head = value head / (heads / key_heads):
+ *   S' = e^{g_t} S_{t-1},  u_t = beta_t (v_t - S'^T k_t),  S_t = S' + k_t u_t^T,  o_t = scale S_t^T q_t.
+ * With qk_norm, q and k are first divided by sqrt(sum of squares + 1e-6) of their rows.  g is a log
+ * decay (<= 0; -inf resets the state), beta in dtype, or in float32 with beta_f32.  q, k, v, out and their gradients have
+ * unit stride in the last dimension and any strides elsewhere; `stride` holds those of (batch, token,
+ * head).  States are float32 and contiguous.  key_dim <= SSM_DELTA_MAX_KEY.  Backward and forward share
+ * the struct; every sum runs in a fixed order. */
+#define SSM_DELTA_MAX_KEY 128
+typedef struct ssm_delta_args {
+  int64_t batch, seqlen, key_heads, heads, key_dim, value_dim;
+  int32_t dtype;           /* SSM_F32, SSM_BF16 or SSM_F16: q, k, v, out, dout, dq, dk, dv */
+  int32_t beta_f32;        /* nonzero: beta and dbeta are float32; 0: dtype */
+  int32_t qk_norm;
+  float scale;
+  ssm_tensor q, k;         /* (B,L,key_heads,key_dim) */
+  ssm_tensor v;            /* (B,L,heads,value_dim) */
+  ssm_tensor g;            /* (B,L,heads) float32 */
+  ssm_tensor beta;         /* (B,L,heads) */
+  const float *h0;         /* (B,heads,key_dim,value_dim), optional: zeros */
+  ssm_tensor out;          /* forward: (B,L,heads,value_dim) */
+  float *last;             /* forward: (B,heads,key_dim,value_dim), optional */
+  void *saved;             /* ssm_delta_saved_bytes(): written by the forward when given, read by the
+                              backward (every chunk's entering state and corrected values) */
+  ssm_tensor dout;         /* backward: as out */
+  const float *dlast;      /* backward: as last, optional */
+  ssm_tensor dq, dk, dv;   /* backward: as q, k, v */
+  ssm_tensor dg, dbeta;    /* backward: as g, beta */
+  float *dh0;              /* backward: as h0, optional */
+  void *workspace;         /* ssm_delta_fwd_workspace_bytes() / ssm_delta_bwd_workspace_bytes() */
+  int64_t workspace_bytes;
+} ssm_delta_args;
+
+/* One token of the same recurrence per batch row, the state updated in place. `stride` of q, k, v, g,
+ * beta and out holds those of (batch, head). */
+typedef struct ssm_delta_step_args {
+  int64_t batch, key_heads, heads, key_dim, value_dim;
+  int32_t dtype, beta_f32, qk_norm;
+  float scale;
+  ssm_tensor q, k;         /* (B,key_heads,key_dim) */
+  ssm_tensor v;            /* (B,heads,value_dim) */
+  ssm_tensor g, beta;      /* (B,heads) */
+  float *h;                /* (B,heads,key_dim,value_dim), read and updated in place */
+  ssm_tensor out;          /* (B,heads,value_dim) */
+} ssm_delta_step_args;
+
+/* ------------------------------------------------------------------ grouped norm
+ * No counterpart in the reference: the per-head norm of a multi-head recurrence's output with its
+ * gate.  Per row and group of `group_size` channels, statistics and arithmetic in float32:
+ *   z = (x - mean) / sqrt(variance + eps) * weight + bias     (center = 0: x / sqrt(mean(x^2) + eps) ...)
+ *   y = z, silu(z) (SSM_GNORM_SILU) or z silu(gate) (SSM_GNORM_GATE).
+ * Rows have unit column stride; group_size <= SSM_GNORM_MAX_GROUP. */
+#define SSM_GNORM_MAX_GROUP 1024
+enum { SSM_GNORM_NONE = 0, SSM_GNORM_SILU = 1, SSM_GNORM_GATE = 2 };
+typedef struct ssm_gnorm_args {
+  int64_t rows, groups, group_size;
+  int32_t dtype;           /* SSM_F32, SSM_BF16 or SSM_F16: x, gate, out, dout, dx, dgate */
+  int32_t activation, center, reserved0;
+  double eps;
+  ssm_tensor x, gate;      /* (rows, groups * group_size): stride[0] = row stride, stride[1] = 1 */
+  const float *weight, *bias;  /* (groups * group_size,), optional: ones, zeros */
+  ssm_tensor out;          /* forward */
+  ssm_tensor dout;         /* backward */
+  ssm_tensor dx, dgate;    /* backward; dgate iff gate */
+  float *dweight, *dbias;  /* backward: (groups * group_size,), optional */
+  void *workspace;         /* backward: ssm_gnorm_workspace_bytes() */
+  int64_t workspace_bytes;
+} ssm_gnorm_args;
+
 /* ------------------------------------------------------------------ entry points */
 int ssm_abi_version(void);
 const char *ssm_last_error(void);
@@ -394,6 +464,9 @@ int ssm_cscan_check(const ssm_cscan_args *args);
 int ssm_disc_check(const ssm_disc_args *args);
 int ssm_conv_check(const ssm_conv_args *args);
 int ssm_norm_check(const ssm_norm_args *args);
+int ssm_delta_check(const ssm_delta_args *args);
+int ssm_delta_step_check(const ssm_delta_step_args *args);
+int ssm_gnorm_check(const ssm_gnorm_args *args);
 
 /* Buffer sizes in bytes (host-only). */
 int64_t ssm_fwd_saved_bytes(const ssm_fwd_args *args);
@@ -406,6 +479,10 @@ int64_t ssm_cscan_workspace_bytes(const ssm_cscan_args *args);   /* backward */
 int64_t ssm_disc_workspace_bytes(const ssm_disc_args *args);
 int64_t ssm_conv_workspace_bytes(const ssm_conv_args *args);
 int64_t ssm_norm_workspace_bytes(const ssm_norm_args *args);
+int64_t ssm_delta_saved_bytes(const ssm_delta_args *args);
+int64_t ssm_delta_fwd_workspace_bytes(const ssm_delta_args *args);
+int64_t ssm_delta_bwd_workspace_bytes(const ssm_delta_args *args);
+int64_t ssm_gnorm_workspace_bytes(const ssm_gnorm_args *args);   /* backward */
 int64_t ssm_decode_stack_workspace_bytes(const ssm_decode_stack_args *args);
 /* Byte offset inside the decode-stack workspace of an int32 status word: ssm_decode_stack sets
  * it to 1 when a token id lies outside [0, vocab) (the reference's nn.Embedding,
@@ -431,6 +508,11 @@ int ssm_conv_fwd(const ssm_conv_args *args, void *stream);
 int ssm_conv_bwd(const ssm_conv_args *args, void *stream);
 int ssm_norm_fwd(const ssm_norm_args *args, void *stream);   /* models/common.py:14-16 */
 int ssm_norm_bwd(const ssm_norm_args *args, void *stream);   /* autograd of :14-16 */
+int ssm_delta_fwd(const ssm_delta_args *args, void *stream);
+int ssm_delta_bwd(const ssm_delta_args *args, void *stream);
+int ssm_delta_step(const ssm_delta_step_args *args, void *stream);
+int ssm_gnorm_fwd(const ssm_gnorm_args *args, void *stream);
+int ssm_gnorm_bwd(const ssm_gnorm_args *args, void *stream);
 
 /* ssm_fwd without allocation.  No counterpart in the reference: for callers that cannot
  * allocate device memory (code under HIP graph capture, tight serving loops, harnesses that

@@ -6,11 +6,13 @@
 // stream is synchronized.  One file-scope device array (`scratch`, below) serves the
 // allocation-free forward ssm_fwd_noalloc.
 #include <algorithm>
+#include <initializer_list>
 #include <math.h>
 #include <mutex>
 #include <stdarg.h>
 #include <stdio.h>
 #include <string.h>
+#include <utility>
 
 #include "../../include/ssm_scan.h"
 #include "ssm_internal.hpp"
@@ -1154,6 +1156,225 @@ int ssm_norm_bwd(const ssm_norm_args *a, void *stream) {
   p.ws = a->workspace;
   hipError_t e = launch_norm(p, a->dtype, true, (hipStream_t)stream);
   return e == hipSuccess ? ok() : hip_fail(e, "ssm_norm_bwd");
+}
+
+// ------------------------------------------------------------------ gated delta rule
+static_assert(SSM_DELTA_MAX_KEY == kDeltaMaxK && SSM_GNORM_MAX_GROUP == kGnormMaxGroup, "the header's limits");
+// What the chunked form and the step share.
+static int delta_common(int64_t B, int64_t Hk, int64_t H, int64_t Dk, int64_t Dv, int dtype, float scale) {
+  if (dtype != SSM_F32 && dtype != SSM_BF16 && dtype != SSM_F16)
+    return fail(SSM_EINVAL, "the gated delta rule takes float32, bfloat16 or float16");
+  if (B < 1 || Hk < 1 || H < 1 || Dk < 1 || Dv < 1)
+    return fail(SSM_EINVAL, "empty problem: batch=%lld key_heads=%lld heads=%lld key_dim=%lld value_dim=%lld",
+                (long long)B, (long long)Hk, (long long)H, (long long)Dk, (long long)Dv);
+  if (Dk > kDeltaMaxK) return fail(SSM_EINVAL, "key_dim=%lld > %d is not supported", (long long)Dk, kDeltaMaxK);
+  if (H % Hk) return fail(SSM_EINVAL, "heads=%lld is not a multiple of key_heads=%lld", (long long)H, (long long)Hk);
+  if (!(scale - scale == 0.0f)) return fail(SSM_EINVAL, "scale must be finite");
+  if (H > (1 << 24) || Dv > (1 << 24) || B > (1LL << 31) || B * H * cdiv(Dv, 16) >= (1LL << 31))
+    return fail(SSM_EINVAL, "batch * heads * value_dim is too large: %lld x %lld x %lld", (long long)B, (long long)H,
+                (long long)Dv);
+  return ok();
+}
+static int need(std::initializer_list<std::pair<const void *, const char *>> ps) {
+  for (const auto &p : ps)
+    if (!p.first) return fail(SSM_EINVAL, "required tensor '%s' is missing", p.second);
+  return ok();
+}
+// Eight elements of a row load as 16-byte words: base and strides are whole words.
+static int rows16(const ssm_tensor &t, int64_t width, int dtype) {
+  const int64_t e = dtype == SSM_F32 ? 4 : 8;
+  return (uintptr_t)t.data % 16 == 0 && width % 8 == 0 && t.stride[0] % e == 0 && t.stride[1] % e == 0 &&
+         t.stride[2] % e == 0;
+}
+
+int ssm_delta_check(const ssm_delta_args *a) {
+  if (!a) return fail(SSM_EINVAL, "null args");
+  int rc = delta_common(a->batch, a->key_heads, a->heads, a->key_dim, a->value_dim, a->dtype, a->scale);
+  if (rc) return rc;
+  if (a->seqlen < 1) return fail(SSM_EINVAL, "empty problem: seqlen=%lld", (long long)a->seqlen);
+  if (a->seqlen > (1LL << 31) || a->batch * a->heads * cdiv(a->seqlen, kDeltaChunk) >= (1LL << 31))
+    return fail(SSM_EINVAL, "batch * heads * seqlen is too large: %lld x %lld x %lld", (long long)a->batch,
+                (long long)a->heads, (long long)a->seqlen);
+  return need({{a->q.data, "q"}, {a->k.data, "k"}, {a->v.data, "v"}, {a->g.data, "g"}, {a->beta.data, "beta"}});
+}
+
+namespace {
+struct DeltaLayout {
+  int64_t states, u, T, rows;  // bytes of one array, 256-byte multiples
+};
+DeltaLayout delta_layout(const ssm_delta_args *a) {
+  const int64_t n = a->batch * a->heads * cdiv(a->seqlen, kDeltaChunk);
+  return {align256(n * a->key_dim * a->value_dim * 4), align256(n * kDeltaChunk * a->value_dim * 4),
+          align256(n * delta_mid_parts(a->dtype) * kDeltaChunk * kDeltaChunk * 2), align256(n * kDeltaRows * 4)};
+}
+DeltaParams delta_params(const ssm_delta_args *a) {
+  DeltaParams p{};
+  p.B = a->batch; p.L = a->seqlen;
+  p.Hk = (int)a->key_heads; p.H = (int)a->heads; p.Dk = (int)a->key_dim; p.Dv = (int)a->value_dim;
+  p.NC = (int)cdiv(a->seqlen, kDeltaChunk);
+  p.qk_norm = a->qk_norm;
+  p.beta32 = a->beta_f32;
+  p.scale = a->scale;
+  p.q = kv(a->q); p.k = kv(a->k); p.v = kv(a->v); p.g = kv(a->g); p.beta = kv(a->beta);
+  p.vq = rows16(a->q, a->key_dim, a->dtype);
+  p.vk = rows16(a->k, a->key_dim, a->dtype);
+  p.vv = rows16(a->v, a->value_dim, a->dtype);
+  const DeltaLayout l = delta_layout(a);
+  char *ws = (char *)a->workspace;
+  p.fT = ws;
+  p.fP = ws + l.T;
+  p.rows = (float *)(ws + 2 * l.T);
+  p.dstates = (float *)(ws + 2 * l.T + l.rows);
+  p.dr = (float *)(ws + 2 * l.T + l.rows + l.states);
+  if (a->saved) {
+    p.states = (float *)a->saved;
+    p.u = (float *)((char *)a->saved + l.states);
+  }
+  return p;
+}
+}  // namespace
+
+int64_t ssm_delta_saved_bytes(const ssm_delta_args *a) {
+  if (ssm_delta_check(a)) return -1;
+  const DeltaLayout l = delta_layout(a);
+  return l.states + l.u;
+}
+int64_t ssm_delta_fwd_workspace_bytes(const ssm_delta_args *a) {
+  if (ssm_delta_check(a)) return -1;
+  const DeltaLayout l = delta_layout(a);
+  return 2 * l.T + l.rows;
+}
+int64_t ssm_delta_bwd_workspace_bytes(const ssm_delta_args *a) {
+  if (ssm_delta_check(a)) return -1;
+  const DeltaLayout l = delta_layout(a);
+  return 2 * l.T + l.rows + l.states + l.u;
+}
+
+int ssm_delta_fwd(const ssm_delta_args *a, void *stream) {
+  int rc = ssm_delta_check(a);
+  if (!rc) rc = need({{a->out.data, "out"}});
+  if (rc) return rc;
+  const int64_t bytes = ssm_delta_fwd_workspace_bytes(a);
+  if (!a->workspace || a->workspace_bytes < bytes)
+    return fail(SSM_ESPACE, "workspace of %lld bytes required", (long long)bytes);
+  DeltaParams p = delta_params(a);
+  p.o = kv(a->out);
+  p.h0 = a->h0;
+  p.last = a->last;
+  hipError_t e = launch_delta_fwd(p, a->dtype, (hipStream_t)stream);
+  return e == hipSuccess ? ok() : hip_fail(e, "ssm_delta_fwd");
+}
+
+int ssm_delta_bwd(const ssm_delta_args *a, void *stream) {
+  int rc = ssm_delta_check(a);
+  if (!rc)
+    rc = need({{a->saved, "saved"}, {a->dout.data, "dout"}, {a->dq.data, "dq"}, {a->dk.data, "dk"}, {a->dv.data, "dv"},
+               {a->dg.data, "dg"}, {a->dbeta.data, "dbeta"}});
+  if (rc) return rc;
+  const int64_t bytes = ssm_delta_bwd_workspace_bytes(a);
+  if (!a->workspace || a->workspace_bytes < bytes)
+    return fail(SSM_ESPACE, "workspace of %lld bytes required", (long long)bytes);
+  DeltaParams p = delta_params(a);
+  p.dout = kv(a->dout); p.dq = kv(a->dq); p.dk = kv(a->dk); p.dv = kv(a->dv); p.dg = kv(a->dg); p.dbeta = kv(a->dbeta);
+  p.vdo = rows16(a->dout, a->value_dim, a->dtype);
+  p.dlast = a->dlast;
+  p.dh0 = a->dh0;
+  hipError_t e = launch_delta_bwd(p, a->dtype, (hipStream_t)stream);
+  return e == hipSuccess ? ok() : hip_fail(e, "ssm_delta_bwd");
+}
+
+int ssm_delta_step_check(const ssm_delta_step_args *a) {
+  if (!a) return fail(SSM_EINVAL, "null args");
+  int rc = delta_common(a->batch, a->key_heads, a->heads, a->key_dim, a->value_dim, a->dtype, a->scale);
+  if (rc) return rc;
+  return need({{a->q.data, "q"}, {a->k.data, "k"}, {a->v.data, "v"}, {a->g.data, "g"}, {a->beta.data, "beta"},
+               {a->h, "h"}, {a->out.data, "out"}});
+}
+int ssm_delta_step(const ssm_delta_step_args *a, void *stream) {
+  int rc = ssm_delta_step_check(a);
+  if (rc) return rc;
+  DeltaStepParams p{};
+  p.B = (int)a->batch; p.Hk = (int)a->key_heads; p.H = (int)a->heads; p.Dk = (int)a->key_dim; p.Dv = (int)a->value_dim;
+  p.qk_norm = a->qk_norm;
+  p.beta32 = a->beta_f32;
+  p.scale = a->scale;
+  p.q = kv(a->q); p.k = kv(a->k); p.v = kv(a->v); p.g = kv(a->g); p.beta = kv(a->beta); p.o = kv(a->out);
+  p.h = a->h;
+  hipError_t e = launch_delta_step(p, a->dtype, (hipStream_t)stream);
+  return e == hipSuccess ? ok() : hip_fail(e, "ssm_delta_step");
+}
+
+// ------------------------------------------------------------------ grouped norm
+static int gnorm_view(const ssm_tensor &t, const char *name) {
+  if (!has(t)) return fail(SSM_EINVAL, "required tensor '%s' is missing", name);
+  if (t.stride[1] != 1) return fail(SSM_EINVAL, "%s must have unit column stride", name);
+  return ok();
+}
+int ssm_gnorm_check(const ssm_gnorm_args *a) {
+  if (!a) return fail(SSM_EINVAL, "null args");
+  if (a->dtype != SSM_F32 && a->dtype != SSM_BF16 && a->dtype != SSM_F16)
+    return fail(SSM_EINVAL, "the grouped norm takes float32, bfloat16 or float16");
+  if (a->rows < 1 || a->groups < 1 || a->group_size < 1)
+    return fail(SSM_EINVAL, "empty grouped norm: rows=%lld groups=%lld group_size=%lld", (long long)a->rows,
+                (long long)a->groups, (long long)a->group_size);
+  if (a->group_size > kGnormMaxGroup)
+    return fail(SSM_EINVAL, "group_size=%lld > %d is not supported", (long long)a->group_size, kGnormMaxGroup);
+  if (a->groups > (1 << 20) || a->rows >= (1LL << 31) || a->rows * a->groups >= (1LL << 31))
+    return fail(SSM_EINVAL, "rows * groups is too large: %lld x %lld", (long long)a->rows, (long long)a->groups);
+  if (a->activation < SSM_GNORM_NONE || a->activation > SSM_GNORM_GATE)
+    return fail(SSM_EINVAL, "unknown activation %d", a->activation);
+  if (!(a->eps >= 0.0)) return fail(SSM_EINVAL, "eps must be >= 0");
+  int rc = gnorm_view(a->x, "x");
+  if (!rc && a->activation == SSM_GNORM_GATE) rc = gnorm_view(a->gate, "gate");
+  return rc ? rc : ok();
+}
+int64_t ssm_gnorm_workspace_bytes(const ssm_gnorm_args *a) {
+  if (ssm_gnorm_check(a)) return -1;
+  const int64_t C = a->groups * a->group_size;
+  return align256(((a->dweight != nullptr) + (a->dbias != nullptr)) * gnorm_slots(a->rows, C) * C * 4);
+}
+static GnormParams gnorm_params(const ssm_gnorm_args *a) {
+  GnormParams p{};
+  p.R = a->rows;
+  p.G = (int)a->groups; p.n = (int)a->group_size; p.center = a->center; p.act = a->activation;
+  p.eps = (float)a->eps;
+  p.x = a->x.data; p.sx = a->x.stride[0];
+  p.gate = a->gate.data; p.sg = a->gate.stride[0];
+  p.w = a->weight; p.b = a->bias;
+  const int64_t e = a->dtype == SSM_F32 ? 4 : 8;
+  auto whole = [&](const ssm_tensor &t) {
+    return !has(t) || ((uintptr_t)t.data % 16 == 0 && (a->rows == 1 || t.stride[0] % e == 0));
+  };
+  p.vec = p.n % e == 0 && (uintptr_t)p.w % 16 == 0 && (uintptr_t)p.b % 16 == 0 && whole(a->x) && whole(a->gate) &&
+          whole(a->out) && whole(a->dout) && whole(a->dx) && whole(a->dgate);
+  return p;
+}
+int ssm_gnorm_fwd(const ssm_gnorm_args *a, void *stream) {
+  int rc = ssm_gnorm_check(a);
+  if (!rc) rc = gnorm_view(a->out, "out");
+  if (rc) return rc;
+  GnormParams p = gnorm_params(a);
+  p.y = a->out.data; p.sy = a->out.stride[0];
+  hipError_t e = launch_gnorm(p, a->dtype, false, (hipStream_t)stream);
+  return e == hipSuccess ? ok() : hip_fail(e, "ssm_gnorm_fwd");
+}
+int ssm_gnorm_bwd(const ssm_gnorm_args *a, void *stream) {
+  int rc = ssm_gnorm_check(a);
+  if (!rc) rc = gnorm_view(a->dout, "dout");
+  if (!rc) rc = gnorm_view(a->dx, "dx");
+  if (!rc && a->activation == SSM_GNORM_GATE) rc = gnorm_view(a->dgate, "dgate");
+  if (rc) return rc;
+  const int64_t bytes = ssm_gnorm_workspace_bytes(a);
+  if (bytes && (!a->workspace || a->workspace_bytes < bytes))
+    return fail(SSM_ESPACE, "workspace of %lld bytes required", (long long)bytes);
+  GnormParams p = gnorm_params(a);
+  p.dout = a->dout.data; p.sdo = a->dout.stride[0];
+  p.dx = a->dx.data; p.sdx = a->dx.stride[0];
+  p.dgate = a->dgate.data; p.sdg = a->dgate.stride[0];
+  p.dw = a->dweight; p.db = a->dbias; p.ws = (float *)a->workspace;
+  p.nblk = (int)gnorm_slots(a->rows, a->groups * a->group_size);
+  hipError_t e = launch_gnorm(p, a->dtype, true, (hipStream_t)stream);
+  return e == hipSuccess ? ok() : hip_fail(e, "ssm_gnorm_bwd");
 }
 
 // ------------------------------------------------------------------ forward without allocation

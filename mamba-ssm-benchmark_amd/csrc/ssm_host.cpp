@@ -463,6 +463,215 @@ py::tuple cscan_backward(const Tensor &x, const Tensor &delta, const Tensor &A, 
   return py::make_tuple(dx, dd, dA, dB, dC, out(dh0));
 }
 
+// ------------------------------------------------------------------ gated delta rule
+// t, or a contiguous copy where its last dimension is strided (the kernels read rows).
+Tensor unit_last(const Tensor &t) {
+  return !t.defined() || t.size(-1) == 1 || t.stride(-1) == 1 ? t : t.contiguous();
+}
+ssm_tensor lead_view(const Tensor &t, int64_t n) {  // the first n strides; the last dimension is unit stride
+  ssm_tensor v{};
+  v.data = t.data_ptr();
+  for (int64_t i = 0; i < n; ++i) v.stride[i] = t.stride(i);
+  return v;
+}
+bool delta_type(at::ScalarType t) { return t == at::kFloat || t == at::kBFloat16 || t == at::kHalf; }
+
+// Shapes and types of one call; `lead` = (B, L) of the chunked form, (B,) of the step.
+void delta_checks(const Tensor &q, const Tensor &k, const Tensor &v, const Tensor &g, const Tensor &beta, const Tensor &h,
+                  int64_t lead) {
+  require_gpu({&q, &k, &v, &g, &beta, &h});
+  for (const Tensor *t : {&k, &v, &g, &beta, &h})
+    TORCH_CHECK_VALUE(!t->defined() || t->device() == q.device(), "tensors on ", q.device().str(), " and ",
+                      t->device().str());
+  const char *const form = lead == 2 ? "(B, L, H, D)" : "(B, H, D)";
+  for (const Tensor *t : {&q, &k, &v})
+    TORCH_CHECK_VALUE(t->dim() == lead + 2, "q, k and v must be ", form, ", got ", shape_str(t->sizes()));
+  const auto dims = v.sizes().slice(0, lead);
+  std::vector<int64_t> wq(dims.begin(), dims.end()), wg = wq, wh{v.size(0), v.size(lead), q.size(-1), v.size(-1)};
+  wq.push_back(q.size(lead));
+  wq.push_back(q.size(-1));
+  wg.push_back(v.size(lead));
+  want("q", q, wq);
+  want("k", k, wq);
+  want("g", g, wg);
+  want("beta", beta, wg);
+  want(lead == 2 ? "h0" : "h", h, wh);
+  TORCH_CHECK_VALUE(q.size(lead) > 0 && v.size(lead) % q.size(lead) == 0, v.size(lead), " value heads are not a multiple of ",
+                    q.size(lead), " key heads");
+  for (const Tensor *t : {&q, &k, &v, &beta})
+    TORCH_CHECK_TYPE(delta_type(t->scalar_type()), "the gated delta rule takes float32, bfloat16 or float16, got ",
+                     t->scalar_type());
+  TORCH_CHECK_TYPE(at::isFloatingType(g.scalar_type()), "g must be floating, got ", g.scalar_type());
+}
+
+template <typename Args>
+void fill_delta(Args &a, const Tensor &q, const Tensor &k, const Tensor &v, const Tensor &g, const Tensor &beta, int64_t lead,
+                double scale, bool qk_norm) {
+  memset(&a, 0, sizeof(a));
+  a.batch = v.size(0); a.key_heads = q.size(lead); a.heads = v.size(lead);
+  a.key_dim = q.size(-1); a.value_dim = v.size(-1);
+  a.dtype = dtype_code(v.scalar_type());
+  a.beta_f32 = beta.scalar_type() == at::kFloat;
+  a.qk_norm = qk_norm;
+  a.scale = (float)scale;
+  a.q = lead_view(q, lead + 1); a.k = lead_view(k, lead + 1); a.v = lead_view(v, lead + 1);
+  a.g = view(g); a.beta = view(beta);
+}
+// The operands as the kernels read them: q, k and v of one type (float32 where they differ), rows of
+// unit stride, g in float32, beta in float32 or that type.
+struct DeltaOps {
+  Tensor q, k, v, g, beta;
+  DeltaOps(const Tensor &q_, const Tensor &k_, const Tensor &v_, const Tensor &g_, const Tensor &beta_) {
+    const at::ScalarType io = q_.scalar_type() == v_.scalar_type() && k_.scalar_type() == v_.scalar_type() ? v_.scalar_type() : at::kFloat;
+    q = unit_last(cast(q_, io)); k = unit_last(cast(k_, io)); v = unit_last(cast(v_, io));
+    g = cast(g_, at::kFloat);
+    beta = beta_.scalar_type() == io ? beta_ : cast(beta_, at::kFloat);
+  }
+};
+
+// (o, last or None, the tensors delta_backward needs)
+py::tuple delta_forward(const Tensor &q_, const Tensor &k_, const Tensor &v_, const Tensor &g_, const Tensor &beta_,
+                        const OptTensor &h0_, double scale, bool qk_norm, bool want_last, bool need_saved,
+                        const py::object &timer) {
+  delta_checks(q_, k_, v_, g_, beta_, get(h0_), 2);
+  const DeltaOps t(q_, k_, v_, g_, beta_);
+  Tensor h0 = cast(get(h0_), at::kFloat);
+  if (h0.defined()) h0 = h0.contiguous();
+  const Tensor o = at::empty(t.v.sizes(), t.v.options());
+  Tensor last, saved;
+  if (want_last) last = empty({t.v.size(0), t.v.size(2), t.q.size(3), t.v.size(3)}, t.v, at::kFloat);
+  ssm_delta_args a;
+  fill_delta(a, t.q, t.k, t.v, t.g, t.beta, 2, scale, qk_norm);
+  a.seqlen = t.v.size(1);
+  a.h0 = h0.defined() ? h0.data_ptr<float>() : nullptr;
+  a.out = lead_view(o, 3);
+  a.last = last.defined() ? last.data_ptr<float>() : nullptr;
+  SSM_BYTES(n, ssm_delta_fwd_workspace_bytes, ssm_delta_check, a, "ssm_delta_fwd");
+  const Tensor ws = bytes(n, o);
+  a.workspace = ws.data_ptr();
+  a.workspace_bytes = n;
+  if (need_saved) {
+    saved = bytes(ssm_delta_saved_bytes(&a), o);
+    a.saved = saved.data_ptr();
+  }
+  const Launch l(o);
+  l.run("ssm_delta_fwd", ssm_delta_fwd, a, timer);
+  return py::make_tuple(o, out(last), py::make_tuple(t.q, t.k, t.v, t.g, t.beta, out(saved)));
+}
+
+// (dq, dk, dv, dg, dbeta, dh0 or None)
+py::tuple delta_backward(const Tensor &q, const Tensor &k, const Tensor &v, const Tensor &g, const Tensor &beta,
+                         const Tensor &saved, const OptTensor &dout_, const OptTensor &dlast_, double scale, bool qk_norm,
+                         bool need_dh0, const py::object &timer) {
+  const Tensor dout = dout_ ? unit_last(cast(*dout_, v.scalar_type())) : at::zeros(v.sizes(), v.options());
+  Tensor dlast = cast(get(dlast_), at::kFloat);
+  if (dlast.defined()) dlast = dlast.contiguous();
+  auto dense = [](const Tensor &t) { return at::empty(t.sizes(), t.options()); };
+  const Tensor dq = dense(q), dk = dense(k), dv = dense(v), dg = dense(g), db = dense(beta);
+  Tensor dh0;
+  if (need_dh0) dh0 = empty({v.size(0), v.size(2), q.size(3), v.size(3)}, v, at::kFloat);
+  ssm_delta_args a;
+  fill_delta(a, q, k, v, g, beta, 2, scale, qk_norm);
+  a.seqlen = v.size(1);
+  a.saved = saved.data_ptr();
+  a.dout = lead_view(dout, 3);
+  a.dlast = dlast.defined() ? dlast.data_ptr<float>() : nullptr;
+  a.dq = lead_view(dq, 3); a.dk = lead_view(dk, 3); a.dv = lead_view(dv, 3);
+  a.dg = view(dg); a.dbeta = view(db);
+  a.dh0 = dh0.defined() ? dh0.data_ptr<float>() : nullptr;
+  SSM_BYTES(n, ssm_delta_bwd_workspace_bytes, ssm_delta_check, a, "ssm_delta_bwd");
+  const Tensor ws = bytes(n, v);
+  a.workspace = ws.data_ptr();
+  a.workspace_bytes = n;
+  const Launch l(v);
+  l.run("ssm_delta_bwd", ssm_delta_bwd, a, timer);
+  return py::make_tuple(dq, dk, dv, dg, db, out(dh0));
+}
+
+Tensor delta_step(const Tensor &h, const Tensor &q_, const Tensor &k_, const Tensor &v_, const Tensor &g_, const Tensor &beta_,
+                  double scale, bool qk_norm, const py::object &timer) {
+  delta_checks(q_, k_, v_, g_, beta_, h, 1);
+  TORCH_CHECK_VALUE(h.scalar_type() == at::kFloat && h.is_contiguous(), "the state must be contiguous float32, got ",
+                    h.scalar_type(), " with strides ", h.strides());
+  const DeltaOps t(q_, k_, v_, g_, beta_);
+  const Tensor o = at::empty(t.v.sizes(), t.v.options());
+  ssm_delta_step_args a;
+  fill_delta(a, t.q, t.k, t.v, t.g, t.beta, 1, scale, qk_norm);
+  a.h = h.data_ptr<float>();
+  a.out = lead_view(o, 2);
+  const Launch l(o);
+  l.run("ssm_delta_step", ssm_delta_step, a, timer);
+  return o.scalar_type() == v_.scalar_type() ? o : o.to(v_.scalar_type());
+}
+
+// ------------------------------------------------------------------ grouped norm
+ssm_gnorm_args gnorm_args(const Tensor &x2, const Tensor &w, const Tensor &b, const Tensor &gate2, int64_t groups, int act,
+                          bool center, double eps) {
+  ssm_gnorm_args a;
+  memset(&a, 0, sizeof(a));
+  a.rows = x2.size(0);
+  a.groups = groups;
+  a.group_size = x2.size(1) / groups;
+  a.dtype = dtype_code(x2.scalar_type());
+  a.activation = act;
+  a.center = center;
+  a.eps = eps;
+  a.x = view(x2);
+  a.gate = view(gate2);
+  a.weight = w.defined() ? w.data_ptr<float>() : nullptr;
+  a.bias = b.defined() ? b.data_ptr<float>() : nullptr;
+  return a;
+}
+Tensor f32(const OptTensor &t) { return t ? cast(*t, at::kFloat).contiguous() : Tensor(); }
+
+// (y, x as rows, weight, bias, gate as rows)
+py::tuple gnorm_forward(const Tensor &x, const OptTensor &weight, const OptTensor &bias, const OptTensor &gate, int64_t groups,
+                        int act, bool center, double eps) {
+  const Tensor g = get(gate), w_ = get(weight), b_ = get(bias);
+  require_gpu({&x, &g, &w_, &b_});
+  TORCH_CHECK_VALUE(x.dim() >= 1 && x.size(-1) > 0 && groups > 0 && x.size(-1) % groups == 0, "the last dimension of x, ",
+                    shape_str(x.sizes()), ", is not ", groups, " whole groups");
+  TORCH_CHECK_TYPE(delta_type(x.scalar_type()), "group_norm takes float32, bfloat16 or float16, got ", x.scalar_type());
+  want("weight", w_, {x.size(-1)});
+  want("bias", b_, {x.size(-1)});
+  want("gate", g, x.sizes());
+  const Tensor x2 = rows(x, x.size(-1)), w = f32(weight), b = f32(bias);
+  const Tensor g2 = g.defined() ? rows(cast(g, x.scalar_type()), x.size(-1)) : g;
+  const Tensor o = at::empty(x2.sizes(), x2.options());
+  ssm_gnorm_args a = gnorm_args(x2, w, b, g2, groups, act, center, eps);
+  a.out = view(o);
+  const Launch l(x);
+  l.run("ssm_gnorm_fwd", ssm_gnorm_fwd, a);
+  return py::make_tuple(o.view(x.sizes()), x2, out(w), out(b), out(g2));
+}
+
+// (dx, dweight, dbias, dgate), the last three None where their operand is
+py::tuple gnorm_backward(const Tensor &x2, const OptTensor &weight, const OptTensor &bias, const OptTensor &gate,
+                         const Tensor &dout, int64_t groups, int act, bool center, double eps, bool need_dw, bool need_db) {
+  const Tensor w = get(weight), b = get(bias), g2 = get(gate), dy = rows(cast(dout, x2.scalar_type()), x2.size(1));
+  const Tensor dx = at::empty(x2.sizes(), x2.options());
+  const Tensor dgate = g2.defined() ? at::empty(x2.sizes(), x2.options()) : g2;
+  const Tensor dw = need_dw ? empty({x2.size(1)}, x2, at::kFloat) : Tensor();
+  const Tensor db = need_db ? empty({x2.size(1)}, x2, at::kFloat) : Tensor();
+  ssm_gnorm_args a = gnorm_args(x2, w, b, g2, groups, act, center, eps);
+  a.dout = view(dy);
+  a.dx = view(dx);
+  a.dgate = view(dgate);
+  a.dweight = need_dw ? dw.data_ptr<float>() : nullptr;
+  a.dbias = need_db ? db.data_ptr<float>() : nullptr;
+  SSM_BYTES(n, ssm_gnorm_workspace_bytes, ssm_gnorm_check, a, "ssm_gnorm_bwd");
+  Tensor ws;
+  if (n) {
+    ws = bytes(n, x2);
+    a.workspace = ws.data_ptr();
+    a.workspace_bytes = n;
+  }
+  const Launch l(x2);
+  l.run("ssm_gnorm_bwd", ssm_gnorm_bwd, a);
+  const auto shape = dout.sizes();
+  return py::make_tuple(dx.view(shape), out(dw), out(db), g2.defined() ? py::cast(dgate.view(shape)) : py::none());
+}
+
 // ------------------------------------------------------------------ decode
 // The weights of a block stack's token step, laid out once; a step brings tokens and states.
 struct DecodePlan {
@@ -581,6 +790,13 @@ PYBIND11_MODULE(_ssmhost, m) {
   m.def("lscan_backward", torch::wrap_pybind_function(lscan_backward));
   m.def("cscan_forward", torch::wrap_pybind_function(cscan_forward));
   m.def("cscan_backward", torch::wrap_pybind_function(cscan_backward));
+  m.def("delta_checks", [](const Tensor &q, const Tensor &k, const Tensor &v, const Tensor &g, const Tensor &beta,
+                           const OptTensor &h) { delta_checks(q, k, v, g, beta, get(h), 2); });
+  m.def("delta_forward", torch::wrap_pybind_function(delta_forward));
+  m.def("delta_backward", torch::wrap_pybind_function(delta_backward));
+  m.def("delta_step", torch::wrap_pybind_function(delta_step));
+  m.def("gnorm_forward", torch::wrap_pybind_function(gnorm_forward));
+  m.def("gnorm_backward", torch::wrap_pybind_function(gnorm_backward));
   m.attr("ABI_VERSION") = SSM_ABI_VERSION;  // of the header the argument structs above were compiled from
   py::class_<DecodePlan>(m, "DecodePlan")
       .def(py::init<const std::vector<std::pair<std::vector<Tensor>, double>> &, Tensor, int64_t, int64_t, int64_t, int64_t,

@@ -293,6 +293,61 @@ hipError_t launch_dec_scan(const DecScanParams &p, int method, hipStream_t s);
 hipError_t launch_dec_out(const DecOutParams &p, hipStream_t s);
 hipError_t launch_dec_head(const DecInParams &p, hipStream_t s);
 
+// Gated delta rule.  Tensors' last dimension has unit stride; views' strides are batch, token, head.
+constexpr int kDeltaChunk = 64;        // tokens per chunk
+constexpr int kDeltaRows = 8 * 64;     // floats of row factors per chunk
+constexpr int kDeltaMaxK = 128;        // key width of the chunked kernels and the step
+struct DeltaParams {
+  int64_t B, L;
+  int Hk, H, Dk, Dv, NC, qk_norm, beta32;
+  float scale;
+  int vq, vk, vv, vo, vdo;             // 16-byte loads fit the view's rows
+  KView q, k, v, g, beta, o;           // (B, L, Hk, Dk), (B, L, H, Dv), (B, L, H)
+  const float *h0;                     // (B, H, Dk, Dv) or null
+  float *last;
+  void *fT, *fP;                       // operand fragments of T - I and P, or of their transposes (backward)
+  float *rows;                         // (B H, NC, kDeltaRows)
+  float *states, *u;                   // saved: (B H, NC, Dk, Dv) entering states, (B H, NC, 64, Dv) U
+  KView dout, dq, dk, dv, dg, dbeta;
+  const float *dlast;
+  float *dh0, *dstates, *dr;           // gradients of the leaving states and R, laid out as states and u
+};
+// bf16 parts that hold a float32 intermediate
+inline int delta_mid_parts(int dtype) { return dtype == 0 ? 3 : 2; }
+hipError_t launch_delta_fwd(const DeltaParams &p, int dtype, hipStream_t s);
+hipError_t launch_delta_bwd(const DeltaParams &p, int dtype, hipStream_t s);
+struct DeltaStepParams {
+  int B, Hk, H, Dk, Dv, qk_norm, beta32;
+  float scale;
+  KView q, k, v, g, beta, o;           // strides: batch, head
+  float *h;                            // (B, H, Dk, Dv), updated in place
+};
+hipError_t launch_delta_step(const DeltaStepParams &p, int dtype, hipStream_t s);
+
+// Grouped norm over the last dimension.
+constexpr int kGnormMaxGroup = 1024;
+constexpr int kGnormLanes = 1 << 17;   // lanes of the backward, about: 2048 wavefronts
+struct GnormParams {
+  int64_t R;
+  int G, n, center, act;               // act: 0 none, 1 SiLU of the result, 2 gate
+  float eps;
+  int vec;                             // rows load 16 bytes at a time
+  const void *x, *gate, *dout;
+  const float *w, *b;
+  void *y, *dx, *dgate;
+  int64_t sx, sg, sdo, sy, sdx, sdg;   // row strides
+  float *dw, *db;                      // (C,) or null
+  float *ws;                           // (1 or 2, nblk, C): partial dw, db
+  int nblk;                            // row slots of the backward
+};
+// Row slots: enough lane groups for kGnormLanes, at most one per row.  A group takes at least n / 8 lanes
+// (8 channels of 16 bits per load), so this is within a factor of 8 of it for every variant.
+inline int64_t gnorm_slots(int64_t R, int64_t C) {
+  const int64_t want = kGnormLanes * 8 / C;
+  return want < 1 ? 1 : want < R ? want : R;
+}
+hipError_t launch_gnorm(const GnormParams &p, int dtype, bool bwd, hipStream_t s);
+
 // Runs the summary and carry passes first when p.nseg > 1.
 hipError_t launch_fwd(const FwdParams &p, int dtype, int method, int np, hipStream_t s);
 hipError_t launch_bwd(const BwdParams &p, int dtype, int method, int np, hipStream_t s);

@@ -11,7 +11,7 @@ import os
 import torch
 
 LIB_PATH = os.path.join(os.path.dirname(os.path.abspath(__file__)), "libssmscan.so")
-ABI_VERSION = 8
+ABI_VERSION = 9
 
 OK, EINVAL, EKEY, ESPACE, EHIP = 0, 1, 2, 3, 4
 ZOH, EULER, BILINEAR = 0, 1, 2
@@ -141,6 +141,33 @@ class NormArgs(ctypes.Structure):
                 ("workspace", c_vp), ("workspace_bytes", c_i64)]
 
 
+class DeltaArgs(ctypes.Structure):
+    _fields_ = [("batch", c_i64), ("seqlen", c_i64), ("key_heads", c_i64), ("heads", c_i64),
+                ("key_dim", c_i64), ("value_dim", c_i64),
+                ("dtype", c_i32), ("beta_f32", c_i32), ("qk_norm", c_i32), ("scale", ctypes.c_float),
+                ("q", Tensor), ("k", Tensor), ("v", Tensor), ("g", Tensor), ("beta", Tensor),
+                ("h0", c_vp), ("out", Tensor), ("last", c_vp), ("saved", c_vp),
+                ("dout", Tensor), ("dlast", c_vp), ("dq", Tensor), ("dk", Tensor), ("dv", Tensor),
+                ("dg", Tensor), ("dbeta", Tensor), ("dh0", c_vp),
+                ("workspace", c_vp), ("workspace_bytes", c_i64)]
+
+
+class DeltaStepArgs(ctypes.Structure):
+    _fields_ = [("batch", c_i64), ("key_heads", c_i64), ("heads", c_i64), ("key_dim", c_i64), ("value_dim", c_i64),
+                ("dtype", c_i32), ("beta_f32", c_i32), ("qk_norm", c_i32), ("scale", ctypes.c_float),
+                ("q", Tensor), ("k", Tensor), ("v", Tensor), ("g", Tensor), ("beta", Tensor),
+                ("h", c_vp), ("out", Tensor)]
+
+
+class GnormArgs(ctypes.Structure):
+    _fields_ = [("rows", c_i64), ("groups", c_i64), ("group_size", c_i64),
+                ("dtype", c_i32), ("activation", c_i32), ("center", c_i32), ("reserved0", c_i32),
+                ("eps", ctypes.c_double),
+                ("x", Tensor), ("gate", Tensor), ("weight", c_vp), ("bias", c_vp), ("out", Tensor),
+                ("dout", Tensor), ("dx", Tensor), ("dgate", Tensor), ("dweight", c_vp), ("dbias", c_vp),
+                ("workspace", c_vp), ("workspace_bytes", c_i64)]
+
+
 # name -> (restype, argtypes)
 _SIGS = {
     "ssm_abi_version": (c_i32, []),
@@ -184,6 +211,18 @@ _SIGS = {
     "ssm_conv_bwd": (c_i32, [ctypes.POINTER(ConvArgs), c_vp]),
     "ssm_norm_fwd": (c_i32, [ctypes.POINTER(NormArgs), c_vp]),
     "ssm_norm_bwd": (c_i32, [ctypes.POINTER(NormArgs), c_vp]),
+    "ssm_delta_check": (c_i32, [ctypes.POINTER(DeltaArgs)]),
+    "ssm_delta_step_check": (c_i32, [ctypes.POINTER(DeltaStepArgs)]),
+    "ssm_gnorm_check": (c_i32, [ctypes.POINTER(GnormArgs)]),
+    "ssm_delta_saved_bytes": (c_i64, [ctypes.POINTER(DeltaArgs)]),
+    "ssm_delta_fwd_workspace_bytes": (c_i64, [ctypes.POINTER(DeltaArgs)]),
+    "ssm_delta_bwd_workspace_bytes": (c_i64, [ctypes.POINTER(DeltaArgs)]),
+    "ssm_gnorm_workspace_bytes": (c_i64, [ctypes.POINTER(GnormArgs)]),
+    "ssm_delta_fwd": (c_i32, [ctypes.POINTER(DeltaArgs), c_vp]),
+    "ssm_delta_bwd": (c_i32, [ctypes.POINTER(DeltaArgs), c_vp]),
+    "ssm_delta_step": (c_i32, [ctypes.POINTER(DeltaStepArgs), c_vp]),
+    "ssm_gnorm_fwd": (c_i32, [ctypes.POINTER(GnormArgs), c_vp]),
+    "ssm_gnorm_bwd": (c_i32, [ctypes.POINTER(GnormArgs), c_vp]),
     "ssm_cscan_tile": (c_i64, [c_i32, c_i32]),
     "ssm_default_chunk": (c_i64, [c_i64]),
     "ssm_scan_blocks": (c_i64, [c_i64, c_i64, c_i64, c_i64, c_i64, ctypes.POINTER(c_i64), c_i64]),

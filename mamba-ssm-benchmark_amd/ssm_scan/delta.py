@@ -1,0 +1,69 @@
+"""The gated delta rule on the HIP engine: a recurrence with a matrix state per head.
+
+No counterpart in the reference, whose scan has a diagonal state (models/scan.py:264-274); the
+calls follow that scan's contract (h0 in, last state out, the state of a step updated in place).
+Per batch row and value head, with S (Dk, Dv):
+
+    S' = e^{g_t} S_{t-1}      u_t = beta_t (v_t - S'^T k_t)      S_t = S' + k_t u_t^T
+    o_t = scale S_t^T q_t
+
+``gated_delta_rule`` runs whole sequences (training, prefill; differentiable in every tensor),
+``gated_delta_step`` one token per stream.  Key heads may be fewer than value heads (value head h
+reads key head h // (H // Hk)); their gradients are summed over the heads that share them.
+Products run on the matrix cores over bf16 parts of the operands (one part for bf16 inputs, two
+for fp16 and for the float32 intermediates beside them, three for float32 inputs); states,
+decays, norms and sums are float32 or wider, and every sum runs in a fixed order.
+"""
+
+import torch
+
+from . import _abi, profiling
+
+MAX_KEY_DIM = 128
+
+
+class GatedDeltaRuleFn(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, q, k, v, g, beta, h0, scale, qk_norm, want_last):
+        need = any(ctx.needs_input_grad[:6])
+        o, last, tensors = _abi.host().delta_forward(q, k, v, g, beta, h0, scale, qk_norm, want_last, need,
+                                                     profiling.active())
+        if need:
+            ctx.save_for_backward(*tensors)
+        ctx.set_materialize_grads(False)
+        ctx.settings = scale, qk_norm
+        ctx.dtypes = [t.dtype for t in (q, k, v, g, beta)] + [None if h0 is None else h0.dtype]
+        return (o if o.dtype == v.dtype else o.to(v.dtype)), last
+
+    @staticmethod
+    def backward(ctx, dout, dlast):
+        if dout is None and dlast is None:
+            return (None,) * 9
+        grads = _abi.host().delta_backward(*ctx.saved_tensors, dout, dlast, *ctx.settings, ctx.needs_input_grad[5],
+                                           profiling.active())
+        return tuple(d if d is None or d.dtype == t else d.to(t) for d, t in zip(grads, ctx.dtypes)) + (None,) * 3
+
+
+def gated_delta_rule(q, k, v, g, beta, h0=None, scale=None, qk_norm=False, return_last_state=False):
+    """o (B, L, H, Dv) in v's dtype; with return_last_state, (o, last (B, H, Dk, Dv) float32).
+
+    q, k (B, L, Hk, Dk), Dk <= 128, Hk dividing H; v (B, L, H, Dv); all float32, bfloat16 or float16
+    (read in place with any strides whose last one is 1).  g (B, L, H): log decays (<= 0; -inf forgets
+    the state, as at a document's start); beta (B, L, H).  h0 (B, H, Dk, Dv): the state before the first
+    token, zeros if None.  scale: Dk^-0.5 if None.  qk_norm divides q and k by sqrt(sum of squares + 1e-6)
+    over Dk first."""
+    scale = float(q.shape[-1] ** -0.5 if scale is None else scale)
+    if v.dim() == 4 and v.numel() == 0 and v.shape[2] and v.shape[3]:   # no token: the state passes through
+        _abi.host().delta_checks(q, k, v, g, beta, h0)
+        last = v.new_zeros((v.shape[0], v.shape[2], q.shape[-1], v.shape[3]), dtype=torch.float32) if h0 is None \
+            else h0.float()
+        return (v * 1, last) if return_last_state else v * 1
+    o, last = GatedDeltaRuleFn.apply(q, k, v, g, beta, h0, scale, bool(qk_norm), bool(return_last_state))
+    return (o, last) if return_last_state else o
+
+
+def gated_delta_step(h, q, k, v, g, beta, scale=None, qk_norm=False):
+    """One token per stream: o (B, H, Dv) in v's dtype; h (B, H, Dk, Dv), contiguous float32, is updated
+    in place.  q, k (B, Hk, Dk), v (B, H, Dv), g and beta (B, H) as in gated_delta_rule."""
+    scale = float(q.shape[-1] ** -0.5 if scale is None else scale)
+    return _abi.host().delta_step(h, q, k, v, g, beta, scale, bool(qk_norm), profiling.active())
