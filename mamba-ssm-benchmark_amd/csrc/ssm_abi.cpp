@@ -1180,11 +1180,10 @@ static int need(std::initializer_list<std::pair<const void *, const char *>> ps)
     if (!p.first) return fail(SSM_EINVAL, "required tensor '%s' is missing", p.second);
   return ok();
 }
-// Eight elements of a row load as 16-byte words: base and strides are whole words.
-static int rows16(const ssm_tensor &t, int64_t width, int dtype) {
-  const int64_t e = dtype == SSM_F32 ? 4 : 8;
-  return (uintptr_t)t.data % 16 == 0 && width % 8 == 0 && t.stride[0] % e == 0 && t.stride[1] % e == 0 &&
-         t.stride[2] % e == 0;
+// Rows are whole, aligned words of 4 elements.
+static int rows4(const ssm_tensor &t, int64_t width, int dtype) {
+  return (uintptr_t)t.data % (dtype == SSM_F32 ? 16 : 8) == 0 && width % 4 == 0 && t.stride[0] % 4 == 0 &&
+         t.stride[1] % 4 == 0 && t.stride[2] % 4 == 0;
 }
 
 int ssm_delta_check(const ssm_delta_args *a) {
@@ -1200,35 +1199,47 @@ int ssm_delta_check(const ssm_delta_args *a) {
 
 namespace {
 struct DeltaLayout {
-  int64_t states, u, T, rows;  // bytes of one array, 256-byte multiples
+  int64_t states, values, square, keys, rows;  // bytes of one array, 256-byte multiples
 };
 DeltaLayout delta_layout(const ssm_delta_args *a) {
-  const int64_t n = a->batch * a->heads * cdiv(a->seqlen, kDeltaChunk);
-  return {align256(n * a->key_dim * a->value_dim * 4), align256(n * kDeltaChunk * a->value_dim * 4),
-          align256(n * delta_mid_parts(a->dtype) * kDeltaChunk * kDeltaChunk * 2), align256(n * kDeltaRows * 4)};
+  const int64_t nc = cdiv(a->seqlen, kDeltaChunk), n = a->batch * a->heads * nc, v = cdiv(a->value_dim, 16) * 16;
+  return {align256(n * cdiv(a->key_dim, 16) * 16 * v * 4), align256(n * kDeltaChunk * v * 4),
+          align256(n * kDeltaMidParts * kDeltaChunk * kDeltaChunk * 2),
+          align256(a->batch * a->key_heads * nc * delta_in_parts(a->dtype) * kDeltaChunk * delta_width(a->key_dim) * 2),
+          align256(n * kDeltaRows * 4)};
 }
-DeltaParams delta_params(const ssm_delta_args *a) {
+DeltaParams delta_params(const ssm_delta_args *a, bool bwd) {
   DeltaParams p{};
   p.B = a->batch; p.L = a->seqlen;
   p.Hk = (int)a->key_heads; p.H = (int)a->heads; p.Dk = (int)a->key_dim; p.Dv = (int)a->value_dim;
   p.NC = (int)cdiv(a->seqlen, kDeltaChunk);
+  p.VT = (int)cdiv(a->value_dim, 16);
+  p.Dkp = (int)cdiv(a->key_dim, 16) * 16;
   p.qk_norm = a->qk_norm;
   p.beta32 = a->beta_f32;
   p.scale = a->scale;
   p.q = kv(a->q); p.k = kv(a->k); p.v = kv(a->v); p.g = kv(a->g); p.beta = kv(a->beta);
-  p.vq = rows16(a->q, a->key_dim, a->dtype);
-  p.vk = rows16(a->k, a->key_dim, a->dtype);
-  p.vv = rows16(a->v, a->value_dim, a->dtype);
+  p.vq = rows4(a->q, a->key_dim, a->dtype);
+  p.vk = rows4(a->k, a->key_dim, a->dtype);
+  p.vv = rows4(a->v, a->value_dim, a->dtype);
   const DeltaLayout l = delta_layout(a);
   char *ws = (char *)a->workspace;
-  p.fT = ws;
-  p.fP = ws + l.T;
-  p.rows = (float *)(ws + 2 * l.T);
-  p.dstates = (float *)(ws + 2 * l.T + l.rows);
-  p.dr = (float *)(ws + 2 * l.T + l.rows + l.states);
+  auto take = [&](int64_t bytes) {
+    char *at = ws;
+    ws += bytes;
+    return at;
+  };
+  p.fT = take(l.square); p.fP = take(l.square);
+  p.fK = take(l.keys); p.fQ = take(l.keys); p.fKt = take(l.keys);
+  p.rows = (float *)take(l.rows);
+  if (bwd) {
+    p.fQt = take(l.keys);
+    p.dstates = (float *)take(l.states);
+    p.dr = (float *)take(l.values);
+  }
   if (a->saved) {
     p.states = (float *)a->saved;
-    p.u = (float *)((char *)a->saved + l.states);
+    p.y = (float *)((char *)a->saved + l.states);
   }
   return p;
 }
@@ -1237,17 +1248,17 @@ DeltaParams delta_params(const ssm_delta_args *a) {
 int64_t ssm_delta_saved_bytes(const ssm_delta_args *a) {
   if (ssm_delta_check(a)) return -1;
   const DeltaLayout l = delta_layout(a);
-  return l.states + l.u;
+  return l.states + l.values;
 }
 int64_t ssm_delta_fwd_workspace_bytes(const ssm_delta_args *a) {
   if (ssm_delta_check(a)) return -1;
   const DeltaLayout l = delta_layout(a);
-  return 2 * l.T + l.rows;
+  return 2 * l.square + 3 * l.keys + l.rows;
 }
 int64_t ssm_delta_bwd_workspace_bytes(const ssm_delta_args *a) {
   if (ssm_delta_check(a)) return -1;
   const DeltaLayout l = delta_layout(a);
-  return 2 * l.T + l.rows + l.states + l.u;
+  return 2 * l.square + 4 * l.keys + l.rows + l.states + l.values;
 }
 
 int ssm_delta_fwd(const ssm_delta_args *a, void *stream) {
@@ -1257,8 +1268,9 @@ int ssm_delta_fwd(const ssm_delta_args *a, void *stream) {
   const int64_t bytes = ssm_delta_fwd_workspace_bytes(a);
   if (!a->workspace || a->workspace_bytes < bytes)
     return fail(SSM_ESPACE, "workspace of %lld bytes required", (long long)bytes);
-  DeltaParams p = delta_params(a);
+  DeltaParams p = delta_params(a, false);
   p.o = kv(a->out);
+  p.vo = rows4(a->out, a->value_dim, a->dtype);
   p.h0 = a->h0;
   p.last = a->last;
   hipError_t e = launch_delta_fwd(p, a->dtype, (hipStream_t)stream);
@@ -1274,9 +1286,12 @@ int ssm_delta_bwd(const ssm_delta_args *a, void *stream) {
   const int64_t bytes = ssm_delta_bwd_workspace_bytes(a);
   if (!a->workspace || a->workspace_bytes < bytes)
     return fail(SSM_ESPACE, "workspace of %lld bytes required", (long long)bytes);
-  DeltaParams p = delta_params(a);
+  DeltaParams p = delta_params(a, true);
   p.dout = kv(a->dout); p.dq = kv(a->dq); p.dk = kv(a->dk); p.dv = kv(a->dv); p.dg = kv(a->dg); p.dbeta = kv(a->dbeta);
-  p.vdo = rows16(a->dout, a->value_dim, a->dtype);
+  p.vdo = rows4(a->dout, a->value_dim, a->dtype);
+  p.vdv = rows4(a->dv, a->value_dim, a->dtype);
+  p.vdq = rows4(a->dq, a->key_dim, a->dtype);
+  p.vdk = rows4(a->dk, a->key_dim, a->dtype);
   p.dlast = a->dlast;
   p.dh0 = a->dh0;
   hipError_t e = launch_delta_bwd(p, a->dtype, (hipStream_t)stream);

@@ -1,8 +1,9 @@
 // Gated delta rule, chunked forward (the mathematics and the operand layouts: ssm_delta.hpp).
 //
-//   k_delta_prep  one workgroup per (batch row, value head, chunk): decays, norms, T and P
-//   k_delta_fwd   one workgroup per (batch row, value head, 16 NV columns of v): the columns of S do
-//                 not mix, so each walks the chunks with its own columns in registers
+//   k_delta_prep  one workgroup per (batch row, value head, chunk): decays, norms, T, P and the keys' and
+//                 queries' operand fragments
+//   k_delta_fwd   one workgroup per (batch row, value head, 16 columns of v): the columns of S do not
+//                 mix, so each walks the chunks with its own columns in registers
 #include "ssm_delta.hpp"
 
 namespace ssm {
@@ -22,31 +23,42 @@ __device__ __forceinline__ void put16(float *m, int lane, f4 c, float sign) {
   for (int i = 0; i < 4; ++i) m[(4 * (lane / 16) + i) * PITCH + lane % 16] = sign * c[i];
 }
 
-// Writes T - I and P (TR: their transposes) as operand fragments, and the row factors.
+// Writes T - I and P as operand fragments, the row factors, and, for the first of the value heads that
+// share a key head, the fragments of K and Q.  BWD: the transposes of T = (I + strictly lower(beta_i
+// e^{G_i - G_j} k_i.k_j))^-1, which the gradient takes, and of P.
 // T is inverted in float32: the four 16 x 16 diagonal blocks by substitution, one wavefront each, the
 // rest by T10 = -T11 (L10 T00) for blocks of 16, then of 32 rows.
-template <typename IT, int DK, bool TR>
+template <typename IT, int DK, bool BWD>
 __global__ void __launch_bounds__(kDT) k_delta_prep(const DeltaParams p) {
-  constexpr int NK = DParts<IT>::in, NM = DParts<IT>::mid, KS = DK / 32, KP = DK + 8, FP = kC + 4;
-  __shared__ __align__(16) __bf16 Kr[NK][kC][KP];
-  __shared__ __align__(16) float Lm[kC][FP], Pm[kC][FP];
+  constexpr int NK = DParts<IT>::in, NM = DParts<IT>::mid, NP = BWD ? NM : DParts<IT>::out, KS = DK / 32, FP = kC + 4;
+  __shared__ __align__(16) __bf16 Kf[NK][4 * KS * 64 * 8], Qf[NK][4 * KS * 64 * 8];  // as in memory
+  __shared__ __align__(16) float Lm[kC][FP], Yr[32 * FP];
   __shared__ double Gs[kC];
   __shared__ float fk[kC], fq[kC], bs[kC];
-  const int tid = threadIdx.x, lane = tid % 64, w = tid / 64, r16 = lane % 16, kg = lane / 16;
+  const int tid = threadIdx.x, lane = tid % 64, w = wave_id(), r16 = lane % 16, kg = lane / 16;
   const int64_t ch = blockIdx.x;
-  const int bh = (int)(ch / p.NC), c = (int)(ch % p.NC), b = bh / p.H, h = bh % p.H, hk = h / (p.H / p.Hk);
-  const int64_t t0 = (int64_t)c * kC, t = t0 + 16 * w + r16;
+  const int group = p.H / p.Hk, bh = (int)(ch / p.NC), c = (int)(ch % p.NC), b = bh / p.H, h = bh % p.H, hk = h / group;
+  const int64_t t0 = (int64_t)c * kC, t = t0 + 16 * w + r16, kch = ((int64_t)b * p.Hk + hk) * p.NC + c;
   const IT *kp = (const IT *)p.k.p + b * p.k.s0 + t * p.k.s1 + hk * p.k.s2;
   const IT *qp = (const IT *)p.q.p + b * p.q.s0 + t * p.q.s1 + hk * p.q.s2;
   const int have = t < p.L ? p.Dk : 0;
+  const bool first = h % group == 0;
   bf8 K[KS][NK], Q[KS][NK];
 #pragma unroll
   for (int s = 0; s < KS; ++s) {
-    const int e = 32 * s + 8 * kg;
-    row_frag<IT, NK>(kp + e, have - e, p.vk, K[s]);
-    row_frag<IT, NK>(qp + e, have - e, p.vq, Q[s]);
+    const int e = 32 * s + 4 * kg;
+    Raw4<IT> x[4] = {load4(kp + e, have - e, p.vk), load4(kp + e + 16, have - e - 16, p.vk),
+                     load4(qp + e, have - e, p.vq), load4(qp + e + 16, have - e - 16, p.vq)};
+    bf4 a[4][NK];
 #pragma unroll
-    for (int n = 0; n < NK; ++n) *(bf8 *)&Kr[n][16 * w + r16][e] = K[s][n];
+    for (int i = 0; i < 4; ++i) to_parts<IT, NK>(x[i], a[i]);
+#pragma unroll
+    for (int n = 0; n < NK; ++n) {
+      K[s][n] = __builtin_shufflevector(a[0][n], a[1][n], 0, 1, 2, 3, 4, 5, 6, 7);
+      Q[s][n] = __builtin_shufflevector(a[2][n], a[3][n], 0, 1, 2, 3, 4, 5, 6, 7);
+      *(bf8 *)&Kf[n][((w * KS + s) * 64 + lane) * 8] = K[s][n];
+      *(bf8 *)&Qf[n][((w * KS + s) * 64 + lane) * 8] = Q[s][n];
+    }
   }
   if (w == 0) {
     const int64_t tt = t0 + lane;
@@ -67,8 +79,8 @@ __global__ void __launch_bounds__(kDT) k_delta_prep(const DeltaParams p) {
     f4 kk = 0, qq = 0;
 #pragma unroll
     for (int s = 0; s < KS; ++s) {
-      kk = mma(K[s], K[s], kk);
-      qq = mma(Q[s], Q[s], qq);
+      kk = mma<NK>(K[s], K[s], kk);
+      qq = mma<NK>(Q[s], Q[s], qq);
     }
 #pragma unroll
     for (int i = 0; i < 4; ++i)
@@ -78,34 +90,54 @@ __global__ void __launch_bounds__(kDT) k_delta_prep(const DeltaParams p) {
       }
   }
   __syncthreads();
+  if (first) {
+    __bf16 *const gK = (__bf16 *)p.fK + kch * NK * kC * DK, *const gQ = (__bf16 *)p.fQ + kch * NK * kC * DK;
+    __bf16 *const gKt = (__bf16 *)p.fKt + kch * NK * kC * DK, *const gQt = BWD ? (__bf16 *)p.fQt + kch * NK * kC * DK : nullptr;
 #pragma unroll
-  for (int jt = 0; jt < 4; ++jt) {
-    f4 kk = 0, qk = 0;
-    const int col = 16 * jt + r16;
-    if (jt <= w) {
+    for (int n = 0; n < NK; ++n) {
 #pragma unroll
       for (int s = 0; s < KS; ++s) {
-        bf8 B[NK];
-        lds_frag<NK, KP>(&Kr[0][0][0], kC * KP, col, 32 * s + 8 * kg, B);
-        kk = mma(K[s], B, kk);
-        qk = mma(Q[s], B, qk);
+        *(bf8 *)(gK + n * kC * DK + ((w * KS + s) * 64 + lane) * 8) = K[s][n];
+        *(bf8 *)(gQ + n * kC * DK + ((w * KS + s) * 64 + lane) * 8) = Q[s][n];
       }
-    }
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const int row = 16 * w + 4 * kg + i;
-      float l = 0, pr = 0;
-      if (col <= row) {
-        const float e = fexp((float)(Gs[row] - Gs[col])) * fk[col];
-        pr = e * fq[row] * qk[i];
-        if (col < row) l = bs[row] * fk[row] * e * kk[i];
+      for (int x = 0; x < DK / 32; ++x) {  // key tile kt, step s of tokens
+        const int kt = w + 4 * (x / 2), s = x % 2, row = 4 * kg + r16 / 4;
+        const int lo = ((2 * s * KS + kt / 2) * 64 + (lane % 4) * 16 + row) * 8 + 4 * (kt % 2), hi = lo + KS * 64 * 8;
+        *(bf8 *)(gKt + n * kC * DK + ((2 * kt + s) * 64 + lane) * 8) = read_tr(&Kf[n][lo], &Kf[n][hi]);
+        if (BWD) *(bf8 *)(gQt + n * kC * DK + ((2 * kt + s) * 64 + lane) * 8) = read_tr(&Qf[n][lo], &Qf[n][hi]);
       }
-      Lm[row][col] = l;
-      Pm[row][col] = pr;
     }
   }
+  f4 P[4];  // P_ij, token tile w as i, j = 16 x + 4 kg + r; BWD: tile w as j, i = 16 x + 4 kg + r
+#pragma unroll
+  for (int x = 0; x < 4; ++x) {
+    f4 kk = 0, qk = 0;
+#pragma unroll
+    for (int s = 0; s < KS; ++s) {
+      bf8 A[NK];
+      if (x <= w) {
+        load_frag<NK>(&Kf[0][0], 4 * KS * 64 * 8, x * KS + s, lane, A);
+        kk = mma<NK>(A, K[s], kk);
+        if (!BWD) qk = mma<NK>(A, Q[s], qk);
+      }
+      if (BWD && x >= w) {
+        load_frag<NK>(&Qf[0][0], 4 * KS * 64 * 8, x * KS + s, lane, A);
+        qk = mma<NK>(A, K[s], qk);
+      }
+    }
+    const int own = 16 * w + r16;
+    f4 l;
+#pragma unroll
+    for (int r = 0; r < 4; ++r) {
+      const int at = 16 * x + 4 * kg + r;
+      l[r] = at < own ? fexp((float)(Gs[own] - Gs[at])) * fk[own] * fk[at] * (BWD ? bs[own] : bs[at]) * kk[r] : 0.0f;
+      if (BWD) P[x][r] = own <= at ? fexp((float)(Gs[at] - Gs[own])) * fq[at] * fk[own] * qk[r] : 0.0f;
+      else P[x][r] = at <= own ? fexp((float)(Gs[own] - Gs[at])) * fq[own] * fk[at] * qk[r] : 0.0f;
+    }
+    *(f4 *)&Lm[own][16 * x + 4 * kg] = l;
+  }
   __syncthreads();
-  float *Yr = (float *)&Kr[0][0][0];  // the keys are no longer read: scratch of 32 x FP floats
   {
     const float *D = &Lm[16 * w][16 * w];
     float x[16];
@@ -147,22 +179,21 @@ __global__ void __launch_bounds__(kDT) k_delta_prep(const DeltaParams p) {
   __syncthreads();
 #pragma unroll
   for (int s = 0; s < 2; ++s) {
-    const int row = 16 * w + r16, e = 32 * s + 8 * kg;
-    f8 x, y;
+    const int own = 16 * w + r16;
+    f8 x;
 #pragma unroll
     for (int j = 0; j < 8; ++j) {
-      x[j] = TR ? Lm[e + j][row] : Lm[row][e + j];
-      if (e + j == row) x[j] = 0;  // T - I
-      y[j] = TR ? Pm[e + j][row] : Pm[row][e + j];
+      const int e = 32 * s + 16 * (j / 4) + 4 * kg + j % 4;
+      x[j] = e == own ? 0.0f : BWD ? Lm[e][own] : Lm[own][e];
     }
-    bf8 a[NM];
-    const int64_t at = ch * NM * kFrag + ((2 * w + s) * 64 + lane) * 8;
+    const int64_t at = ((2 * w + s) * 64 + lane) * 8;
+    bf8 a[NM], q[NP];
     split_parts<NM>(x, a);
 #pragma unroll
-    for (int n = 0; n < NM; ++n) *(bf8 *)((__bf16 *)p.fT + at + n * kFrag) = a[n];
-    split_parts<NM>(y, a);
+    for (int n = 0; n < NM; ++n) *(bf8 *)((__bf16 *)p.fT + (ch * NM + n) * kFrag + at) = a[n];
+    split_parts<NP>((f8)__builtin_shufflevector(P[2 * s], P[2 * s + 1], 0, 1, 2, 3, 4, 5, 6, 7), q);
 #pragma unroll
-    for (int n = 0; n < NM; ++n) *(bf8 *)((__bf16 *)p.fP + at + n * kFrag) = a[n];
+    for (int n = 0; n < NP; ++n) *(bf8 *)((__bf16 *)p.fP + (ch * NP + n) * kFrag + at) = q[n];
   }
   if (tid < kC) {
     float *rows = p.rows + ch * kDeltaRows;
@@ -178,171 +209,137 @@ __global__ void __launch_bounds__(kDT) k_delta_prep(const DeltaParams p) {
   }
 }
 
-template <typename IT, int DK, int NV>
-__global__ void __launch_bounds__(kDT) k_delta_fwd(const DeltaParams p) {
-  constexpr int NK = DParts<IT>::in, NM = DParts<IT>::mid, KS = DK / 32, KP = DK + 8, BV = 16 * NV, RT = DK / 64;
-  __shared__ __align__(16) __bf16 Kr[NK][kC][KP];                       // keys, row per token
-  __shared__ __align__(16) __bf16 St[NM][BV][KP];                       // state, row per column of v
-  __shared__ __align__(16) __bf16 Rt[NM][BV][kCP], Ut[NM][BV][kCP], Wt[NM][BV][kCP];  // R, U, c U, row per column
-  const int tid = threadIdx.x, lane = tid % 64, w = tid / 64, r16 = lane % 16, kg = lane / 16;
+// Everything that does not hang on the state is read a chunk ahead, into the registers that the chunk has
+// just used.  All products are of transposes: rows are the 16 columns of v, so a lane holds 4 columns of
+// one token or key, and moves them as one word.
+template <typename IT, int DK>
+__global__ void __launch_bounds__(kDT, DK * sizeof(IT) <= 256 ? 2 : 1) k_delta_fwd(const DeltaParams p) {
+  constexpr int NK = DParts<IT>::in, NM = DParts<IT>::mid, NP = DParts<IT>::out, KS = DK / 32, RT = DK / 64;
+  __shared__ __align__(16) VTile<NM, DK> St;
+  __shared__ __align__(16) VTile<NM, kC> Xt, Wt;
+  __shared__ __align__(16) VTile<NP, kC> Ut;
+  const int tid = threadIdx.x, lane = tid % 64, w = wave_id(), r16 = lane % 16, kg = lane / 16;
   int bh, vt;
-  delta_tile((p.Dv + BV - 1) / BV, (int)p.B * p.H, bh, vt);
-  const int b = bh / p.H, h = bh % p.H, hk = h / (p.H / p.Hk), v0 = vt * BV;
-  const int tr = 16 * w + 4 * kg;  // the lane's token rows of a result tile: tr + i
-  const IT *kb = (const IT *)p.k.p + b * p.k.s0 + hk * p.k.s2, *qb = (const IT *)p.q.p + b * p.q.s0 + hk * p.q.s2;
-  const IT *vb = (const IT *)p.v.p + b * p.v.s0 + h * p.v.s2;
-  IT *ob = (IT *)p.o.p + b * p.o.s0 + h * p.o.s2;
+  delta_tile(p.VT, (int)p.B * p.H, bh, vt);
+  const int b = bh / p.H, h = bh % p.H, hk = h / (p.H / p.Hk), v0 = 16 * vt + 4 * kg, have = p.Dv - v0;
+  const int tok = 16 * w + r16;
+  const IT *vp = (const IT *)p.v.p + b * p.v.s0 + h * p.v.s2 + v0;
+  IT *op = (IT *)p.o.p + b * p.o.s0 + h * p.o.s2 + v0;
+  const int64_t ch0 = (int64_t)bh * p.NC, kch0 = ((int64_t)b * p.Hk + hk) * p.NC;
 
-  f4 S[RT][NV];  // rows 16 (RT w + r) + 4 kg + i, columns v0 + 16 n + r16
+  f4 S[RT];  // S[key][v0 + i] of key 16 (RT w + r) + r16
 #pragma unroll
-  for (int r = 0; r < RT; ++r)
+  for (int r = 0; r < RT; ++r) {
+    const int key = 16 * (RT * w + r) + r16;
 #pragma unroll
-    for (int n = 0; n < NV; ++n)
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const int kr = 16 * (RT * w + r) + 4 * kg + i, vc = v0 + 16 * n + r16;
-        S[r][n][i] = p.h0 && kr < p.Dk && vc < p.Dv ? p.h0[((int64_t)bh * p.Dk + kr) * p.Dv + vc] : 0.0f;
-      }
-
-  for (int c = 0; c < p.NC; ++c) {
-    const int64_t t0 = (int64_t)c * kC, ch = (int64_t)bh * p.NC + c;
-    const float *rows = delta_rows(p, ch);
-#pragma unroll
-    for (int r = 0; r < RT; ++r)
-#pragma unroll
-      for (int n = 0; n < NV; ++n) {
-        bf4 parts[NM];
-        split_parts<NM>(S[r][n], parts);
-#pragma unroll
-        for (int m = 0; m < NM; ++m) *(bf4 *)&St[m][16 * n + r16][16 * (RT * w + r) + 4 * kg] = parts[m];
-        if (p.states) {
-#pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            const int kr = 16 * (RT * w + r) + 4 * kg + i, vc = v0 + 16 * n + r16;
-            if (kr < p.Dk && vc < p.Dv) p.states[(ch * p.Dk + kr) * p.Dv + vc] = S[r][n][i];
-          }
-        }
-      }
-    const int64_t t = t0 + 16 * w + r16;
-    const int have = t < p.L ? p.Dk : 0;
-    bf8 K[KS][NK], Q[KS][NK];
+    for (int i = 0; i < 4; ++i)
+      S[r][i] = p.h0 && key < p.Dk && i < have ? p.h0[((int64_t)bh * p.Dk + key) * p.Dv + v0 + i] : 0.0f;
+  }
+  bf8 K[KS][NK], Q[KS][NK], T[2][NM], P[2][NP], Kt[RT][2][NK];
+  Raw4<IT> v;
+  float fa, be, fc, fd;
+  double GC;
+  auto load_rows = [&](int c) {
+    const float *rows = delta_rows(p, ch0 + c);
+    fa = rows[tok]; be = rows[kC + tok]; fc = rows[2 * kC + tok]; fd = rows[3 * kC + tok];
+    GC = chunk_sum(rows);
+  };
+  auto load_kq = [&](int c) {
+    const __bf16 *k = key_frags<DK, NK>(p.fK, kch0 + c), *q = key_frags<DK, NK>(p.fQ, kch0 + c);
 #pragma unroll
     for (int s = 0; s < KS; ++s) {
-      const int e = 32 * s + 8 * kg;
-      row_frag<IT, NK>(kb + t * p.k.s1 + e, have - e, p.vk, K[s]);
-      row_frag<IT, NK>(qb + t * p.q.s1 + e, have - e, p.vq, Q[s]);
-#pragma unroll
-      for (int n = 0; n < NK; ++n) *(bf8 *)&Kr[n][16 * w + r16][e] = K[s][n];
+      load_frag<NK>(k, kC * DK, w * KS + s, lane, K[s]);
+      load_frag<NK>(q, kC * DK, w * KS + s, lane, Q[s]);
     }
-    const f4 fa = row4(rows, 0, tr), be = row4(rows, 1, tr), fc = row4(rows, 2, tr), fd = row4(rows, 3, tr);
-    const float eC = chunk_decay(rows);
-    lds_barrier();
-    f4 U[NV], O[NV];
+  };
+  auto load_v = [&](int c) {
+    const int64_t t = (int64_t)c * kC + tok;
+    v = load4(vp + t * p.v.s1, t < p.L ? have : 0, p.vv);
+  };
+  auto load_t = [&](int c) {  // T is lower triangular
 #pragma unroll
-    for (int n = 0; n < NV; ++n) {
-      f4 x = 0, o = 0;
-#pragma unroll
-      for (int s = 0; s < KS; ++s) {
-        bf8 B[NM];
-        lds_frag<NM, KP>(&St[0][0][0], BV * KP, 16 * n + r16, 32 * s + 8 * kg, B);
-        x = mma(K[s], B, x);
-        o = mma(Q[s], B, o);
-      }
-      const int vc = v0 + 16 * n + r16;
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const float v = t0 + tr + i < p.L && vc < p.Dv ? Conv<IT>::load(vb + (t0 + tr + i) * p.v.s1 + vc) : 0.0f;
-        U[n][i] = be[i] * fmaf(-fa[i], x[i], v);
-      }
-      O[n] = fd * o;
-      bf4 parts[NM];
-      split_parts<NM>(U[n], parts);
-#pragma unroll
-      for (int m = 0; m < NM; ++m) *(bf4 *)&Rt[m][16 * n + r16][tr] = parts[m];
-    }
-    lds_barrier();
-#pragma unroll
-    for (int s = 0; s < 2; ++s) {  // U = R + (T - I) R; T is lower triangular
-      if (s <= w / 2) {
-        bf8 A[NM];
-#pragma unroll
-        for (int m = 0; m < NM; ++m) A[m] = *(const bf8 *)((const __bf16 *)p.fT + (ch * NM + m) * kFrag + ((2 * w + s) * 64 + lane) * 8);
-#pragma unroll
-        for (int n = 0; n < NV; ++n) {
-          bf8 B[NM];
-          lds_frag<NM, kCP>(&Rt[0][0][0], BV * kCP, 16 * n + r16, 32 * s + 8 * kg, B);
-          U[n] = mma(A, B, U[n]);
-        }
-      }
-    }
-#pragma unroll
-    for (int n = 0; n < NV; ++n) {
-      bf4 parts[NM];
-      split_parts<NM>(U[n], parts);
-#pragma unroll
-      for (int m = 0; m < NM; ++m) *(bf4 *)&Ut[m][16 * n + r16][tr] = parts[m];
-      split_parts<NM>((f4)(fc * U[n]), parts);
-#pragma unroll
-      for (int m = 0; m < NM; ++m) *(bf4 *)&Wt[m][16 * n + r16][tr] = parts[m];
-      if (p.u) {
-        const int vc = v0 + 16 * n + r16;
-        if (vc < p.Dv) {
-#pragma unroll
-          for (int i = 0; i < 4; ++i) p.u[(ch * kC + tr + i) * p.Dv + vc] = U[n][i];
-        }
-      }
-    }
-    lds_barrier();
+    for (int s = 0; s < 2; ++s)
+      if (s <= w / 2) load_frag<NM>((const __bf16 *)p.fT + (ch0 + c) * NM * kFrag, kFrag, 2 * w + s, lane, T[s]);
+  };
+  auto load_p = [&](int c) {
+    const __bf16 *kt = key_frags<DK, NK>(p.fKt, kch0 + c);
 #pragma unroll
     for (int s = 0; s < 2; ++s) {
+#pragma unroll
+      for (int r = 0; r < RT; ++r) load_frag<NK>(kt, kC * DK, 2 * (RT * w + r) + s, lane, Kt[r][s]);
+      if (s <= w / 2) load_frag<NP>((const __bf16 *)p.fP + (ch0 + c) * NP * kFrag, kFrag, 2 * w + s, lane, P[s]);
+    }
+  };
+  load_rows(0);
+  load_kq(0);
+  load_v(0);
+  load_t(0);
+  load_p(0);
+  for (int c = 0; c < p.NC; ++c) {
+    const int64_t t = (int64_t)c * kC + tok, ch = ch0 + c;
+    const int next = c + 1 < p.NC ? c + 1 : c;
+#pragma unroll
+    for (int r = 0; r < RT; ++r) {
+      const int key = 16 * (RT * w + r) + r16;
+      St.put(key, kg, S[r]);
+      if (p.states && key < p.Dkp) *(f4 *)(state_of(p.states, p, ch, vt) + (unsigned)(16 * key + 4 * kg)) = S[r];
+    }
+    lds_barrier();
+    f4 x = 0, o = 0;
+#pragma unroll
+    for (int s = 0; s < KS; ++s) {
+      bf8 A[NM];
+      St.get(s, lane, A);
+      x = mma<NM>(A, K[s], x);
+      o = mma<NP>(A, Q[s], o);
+    }
+    load_kq(next);
+    f4 y = to_f4(v) - fa * x;
+    load_v(next);
+    o *= fd;
+    Xt.put(tok, kg, y);
+    const float bu = be, bc = be * fc, eC = fexp((float)GC);
+    load_rows(next);
+    lds_barrier();
+#pragma unroll
+    for (int s = 0; s < 2; ++s)  // Y = X + (T - I) X
       if (s <= w / 2) {
         bf8 A[NM];
-#pragma unroll
-        for (int m = 0; m < NM; ++m) A[m] = *(const bf8 *)((const __bf16 *)p.fP + (ch * NM + m) * kFrag + ((2 * w + s) * 64 + lane) * 8);
-#pragma unroll
-        for (int n = 0; n < NV; ++n) {
-          bf8 B[NM];
-          lds_frag<NM, kCP>(&Ut[0][0][0], BV * kCP, 16 * n + r16, 32 * s + 8 * kg, B);
-          O[n] = mma(A, B, O[n]);
-        }
+        Xt.get(s, lane, A);
+        y = mma<NM>(A, T[s], y);
       }
-    }
+    load_t(next);
+    Wt.put(tok, kg, bc * y);
+    Ut.put(tok, kg, bu * y);
+    if (p.y) *(f4 *)(value_of(p.y, p, ch, vt) + (unsigned)(16 * tok + 4 * kg)) = y;
+    lds_barrier();
 #pragma unroll
-    for (int n = 0; n < NV; ++n) {
-      const int vc = v0 + 16 * n + r16;
-#pragma unroll
-      for (int i = 0; i < 4; ++i)
-        if (t0 + tr + i < p.L && vc < p.Dv) Conv<IT>::store(ob + (t0 + tr + i) * p.o.s1 + vc, O[n][i]);
-    }
-#pragma unroll
-    for (int r = 0; r < RT; ++r)
-#pragma unroll
-      for (int n = 0; n < NV; ++n) S[r][n] *= eC;
+    for (int r = 0; r < RT; ++r) S[r] *= eC;
 #pragma unroll
     for (int s = 0; s < 2; ++s) {
-      bf8 A[RT][NK];
+      bf8 A[NM];
+      Wt.get(s, lane, A);
 #pragma unroll
-      for (int r = 0; r < RT; ++r) lds_frag_t<NK, KP>(&Kr[0][0][0], kC * KP, 32 * s, 16 * (RT * w + r), lane, A[r]);
-#pragma unroll
-      for (int n = 0; n < NV; ++n) {
-        bf8 B[NM];
-        lds_frag<NM, kCP>(&Wt[0][0][0], BV * kCP, 16 * n + r16, 32 * s + 8 * kg, B);
-#pragma unroll
-        for (int r = 0; r < RT; ++r) S[r][n] = mma(A[r], B, S[r][n]);
-      }
+      for (int r = 0; r < RT; ++r) S[r] = mma<NM>(A, Kt[r][s], S[r]);
     }
-    lds_barrier();  // the keys and Wt are read, the next chunk may write
+#pragma unroll
+    for (int s = 0; s < 2; ++s)
+      if (s <= w / 2) {
+        bf8 A[NP];
+        Ut.get(s, lane, A);
+        o = mma<NP>(A, P[s], o);
+      }
+    load_p(next);
+    store4(op + t * p.o.s1, o, t < p.L ? have : 0, p.vo);
   }
   if (p.last) {
 #pragma unroll
-    for (int r = 0; r < RT; ++r)
+    for (int r = 0; r < RT; ++r) {
+      const int key = 16 * (RT * w + r) + r16;
 #pragma unroll
-      for (int n = 0; n < NV; ++n)
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const int kr = 16 * (RT * w + r) + 4 * kg + i, vc = v0 + 16 * n + r16;
-          if (kr < p.Dk && vc < p.Dv) p.last[((int64_t)bh * p.Dk + kr) * p.Dv + vc] = S[r][n][i];
-        }
+      for (int i = 0; i < 4; ++i)
+        if (key < p.Dk && i < have) p.last[((int64_t)bh * p.Dk + key) * p.Dv + v0 + i] = S[r][i];
+    }
   }
 }
 
@@ -350,8 +347,7 @@ template <typename IT, int DK>
 static hipError_t delta_fwd(const DeltaParams &p, hipStream_t s) {
   const unsigned heads = (unsigned)(p.B * p.H);
   hipLaunchKernelGGL((k_delta_prep<IT, DK, false>), dim3(heads * (unsigned)p.NC), dim3(kDT), 0, s, p);
-  constexpr int NV = 1;
-  hipLaunchKernelGGL((k_delta_fwd<IT, DK, NV>), dim3(heads * (unsigned)((p.Dv + 16 * NV - 1) / (16 * NV))), dim3(kDT), 0, s, p);
+  hipLaunchKernelGGL((k_delta_fwd<IT, DK>), dim3(heads * (unsigned)p.VT), dim3(kDT), 0, s, p);
   return hipGetLastError();
 }
 template <typename IT>
@@ -362,7 +358,7 @@ hipError_t launch_delta_fwd(const DeltaParams &p, int dtype, hipStream_t s) {
   return dtype == 0 ? delta_fwd_k<float>(p, s) : dtype == 1 ? delta_fwd_k<bf16_t>(p, s) : delta_fwd_k<f16_t>(p, s);
 }
 
-// The transposed prep of the backward.
+// The backward's preparation.
 template <typename IT>
 static hipError_t delta_prep_t(const DeltaParams &p, hipStream_t s) {
   const dim3 grid((unsigned)(p.B * p.H) * (unsigned)p.NC);

@@ -3,17 +3,25 @@
 // Per batch row and value head, with the state S (Dk, Dv):
 //   S' = e^{g_t} S_{t-1},  u_t = beta_t (v_t - S'^T k_t),  S_t = S' + k_t u_t^T,  o_t = scale S_t^T q_t.
 // Over a chunk of kC tokens with G = cumsum(g) and the entering state S0 this is
-//   X = V - e^G K S0,  R = beta X,  U = T R,  T = (I + strictly lower(beta_i e^{G_i - G_j} k_i.k_j))^-1
+//   X = V - e^G K S0,  Y = T X,  U = beta Y,  T = (I + strictly lower(e^{G_i - G_j} k_i.k_j beta_j))^-1
 //   O = scale e^G Q S0 + P U,  P_ij = scale e^{G_i - G_j} q_i.k_j (j <= i),  S1 = e^{G_C} S0 + K^T (e^{G_C - G} U)
 // so that everything but the factors is products of 64-row tiles, which run on the matrix cores.
 // Every exponent is a difference of later minus earlier cumulative decays, taken in float64.
 //
-// Products take bf16 operands and accumulate in float32.  A float32 operand is held as the sum of NS
-// bf16 parts (x = p0 + p1 + ..., each the rounding of what the earlier ones leave), and a product of
-// parts i and j is formed where i + j < the larger count: bf16 inputs are one part and exact, fp16
-// inputs two and exact.  With two parts an operand is off by 2^-18 of itself at most, with three by
-// 2^-26; one part alone (2^-9) would show in the float32 state and in dg.
+// Products take bf16 operands and accumulate in float32.  A float32 operand is held as the sum of
+// bf16 parts (x = p0 + p1 + ..., each the rounding of what the earlier ones leave: 8 significant bits
+// each, so one part is off by 2^-8 of the operand at most, two by 2^-16, three by 2^-24), and a product
+// of parts i and j is formed where i + j is below the count of parts kept.  bf16 inputs are one part and
+// exact, fp16 inputs two and exact, float32 inputs three.  The state, its gradient and everything on the
+// way to them have three parts, whatever the inputs' type: they are float32 outputs, as dg is.  What
+// only reaches outputs of 16 bits has two (DParts::out).
+//
+// Where the contraction index is stored.  A lane's 8 elements of a fragment of 32 are, in this order,
+// 4 kg + 0..3 and 16 + 4 kg + 0..3 (kg = lane / 16): the order in which lanes hold the rows of two
+// 16 x 16 results, so that results and transposing LDS reads become operands without a permutation.
 #pragma once
+
+#include <type_traits>
 
 #include "ssm_device.hpp"
 #include "ssm_internal.hpp"
@@ -29,15 +37,14 @@ typedef float f8 __attribute__((ext_vector_type(8)));
 typedef short s4 __attribute__((ext_vector_type(4)));
 
 constexpr int kC = kDeltaChunk;   // tokens per chunk
-constexpr int kCP = kC + 8;       // LDS row of kC bf16, padded by 16 bytes: rows on distinct bank groups
-constexpr int kDT = 256;          // threads of a workgroup: wavefront w owns token rows 16 w .. 16 w + 15
+constexpr int kDT = 256;          // threads of the walks: wavefront w owns tokens 16 w .. 16 w + 15
 constexpr int kFrag = kC * kC;    // elements of one part of a 64 x 64 matrix stored as operand fragments
 
-// Parts of an input of type IT, and of float32 intermediates beside it.
+// Parts of an input of type IT, of float32 intermediates beside it, and of those that only reach outputs of type IT.
 template <typename IT> struct DParts;
-template <> struct DParts<bf16_t> { static constexpr int in = 1, mid = 2; };
-template <> struct DParts<f16_t> { static constexpr int in = 2, mid = 2; };
-template <> struct DParts<float> { static constexpr int in = 3, mid = 3; };
+template <> struct DParts<bf16_t> { static constexpr int in = 1, mid = 3, out = 2; };
+template <> struct DParts<f16_t> { static constexpr int in = 2, mid = 3, out = 2; };
+template <> struct DParts<float> { static constexpr int in = 3, mid = 3, out = 3; };
 
 template <int N, typename F, typename V>
 __device__ __forceinline__ void split_parts(F x, V (&p)[N]) {
@@ -48,74 +55,100 @@ __device__ __forceinline__ void split_parts(F x, V (&p)[N]) {
   }
 }
 
-// acc += a b over one step of 32: lane l holds row (a) or column (b) l % 16, elements 8 (l / 16) + j
-// of the step; of the 16 x 16 result it holds column l % 16, rows 4 (l / 16) + i.
-template <int NA, int NB>
+// acc += a b over one step of 32: lane l holds row (a) or column (b) l % 16, of the 16 x 16 result
+// column l % 16, rows 4 (l / 16) + i.  The first M parts are kept, the smallest products come first.
+template <int M, int NA, int NB>
 __device__ __forceinline__ f4 mma(const bf8 (&a)[NA], const bf8 (&b)[NB], f4 acc) {
-  constexpr int M = NA > NB ? NA : NB;
 #pragma unroll
-  for (int s = M - 1; s >= 0; --s)  // the smallest products first
+  for (int s = M - 1; s >= 0; --s)
 #pragma unroll
     for (int i = 0; i < NA; ++i)
       if (s - i >= 0 && s - i < NB) acc = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a[i], b[s - i], acc, 0, 0, 0);
   return acc;
 }
 
-// Operand fragment of one step from an LDS matrix whose rows are the operand's rows / columns.
-template <int N, int PITCH>
-__device__ __forceinline__ void lds_frag(const __bf16 *m, int part, int row, int col, bf8 (&f)[N]) {
-#pragma unroll
-  for (int n = 0; n < N; ++n) f[n] = *(const bf8 *)(m + n * part + row * PITCH + col);
-}
-// The same from a matrix stored the other way round (rows are the contraction index): the transposing
-// LDS read gives lane l of 16 the column l of the 4 rows whose 8-byte pieces the 16 lanes address.
-template <int N, int PITCH>
-__device__ __forceinline__ void lds_frag_t(const __bf16 *m, int part, int k0, int col0, int lane, bf8 (&f)[N]) {
-  const int r = k0 + (lane / 16) * 8 + (lane % 16) / 4, c = col0 + (lane % 4) * 4;
-#pragma unroll
-  for (int n = 0; n < N; ++n) {
-    typedef __attribute__((address_space(3))) s4 *P;
-    const __bf16 *p = m + n * part + r * PITCH + c;
-    const s4 a = __builtin_amdgcn_ds_read_tr16_b64_v4i16((P)p);
-    const s4 b = __builtin_amdgcn_ds_read_tr16_b64_v4i16((P)(p + 4 * PITCH));
-    f[n] = __builtin_bit_cast(bf8, __builtin_shufflevector(a, b, 0, 1, 2, 3, 4, 5, 6, 7));
-  }
+// The transposing LDS read: lane l of 16 gets column l of the 4 rows whose 8-byte pieces the 16 lanes address.
+__device__ __forceinline__ bf8 read_tr(const __bf16 *lo, const __bf16 *hi) {
+  typedef __attribute__((address_space(3))) s4 *P;
+  const s4 a = __builtin_amdgcn_ds_read_tr16_b64_v4i16((P)lo), b = __builtin_amdgcn_ds_read_tr16_b64_v4i16((P)hi);
+  return __builtin_bit_cast(bf8, __builtin_shufflevector(a, b, 0, 1, 2, 3, 4, 5, 6, 7));
 }
 
-// Eight consecutive elements of a row as floats, 0 from `have` on; vec: the row is 16-byte aligned
-// and `have` is a multiple of 8.
-template <typename IT>
-__device__ __forceinline__ f8 row8(const IT *p, int have, bool vec) {
-  f8 x = 0;
-  if (vec) {
-    if (have > 0) {
-      if constexpr (sizeof(IT) == 4) {
-        const f4 a = *(const f4 *)p, b = *(const f4 *)(p + 4);
-        x = __builtin_shufflevector(a, b, 0, 1, 2, 3, 4, 5, 6, 7);
-      } else {
-        struct alignas(16) Pack { IT e[8]; };
-        const Pack k = *(const Pack *)p;
+// An intermediate of R rows (keys or tokens, the next product's contraction index) by 16 columns of v in
+// LDS, N parts.  A row is four 8-byte pieces; rows 8..15 of every 16 swap its halves, so that neither the
+// writes (16 rows by two pieces in 32 lanes) nor the reads (8 rows by four) meet twice in a bank.
+template <int N, int R> struct VTile {
+  __bf16 e[N][R * 16];
+  // x: row `row`, columns 4 kg + i
+  __device__ __forceinline__ void put(int row, int kg, f4 x) {
+    bf4 p[N];
+    split_parts<N>(x, p);
+    put_parts(row, kg, p);
+  }
+  __device__ __forceinline__ void put_parts(int row, int kg, const bf4 (&p)[N]) {
 #pragma unroll
-        for (int j = 0; j < 8; ++j) x[j] = Conv<IT>::load(&k.e[j]);
-      }
-    }
+    for (int n = 0; n < N; ++n) *(bf4 *)&e[n][row * 16 + ((kg ^ ((row >> 2) & 2)) * 4)] = p[n];
+  }
+  // operand of rows 32 s .. 32 s + 31: lane = column of v
+  __device__ __forceinline__ void get(int s, int lane, bf8 (&f)[N]) const {
+    const int row = 32 * s + 4 * (lane / 16) + (lane % 16) / 4, at = row * 16 + ((lane % 4) ^ ((row >> 2) & 2)) * 4;
+#pragma unroll
+    for (int n = 0; n < N; ++n) f[n] = read_tr(&e[n][at], &e[n][at + 256]);
+  }
+};
+
+// Fragment `at` (of 64 lanes x 8) of an array of N parts, `part` elements each.
+template <int N>
+__device__ __forceinline__ void load_frag(const __bf16 *m, int64_t part, int at, int lane, bf8 (&f)[N]) {
+#pragma unroll
+  for (int n = 0; n < N; ++n) f[n] = *(const bf8 *)(m + n * part + at * 512 + (unsigned)(lane * 8));
+}
+
+__device__ __forceinline__ int wave_id() { return __builtin_amdgcn_readfirstlane(threadIdx.x / 64); }
+
+// Four consecutive elements of a row, 0 from `have` on; vec: rows are whole words of 4 elements.
+template <typename IT> struct alignas(4 * sizeof(IT)) Raw4 { IT e[4]; };
+template <typename IT>
+__device__ __forceinline__ Raw4<IT> load4(const IT *p, int have, bool vec) {
+  Raw4<IT> x{};
+  if (vec) {
+    if (have > 0) x = *(const Raw4<IT> *)p;
   } else {
 #pragma unroll
-    for (int j = 0; j < 8; ++j)
-      if (j < have) x[j] = Conv<IT>::load(p + j);
+    for (int j = 0; j < 4; ++j)
+      if (j < have) x.e[j] = p[j];
   }
   return x;
 }
-// The same as operand parts; bf16 rows need no conversion.
+template <typename IT>
+__device__ __forceinline__ f4 to_f4(const Raw4<IT> &x) {
+  f4 r;
+#pragma unroll
+  for (int j = 0; j < 4; ++j) r[j] = Conv<IT>::load(&x.e[j]);
+  return r;
+}
+// The same as operand parts.
 template <typename IT, int N>
-__device__ __forceinline__ void row_frag(const IT *p, int have, bool vec, bf8 (&f)[N]) {
-  if constexpr (sizeof(IT) == 2 && N == 1) {
-    if (vec) {
-      f[0] = have > 0 ? *(const bf8 *)p : (bf8)(__bf16)0.0f;
-      return;
-    }
+__device__ __forceinline__ void to_parts(const Raw4<IT> &x, bf4 (&p)[N]) {
+  if constexpr (std::is_same_v<IT, bf16_t> && N == 1) p[0] = __builtin_bit_cast(bf4, x);
+  else split_parts<N>(to_f4<IT>(x), p);
+}
+template <typename IT>
+__device__ __forceinline__ void store4(IT *p, f4 x, int have, bool vec) {
+  Raw4<IT> r;
+  if constexpr (std::is_same_v<IT, bf16_t>) {
+    r = __builtin_bit_cast(Raw4<IT>, __builtin_convertvector(x, bf4));
+  } else {
+#pragma unroll
+    for (int j = 0; j < 4; ++j) Conv<IT>::store(&r.e[j], x[j]);
   }
-  split_parts<N>(row8<IT>(p, have, vec), f);
+  if (vec) {
+    if (have > 0) *(Raw4<IT> *)p = r;
+  } else {
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+      if (j < have) p[j] = r.e[j];
+  }
 }
 
 // Element `at` of a tensor that is float32 or of type IT.
@@ -147,7 +180,22 @@ __device__ __forceinline__ void delta_tile(int nv, int heads, int &bh, int &vt) 
 // Row factors of a chunk, kDeltaRows floats: [0] a = |k|^-1 e^G, [1] beta, [2] c = |k|^-1 e^{G_C - G},
 // [3] d = scale |q|^-1 e^G, [4] |k|^-1, [5] scale |q|^-1 (the norms are 1 without qk_norm), [6..7] G as float64.
 __device__ __forceinline__ const float *delta_rows(const DeltaParams &p, int64_t ch) { return p.rows + ch * kDeltaRows; }
-__device__ __forceinline__ f4 row4(const float *rows, int which, int r) { return *(const f4 *)(rows + which * kC + r); }
-__device__ __forceinline__ float chunk_decay(const float *rows) { return fexp((float)((const double *)(rows + 6 * kC))[kC - 1]); }
+__device__ __forceinline__ double chunk_sum(const float *rows) { return ((const double *)(rows + 6 * kC))[kC - 1]; }
+
+// Arrays of operand fragments.  Per chunk and key head, in DParts::in parts of 64 DK: the rows of K and Q
+// (token tile w, step s of keys: fragment w DK/32 + s) and their columns (key tile t, step s of tokens:
+// fragment 2 t + s).  Per chunk and head, of kFrag each: T and P or their transposes (token tile w, step s:
+// fragment 2 w + s).
+template <int DK, int N>
+__device__ __forceinline__ const __bf16 *key_frags(const void *f, int64_t kch) { return (const __bf16 *)f + kch * N * kC * DK; }
+
+// The states and the values by chunk, head and 16 columns of v: element (row, column)
+// (rows are added as 32-bit lane offsets).
+__device__ __forceinline__ float *state_of(float *m, const DeltaParams &p, int64_t ch, int vt) {
+  return m + (ch * p.VT + vt) * p.Dkp * 16;
+}
+__device__ __forceinline__ float *value_of(float *m, const DeltaParams &p, int64_t ch, int vt) {
+  return m + (ch * p.VT + vt) * kC * 16;
+}
 
 }  // namespace ssm

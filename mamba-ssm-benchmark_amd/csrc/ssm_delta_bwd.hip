@@ -1,17 +1,18 @@
-// Gated delta rule, backward of the chunked form (notation: ssm_delta.hpp).  With D = dS1, the gradient of
-// the state leaving a chunk, a = |k|^-1 e^G, c = |k|^-1 e^{G_C - G}, d = scale |q|^-1 e^G:
-//   dU = P^T dO + c K D,  dR = T^T dU,  dV = beta dR
+// Gated delta rule, backward of the chunked form (notation: ssm_delta.hpp).  With D the gradient of the state
+// leaving a chunk, a = |k|^-1 e^G, c = |k|^-1 e^{G_C - G}, d = scale |q|^-1 e^G, e_ij = e^{G_i - G_j}, and here
+// T = (I + strictly lower(beta_i e_ij k_i.k_j))^-1:
+//   dU = P^T dO + c K D,  dR = T^T dU,  dV = beta dR,  dbeta = dR.Y (row dots)
 //   dS0 = e^{G_C} D + Q^T (d dO) - K^T (beta a dR)
-// k_delta_bwd walks the chunks backward, one workgroup per 16 NV columns of v like the forward, and
-// leaves D and dR of every chunk; k_delta_grad then treats every chunk by itself, one workgroup per
-// (batch row, key head, chunk), adding the value heads that share the key head in registers.  With
-// A = dO U^T and N = dR U^T, k^ and q^ the normalised rows and e_ij = e^{G_i - G_j}:
-//   dq^ = scale (e^G dO S0^T + (A e)_{j <= i} K^)
-//   dk^ = e^{G_C - G} U D^T + (scale A e)^T_{j <= i} Q^ - (beta N e and its transpose)_{j < i} K^ - beta e^G dR S0^T
-//   dbeta_i = dR_i.v_i - e^{G_i} k^_i.(dR S0^T)_i - sum_{j < i} N_ij e_ij k^_i.k^_j
-//   dG_i, G's gradient: every factor e^x times its derivative, x's terms of G with their signs; dg is its
-//   sum from i to the chunk's end.  Each product enters a row and a column sum with the same value, so
-//   that what does not straddle a token cancels to rounding.
+// k_delta_bwd walks the chunks backward, one workgroup per 16 columns of v like the forward, and leaves D and
+// dR of every chunk; k_delta_grad then treats every chunk by itself, one workgroup per (batch row, key head,
+// chunk), adding the value heads that share the key head in registers.  With U = beta Y and the lower
+// triangular J_ij = scale |q_i|^-1 |k_j|^-1 e_ij dO_i.U_j, H_ij = beta_i |k_i|^-1 |k_j|^-1 e_ij dR_i.U_j (i > j):
+//   dq' = d dO S0^T + J K,   dk' = c U D^T - beta a dR S0^T + J^T Q - (H + H^T) K
+// of which dq, dk are what the norms leave: dq = dq' - q (q.dq') / (|q|^2), likewise dk.
+// G enters O_i by a factor e^{G_i}, and every path from v_i by e^{-G_i}, whence G's gradient is dO_i.O_i -
+// dV_i.v_i, with dO_i.O_i = q_i.dq'_i since O is linear in q.  The state that leaves has the factor e^{G_C}:
+//   dg_t = <D, S1> + sum over i >= t of (q_i.dq'_i - dV_i.v_i),  <D, S1> = e^{G_C} <D, S0> + sum_j k_j.(c U D^T)_j
+// Every chunk starts from its own <D, S1>, so that at most 64 terms are added to it.
 #include "ssm_delta.hpp"
 #include "ssm_dpp.hpp"
 
@@ -19,555 +20,465 @@ namespace ssm {
 
 hipError_t launch_delta_prep_t(const DeltaParams &p, int dtype, hipStream_t s);
 
-template <typename IT, int DK, int NV>
-__global__ void __launch_bounds__(kDT) k_delta_bwd(const DeltaParams p) {
-  constexpr int NK = DParts<IT>::in, NM = DParts<IT>::mid, KS = DK / 32, KP = DK + 8, BV = 16 * NV, RT = DK / 64;
-  __shared__ __align__(16) __bf16 Kr[NK][kC][KP], Qr[NK][kC][KP];  // keys and queries, row per token
-  __shared__ __align__(16) __bf16 Dt[NM][BV][KP];                  // D, row per column of v
-  __shared__ __align__(16) __bf16 Ot[NK][BV][kCP];                 // dO, row per column of v; below d dO, dU, -beta a dR
-  __shared__ __align__(16) __bf16 Et[NM][BV][kCP], Xt[NM][BV][kCP], Yt[NM][BV][kCP];
-  const int tid = threadIdx.x, lane = tid % 64, w = tid / 64, r16 = lane % 16, kg = lane / 16;
+template <typename IT, int DK>
+__global__ void __launch_bounds__(kDT, DK * sizeof(IT) <= 256 ? 2 : 1) k_delta_bwd(const DeltaParams p) {
+  constexpr int NK = DParts<IT>::in, NM = DParts<IT>::mid, KS = DK / 32, RT = DK / 64;
+  __shared__ __align__(16) VTile<NM, DK> Dt;
+  __shared__ __align__(16) VTile<NK, kC> Ot;          // dO
+  __shared__ __align__(16) VTile<NM, kC> Et, Xt, Yt;  // d dO, dU, -beta a dR
+  const int tid = threadIdx.x, lane = tid % 64, w = wave_id(), r16 = lane % 16, kg = lane / 16;
   int bh, vt;
-  delta_tile((p.Dv + BV - 1) / BV, (int)p.B * p.H, bh, vt);
-  const int b = bh / p.H, h = bh % p.H, hk = h / (p.H / p.Hk), v0 = vt * BV;
-  const int tr = 16 * w + 4 * kg;
-  const IT *kb = (const IT *)p.k.p + b * p.k.s0 + hk * p.k.s2, *qb = (const IT *)p.q.p + b * p.q.s0 + hk * p.q.s2;
-  const IT *ob = (const IT *)p.dout.p + b * p.dout.s0 + h * p.dout.s2;
-  IT *vb = (IT *)p.dv.p + b * p.dv.s0 + h * p.dv.s2;
+  delta_tile(p.VT, (int)p.B * p.H, bh, vt);
+  const int b = bh / p.H, h = bh % p.H, hk = h / (p.H / p.Hk), v0 = 16 * vt + 4 * kg, have = p.Dv - v0;
+  const int tok = 16 * w + r16;
+  const IT *dop = (const IT *)p.dout.p + b * p.dout.s0 + h * p.dout.s2 + v0;
+  IT *dvp = (IT *)p.dv.p + b * p.dv.s0 + h * p.dv.s2 + v0;
+  const int64_t ch0 = (int64_t)bh * p.NC, kch0 = ((int64_t)b * p.Hk + hk) * p.NC;
 
-  f4 D[RT][NV];  // rows 16 (RT w + r) + 4 kg + i, columns v0 + 16 n + r16
+  f4 D[RT];  // D[key][v0 + i] of key 16 (RT w + r) + r16
 #pragma unroll
-  for (int r = 0; r < RT; ++r)
+  for (int r = 0; r < RT; ++r) {
+    const int key = 16 * (RT * w + r) + r16;
 #pragma unroll
-    for (int n = 0; n < NV; ++n)
+    for (int i = 0; i < 4; ++i)
+      D[r][i] = p.dlast && key < p.Dk && i < have ? p.dlast[((int64_t)bh * p.Dk + key) * p.Dv + v0 + i] : 0.0f;
+  }
+  bf8 K[KS][NK], T[2][NM], P[2][NM], Kt[RT][2][NK], Qt[RT][2][NK];
+  Raw4<IT> go;
+  float fa, be, fc, fd;
+  double GC;
+  auto load_rows = [&](int c) {
+    const float *rows = delta_rows(p, ch0 + c);
+    fa = rows[tok]; be = rows[kC + tok]; fc = rows[2 * kC + tok]; fd = rows[3 * kC + tok];
+    GC = chunk_sum(rows);
+  };
+  auto load_o = [&](int c) {
+    const int64_t t = (int64_t)c * kC + tok;
+    go = load4(dop + t * p.dout.s1, t < p.L ? have : 0, p.vdo);
+  };
+  auto load_kp = [&](int c) {  // the transposes of T and P are upper triangular
+    const __bf16 *k = key_frags<DK, NK>(p.fK, kch0 + c);
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const int kr = 16 * (RT * w + r) + 4 * kg + i, vc = v0 + 16 * n + r16;
-        D[r][n][i] = p.dlast && kr < p.Dk && vc < p.Dv ? p.dlast[((int64_t)bh * p.Dk + kr) * p.Dv + vc] : 0.0f;
-      }
-
-  for (int c = p.NC - 1; c >= 0; --c) {
-    const int64_t t0 = (int64_t)c * kC, ch = (int64_t)bh * p.NC + c;
-    const float *rows = delta_rows(p, ch);
+    for (int s = 0; s < KS; ++s) load_frag<NK>(k, kC * DK, w * KS + s, lane, K[s]);
 #pragma unroll
-    for (int r = 0; r < RT; ++r)
+    for (int s = 0; s < 2; ++s)
+      if (s >= w / 2) load_frag<NM>((const __bf16 *)p.fP + (ch0 + c) * NM * kFrag, kFrag, 2 * w + s, lane, P[s]);
+  };
+  auto load_t = [&](int c) {
 #pragma unroll
-      for (int n = 0; n < NV; ++n) {
-        bf4 parts[NM];
-        split_parts<NM>(D[r][n], parts);
+    for (int s = 0; s < 2; ++s)
+      if (s >= w / 2) load_frag<NM>((const __bf16 *)p.fT + (ch0 + c) * NM * kFrag, kFrag, 2 * w + s, lane, T[s]);
+  };
+  auto load_cols = [&](int c) {
+    const __bf16 *kt = key_frags<DK, NK>(p.fKt, kch0 + c), *qt = key_frags<DK, NK>(p.fQt, kch0 + c);
 #pragma unroll
-        for (int m = 0; m < NM; ++m) *(bf4 *)&Dt[m][16 * n + r16][16 * (RT * w + r) + 4 * kg] = parts[m];
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const int kr = 16 * (RT * w + r) + 4 * kg + i, vc = v0 + 16 * n + r16;
-          if (kr < p.Dk && vc < p.Dv) p.dstates[(ch * p.Dk + kr) * p.Dv + vc] = D[r][n][i];
-        }
-      }
-    const int64_t t = t0 + 16 * w + r16;
-    const int have = t < p.L ? p.Dk : 0;
-    bf8 K[KS][NK];
-#pragma unroll
-    for (int s = 0; s < KS; ++s) {
-      const int e = 32 * s + 8 * kg;
-      bf8 Q[NK];
-      row_frag<IT, NK>(kb + t * p.k.s1 + e, have - e, p.vk, K[s]);
-      row_frag<IT, NK>(qb + t * p.q.s1 + e, have - e, p.vq, Q);
-#pragma unroll
-      for (int n = 0; n < NK; ++n) {
-        *(bf8 *)&Kr[n][16 * w + r16][e] = K[s][n];
-        *(bf8 *)&Qr[n][16 * w + r16][e] = Q[n];
-      }
-    }
-    const f4 fa = row4(rows, 0, tr), be = row4(rows, 1, tr), fc = row4(rows, 2, tr), fd = row4(rows, 3, tr);
-    const float eC = chunk_decay(rows);
-#pragma unroll
-    for (int n = 0; n < NV; ++n) {
-      const int vc = v0 + 16 * n + r16;
-      f4 x;
-#pragma unroll
-      for (int i = 0; i < 4; ++i)
-        x[i] = t0 + tr + i < p.L && vc < p.Dv ? Conv<IT>::load(ob + (t0 + tr + i) * p.dout.s1 + vc) : 0.0f;
-      bf4 in[NK], mid[NM];
-      split_parts<NK>(x, in);
-#pragma unroll
-      for (int m = 0; m < NK; ++m) *(bf4 *)&Ot[m][16 * n + r16][tr] = in[m];
-      split_parts<NM>((f4)(fd * x), mid);
-#pragma unroll
-      for (int m = 0; m < NM; ++m) *(bf4 *)&Et[m][16 * n + r16][tr] = mid[m];
-    }
-    lds_barrier();
-    f4 X[NV];
-#pragma unroll
-    for (int n = 0; n < NV; ++n) {
-      f4 x = 0;
-#pragma unroll
-      for (int s = 0; s < KS; ++s) {
-        bf8 B[NM];
-        lds_frag<NM, KP>(&Dt[0][0][0], BV * KP, 16 * n + r16, 32 * s + 8 * kg, B);
-        x = mma(K[s], B, x);
-      }
-      X[n] = fc * x;
-    }
-#pragma unroll
-    for (int s = 0; s < 2; ++s) {  // P^T is upper triangular
-      if (s >= w / 2) {
-        bf8 A[NM];
-#pragma unroll
-        for (int m = 0; m < NM; ++m) A[m] = *(const bf8 *)((const __bf16 *)p.fP + (ch * NM + m) * kFrag + ((2 * w + s) * 64 + lane) * 8);
-#pragma unroll
-        for (int n = 0; n < NV; ++n) {
-          bf8 B[NK];
-          lds_frag<NK, kCP>(&Ot[0][0][0], BV * kCP, 16 * n + r16, 32 * s + 8 * kg, B);
-          X[n] = mma(A, B, X[n]);
-        }
-      }
-    }
-#pragma unroll
-    for (int n = 0; n < NV; ++n) {
-      bf4 parts[NM];
-      split_parts<NM>(X[n], parts);
-#pragma unroll
-      for (int m = 0; m < NM; ++m) *(bf4 *)&Xt[m][16 * n + r16][tr] = parts[m];
-    }
-    lds_barrier();
-#pragma unroll
-    for (int s = 0; s < 2; ++s) {
-      if (s >= w / 2) {
-        bf8 A[NM];
-#pragma unroll
-        for (int m = 0; m < NM; ++m) A[m] = *(const bf8 *)((const __bf16 *)p.fT + (ch * NM + m) * kFrag + ((2 * w + s) * 64 + lane) * 8);
-#pragma unroll
-        for (int n = 0; n < NV; ++n) {
-          bf8 B[NM];
-          lds_frag<NM, kCP>(&Xt[0][0][0], BV * kCP, 16 * n + r16, 32 * s + 8 * kg, B);
-          X[n] = mma(A, B, X[n]);
-        }
-      }
-    }
-#pragma unroll
-    for (int n = 0; n < NV; ++n) {
-      bf4 parts[NM];
-      split_parts<NM>((f4)(-be * fa * X[n]), parts);
-#pragma unroll
-      for (int m = 0; m < NM; ++m) *(bf4 *)&Yt[m][16 * n + r16][tr] = parts[m];
-      const int vc = v0 + 16 * n + r16;
-      if (vc < p.Dv) {
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          p.dr[(ch * kC + tr + i) * p.Dv + vc] = X[n][i];
-          if (t0 + tr + i < p.L) Conv<IT>::store(vb + (t0 + tr + i) * p.dv.s1 + vc, be[i] * X[n][i]);
-        }
-      }
-    }
-    lds_barrier();
-#pragma unroll
-    for (int r = 0; r < RT; ++r)
-#pragma unroll
-      for (int n = 0; n < NV; ++n) D[r][n] *= eC;
-#pragma unroll
-    for (int s = 0; s < 2; ++s) {
-      bf8 A[RT][NK], Q[RT][NK];
+    for (int s = 0; s < 2; ++s)
 #pragma unroll
       for (int r = 0; r < RT; ++r) {
-        lds_frag_t<NK, KP>(&Kr[0][0][0], kC * KP, 32 * s, 16 * (RT * w + r), lane, A[r]);
-        lds_frag_t<NK, KP>(&Qr[0][0][0], kC * KP, 32 * s, 16 * (RT * w + r), lane, Q[r]);
+        load_frag<NK>(kt, kC * DK, 2 * (RT * w + r) + s, lane, Kt[r][s]);
+        load_frag<NK>(qt, kC * DK, 2 * (RT * w + r) + s, lane, Qt[r][s]);
       }
+  };
+  load_rows(p.NC - 1);
+  load_o(p.NC - 1);
+  load_kp(p.NC - 1);
+  load_t(p.NC - 1);
+  load_cols(p.NC - 1);
+  for (int c = p.NC - 1; c >= 0; --c) {
+    const int64_t t = (int64_t)c * kC + tok, ch = ch0 + c;
+    const int next = c ? c - 1 : 0;
 #pragma unroll
-      for (int n = 0; n < NV; ++n) {
-        bf8 E[NM], Y[NM];
-        lds_frag<NM, kCP>(&Et[0][0][0], BV * kCP, 16 * n + r16, 32 * s + 8 * kg, E);
-        lds_frag<NM, kCP>(&Yt[0][0][0], BV * kCP, 16 * n + r16, 32 * s + 8 * kg, Y);
+    for (int r = 0; r < RT; ++r) {
+      const int key = 16 * (RT * w + r) + r16;
+      Dt.put(key, kg, D[r]);
+      if (key < p.Dkp) *(f4 *)(state_of(p.dstates, p, ch, vt) + (unsigned)(16 * key + 4 * kg)) = D[r];
+    }
+    {
+      bf4 o[NK];
+      to_parts<IT, NK>(go, o);
+      Ot.put_parts(tok, kg, o);
+      Et.put(tok, kg, fd * to_f4(go));
+    }
+    load_o(next);
+    const float cc = fc, bu = be, by = -be * fa, eC = fexp((float)GC);
+    load_rows(next);
+    lds_barrier();
+    f4 x = 0;
 #pragma unroll
-        for (int r = 0; r < RT; ++r) D[r][n] = mma(A[r], Y, mma(Q[r], E, D[r][n]));
+    for (int s = 0; s < KS; ++s) {
+      bf8 A[NM];
+      Dt.get(s, lane, A);
+      x = mma<NM>(A, K[s], x);
+    }
+    x *= cc;
+#pragma unroll
+    for (int s = 0; s < 2; ++s)
+      if (s >= w / 2) {
+        bf8 A[NK];
+        Ot.get(s, lane, A);
+        x = mma<NM>(A, P[s], x);
       }
+    load_kp(next);
+    Xt.put(tok, kg, x);
+    lds_barrier();
+#pragma unroll
+    for (int s = 0; s < 2; ++s)  // dR = dU + (T^T - I) dU
+      if (s >= w / 2) {
+        bf8 A[NM];
+        Xt.get(s, lane, A);
+        x = mma<NM>(A, T[s], x);
+      }
+    load_t(next);
+    Yt.put(tok, kg, by * x);
+    *(f4 *)(value_of(p.dr, p, ch, vt) + (unsigned)(16 * tok + 4 * kg)) = x;
+    store4(dvp + t * p.dv.s1, (f4)(bu * x), t < p.L ? have : 0, p.vdv);
+#pragma unroll
+    for (int r = 0; r < RT; ++r) D[r] *= eC;
+#pragma unroll
+    for (int s = 0; s < 2; ++s) {
+      bf8 A[NM];
+      Et.get(s, lane, A);
+#pragma unroll
+      for (int r = 0; r < RT; ++r) D[r] = mma<NM>(A, Qt[r][s], D[r]);
     }
     lds_barrier();
+#pragma unroll
+    for (int s = 0; s < 2; ++s) {
+      bf8 A[NM];
+      Yt.get(s, lane, A);
+#pragma unroll
+      for (int r = 0; r < RT; ++r) D[r] = mma<NM>(A, Kt[r][s], D[r]);
+    }
+    load_cols(next);
   }
   if (p.dh0) {
 #pragma unroll
-    for (int r = 0; r < RT; ++r)
+    for (int r = 0; r < RT; ++r) {
+      const int key = 16 * (RT * w + r) + r16;
 #pragma unroll
-      for (int n = 0; n < NV; ++n)
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const int kr = 16 * (RT * w + r) + 4 * kg + i, vc = v0 + 16 * n + r16;
-          if (kr < p.Dk && vc < p.Dv) p.dh0[((int64_t)bh * p.Dk + kr) * p.Dv + vc] = D[r][n][i];
-        }
-  }
-}
-
-// Element (row, col) of an LDS matrix of N parts.
-template <int N, int PITCH>
-__device__ __forceinline__ float lds_elem(const __bf16 *m, int part, int row, int col) {
-  float s = 0;
-#pragma unroll
-  for (int n = N - 1; n >= 0; --n) s += (float)m[n * part + row * PITCH + col];
-  return s;
-}
-
-template <typename IT, int DK>
-__global__ void __launch_bounds__(kDT) k_delta_grad(const DeltaParams p) {
-  constexpr int NK = DParts<IT>::in, NM = DParts<IT>::mid, KS = DK / 32, KP = DK + 8, CT = DK / 64;
-  constexpr int SV = 32, SP = SV + 8;  // columns of v staged at a time
-  constexpr int kSlab = (NK + 2 * NM) * kC * SP, kE = NM * kC * kCP;
-  __shared__ __align__(16) __bf16 Kr[NK][kC][KP], Qr[NK][kC][KP];
-  __shared__ __align__(16) __bf16 buf[kSlab > kE ? kSlab : kE];  // slabs of dO, dR, U; then a 64 x 64 operand
-  __shared__ double Gs[kC];
-  __shared__ float red[4][4][kC], colsum[4][kC], rowg[kC], rowb[kC], bt[kC], sdot[4];
-  __bf16 *const Os = buf, *const Rs = Os + NK * kC * SP, *const Us = Rs + NM * kC * SP, *const Es = buf;
-  const int tid = threadIdx.x, lane = tid % 64, w = tid / 64, r16 = lane % 16, kg = lane / 16;
-  const int c = blockIdx.x % p.NC, bk = blockIdx.x / p.NC, b = bk / p.Hk, hk = bk % p.Hk, group = p.H / p.Hk;
-  const int64_t t0 = (int64_t)c * kC;
-  const bool vec32 = p.Dv % 8 == 0;
-  {
-    const int64_t t = t0 + 16 * w + r16;
-    const int have = t < p.L ? p.Dk : 0;
-    const IT *kp = (const IT *)p.k.p + b * p.k.s0 + t * p.k.s1 + hk * p.k.s2;
-    const IT *qp = (const IT *)p.q.p + b * p.q.s0 + t * p.q.s1 + hk * p.q.s2;
-#pragma unroll
-    for (int s = 0; s < KS; ++s) {
-      const int e = 32 * s + 8 * kg;
-      bf8 f[NK];
-      row_frag<IT, NK>(kp + e, have - e, p.vk, f);
-#pragma unroll
-      for (int n = 0; n < NK; ++n) *(bf8 *)&Kr[n][16 * w + r16][e] = f[n];
-      row_frag<IT, NK>(qp + e, have - e, p.vq, f);
-#pragma unroll
-      for (int n = 0; n < NK; ++n) *(bf8 *)&Qr[n][16 * w + r16][e] = f[n];
+      for (int i = 0; i < 4; ++i)
+        if (key < p.Dk && i < have) p.dh0[((int64_t)bh * p.Dk + key) * p.Dv + v0 + i] = D[r][i];
     }
   }
-  f4 Yq[4][CT], Zk[4][CT];  // token rows 16 it + 4 kg + i, key columns 16 (CT w + ct) + r16
+}
+
+__device__ __forceinline__ float kg_sum(float v) {  // over the four lanes of a column
+  v += __shfl_xor(v, 16);
+  return v + __shfl_xor(v, 32);
+}
+
+// Wavefront w owns keys 16 w .. 16 w + 15 (DK / 16 wavefronts).  Results are transposed, so that a lane
+// holds 4 keys of one token.  The values are staged 32 columns at a time, as fragments in two buffers, the
+// states go from memory to registers, both one slab ahead.
+template <typename IT, int DK>
+__global__ void __launch_bounds__(4 * DK) k_delta_grad(const DeltaParams p) {
+  constexpr int NK = DParts<IT>::in, NM = DParts<IT>::mid, NP = DParts<IT>::out, NT = 4 * DK, NW = DK / 16;
+  constexpr int NJ = 16 / NW;                    // tiles of J and H per wavefront
+  constexpr int SF = 4 * 64 * 8;                 // staged elements of one part: 64 tokens x 32 columns
+  constexpr int kStage = (NK + NM + NP) * SF, JP = kC + 8, kE = (NM + NP) * kC * JP, PT = 512 / NT;
+  __shared__ __align__(16) __bf16 buf[2 * kStage > kE ? 2 * kStage : kE];  // dO, U, dR; then J and H
+  __shared__ double Gs[kC];
+  __shared__ float red[NW][2][kC], rowb[kC], rowv[kC], sdot[NW];
+  const int tid = threadIdx.x, lane = tid % 64, w = wave_id(), r16 = lane % 16, kg = lane / 16;
+  const int c = blockIdx.x % p.NC, bk = blockIdx.x / p.NC, b = bk / p.Hk, hk = bk % p.Hk, group = p.H / p.Hk;
+  const int64_t t0 = (int64_t)c * kC, kch = (int64_t)bk * p.NC + c;
+  const int wi = w * NJ / 4, wj = w * NJ % 4;    // J's tiles (wi, wj .. wj + NJ - 1)
+  const bool keys = 16 * w < p.Dkp;
+  const __bf16 *fK = key_frags<DK, NK>(p.fK, kch), *fQ = key_frags<DK, NK>(p.fQ, kch);
+  const __bf16 *fKt = key_frags<DK, NK>(p.fKt, kch), *fQt = key_frags<DK, NK>(p.fQt, kch);
+  // Makes the compiler read K and Q anew where they are used: kept over the slabs, they would spill.
+  auto reread = [&] { asm volatile("" : "+s"(fK), "+s"(fQ), "+s"(fKt), "+s"(fQt)); };
+  const int slabs = (p.VT + 1) / 2;
+  const int64_t ao = r16 * p.dout.s1 + 4 * kg, av = r16 * p.v.s1 + 4 * kg;
+  __bf16 *const Jm = buf, *const Hm = buf + NM * kC * JP;
+
+  // K or Q of token 16 it + r16, keys 16 w + 4 kg + i
+  auto elems = [&](const __bf16 *f, int it) {
+    f4 x = 0;
 #pragma unroll
-  for (int it = 0; it < 4; ++it)
+    for (int n = NK - 1; n >= 0; --n)
+      x += __builtin_convertvector(*(const bf4 *)(f + n * kC * DK + (it * (DK / 32) + w / 2) * 512 + 4 * (w % 2) + (unsigned)(lane * 8)), f4);
+    return x;
+  };
+
+  f4 Yq[4], Zk[4];  // dq', dk' of token 16 it + r16, keys 16 w + 4 kg + i
 #pragma unroll
-    for (int ct = 0; ct < CT; ++ct) Yq[it][ct] = Zk[it][ct] = 0;
+  for (int it = 0; it < 4; ++it) Yq[it] = Zk[it] = 0;
   const float *rows = nullptr;
 
   for (int hg = 0; hg < group; ++hg) {
     const int h = hk * group + hg;
     const int64_t ch = ((int64_t)b * p.H + h) * p.NC + c;
     rows = delta_rows(p, ch);
-    const IT *ob = (const IT *)p.dout.p + b * p.dout.s0 + h * p.dout.s2, *vb = (const IT *)p.v.p + b * p.v.s0 + h * p.v.s2;
-    f4 F1[4][CT], F2[4][CT], F3[4][CT], A[4], N[4];  // dO S0^T, U D^T, dR S0^T; row tile w of dO U^T, dR U^T
+    const IT *dop = (const IT *)p.dout.p + b * p.dout.s0 + h * p.dout.s2, *vp = (const IT *)p.v.p + b * p.v.s0 + h * p.v.s2;
+    f4 F1[4], F2[4], F3[4], A[NJ], N[NJ];  // S0 dO^T, D U^T, S0 dR^T; tiles of dO U^T, dR U^T, transposed
 #pragma unroll
-    for (int it = 0; it < 4; ++it) {
-      A[it] = N[it] = 0;
+    for (int it = 0; it < 4; ++it) F1[it] = F2[it] = F3[it] = 0;
 #pragma unroll
-      for (int ct = 0; ct < CT; ++ct) F1[it][ct] = F2[it][ct] = F3[it][ct] = 0;
-    }
-    float sd = 0, rv = 0;  // <S0, D>, dR.v of row tid / 4
+    for (int j = 0; j < NJ; ++j) A[j] = N[j] = 0;
+    float sd = 0, rv[PT], rb[PT];  // <S0, D>; dR.v and dR.Y of the staged tokens
+    f4 sv[2], dv[2], yv[PT], xv[PT];
+    Raw4<IT> go[PT], vv[PT];
+    // staged piece x of this thread: half sh of the slab, token st, columns 4 kg + i
+    auto stage_of = [&](int x, int &sh, int &it) {
+      sh = (w + x * NW) / 4;
+      it = (w + x * NW) % 4;
+    };
+    auto load = [&](int s) {
+#pragma unroll
+      for (int x = 0; x < 2; ++x) {
+        const int vt = 2 * s + x;
+        const bool in = keys && vt < p.VT;
+        sv[x] = in ? *(const f4 *)(state_of(p.states, p, ch, vt) + 256 * w + (unsigned)(16 * r16 + 4 * kg)) : (f4)0.0f;
+        dv[x] = in ? *(const f4 *)(state_of(p.dstates, p, ch, vt) + 256 * w + (unsigned)(16 * r16 + 4 * kg)) : (f4)0.0f;
+      }
+#pragma unroll
+      for (int x = 0; x < PT; ++x) {
+        int sh, it;
+        stage_of(x, sh, it);
+        const int vt = 2 * s + sh, have = t0 + 16 * it + r16 < p.L ? p.Dv - 16 * vt - 4 * kg : 0;
+        yv[x] = vt < p.VT ? *(const f4 *)(value_of(p.y, p, ch, vt) + 256 * it + (unsigned)(16 * r16 + 4 * kg)) : (f4)0.0f;
+        xv[x] = vt < p.VT ? *(const f4 *)(value_of(p.dr, p, ch, vt) + 256 * it + (unsigned)(16 * r16 + 4 * kg)) : (f4)0.0f;
+        go[x] = load4(dop + (t0 + 16 * it) * p.dout.s1 + 16 * vt + ao, have, p.vdo);
+        vv[x] = load4(vp + (t0 + 16 * it) * p.v.s1 + 16 * vt + av, have, p.vv);
+      }
+    };
+    load(0);
     if (tid < kC) Gs[tid] = ((const double *)(rows + 6 * kC))[tid];
-    for (int d0 = 0; d0 < p.Dv; d0 += SV) {
-      if (d0) lds_barrier();
+#pragma unroll
+    for (int x = 0; x < PT; ++x) rv[x] = rb[x] = 0;
+    for (int s = 0; s < slabs; ++s) {
+      __bf16 *const Os = buf + (s & 1) * kStage, *const Us = Os + NK * SF, *const Rs = Us + NM * SF;
+#pragma unroll
+      for (int x = 0; x < PT; ++x) {
+        int sh, it;
+        stage_of(x, sh, it);
+        const int at = (it * 64 + lane) * 8 + 4 * sh;
+        const float be = rows[kC + 16 * it + r16];
+        bf4 o[NK], u[NM], r[NP];
+        to_parts<IT, NK>(go[x], o);
+        split_parts<NM>((f4)(be * yv[x]), u);
+        split_parts<NP>(xv[x], r);
+        const f4 v = to_f4(vv[x]);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          rv[x] = fmaf(xv[x][i], v[i], rv[x]);
+          rb[x] = fmaf(xv[x][i], yv[x][i], rb[x]);
+        }
+#pragma unroll
+        for (int n = 0; n < NK; ++n) *(bf4 *)(Os + n * SF + at) = o[n];
+#pragma unroll
+        for (int n = 0; n < NM; ++n) *(bf4 *)(Us + n * SF + at) = u[n];
+#pragma unroll
+        for (int n = 0; n < NP; ++n) *(bf4 *)(Rs + n * SF + at) = r[n];
+      }
+      bf8 SA[NM], DA[NM];
       {
-        const int row = tid / 4, e = 8 * (tid % 4), have = p.Dv - d0 - e;
-        const int64_t t = t0 + row, at = (ch * kC + row) * p.Dv + d0 + e;
-        bf8 in[NK], mid[NM];
-        row_frag<IT, NK>(ob + t * p.dout.s1 + d0 + e, t < p.L ? have : 0, p.vdo, in);
+        const f8 x = __builtin_shufflevector(sv[0], sv[1], 0, 1, 2, 3, 4, 5, 6, 7);
+        const f8 y = __builtin_shufflevector(dv[0], dv[1], 0, 1, 2, 3, 4, 5, 6, 7);
 #pragma unroll
-        for (int n = 0; n < NK; ++n) *(bf8 *)(Os + (n * kC + row) * SP + e) = in[n];
-        const f8 x = row8<float>(p.dr + at, have, vec32), v = row8<IT>(vb + t * p.v.s1 + d0 + e, t < p.L ? have : 0, p.vv);
-#pragma unroll
-        for (int j = 0; j < 8; ++j) rv = fmaf(x[j], v[j], rv);
-        split_parts<NM>(x, mid);
-#pragma unroll
-        for (int n = 0; n < NM; ++n) *(bf8 *)(Rs + (n * kC + row) * SP + e) = mid[n];
-        split_parts<NM>(row8<float>(p.u + at, have, vec32), mid);
-#pragma unroll
-        for (int n = 0; n < NM; ++n) *(bf8 *)(Us + (n * kC + row) * SP + e) = mid[n];
+        for (int j = 0; j < 8; ++j) sd = fmaf(x[j], y[j], sd);
+        split_parts<NM>(x, SA);
+        split_parts<NM>(y, DA);
       }
-      bf8 SB[CT][NM], DB[CT][NM];
-#pragma unroll
-      for (int ct = 0; ct < CT; ++ct) {
-        const int kr = 16 * (CT * w + ct) + r16, have = kr < p.Dk ? p.Dv - d0 - 8 * kg : 0;
-        const int64_t at = (ch * p.Dk + kr) * p.Dv + d0 + 8 * kg;
-        const f8 s = row8<float>(p.states + at, have, vec32), d = row8<float>(p.dstates + at, have, vec32);
-#pragma unroll
-        for (int j = 0; j < 8; ++j) sd = fmaf(s[j], d[j], sd);
-        split_parts<NM>(s, SB[ct]);
-        split_parts<NM>(d, DB[ct]);
-      }
-      lds_barrier();
+      if (s + 1 < slabs) load(s + 1);
+      lds_barrier();  // the other buffer's readers are a barrier behind
 #pragma unroll
       for (int it = 0; it < 4; ++it) {
-        bf8 O[NK], R[NM], U[NM];
-        lds_frag<NK, SP>(Os, kC * SP, 16 * it + r16, 8 * kg, O);
-        lds_frag<NM, SP>(Rs, kC * SP, 16 * it + r16, 8 * kg, R);
-        lds_frag<NM, SP>(Us, kC * SP, 16 * it + r16, 8 * kg, U);
+        bf8 O[NK], U[NM], R[NP];
+        load_frag<NK>(Os, SF, it, lane, O);
+        load_frag<NM>(Us, SF, it, lane, U);
+        load_frag<NP>(Rs, SF, it, lane, R);
+        F1[it] = mma<NM>(SA, O, F1[it]);
+        F3[it] = mma<NP>(SA, R, F3[it]);
+        F2[it] = mma<NM>(DA, U, F2[it]);
+        if (it == wi) {
 #pragma unroll
-        for (int ct = 0; ct < CT; ++ct) {
-          F1[it][ct] = mma(O, SB[ct], F1[it][ct]);
-          F3[it][ct] = mma(R, SB[ct], F3[it][ct]);
-          F2[it][ct] = mma(U, DB[ct], F2[it][ct]);
+          for (int j = 0; j < NJ; ++j)
+            if (wj + j <= wi) {
+              bf8 Uj[NM];
+              load_frag<NM>(Us, SF, wj + j, lane, Uj);
+              A[j] = mma<NM>(Uj, O, A[j]);
+              N[j] = mma<NP>(Uj, R, N[j]);
+            }
         }
-        if (it <= w) {
-          bf8 Ow[NK], Rw[NM];
-          lds_frag<NK, SP>(Os, kC * SP, 16 * w + r16, 8 * kg, Ow);
-          lds_frag<NM, SP>(Rs, kC * SP, 16 * w + r16, 8 * kg, Rw);
-          A[it] = mma(Ow, U, A[it]);
-          N[it] = mma(Rw, U, N[it]);
-        }
+        __builtin_amdgcn_sched_barrier(0);  // one token tile's operands in registers at a time
       }
     }
-    rv += __shfl_xor(rv, 1);
-    rv += __shfl_xor(rv, 2);
-    if (tid % 4 == 0) bt[tid / 4] = rv;
-#pragma unroll
-    for (int m = 1; m < 64; m *= 2) sd += __shfl_xor(sd, m);
+    sd = group_sum<64>(sd);
     if (lane == 0) sdot[w] = sd;
-
-    // row dots with the rows of Q and K, and the state terms of dq, dk
-    const double GC = Gs[kC - 1];
+#pragma unroll
+    for (int x = 0; x < PT; ++x) {
+      rv[x] = kg_sum(rv[x]);
+      rb[x] = kg_sum(rb[x]);
+    }
+    lds_barrier();  // the slabs are read; red, rowv and rowb of the head before are too
+    // the two halves of the slabs are wavefronts 0..3 and 4..7, or one wavefront's two pieces
+    if constexpr (PT == 2) {
+      if (kg == 0) {
+        rowv[16 * w + r16] = rv[0] + rv[PT - 1];
+        rowb[16 * w + r16] = rb[0] + rb[PT - 1];
+      }
+    } else if (w >= 4 && kg == 0) {
+      rowv[16 * (w - 4) + r16] = rv[0];
+      rowb[16 * (w - 4) + r16] = rb[0];
+    }
+    {  // J and H
+      const int i = 16 * wi + r16;
+      const float fqi = rows[5 * kC + i], fki = rows[4 * kC + i] * rows[kC + i];
+      const double Gi = Gs[i];
+#pragma unroll
+      for (int j = 0; j < NJ; ++j) {
+        f4 jv, hv;
+#pragma unroll
+        for (int x = 0; x < 4; ++x) {
+          const int jj = 16 * (wj + j) + 4 * kg + x;
+          const float e = jj <= i ? fexp((float)(Gi - Gs[jj])) * rows[4 * kC + jj] : 0.0f;
+          jv[x] = jj <= i ? fqi * e * A[j][x] : 0.0f;
+          hv[x] = jj < i ? -fki * e * N[j][x] : 0.0f;
+        }
+        bf4 jp[NM], hp[NP];
+        split_parts<NM>(jv, jp);
+        split_parts<NP>(hv, hp);
+#pragma unroll
+        for (int n = 0; n < NM; ++n) *(bf4 *)(Jm + (n * kC + i) * JP + 16 * (wj + j) + 4 * kg) = jp[n];
+#pragma unroll
+        for (int n = 0; n < NP; ++n) *(bf4 *)(Hm + (n * kC + i) * JP + 16 * (wj + j) + 4 * kg) = hp[n];
+      }
+    }
+    reread();
+    bf8 Kt[2][NK], Qt[2][NK];
+#pragma unroll
+    for (int s = 0; s < 2; ++s) {
+      load_frag<NK>(fKt, kC * DK, 2 * w + s, lane, Kt[s]);
+      load_frag<NK>(fQt, kC * DK, 2 * w + s, lane, Qt[s]);
+    }
+    float cd = 0;
 #pragma unroll
     for (int it = 0; it < 4; ++it) {
-      const int r0 = 16 * it + 4 * kg;
-      const f4 fa = row4(rows, 0, r0), be = row4(rows, 1, r0), fc = row4(rows, 2, r0), fd = row4(rows, 3, r0);
+      const int tok = 16 * it + r16;
+      const float fa = rows[tok], be = rows[kC + tok], fc = rows[2 * kC + tok], fd = rows[3 * kC + tok];
+      const f4 ke = elems(fK, it), f2 = fc * F2[it];
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const float eG = fexp((float)Gs[r0 + i]), cG = fexp((float)(GC - Gs[r0 + i]));
-        float v1 = 0, v2 = 0, v3 = 0;
-#pragma unroll
-        for (int ct = 0; ct < CT; ++ct) {
-          const int col = 16 * (CT * w + ct) + r16;
-          const float q = lds_elem<NK, KP>(&Qr[0][0][0], kC * KP, r0 + i, col), k = lds_elem<NK, KP>(&Kr[0][0][0], kC * KP, r0 + i, col);
-          v1 = fmaf(q, F1[it][ct][i], v1);
-          v2 = fmaf(k, F2[it][ct][i], v2);
-          v3 = fmaf(k, F3[it][ct][i], v3);
-          Yq[it][ct][i] = fmaf(eG, F1[it][ct][i], Yq[it][ct][i]);
-          Zk[it][ct][i] += cG * F2[it][ct][i] - be[i] * eG * F3[it][ct][i];
-        }
-        v1 = row_sum(v1);
-        v2 = row_sum(v2);
-        v3 = row_sum(v3);
-        if (r16 == 0) {
-          red[w][0][r0 + i] = fd[i] * v1 - be[i] * fa[i] * v3;
-          red[w][1][r0 + i] = fc[i] * v2;
-          red[w][2][r0 + i] = -fa[i] * v3;
-        }
-      }
+      for (int i = 0; i < 4; ++i) cd = fmaf(ke[i], f2[i], cd);
+      F1[it] *= fd;
+      Zk[it] += f2 - (be * fa) * F3[it];
     }
-    // the masked products within the chunk, row tile w
-    f4 E2[4], E3[4];
-    f4 fqr = row4(rows, 5, 16 * w + 4 * kg), fkr = row4(rows, 4, 16 * w + 4 * kg), ber = row4(rows, 1, 16 * w + 4 * kg);
-    f4 rg = 0, rb = 0;
-    lds_barrier();  // the slabs are read
+    cd = group_sum<64>(cd);
+    if (lane == 0) red[w][1][0] = cd;
+    lds_barrier();
 #pragma unroll
-    for (int jt = 0; jt < 4; ++jt) {
-      const int col = 16 * jt + r16;
-      f4 kk = 0, qk = 0;
-      if (jt <= w) {
+    for (int s = 0; s < 2; ++s) {
 #pragma unroll
-        for (int s = 0; s < KS; ++s) {
-          bf8 B[NK], Kw[NK], Qw[NK];
-          lds_frag<NK, KP>(&Kr[0][0][0], kC * KP, col, 32 * s + 8 * kg, B);
-          lds_frag<NK, KP>(&Kr[0][0][0], kC * KP, 16 * w + r16, 32 * s + 8 * kg, Kw);
-          lds_frag<NK, KP>(&Qr[0][0][0], kC * KP, 16 * w + r16, 32 * s + 8 * kg, Qw);
-          kk = mma(Kw, B, kk);
-          qk = mma(Qw, B, qk);
-        }
-      }
-      const float fkc = rows[4 * kC + col];
-      float cs = 0;
+      for (int it = 0; it < 4; ++it) {
+        const int at = (16 * it + r16) * JP + 32 * s + 4 * kg;                                   // row it, columns of step s
+        const int tr = (32 * s + 4 * kg + r16 / 4) * JP + 16 * it + 4 * (r16 % 4);               // rows of step s, column it
+        if (s <= it / 2) {
+          bf8 B[NM], C[NP];
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const int row = 16 * w + 4 * kg + i;
-        float e1 = 0, e2 = 0, e3 = 0;
-        if (col <= row) {
-          const float e = fexp((float)(Gs[row] - Gs[col]));
-          e1 = A[jt][i] * e;
-          e2 = e1 * fqr[i];
-          if (col < row) {
-            const float nm = N[jt][i] * e * fkr[i] * fkc * kk[i];
-            e3 = N[jt][i] * e * ber[i];
-            rb[i] += nm;
-            const float z = e2 * fkc * qk[i] - ber[i] * nm;
-            rg[i] += z;
-            cs += z;
+          for (int n = 0; n < NM; ++n) {
+            const __bf16 *m = Jm + n * kC * JP + at;
+            B[n] = __builtin_shufflevector(*(const bf4 *)m, *(const bf4 *)(m + 16), 0, 1, 2, 3, 4, 5, 6, 7);
           }
-          e1 *= fkc;
-        }
-        E2[jt][i] = e2;
-        E3[jt][i] = e3;
-        float x = e1;
 #pragma unroll
-        for (int m = 0; m < NM; ++m) {
-          const __bf16 q = (__bf16)x;
-          Es[(m * kC + row) * kCP + col] = q;
-          x -= (float)q;
+          for (int n = 0; n < NP; ++n) {
+            const __bf16 *m = Hm + n * kC * JP + at;
+            C[n] = __builtin_shufflevector(*(const bf4 *)m, *(const bf4 *)(m + 16), 0, 1, 2, 3, 4, 5, 6, 7);
+          }
+          F1[it] = mma<NM>(Kt[s], B, F1[it]);
+          Zk[it] = mma<NP>(Kt[s], C, Zk[it]);
         }
+        if (s >= it / 2) {
+          bf8 B[NP], C[NP];
+#pragma unroll
+          for (int n = 0; n < NP; ++n) {
+            B[n] = read_tr(Jm + n * kC * JP + tr, Jm + (n * kC + 16) * JP + tr);
+            C[n] = read_tr(Hm + n * kC * JP + tr, Hm + (n * kC + 16) * JP + tr);
+          }
+          Zk[it] = mma<NP>(Qt[s], B, Zk[it]);
+          Zk[it] = mma<NP>(Kt[s], C, Zk[it]);
+        }
+        __builtin_amdgcn_sched_barrier(0);
       }
-      cs += __shfl_xor(cs, 16);
-      cs += __shfl_xor(cs, 32);
-      if (kg == 0) colsum[w][col] = cs;
     }
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      rg[i] = row_sum(rg[i]);
-      rb[i] = row_sum(rb[i]);
-      if (r16 == 0) {
-        rowg[16 * w + 4 * kg + i] = rg[i];
-        rowb[16 * w + 4 * kg + i] = rb[i];
+    for (int it = 0; it < 4; ++it) {
+      const f4 q = elems(fQ, it) * F1[it];
+      const float x = kg_sum((q[0] + q[1]) + (q[2] + q[3]));
+      if (kg == 0) red[w][0][16 * it + r16] = x;
+      Yq[it] += F1[it];
+    }
+    if constexpr (PT == 1) {
+      if (w < 4 && kg == 0) {
+        rowv[16 * w + r16] += rv[0];
+        rowb[16 * w + r16] += rb[0];
       }
     }
     lds_barrier();
     if (w == 0) {  // dbeta and dg of the head
-      float g = rowg[lane], cv = 0, db = bt[lane] - rowb[lane];
+      const float db = rowb[lane];
+      double s = -(double)rows[kC + lane] * rowv[lane], all = 0, ss = 0;
 #pragma unroll
-      for (int k = 0; k < 4; ++k) {
-        g += red[k][0][lane] - colsum[k][lane];
-        cv += red[k][1][lane];
-        db += red[k][2][lane];
+      for (int k = 0; k < NW; ++k) {
+        s += red[k][0][lane];
+        all += red[k][1][0];
+        ss += sdot[k];
       }
-      double s = (double)g - cv, all = cv;
 #pragma unroll
       for (int d = 1; d < 64; d *= 2) {
         const double up = __shfl_down(s, d);
         if (lane + d < 64) s += up;
-        all += __shfl_xor(all, d);
       }
-      s += all + (double)chunk_decay(rows) * ((double)sdot[0] + sdot[1] + sdot[2] + sdot[3]);
+      s += all + (double)fexp((float)Gs[kC - 1]) * ss;
       const int64_t t = t0 + lane;
       if (t < p.L) {
         ((float *)p.dg.p)[b * p.dg.s0 + t * p.dg.s1 + h * p.dg.s2] = (float)s;
         store_either<IT>((void *)p.dbeta.p, p.beta32, b * p.dbeta.s0 + t * p.dbeta.s1 + h * p.dbeta.s2, db);
       }
     }
-    // dq^ += (A e) K
-#pragma unroll
-    for (int s = 0; s < 2; ++s) {
-      bf8 B[CT][NK];
-#pragma unroll
-      for (int ct = 0; ct < CT; ++ct) lds_frag_t<NK, KP>(&Kr[0][0][0], kC * KP, 32 * s, 16 * (CT * w + ct), lane, B[ct]);
-#pragma unroll
-      for (int it = 2 * s; it < 4; ++it) {
-        bf8 E[NM];
-        lds_frag<NM, kCP>(Es, kC * kCP, 16 * it + r16, 32 * s + 8 * kg, E);
-#pragma unroll
-        for (int ct = 0; ct < CT; ++ct) Yq[it][ct] = mma(E, B[ct], Yq[it][ct]);
-      }
-    }
-    lds_barrier();
-#pragma unroll
-    for (int jt = 0; jt < 4; ++jt) {
-      bf4 parts[NM];
-      split_parts<NM>(E2[jt], parts);
-#pragma unroll
-      for (int m = 0; m < NM; ++m) *(bf4 *)(Es + (m * kC + 16 * jt + r16) * kCP + 16 * w + 4 * kg) = parts[m];
-    }
-    lds_barrier();
-    // dk^ += (scale A e)^T Q
-#pragma unroll
-    for (int s = 0; s < 2; ++s) {
-      bf8 B[CT][NK];
-#pragma unroll
-      for (int ct = 0; ct < CT; ++ct) lds_frag_t<NK, KP>(&Qr[0][0][0], kC * KP, 32 * s, 16 * (CT * w + ct), lane, B[ct]);
-#pragma unroll
-      for (int it = 0; it < 2 + 2 * s; ++it) {
-        bf8 E[NM];
-        lds_frag<NM, kCP>(Es, kC * kCP, 16 * it + r16, 32 * s + 8 * kg, E);
-#pragma unroll
-        for (int ct = 0; ct < CT; ++ct) Zk[it][ct] = mma(E, B[ct], Zk[it][ct]);
-      }
-    }
-    lds_barrier();
-#pragma unroll
-    for (int jt = 0; jt < 4; ++jt) {
-      if (jt > w) continue;
-      const int col = 16 * jt + r16;
-      const float fkc = rows[4 * kC + col];
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const int row = 16 * w + 4 * kg + i;
-        if (col > row) continue;
-        float x = -E3[jt][i] * fkc, y = -E3[jt][i] * fkr[i];
-#pragma unroll
-        for (int m = 0; m < NM; ++m) {
-          const __bf16 xq = (__bf16)x, yq = (__bf16)y;
-          Es[(m * kC + row) * kCP + col] = xq;
-          if (col < row) Es[(m * kC + col) * kCP + row] = yq;
-          x -= (float)xq;
-          y -= (float)yq;
-        }
-      }
-    }
-    lds_barrier();
-    // dk^ -= (beta N e and its transpose) K
-#pragma unroll
-    for (int s = 0; s < 2; ++s) {
-      bf8 B[CT][NK];
-#pragma unroll
-      for (int ct = 0; ct < CT; ++ct) lds_frag_t<NK, KP>(&Kr[0][0][0], kC * KP, 32 * s, 16 * (CT * w + ct), lane, B[ct]);
-#pragma unroll
-      for (int it = 0; it < 4; ++it) {
-        bf8 E[NM];
-        lds_frag<NM, kCP>(Es, kC * kCP, 16 * it + r16, 32 * s + 8 * kg, E);
-#pragma unroll
-        for (int ct = 0; ct < CT; ++ct) Zk[it][ct] = mma(E, B[ct], Zk[it][ct]);
-      }
-    }
-    lds_barrier();
+    lds_barrier();  // J, H, Gs and sdot are read
   }
 
-  // through the norms: dq = |q|^-1 (dq^ - q^ (q^.dq^)), likewise dk
+  // through the norms
+  reread();
   if (p.qk_norm) {
 #pragma unroll
-    for (int it = 0; it < 4; ++it)
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const int row = 16 * it + 4 * kg + i;
-        float sq = 0, sk = 0;
-#pragma unroll
-        for (int ct = 0; ct < CT; ++ct) {
-          const int col = 16 * (CT * w + ct) + r16;
-          sq = fmaf(lds_elem<NK, KP>(&Qr[0][0][0], kC * KP, row, col), Yq[it][ct][i], sq);
-          sk = fmaf(lds_elem<NK, KP>(&Kr[0][0][0], kC * KP, row, col), Zk[it][ct][i], sk);
-        }
-        sq = row_sum(sq);
-        sk = row_sum(sk);
-        if (r16 == 0) {
-          red[w][0][row] = sq;
-          red[w][1][row] = sk;
-        }
+    for (int it = 0; it < 4; ++it) {
+      const f4 q = elems(fQ, it) * Yq[it], k = elems(fK, it) * Zk[it];
+      const float sq = kg_sum((q[0] + q[1]) + (q[2] + q[3])), sk = kg_sum((k[0] + k[1]) + (k[2] + k[3]));
+      if (kg == 0) {
+        red[w][0][16 * it + r16] = sq;
+        red[w][1][16 * it + r16] = sk;
       }
+    }
     lds_barrier();
   }
   IT *dqb = (IT *)p.dq.p + b * p.dq.s0 + hk * p.dq.s2, *dkb = (IT *)p.dk.p + b * p.dk.s0 + hk * p.dk.s2;
+  const int e = 16 * w + 4 * kg;
 #pragma unroll
   for (int it = 0; it < 4; ++it) {
-    const int r0 = 16 * it + 4 * kg;
-    const f4 fk = row4(rows, 4, r0), fq = row4(rows, 5, r0);
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const int row = r0 + i;
+    const int tok = 16 * it + r16, have = t0 + tok < p.L ? p.Dk - e : 0;
+    f4 y = Yq[it], z = Zk[it];
+    if (p.qk_norm) {
       float sq = 0, sk = 0;
-      if (p.qk_norm) {
-        const float nq = fq[i] / p.scale;
-        sq = nq * nq * (red[0][0][row] + red[1][0][row] + red[2][0][row] + red[3][0][row]);
-        sk = fk[i] * fk[i] * (red[0][1][row] + red[1][1][row] + red[2][1][row] + red[3][1][row]);
-      }
 #pragma unroll
-      for (int ct = 0; ct < CT; ++ct) {
-        const int col = 16 * (CT * w + ct) + r16;
-        if (t0 + row < p.L && col < p.Dk) {
-          float y = Yq[it][ct][i], z = Zk[it][ct][i];
-          if (p.qk_norm) {
-            y = fmaf(-sq, lds_elem<NK, KP>(&Qr[0][0][0], kC * KP, row, col), y);
-            z = fmaf(-sk, lds_elem<NK, KP>(&Kr[0][0][0], kC * KP, row, col), z);
-          }
-          Conv<IT>::store(dqb + (t0 + row) * p.dq.s1 + col, fq[i] * y);
-          Conv<IT>::store(dkb + (t0 + row) * p.dk.s1 + col, fk[i] * z);
-        }
+      for (int k = 0; k < NW; ++k) {
+        sq += red[k][0][tok];
+        sk += red[k][1][tok];
       }
+      const float fk = rows[4 * kC + tok], nq = rows[5 * kC + tok] / p.scale;
+      y -= (nq * nq * sq) * elems(fQ, it);
+      z -= (fk * fk * sk) * elems(fK, it);
     }
+    store4(dqb + (t0 + tok) * p.dq.s1 + e, y, have, p.vdq);
+    store4(dkb + (t0 + tok) * p.dk.s1 + e, z, have, p.vdk);
   }
 }
 
 template <typename IT, int DK>
 static hipError_t delta_bwd(const DeltaParams &p, hipStream_t s) {
-  constexpr int NV = 1;
-  hipLaunchKernelGGL((k_delta_bwd<IT, DK, NV>), dim3((unsigned)(p.B * p.H) * (unsigned)((p.Dv + 16 * NV - 1) / (16 * NV))),
-                     dim3(kDT), 0, s, p);
-  hipLaunchKernelGGL((k_delta_grad<IT, DK>), dim3((unsigned)(p.B * p.Hk) * (unsigned)p.NC), dim3(kDT), 0, s, p);
+  hipLaunchKernelGGL((k_delta_bwd<IT, DK>), dim3((unsigned)(p.B * p.H) * (unsigned)p.VT), dim3(kDT), 0, s, p);
+  hipLaunchKernelGGL((k_delta_grad<IT, DK>), dim3((unsigned)(p.B * p.Hk) * (unsigned)p.NC), dim3(4 * DK), 0, s, p);
   return hipGetLastError();
 }
 template <typename IT>

@@ -300,20 +300,22 @@ constexpr int kDeltaMaxK = 128;        // key width of the chunked kernels and t
 struct DeltaParams {
   int64_t B, L;
   int Hk, H, Dk, Dv, NC, qk_norm, beta32;
+  int VT, Dkp;                         // 16-column tiles of v, Dk in whole tiles of 16
   float scale;
-  int vq, vk, vv, vo, vdo;             // 16-byte loads fit the view's rows
+  int vq, vk, vv, vo, vdo, vdq, vdk, vdv;  // the view's rows are whole words of 4 elements
   KView q, k, v, g, beta, o;           // (B, L, Hk, Dk), (B, L, H, Dv), (B, L, H)
   const float *h0;                     // (B, H, Dk, Dv) or null
   float *last;
-  void *fT, *fP;                       // operand fragments of T - I and P, or of their transposes (backward)
+  void *fT, *fP, *fK, *fQ, *fKt, *fQt; // operand fragments (fQt: backward only)
   float *rows;                         // (B H, NC, kDeltaRows)
-  float *states, *u;                   // saved: (B H, NC, Dk, Dv) entering states, (B H, NC, 64, Dv) U
+  float *states, *y;                   // saved: (B H, NC, VT, Dkp, 16) entering states, (B H, NC, VT, 64, 16) Y
   KView dout, dq, dk, dv, dg, dbeta;
   const float *dlast;
-  float *dh0, *dstates, *dr;           // gradients of the leaving states and R, laid out as states and u
+  float *dh0, *dstates, *dr;           // gradients of the leaving states and dR, laid out as states and y
 };
-// bf16 parts that hold a float32 intermediate
-inline int delta_mid_parts(int dtype) { return dtype == 0 ? 3 : 2; }
+constexpr int kDeltaMidParts = 3;      // bf16 parts of a float32 intermediate
+inline int delta_in_parts(int dtype) { return dtype == 0 ? 3 : dtype == 1 ? 1 : 2; }
+inline int delta_width(int64_t Dk) { return Dk <= 64 ? 64 : 128; }  // keys of the kernel variant
 hipError_t launch_delta_fwd(const DeltaParams &p, int dtype, hipStream_t s);
 hipError_t launch_delta_bwd(const DeltaParams &p, int dtype, hipStream_t s);
 struct DeltaStepParams {
