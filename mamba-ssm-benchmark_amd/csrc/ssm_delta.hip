@@ -44,14 +44,22 @@ __global__ void __launch_bounds__(kDT) k_delta_prep(const DeltaParams p) {
   const int have = t < p.L ? p.Dk : 0;
   const bool first = h % group == 0;
   bf8 K[KS][NK], Q[KS][NK];
+  Raw4<IT> x[KS][4];
+  const IT *const ks = (const IT *)p.k.p, *const qs = (const IT *)p.q.p;
 #pragma unroll
   for (int s = 0; s < KS; ++s) {
     const int e = 32 * s + 4 * kg;
-    Raw4<IT> x[4] = {load4(kp + e, have - e, p.vk), load4(kp + e + 16, have - e - 16, p.vk),
-                     load4(qp + e, have - e, p.vq), load4(qp + e + 16, have - e - 16, p.vq)};
+    x[s][0] = load4(kp + e, ks, have - e, p.vk);
+    x[s][1] = load4(kp + e + 16, ks, have - e - 16, p.vk);
+    x[s][2] = load4(qp + e, qs, have - e, p.vq);
+    x[s][3] = load4(qp + e + 16, qs, have - e - 16, p.vq);
+  }
+#pragma unroll
+  for (int s = 0; s < KS; ++s) {
+    const int e = 32 * s + 4 * kg;
     bf4 a[4][NK];
 #pragma unroll
-    for (int i = 0; i < 4; ++i) to_parts<IT, NK>(x[i], a[i]);
+    for (int i = 0; i < 4; ++i) to_parts<IT, NK>(x[s][i], have - e - 16 * (i % 2) > 0, a[i]);
 #pragma unroll
     for (int n = 0; n < NK; ++n) {
       K[s][n] = __builtin_shufflevector(a[0][n], a[1][n], 0, 1, 2, 3, 4, 5, 6, 7);
@@ -199,50 +207,50 @@ __global__ void __launch_bounds__(kDT) k_delta_prep(const DeltaParams p) {
     float *rows = p.rows + ch * kDeltaRows;
     const double G = Gs[tid];
     const float eG = fexp((float)G);
-    rows[tid] = fk[tid] * eG;
-    rows[kC + tid] = bs[tid];
-    rows[2 * kC + tid] = fk[tid] * fexp((float)(Gs[kC - 1] - G));
-    rows[3 * kC + tid] = fq[tid] * eG;
+    *(f4 *)(rows + 4 * tid) = f4{fk[tid] * eG, bs[tid], fk[tid] * fexp((float)(Gs[kC - 1] - G)), fq[tid] * eG};
     rows[4 * kC + tid] = fk[tid];
     rows[5 * kC + tid] = fq[tid];
     ((double *)(rows + 6 * kC))[tid] = G;
+    if (tid == kC - 1) rows[8 * kC] = eG;
   }
 }
 
 // Everything that does not hang on the state is read a chunk ahead, into the registers that the chunk has
-// just used.  All products are of transposes: rows are the 16 columns of v, so a lane holds 4 columns of
-// one token or key, and moves them as one word.
-template <typename IT, int DK>
-__global__ void __launch_bounds__(kDT, DK * sizeof(IT) <= 256 ? 2 : 1) k_delta_fwd(const DeltaParams p) {
+// just used.  All products are of transposes: rows are 16 columns of v, so a lane holds 4 columns of
+// one token or key, and moves them as one word.  A workgroup walks NV tiles of 16 columns.
+template <typename IT, int DK, int NV>
+__global__ void __launch_bounds__(kDT, DK * sizeof(IT) * NV <= 256 ? 2 : 1) k_delta_fwd(const DeltaParams p) {
   constexpr int NK = DParts<IT>::in, NM = DParts<IT>::mid, NP = DParts<IT>::out, KS = DK / 32, RT = DK / 64;
-  __shared__ __align__(16) VTile<NM, DK> St;
-  __shared__ __align__(16) VTile<NM, kC> Xt, Wt;
-  __shared__ __align__(16) VTile<NP, kC> Ut;
-  const int tid = threadIdx.x, lane = tid % 64, w = wave_id(), r16 = lane % 16, kg = lane / 16;
+  __shared__ __align__(16) VTile<NM, DK> St[NV];
+  __shared__ __align__(16) VTile<NM, kC> Xt[NV], Wt[NV];
+  __shared__ __align__(16) VTile<NP, kC> Ut[NV];
+  const int lane = threadIdx.x % 64, w = wave_id(), r16 = lane % 16, kg = lane / 16;
   int bh, vt;
-  delta_tile(p.VT, (int)p.B * p.H, bh, vt);
+  delta_tile((p.VT + NV - 1) / NV, (int)p.B * p.H, bh, vt);
+  vt *= NV;
   const int b = bh / p.H, h = bh % p.H, hk = h / (p.H / p.Hk), v0 = 16 * vt + 4 * kg, have = p.Dv - v0;
   const int tok = 16 * w + r16;
   const IT *vp = (const IT *)p.v.p + b * p.v.s0 + h * p.v.s2 + v0;
   IT *op = (IT *)p.o.p + b * p.o.s0 + h * p.o.s2 + v0;
   const int64_t ch0 = (int64_t)bh * p.NC, kch0 = ((int64_t)b * p.Hk + hk) * p.NC;
 
-  f4 S[RT];  // S[key][v0 + i] of key 16 (RT w + r) + r16
+  f4 S[NV][RT];  // S[key][v0 + 16 n + i] of key 16 (RT w + r) + r16
 #pragma unroll
-  for (int r = 0; r < RT; ++r) {
-    const int key = 16 * (RT * w + r) + r16;
+  for (int n = 0; n < NV; ++n)
 #pragma unroll
-    for (int i = 0; i < 4; ++i)
-      S[r][i] = p.h0 && key < p.Dk && i < have ? p.h0[((int64_t)bh * p.Dk + key) * p.Dv + v0 + i] : 0.0f;
-  }
+    for (int r = 0; r < RT; ++r) {
+      const int key = 16 * (RT * w + r) + r16;
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+        S[n][r][i] = p.h0 && key < p.Dk && 16 * n + i < have ? p.h0[((int64_t)bh * p.Dk + key) * p.Dv + v0 + 16 * n + i] : 0.0f;
+    }
   bf8 K[KS][NK], Q[KS][NK], T[2][NM], P[2][NP], Kt[RT][2][NK];
-  Raw4<IT> v;
-  float fa, be, fc, fd;
-  double GC;
+  Raw4<IT> v[NV];
+  f4 row;  // a, beta, c, d of the token
+  float eC;
   auto load_rows = [&](int c) {
-    const float *rows = delta_rows(p, ch0 + c);
-    fa = rows[tok]; be = rows[kC + tok]; fc = rows[2 * kC + tok]; fd = rows[3 * kC + tok];
-    GC = chunk_sum(rows);
+    row = token_row(delta_rows(p, ch0 + c), tok);
+    eC = chunk_decay(delta_rows(p, ch0 + c));
   };
   auto load_kq = [&](int c) {
     const __bf16 *k = key_frags<DK, NK>(p.fK, kch0 + c), *q = key_frags<DK, NK>(p.fQ, kch0 + c);
@@ -254,7 +262,8 @@ __global__ void __launch_bounds__(kDT, DK * sizeof(IT) <= 256 ? 2 : 1) k_delta_f
   };
   auto load_v = [&](int c) {
     const int64_t t = (int64_t)c * kC + tok;
-    v = load4(vp + t * p.v.s1, t < p.L ? have : 0, p.vv);
+#pragma unroll
+    for (int n = 0; n < NV; ++n) v[n] = load4(vp + t * p.v.s1 + 16 * n, (const IT *)p.v.p, t < p.L ? have - 16 * n : 0, p.vv);
   };
   auto load_t = [&](int c) {  // T is lower triangular
 #pragma unroll
@@ -271,75 +280,101 @@ __global__ void __launch_bounds__(kDT, DK * sizeof(IT) <= 256 ? 2 : 1) k_delta_f
     }
   };
   load_rows(0);
-  load_kq(0);
   load_v(0);
+  load_kq(0);
   load_t(0);
   load_p(0);
   for (int c = 0; c < p.NC; ++c) {
     const int64_t t = (int64_t)c * kC + tok, ch = ch0 + c;
     const int next = c + 1 < p.NC ? c + 1 : c;
 #pragma unroll
-    for (int r = 0; r < RT; ++r) {
-      const int key = 16 * (RT * w + r) + r16;
-      St.put(key, kg, S[r]);
-      if (p.states && key < p.Dkp) *(f4 *)(state_of(p.states, p, ch, vt) + (unsigned)(16 * key + 4 * kg)) = S[r];
-    }
-    lds_barrier();
-    f4 x = 0, o = 0;
+    for (int n = 0; n < NV; ++n)
 #pragma unroll
-    for (int s = 0; s < KS; ++s) {
-      bf8 A[NM];
-      St.get(s, lane, A);
-      x = mma<NM>(A, K[s], x);
-      o = mma<NP>(A, Q[s], o);
+      for (int r = 0; r < RT; ++r) {
+        const int key = 16 * (RT * w + r) + r16;
+        St[n].put(key, kg, S[n][r]);
+        if (p.states && key < p.Dkp && vt + n < p.VT)
+          *(f4 *)(state_of(p.states, p, ch, vt + n) + (unsigned)(16 * key + 4 * kg)) = S[n][r];
+      }
+    lds_barrier();
+    f4 x[NV], o[NV], y[NV];
+#pragma unroll
+    for (int n = 0; n < NV; ++n) x[n] = o[n] = 0;
+#pragma unroll
+    for (int s = 0; s < KS; ++s)
+#pragma unroll
+      for (int n = 0; n < NV; ++n) {
+        bf8 A[NM];
+        St[n].get(s, lane, A);
+        x[n] = mma<NM>(A, K[s], x[n]);
+        o[n] = mma<NP>(A, Q[s], o[n]);
+      }
+#pragma unroll
+    for (int n = 0; n < NV; ++n) {
+      y[n] = to_f4<IT>(v[n], t < p.L && have - 16 * n > 0) - row[0] * x[n];
+      o[n] *= row[3];
+      Xt[n].put(tok, kg, y[n]);
     }
-    load_kq(next);
-    f4 y = to_f4(v) - fa * x;
-    load_v(next);
-    o *= fd;
-    Xt.put(tok, kg, y);
-    const float bu = be, bc = be * fc, eC = fexp((float)GC);
+    const float bu = row[1], bc = row[1] * row[2], decay = eC;
     load_rows(next);
+    load_v(next);
+    load_kq(next);
     lds_barrier();
 #pragma unroll
     for (int s = 0; s < 2; ++s)  // Y = X + (T - I) X
       if (s <= w / 2) {
-        bf8 A[NM];
-        Xt.get(s, lane, A);
-        y = mma<NM>(A, T[s], y);
+#pragma unroll
+        for (int n = 0; n < NV; ++n) {
+          bf8 A[NM];
+          Xt[n].get(s, lane, A);
+          y[n] = mma<NM>(A, T[s], y[n]);
+        }
       }
+#pragma unroll
+    for (int n = 0; n < NV; ++n) {
+      Wt[n].put(tok, kg, bc * y[n]);
+      Ut[n].put(tok, kg, bu * y[n]);
+      if (p.y && vt + n < p.VT) *(f4 *)(value_of(p.y, p, ch, vt + n) + (unsigned)(16 * tok + 4 * kg)) = y[n];
+    }
     load_t(next);
-    Wt.put(tok, kg, bc * y);
-    Ut.put(tok, kg, bu * y);
-    if (p.y) *(f4 *)(value_of(p.y, p, ch, vt) + (unsigned)(16 * tok + 4 * kg)) = y;
     lds_barrier();
 #pragma unroll
-    for (int r = 0; r < RT; ++r) S[r] *= eC;
+    for (int n = 0; n < NV; ++n)
 #pragma unroll
-    for (int s = 0; s < 2; ++s) {
-      bf8 A[NM];
-      Wt.get(s, lane, A);
+      for (int r = 0; r < RT; ++r) S[n][r] *= decay;
 #pragma unroll
-      for (int r = 0; r < RT; ++r) S[r] = mma<NM>(A, Kt[r][s], S[r]);
-    }
+    for (int s = 0; s < 2; ++s)
+#pragma unroll
+      for (int n = 0; n < NV; ++n) {
+        bf8 A[NM];
+        Wt[n].get(s, lane, A);
+#pragma unroll
+        for (int r = 0; r < RT; ++r) S[n][r] = mma<NM>(A, Kt[r][s], S[n][r]);
+      }
 #pragma unroll
     for (int s = 0; s < 2; ++s)
       if (s <= w / 2) {
-        bf8 A[NP];
-        Ut.get(s, lane, A);
-        o = mma<NP>(A, P[s], o);
+#pragma unroll
+        for (int n = 0; n < NV; ++n) {
+          bf8 A[NP];
+          Ut[n].get(s, lane, A);
+          o[n] = mma<NP>(A, P[s], o[n]);
+        }
       }
     load_p(next);
-    store4(op + t * p.o.s1, o, t < p.L ? have : 0, p.vo);
+#pragma unroll
+    for (int n = 0; n < NV; ++n) store4(op + t * p.o.s1 + 16 * n, o[n], t < p.L ? have - 16 * n : 0, p.vo);
   }
   if (p.last) {
 #pragma unroll
-    for (int r = 0; r < RT; ++r) {
-      const int key = 16 * (RT * w + r) + r16;
+    for (int n = 0; n < NV; ++n)
 #pragma unroll
-      for (int i = 0; i < 4; ++i)
-        if (key < p.Dk && i < have) p.last[((int64_t)bh * p.Dk + key) * p.Dv + v0 + i] = S[r][i];
-    }
+      for (int r = 0; r < RT; ++r) {
+        const int key = 16 * (RT * w + r) + r16;
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+          if (key < p.Dk && 16 * n + i < have) p.last[((int64_t)bh * p.Dk + key) * p.Dv + v0 + 16 * n + i] = S[n][r][i];
+      }
   }
 }
 
@@ -347,7 +382,10 @@ template <typename IT, int DK>
 static hipError_t delta_fwd(const DeltaParams &p, hipStream_t s) {
   const unsigned heads = (unsigned)(p.B * p.H);
   hipLaunchKernelGGL((k_delta_prep<IT, DK, false>), dim3(heads * (unsigned)p.NC), dim3(kDT), 0, s, p);
-  hipLaunchKernelGGL((k_delta_fwd<IT, DK>), dim3(heads * (unsigned)p.VT), dim3(kDT), 0, s, p);
+  if (delta_pairs(p))
+    hipLaunchKernelGGL((k_delta_fwd<IT, DK, 2>), dim3((unsigned)(p.B * p.H) * (unsigned)((p.VT + 1) / 2)), dim3(kDT), 0, s, p);
+  else
+    hipLaunchKernelGGL((k_delta_fwd<IT, DK, 1>), dim3((unsigned)(p.B * p.H) * (unsigned)p.VT), dim3(kDT), 0, s, p);
   return hipGetLastError();
 }
 template <typename IT>

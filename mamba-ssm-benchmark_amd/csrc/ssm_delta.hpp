@@ -106,22 +106,23 @@ __device__ __forceinline__ void load_frag(const __bf16 *m, int64_t part, int at,
 
 __device__ __forceinline__ int wave_id() { return __builtin_amdgcn_readfirstlane(threadIdx.x / 64); }
 
-// Four consecutive elements of a row, 0 from `have` on; vec: rows are whole words of 4 elements.
-template <typename IT> struct alignas(4 * sizeof(IT)) Raw4 { IT e[4]; };
+// Four consecutive elements of a row as words.  vec: rows are whole words of 4 elements; the words are then
+// read whether `have` > 0 or not (from `safe`, any readable element), so that nothing waits for them before
+// their use, which takes 0 in their place.  Otherwise the elements from `have` on are 0.
+template <typename IT> using Raw4 = unsigned __attribute__((ext_vector_type(sizeof(IT))));
+template <typename IT> struct alignas(4 * sizeof(IT)) Four { IT e[4]; };
 template <typename IT>
-__device__ __forceinline__ Raw4<IT> load4(const IT *p, int have, bool vec) {
-  Raw4<IT> x{};
-  if (vec) {
-    if (have > 0) x = *(const Raw4<IT> *)p;
-  } else {
+__device__ __forceinline__ Raw4<IT> load4(const IT *p, const IT *safe, int have, bool vec) {
+  if (vec) return *(const Raw4<IT> *)(have > 0 ? p : safe);
+  Four<IT> x{};
 #pragma unroll
-    for (int j = 0; j < 4; ++j)
-      if (j < have) x.e[j] = p[j];
-  }
-  return x;
+  for (int j = 0; j < 4; ++j)
+    if (j < have) x.e[j] = p[j];
+  return __builtin_bit_cast(Raw4<IT>, x);
 }
 template <typename IT>
-__device__ __forceinline__ f4 to_f4(const Raw4<IT> &x) {
+__device__ __forceinline__ f4 to_f4(Raw4<IT> w, bool live) {
+  const Four<IT> x = __builtin_bit_cast(Four<IT>, live ? w : (Raw4<IT>)0u);
   f4 r;
 #pragma unroll
   for (int j = 0; j < 4; ++j) r[j] = Conv<IT>::load(&x.e[j]);
@@ -129,21 +130,21 @@ __device__ __forceinline__ f4 to_f4(const Raw4<IT> &x) {
 }
 // The same as operand parts.
 template <typename IT, int N>
-__device__ __forceinline__ void to_parts(const Raw4<IT> &x, bf4 (&p)[N]) {
-  if constexpr (std::is_same_v<IT, bf16_t> && N == 1) p[0] = __builtin_bit_cast(bf4, x);
-  else split_parts<N>(to_f4<IT>(x), p);
+__device__ __forceinline__ void to_parts(Raw4<IT> x, bool live, bf4 (&p)[N]) {
+  if constexpr (std::is_same_v<IT, bf16_t> && N == 1) p[0] = __builtin_bit_cast(bf4, live ? x : (Raw4<IT>)0u);
+  else split_parts<N>(to_f4<IT>(x, live), p);
 }
 template <typename IT>
 __device__ __forceinline__ void store4(IT *p, f4 x, int have, bool vec) {
-  Raw4<IT> r;
+  Four<IT> r;
   if constexpr (std::is_same_v<IT, bf16_t>) {
-    r = __builtin_bit_cast(Raw4<IT>, __builtin_convertvector(x, bf4));
+    r = __builtin_bit_cast(Four<IT>, __builtin_convertvector(x, bf4));
   } else {
 #pragma unroll
     for (int j = 0; j < 4; ++j) Conv<IT>::store(&r.e[j], x[j]);
   }
   if (vec) {
-    if (have > 0) *(Raw4<IT> *)p = r;
+    if (have > 0) *(Raw4<IT> *)p = __builtin_bit_cast(Raw4<IT>, r);
   } else {
 #pragma unroll
     for (int j = 0; j < 4; ++j)
@@ -177,10 +178,14 @@ __device__ __forceinline__ void delta_tile(int nv, int heads, int &bh, int &vt) 
   }
 }
 
-// Row factors of a chunk, kDeltaRows floats: [0] a = |k|^-1 e^G, [1] beta, [2] c = |k|^-1 e^{G_C - G},
-// [3] d = scale |q|^-1 e^G, [4] |k|^-1, [5] scale |q|^-1 (the norms are 1 without qk_norm), [6..7] G as float64.
+// Row factors of a chunk, kDeltaRows floats: per token a = |k|^-1 e^G, beta, c = |k|^-1 e^{G_C - G} and
+// d = scale |q|^-1 e^G; then [4] |k|^-1, [5] scale |q|^-1 (the norms are 1 without qk_norm), [6..7] G as
+// float64, [8] e^{G_C}, which every lane wants: read by the scalar unit.
 __device__ __forceinline__ const float *delta_rows(const DeltaParams &p, int64_t ch) { return p.rows + ch * kDeltaRows; }
-__device__ __forceinline__ double chunk_sum(const float *rows) { return ((const double *)(rows + 6 * kC))[kC - 1]; }
+__device__ __forceinline__ f4 token_row(const float *rows, int tok) { return *(const f4 *)(rows + (unsigned)(4 * tok)); }
+__device__ __forceinline__ float chunk_decay(const float *rows) {
+  return *(const __attribute__((address_space(4))) float *)(uintptr_t)(rows + 8 * kC);
+}
 
 // Arrays of operand fragments.  Per chunk and key head, in DParts::in parts of 64 DK: the rows of K and Q
 // (token tile w, step s of keys: fragment w DK/32 + s) and their columns (key tile t, step s of tokens:
@@ -197,5 +202,10 @@ __device__ __forceinline__ float *state_of(float *m, const DeltaParams &p, int64
 __device__ __forceinline__ float *value_of(float *m, const DeltaParams &p, int64_t ch, int vt) {
   return m + (ch * p.VT + vt) * kC * 16;
 }
+
+// Whether a wavefront of the walks takes two tiles of 16 columns of v.  Every read of memory takes a compute
+// unit's address unit 16 cycles, whatever its width, and the fragments' reads are the most of them; two
+// tiles share them.  Below one workgroup a compute unit the pair only leaves compute units without work.
+inline bool delta_pairs(const DeltaParams &p) { return p.B * p.H * ((p.VT + 1) / 2) >= 256; }
 
 }  // namespace ssm

@@ -20,41 +20,45 @@ namespace ssm {
 
 hipError_t launch_delta_prep_t(const DeltaParams &p, int dtype, hipStream_t s);
 
-template <typename IT, int DK>
-__global__ void __launch_bounds__(kDT, DK * sizeof(IT) <= 256 ? 2 : 1) k_delta_bwd(const DeltaParams p) {
+template <typename IT, int DK, int NV>
+__global__ void __launch_bounds__(kDT, DK * sizeof(IT) * NV <= 256 ? 2 : 1) k_delta_bwd(const DeltaParams p) {
   constexpr int NK = DParts<IT>::in, NM = DParts<IT>::mid, KS = DK / 32, RT = DK / 64;
-  __shared__ __align__(16) VTile<NM, DK> Dt;
-  __shared__ __align__(16) VTile<NK, kC> Ot;          // dO
-  __shared__ __align__(16) VTile<NM, kC> Et, Xt, Yt;  // d dO, dU, -beta a dR
-  const int tid = threadIdx.x, lane = tid % 64, w = wave_id(), r16 = lane % 16, kg = lane / 16;
+  __shared__ __align__(16) VTile<NM, DK> Dt[NV];
+  __shared__ __align__(16) VTile<NK, kC> Ot[NV];              // dO
+  __shared__ __align__(16) VTile<NM, kC> Et[NV], Xt[NV], Yt[NV];  // d dO, dU, -beta a dR
+  const int lane = threadIdx.x % 64, w = wave_id(), r16 = lane % 16, kg = lane / 16;
   int bh, vt;
-  delta_tile(p.VT, (int)p.B * p.H, bh, vt);
+  delta_tile((p.VT + NV - 1) / NV, (int)p.B * p.H, bh, vt);
+  vt *= NV;
   const int b = bh / p.H, h = bh % p.H, hk = h / (p.H / p.Hk), v0 = 16 * vt + 4 * kg, have = p.Dv - v0;
   const int tok = 16 * w + r16;
   const IT *dop = (const IT *)p.dout.p + b * p.dout.s0 + h * p.dout.s2 + v0;
   IT *dvp = (IT *)p.dv.p + b * p.dv.s0 + h * p.dv.s2 + v0;
   const int64_t ch0 = (int64_t)bh * p.NC, kch0 = ((int64_t)b * p.Hk + hk) * p.NC;
 
-  f4 D[RT];  // D[key][v0 + i] of key 16 (RT w + r) + r16
+  f4 D[NV][RT];  // D[key][v0 + 16 n + i] of key 16 (RT w + r) + r16
 #pragma unroll
-  for (int r = 0; r < RT; ++r) {
-    const int key = 16 * (RT * w + r) + r16;
+  for (int n = 0; n < NV; ++n)
 #pragma unroll
-    for (int i = 0; i < 4; ++i)
-      D[r][i] = p.dlast && key < p.Dk && i < have ? p.dlast[((int64_t)bh * p.Dk + key) * p.Dv + v0 + i] : 0.0f;
-  }
+    for (int r = 0; r < RT; ++r) {
+      const int key = 16 * (RT * w + r) + r16;
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+        D[n][r][i] = p.dlast && key < p.Dk && 16 * n + i < have ? p.dlast[((int64_t)bh * p.Dk + key) * p.Dv + v0 + 16 * n + i] : 0.0f;
+    }
   bf8 K[KS][NK], T[2][NM], P[2][NM], Kt[RT][2][NK], Qt[RT][2][NK];
-  Raw4<IT> go;
-  float fa, be, fc, fd;
-  double GC;
+  Raw4<IT> go[NV];
+  f4 row;  // a, beta, c, d of the token
+  float eC;
   auto load_rows = [&](int c) {
-    const float *rows = delta_rows(p, ch0 + c);
-    fa = rows[tok]; be = rows[kC + tok]; fc = rows[2 * kC + tok]; fd = rows[3 * kC + tok];
-    GC = chunk_sum(rows);
+    row = token_row(delta_rows(p, ch0 + c), tok);
+    eC = chunk_decay(delta_rows(p, ch0 + c));
   };
   auto load_o = [&](int c) {
     const int64_t t = (int64_t)c * kC + tok;
-    go = load4(dop + t * p.dout.s1, t < p.L ? have : 0, p.vdo);
+#pragma unroll
+    for (int n = 0; n < NV; ++n)
+      go[n] = load4(dop + t * p.dout.s1 + 16 * n, (const IT *)p.dout.p, t < p.L ? have - 16 * n : 0, p.vdo);
   };
   auto load_kp = [&](int c) {  // the transposes of T and P are upper triangular
     const __bf16 *k = key_frags<DK, NK>(p.fK, kch0 + c);
@@ -69,96 +73,119 @@ __global__ void __launch_bounds__(kDT, DK * sizeof(IT) <= 256 ? 2 : 1) k_delta_b
     for (int s = 0; s < 2; ++s)
       if (s >= w / 2) load_frag<NM>((const __bf16 *)p.fT + (ch0 + c) * NM * kFrag, kFrag, 2 * w + s, lane, T[s]);
   };
-  auto load_cols = [&](int c) {
-    const __bf16 *kt = key_frags<DK, NK>(p.fKt, kch0 + c), *qt = key_frags<DK, NK>(p.fQt, kch0 + c);
+  auto load_cols = [&](const void *m, int c, bf8 (&f)[RT][2][NK]) {
+    const __bf16 *kt = key_frags<DK, NK>(m, kch0 + c);
 #pragma unroll
     for (int s = 0; s < 2; ++s)
 #pragma unroll
-      for (int r = 0; r < RT; ++r) {
-        load_frag<NK>(kt, kC * DK, 2 * (RT * w + r) + s, lane, Kt[r][s]);
-        load_frag<NK>(qt, kC * DK, 2 * (RT * w + r) + s, lane, Qt[r][s]);
-      }
+      for (int r = 0; r < RT; ++r) load_frag<NK>(kt, kC * DK, 2 * (RT * w + r) + s, lane, f[r][s]);
   };
   load_rows(p.NC - 1);
   load_o(p.NC - 1);
   load_kp(p.NC - 1);
   load_t(p.NC - 1);
-  load_cols(p.NC - 1);
+  load_cols(p.fQt, p.NC - 1, Qt);
+  load_cols(p.fKt, p.NC - 1, Kt);
   for (int c = p.NC - 1; c >= 0; --c) {
     const int64_t t = (int64_t)c * kC + tok, ch = ch0 + c;
     const int next = c ? c - 1 : 0;
 #pragma unroll
-    for (int r = 0; r < RT; ++r) {
-      const int key = 16 * (RT * w + r) + r16;
-      Dt.put(key, kg, D[r]);
-      if (key < p.Dkp) *(f4 *)(state_of(p.dstates, p, ch, vt) + (unsigned)(16 * key + 4 * kg)) = D[r];
-    }
-    {
-      bf4 o[NK];
-      to_parts<IT, NK>(go, o);
-      Ot.put_parts(tok, kg, o);
-      Et.put(tok, kg, fd * to_f4(go));
-    }
-    load_o(next);
-    const float cc = fc, bu = be, by = -be * fa, eC = fexp((float)GC);
-    load_rows(next);
-    lds_barrier();
-    f4 x = 0;
+    for (int n = 0; n < NV; ++n) {
 #pragma unroll
-    for (int s = 0; s < KS; ++s) {
-      bf8 A[NM];
-      Dt.get(s, lane, A);
-      x = mma<NM>(A, K[s], x);
+      for (int r = 0; r < RT; ++r) {
+        const int key = 16 * (RT * w + r) + r16;
+        Dt[n].put(key, kg, D[n][r]);
+        if (key < p.Dkp && vt + n < p.VT)
+          *(f4 *)(state_of(p.dstates, p, ch, vt + n) + (unsigned)(16 * key + 4 * kg)) = D[n][r];
+      }
+      bf4 o[NK];
+      const bool live = t < p.L && have - 16 * n > 0;
+      to_parts<IT, NK>(go[n], live, o);
+      Ot[n].put_parts(tok, kg, o);
+      Et[n].put(tok, kg, row[3] * to_f4<IT>(go[n], live));
     }
-    x *= cc;
+    const float cc = row[2], bu = row[1], by = -row[1] * row[0], decay = eC;
+    load_rows(next);
+    load_o(next);
+    lds_barrier();
+    f4 x[NV];
+#pragma unroll
+    for (int n = 0; n < NV; ++n) x[n] = 0;
+#pragma unroll
+    for (int s = 0; s < KS; ++s)
+#pragma unroll
+      for (int n = 0; n < NV; ++n) {
+        bf8 A[NM];
+        Dt[n].get(s, lane, A);
+        x[n] = mma<NM>(A, K[s], x[n]);
+      }
+#pragma unroll
+    for (int n = 0; n < NV; ++n) x[n] *= cc;
 #pragma unroll
     for (int s = 0; s < 2; ++s)
       if (s >= w / 2) {
-        bf8 A[NK];
-        Ot.get(s, lane, A);
-        x = mma<NM>(A, P[s], x);
+#pragma unroll
+        for (int n = 0; n < NV; ++n) {
+          bf8 A[NK];
+          Ot[n].get(s, lane, A);
+          x[n] = mma<NM>(A, P[s], x[n]);
+        }
       }
+#pragma unroll
+    for (int n = 0; n < NV; ++n) Xt[n].put(tok, kg, x[n]);
     load_kp(next);
-    Xt.put(tok, kg, x);
     lds_barrier();
 #pragma unroll
     for (int s = 0; s < 2; ++s)  // dR = dU + (T^T - I) dU
       if (s >= w / 2) {
-        bf8 A[NM];
-        Xt.get(s, lane, A);
-        x = mma<NM>(A, T[s], x);
+#pragma unroll
+        for (int n = 0; n < NV; ++n) {
+          bf8 A[NM];
+          Xt[n].get(s, lane, A);
+          x[n] = mma<NM>(A, T[s], x[n]);
+        }
       }
-    load_t(next);
-    Yt.put(tok, kg, by * x);
-    *(f4 *)(value_of(p.dr, p, ch, vt) + (unsigned)(16 * tok + 4 * kg)) = x;
-    store4(dvp + t * p.dv.s1, (f4)(bu * x), t < p.L ? have : 0, p.vdv);
 #pragma unroll
-    for (int r = 0; r < RT; ++r) D[r] *= eC;
+    for (int n = 0; n < NV; ++n) {
+      Yt[n].put(tok, kg, by * x[n]);
+      if (vt + n < p.VT) *(f4 *)(value_of(p.dr, p, ch, vt + n) + (unsigned)(16 * tok + 4 * kg)) = x[n];
+      store4(dvp + t * p.dv.s1 + 16 * n, (f4)(bu * x[n]), t < p.L ? have - 16 * n : 0, p.vdv);
 #pragma unroll
-    for (int s = 0; s < 2; ++s) {
-      bf8 A[NM];
-      Et.get(s, lane, A);
-#pragma unroll
-      for (int r = 0; r < RT; ++r) D[r] = mma<NM>(A, Qt[r][s], D[r]);
+      for (int r = 0; r < RT; ++r) D[n][r] *= decay;
     }
+    load_t(next);
+#pragma unroll
+    for (int s = 0; s < 2; ++s)
+#pragma unroll
+      for (int n = 0; n < NV; ++n) {
+        bf8 A[NM];
+        Et[n].get(s, lane, A);
+#pragma unroll
+        for (int r = 0; r < RT; ++r) D[n][r] = mma<NM>(A, Qt[r][s], D[n][r]);
+      }
+    load_cols(p.fQt, next, Qt);
     lds_barrier();
 #pragma unroll
-    for (int s = 0; s < 2; ++s) {
-      bf8 A[NM];
-      Yt.get(s, lane, A);
+    for (int s = 0; s < 2; ++s)
 #pragma unroll
-      for (int r = 0; r < RT; ++r) D[r] = mma<NM>(A, Kt[r][s], D[r]);
-    }
-    load_cols(next);
+      for (int n = 0; n < NV; ++n) {
+        bf8 A[NM];
+        Yt[n].get(s, lane, A);
+#pragma unroll
+        for (int r = 0; r < RT; ++r) D[n][r] = mma<NM>(A, Kt[r][s], D[n][r]);
+      }
+    load_cols(p.fKt, next, Kt);
   }
   if (p.dh0) {
 #pragma unroll
-    for (int r = 0; r < RT; ++r) {
-      const int key = 16 * (RT * w + r) + r16;
+    for (int n = 0; n < NV; ++n)
 #pragma unroll
-      for (int i = 0; i < 4; ++i)
-        if (key < p.Dk && i < have) p.dh0[((int64_t)bh * p.Dk + key) * p.Dv + v0 + i] = D[r][i];
-    }
+      for (int r = 0; r < RT; ++r) {
+        const int key = 16 * (RT * w + r) + r16;
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+          if (key < p.Dk && 16 * n + i < have) p.dh0[((int64_t)bh * p.Dk + key) * p.Dv + v0 + 16 * n + i] = D[n][r][i];
+      }
   }
 }
 
@@ -239,8 +266,8 @@ __global__ void __launch_bounds__(4 * DK) k_delta_grad(const DeltaParams p) {
         const int vt = 2 * s + sh, have = t0 + 16 * it + r16 < p.L ? p.Dv - 16 * vt - 4 * kg : 0;
         yv[x] = vt < p.VT ? *(const f4 *)(value_of(p.y, p, ch, vt) + 256 * it + (unsigned)(16 * r16 + 4 * kg)) : (f4)0.0f;
         xv[x] = vt < p.VT ? *(const f4 *)(value_of(p.dr, p, ch, vt) + 256 * it + (unsigned)(16 * r16 + 4 * kg)) : (f4)0.0f;
-        go[x] = load4(dop + (t0 + 16 * it) * p.dout.s1 + 16 * vt + ao, have, p.vdo);
-        vv[x] = load4(vp + (t0 + 16 * it) * p.v.s1 + 16 * vt + av, have, p.vv);
+        go[x] = load4(dop + (t0 + 16 * it) * p.dout.s1 + 16 * vt + ao, (const IT *)p.dout.p, have, p.vdo);
+        vv[x] = load4(vp + (t0 + 16 * it) * p.v.s1 + 16 * vt + av, (const IT *)p.v.p, have, p.vv);
       }
     };
     load(0);
@@ -254,12 +281,13 @@ __global__ void __launch_bounds__(4 * DK) k_delta_grad(const DeltaParams p) {
         int sh, it;
         stage_of(x, sh, it);
         const int at = (it * 64 + lane) * 8 + 4 * sh;
-        const float be = rows[kC + 16 * it + r16];
+        const float be = rows[4 * (16 * it + r16) + 1];
         bf4 o[NK], u[NM], r[NP];
-        to_parts<IT, NK>(go[x], o);
+        const bool live = t0 + 16 * it + r16 < p.L && p.Dv - 32 * s - 16 * sh - 4 * kg > 0;
+        to_parts<IT, NK>(go[x], live, o);
         split_parts<NM>((f4)(be * yv[x]), u);
         split_parts<NP>(xv[x], r);
-        const f4 v = to_f4(vv[x]);
+        const f4 v = to_f4<IT>(vv[x], live);
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
           rv[x] = fmaf(xv[x][i], v[i], rv[x]);
@@ -325,7 +353,7 @@ __global__ void __launch_bounds__(4 * DK) k_delta_grad(const DeltaParams p) {
     }
     {  // J and H
       const int i = 16 * wi + r16;
-      const float fqi = rows[5 * kC + i], fki = rows[4 * kC + i] * rows[kC + i];
+      const float fqi = rows[5 * kC + i], fki = rows[4 * kC + i] * rows[4 * i + 1];
       const double Gi = Gs[i];
 #pragma unroll
       for (int j = 0; j < NJ; ++j) {
@@ -357,12 +385,11 @@ __global__ void __launch_bounds__(4 * DK) k_delta_grad(const DeltaParams p) {
 #pragma unroll
     for (int it = 0; it < 4; ++it) {
       const int tok = 16 * it + r16;
-      const float fa = rows[tok], be = rows[kC + tok], fc = rows[2 * kC + tok], fd = rows[3 * kC + tok];
-      const f4 ke = elems(fK, it), f2 = fc * F2[it];
+      const f4 row = token_row(rows, tok), ke = elems(fK, it), f2 = row[2] * F2[it];
 #pragma unroll
       for (int i = 0; i < 4; ++i) cd = fmaf(ke[i], f2[i], cd);
-      F1[it] *= fd;
-      Zk[it] += f2 - (be * fa) * F3[it];
+      F1[it] *= row[3];
+      Zk[it] += f2 - (row[1] * row[0]) * F3[it];
     }
     cd = group_sum<64>(cd);
     if (lane == 0) red[w][1][0] = cd;
@@ -417,7 +444,7 @@ __global__ void __launch_bounds__(4 * DK) k_delta_grad(const DeltaParams p) {
     lds_barrier();
     if (w == 0) {  // dbeta and dg of the head
       const float db = rowb[lane];
-      double s = -(double)rows[kC + lane] * rowv[lane], all = 0, ss = 0;
+      double s = -(double)rows[4 * lane + 1] * rowv[lane], all = 0, ss = 0;
 #pragma unroll
       for (int k = 0; k < NW; ++k) {
         s += red[k][0][lane];
@@ -429,7 +456,7 @@ __global__ void __launch_bounds__(4 * DK) k_delta_grad(const DeltaParams p) {
         const double up = __shfl_down(s, d);
         if (lane + d < 64) s += up;
       }
-      s += all + (double)fexp((float)Gs[kC - 1]) * ss;
+      s += all + (double)chunk_decay(rows) * ss;
       const int64_t t = t0 + lane;
       if (t < p.L) {
         ((float *)p.dg.p)[b * p.dg.s0 + t * p.dg.s1 + h * p.dg.s2] = (float)s;
@@ -477,7 +504,10 @@ __global__ void __launch_bounds__(4 * DK) k_delta_grad(const DeltaParams p) {
 
 template <typename IT, int DK>
 static hipError_t delta_bwd(const DeltaParams &p, hipStream_t s) {
-  hipLaunchKernelGGL((k_delta_bwd<IT, DK>), dim3((unsigned)(p.B * p.H) * (unsigned)p.VT), dim3(kDT), 0, s, p);
+  if (delta_pairs(p))
+    hipLaunchKernelGGL((k_delta_bwd<IT, DK, 2>), dim3((unsigned)(p.B * p.H) * (unsigned)((p.VT + 1) / 2)), dim3(kDT), 0, s, p);
+  else
+    hipLaunchKernelGGL((k_delta_bwd<IT, DK, 1>), dim3((unsigned)(p.B * p.H) * (unsigned)p.VT), dim3(kDT), 0, s, p);
   hipLaunchKernelGGL((k_delta_grad<IT, DK>), dim3((unsigned)(p.B * p.Hk) * (unsigned)p.NC), dim3(4 * DK), 0, s, p);
   return hipGetLastError();
 }
