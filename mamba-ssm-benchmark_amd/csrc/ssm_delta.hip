@@ -9,12 +9,12 @@
 namespace ssm {
 
 // c(16 x 16) += a b from float32 LDS matrices: a's rows and b's columns of 16.
-template <int PITCH>
+template <int PA, int PB>
 __device__ __forceinline__ f4 mma_f32(const float *a, const float *b, int lane, f4 c) {
 #pragma unroll
   for (int k = 0; k < 4; ++k)
-    c = __builtin_amdgcn_mfma_f32_16x16x4f32(a[(lane % 16) * PITCH + 4 * k + lane / 16],
-                                             b[(4 * k + lane / 16) * PITCH + lane % 16], c, 0, 0, 0);
+    c = __builtin_amdgcn_mfma_f32_16x16x4f32(a[(lane % 16) * PA + 4 * k + lane / 16],
+                                             b[(4 * k + lane / 16) * PB + lane % 16], c, 0, 0, 0);
   return c;
 }
 template <int PITCH>
@@ -29,20 +29,26 @@ __device__ __forceinline__ void put16(float *m, int lane, f4 c, float sign) {
 // T is inverted in float32: the four 16 x 16 diagonal blocks by substitution, one wavefront each, the
 // rest by T10 = -T11 (L10 T00) for blocks of 16, then of 32 rows.
 template <typename IT, int DK, bool BWD>
-__global__ void __launch_bounds__(kDT) k_delta_prep(const DeltaParams p) {
-  constexpr int NK = DParts<IT>::in, NM = DParts<IT>::mid, NP = BWD ? NM : DParts<IT>::out, KS = DK / 32, FP = kC + 4;
-  __shared__ __align__(16) __bf16 Kf[NK][4 * KS * 64 * 8], Qf[NK][4 * KS * 64 * 8];  // as in memory
-  __shared__ __align__(16) float Lm[kC][FP], Yr[32 * FP];
-  __shared__ double Gs[kC];
-  __shared__ float fk[kC], fq[kC], bs[kC];
-  const int tid = threadIdx.x, lane = tid % 64, w = wave_id(), r16 = lane % 16, kg = lane / 16;
+__global__ void __launch_bounds__(kDT, 4 - DParts<IT>::in) k_delta_prep(const DeltaParams p) {
+  constexpr int NK = DParts<IT>::in, NM = DParts<IT>::mid, NP = BWD ? NM : DParts<IT>::out, KS = DK / 32, FP = kC + 4, YP = 32 + 4;
+  constexpr int kRowsOf = 4 * KS * 64 * 8;  // elements of one part of K or Q
+  __shared__ __align__(16) __bf16 Kf[NK][kRowsOf], Qf[BWD ? NK : 1][BWD ? kRowsOf : 8];  // as in memory
+  __shared__ __align__(16) float Lm[kC][FP];
+  __shared__ float Gh[kC], Gl[kC], fk[kC], fq[kC], bs[kC];  // G as the sum of two floats
+  static_assert(sizeof(Kf) >= sizeof(float) * 32 * YP, "the inversion's scratch");
+  float *const Yr = (float *)&Kf[0][0];                     // ... lies where the keys were
+  const int tid = threadIdx.x, lane = tid % 64, w = wave_id(), r16 = lane % 16, kg = lane / 16, own = 16 * w + r16;
   const int64_t ch = blockIdx.x;
   const int group = p.H / p.Hk, bh = (int)(ch / p.NC), c = (int)(ch % p.NC), b = bh / p.H, h = bh % p.H, hk = h / group;
-  const int64_t t0 = (int64_t)c * kC, t = t0 + 16 * w + r16, kch = ((int64_t)b * p.Hk + hk) * p.NC + c;
+  const int64_t t0 = (int64_t)c * kC, t = t0 + own, kch = ((int64_t)b * p.Hk + hk) * p.NC + c;
   const IT *kp = (const IT *)p.k.p + b * p.k.s0 + t * p.k.s1 + hk * p.k.s2;
   const IT *qp = (const IT *)p.q.p + b * p.q.s0 + t * p.q.s1 + hk * p.q.s2;
   const int have = t < p.L ? p.Dk : 0;
   const bool first = h % group == 0;
+  float head_in = 0;  // wavefront 0: g, 1: beta, of token `lane`
+  if (w < 2 && t0 + lane < p.L)
+    head_in = w ? load_either<IT>(p.beta.p, p.beta32, b * p.beta.s0 + (t0 + lane) * p.beta.s1 + h * p.beta.s2)
+                : ((const float *)p.g.p)[b * p.g.s0 + (t0 + lane) * p.g.s1 + h * p.g.s2];
   bf8 K[KS][NK], Q[KS][NK];
   Raw4<IT> x[KS][4];
   const IT *const ks = (const IT *)p.k.p, *const qs = (const IT *)p.q.p;
@@ -54,50 +60,46 @@ __global__ void __launch_bounds__(kDT) k_delta_prep(const DeltaParams p) {
     x[s][2] = load4(qp + e, qs, have - e, p.vq);
     x[s][3] = load4(qp + e + 16, qs, have - e - 16, p.vq);
   }
+  if (w == 0) {
+    double G = (double)head_in;
+    if (G < -1e4) G = -1e4;  // e^-1e4 is 0 in either width, and -inf would make inf - inf of the differences
+    G = wave_scan_f64(G);
+    Gh[lane] = (float)G;
+    Gl[lane] = (float)(G - (double)(float)G);
+  } else if (w == 1) {
+    bs[lane] = head_in;
+  }
+  float kk = 0, qq = 0;  // sums of squares
 #pragma unroll
   for (int s = 0; s < KS; ++s) {
     const int e = 32 * s + 4 * kg;
     bf4 a[4][NK];
 #pragma unroll
-    for (int i = 0; i < 4; ++i) to_parts<IT, NK>(x[s][i], have - e - 16 * (i % 2) > 0, a[i]);
+    for (int i = 0; i < 4; ++i) {
+      const bool live = have - e - 16 * (i % 2) > 0;
+      to_parts<IT, NK>(x[s][i], live, a[i]);
+      const f4 f = to_f4<IT>(x[s][i], live);
+#pragma unroll
+      for (int j = 0; j < 4; ++j) (i < 2 ? kk : qq) = fmaf(f[j], f[j], i < 2 ? kk : qq);
+    }
 #pragma unroll
     for (int n = 0; n < NK; ++n) {
       K[s][n] = __builtin_shufflevector(a[0][n], a[1][n], 0, 1, 2, 3, 4, 5, 6, 7);
       Q[s][n] = __builtin_shufflevector(a[2][n], a[3][n], 0, 1, 2, 3, 4, 5, 6, 7);
       *(bf8 *)&Kf[n][((w * KS + s) * 64 + lane) * 8] = K[s][n];
-      *(bf8 *)&Qf[n][((w * KS + s) * 64 + lane) * 8] = Q[s][n];
+      if (BWD) *(bf8 *)&Qf[n][((w * KS + s) * 64 + lane) * 8] = Q[s][n];
     }
   }
-  if (w == 0) {
-    const int64_t tt = t0 + lane;
-    double g = 0;
-    if (tt < p.L) g = (double)((const float *)p.g.p)[b * p.g.s0 + tt * p.g.s1 + h * p.g.s2];
-    if (g < -1e4) g = -1e4;  // e^-1e4 is 0 in either width, and -inf would make inf - inf of the differences
-#pragma unroll
-    for (int d = 1; d < 64; d *= 2) {
-      const double up = __shfl_up(g, d);
-      if (lane >= d) g += up;
-    }
-    Gs[lane] = g;
-  } else if (w == 1) {
-    const int64_t tt = t0 + lane;
-    bs[lane] = tt < p.L ? load_either<IT>(p.beta.p, p.beta32, b * p.beta.s0 + tt * p.beta.s1 + h * p.beta.s2) : 0.0f;
+  float nk = 1.0f, nq = p.scale;
+  if (p.qk_norm) {
+    nk = 1.0f / sqrtf(kg_sum(kk) + 1e-6f);
+    nq = p.scale / sqrtf(kg_sum(qq) + 1e-6f);
   }
-  {  // the norms are the diagonals of K K^T and Q Q^T
-    f4 kk = 0, qq = 0;
-#pragma unroll
-    for (int s = 0; s < KS; ++s) {
-      kk = mma<NK>(K[s], K[s], kk);
-      qq = mma<NK>(Q[s], Q[s], qq);
-    }
-#pragma unroll
-    for (int i = 0; i < 4; ++i)
-      if (4 * kg + i == r16) {
-        fk[16 * w + r16] = p.qk_norm ? 1.0f / sqrtf(kk[i] + 1e-6f) : 1.0f;
-        fq[16 * w + r16] = p.qk_norm ? p.scale / sqrtf(qq[i] + 1e-6f) : p.scale;
-      }
+  if (kg == 0) {
+    fk[own] = nk;
+    fq[own] = nq;
   }
-  __syncthreads();
+  lds_barrier();
   if (first) {
     __bf16 *const gK = (__bf16 *)p.fK + kch * NK * kC * DK, *const gQ = (__bf16 *)p.fQ + kch * NK * kC * DK;
     __bf16 *const gKt = (__bf16 *)p.fKt + kch * NK * kC * DK, *const gQt = BWD ? (__bf16 *)p.fQt + kch * NK * kC * DK : nullptr;
@@ -105,47 +107,76 @@ __global__ void __launch_bounds__(kDT) k_delta_prep(const DeltaParams p) {
     for (int n = 0; n < NK; ++n) {
 #pragma unroll
       for (int s = 0; s < KS; ++s) {
-        *(bf8 *)(gK + n * kC * DK + ((w * KS + s) * 64 + lane) * 8) = K[s][n];
-        *(bf8 *)(gQ + n * kC * DK + ((w * KS + s) * 64 + lane) * 8) = Q[s][n];
+        *(bf8 *)(gK + n * kC * DK + (w * KS + s) * 512 + (unsigned)(lane * 8)) = K[s][n];
+        *(bf8 *)(gQ + n * kC * DK + (w * KS + s) * 512 + (unsigned)(lane * 8)) = Q[s][n];
       }
 #pragma unroll
-      for (int x = 0; x < DK / 32; ++x) {  // key tile kt, step s of tokens
-        const int kt = w + 4 * (x / 2), s = x % 2, row = 4 * kg + r16 / 4;
+      for (int y = 0; y < DK / 32; ++y) {  // key tile kt, step s of tokens
+        const int kt = w + 4 * (y / 2), s = y % 2, row = 4 * kg + r16 / 4;
         const int lo = ((2 * s * KS + kt / 2) * 64 + (lane % 4) * 16 + row) * 8 + 4 * (kt % 2), hi = lo + KS * 64 * 8;
-        *(bf8 *)(gKt + n * kC * DK + ((2 * kt + s) * 64 + lane) * 8) = read_tr(&Kf[n][lo], &Kf[n][hi]);
-        if (BWD) *(bf8 *)(gQt + n * kC * DK + ((2 * kt + s) * 64 + lane) * 8) = read_tr(&Qf[n][lo], &Qf[n][hi]);
+        *(bf8 *)(gKt + n * kC * DK + (2 * kt + s) * 512 + (unsigned)(lane * 8)) = read_tr(&Kf[n][lo], &Kf[n][hi]);
+        if (BWD) *(bf8 *)(gQt + n * kC * DK + (2 * kt + s) * 512 + (unsigned)(lane * 8)) = read_tr(&Qf[BWD ? n : 0][lo], &Qf[BWD ? n : 0][hi]);
       }
     }
   }
-  f4 P[4];  // P_ij, token tile w as i, j = 16 x + 4 kg + r; BWD: tile w as j, i = 16 x + 4 kg + r
+  {
+    const float gh = Gh[own], gl = Gl[own], be = bs[own];
+    f4 P[4];  // P_ij, token tile w as i, j = 16 x + 4 kg + r; BWD: tile w as j, i = 16 x + 4 kg + r
 #pragma unroll
-  for (int x = 0; x < 4; ++x) {
-    f4 kk = 0, qk = 0;
+    for (int x = 0; x < 4; ++x) {
+      f4 l = 0, ln = 0, qk = 0;
+      const int at = 16 * x + 4 * kg;
+      const f4 xh = *(const f4 *)&Gh[at], xl = *(const f4 *)&Gl[at], xk = *(const f4 *)&fk[at];
+      if (x <= w) {  // L, and P but in BWD
 #pragma unroll
-    for (int s = 0; s < KS; ++s) {
-      bf8 A[NK];
-      if (x <= w) {
-        load_frag<NK>(&Kf[0][0], 4 * KS * 64 * 8, x * KS + s, lane, A);
-        kk = mma<NK>(A, K[s], kk);
-        if (!BWD) qk = mma<NK>(A, Q[s], qk);
+        for (int s = 0; s < KS; ++s) {
+          bf8 A[NK];
+          load_frag<NK>(&Kf[0][0], kRowsOf, x * KS + s, lane, A);
+          l = mma<NK>(A, K[s], l);
+          if (!BWD) qk = mma<NK>(A, Q[s], qk);
+        }
+        const f4 xb = *(const f4 *)&bs[at];
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+          const float e = fexp((gh - xh[r]) + (gl - xl[r])) * xk[r];
+          ln[r] = at + r < own ? nk * e * (BWD ? be : xb[r]) * l[r] : 0.0f;
+          if (!BWD) qk[r] = at + r <= own ? nq * e * qk[r] : 0.0f;
+        }
       }
       if (BWD && x >= w) {
-        load_frag<NK>(&Qf[0][0], 4 * KS * 64 * 8, x * KS + s, lane, A);
-        qk = mma<NK>(A, K[s], qk);
-      }
-    }
-    const int own = 16 * w + r16;
-    f4 l;
 #pragma unroll
-    for (int r = 0; r < 4; ++r) {
-      const int at = 16 * x + 4 * kg + r;
-      l[r] = at < own ? fexp((float)(Gs[own] - Gs[at])) * fk[own] * fk[at] * (BWD ? bs[own] : bs[at]) * kk[r] : 0.0f;
-      if (BWD) P[x][r] = own <= at ? fexp((float)(Gs[at] - Gs[own])) * fq[at] * fk[own] * qk[r] : 0.0f;
-      else P[x][r] = at <= own ? fexp((float)(Gs[own] - Gs[at])) * fq[own] * fk[at] * qk[r] : 0.0f;
+        for (int s = 0; s < KS; ++s) {
+          bf8 A[NK];
+          load_frag<NK>(&Qf[0][0], kRowsOf, x * KS + s, lane, A);
+          qk = mma<NK>(A, K[s], qk);
+        }
+        const f4 xq = *(const f4 *)&fq[at];
+#pragma unroll
+        for (int r = 0; r < 4; ++r) qk[r] = own <= at + r ? fexp((xh[r] - gh) + (xl[r] - gl)) * xq[r] * nk * qk[r] : 0.0f;
+      }
+      P[x] = qk;
+      *(f4 *)&Lm[own][at] = ln;
     }
-    *(f4 *)&Lm[own][16 * x + 4 * kg] = l;
+#pragma unroll
+    for (int s = 0; s < 2; ++s)
+      if (BWD ? s >= w / 2 : s <= w / 2) {  // the walks read no other
+        bf8 q[NP];
+        split_parts<NP>((f8)__builtin_shufflevector(P[2 * s], P[2 * s + 1], 0, 1, 2, 3, 4, 5, 6, 7), q);
+#pragma unroll
+        for (int n = 0; n < NP; ++n) *(bf8 *)((__bf16 *)p.fP + (ch * NP + n) * kFrag + (2 * w + s) * 512 + (unsigned)(lane * 8)) = q[n];
+      }
   }
-  __syncthreads();
+  if (tid < kC) {
+    float *rows = p.rows + ch * kDeltaRows;
+    const float gh = Gh[tid], gl = Gl[tid], eG = fexp(gh);
+    *(f4 *)(rows + 4 * tid) = f4{fk[tid] * eG, bs[tid], fk[tid] * fexp((Gh[kC - 1] - gh) + (Gl[kC - 1] - gl)), fq[tid] * eG};
+    rows[4 * kC + tid] = fk[tid];
+    rows[5 * kC + tid] = fq[tid];
+    rows[6 * kC + tid] = gh;
+    rows[7 * kC + tid] = gl;
+    if (tid == kC - 1) rows[8 * kC] = eG;
+  }
+  wave_lds_sync();  // the diagonal block is this wavefront's own
   {
     const float *D = &Lm[16 * w][16 * w];
     float x[16];
@@ -159,60 +190,46 @@ __global__ void __launch_bounds__(kDT) k_delta_prep(const DeltaParams p) {
     wave_lds_sync();
     if (kg == 0) {
 #pragma unroll
-      for (int i = 0; i < 16; ++i) Lm[16 * w + i][16 * w + r16] = x[i];
+      for (int i = 0; i < 16; ++i) Lm[16 * w + i][own] = x[i];
     }
   }
-  __syncthreads();
+  lds_barrier();
   if (w < 2) {
-    float *Y = Yr + 16 * w * FP;
-    put16<FP>(Y, lane, mma_f32<FP>(&Lm[32 * w + 16][32 * w], &Lm[32 * w][32 * w], lane, (f4)0.0f), 1.0f);
+    float *Y = Yr + 16 * w * YP;
+    put16<YP>(Y, lane, mma_f32<FP, FP>(&Lm[32 * w + 16][32 * w], &Lm[32 * w][32 * w], lane, (f4)0.0f), 1.0f);
     wave_lds_sync();
-    const f4 t10 = mma_f32<FP>(&Lm[32 * w + 16][32 * w + 16], Y, lane, (f4)0.0f);
+    const f4 t10 = mma_f32<FP, YP>(&Lm[32 * w + 16][32 * w + 16], Y, lane, (f4)0.0f);
     wave_lds_sync();
     put16<FP>(&Lm[32 * w + 16][32 * w], lane, t10, -1.0f);
   }
-  __syncthreads();
+  lds_barrier();
   const int r = w / 2, cc = w % 2;
   {
     f4 y = 0;
-    for (int k = cc; k < 2; ++k) y = mma_f32<FP>(&Lm[32 + 16 * r][16 * k], &Lm[16 * k][16 * cc], lane, y);
-    put16<FP>(Yr + 16 * r * FP + 16 * cc, lane, y, 1.0f);
+    for (int k = cc; k < 2; ++k) y = mma_f32<FP, FP>(&Lm[32 + 16 * r][16 * k], &Lm[16 * k][16 * cc], lane, y);
+    put16<YP>(Yr + 16 * r * YP + 16 * cc, lane, y, 1.0f);
   }
-  __syncthreads();
+  lds_barrier();
   {
     f4 y = 0;
-    for (int k = 0; k <= r; ++k) y = mma_f32<FP>(&Lm[32 + 16 * r][32 + 16 * k], Yr + 16 * k * FP + 16 * cc, lane, y);
+    for (int k = 0; k <= r; ++k) y = mma_f32<FP, YP>(&Lm[32 + 16 * r][32 + 16 * k], Yr + 16 * k * YP + 16 * cc, lane, y);
     put16<FP>(&Lm[32 + 16 * r][16 * cc], lane, y, -1.0f);
   }
-  __syncthreads();
+  lds_barrier();
 #pragma unroll
-  for (int s = 0; s < 2; ++s) {
-    const int own = 16 * w + r16;
-    f8 x;
+  for (int s = 0; s < 2; ++s)
+    if (BWD ? s >= w / 2 : s <= w / 2) {
+      f8 x;
 #pragma unroll
-    for (int j = 0; j < 8; ++j) {
-      const int e = 32 * s + 16 * (j / 4) + 4 * kg + j % 4;
-      x[j] = e == own ? 0.0f : BWD ? Lm[e][own] : Lm[own][e];
+      for (int j = 0; j < 8; ++j) {
+        const int e = 32 * s + 16 * (j / 4) + 4 * kg + j % 4;
+        x[j] = e == own ? 0.0f : BWD ? Lm[e][own] : Lm[own][e];
+      }
+      bf8 a[NM];
+      split_parts<NM>(x, a);
+#pragma unroll
+      for (int n = 0; n < NM; ++n) *(bf8 *)((__bf16 *)p.fT + (ch * NM + n) * kFrag + (2 * w + s) * 512 + (unsigned)(lane * 8)) = a[n];
     }
-    const int64_t at = ((2 * w + s) * 64 + lane) * 8;
-    bf8 a[NM], q[NP];
-    split_parts<NM>(x, a);
-#pragma unroll
-    for (int n = 0; n < NM; ++n) *(bf8 *)((__bf16 *)p.fT + (ch * NM + n) * kFrag + at) = a[n];
-    split_parts<NP>((f8)__builtin_shufflevector(P[2 * s], P[2 * s + 1], 0, 1, 2, 3, 4, 5, 6, 7), q);
-#pragma unroll
-    for (int n = 0; n < NP; ++n) *(bf8 *)((__bf16 *)p.fP + (ch * NP + n) * kFrag + at) = q[n];
-  }
-  if (tid < kC) {
-    float *rows = p.rows + ch * kDeltaRows;
-    const double G = Gs[tid];
-    const float eG = fexp((float)G);
-    *(f4 *)(rows + 4 * tid) = f4{fk[tid] * eG, bs[tid], fk[tid] * fexp((float)(Gs[kC - 1] - G)), fq[tid] * eG};
-    rows[4 * kC + tid] = fk[tid];
-    rows[5 * kC + tid] = fq[tid];
-    ((double *)(rows + 6 * kC))[tid] = G;
-    if (tid == kC - 1) rows[8 * kC] = eG;
-  }
 }
 
 // Everything that does not hang on the state is read a chunk ahead, into the registers that the chunk has

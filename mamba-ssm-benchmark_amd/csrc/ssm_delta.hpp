@@ -6,7 +6,8 @@
 //   X = V - e^G K S0,  Y = T X,  U = beta Y,  T = (I + strictly lower(e^{G_i - G_j} k_i.k_j beta_j))^-1
 //   O = scale e^G Q S0 + P U,  P_ij = scale e^{G_i - G_j} q_i.k_j (j <= i),  S1 = e^{G_C} S0 + K^T (e^{G_C - G} U)
 // so that everything but the factors is products of 64-row tiles, which run on the matrix cores.
-// Every exponent is a difference of later minus earlier cumulative decays, taken in float64.
+// Every exponent is a difference of later minus earlier cumulative decays, which are summed in float64 and
+// kept as two floats, so that the difference is off by its own rounding only.
 //
 // Products take bf16 operands and accumulate in float32.  A float32 operand is held as the sum of
 // bf16 parts (x = p0 + p1 + ..., each the rounding of what the earlier ones leave: 8 significant bits
@@ -163,6 +164,27 @@ __device__ __forceinline__ void store_either(void *t, bool f32, int64_t at, floa
   else Conv<IT>::store((IT *)t + at, v);
 }
 
+__device__ __forceinline__ float kg_sum(float v) {  // over the four lanes of a column
+  v += __shfl_xor(v, 16);
+  return v + __shfl_xor(v, 32);
+}
+// Inclusive sums over the wavefront's lanes.
+template <int CTRL, int ROWS>
+__device__ __forceinline__ double scan_part(double v) {
+  const unsigned long long u = __builtin_bit_cast(unsigned long long, v);
+  const unsigned lo = (unsigned)__builtin_amdgcn_update_dpp(0, (int)(unsigned)u, CTRL, ROWS, 0xF, false);
+  const unsigned hi = (unsigned)__builtin_amdgcn_update_dpp(0, (int)(unsigned)(u >> 32), CTRL, ROWS, 0xF, false);
+  return v + __builtin_bit_cast(double, ((unsigned long long)hi << 32) | lo);
+}
+__device__ __forceinline__ double wave_scan_f64(double v) {
+  v = scan_part<0x111, 0xF>(v);  // row_shr:1, 2, 4, 8
+  v = scan_part<0x112, 0xF>(v);
+  v = scan_part<0x114, 0xF>(v);
+  v = scan_part<0x118, 0xF>(v);
+  v = scan_part<0x142, 0xA>(v);  // row_bcast:15 into rows 1 and 3
+  return scan_part<0x143, 0xC>(v);  // row_bcast:31 into rows 2 and 3
+}
+
 __device__ __forceinline__ float fexp(float x) { return fast_exp2(x * LOG2E); }
 
 // Head, chunk-independent addressing.  Workgroup l runs on XCD l % 8: the NV column tiles of a head
@@ -179,8 +201,8 @@ __device__ __forceinline__ void delta_tile(int nv, int heads, int &bh, int &vt) 
 }
 
 // Row factors of a chunk, kDeltaRows floats: per token a = |k|^-1 e^G, beta, c = |k|^-1 e^{G_C - G} and
-// d = scale |q|^-1 e^G; then [4] |k|^-1, [5] scale |q|^-1 (the norms are 1 without qk_norm), [6..7] G as
-// float64, [8] e^{G_C}, which every lane wants: read by the scalar unit.
+// d = scale |q|^-1 e^G; then [4] |k|^-1, [5] scale |q|^-1 (the norms are 1 without qk_norm), [6] + [7] G
+// as the sum of two floats, [8] e^{G_C}, which every lane wants: read by the scalar unit.
 __device__ __forceinline__ const float *delta_rows(const DeltaParams &p, int64_t ch) { return p.rows + ch * kDeltaRows; }
 __device__ __forceinline__ f4 token_row(const float *rows, int tok) { return *(const f4 *)(rows + (unsigned)(4 * tok)); }
 __device__ __forceinline__ float chunk_decay(const float *rows) {

@@ -189,55 +189,65 @@ __global__ void __launch_bounds__(kDT, DK * sizeof(IT) * NV <= 256 ? 2 : 1) k_de
   }
 }
 
-__device__ __forceinline__ float kg_sum(float v) {  // over the four lanes of a column
-  v += __shfl_xor(v, 16);
-  return v + __shfl_xor(v, 32);
-}
-
 // Wavefront w owns keys 16 w .. 16 w + 15 (DK / 16 wavefronts).  Results are transposed, so that a lane
-// holds 4 keys of one token.  The values are staged 32 columns at a time, as fragments in two buffers, the
-// states go from memory to registers, both one slab ahead.
-template <typename IT, int DK>
+// holds 4 keys of one token.  The values are staged 32 columns (a slab) at a time, as fragments in two buffers,
+// the states go from memory to registers, both one slab ahead; what the products of the chunk's end want is
+// read during the last slab.  SHARED: several value heads add to dq', dk', which wait in LDS meanwhile.
+template <typename IT, int DK, bool SHARED>
 __global__ void __launch_bounds__(4 * DK) k_delta_grad(const DeltaParams p) {
   constexpr int NK = DParts<IT>::in, NM = DParts<IT>::mid, NP = DParts<IT>::out, NT = 4 * DK, NW = DK / 16;
   constexpr int NJ = 16 / NW;                    // tiles of J and H per wavefront
   constexpr int SF = 4 * 64 * 8;                 // staged elements of one part: 64 tokens x 32 columns
   constexpr int kStage = (NK + NM + NP) * SF, JP = kC + 8, kE = (NM + NP) * kC * JP, PT = 512 / NT;
   __shared__ __align__(16) __bf16 buf[2 * kStage > kE ? 2 * kStage : kE];  // dO, U, dR; then J and H
-  __shared__ double Gs[kC];
-  __shared__ float red[NW][2][kC], rowb[kC], rowv[kC], sdot[NW];
+  __shared__ __align__(16) f4 sum[SHARED ? 8 : 1][SHARED ? NT : 1];
+  __shared__ __align__(16) float rows[kDeltaRows];
+  __shared__ float red[NW][kC], norm[NW][2][kC], rowb[kC], rowv[kC], sdot[NW], cdot[NW];
   const int tid = threadIdx.x, lane = tid % 64, w = wave_id(), r16 = lane % 16, kg = lane / 16;
-  const int c = blockIdx.x % p.NC, bk = blockIdx.x / p.NC, b = bk / p.Hk, hk = bk % p.Hk, group = p.H / p.Hk;
+  const int c = blockIdx.x % p.NC, bk = blockIdx.x / p.NC, b = bk / p.Hk, hk = bk % p.Hk, group = SHARED ? p.H / p.Hk : 1;
   const int64_t t0 = (int64_t)c * kC, kch = (int64_t)bk * p.NC + c;
   const int wi = w * NJ / 4, wj = w * NJ % 4;    // J's tiles (wi, wj .. wj + NJ - 1)
   const bool keys = 16 * w < p.Dkp;
-  const __bf16 *fK = key_frags<DK, NK>(p.fK, kch), *fQ = key_frags<DK, NK>(p.fQ, kch);
-  const __bf16 *fKt = key_frags<DK, NK>(p.fKt, kch), *fQt = key_frags<DK, NK>(p.fQt, kch);
-  // Makes the compiler read K and Q anew where they are used: kept over the slabs, they would spill.
-  auto reread = [&] { asm volatile("" : "+s"(fK), "+s"(fQ), "+s"(fKt), "+s"(fQt)); };
   const int slabs = (p.VT + 1) / 2;
   const int64_t ao = r16 * p.dout.s1 + 4 * kg, av = r16 * p.v.s1 + 4 * kg;
+  const unsigned at16 = 16 * r16 + 4 * kg;
   __bf16 *const Jm = buf, *const Hm = buf + NM * kC * JP;
 
-  // K or Q of token 16 it + r16, keys 16 w + 4 kg + i
-  auto elems = [&](const __bf16 *f, int it) {
-    f4 x = 0;
+  bf8 Kt[2][NK], Qt[2][NK];  // K and Q by columns: keys 16 w + r16
+  bf4 Ke[4][NK], Qe[4][NK];  // K and Q of token 16 it + r16, keys 16 w + 4 kg + i
+  auto load_keys = [&] {
+    const __bf16 *kt = key_frags<DK, NK>(p.fKt, kch), *qt = key_frags<DK, NK>(p.fQt, kch);
+    const __bf16 *k = key_frags<DK, NK>(p.fK, kch), *q = key_frags<DK, NK>(p.fQ, kch);
+    asm volatile("" : "+s"(kt), "+s"(qt), "+s"(k), "+s"(q));  // read for every head anew: kept over its slabs, they would spill
 #pragma unroll
-    for (int n = NK - 1; n >= 0; --n)
-      x += __builtin_convertvector(*(const bf4 *)(f + n * kC * DK + (it * (DK / 32) + w / 2) * 512 + 4 * (w % 2) + (unsigned)(lane * 8)), f4);
-    return x;
+    for (int it = 0; it < 4; ++it)
+#pragma unroll
+      for (int n = 0; n < NK; ++n) {
+        const int at = n * kC * DK + (it * (DK / 32) + w / 2) * 512 + 4 * (w % 2);
+        Ke[it][n] = *(const bf4 *)(k + at + (unsigned)(lane * 8));
+        Qe[it][n] = *(const bf4 *)(q + at + (unsigned)(lane * 8));
+      }
+#pragma unroll
+    for (int s = 0; s < 2; ++s) {
+      load_frag<NK>(kt, kC * DK, 2 * w + s, lane, Kt[s]);
+      load_frag<NK>(qt, kC * DK, 2 * w + s, lane, Qt[s]);
+    }
+  };
+  auto whole = [](const bf4 (&x)[NK]) {
+    f4 r = __builtin_convertvector(x[NK - 1], f4);
+#pragma unroll
+    for (int n = NK - 2; n >= 0; --n) r += __builtin_convertvector(x[n], f4);
+    return r;
   };
 
-  f4 Yq[4], Zk[4];  // dq', dk' of token 16 it + r16, keys 16 w + 4 kg + i
-#pragma unroll
-  for (int it = 0; it < 4; ++it) Yq[it] = Zk[it] = 0;
-  const float *rows = nullptr;
-
+  f4 Y[4], Z[4];  // dq', dk' of token 16 it + r16, keys 16 w + 4 kg + i
   for (int hg = 0; hg < group; ++hg) {
     const int h = hk * group + hg;
     const int64_t ch = ((int64_t)b * p.H + h) * p.NC + c;
-    rows = delta_rows(p, ch);
-    const IT *dop = (const IT *)p.dout.p + b * p.dout.s0 + h * p.dout.s2, *vp = (const IT *)p.v.p + b * p.v.s0 + h * p.v.s2;
+    const IT *dop = (const IT *)p.dout.p + b * p.dout.s0 + h * p.dout.s2 + t0 * p.dout.s1;
+    const IT *vp = (const IT *)p.v.p + b * p.v.s0 + h * p.v.s2 + t0 * p.v.s1;
+    const float *Sp = state_of(p.states, p, ch, 0) + 256 * w, *Dp = state_of(p.dstates, p, ch, 0) + 256 * w;
+    const float *yp = value_of(p.y, p, ch, 0), *xp = value_of(p.dr, p, ch, 0);
     f4 F1[4], F2[4], F3[4], A[NJ], N[NJ];  // S0 dO^T, D U^T, S0 dR^T; tiles of dO U^T, dR U^T, transposed
 #pragma unroll
     for (int it = 0; it < 4; ++it) F1[it] = F2[it] = F3[it] = 0;
@@ -246,52 +256,41 @@ __global__ void __launch_bounds__(4 * DK) k_delta_grad(const DeltaParams p) {
     float sd = 0, rv[PT], rb[PT];  // <S0, D>; dR.v and dR.Y of the staged tokens
     f4 sv[2], dv[2], yv[PT], xv[PT];
     Raw4<IT> go[PT], vv[PT];
-    // staged piece x of this thread: half sh of the slab, token st, columns 4 kg + i
-    auto stage_of = [&](int x, int &sh, int &it) {
-      sh = (w + x * NW) / 4;
-      it = (w + x * NW) % 4;
-    };
+    // staged piece x of this wavefront: half (w + x NW) / 4 of the slab, tokens 16 (w + x NW) % 4 + r16, columns 4 kg + i
     auto load = [&](int s) {
 #pragma unroll
-      for (int x = 0; x < 2; ++x) {
-        const int vt = 2 * s + x;
-        const bool in = keys && vt < p.VT;
-        sv[x] = in ? *(const f4 *)(state_of(p.states, p, ch, vt) + 256 * w + (unsigned)(16 * r16 + 4 * kg)) : (f4)0.0f;
-        dv[x] = in ? *(const f4 *)(state_of(p.dstates, p, ch, vt) + 256 * w + (unsigned)(16 * r16 + 4 * kg)) : (f4)0.0f;
+      for (int x = 0; x < PT; ++x) {
+        const int vt = 2 * s + (w + x * NW) / 4, it = (w + x * NW) % 4, have = t0 + 16 * it + r16 < p.L ? p.Dv - 16 * vt - 4 * kg : 0;
+        const int vc = vt < p.VT ? vt : 0;
+        yv[x] = *(const f4 *)(yp + vc * (kC * 16) + 256 * it + at16);
+        xv[x] = *(const f4 *)(xp + vc * (kC * 16) + 256 * it + at16);
+        go[x] = load4(dop + 16 * it * p.dout.s1 + 16 * vt + ao, (const IT *)p.dout.p, have, p.vdo);
+        vv[x] = load4(vp + 16 * it * p.v.s1 + 16 * vt + av, (const IT *)p.v.p, have, p.vv);
       }
 #pragma unroll
-      for (int x = 0; x < PT; ++x) {
-        int sh, it;
-        stage_of(x, sh, it);
-        const int vt = 2 * s + sh, have = t0 + 16 * it + r16 < p.L ? p.Dv - 16 * vt - 4 * kg : 0;
-        yv[x] = vt < p.VT ? *(const f4 *)(value_of(p.y, p, ch, vt) + 256 * it + (unsigned)(16 * r16 + 4 * kg)) : (f4)0.0f;
-        xv[x] = vt < p.VT ? *(const f4 *)(value_of(p.dr, p, ch, vt) + 256 * it + (unsigned)(16 * r16 + 4 * kg)) : (f4)0.0f;
-        go[x] = load4(dop + (t0 + 16 * it) * p.dout.s1 + 16 * vt + ao, (const IT *)p.dout.p, have, p.vdo);
-        vv[x] = load4(vp + (t0 + 16 * it) * p.v.s1 + 16 * vt + av, (const IT *)p.v.p, have, p.vv);
+      for (int x = 0; x < 2; ++x) {
+        const int64_t vc = (keys && 2 * s + x < p.VT ? 2 * s + x : 0) * (int64_t)(p.Dkp * 16) - (keys ? 0 : 256 * w);
+        sv[x] = *(const f4 *)(Sp + vc + at16);
+        dv[x] = *(const f4 *)(Dp + vc + at16);
       }
     };
-    load(0);
-    if (tid < kC) Gs[tid] = ((const double *)(rows + 6 * kC))[tid];
-#pragma unroll
-    for (int x = 0; x < PT; ++x) rv[x] = rb[x] = 0;
-    for (int s = 0; s < slabs; ++s) {
+    bf8 SA[NM], DA[NM];
+    auto stage = [&](int s) {
       __bf16 *const Os = buf + (s & 1) * kStage, *const Us = Os + NK * SF, *const Rs = Us + NM * SF;
 #pragma unroll
       for (int x = 0; x < PT; ++x) {
-        int sh, it;
-        stage_of(x, sh, it);
-        const int at = (it * 64 + lane) * 8 + 4 * sh;
+        const int sh = (w + x * NW) / 4, it = (w + x * NW) % 4, at = (it * 64 + lane) * 8 + 4 * sh;
+        const bool in = 2 * s + sh < p.VT, live = t0 + 16 * it + r16 < p.L && p.Dv - 32 * s - 16 * sh - 4 * kg > 0;
         const float be = rows[4 * (16 * it + r16) + 1];
+        const f4 yy = in ? yv[x] : (f4)0.0f, xx = in ? xv[x] : (f4)0.0f, v = to_f4<IT>(vv[x], live);
         bf4 o[NK], u[NM], r[NP];
-        const bool live = t0 + 16 * it + r16 < p.L && p.Dv - 32 * s - 16 * sh - 4 * kg > 0;
         to_parts<IT, NK>(go[x], live, o);
-        split_parts<NM>((f4)(be * yv[x]), u);
-        split_parts<NP>(xv[x], r);
-        const f4 v = to_f4<IT>(vv[x], live);
+        split_parts<NM>((f4)(be * yy), u);
+        split_parts<NP>(xx, r);
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-          rv[x] = fmaf(xv[x][i], v[i], rv[x]);
-          rb[x] = fmaf(xv[x][i], yv[x][i], rb[x]);
+          rv[x] = fmaf(xx[i], v[i], rv[x]);
+          rb[x] = fmaf(xx[i], yy[i], rb[x]);
         }
 #pragma unroll
         for (int n = 0; n < NK; ++n) *(bf4 *)(Os + n * SF + at) = o[n];
@@ -300,17 +299,20 @@ __global__ void __launch_bounds__(4 * DK) k_delta_grad(const DeltaParams p) {
 #pragma unroll
         for (int n = 0; n < NP; ++n) *(bf4 *)(Rs + n * SF + at) = r[n];
       }
-      bf8 SA[NM], DA[NM];
-      {
-        const f8 x = __builtin_shufflevector(sv[0], sv[1], 0, 1, 2, 3, 4, 5, 6, 7);
-        const f8 y = __builtin_shufflevector(dv[0], dv[1], 0, 1, 2, 3, 4, 5, 6, 7);
+      f8 x = __builtin_shufflevector(sv[0], sv[1], 0, 1, 2, 3, 4, 5, 6, 7);
+      f8 y = __builtin_shufflevector(dv[0], dv[1], 0, 1, 2, 3, 4, 5, 6, 7);
+      if (!keys || 2 * s + 1 >= p.VT) {
 #pragma unroll
-        for (int j = 0; j < 8; ++j) sd = fmaf(x[j], y[j], sd);
-        split_parts<NM>(x, SA);
-        split_parts<NM>(y, DA);
+        for (int j = 0; j < 8; ++j)
+          if (!keys || j >= 4) x[j] = y[j] = 0;
       }
-      if (s + 1 < slabs) load(s + 1);
-      lds_barrier();  // the other buffer's readers are a barrier behind
+#pragma unroll
+      for (int j = 0; j < 8; ++j) sd = fmaf(x[j], y[j], sd);
+      split_parts<NM>(x, SA);
+      split_parts<NM>(y, DA);
+    };
+    auto multiply = [&](int s) {
+      const __bf16 *const Os = buf + (s & 1) * kStage, *const Us = Os + NK * SF, *const Rs = Us + NM * SF;
 #pragma unroll
       for (int it = 0; it < 4; ++it) {
         bf8 O[NK], U[NM], R[NP];
@@ -332,7 +334,31 @@ __global__ void __launch_bounds__(4 * DK) k_delta_grad(const DeltaParams p) {
         }
         __builtin_amdgcn_sched_barrier(0);  // one token tile's operands in registers at a time
       }
+    };
+    {
+      const float *m = delta_rows(p, ch);
+      float x[(kDeltaRows + NT - 1) / NT];
+#pragma unroll
+      for (int i = 0; i < (kDeltaRows + NT - 1) / NT; ++i) x[i] = m[tid + i * NT < kDeltaRows ? tid + i * NT : 0];
+      load(0);
+#pragma unroll
+      for (int i = 0; i < (kDeltaRows + NT - 1) / NT; ++i)
+        if (tid + i * NT < kDeltaRows) rows[tid + i * NT] = x[i];
     }
+#pragma unroll
+    for (int x = 0; x < PT; ++x) rv[x] = rb[x] = 0;
+    lds_barrier();
+    for (int s = 0; s + 1 < slabs; ++s) {
+      stage(s);
+      load(s + 1);
+      lds_barrier();  // the other buffer's readers are a barrier behind
+      multiply(s);
+    }
+    stage(slabs - 1);
+    load_keys();
+    lds_barrier();
+    multiply(slabs - 1);
+
     sd = group_sum<64>(sd);
     if (lane == 0) sdot[w] = sd;
 #pragma unroll
@@ -340,66 +366,55 @@ __global__ void __launch_bounds__(4 * DK) k_delta_grad(const DeltaParams p) {
       rv[x] = kg_sum(rv[x]);
       rb[x] = kg_sum(rb[x]);
     }
-    lds_barrier();  // the slabs are read; red, rowv and rowb of the head before are too
-    // the two halves of the slabs are wavefronts 0..3 and 4..7, or one wavefront's two pieces
-    if constexpr (PT == 2) {
-      if (kg == 0) {
-        rowv[16 * w + r16] = rv[0] + rv[PT - 1];
-        rowb[16 * w + r16] = rb[0] + rb[PT - 1];
-      }
-    } else if (w >= 4 && kg == 0) {
-      rowv[16 * (w - 4) + r16] = rv[0];
-      rowb[16 * (w - 4) + r16] = rb[0];
+    lds_barrier();  // the slabs are read
+    // the two halves of the slabs are one wavefront's two pieces, or wavefronts 0..3 and 4..7
+    if (kg == 0 && (PT == 2 || w >= 4)) {
+      rowv[16 * (w % 4) + r16] = PT == 2 ? rv[0] + rv[PT - 1] : rv[0];
+      rowb[16 * (w % 4) + r16] = PT == 2 ? rb[0] + rb[PT - 1] : rb[0];
     }
     {  // J and H
       const int i = 16 * wi + r16;
-      const float fqi = rows[5 * kC + i], fki = rows[4 * kC + i] * rows[4 * i + 1];
-      const double Gi = Gs[i];
+      const float fqi = rows[5 * kC + i], fki = rows[4 * kC + i] * rows[4 * i + 1], gh = rows[6 * kC + i], gl = rows[7 * kC + i];
 #pragma unroll
       for (int j = 0; j < NJ; ++j) {
-        f4 jv, hv;
+        const int at = 16 * (wj + j) + 4 * kg;
+        f4 jv = 0, hv = 0;
+        if (wj + j <= wi) {
+          const f4 xk = *(const f4 *)(rows + 4 * kC + at), xh = *(const f4 *)(rows + 6 * kC + at), xl = *(const f4 *)(rows + 7 * kC + at);
 #pragma unroll
-        for (int x = 0; x < 4; ++x) {
-          const int jj = 16 * (wj + j) + 4 * kg + x;
-          const float e = jj <= i ? fexp((float)(Gi - Gs[jj])) * rows[4 * kC + jj] : 0.0f;
-          jv[x] = jj <= i ? fqi * e * A[j][x] : 0.0f;
-          hv[x] = jj < i ? -fki * e * N[j][x] : 0.0f;
+          for (int x = 0; x < 4; ++x) {
+            const float e = fexp((gh - xh[x]) + (gl - xl[x])) * xk[x];
+            jv[x] = at + x <= i ? fqi * e * A[j][x] : 0.0f;
+            hv[x] = at + x < i ? -fki * e * N[j][x] : 0.0f;
+          }
         }
         bf4 jp[NM], hp[NP];
         split_parts<NM>(jv, jp);
         split_parts<NP>(hv, hp);
 #pragma unroll
-        for (int n = 0; n < NM; ++n) *(bf4 *)(Jm + (n * kC + i) * JP + 16 * (wj + j) + 4 * kg) = jp[n];
+        for (int n = 0; n < NM; ++n) *(bf4 *)(Jm + (n * kC + i) * JP + at) = jp[n];
 #pragma unroll
-        for (int n = 0; n < NP; ++n) *(bf4 *)(Hm + (n * kC + i) * JP + 16 * (wj + j) + 4 * kg) = hp[n];
+        for (int n = 0; n < NP; ++n) *(bf4 *)(Hm + (n * kC + i) * JP + at) = hp[n];
       }
-    }
-    reread();
-    bf8 Kt[2][NK], Qt[2][NK];
-#pragma unroll
-    for (int s = 0; s < 2; ++s) {
-      load_frag<NK>(fKt, kC * DK, 2 * w + s, lane, Kt[s]);
-      load_frag<NK>(fQt, kC * DK, 2 * w + s, lane, Qt[s]);
     }
     float cd = 0;
 #pragma unroll
     for (int it = 0; it < 4; ++it) {
-      const int tok = 16 * it + r16;
-      const f4 row = token_row(rows, tok), ke = elems(fK, it), f2 = row[2] * F2[it];
+      const f4 row = token_row(rows, 16 * it + r16), ke = whole(Ke[it]), f2 = row[2] * F2[it];
 #pragma unroll
       for (int i = 0; i < 4; ++i) cd = fmaf(ke[i], f2[i], cd);
-      F1[it] *= row[3];
-      Zk[it] += f2 - (row[1] * row[0]) * F3[it];
+      Y[it] = row[3] * F1[it];
+      Z[it] = f2 - (row[1] * row[0]) * F3[it];
     }
     cd = group_sum<64>(cd);
-    if (lane == 0) red[w][1][0] = cd;
+    if (lane == 0) cdot[w] = cd;
     lds_barrier();
 #pragma unroll
     for (int s = 0; s < 2; ++s) {
 #pragma unroll
       for (int it = 0; it < 4; ++it) {
-        const int at = (16 * it + r16) * JP + 32 * s + 4 * kg;                                   // row it, columns of step s
-        const int tr = (32 * s + 4 * kg + r16 / 4) * JP + 16 * it + 4 * (r16 % 4);               // rows of step s, column it
+        const int at = (16 * it + r16) * JP + 32 * s + 4 * kg;                          // row it, columns of step s
+        const int tr = (32 * s + 4 * kg + r16 / 4) * JP + 16 * it + 4 * (r16 % 4);      // rows of step s, column it
         if (s <= it / 2) {
           bf8 B[NM], C[NP];
 #pragma unroll
@@ -412,8 +427,8 @@ __global__ void __launch_bounds__(4 * DK) k_delta_grad(const DeltaParams p) {
             const __bf16 *m = Hm + n * kC * JP + at;
             C[n] = __builtin_shufflevector(*(const bf4 *)m, *(const bf4 *)(m + 16), 0, 1, 2, 3, 4, 5, 6, 7);
           }
-          F1[it] = mma<NM>(Kt[s], B, F1[it]);
-          Zk[it] = mma<NP>(Kt[s], C, Zk[it]);
+          Y[it] = mma<NM>(Kt[s], B, Y[it]);
+          Z[it] = mma<NP>(Kt[s], C, Z[it]);
         }
         if (s >= it / 2) {
           bf8 B[NP], C[NP];
@@ -422,83 +437,81 @@ __global__ void __launch_bounds__(4 * DK) k_delta_grad(const DeltaParams p) {
             B[n] = read_tr(Jm + n * kC * JP + tr, Jm + (n * kC + 16) * JP + tr);
             C[n] = read_tr(Hm + n * kC * JP + tr, Hm + (n * kC + 16) * JP + tr);
           }
-          Zk[it] = mma<NP>(Qt[s], B, Zk[it]);
-          Zk[it] = mma<NP>(Kt[s], C, Zk[it]);
+          Z[it] = mma<NP>(Qt[s], B, Z[it]);
+          Z[it] = mma<NP>(Kt[s], C, Z[it]);
         }
-        __builtin_amdgcn_sched_barrier(0);
       }
     }
 #pragma unroll
     for (int it = 0; it < 4; ++it) {
-      const f4 q = elems(fQ, it) * F1[it];
+      const f4 q = whole(Qe[it]) * Y[it];
       const float x = kg_sum((q[0] + q[1]) + (q[2] + q[3]));
-      if (kg == 0) red[w][0][16 * it + r16] = x;
-      Yq[it] += F1[it];
+      if (kg == 0) red[w][16 * it + r16] = x;
     }
-    if constexpr (PT == 1) {
-      if (w < 4 && kg == 0) {
-        rowv[16 * w + r16] += rv[0];
-        rowb[16 * w + r16] += rb[0];
+    if (PT == 1 && w < 4 && kg == 0) {
+      rowv[16 * w + r16] += rv[0];
+      rowb[16 * w + r16] += rb[0];
+    }
+    if (SHARED) {
+#pragma unroll
+      for (int it = 0; it < 4; ++it) {
+        if (hg) {
+          Y[it] += sum[it][tid];
+          Z[it] += sum[4 + it][tid];
+        }
+        sum[it][tid] = Y[it];
+        sum[4 + it][tid] = Z[it];
+      }
+    }
+    if (p.qk_norm && hg + 1 == group) {
+#pragma unroll
+      for (int it = 0; it < 4; ++it) {
+        const f4 q = whole(Qe[it]) * Y[it], k = whole(Ke[it]) * Z[it];
+        const float sq = kg_sum((q[0] + q[1]) + (q[2] + q[3])), sk = kg_sum((k[0] + k[1]) + (k[2] + k[3]));
+        if (kg == 0) {
+          norm[w][0][16 * it + r16] = sq;
+          norm[w][1][16 * it + r16] = sk;
+        }
       }
     }
     lds_barrier();
     if (w == 0) {  // dbeta and dg of the head
-      const float db = rowb[lane];
       double s = -(double)rows[4 * lane + 1] * rowv[lane], all = 0, ss = 0;
 #pragma unroll
       for (int k = 0; k < NW; ++k) {
-        s += red[k][0][lane];
-        all += red[k][1][0];
+        s += red[k][lane];
+        all += cdot[k];
         ss += sdot[k];
       }
-#pragma unroll
-      for (int d = 1; d < 64; d *= 2) {
-        const double up = __shfl_down(s, d);
-        if (lane + d < 64) s += up;
-      }
-      s += all + (double)chunk_decay(rows) * ss;
+      const double upto = wave_scan_f64(s);  // the sum from i on is the whole less what is before i
+      const double from = (__shfl(upto, 63) - upto) + s + all + (double)rows[8 * kC] * ss;
       const int64_t t = t0 + lane;
       if (t < p.L) {
-        ((float *)p.dg.p)[b * p.dg.s0 + t * p.dg.s1 + h * p.dg.s2] = (float)s;
-        store_either<IT>((void *)p.dbeta.p, p.beta32, b * p.dbeta.s0 + t * p.dbeta.s1 + h * p.dbeta.s2, db);
+        ((float *)p.dg.p)[b * p.dg.s0 + t * p.dg.s1 + h * p.dg.s2] = (float)from;
+        store_either<IT>((void *)p.dbeta.p, p.beta32, b * p.dbeta.s0 + t * p.dbeta.s1 + h * p.dbeta.s2, rowb[lane]);
       }
     }
-    lds_barrier();  // J, H, Gs and sdot are read
+    if (hg + 1 < group) lds_barrier();  // J, H, rows and the sums are read
   }
 
-  // through the norms
-  reread();
-  if (p.qk_norm) {
-#pragma unroll
-    for (int it = 0; it < 4; ++it) {
-      const f4 q = elems(fQ, it) * Yq[it], k = elems(fK, it) * Zk[it];
-      const float sq = kg_sum((q[0] + q[1]) + (q[2] + q[3])), sk = kg_sum((k[0] + k[1]) + (k[2] + k[3]));
-      if (kg == 0) {
-        red[w][0][16 * it + r16] = sq;
-        red[w][1][16 * it + r16] = sk;
-      }
-    }
-    lds_barrier();
-  }
   IT *dqb = (IT *)p.dq.p + b * p.dq.s0 + hk * p.dq.s2, *dkb = (IT *)p.dk.p + b * p.dk.s0 + hk * p.dk.s2;
   const int e = 16 * w + 4 * kg;
 #pragma unroll
   for (int it = 0; it < 4; ++it) {
     const int tok = 16 * it + r16, have = t0 + tok < p.L ? p.Dk - e : 0;
-    f4 y = Yq[it], z = Zk[it];
-    if (p.qk_norm) {
+    if (p.qk_norm) {  // through the norms
       float sq = 0, sk = 0;
 #pragma unroll
       for (int k = 0; k < NW; ++k) {
-        sq += red[k][0][tok];
-        sk += red[k][1][tok];
+        sq += norm[k][0][tok];
+        sk += norm[k][1][tok];
       }
       const float fk = rows[4 * kC + tok], nq = rows[5 * kC + tok] / p.scale;
-      y -= (nq * nq * sq) * elems(fQ, it);
-      z -= (fk * fk * sk) * elems(fK, it);
+      Y[it] -= (nq * nq * sq) * whole(Qe[it]);
+      Z[it] -= (fk * fk * sk) * whole(Ke[it]);
     }
-    store4(dqb + (t0 + tok) * p.dq.s1 + e, y, have, p.vdq);
-    store4(dkb + (t0 + tok) * p.dk.s1 + e, z, have, p.vdk);
+    store4(dqb + (t0 + tok) * p.dq.s1 + e, Y[it], have, p.vdq);
+    store4(dkb + (t0 + tok) * p.dk.s1 + e, Z[it], have, p.vdk);
   }
 }
 
@@ -508,7 +521,9 @@ static hipError_t delta_bwd(const DeltaParams &p, hipStream_t s) {
     hipLaunchKernelGGL((k_delta_bwd<IT, DK, 2>), dim3((unsigned)(p.B * p.H) * (unsigned)((p.VT + 1) / 2)), dim3(kDT), 0, s, p);
   else
     hipLaunchKernelGGL((k_delta_bwd<IT, DK, 1>), dim3((unsigned)(p.B * p.H) * (unsigned)p.VT), dim3(kDT), 0, s, p);
-  hipLaunchKernelGGL((k_delta_grad<IT, DK>), dim3((unsigned)(p.B * p.Hk) * (unsigned)p.NC), dim3(4 * DK), 0, s, p);
+  const dim3 grid((unsigned)(p.B * p.Hk) * (unsigned)p.NC);
+  if (p.H > p.Hk) hipLaunchKernelGGL((k_delta_grad<IT, DK, true>), grid, dim3(4 * DK), 0, s, p);
+  else hipLaunchKernelGGL((k_delta_grad<IT, DK, false>), grid, dim3(4 * DK), 0, s, p);
   return hipGetLastError();
 }
 template <typename IT>
