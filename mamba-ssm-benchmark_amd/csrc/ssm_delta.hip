@@ -39,8 +39,8 @@ __global__ void __launch_bounds__(kDT, 4 - DParts<IT>::in) k_delta_prep(const De
   float *const Yr = (float *)&Kf[0][0];                     // ... lies where the keys were
   const int tid = threadIdx.x, lane = tid % 64, w = wave_id(), r16 = lane % 16, kg = lane / 16, own = 16 * w + r16;
   const int64_t ch = blockIdx.x;
-  const int group = p.H / p.Hk, bh = (int)(ch / p.NC), c = (int)(ch % p.NC), b = bh / p.H, h = bh % p.H, hk = h / group;
-  const int64_t t0 = (int64_t)c * kC, t = t0 + own, kch = ((int64_t)b * p.Hk + hk) * p.NC + c;
+  const int heads = (int)p.B * p.H, group = p.H / p.Hk, bh = (int)(ch % heads), c = (int)(ch / heads), b = bh / p.H, h = bh % p.H, hk = h / group;
+  const int64_t t0 = (int64_t)c * kC, t = t0 + own, kch = ((int64_t)c * p.B + b) * p.Hk + hk;
   const IT *kp = (const IT *)p.k.p + b * p.k.s0 + t * p.k.s1 + hk * p.k.s2;
   const IT *qp = (const IT *)p.q.p + b * p.q.s0 + t * p.q.s1 + hk * p.q.s2;
   const int have = t < p.L ? p.Dk : 0;
@@ -232,157 +232,29 @@ __global__ void __launch_bounds__(kDT, 4 - DParts<IT>::in) k_delta_prep(const De
     }
 }
 
+// The chain from state to state is what bounds the walk, so four wavefronts do nothing else and four more
+// take the outputs (Q S, P U and the stores) from what the chain leaves in LDS, while it goes on.
 // Everything that does not hang on the state is read a chunk ahead, into the registers that the chunk has
 // just used.  All products are of transposes: rows are 16 columns of v, so a lane holds 4 columns of
 // one token or key, and moves them as one word.  A workgroup walks NV tiles of 16 columns.
 template <typename IT, int DK, int NV>
-__global__ void __launch_bounds__(kDT, DK * sizeof(IT) * NV <= 256 ? 2 : 1) k_delta_fwd(const DeltaParams p) {
+__global__ void __launch_bounds__(2 * kDT) k_delta_fwd(const DeltaParams p) {
   constexpr int NK = DParts<IT>::in, NM = DParts<IT>::mid, NP = DParts<IT>::out, KS = DK / 32, RT = DK / 64;
   __shared__ __align__(16) VTile<NM, DK> St[NV];
-  __shared__ __align__(16) VTile<NM, kC> Xt[NV], Wt[NV];
+  __shared__ __align__(16) VTile<NM, kC> Xt[NV], Wt[NV];  // X, c U
   __shared__ __align__(16) VTile<NP, kC> Ut[NV];
-  const int lane = threadIdx.x % 64, w = wave_id(), r16 = lane % 16, kg = lane / 16;
+  const int lane = threadIdx.x % 64, w = wave_id() % 4, r16 = lane % 16, kg = lane / 16;
   int bh, vt;
   delta_tile((p.VT + NV - 1) / NV, (int)p.B * p.H, bh, vt);
   vt *= NV;
   const int b = bh / p.H, h = bh % p.H, hk = h / (p.H / p.Hk), v0 = 16 * vt + 4 * kg, have = p.Dv - v0;
   const int tok = 16 * w + r16;
-  const IT *vp = (const IT *)p.v.p + b * p.v.s0 + h * p.v.s2 + v0;
-  IT *op = (IT *)p.o.p + b * p.o.s0 + h * p.o.s2 + v0;
-  const int64_t ch0 = (int64_t)bh * p.NC, kch0 = ((int64_t)b * p.Hk + hk) * p.NC;
+  auto at = [&](int c) { return (int64_t)c * p.B * p.H + bh; };
+  auto kat = [&](int c) { return ((int64_t)c * p.B + b) * p.Hk + hk; };
 
-  f4 S[NV][RT];  // S[key][v0 + 16 n + i] of key 16 (RT w + r) + r16
-#pragma unroll
-  for (int n = 0; n < NV; ++n)
-#pragma unroll
-    for (int r = 0; r < RT; ++r) {
-      const int key = 16 * (RT * w + r) + r16;
-#pragma unroll
-      for (int i = 0; i < 4; ++i)
-        S[n][r][i] = p.h0 && key < p.Dk && 16 * n + i < have ? p.h0[((int64_t)bh * p.Dk + key) * p.Dv + v0 + 16 * n + i] : 0.0f;
-    }
-  bf8 K[KS][NK], Q[KS][NK], T[2][NM], P[2][NP], Kt[RT][2][NK];
-  Raw4<IT> v[NV];
-  f4 row;  // a, beta, c, d of the token
-  float eC;
-  auto load_rows = [&](int c) {
-    row = token_row(delta_rows(p, ch0 + c), tok);
-    eC = chunk_decay(delta_rows(p, ch0 + c));
-  };
-  auto load_kq = [&](int c) {
-    const __bf16 *k = key_frags<DK, NK>(p.fK, kch0 + c), *q = key_frags<DK, NK>(p.fQ, kch0 + c);
-#pragma unroll
-    for (int s = 0; s < KS; ++s) {
-      load_frag<NK>(k, kC * DK, w * KS + s, lane, K[s]);
-      load_frag<NK>(q, kC * DK, w * KS + s, lane, Q[s]);
-    }
-  };
-  auto load_v = [&](int c) {
-    const int64_t t = (int64_t)c * kC + tok;
-#pragma unroll
-    for (int n = 0; n < NV; ++n) v[n] = load4(vp + t * p.v.s1 + 16 * n, (const IT *)p.v.p, t < p.L ? have - 16 * n : 0, p.vv);
-  };
-  auto load_t = [&](int c) {  // T is lower triangular
-#pragma unroll
-    for (int s = 0; s < 2; ++s)
-      if (s <= w / 2) load_frag<NM>((const __bf16 *)p.fT + (ch0 + c) * NM * kFrag, kFrag, 2 * w + s, lane, T[s]);
-  };
-  auto load_p = [&](int c) {
-    const __bf16 *kt = key_frags<DK, NK>(p.fKt, kch0 + c);
-#pragma unroll
-    for (int s = 0; s < 2; ++s) {
-#pragma unroll
-      for (int r = 0; r < RT; ++r) load_frag<NK>(kt, kC * DK, 2 * (RT * w + r) + s, lane, Kt[r][s]);
-      if (s <= w / 2) load_frag<NP>((const __bf16 *)p.fP + (ch0 + c) * NP * kFrag, kFrag, 2 * w + s, lane, P[s]);
-    }
-  };
-  load_rows(0);
-  load_v(0);
-  load_kq(0);
-  load_t(0);
-  load_p(0);
-  for (int c = 0; c < p.NC; ++c) {
-    const int64_t t = (int64_t)c * kC + tok, ch = ch0 + c;
-    const int next = c + 1 < p.NC ? c + 1 : c;
-#pragma unroll
-    for (int n = 0; n < NV; ++n)
-#pragma unroll
-      for (int r = 0; r < RT; ++r) {
-        const int key = 16 * (RT * w + r) + r16;
-        St[n].put(key, kg, S[n][r]);
-        if (p.states && key < p.Dkp && vt + n < p.VT)
-          *(f4 *)(state_of(p.states, p, ch, vt + n) + (unsigned)(16 * key + 4 * kg)) = S[n][r];
-      }
-    lds_barrier();
-    f4 x[NV], o[NV], y[NV];
-#pragma unroll
-    for (int n = 0; n < NV; ++n) x[n] = o[n] = 0;
-#pragma unroll
-    for (int s = 0; s < KS; ++s)
-#pragma unroll
-      for (int n = 0; n < NV; ++n) {
-        bf8 A[NM];
-        St[n].get(s, lane, A);
-        x[n] = mma<NM>(A, K[s], x[n]);
-        o[n] = mma<NP>(A, Q[s], o[n]);
-      }
-#pragma unroll
-    for (int n = 0; n < NV; ++n) {
-      y[n] = to_f4<IT>(v[n], t < p.L && have - 16 * n > 0) - row[0] * x[n];
-      o[n] *= row[3];
-      Xt[n].put(tok, kg, y[n]);
-    }
-    const float bu = row[1], bc = row[1] * row[2], decay = eC;
-    load_rows(next);
-    load_v(next);
-    load_kq(next);
-    lds_barrier();
-#pragma unroll
-    for (int s = 0; s < 2; ++s)  // Y = X + (T - I) X
-      if (s <= w / 2) {
-#pragma unroll
-        for (int n = 0; n < NV; ++n) {
-          bf8 A[NM];
-          Xt[n].get(s, lane, A);
-          y[n] = mma<NM>(A, T[s], y[n]);
-        }
-      }
-#pragma unroll
-    for (int n = 0; n < NV; ++n) {
-      Wt[n].put(tok, kg, bc * y[n]);
-      Ut[n].put(tok, kg, bu * y[n]);
-      if (p.y && vt + n < p.VT) *(f4 *)(value_of(p.y, p, ch, vt + n) + (unsigned)(16 * tok + 4 * kg)) = y[n];
-    }
-    load_t(next);
-    lds_barrier();
-#pragma unroll
-    for (int n = 0; n < NV; ++n)
-#pragma unroll
-      for (int r = 0; r < RT; ++r) S[n][r] *= decay;
-#pragma unroll
-    for (int s = 0; s < 2; ++s)
-#pragma unroll
-      for (int n = 0; n < NV; ++n) {
-        bf8 A[NM];
-        Wt[n].get(s, lane, A);
-#pragma unroll
-        for (int r = 0; r < RT; ++r) S[n][r] = mma<NM>(A, Kt[r][s], S[n][r]);
-      }
-#pragma unroll
-    for (int s = 0; s < 2; ++s)
-      if (s <= w / 2) {
-#pragma unroll
-        for (int n = 0; n < NV; ++n) {
-          bf8 A[NP];
-          Ut[n].get(s, lane, A);
-          o[n] = mma<NP>(A, P[s], o[n]);
-        }
-      }
-    load_p(next);
-#pragma unroll
-    for (int n = 0; n < NV; ++n) store4(op + t * p.o.s1 + 16 * n, o[n], t < p.L ? have - 16 * n : 0, p.vo);
-  }
-  if (p.last) {
+  if (wave_id() < 4) {
+    const IT *vp = (const IT *)p.v.p + b * p.v.s0 + h * p.v.s2 + v0;
+    f4 S[NV][RT];  // S[key][v0 + 16 n + i] of key 16 (RT w + r) + r16
 #pragma unroll
     for (int n = 0; n < NV; ++n)
 #pragma unroll
@@ -390,8 +262,174 @@ __global__ void __launch_bounds__(kDT, DK * sizeof(IT) * NV <= 256 ? 2 : 1) k_de
         const int key = 16 * (RT * w + r) + r16;
 #pragma unroll
         for (int i = 0; i < 4; ++i)
-          if (key < p.Dk && 16 * n + i < have) p.last[((int64_t)bh * p.Dk + key) * p.Dv + v0 + 16 * n + i] = S[n][r][i];
+          S[n][r][i] = p.h0 && key < p.Dk && 16 * n + i < have ? p.h0[((int64_t)bh * p.Dk + key) * p.Dv + v0 + 16 * n + i] : 0.0f;
       }
+    bf8 K[KS][NK], T[2][NM], Kt[RT][2][NK];
+    Raw4<IT> v[NV];
+    f4 row;  // a, beta, c, d of the token
+    float eC;
+    auto load_v = [&](int c) {
+      const int64_t t = (int64_t)c * kC + tok;
+#pragma unroll
+      for (int n = 0; n < NV; ++n) v[n] = load4(vp + t * p.v.s1 + 16 * n, (const IT *)p.v.p, t < p.L ? have - 16 * n : 0, p.vv);
+      row = token_row(delta_rows(p, at(c)), tok);
+      eC = chunk_decay(delta_rows(p, at(c)));
+    };
+    auto load_k = [&](int c) {
+#pragma unroll
+      for (int s = 0; s < KS; ++s) load_frag<NK>(key_frags<DK, NK>(p.fK, kat(c)), kC * DK, w * KS + s, lane, K[s]);
+    };
+    auto load_t = [&](int c) {  // T is lower triangular
+#pragma unroll
+      for (int s = 0; s < 2; ++s)
+        if (s <= w / 2) load_frag<NM>((const __bf16 *)p.fT + at(c) * NM * kFrag, kFrag, 2 * w + s, lane, T[s]);
+    };
+    auto load_kt = [&](int c) {
+#pragma unroll
+      for (int s = 0; s < 2; ++s)
+#pragma unroll
+        for (int r = 0; r < RT; ++r) load_frag<NK>(key_frags<DK, NK>(p.fKt, kat(c)), kC * DK, 2 * (RT * w + r) + s, lane, Kt[r][s]);
+    };
+    load_k(0);
+    load_v(0);
+    load_t(0);
+    load_kt(0);
+    for (int c = 0; c < p.NC; ++c) {
+      const int64_t t = (int64_t)c * kC + tok;
+      const int next = c + 1 < p.NC ? c + 1 : c;
+#pragma unroll
+      for (int n = 0; n < NV; ++n)
+#pragma unroll
+        for (int r = 0; r < RT; ++r) St[n].put(16 * (RT * w + r) + r16, kg, S[n][r]);
+      lds_barrier();
+      f4 x[NV], y[NV];
+#pragma unroll
+      for (int n = 0; n < NV; ++n) x[n] = 0;
+#pragma unroll
+      for (int s = 0; s < KS; ++s)
+#pragma unroll
+        for (int n = 0; n < NV; ++n) {
+          bf8 A[NM];
+          St[n].get(s, lane, A);
+          x[n] = mma<NM>(A, K[s], x[n]);
+        }
+#pragma unroll
+      for (int n = 0; n < NV; ++n) {
+        y[n] = to_f4<IT>(v[n], t < p.L && have - 16 * n > 0) - row[0] * x[n];
+        Xt[n].put(tok, kg, y[n]);
+      }
+      const float bu = row[1], bc = row[1] * row[2], decay = eC;
+      load_k(next);
+      load_v(next);
+      lds_barrier();
+#pragma unroll
+      for (int s = 0; s < 2; ++s)  // Y = X + (T - I) X
+        if (s <= w / 2) {
+#pragma unroll
+          for (int n = 0; n < NV; ++n) {
+            bf8 A[NM];
+            Xt[n].get(s, lane, A);
+            y[n] = mma<NM>(A, T[s], y[n]);
+          }
+        }
+#pragma unroll
+      for (int n = 0; n < NV; ++n) {
+        Wt[n].put(tok, kg, bc * y[n]);
+        Ut[n].put(tok, kg, bu * y[n]);
+      }
+      load_t(next);
+      lds_barrier();
+#pragma unroll
+      for (int n = 0; n < NV; ++n)
+#pragma unroll
+        for (int r = 0; r < RT; ++r) S[n][r] *= decay;
+#pragma unroll
+      for (int s = 0; s < 2; ++s)
+#pragma unroll
+        for (int n = 0; n < NV; ++n) {
+          bf8 A[NM];
+          Wt[n].get(s, lane, A);
+#pragma unroll
+          for (int r = 0; r < RT; ++r) S[n][r] = mma<NM>(A, Kt[r][s], S[n][r]);
+        }
+      load_kt(next);
+      if (p.y) {
+#pragma unroll
+        for (int n = 0; n < NV; ++n)
+          if (vt + n < p.VT) *(f4 *)(value_of(p.y, p, at(c), vt + n) + (unsigned)(16 * tok + 4 * kg)) = y[n];
+      }
+    }
+    if (p.last) {
+#pragma unroll
+      for (int n = 0; n < NV; ++n)
+#pragma unroll
+        for (int r = 0; r < RT; ++r) {
+          const int key = 16 * (RT * w + r) + r16;
+#pragma unroll
+          for (int i = 0; i < 4; ++i)
+            if (key < p.Dk && 16 * n + i < have) p.last[((int64_t)bh * p.Dk + key) * p.Dv + v0 + 16 * n + i] = S[n][r][i];
+        }
+    }
+  } else {
+    IT *op = (IT *)p.o.p + b * p.o.s0 + h * p.o.s2 + v0;
+    bf8 Q[KS][NK], P[2][NP];
+    float fd;
+    auto load_q = [&](int c) {
+#pragma unroll
+      for (int s = 0; s < KS; ++s) load_frag<NK>(key_frags<DK, NK>(p.fQ, kat(c)), kC * DK, w * KS + s, lane, Q[s]);
+      fd = delta_rows(p, at(c))[(unsigned)(4 * tok + 3)];
+    };
+    auto load_p = [&](int c) {
+#pragma unroll
+      for (int s = 0; s < 2; ++s)
+        if (s <= w / 2) load_frag<NP>((const __bf16 *)p.fP + at(c) * NP * kFrag, kFrag, 2 * w + s, lane, P[s]);
+    };
+    load_q(0);
+    load_p(0);
+    for (int c = 0; c < p.NC; ++c) {
+      const int64_t t = (int64_t)c * kC + tok;
+      const int next = c + 1 < p.NC ? c + 1 : c;
+      lds_barrier();
+      f4 o[NV];
+#pragma unroll
+      for (int n = 0; n < NV; ++n) o[n] = 0;
+#pragma unroll
+      for (int s = 0; s < KS; ++s)
+#pragma unroll
+        for (int n = 0; n < NV; ++n) {
+          bf8 A[NP];
+          St[n].get(s, lane, A);
+          o[n] = mma<NP>(A, Q[s], o[n]);
+        }
+#pragma unroll
+      for (int n = 0; n < NV; ++n) o[n] *= fd;
+      if (p.states) {
+#pragma unroll
+        for (int n = 0; n < NV; ++n)
+#pragma unroll
+          for (int r = 0; r < RT; ++r) {
+            const int key = 16 * (RT * w + r) + r16;
+            if (key < p.Dkp && vt + n < p.VT)
+              *(f4 *)(state_of(p.states, p, at(c), vt + n) + (unsigned)(16 * key + 4 * kg)) = St[n].whole(key, kg);
+          }
+      }
+      load_q(next);
+      lds_barrier();
+      lds_barrier();
+#pragma unroll
+      for (int s = 0; s < 2; ++s)
+        if (s <= w / 2) {
+#pragma unroll
+          for (int n = 0; n < NV; ++n) {
+            bf8 A[NP];
+            Ut[n].get(s, lane, A);
+            o[n] = mma<NP>(A, P[s], o[n]);
+          }
+        }
+      load_p(next);
+#pragma unroll
+      for (int n = 0; n < NV; ++n) store4(op + t * p.o.s1 + 16 * n, o[n], t < p.L ? have - 16 * n : 0, p.vo);
+    }
   }
 }
 
@@ -400,9 +438,9 @@ static hipError_t delta_fwd(const DeltaParams &p, hipStream_t s) {
   const unsigned heads = (unsigned)(p.B * p.H);
   hipLaunchKernelGGL((k_delta_prep<IT, DK, false>), dim3(heads * (unsigned)p.NC), dim3(kDT), 0, s, p);
   if (delta_pairs(p))
-    hipLaunchKernelGGL((k_delta_fwd<IT, DK, 2>), dim3((unsigned)(p.B * p.H) * (unsigned)((p.VT + 1) / 2)), dim3(kDT), 0, s, p);
+    hipLaunchKernelGGL((k_delta_fwd<IT, DK, 2>), dim3((unsigned)(p.B * p.H) * (unsigned)((p.VT + 1) / 2)), dim3(2 * kDT), 0, s, p);
   else
-    hipLaunchKernelGGL((k_delta_fwd<IT, DK, 1>), dim3((unsigned)(p.B * p.H) * (unsigned)p.VT), dim3(kDT), 0, s, p);
+    hipLaunchKernelGGL((k_delta_fwd<IT, DK, 1>), dim3((unsigned)(p.B * p.H) * (unsigned)p.VT), dim3(2 * kDT), 0, s, p);
   return hipGetLastError();
 }
 template <typename IT>

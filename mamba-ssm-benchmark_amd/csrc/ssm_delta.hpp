@@ -38,7 +38,7 @@ typedef float f8 __attribute__((ext_vector_type(8)));
 typedef short s4 __attribute__((ext_vector_type(4)));
 
 constexpr int kC = kDeltaChunk;   // tokens per chunk
-constexpr int kDT = 256;          // threads of the walks: wavefront w owns tokens 16 w .. 16 w + 15
+constexpr int kDT = 256;          // four wavefronts: wavefront w owns tokens 16 w .. 16 w + 15
 constexpr int kFrag = kC * kC;    // elements of one part of a 64 x 64 matrix stored as operand fragments
 
 // Parts of an input of type IT, of float32 intermediates beside it, and of those that only reach outputs of type IT.
@@ -90,11 +90,19 @@ template <int N, int R> struct VTile {
 #pragma unroll
     for (int n = 0; n < N; ++n) *(bf4 *)&e[n][row * 16 + ((kg ^ ((row >> 2) & 2)) * 4)] = p[n];
   }
+  // the value of (row, columns 4 kg + i): the parts' sum, exact with three
+  __device__ __forceinline__ f4 whole(int row, int kg) const {
+    f4 x = 0;
+#pragma unroll
+    for (int n = N - 1; n >= 0; --n) x += __builtin_convertvector(*(const bf4 *)&e[n][row * 16 + ((kg ^ ((row >> 2) & 2)) * 4)], f4);
+    return x;
+  }
   // operand of rows 32 s .. 32 s + 31: lane = column of v
-  __device__ __forceinline__ void get(int s, int lane, bf8 (&f)[N]) const {
+  template <int M>
+  __device__ __forceinline__ void get(int s, int lane, bf8 (&f)[M]) const {  // the first M parts
     const int row = 32 * s + 4 * (lane / 16) + (lane % 16) / 4, at = row * 16 + ((lane % 4) ^ ((row >> 2) & 2)) * 4;
 #pragma unroll
-    for (int n = 0; n < N; ++n) f[n] = read_tr(&e[n][at], &e[n][at + 256]);
+    for (int n = 0; n < M; ++n) f[n] = read_tr(&e[n][at], &e[n][at + 256]);
   }
 };
 
@@ -164,9 +172,15 @@ __device__ __forceinline__ void store_either(void *t, bool f32, int64_t at, floa
   else Conv<IT>::store((IT *)t + at, v);
 }
 
-__device__ __forceinline__ float kg_sum(float v) {  // over the four lanes of a column
-  v += __shfl_xor(v, 16);
-  return v + __shfl_xor(v, 32);
+// Sum over the four lanes of a column (l % 16).
+__device__ __forceinline__ float kg_sum(float v) {
+  const unsigned a = __builtin_bit_cast(unsigned, v);
+  const auto x = __builtin_amdgcn_permlane16_swap(a, a, false, false);  // even rows, odd rows
+  const unsigned x0 = x[0], x1 = x[1];
+  const unsigned b = __builtin_bit_cast(unsigned, __builtin_bit_cast(float, x0) + __builtin_bit_cast(float, x1));
+  const auto y = __builtin_amdgcn_permlane32_swap(b, b, false, false);  // lower half, upper half
+  const unsigned y0 = y[0], y1 = y[1];
+  return __builtin_bit_cast(float, y0) + __builtin_bit_cast(float, y1);
 }
 // Inclusive sums over the wavefront's lanes.
 template <int CTRL, int ROWS>

@@ -20,163 +20,32 @@ namespace ssm {
 
 hipError_t launch_delta_prep_t(const DeltaParams &p, int dtype, hipStream_t s);
 
+// As in the forward, four wavefronts walk the chain and four more prepare what it takes: P^T dO of the chunk
+// to come, d dO and Q^T (d dO), and they store D.
 template <typename IT, int DK, int NV>
-__global__ void __launch_bounds__(kDT, DK * sizeof(IT) * NV <= 256 ? 2 : 1) k_delta_bwd(const DeltaParams p) {
+__global__ void __launch_bounds__(2 * kDT) k_delta_bwd(const DeltaParams p) {
   constexpr int NK = DParts<IT>::in, NM = DParts<IT>::mid, KS = DK / 32, RT = DK / 64;
   __shared__ __align__(16) VTile<NM, DK> Dt[NV];
-  __shared__ __align__(16) VTile<NK, kC> Ot[NV];              // dO
+  __shared__ __align__(16) VTile<NK, kC> Ot[NV];                  // dO
   __shared__ __align__(16) VTile<NM, kC> Et[NV], Xt[NV], Yt[NV];  // d dO, dU, -beta a dR
-  const int lane = threadIdx.x % 64, w = wave_id(), r16 = lane % 16, kg = lane / 16;
+  __shared__ __align__(16) f4 Gt[NV][kDT], Rt[NV][RT][kDT], Zt[NV][kDT];  // P^T dO, Q^T (d dO), dR, by lane
+  const int lane = threadIdx.x % 64, w = wave_id() % 4, r16 = lane % 16, kg = lane / 16, me = threadIdx.x % kDT;
   int bh, vt;
   delta_tile((p.VT + NV - 1) / NV, (int)p.B * p.H, bh, vt);
   vt *= NV;
   const int b = bh / p.H, h = bh % p.H, hk = h / (p.H / p.Hk), v0 = 16 * vt + 4 * kg, have = p.Dv - v0;
   const int tok = 16 * w + r16;
-  const IT *dop = (const IT *)p.dout.p + b * p.dout.s0 + h * p.dout.s2 + v0;
-  IT *dvp = (IT *)p.dv.p + b * p.dv.s0 + h * p.dv.s2 + v0;
-  const int64_t ch0 = (int64_t)bh * p.NC, kch0 = ((int64_t)b * p.Hk + hk) * p.NC;
-
-  f4 D[NV][RT];  // D[key][v0 + 16 n + i] of key 16 (RT w + r) + r16
-#pragma unroll
-  for (int n = 0; n < NV; ++n)
-#pragma unroll
-    for (int r = 0; r < RT; ++r) {
-      const int key = 16 * (RT * w + r) + r16;
-#pragma unroll
-      for (int i = 0; i < 4; ++i)
-        D[n][r][i] = p.dlast && key < p.Dk && 16 * n + i < have ? p.dlast[((int64_t)bh * p.Dk + key) * p.Dv + v0 + 16 * n + i] : 0.0f;
-    }
-  bf8 K[KS][NK], T[2][NM], P[2][NM], Kt[RT][2][NK], Qt[RT][2][NK];
-  Raw4<IT> go[NV];
-  f4 row;  // a, beta, c, d of the token
-  float eC;
-  auto load_rows = [&](int c) {
-    row = token_row(delta_rows(p, ch0 + c), tok);
-    eC = chunk_decay(delta_rows(p, ch0 + c));
-  };
-  auto load_o = [&](int c) {
-    const int64_t t = (int64_t)c * kC + tok;
-#pragma unroll
-    for (int n = 0; n < NV; ++n)
-      go[n] = load4(dop + t * p.dout.s1 + 16 * n, (const IT *)p.dout.p, t < p.L ? have - 16 * n : 0, p.vdo);
-  };
-  auto load_kp = [&](int c) {  // the transposes of T and P are upper triangular
-    const __bf16 *k = key_frags<DK, NK>(p.fK, kch0 + c);
-#pragma unroll
-    for (int s = 0; s < KS; ++s) load_frag<NK>(k, kC * DK, w * KS + s, lane, K[s]);
-#pragma unroll
-    for (int s = 0; s < 2; ++s)
-      if (s >= w / 2) load_frag<NM>((const __bf16 *)p.fP + (ch0 + c) * NM * kFrag, kFrag, 2 * w + s, lane, P[s]);
-  };
-  auto load_t = [&](int c) {
-#pragma unroll
-    for (int s = 0; s < 2; ++s)
-      if (s >= w / 2) load_frag<NM>((const __bf16 *)p.fT + (ch0 + c) * NM * kFrag, kFrag, 2 * w + s, lane, T[s]);
-  };
+  auto at = [&](int c) { return (int64_t)c * p.B * p.H + bh; };
+  auto kat = [&](int c) { return ((int64_t)c * p.B + b) * p.Hk + hk; };
   auto load_cols = [&](const void *m, int c, bf8 (&f)[RT][2][NK]) {
-    const __bf16 *kt = key_frags<DK, NK>(m, kch0 + c);
 #pragma unroll
     for (int s = 0; s < 2; ++s)
 #pragma unroll
-      for (int r = 0; r < RT; ++r) load_frag<NK>(kt, kC * DK, 2 * (RT * w + r) + s, lane, f[r][s]);
+      for (int r = 0; r < RT; ++r) load_frag<NK>(key_frags<DK, NK>(m, kat(c)), kC * DK, 2 * (RT * w + r) + s, lane, f[r][s]);
   };
-  load_rows(p.NC - 1);
-  load_o(p.NC - 1);
-  load_kp(p.NC - 1);
-  load_t(p.NC - 1);
-  load_cols(p.fQt, p.NC - 1, Qt);
-  load_cols(p.fKt, p.NC - 1, Kt);
-  for (int c = p.NC - 1; c >= 0; --c) {
-    const int64_t t = (int64_t)c * kC + tok, ch = ch0 + c;
-    const int next = c ? c - 1 : 0;
-#pragma unroll
-    for (int n = 0; n < NV; ++n) {
-#pragma unroll
-      for (int r = 0; r < RT; ++r) {
-        const int key = 16 * (RT * w + r) + r16;
-        Dt[n].put(key, kg, D[n][r]);
-        if (key < p.Dkp && vt + n < p.VT)
-          *(f4 *)(state_of(p.dstates, p, ch, vt + n) + (unsigned)(16 * key + 4 * kg)) = D[n][r];
-      }
-      bf4 o[NK];
-      const bool live = t < p.L && have - 16 * n > 0;
-      to_parts<IT, NK>(go[n], live, o);
-      Ot[n].put_parts(tok, kg, o);
-      Et[n].put(tok, kg, row[3] * to_f4<IT>(go[n], live));
-    }
-    const float cc = row[2], bu = row[1], by = -row[1] * row[0], decay = eC;
-    load_rows(next);
-    load_o(next);
-    lds_barrier();
-    f4 x[NV];
-#pragma unroll
-    for (int n = 0; n < NV; ++n) x[n] = 0;
-#pragma unroll
-    for (int s = 0; s < KS; ++s)
-#pragma unroll
-      for (int n = 0; n < NV; ++n) {
-        bf8 A[NM];
-        Dt[n].get(s, lane, A);
-        x[n] = mma<NM>(A, K[s], x[n]);
-      }
-#pragma unroll
-    for (int n = 0; n < NV; ++n) x[n] *= cc;
-#pragma unroll
-    for (int s = 0; s < 2; ++s)
-      if (s >= w / 2) {
-#pragma unroll
-        for (int n = 0; n < NV; ++n) {
-          bf8 A[NK];
-          Ot[n].get(s, lane, A);
-          x[n] = mma<NM>(A, P[s], x[n]);
-        }
-      }
-#pragma unroll
-    for (int n = 0; n < NV; ++n) Xt[n].put(tok, kg, x[n]);
-    load_kp(next);
-    lds_barrier();
-#pragma unroll
-    for (int s = 0; s < 2; ++s)  // dR = dU + (T^T - I) dU
-      if (s >= w / 2) {
-#pragma unroll
-        for (int n = 0; n < NV; ++n) {
-          bf8 A[NM];
-          Xt[n].get(s, lane, A);
-          x[n] = mma<NM>(A, T[s], x[n]);
-        }
-      }
-#pragma unroll
-    for (int n = 0; n < NV; ++n) {
-      Yt[n].put(tok, kg, by * x[n]);
-      if (vt + n < p.VT) *(f4 *)(value_of(p.dr, p, ch, vt + n) + (unsigned)(16 * tok + 4 * kg)) = x[n];
-      store4(dvp + t * p.dv.s1 + 16 * n, (f4)(bu * x[n]), t < p.L ? have - 16 * n : 0, p.vdv);
-#pragma unroll
-      for (int r = 0; r < RT; ++r) D[n][r] *= decay;
-    }
-    load_t(next);
-#pragma unroll
-    for (int s = 0; s < 2; ++s)
-#pragma unroll
-      for (int n = 0; n < NV; ++n) {
-        bf8 A[NM];
-        Et[n].get(s, lane, A);
-#pragma unroll
-        for (int r = 0; r < RT; ++r) D[n][r] = mma<NM>(A, Qt[r][s], D[n][r]);
-      }
-    load_cols(p.fQt, next, Qt);
-    lds_barrier();
-#pragma unroll
-    for (int s = 0; s < 2; ++s)
-#pragma unroll
-      for (int n = 0; n < NV; ++n) {
-        bf8 A[NM];
-        Yt[n].get(s, lane, A);
-#pragma unroll
-        for (int r = 0; r < RT; ++r) D[n][r] = mma<NM>(A, Kt[r][s], D[n][r]);
-      }
-    load_cols(p.fKt, next, Kt);
-  }
-  if (p.dh0) {
+
+  if (wave_id() < 4) {
+    f4 D[NV][RT];  // D[key][v0 + 16 n + i] of key 16 (RT w + r) + r16
 #pragma unroll
     for (int n = 0; n < NV; ++n)
 #pragma unroll
@@ -184,8 +53,202 @@ __global__ void __launch_bounds__(kDT, DK * sizeof(IT) * NV <= 256 ? 2 : 1) k_de
         const int key = 16 * (RT * w + r) + r16;
 #pragma unroll
         for (int i = 0; i < 4; ++i)
-          if (key < p.Dk && 16 * n + i < have) p.dh0[((int64_t)bh * p.Dk + key) * p.Dv + v0 + 16 * n + i] = D[n][r][i];
+          D[n][r][i] = p.dlast && key < p.Dk && 16 * n + i < have ? p.dlast[((int64_t)bh * p.Dk + key) * p.Dv + v0 + 16 * n + i] : 0.0f;
       }
+    bf8 K[KS][NK], T[2][NM], Kt[RT][2][NK];
+    f4 row;  // a, beta, c, d of the token
+    float eC;
+    auto load_k = [&](int c) {
+#pragma unroll
+      for (int s = 0; s < KS; ++s) load_frag<NK>(key_frags<DK, NK>(p.fK, kat(c)), kC * DK, w * KS + s, lane, K[s]);
+      row = token_row(delta_rows(p, at(c)), tok);
+      eC = chunk_decay(delta_rows(p, at(c)));
+    };
+    auto load_t = [&](int c) {  // the transpose of T is upper triangular
+#pragma unroll
+      for (int s = 0; s < 2; ++s)
+        if (s >= w / 2) load_frag<NM>((const __bf16 *)p.fT + at(c) * NM * kFrag, kFrag, 2 * w + s, lane, T[s]);
+    };
+    load_k(p.NC - 1);
+    load_t(p.NC - 1);
+    load_cols(p.fKt, p.NC - 1, Kt);
+    lds_barrier();  // the first chunk's dO
+    for (int c = p.NC - 1; c >= 0; --c) {
+      const int64_t t = (int64_t)c * kC + tok;
+      const int next = c ? c - 1 : 0;
+#pragma unroll
+      for (int n = 0; n < NV; ++n)
+#pragma unroll
+        for (int r = 0; r < RT; ++r) Dt[n].put(16 * (RT * w + r) + r16, kg, D[n][r]);
+      lds_barrier();
+      f4 x[NV];
+#pragma unroll
+      for (int n = 0; n < NV; ++n) x[n] = 0;
+#pragma unroll
+      for (int s = 0; s < KS; ++s)
+#pragma unroll
+        for (int n = 0; n < NV; ++n) {
+          bf8 A[NM];
+          Dt[n].get(s, lane, A);
+          x[n] = mma<NM>(A, K[s], x[n]);
+        }
+#pragma unroll
+      for (int n = 0; n < NV; ++n) {
+        x[n] = row[2] * x[n] + Gt[n][me];
+        Xt[n].put(tok, kg, x[n]);
+      }
+      const float by = -row[1] * row[0], decay = eC;
+      load_k(next);
+      lds_barrier();
+#pragma unroll
+      for (int s = 0; s < 2; ++s)  // dR = dU + (T^T - I) dU
+        if (s >= w / 2) {
+#pragma unroll
+          for (int n = 0; n < NV; ++n) {
+            bf8 A[NM];
+            Xt[n].get(s, lane, A);
+            x[n] = mma<NM>(A, T[s], x[n]);
+          }
+        }
+#pragma unroll
+      for (int n = 0; n < NV; ++n) {
+        Yt[n].put(tok, kg, by * x[n]);
+        Zt[n][me] = x[n];
+      }
+      load_t(next);
+      lds_barrier();
+#pragma unroll
+      for (int n = 0; n < NV; ++n)
+#pragma unroll
+        for (int r = 0; r < RT; ++r) D[n][r] = decay * D[n][r] + Rt[n][r][me];
+#pragma unroll
+      for (int s = 0; s < 2; ++s)
+#pragma unroll
+        for (int n = 0; n < NV; ++n) {
+          bf8 A[NM];
+          Yt[n].get(s, lane, A);
+#pragma unroll
+          for (int r = 0; r < RT; ++r) D[n][r] = mma<NM>(A, Kt[r][s], D[n][r]);
+        }
+      load_cols(p.fKt, next, Kt);
+    }
+    if (p.dh0) {
+#pragma unroll
+      for (int n = 0; n < NV; ++n)
+#pragma unroll
+        for (int r = 0; r < RT; ++r) {
+          const int key = 16 * (RT * w + r) + r16;
+#pragma unroll
+          for (int i = 0; i < 4; ++i)
+            if (key < p.Dk && 16 * n + i < have) p.dh0[((int64_t)bh * p.Dk + key) * p.Dv + v0 + 16 * n + i] = D[n][r][i];
+        }
+    }
+  } else {
+    const IT *dop = (const IT *)p.dout.p + b * p.dout.s0 + h * p.dout.s2 + v0;
+    IT *dvp = (IT *)p.dv.p + b * p.dv.s0 + h * p.dv.s2 + v0;
+    bf8 P[2][NM], Qt[RT][2][NK];
+    Raw4<IT> go[NV], next_go[NV];  // dO of this chunk and of the one to come
+    auto load_o = [&](int c, Raw4<IT> (&g)[NV]) {
+      const int64_t t = (int64_t)c * kC + tok;
+#pragma unroll
+      for (int n = 0; n < NV; ++n)
+        g[n] = load4(dop + t * p.dout.s1 + 16 * n, (const IT *)p.dout.p, t < p.L ? have - 16 * n : 0, p.vdo);
+    };
+    auto load_p = [&](int c) {  // so is that of P
+#pragma unroll
+      for (int s = 0; s < 2; ++s)
+        if (s >= w / 2) load_frag<NM>((const __bf16 *)p.fP + at(c) * NM * kFrag, kFrag, 2 * w + s, lane, P[s]);
+    };
+    auto put_o = [&](int c, Raw4<IT> (&g)[NV]) {
+      const int64_t t = (int64_t)c * kC + tok;
+#pragma unroll
+      for (int n = 0; n < NV; ++n) {
+        bf4 o[NK];
+        to_parts<IT, NK>(g[n], t < p.L && have - 16 * n > 0, o);
+        Ot[n].put_parts(tok, kg, o);
+      }
+    };
+    auto make_g = [&] {
+      f4 g[NV];
+#pragma unroll
+      for (int n = 0; n < NV; ++n) g[n] = 0;
+#pragma unroll
+      for (int s = 0; s < 2; ++s)
+        if (s >= w / 2) {
+#pragma unroll
+          for (int n = 0; n < NV; ++n) {
+            bf8 A[NK];
+            Ot[n].get(s, lane, A);
+            g[n] = mma<NM>(A, P[s], g[n]);
+          }
+        }
+#pragma unroll
+      for (int n = 0; n < NV; ++n) Gt[n][me] = g[n];
+    };
+    load_o(p.NC - 1, go);
+    load_p(p.NC - 1);
+    load_cols(p.fQt, p.NC - 1, Qt);
+    f4 row = token_row(delta_rows(p, at(p.NC - 1)), tok);  // a, beta, c, d of the token
+    put_o(p.NC - 1, go);
+    load_o(p.NC > 1 ? p.NC - 2 : 0, next_go);
+    lds_barrier();
+    make_g();
+    load_p(p.NC > 1 ? p.NC - 2 : 0);
+    for (int c = p.NC - 1; c >= 0; --c) {
+      const int64_t t = (int64_t)c * kC + tok;
+      const int next = c ? c - 1 : 0, after = c > 1 ? c - 2 : 0;
+      const float be = row[1], fd = row[3];
+      lds_barrier();
+#pragma unroll
+      for (int n = 0; n < NV; ++n) Et[n].put(tok, kg, fd * to_f4<IT>(go[n], t < p.L && have - 16 * n > 0));
+      put_o(next, next_go);
+#pragma unroll
+      for (int n = 0; n < NV; ++n) go[n] = next_go[n];
+      load_o(after, next_go);
+      row = token_row(delta_rows(p, at(next)), tok);
+      f4 D[NV][RT];
+#pragma unroll
+      for (int n = 0; n < NV; ++n)
+#pragma unroll
+        for (int r = 0; r < RT; ++r) D[n][r] = Dt[n].whole(16 * (RT * w + r) + r16, kg);
+      lds_barrier();
+      f4 R[NV][RT];
+#pragma unroll
+      for (int n = 0; n < NV; ++n)
+#pragma unroll
+        for (int r = 0; r < RT; ++r) R[n][r] = 0;
+#pragma unroll
+      for (int s = 0; s < 2; ++s)
+#pragma unroll
+        for (int n = 0; n < NV; ++n) {
+          bf8 A[NM];
+          Et[n].get(s, lane, A);
+#pragma unroll
+          for (int r = 0; r < RT; ++r) R[n][r] = mma<NM>(A, Qt[r][s], R[n][r]);
+        }
+#pragma unroll
+      for (int n = 0; n < NV; ++n)
+#pragma unroll
+        for (int r = 0; r < RT; ++r) Rt[n][r][me] = R[n][r];
+      make_g();
+      load_cols(p.fQt, next, Qt);
+      load_p(after);
+      lds_barrier();
+      // no store stands before a barrier that the chain has to wait at
+#pragma unroll
+      for (int n = 0; n < NV; ++n) {
+        const f4 x = Zt[n][me];
+        if (vt + n < p.VT) {
+          *(f4 *)(value_of(p.dr, p, at(c), vt + n) + (unsigned)(16 * tok + 4 * kg)) = x;
+#pragma unroll
+          for (int r = 0; r < RT; ++r) {
+            const int key = 16 * (RT * w + r) + r16;
+            if (key < p.Dkp) *(f4 *)(state_of(p.dstates, p, at(c), vt + n) + (unsigned)(16 * key + 4 * kg)) = D[n][r];
+          }
+        }
+        store4(dvp + t * p.dv.s1 + 16 * n, (f4)(be * x), t < p.L ? have - 16 * n : 0, p.vdv);
+      }
+    }
   }
 }
 
@@ -194,7 +257,7 @@ __global__ void __launch_bounds__(kDT, DK * sizeof(IT) * NV <= 256 ? 2 : 1) k_de
 // the states go from memory to registers, both one slab ahead; what the products of the chunk's end want is
 // read during the last slab.  SHARED: several value heads add to dq', dk', which wait in LDS meanwhile.
 template <typename IT, int DK, bool SHARED>
-__global__ void __launch_bounds__(4 * DK) k_delta_grad(const DeltaParams p) {
+__global__ void __launch_bounds__(4 * DK, 2) k_delta_grad(const DeltaParams p) {
   constexpr int NK = DParts<IT>::in, NM = DParts<IT>::mid, NP = DParts<IT>::out, NT = 4 * DK, NW = DK / 16;
   constexpr int NJ = 16 / NW;                    // tiles of J and H per wavefront
   constexpr int SF = 4 * 64 * 8;                 // staged elements of one part: 64 tokens x 32 columns
@@ -204,8 +267,8 @@ __global__ void __launch_bounds__(4 * DK) k_delta_grad(const DeltaParams p) {
   __shared__ __align__(16) float rows[kDeltaRows];
   __shared__ float red[NW][kC], norm[NW][2][kC], rowb[kC], rowv[kC], sdot[NW], cdot[NW];
   const int tid = threadIdx.x, lane = tid % 64, w = wave_id(), r16 = lane % 16, kg = lane / 16;
-  const int c = blockIdx.x % p.NC, bk = blockIdx.x / p.NC, b = bk / p.Hk, hk = bk % p.Hk, group = SHARED ? p.H / p.Hk : 1;
-  const int64_t t0 = (int64_t)c * kC, kch = (int64_t)bk * p.NC + c;
+  const int keyed = (int)p.B * p.Hk, c = blockIdx.x / keyed, bk = blockIdx.x % keyed, b = bk / p.Hk, hk = bk % p.Hk, group = SHARED ? p.H / p.Hk : 1;
+  const int64_t t0 = (int64_t)c * kC, kch = blockIdx.x;
   const int wi = w * NJ / 4, wj = w * NJ % 4;    // J's tiles (wi, wj .. wj + NJ - 1)
   const bool keys = 16 * w < p.Dkp;
   const int slabs = (p.VT + 1) / 2;
@@ -215,23 +278,17 @@ __global__ void __launch_bounds__(4 * DK) k_delta_grad(const DeltaParams p) {
 
   bf8 Kt[2][NK], Qt[2][NK];  // K and Q by columns: keys 16 w + r16
   bf4 Ke[4][NK], Qe[4][NK];  // K and Q of token 16 it + r16, keys 16 w + 4 kg + i
-  auto load_keys = [&] {
-    const __bf16 *kt = key_frags<DK, NK>(p.fKt, kch), *qt = key_frags<DK, NK>(p.fQt, kch);
-    const __bf16 *k = key_frags<DK, NK>(p.fK, kch), *q = key_frags<DK, NK>(p.fQ, kch);
-    asm volatile("" : "+s"(kt), "+s"(qt), "+s"(k), "+s"(q));  // read for every head anew: kept over its slabs, they would spill
+  const __bf16 *kt = key_frags<DK, NK>(p.fKt, kch), *qt = key_frags<DK, NK>(p.fQt, kch);
+  const __bf16 *kr = key_frags<DK, NK>(p.fK, kch), *qr = key_frags<DK, NK>(p.fQ, kch);
+  auto load_keys = [&](int it) {
+    asm volatile("" : "+s"(kt), "+s"(qt), "+s"(kr), "+s"(qr));  // read for every head anew: kept over its slabs, they would spill
 #pragma unroll
-    for (int it = 0; it < 4; ++it)
-#pragma unroll
-      for (int n = 0; n < NK; ++n) {
-        const int at = n * kC * DK + (it * (DK / 32) + w / 2) * 512 + 4 * (w % 2);
-        Ke[it][n] = *(const bf4 *)(k + at + (unsigned)(lane * 8));
-        Qe[it][n] = *(const bf4 *)(q + at + (unsigned)(lane * 8));
-      }
-#pragma unroll
-    for (int s = 0; s < 2; ++s) {
-      load_frag<NK>(kt, kC * DK, 2 * w + s, lane, Kt[s]);
-      load_frag<NK>(qt, kC * DK, 2 * w + s, lane, Qt[s]);
+    for (int n = 0; n < NK; ++n) {
+      const int at = n * kC * DK + (it * (DK / 32) + w / 2) * 512 + 4 * (w % 2);
+      Ke[it][n] = *(const bf4 *)(kr + at + (unsigned)(lane * 8));
+      Qe[it][n] = *(const bf4 *)(qr + at + (unsigned)(lane * 8));
     }
+    load_frag<NK>(it < 2 ? kt : qt, kC * DK, 2 * w + it % 2, lane, it < 2 ? Kt[it % 2] : Qt[it % 2]);
   };
   auto whole = [](const bf4 (&x)[NK]) {
     f4 r = __builtin_convertvector(x[NK - 1], f4);
@@ -243,10 +300,10 @@ __global__ void __launch_bounds__(4 * DK) k_delta_grad(const DeltaParams p) {
   f4 Y[4], Z[4];  // dq', dk' of token 16 it + r16, keys 16 w + 4 kg + i
   for (int hg = 0; hg < group; ++hg) {
     const int h = hk * group + hg;
-    const int64_t ch = ((int64_t)b * p.H + h) * p.NC + c;
+    const int64_t ch = ((int64_t)c * p.B + b) * p.H + h;
     const IT *dop = (const IT *)p.dout.p + b * p.dout.s0 + h * p.dout.s2 + t0 * p.dout.s1;
     const IT *vp = (const IT *)p.v.p + b * p.v.s0 + h * p.v.s2 + t0 * p.v.s1;
-    const float *Sp = state_of(p.states, p, ch, 0) + 256 * w, *Dp = state_of(p.dstates, p, ch, 0) + 256 * w;
+    const float *Sp = state_of(p.states, p, ch, 0) + (keys ? 256 * w : 0), *Dp = state_of(p.dstates, p, ch, 0) + (keys ? 256 * w : 0);
     const float *yp = value_of(p.y, p, ch, 0), *xp = value_of(p.dr, p, ch, 0);
     f4 F1[4], F2[4], F3[4], A[NJ], N[NJ];  // S0 dO^T, D U^T, S0 dR^T; tiles of dO U^T, dR U^T, transposed
 #pragma unroll
@@ -257,22 +314,25 @@ __global__ void __launch_bounds__(4 * DK) k_delta_grad(const DeltaParams p) {
     f4 sv[2], dv[2], yv[PT], xv[PT];
     Raw4<IT> go[PT], vv[PT];
     // staged piece x of this wavefront: half (w + x NW) / 4 of the slab, tokens 16 (w + x NW) % 4 + r16, columns 4 kg + i
-    auto load = [&](int s) {
+    auto load_values = [&](int s) {
+#pragma unroll
+      for (int x = 0; x < PT; ++x) {
+        const int vt = 2 * s + (w + x * NW) / 4, it = (w + x * NW) % 4, at = (vt < p.VT ? vt : 0) * (kC * 16) + 256 * it;
+        yv[x] = *(const f4 *)(yp + at + at16);
+        xv[x] = *(const f4 *)(xp + at + at16);
+      }
+    };
+    auto load_inputs = [&](int s) {
 #pragma unroll
       for (int x = 0; x < PT; ++x) {
         const int vt = 2 * s + (w + x * NW) / 4, it = (w + x * NW) % 4, have = t0 + 16 * it + r16 < p.L ? p.Dv - 16 * vt - 4 * kg : 0;
-        const int vc = vt < p.VT ? vt : 0;
-        yv[x] = *(const f4 *)(yp + vc * (kC * 16) + 256 * it + at16);
-        xv[x] = *(const f4 *)(xp + vc * (kC * 16) + 256 * it + at16);
         go[x] = load4(dop + 16 * it * p.dout.s1 + 16 * vt + ao, (const IT *)p.dout.p, have, p.vdo);
         vv[x] = load4(vp + 16 * it * p.v.s1 + 16 * vt + av, (const IT *)p.v.p, have, p.vv);
       }
+    };
+    auto load_states = [&](int s, const float *m, f4 (&v)[2]) {
 #pragma unroll
-      for (int x = 0; x < 2; ++x) {
-        const int64_t vc = (keys && 2 * s + x < p.VT ? 2 * s + x : 0) * (int64_t)(p.Dkp * 16) - (keys ? 0 : 256 * w);
-        sv[x] = *(const f4 *)(Sp + vc + at16);
-        dv[x] = *(const f4 *)(Dp + vc + at16);
-      }
+      for (int x = 0; x < 2; ++x) v[x] = *(const f4 *)(m + (2 * s + x < p.VT ? 2 * s + x : 0) * (int64_t)(p.Dkp * 16) + at16);
     };
     bf8 SA[NM], DA[NM];
     auto stage = [&](int s) {
@@ -299,6 +359,8 @@ __global__ void __launch_bounds__(4 * DK) k_delta_grad(const DeltaParams p) {
 #pragma unroll
         for (int n = 0; n < NP; ++n) *(bf4 *)(Rs + n * SF + at) = r[n];
       }
+    };
+    auto split_states = [&](int s) {
       f8 x = __builtin_shufflevector(sv[0], sv[1], 0, 1, 2, 3, 4, 5, 6, 7);
       f8 y = __builtin_shufflevector(dv[0], dv[1], 0, 1, 2, 3, 4, 5, 6, 7);
       if (!keys || 2 * s + 1 >= p.VT) {
@@ -311,7 +373,9 @@ __global__ void __launch_bounds__(4 * DK) k_delta_grad(const DeltaParams p) {
       split_parts<NM>(x, SA);
       split_parts<NM>(y, DA);
     };
-    auto multiply = [&](int s) {
+    // The slab's products; after those of token tile `it` comes read(it), so that the reads' issue (16 cycles of
+    // the compute unit's address unit each) falls into the time of the products.
+    auto multiply = [&](int s, auto read) {
       const __bf16 *const Os = buf + (s & 1) * kStage, *const Us = Os + NK * SF, *const Rs = Us + NM * SF;
 #pragma unroll
       for (int it = 0; it < 4; ++it) {
@@ -332,6 +396,7 @@ __global__ void __launch_bounds__(4 * DK) k_delta_grad(const DeltaParams p) {
               N[j] = mma<NP>(Uj, R, N[j]);
             }
         }
+        read(it);
         __builtin_amdgcn_sched_barrier(0);  // one token tile's operands in registers at a time
       }
     };
@@ -340,7 +405,10 @@ __global__ void __launch_bounds__(4 * DK) k_delta_grad(const DeltaParams p) {
       float x[(kDeltaRows + NT - 1) / NT];
 #pragma unroll
       for (int i = 0; i < (kDeltaRows + NT - 1) / NT; ++i) x[i] = m[tid + i * NT < kDeltaRows ? tid + i * NT : 0];
-      load(0);
+      load_values(0);
+      load_inputs(0);
+      load_states(0, Sp, sv);
+      load_states(0, Dp, dv);
 #pragma unroll
       for (int i = 0; i < (kDeltaRows + NT - 1) / NT; ++i)
         if (tid + i * NT < kDeltaRows) rows[tid + i * NT] = x[i];
@@ -350,14 +418,19 @@ __global__ void __launch_bounds__(4 * DK) k_delta_grad(const DeltaParams p) {
     lds_barrier();
     for (int s = 0; s + 1 < slabs; ++s) {
       stage(s);
-      load(s + 1);
       lds_barrier();  // the other buffer's readers are a barrier behind
-      multiply(s);
+      split_states(s);
+      multiply(s, [&](int it) {
+        if (it == 0) load_values(s + 1);
+        else if (it == 1) load_inputs(s + 1);
+        else if (it == 2) load_states(s + 1, Sp, sv);
+        else load_states(s + 1, Dp, dv);
+      });
     }
     stage(slabs - 1);
-    load_keys();
     lds_barrier();
-    multiply(slabs - 1);
+    split_states(slabs - 1);
+    multiply(slabs - 1, load_keys);
 
     sd = group_sum<64>(sd);
     if (lane == 0) sdot[w] = sd;
@@ -518,9 +591,9 @@ __global__ void __launch_bounds__(4 * DK) k_delta_grad(const DeltaParams p) {
 template <typename IT, int DK>
 static hipError_t delta_bwd(const DeltaParams &p, hipStream_t s) {
   if (delta_pairs(p))
-    hipLaunchKernelGGL((k_delta_bwd<IT, DK, 2>), dim3((unsigned)(p.B * p.H) * (unsigned)((p.VT + 1) / 2)), dim3(kDT), 0, s, p);
+    hipLaunchKernelGGL((k_delta_bwd<IT, DK, 2>), dim3((unsigned)(p.B * p.H) * (unsigned)((p.VT + 1) / 2)), dim3(2 * kDT), 0, s, p);
   else
-    hipLaunchKernelGGL((k_delta_bwd<IT, DK, 1>), dim3((unsigned)(p.B * p.H) * (unsigned)p.VT), dim3(kDT), 0, s, p);
+    hipLaunchKernelGGL((k_delta_bwd<IT, DK, 1>), dim3((unsigned)(p.B * p.H) * (unsigned)p.VT), dim3(2 * kDT), 0, s, p);
   const dim3 grid((unsigned)(p.B * p.Hk) * (unsigned)p.NC);
   if (p.H > p.Hk) hipLaunchKernelGGL((k_delta_grad<IT, DK, true>), grid, dim3(4 * DK), 0, s, p);
   else hipLaunchKernelGGL((k_delta_grad<IT, DK, false>), grid, dim3(4 * DK), 0, s, p);

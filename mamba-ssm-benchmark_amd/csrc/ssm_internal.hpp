@@ -307,8 +307,8 @@ struct DeltaParams {
   const float *h0;                     // (B, H, Dk, Dv) or null
   float *last;
   void *fT, *fP, *fK, *fQ, *fKt, *fQt; // operand fragments (fQt: backward only)
-  float *rows;                         // (B H, NC, kDeltaRows)
-  float *states, *y;                   // saved: (B H, NC, VT, Dkp, 16) entering states, (B H, NC, VT, 64, 16) Y
+  float *rows;                         // (NC, B H, kDeltaRows)
+  float *states, *y;                   // saved: (NC, B H, VT, Dkp, 16) entering states, (NC, B H, VT, 64, 16) Y
   KView dout, dq, dk, dv, dg, dbeta;
   const float *dlast;
   float *dh0, *dstates, *dr;           // gradients of the leaving states and dR, laid out as states and y
