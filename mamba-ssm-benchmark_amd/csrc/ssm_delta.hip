@@ -169,12 +169,12 @@ __global__ void __launch_bounds__(kDT, 4 - DParts<IT>::in) k_delta_prep(const De
   if (tid < kC) {
     float *rows = p.rows + ch * kDeltaRows;
     const float gh = Gh[tid], gl = Gl[tid], eG = fexp(gh);
-    *(f4 *)(rows + 4 * tid) = f4{fk[tid] * eG, bs[tid], fk[tid] * fexp((Gh[kC - 1] - gh) + (Gl[kC - 1] - gl)), fq[tid] * eG};
+    *(f4 *)(rows + 4 * tid) = f4{fk[tid] * eG, bs[tid], fk[tid] * fexp((Gh[kC - 1] - gh) + (Gl[kC - 1] - gl)), fexp(Gh[kC - 1])};
     rows[4 * kC + tid] = fk[tid];
     rows[5 * kC + tid] = fq[tid];
     rows[6 * kC + tid] = gh;
     rows[7 * kC + tid] = gl;
-    if (tid == kC - 1) rows[8 * kC] = eG;
+    rows[8 * kC + tid] = fq[tid] * eG;
   }
   wave_lds_sync();  // the diagonal block is this wavefront's own
   {
@@ -238,7 +238,7 @@ __global__ void __launch_bounds__(kDT, 4 - DParts<IT>::in) k_delta_prep(const De
 // just used.  All products are of transposes: rows are 16 columns of v, so a lane holds 4 columns of
 // one token or key, and moves them as one word.  A workgroup walks NV tiles of 16 columns.
 template <typename IT, int DK, int NV>
-__global__ void __launch_bounds__(2 * kDT) k_delta_fwd(const DeltaParams p) {
+__global__ void __launch_bounds__(2 * kDT) SSM_TWO_WAVES k_delta_fwd(const DeltaParams p) {
   constexpr int NK = DParts<IT>::in, NM = DParts<IT>::mid, NP = DParts<IT>::out, KS = DK / 32, RT = DK / 64;
   __shared__ __align__(16) VTile<NM, DK> St[NV];
   __shared__ __align__(16) VTile<NM, kC> Xt[NV], Wt[NV];  // X, c U
@@ -266,14 +266,12 @@ __global__ void __launch_bounds__(2 * kDT) k_delta_fwd(const DeltaParams p) {
       }
     bf8 K[KS][NK], T[2][NM], Kt[RT][2][NK];
     Raw4<IT> v[NV];
-    f4 row;  // a, beta, c, d of the token
-    float eC;
+    f4 row;  // a, beta, c of the token, e^{G_C}
     auto load_v = [&](int c) {
       const int64_t t = (int64_t)c * kC + tok;
 #pragma unroll
       for (int n = 0; n < NV; ++n) v[n] = load4(vp + t * p.v.s1 + 16 * n, (const IT *)p.v.p, t < p.L ? have - 16 * n : 0, p.vv);
       row = token_row(delta_rows(p, at(c)), tok);
-      eC = chunk_decay(delta_rows(p, at(c)));
     };
     auto load_k = [&](int c) {
 #pragma unroll
@@ -318,7 +316,7 @@ __global__ void __launch_bounds__(2 * kDT) k_delta_fwd(const DeltaParams p) {
         y[n] = to_f4<IT>(v[n], t < p.L && have - 16 * n > 0) - row[0] * x[n];
         Xt[n].put(tok, kg, y[n]);
       }
-      const float bu = row[1], bc = row[1] * row[2], decay = eC;
+      const float bu = row[1], bc = row[1] * row[2], decay = row[3];
       load_k(next);
       load_v(next);
       lds_barrier();
@@ -377,7 +375,7 @@ __global__ void __launch_bounds__(2 * kDT) k_delta_fwd(const DeltaParams p) {
     auto load_q = [&](int c) {
 #pragma unroll
       for (int s = 0; s < KS; ++s) load_frag<NK>(key_frags<DK, NK>(p.fQ, kat(c)), kC * DK, w * KS + s, lane, Q[s]);
-      fd = delta_rows(p, at(c))[(unsigned)(4 * tok + 3)];
+      fd = delta_rows(p, at(c))[8 * kC + (unsigned)tok];
     };
     auto load_p = [&](int c) {
 #pragma unroll

@@ -39,6 +39,9 @@ typedef short s4 __attribute__((ext_vector_type(4)));
 
 constexpr int kC = kDeltaChunk;   // tokens per chunk
 constexpr int kDT = 256;          // four wavefronts: wavefront w owns tokens 16 w .. 16 w + 15
+// The walks and the gradient kernel have one workgroup's two wavefronts on a SIMD: the scheduler may use the
+// registers that more would need.
+#define SSM_TWO_WAVES __attribute__((amdgpu_waves_per_eu(2, 2)))
 constexpr int kFrag = kC * kC;    // elements of one part of a 64 x 64 matrix stored as operand fragments
 
 // Parts of an input of type IT, of float32 intermediates beside it, and of those that only reach outputs of type IT.
@@ -215,13 +218,10 @@ __device__ __forceinline__ void delta_tile(int nv, int heads, int &bh, int &vt) 
 }
 
 // Row factors of a chunk, kDeltaRows floats: per token a = |k|^-1 e^G, beta, c = |k|^-1 e^{G_C - G} and
-// d = scale |q|^-1 e^G; then [4] |k|^-1, [5] scale |q|^-1 (the norms are 1 without qk_norm), [6] + [7] G
-// as the sum of two floats, [8] e^{G_C}, which every lane wants: read by the scalar unit.
+// e^{G_C}, which the chain takes in one read; then [4] |k|^-1, [5] scale |q|^-1 (the norms are 1 without
+// qk_norm), [6] + [7] G as the sum of two floats, [8] d = scale |q|^-1 e^G.
 __device__ __forceinline__ const float *delta_rows(const DeltaParams &p, int64_t ch) { return p.rows + ch * kDeltaRows; }
 __device__ __forceinline__ f4 token_row(const float *rows, int tok) { return *(const f4 *)(rows + (unsigned)(4 * tok)); }
-__device__ __forceinline__ float chunk_decay(const float *rows) {
-  return *(const __attribute__((address_space(4))) float *)(uintptr_t)(rows + 8 * kC);
-}
 
 // Arrays of operand fragments.  Per chunk and key head, in DParts::in parts of 64 DK: the rows of K and Q
 // (token tile w, step s of keys: fragment w DK/32 + s) and their columns (key tile t, step s of tokens:

@@ -23,7 +23,7 @@ hipError_t launch_delta_prep_t(const DeltaParams &p, int dtype, hipStream_t s);
 // As in the forward, four wavefronts walk the chain and four more prepare what it takes: P^T dO of the chunk
 // to come, d dO and Q^T (d dO), and they store D.
 template <typename IT, int DK, int NV>
-__global__ void __launch_bounds__(2 * kDT) k_delta_bwd(const DeltaParams p) {
+__global__ void __launch_bounds__(2 * kDT) SSM_TWO_WAVES k_delta_bwd(const DeltaParams p) {
   constexpr int NK = DParts<IT>::in, NM = DParts<IT>::mid, KS = DK / 32, RT = DK / 64;
   __shared__ __align__(16) VTile<NM, DK> Dt[NV];
   __shared__ __align__(16) VTile<NK, kC> Ot[NV];                  // dO
@@ -56,13 +56,11 @@ __global__ void __launch_bounds__(2 * kDT) k_delta_bwd(const DeltaParams p) {
           D[n][r][i] = p.dlast && key < p.Dk && 16 * n + i < have ? p.dlast[((int64_t)bh * p.Dk + key) * p.Dv + v0 + 16 * n + i] : 0.0f;
       }
     bf8 K[KS][NK], T[2][NM], Kt[RT][2][NK];
-    f4 row;  // a, beta, c, d of the token
-    float eC;
+    f4 row;  // a, beta, c of the token, e^{G_C}
     auto load_k = [&](int c) {
 #pragma unroll
       for (int s = 0; s < KS; ++s) load_frag<NK>(key_frags<DK, NK>(p.fK, kat(c)), kC * DK, w * KS + s, lane, K[s]);
       row = token_row(delta_rows(p, at(c)), tok);
-      eC = chunk_decay(delta_rows(p, at(c)));
     };
     auto load_t = [&](int c) {  // the transpose of T is upper triangular
 #pragma unroll
@@ -97,7 +95,7 @@ __global__ void __launch_bounds__(2 * kDT) k_delta_bwd(const DeltaParams p) {
         x[n] = row[2] * x[n] + Gt[n][me];
         Xt[n].put(tok, kg, x[n]);
       }
-      const float by = -row[1] * row[0], decay = eC;
+      const float by = -row[1] * row[0], decay = row[3];
       load_k(next);
       lds_barrier();
 #pragma unroll
@@ -188,7 +186,7 @@ __global__ void __launch_bounds__(2 * kDT) k_delta_bwd(const DeltaParams p) {
     load_o(p.NC - 1, go);
     load_p(p.NC - 1);
     load_cols(p.fQt, p.NC - 1, Qt);
-    f4 row = token_row(delta_rows(p, at(p.NC - 1)), tok);  // a, beta, c, d of the token
+    float beta = delta_rows(p, at(p.NC - 1))[(unsigned)(4 * tok + 1)], d = delta_rows(p, at(p.NC - 1))[8 * kC + (unsigned)tok];
     put_o(p.NC - 1, go);
     load_o(p.NC > 1 ? p.NC - 2 : 0, next_go);
     lds_barrier();
@@ -197,7 +195,7 @@ __global__ void __launch_bounds__(2 * kDT) k_delta_bwd(const DeltaParams p) {
     for (int c = p.NC - 1; c >= 0; --c) {
       const int64_t t = (int64_t)c * kC + tok;
       const int next = c ? c - 1 : 0, after = c > 1 ? c - 2 : 0;
-      const float be = row[1], fd = row[3];
+      const float be = beta, fd = d;
       lds_barrier();
 #pragma unroll
       for (int n = 0; n < NV; ++n) Et[n].put(tok, kg, fd * to_f4<IT>(go[n], t < p.L && have - 16 * n > 0));
@@ -205,7 +203,8 @@ __global__ void __launch_bounds__(2 * kDT) k_delta_bwd(const DeltaParams p) {
 #pragma unroll
       for (int n = 0; n < NV; ++n) go[n] = next_go[n];
       load_o(after, next_go);
-      row = token_row(delta_rows(p, at(next)), tok);
+      beta = delta_rows(p, at(next))[(unsigned)(4 * tok + 1)];
+      d = delta_rows(p, at(next))[8 * kC + (unsigned)tok];
       f4 D[NV][RT];
 #pragma unroll
       for (int n = 0; n < NV; ++n)
@@ -257,7 +256,7 @@ __global__ void __launch_bounds__(2 * kDT) k_delta_bwd(const DeltaParams p) {
 // the states go from memory to registers, both one slab ahead; what the products of the chunk's end want is
 // read during the last slab.  SHARED: several value heads add to dq', dk', which wait in LDS meanwhile.
 template <typename IT, int DK, bool SHARED>
-__global__ void __launch_bounds__(4 * DK, 2) k_delta_grad(const DeltaParams p) {
+__global__ void __launch_bounds__(4 * DK) SSM_TWO_WAVES k_delta_grad(const DeltaParams p) {
   constexpr int NK = DParts<IT>::in, NM = DParts<IT>::mid, NP = DParts<IT>::out, NT = 4 * DK, NW = DK / 16;
   constexpr int NJ = 16 / NW;                    // tiles of J and H per wavefront
   constexpr int SF = 4 * 64 * 8;                 // staged elements of one part: 64 tokens x 32 columns
@@ -476,7 +475,7 @@ __global__ void __launch_bounds__(4 * DK, 2) k_delta_grad(const DeltaParams p) {
       const f4 row = token_row(rows, 16 * it + r16), ke = whole(Ke[it]), f2 = row[2] * F2[it];
 #pragma unroll
       for (int i = 0; i < 4; ++i) cd = fmaf(ke[i], f2[i], cd);
-      Y[it] = row[3] * F1[it];
+      Y[it] = rows[8 * kC + 16 * it + r16] * F1[it];
       Z[it] = f2 - (row[1] * row[0]) * F3[it];
     }
     cd = group_sum<64>(cd);
@@ -557,7 +556,7 @@ __global__ void __launch_bounds__(4 * DK, 2) k_delta_grad(const DeltaParams p) {
         ss += sdot[k];
       }
       const double upto = wave_scan_f64(s);  // the sum from i on is the whole less what is before i
-      const double from = (__shfl(upto, 63) - upto) + s + all + (double)rows[8 * kC] * ss;
+      const double from = (__shfl(upto, 63) - upto) + s + all + (double)rows[3] * ss;
       const int64_t t = t0 + lane;
       if (t < p.L) {
         ((float *)p.dg.p)[b * p.dg.s0 + t * p.dg.s1 + h * p.dg.s2] = (float)from;

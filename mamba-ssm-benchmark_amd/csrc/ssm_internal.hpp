@@ -295,7 +295,7 @@ hipError_t launch_dec_head(const DecInParams &p, hipStream_t s);
 
 // Gated delta rule.  Tensors' last dimension has unit stride; views' strides are batch, token, head.
 constexpr int kDeltaChunk = 64;        // tokens per chunk
-constexpr int kDeltaRows = 8 * 64 + 4; // floats of row factors per chunk
+constexpr int kDeltaRows = 9 * 64;     // floats of row factors per chunk
 constexpr int kDeltaMaxK = 128;        // key width of the chunked kernels and the step
 struct DeltaParams {
   int64_t B, L;
