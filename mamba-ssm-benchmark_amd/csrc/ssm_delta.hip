@@ -132,8 +132,8 @@ __global__ void __launch_bounds__(kDT, 4 - DParts<IT>::in) k_delta_prep(const De
         for (int s = 0; s < KS; ++s) {
           bf8 A[NK];
           load_frag<NK>(&Kf[0][0], kRowsOf, x * KS + s, lane, A);
-          l = mma<NK>(A, K[s], l);
-          if (!BWD) qk = mma<NK>(A, Q[s], qk);
+          l = mma<NM>(A, K[s], l);
+          if (!BWD) qk = mma<NM>(A, Q[s], qk);
         }
         const f4 xb = *(const f4 *)&bs[at];
 #pragma unroll
@@ -148,7 +148,7 @@ __global__ void __launch_bounds__(kDT, 4 - DParts<IT>::in) k_delta_prep(const De
         for (int s = 0; s < KS; ++s) {
           bf8 A[NK];
           load_frag<NK>(&Qf[0][0], kRowsOf, x * KS + s, lane, A);
-          qk = mma<NK>(A, K[s], qk);
+          qk = mma<NM>(A, K[s], qk);
         }
         const f4 xq = *(const f4 *)&fq[at];
 #pragma unroll
