@@ -7,6 +7,7 @@
 // Nothing here is numerical and nothing is kept between calls but a DecodePlan's weight tensors.
 // Errors of the C ABI become the exception classes of ssm_scan._abi.check.
 #include <torch/csrc/Exceptions.h>
+#include <torch/csrc/autograd/custom_function.h>
 #include <torch/csrc/utils/pybind.h>
 
 #include <ATen/ATen.h>
@@ -14,6 +15,7 @@
 #include <c10/hip/HIPStream.h>
 
 #include <algorithm>
+#include <atomic>
 #include <optional>
 #include <sstream>
 #include <vector>
@@ -23,6 +25,8 @@
 namespace py = pybind11;
 using at::Tensor;
 using OptTensor = std::optional<Tensor>;
+using torch::autograd::AutogradContext;
+using torch::autograd::variable_list;
 
 namespace {
 
@@ -91,6 +95,9 @@ Tensor like(const Tensor &t, at::ScalarType dt) {
 Tensor empty(at::IntArrayRef s, const Tensor &ref, at::ScalarType dt) { return at::empty(s, ref.options().dtype(dt)); }
 Tensor bytes(int64_t n, const Tensor &ref) { return at::empty({std::max<int64_t>(n, 1)}, ref.options().dtype(at::kByte)); }
 
+// profiling.KernelTimers in effect.
+std::atomic<int> timers{0};
+
 // The engine launches on the current device and on torch's current stream there.
 struct Launch {
   c10::DeviceGuard guard;
@@ -109,6 +116,20 @@ struct Launch {
       rc = fn(&args, stream);
     }
     if (!end.is_none()) end.attr("record")();
+    check(rc, what);
+  }
+  // The same from anywhere: a backward node runs on autograd's thread without the GIL, and waiting for it
+  // there would cost a small backward a fifth of its time.  Only a timer needs it.
+  template <typename Args>
+  void run_anywhere(const char *what, int (*fn)(const Args *, void *), const Args &args) const {
+    if (timers.load(std::memory_order_relaxed)) {
+      const py::gil_scoped_acquire gil;
+      return run(what, fn, args, py::module_::import("ssm_scan.profiling").attr("active")());
+    }
+    std::optional<py::gil_scoped_release> release;
+    if (PyGILState_Check()) release.emplace();
+    const int rc = fn(&args, stream);
+    release.reset();
     check(rc, what);
   }
 };
@@ -474,6 +495,12 @@ ssm_tensor lead_view(const Tensor &t, int64_t n) {  // the first n strides; the 
   for (int64_t i = 0; i < n; ++i) v.stride[i] = t.stride(i);
   return v;
 }
+bool needs_grad(std::initializer_list<const Tensor *> ts) {
+  if (!at::GradMode::is_enabled()) return false;
+  for (const Tensor *t : ts)
+    if (t->defined() && t->requires_grad()) return true;
+  return false;
+}
 bool delta_type(at::ScalarType t) { return t == at::kFloat || t == at::kBFloat16 || t == at::kHalf; }
 
 // Shapes and types of one call; `lead` = (B, L) of the chunked form, (B,) of the step.
@@ -529,10 +556,13 @@ struct DeltaOps {
   }
 };
 
-// (o, last or None, the tensors delta_backward needs)
-py::tuple delta_forward(const Tensor &q_, const Tensor &k_, const Tensor &v_, const Tensor &g_, const Tensor &beta_,
-                        const OptTensor &h0_, double scale, bool qk_norm, bool want_last, bool need_saved,
-                        const py::object &timer) {
+// o, last (undefined unless wanted) and the tensors delta_backward needs
+struct DeltaOut {
+  Tensor o, last;
+  variable_list saved;
+};
+DeltaOut delta_forward(const Tensor &q_, const Tensor &k_, const Tensor &v_, const Tensor &g_, const Tensor &beta_,
+                       const OptTensor &h0_, double scale, bool qk_norm, bool want_last, bool need_saved) {
   delta_checks(q_, k_, v_, g_, beta_, get(h0_), 2);
   const DeltaOps t(q_, k_, v_, g_, beta_);
   Tensor h0 = cast(get(h0_), at::kFloat);
@@ -555,16 +585,16 @@ py::tuple delta_forward(const Tensor &q_, const Tensor &k_, const Tensor &v_, co
     a.saved = saved.data_ptr();
   }
   const Launch l(o);
-  l.run("ssm_delta_fwd", ssm_delta_fwd, a, timer);
-  return py::make_tuple(o, out(last), py::make_tuple(t.q, t.k, t.v, t.g, t.beta, out(saved)));
+  l.run_anywhere("ssm_delta_fwd", ssm_delta_fwd, a);
+  return {cast(o, v_.scalar_type()), last, {t.q, t.k, t.v, t.g, t.beta, saved}};
 }
 
-// (dq, dk, dv, dg, dbeta, dh0 or None)
-py::tuple delta_backward(const Tensor &q, const Tensor &k, const Tensor &v, const Tensor &g, const Tensor &beta,
-                         const Tensor &saved, const OptTensor &dout_, const OptTensor &dlast_, double scale, bool qk_norm,
-                         bool need_dh0, const py::object &timer) {
-  const Tensor dout = dout_ ? unit_last(cast(*dout_, v.scalar_type())) : at::zeros(v.sizes(), v.options());
-  Tensor dlast = cast(get(dlast_), at::kFloat);
+// dq, dk, dv, dg, dbeta, dh0 (undefined unless needed)
+variable_list delta_backward(const Tensor &q, const Tensor &k, const Tensor &v, const Tensor &g, const Tensor &beta,
+                             const Tensor &saved, const Tensor &dout_, const Tensor &dlast_, double scale, bool qk_norm,
+                             bool need_dh0) {
+  const Tensor dout = dout_.defined() ? unit_last(cast(dout_, v.scalar_type())) : at::zeros(v.sizes(), v.options());
+  Tensor dlast = cast(dlast_, at::kFloat);
   if (dlast.defined()) dlast = dlast.contiguous();
   auto dense = [](const Tensor &t) { return at::empty(t.sizes(), t.options()); };
   const Tensor dq = dense(q), dk = dense(k), dv = dense(v), dg = dense(g), db = dense(beta);
@@ -584,12 +614,51 @@ py::tuple delta_backward(const Tensor &q, const Tensor &k, const Tensor &v, cons
   a.workspace = ws.data_ptr();
   a.workspace_bytes = n;
   const Launch l(v);
-  l.run("ssm_delta_bwd", ssm_delta_bwd, a, timer);
-  return py::make_tuple(dq, dk, dv, dg, db, out(dh0));
+  l.run_anywhere("ssm_delta_bwd", ssm_delta_bwd, a);
+  return {dq, dk, dv, dg, db, dh0};
+}
+
+// The rule's node in autograd, which runs without the interpreter.
+struct DeltaFn : torch::autograd::Function<DeltaFn> {
+  static variable_list forward(AutogradContext *ctx, const Tensor &q, const Tensor &k, const Tensor &v, const Tensor &g,
+                               const Tensor &beta, const OptTensor &h0, double scale, bool qk_norm, bool want_last) {
+    DeltaOut r = delta_forward(q, k, v, g, beta, h0, scale, qk_norm, want_last, true);
+    ctx->save_for_backward(r.saved);
+    ctx->set_materialize_grads(false);
+    ctx->saved_data["scale"] = scale;
+    ctx->saved_data["qk_norm"] = qk_norm;
+    ctx->saved_data["h0"] = h0.has_value();
+    ctx->saved_data["types"] = std::vector<int64_t>{(int64_t)q.scalar_type(), (int64_t)k.scalar_type(), (int64_t)v.scalar_type(),
+                                                    (int64_t)g.scalar_type(), (int64_t)beta.scalar_type(),
+                                                    (int64_t)(h0 ? h0->scalar_type() : at::kFloat)};
+    return want_last ? variable_list{r.o, r.last} : variable_list{r.o};
+  }
+  static variable_list backward(AutogradContext *ctx, variable_list grads) {
+    const Tensor dlast = grads.size() > 1 ? grads[1] : Tensor();
+    if (!grads[0].defined() && !dlast.defined()) return variable_list(9);
+    const variable_list t = ctx->get_saved_variables();
+    variable_list d = delta_backward(t[0], t[1], t[2], t[3], t[4], t[5], grads[0], dlast, ctx->saved_data["scale"].toDouble(),
+                                     ctx->saved_data["qk_norm"].toBool(),
+                                     ctx->saved_data["h0"].toBool() && ctx->needs_input_grad(5));
+    const auto types = ctx->saved_data["types"].toIntVector();
+    for (size_t i = 0; i < d.size(); ++i) d[i] = cast(d[i], (at::ScalarType)types[i]);
+    d.resize(9);
+    return d;
+  }
+};
+// (o, last or None)
+py::tuple delta(const Tensor &q, const Tensor &k, const Tensor &v, const Tensor &g, const Tensor &beta, const OptTensor &h0,
+                double scale, bool qk_norm, bool want_last) {
+  if (!needs_grad({&q, &k, &v, &g, &beta}) && !(h0 && needs_grad({&*h0}))) {
+    const DeltaOut r = delta_forward(q, k, v, g, beta, h0, scale, qk_norm, want_last, false);
+    return py::make_tuple(r.o, out(r.last));
+  }
+  const variable_list r = DeltaFn::apply(q, k, v, g, beta, h0, scale, qk_norm, want_last);
+  return py::make_tuple(r[0], want_last ? py::cast(r[1]) : py::none());
 }
 
 Tensor delta_step(const Tensor &h, const Tensor &q_, const Tensor &k_, const Tensor &v_, const Tensor &g_, const Tensor &beta_,
-                  double scale, bool qk_norm, const py::object &timer) {
+                  double scale, bool qk_norm) {
   delta_checks(q_, k_, v_, g_, beta_, h, 1);
   TORCH_CHECK_VALUE(h.scalar_type() == at::kFloat && h.is_contiguous(), "the state must be contiguous float32, got ",
                     h.scalar_type(), " with strides ", h.strides());
@@ -600,7 +669,7 @@ Tensor delta_step(const Tensor &h, const Tensor &q_, const Tensor &k_, const Ten
   a.h = h.data_ptr<float>();
   a.out = lead_view(o, 2);
   const Launch l(o);
-  l.run("ssm_delta_step", ssm_delta_step, a, timer);
+  l.run_anywhere("ssm_delta_step", ssm_delta_step, a);
   return o.scalar_type() == v_.scalar_type() ? o : o.to(v_.scalar_type());
 }
 
@@ -624,9 +693,9 @@ ssm_gnorm_args gnorm_args(const Tensor &x2, const Tensor &w, const Tensor &b, co
 }
 Tensor f32(const OptTensor &t) { return t ? cast(*t, at::kFloat).contiguous() : Tensor(); }
 
-// (y, x as rows, weight, bias, gate as rows)
-py::tuple gnorm_forward(const Tensor &x, const OptTensor &weight, const OptTensor &bias, const OptTensor &gate, int64_t groups,
-                        int act, bool center, double eps) {
+// y, x as rows, weight, bias, gate as rows
+variable_list gnorm_forward(const Tensor &x, const OptTensor &weight, const OptTensor &bias, const OptTensor &gate,
+                            int64_t groups, int64_t act, bool center, double eps) {
   const Tensor g = get(gate), w_ = get(weight), b_ = get(bias);
   require_gpu({&x, &g, &w_, &b_});
   TORCH_CHECK_VALUE(x.dim() >= 1 && x.size(-1) > 0 && groups > 0 && x.size(-1) % groups == 0, "the last dimension of x, ",
@@ -641,14 +710,14 @@ py::tuple gnorm_forward(const Tensor &x, const OptTensor &weight, const OptTenso
   ssm_gnorm_args a = gnorm_args(x2, w, b, g2, groups, act, center, eps);
   a.out = view(o);
   const Launch l(x);
-  l.run("ssm_gnorm_fwd", ssm_gnorm_fwd, a);
-  return py::make_tuple(o.view(x.sizes()), x2, out(w), out(b), out(g2));
+  l.run_anywhere("ssm_gnorm_fwd", ssm_gnorm_fwd, a);
+  return {o.view(x.sizes()), x2, w, b, g2};
 }
 
-// (dx, dweight, dbias, dgate), the last three None where their operand is
-py::tuple gnorm_backward(const Tensor &x2, const OptTensor &weight, const OptTensor &bias, const OptTensor &gate,
-                         const Tensor &dout, int64_t groups, int act, bool center, double eps, bool need_dw, bool need_db) {
-  const Tensor w = get(weight), b = get(bias), g2 = get(gate), dy = rows(cast(dout, x2.scalar_type()), x2.size(1));
+// dx, dweight, dbias, dgate, the last three undefined where their operand is
+variable_list gnorm_backward(const Tensor &x2, const Tensor &w, const Tensor &b, const Tensor &g2, const Tensor &dout,
+                             int64_t groups, int64_t act, bool center, double eps, bool need_dw, bool need_db) {
+  const Tensor dy = rows(cast(dout, x2.scalar_type()), x2.size(1));
   const Tensor dx = at::empty(x2.sizes(), x2.options());
   const Tensor dgate = g2.defined() ? at::empty(x2.sizes(), x2.options()) : g2;
   const Tensor dw = need_dw ? empty({x2.size(1)}, x2, at::kFloat) : Tensor();
@@ -667,9 +736,42 @@ py::tuple gnorm_backward(const Tensor &x2, const OptTensor &weight, const OptTen
     a.workspace_bytes = n;
   }
   const Launch l(x2);
-  l.run("ssm_gnorm_bwd", ssm_gnorm_bwd, a);
-  const auto shape = dout.sizes();
-  return py::make_tuple(dx.view(shape), out(dw), out(db), g2.defined() ? py::cast(dgate.view(shape)) : py::none());
+  l.run_anywhere("ssm_gnorm_bwd", ssm_gnorm_bwd, a);
+  return {dx.view(dout.sizes()), dw, db, g2.defined() ? dgate.view(dout.sizes()) : g2};
+}
+
+struct GnormFn : torch::autograd::Function<GnormFn> {
+  static Tensor forward(AutogradContext *ctx, const Tensor &x, const OptTensor &weight, const OptTensor &bias,
+                        const OptTensor &gate, int64_t groups, int64_t act, bool center, double eps) {
+    const variable_list r = gnorm_forward(x, weight, bias, gate, groups, act, center, eps);
+    ctx->save_for_backward({r[1], r[2], r[3], r[4]});
+    ctx->saved_data["groups"] = groups;
+    ctx->saved_data["act"] = act;
+    ctx->saved_data["center"] = center;
+    ctx->saved_data["eps"] = eps;
+    auto type = [&](const OptTensor &t) { return (int64_t)(t ? t->scalar_type() : at::kFloat); };
+    ctx->saved_data["types"] = std::vector<int64_t>{(int64_t)x.scalar_type(), type(weight), type(bias), type(gate)};
+    return r[0];
+  }
+  static variable_list backward(AutogradContext *ctx, variable_list grads) {
+    const variable_list t = ctx->get_saved_variables();
+    // edges are numbered over the tensors that were given
+    const bool dw = t[1].defined() && ctx->needs_input_grad(1);
+    const bool db = t[2].defined() && ctx->needs_input_grad(t[1].defined() ? 2 : 1);
+    variable_list d = gnorm_backward(t[0], t[1], t[2], t[3], grads[0], ctx->saved_data["groups"].toInt(),
+                                     ctx->saved_data["act"].toInt(), ctx->saved_data["center"].toBool(),
+                                     ctx->saved_data["eps"].toDouble(), dw, db);
+    const auto types = ctx->saved_data["types"].toIntVector();
+    for (size_t i = 0; i < d.size(); ++i) d[i] = cast(d[i], (at::ScalarType)types[i]);
+    d.resize(8);
+    return d;
+  }
+};
+Tensor gnorm(const Tensor &x, const OptTensor &weight, const OptTensor &bias, const OptTensor &gate, int64_t groups, int64_t act,
+             bool center, double eps) {
+  const Tensor w = get(weight), b = get(bias), g = get(gate);
+  if (!needs_grad({&x, &w, &b, &g})) return gnorm_forward(x, weight, bias, gate, groups, act, center, eps)[0];
+  return GnormFn::apply(x, weight, bias, gate, groups, act, center, eps);
 }
 
 // ------------------------------------------------------------------ decode
@@ -792,11 +894,10 @@ PYBIND11_MODULE(_ssmhost, m) {
   m.def("cscan_backward", torch::wrap_pybind_function(cscan_backward));
   m.def("delta_checks", [](const Tensor &q, const Tensor &k, const Tensor &v, const Tensor &g, const Tensor &beta,
                            const OptTensor &h) { delta_checks(q, k, v, g, beta, get(h), 2); });
-  m.def("delta_forward", torch::wrap_pybind_function(delta_forward));
-  m.def("delta_backward", torch::wrap_pybind_function(delta_backward));
+  m.def("count_timers", [](int change) { timers += change; });
+  m.def("delta", torch::wrap_pybind_function(delta));
   m.def("delta_step", torch::wrap_pybind_function(delta_step));
-  m.def("gnorm_forward", torch::wrap_pybind_function(gnorm_forward));
-  m.def("gnorm_backward", torch::wrap_pybind_function(gnorm_backward));
+  m.def("gnorm", torch::wrap_pybind_function(gnorm));
   m.attr("ABI_VERSION") = SSM_ABI_VERSION;  // of the header the argument structs above were compiled from
   py::class_<DecodePlan>(m, "DecodePlan")
       .def(py::init<const std::vector<std::pair<std::vector<Tensor>, double>> &, Tensor, int64_t, int64_t, int64_t, int64_t,

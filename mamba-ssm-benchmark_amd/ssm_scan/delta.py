@@ -11,37 +11,15 @@ Per batch row and value head, with S (Dk, Dv):
 ``gated_delta_step`` one token per stream.  Key heads may be fewer than value heads (value head h
 reads key head h // (H // Hk)); their gradients are summed over the heads that share them.
 Products run on the matrix cores over bf16 parts of the operands (one part for bf16 inputs, two
-for fp16 and for the float32 intermediates beside them, three for float32 inputs); states,
+for fp16, three for float32 inputs and for the float32 intermediates); states,
 decays, norms and sums are float32 or wider, and every sum runs in a fixed order.
 """
 
 import torch
 
-from . import _abi, profiling
+from . import _abi
 
 MAX_KEY_DIM = 128
-
-
-class GatedDeltaRuleFn(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx, q, k, v, g, beta, h0, scale, qk_norm, want_last):
-        need = any(ctx.needs_input_grad[:6])
-        o, last, tensors = _abi.host().delta_forward(q, k, v, g, beta, h0, scale, qk_norm, want_last, need,
-                                                     profiling.active())
-        if need:
-            ctx.save_for_backward(*tensors)
-        ctx.set_materialize_grads(False)
-        ctx.settings = scale, qk_norm
-        ctx.dtypes = [t.dtype for t in (q, k, v, g, beta)] + [None if h0 is None else h0.dtype]
-        return (o if o.dtype == v.dtype else o.to(v.dtype)), last
-
-    @staticmethod
-    def backward(ctx, dout, dlast):
-        if dout is None and dlast is None:
-            return (None,) * 9
-        grads = _abi.host().delta_backward(*ctx.saved_tensors, dout, dlast, *ctx.settings, ctx.needs_input_grad[5],
-                                           profiling.active())
-        return tuple(d if d is None or d.dtype == t else d.to(t) for d, t in zip(grads, ctx.dtypes)) + (None,) * 3
 
 
 def gated_delta_rule(q, k, v, g, beta, h0=None, scale=None, qk_norm=False, return_last_state=False):
@@ -58,7 +36,7 @@ def gated_delta_rule(q, k, v, g, beta, h0=None, scale=None, qk_norm=False, retur
         last = v.new_zeros((v.shape[0], v.shape[2], q.shape[-1], v.shape[3]), dtype=torch.float32) if h0 is None \
             else h0.float()
         return (v * 1, last) if return_last_state else v * 1
-    o, last = GatedDeltaRuleFn.apply(q, k, v, g, beta, h0, scale, bool(qk_norm), bool(return_last_state))
+    o, last = _abi.host().delta(q, k, v, g, beta, h0, scale, bool(qk_norm), bool(return_last_state))
     return (o, last) if return_last_state else o
 
 
@@ -66,4 +44,4 @@ def gated_delta_step(h, q, k, v, g, beta, scale=None, qk_norm=False):
     """One token per stream: o (B, H, Dv) in v's dtype; h (B, H, Dk, Dv), contiguous float32, is updated
     in place.  q, k (B, Hk, Dk), v (B, H, Dv), g and beta (B, H) as in gated_delta_rule."""
     scale = float(q.shape[-1] ** -0.5 if scale is None else scale)
-    return _abi.host().delta_step(h, q, k, v, g, beta, scale, bool(qk_norm), profiling.active())
+    return _abi.host().delta_step(h, q, k, v, g, beta, scale, bool(qk_norm))

@@ -5,27 +5,10 @@ norm of each head's output in a multi-head recurrence, with the layer's SiLU gat
 same pass.  Statistics are per row and group, never over positions, so it is causal.
 """
 
-import torch
-
 from . import _abi
 
 MAX_GROUP = 1024
 _ACTIVATIONS = {None: 0, "silu": 1}
-
-
-class GroupNormFn(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx, x, weight, bias, gate, groups, act, center, eps):
-        y, *saved = _abi.host().gnorm_forward(x, weight, bias, gate, groups, act, center, eps)
-        ctx.save_for_backward(*saved)
-        ctx.settings = groups, act, center, eps
-        ctx.dtypes = [None if t is None else t.dtype for t in (x, weight, bias, gate)]
-        return y
-
-    @staticmethod
-    def backward(ctx, dout):
-        grads = _abi.host().gnorm_backward(*ctx.saved_tensors, dout, *ctx.settings, *ctx.needs_input_grad[1:3])
-        return tuple(d if d is None or d.dtype == t else d.to(t) for d, t in zip(grads, ctx.dtypes)) + (None,) * 4
 
 
 def group_norm(x, groups, weight=None, bias=None, gate=None, activation=None, center=True, eps=1e-5):
@@ -43,4 +26,4 @@ def group_norm(x, groups, weight=None, bias=None, gate=None, activation=None, ce
     act = 2 if gate is not None else _ACTIVATIONS[activation]
     if x.numel() == 0 and x.shape[-1]:
         return x * 1   # no rows
-    return GroupNormFn.apply(x, weight, bias, gate, int(groups), act, bool(center), float(eps))
+    return _abi.host().gnorm(x, weight, bias, gate, int(groups), act, bool(center), float(eps))

@@ -9,6 +9,8 @@ recorded and launches are not touched.
 
 import torch
 
+from . import _abi
+
 _active = None
 
 
@@ -20,11 +22,13 @@ class KernelTimer:
         global _active
         self._prev = _active
         _active = self
+        _abi.host().count_timers(1)
         return self
 
     def __exit__(self, *exc):
         global _active
         _active = self._prev
+        _abi.host().count_timers(-1)
         return False
 
     def begin(self, name):
