@@ -8,11 +8,13 @@
 // chunk), adding the value heads that share the key head in registers.  With U = beta Y and the lower
 // triangular J_ij = scale |q_i|^-1 |k_j|^-1 e_ij dO_i.U_j, H_ij = beta_i |k_i|^-1 |k_j|^-1 e_ij dR_i.U_j (i > j):
 //   dq' = d dO S0^T + J K,   dk' = c U D^T - beta a dR S0^T + J^T Q - (H + H^T) K
-// of which dq, dk are what the norms leave: dq = dq' - q (q.dq') / (|q|^2), likewise dk.
-// G enters O_i by a factor e^{G_i}, and every path from v_i by e^{-G_i}, whence G's gradient is dO_i.O_i -
-// dV_i.v_i, with dO_i.O_i = q_i.dq'_i since O is linear in q.  The state that leaves has the factor e^{G_C}:
-//   dg_t = <D, S1> + sum over i >= t of (q_i.dq'_i - dV_i.v_i),  <D, S1> = e^{G_C} <D, S0> + sum_j k_j.(c U D^T)_j
-// Every chunk starts from its own <D, S1>, so that at most 64 terms are added to it.
+// of which dq, dk are what the norms leave: dq = dq' - q (q.dq') / |q|^2, likewise dk.
+// G's gradient dG_i: every product of a pair i > j, J_ij q_i.k_j of the outputs and H_ij k_i.k_j of the system,
+// has a factor e^{G_i - G_j} and enters row i and, with the other sign, column j, so that in the sum from t on a
+// pair that does not straddle t cancels to its rounding; J's diagonal has no factor and is kept apart.  The
+// state that enters has e^{G_i} in row i; what goes into the leaving state has e^{G_C - G_j}:
+//   dG_i = q_i.(d dO S0^T + J K)_i + k_i.(H K - J^T Q - H^T K - beta a dR S0^T)_i   (J, H below the diagonal; H with its sign)
+//   dg_t = sum over i >= t of dG_i + sum over j < t of k_j.(c U D^T)_j + e^{G_C} <D, S0>
 #include "ssm_delta.hpp"
 #include "ssm_dpp.hpp"
 
@@ -257,21 +259,21 @@ __global__ void __launch_bounds__(2 * kDT) SSM_TWO_WAVES k_delta_bwd(const Delta
 // read during the last slab.  SHARED: several value heads add to dq', dk', which wait in LDS meanwhile.
 template <typename IT, int DK, bool SHARED>
 __global__ void __launch_bounds__(4 * DK) SSM_TWO_WAVES k_delta_grad(const DeltaParams p) {
-  constexpr int NK = DParts<IT>::in, NM = DParts<IT>::mid, NP = DParts<IT>::out, NT = 4 * DK, NW = DK / 16;
+  constexpr int NK = DParts<IT>::in, NM = DParts<IT>::mid, NT = 4 * DK, NW = DK / 16;
   constexpr int NJ = 16 / NW;                    // tiles of J and H per wavefront
   constexpr int SF = 4 * 64 * 8;                 // staged elements of one part: 64 tokens x 32 columns
-  constexpr int kStage = (NK + NM + NP) * SF, JP = kC + 8, kE = (NM + NP) * kC * JP, PT = 512 / NT;
+  constexpr int kStage = (NK + 2 * NM) * SF, JP = kC + 8, kE = 2 * NM * kC * JP, PT = 512 / NT;
   __shared__ __align__(16) __bf16 buf[2 * kStage > kE ? 2 * kStage : kE];  // dO, U, dR; then J and H
   __shared__ __align__(16) f4 sum[SHARED ? 8 : 1][SHARED ? NT : 1];
   __shared__ __align__(16) float rows[kDeltaRows];
-  __shared__ float red[NW][kC], norm[NW][2][kC], rowb[kC], rowv[kC], sdot[NW], cdot[NW];
+  __shared__ float red[NW][2][kC], norm[NW][2][kC], rowb[kC], diag[kC], sdot[NW];
   const int tid = threadIdx.x, lane = tid % 64, w = wave_id(), r16 = lane % 16, kg = lane / 16;
   const int keyed = (int)p.B * p.Hk, c = blockIdx.x / keyed, bk = blockIdx.x % keyed, b = bk / p.Hk, hk = bk % p.Hk, group = SHARED ? p.H / p.Hk : 1;
   const int64_t t0 = (int64_t)c * kC, kch = blockIdx.x;
   const int wi = w * NJ / 4, wj = w * NJ % 4;    // J's tiles (wi, wj .. wj + NJ - 1)
   const bool keys = 16 * w < p.Dkp;
   const int slabs = (p.VT + 1) / 2;
-  const int64_t ao = r16 * p.dout.s1 + 4 * kg, av = r16 * p.v.s1 + 4 * kg;
+  const int64_t ao = r16 * p.dout.s1 + 4 * kg;
   const unsigned at16 = 16 * r16 + 4 * kg;
   __bf16 *const Jm = buf, *const Hm = buf + NM * kC * JP;
 
@@ -301,7 +303,6 @@ __global__ void __launch_bounds__(4 * DK) SSM_TWO_WAVES k_delta_grad(const Delta
     const int h = hk * group + hg;
     const int64_t ch = ((int64_t)c * p.B + b) * p.H + h;
     const IT *dop = (const IT *)p.dout.p + b * p.dout.s0 + h * p.dout.s2 + t0 * p.dout.s1;
-    const IT *vp = (const IT *)p.v.p + b * p.v.s0 + h * p.v.s2 + t0 * p.v.s1;
     const float *Sp = state_of(p.states, p, ch, 0) + (keys ? 256 * w : 0), *Dp = state_of(p.dstates, p, ch, 0) + (keys ? 256 * w : 0);
     const float *yp = value_of(p.y, p, ch, 0), *xp = value_of(p.dr, p, ch, 0);
     f4 F1[4], F2[4], F3[4], A[NJ], N[NJ];  // S0 dO^T, D U^T, S0 dR^T; tiles of dO U^T, dR U^T, transposed
@@ -309,9 +310,9 @@ __global__ void __launch_bounds__(4 * DK) SSM_TWO_WAVES k_delta_grad(const Delta
     for (int it = 0; it < 4; ++it) F1[it] = F2[it] = F3[it] = 0;
 #pragma unroll
     for (int j = 0; j < NJ; ++j) A[j] = N[j] = 0;
-    float sd = 0, rv[PT], rb[PT];  // <S0, D>; dR.v and dR.Y of the staged tokens
+    float sd = 0, rb[PT];  // <S0, D>; dR.Y of the staged tokens
     f4 sv[2], dv[2], yv[PT], xv[PT];
-    Raw4<IT> go[PT], vv[PT];
+    Raw4<IT> go[PT];
     // staged piece x of this wavefront: half (w + x NW) / 4 of the slab, tokens 16 (w + x NW) % 4 + r16, columns 4 kg + i
     auto load_values = [&](int s) {
 #pragma unroll
@@ -326,7 +327,6 @@ __global__ void __launch_bounds__(4 * DK) SSM_TWO_WAVES k_delta_grad(const Delta
       for (int x = 0; x < PT; ++x) {
         const int vt = 2 * s + (w + x * NW) / 4, it = (w + x * NW) % 4, have = t0 + 16 * it + r16 < p.L ? p.Dv - 16 * vt - 4 * kg : 0;
         go[x] = load4(dop + 16 * it * p.dout.s1 + 16 * vt + ao, (const IT *)p.dout.p, have, p.vdo);
-        vv[x] = load4(vp + 16 * it * p.v.s1 + 16 * vt + av, (const IT *)p.v.p, have, p.vv);
       }
     };
     auto load_states = [&](int s, const float *m, f4 (&v)[2]) {
@@ -341,22 +341,19 @@ __global__ void __launch_bounds__(4 * DK) SSM_TWO_WAVES k_delta_grad(const Delta
         const int sh = (w + x * NW) / 4, it = (w + x * NW) % 4, at = (it * 64 + lane) * 8 + 4 * sh;
         const bool in = 2 * s + sh < p.VT, live = t0 + 16 * it + r16 < p.L && p.Dv - 32 * s - 16 * sh - 4 * kg > 0;
         const float be = rows[4 * (16 * it + r16) + 1];
-        const f4 yy = in ? yv[x] : (f4)0.0f, xx = in ? xv[x] : (f4)0.0f, v = to_f4<IT>(vv[x], live);
-        bf4 o[NK], u[NM], r[NP];
+        const f4 yy = in ? yv[x] : (f4)0.0f, xx = in ? xv[x] : (f4)0.0f;
+        bf4 o[NK], u[NM], r[NM];
         to_parts<IT, NK>(go[x], live, o);
         split_parts<NM>((f4)(be * yy), u);
-        split_parts<NP>(xx, r);
+        split_parts<NM>(xx, r);
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          rv[x] = fmaf(xx[i], v[i], rv[x]);
-          rb[x] = fmaf(xx[i], yy[i], rb[x]);
-        }
+        for (int i = 0; i < 4; ++i) rb[x] = fmaf(xx[i], yy[i], rb[x]);
 #pragma unroll
         for (int n = 0; n < NK; ++n) *(bf4 *)(Os + n * SF + at) = o[n];
 #pragma unroll
         for (int n = 0; n < NM; ++n) *(bf4 *)(Us + n * SF + at) = u[n];
 #pragma unroll
-        for (int n = 0; n < NP; ++n) *(bf4 *)(Rs + n * SF + at) = r[n];
+        for (int n = 0; n < NM; ++n) *(bf4 *)(Rs + n * SF + at) = r[n];
       }
     };
     auto split_states = [&](int s) {
@@ -378,12 +375,12 @@ __global__ void __launch_bounds__(4 * DK) SSM_TWO_WAVES k_delta_grad(const Delta
       const __bf16 *const Os = buf + (s & 1) * kStage, *const Us = Os + NK * SF, *const Rs = Us + NM * SF;
 #pragma unroll
       for (int it = 0; it < 4; ++it) {
-        bf8 O[NK], U[NM], R[NP];
+        bf8 O[NK], U[NM], R[NM];
         load_frag<NK>(Os, SF, it, lane, O);
         load_frag<NM>(Us, SF, it, lane, U);
-        load_frag<NP>(Rs, SF, it, lane, R);
+        load_frag<NM>(Rs, SF, it, lane, R);
         F1[it] = mma<NM>(SA, O, F1[it]);
-        F3[it] = mma<NP>(SA, R, F3[it]);
+        F3[it] = mma<NM>(SA, R, F3[it]);
         F2[it] = mma<NM>(DA, U, F2[it]);
         if (it == wi) {
 #pragma unroll
@@ -392,7 +389,7 @@ __global__ void __launch_bounds__(4 * DK) SSM_TWO_WAVES k_delta_grad(const Delta
               bf8 Uj[NM];
               load_frag<NM>(Us, SF, wj + j, lane, Uj);
               A[j] = mma<NM>(Uj, O, A[j]);
-              N[j] = mma<NP>(Uj, R, N[j]);
+              N[j] = mma<NM>(Uj, R, N[j]);
             }
         }
         read(it);
@@ -413,7 +410,7 @@ __global__ void __launch_bounds__(4 * DK) SSM_TWO_WAVES k_delta_grad(const Delta
         if (tid + i * NT < kDeltaRows) rows[tid + i * NT] = x[i];
     }
 #pragma unroll
-    for (int x = 0; x < PT; ++x) rv[x] = rb[x] = 0;
+    for (int x = 0; x < PT; ++x) rb[x] = 0;
     lds_barrier();
     for (int s = 0; s + 1 < slabs; ++s) {
       stage(s);
@@ -434,16 +431,10 @@ __global__ void __launch_bounds__(4 * DK) SSM_TWO_WAVES k_delta_grad(const Delta
     sd = group_sum<64>(sd);
     if (lane == 0) sdot[w] = sd;
 #pragma unroll
-    for (int x = 0; x < PT; ++x) {
-      rv[x] = kg_sum(rv[x]);
-      rb[x] = kg_sum(rb[x]);
-    }
+    for (int x = 0; x < PT; ++x) rb[x] = kg_sum(rb[x]);
     lds_barrier();  // the slabs are read
     // the two halves of the slabs are one wavefront's two pieces, or wavefronts 0..3 and 4..7
-    if (kg == 0 && (PT == 2 || w >= 4)) {
-      rowv[16 * (w % 4) + r16] = PT == 2 ? rv[0] + rv[PT - 1] : rv[0];
-      rowb[16 * (w % 4) + r16] = PT == 2 ? rb[0] + rb[PT - 1] : rb[0];
-    }
+    if (kg == 0 && (PT == 2 || w >= 4)) rowb[16 * (w % 4) + r16] = PT == 2 ? rb[0] + rb[PT - 1] : rb[0];
     {  // J and H
       const int i = 16 * wi + r16;
       const float fqi = rows[5 * kC + i], fki = rows[4 * kC + i] * rows[4 * i + 1], gh = rows[6 * kC + i], gl = rows[7 * kC + i];
@@ -456,30 +447,30 @@ __global__ void __launch_bounds__(4 * DK) SSM_TWO_WAVES k_delta_grad(const Delta
 #pragma unroll
           for (int x = 0; x < 4; ++x) {
             const float e = fexp((gh - xh[x]) + (gl - xl[x])) * xk[x];
-            jv[x] = at + x <= i ? fqi * e * A[j][x] : 0.0f;
+            jv[x] = at + x < i ? fqi * e * A[j][x] : 0.0f;
+            if (at + x == i) diag[i] = fqi * e * A[j][x];
             hv[x] = at + x < i ? -fki * e * N[j][x] : 0.0f;
           }
         }
-        bf4 jp[NM], hp[NP];
+        bf4 jp[NM], hp[NM];
         split_parts<NM>(jv, jp);
-        split_parts<NP>(hv, hp);
+        split_parts<NM>(hv, hp);
 #pragma unroll
         for (int n = 0; n < NM; ++n) *(bf4 *)(Jm + (n * kC + i) * JP + at) = jp[n];
 #pragma unroll
-        for (int n = 0; n < NP; ++n) *(bf4 *)(Hm + (n * kC + i) * JP + at) = hp[n];
+        for (int n = 0; n < NM; ++n) *(bf4 *)(Hm + (n * kC + i) * JP + at) = hp[n];
       }
     }
-    float cd = 0;
 #pragma unroll
     for (int it = 0; it < 4; ++it) {
-      const f4 row = token_row(rows, 16 * it + r16), ke = whole(Ke[it]), f2 = row[2] * F2[it];
-#pragma unroll
-      for (int i = 0; i < 4; ++i) cd = fmaf(ke[i], f2[i], cd);
+      const f4 row = token_row(rows, 16 * it + r16), f2 = row[2] * F2[it], c = whole(Ke[it]) * f2;
+      const float x = kg_sum((c[0] + c[1]) + (c[2] + c[3]));
+      if (kg == 0) red[w][1][16 * it + r16] = x;
       Y[it] = rows[8 * kC + 16 * it + r16] * F1[it];
-      Z[it] = f2 - (row[1] * row[0]) * F3[it];
+      Z[it] = f2;
+      F2[it] = -(row[1] * row[0]) * F3[it];  // from here on F2 and F3 are what dG takes with a plus and with a minus
+      F3[it] = 0;
     }
-    cd = group_sum<64>(cd);
-    if (lane == 0) cdot[w] = cd;
     lds_barrier();
 #pragma unroll
     for (int s = 0; s < 2; ++s) {
@@ -488,42 +479,41 @@ __global__ void __launch_bounds__(4 * DK) SSM_TWO_WAVES k_delta_grad(const Delta
         const int at = (16 * it + r16) * JP + 32 * s + 4 * kg;                          // row it, columns of step s
         const int tr = (32 * s + 4 * kg + r16 / 4) * JP + 16 * it + 4 * (r16 % 4);      // rows of step s, column it
         if (s <= it / 2) {
-          bf8 B[NM], C[NP];
+          bf8 B[NM], C[NM];
 #pragma unroll
           for (int n = 0; n < NM; ++n) {
             const __bf16 *m = Jm + n * kC * JP + at;
             B[n] = __builtin_shufflevector(*(const bf4 *)m, *(const bf4 *)(m + 16), 0, 1, 2, 3, 4, 5, 6, 7);
           }
 #pragma unroll
-          for (int n = 0; n < NP; ++n) {
+          for (int n = 0; n < NM; ++n) {
             const __bf16 *m = Hm + n * kC * JP + at;
             C[n] = __builtin_shufflevector(*(const bf4 *)m, *(const bf4 *)(m + 16), 0, 1, 2, 3, 4, 5, 6, 7);
           }
           Y[it] = mma<NM>(Kt[s], B, Y[it]);
-          Z[it] = mma<NP>(Kt[s], C, Z[it]);
+          F2[it] = mma<NM>(Kt[s], C, F2[it]);
         }
         if (s >= it / 2) {
-          bf8 B[NP], C[NP];
+          bf8 B[NM], C[NM];
 #pragma unroll
-          for (int n = 0; n < NP; ++n) {
+          for (int n = 0; n < NM; ++n) {
             B[n] = read_tr(Jm + n * kC * JP + tr, Jm + (n * kC + 16) * JP + tr);
             C[n] = read_tr(Hm + n * kC * JP + tr, Hm + (n * kC + 16) * JP + tr);
           }
-          Z[it] = mma<NP>(Qt[s], B, Z[it]);
-          Z[it] = mma<NP>(Kt[s], C, Z[it]);
+          F3[it] = mma<NM>(Qt[s], B, F3[it]);
+          F3[it] = mma<NM>(Kt[s], C, F3[it]);
         }
       }
     }
 #pragma unroll
     for (int it = 0; it < 4; ++it) {
-      const f4 q = whole(Qe[it]) * Y[it];
-      const float x = kg_sum((q[0] + q[1]) + (q[2] + q[3]));
-      if (kg == 0) red[w][16 * it + r16] = x;
+      const f4 q = whole(Qe[it]), k = whole(Ke[it]), z = q * Y[it] + k * (F2[it] - F3[it]);
+      const float x = kg_sum((z[0] + z[1]) + (z[2] + z[3])), own = diag[16 * it + r16];
+      if (kg == 0) red[w][0][16 * it + r16] = x;
+      Y[it] += own * k;
+      Z[it] += (F2[it] + F3[it]) + own * q;
     }
-    if (PT == 1 && w < 4 && kg == 0) {
-      rowv[16 * w + r16] += rv[0];
-      rowb[16 * w + r16] += rb[0];
-    }
+    if (PT == 1 && w < 4 && kg == 0) rowb[16 * w + r16] += rb[0];
     if (SHARED) {
 #pragma unroll
       for (int it = 0; it < 4; ++it) {
@@ -548,15 +538,16 @@ __global__ void __launch_bounds__(4 * DK) SSM_TWO_WAVES k_delta_grad(const Delta
     }
     lds_barrier();
     if (w == 0) {  // dbeta and dg of the head
-      double s = -(double)rows[4 * lane + 1] * rowv[lane], all = 0, ss = 0;
+      double s = 0, k = 0, ss = 0;
 #pragma unroll
-      for (int k = 0; k < NW; ++k) {
-        s += red[k][lane];
-        all += cdot[k];
-        ss += sdot[k];
+      for (int n = 0; n < NW; ++n) {
+        s += red[n][0][lane];
+        k += red[n][1][lane];
+        ss += sdot[n];
       }
-      const double upto = wave_scan_f64(s);  // the sum from i on is the whole less what is before i
-      const double from = (__shfl(upto, 63) - upto) + s + all + (double)rows[3] * ss;
+      // the sum from t on is the whole less what is before t
+      const double upto = wave_scan_f64(s), before = wave_scan_f64(k) - k;
+      const double from = (__shfl(upto, 63) - upto) + s + before + (double)rows[3] * ss;
       const int64_t t = t0 + lane;
       if (t < p.L) {
         ((float *)p.dg.p)[b * p.dg.s0 + t * p.dg.s1 + h * p.dg.s2] = (float)from;

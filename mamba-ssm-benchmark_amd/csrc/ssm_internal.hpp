@@ -328,7 +328,7 @@ hipError_t launch_delta_step(const DeltaStepParams &p, int dtype, hipStream_t s)
 
 // Grouped norm over the last dimension.
 constexpr int kGnormMaxGroup = 1024;
-constexpr int kGnormLanes = 1 << 17;   // lanes of the backward, about: 2048 wavefronts
+constexpr int kGnormLanes = 1 << 18;   // lanes of the backward, about: 4 wavefronts a SIMD hide its loads
 struct GnormParams {
   int64_t R;
   int G, n, center, act;               // act: 0 none, 1 SiLU of the result, 2 gate

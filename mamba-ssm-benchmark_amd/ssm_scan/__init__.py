@@ -8,6 +8,7 @@ Drop-in counterpart of the reference's scan path:
   ssm_scan.norm      <-> RMSNorm of models/common.py:8-16
   ssm_scan.delta     the gated delta rule, a recurrence with a matrix state per head (no counterpart)
   ssm_scan.group_norm  the grouped, gated norm of its output (no counterpart)
+  ssm_scan.delta_mixer  GatedDeltaMixer, a layer of both for training, prefill and decode (no counterpart)
   ssm_scan.block     <-> the Mamba mixer, block and Mamba-only LM of models/mamba.py, models/lm.py
   ssm_scan.decode    <-> a fused per-layer decode step for benchmarks/bench_decode.py's loop
 All compute runs in libssmscan.so (hand-written HIP kernels behind a C ABI, see
