@@ -1,11 +1,10 @@
 """Gated delta rule kernels against the float64 token-by-token oracle (oracle/delta_ref.py).
 
-Tolerances.  An output in a 16-bit type is off by half a step of its value (2^-9 relative for the 8
-significant bits of bf16, 2^-12 for fp16) on top of the arithmetic's error.  The arithmetic is a chain
-of eight tile products (K S, R, T R, P U, K^T U, and their counterparts in the gradients), each taken
-with operands off by at most 2^-18 (two bf16 parts) or summed in float32 over up to 128 terms (2^-20, the
-bound for float32 inputs with three parts): eight times that of the tensor's largest magnitude is
-allowed, 2^-15 and 2^-17.  Both are doubled for gradients, whose operands are themselves such results.
+Tolerances.  An output in a 16-bit type is off by half a step of its value (eps / 2: 2^-8 for bf16, 2^-11
+for fp16) on top of the arithmetic's error.  The arithmetic is a chain of eight tile products (K S, X, T X,
+P U, K^T U, and their counterparts in the gradients), summed in float32 over up to 128 terms (2^-20, with
+operands off by 2^-24): eight times 2^-20 of the tensor's largest magnitude, 2^-17.  For 16-bit inputs
+Q S and P U have operands off by 2^-16, twice that is 2^-15.  Both are doubled for gradients, whose operands are themselves such results.
 With qk_norm, dq = (d - q^ (q^.d)) / |q| is the rest of a cancellation (for Dk = 1 all but 1e-6 of d
 cancels): its error goes by d / |q|, whose largest entry the oracle gives."""
 
