@@ -319,6 +319,7 @@ __global__ void __launch_bounds__(2 * kDT) SSM_TWO_WAVES k_delta_fwd(const Delta
           St[n].get(s, lane, A);
           x[n] = mma<NM>(A, K[s], x[n]);
         }
+      read_ahead<KS * NM * 2 * NV, KS * products(NM, NM, NK) * NV, 12>();
 #pragma unroll
       for (int n = 0; n < NV; ++n) {
         y[n] = to_f4<IT>(v[n], t < p.L && have - 16 * n > 0) - row[0] * x[n];
@@ -328,15 +329,17 @@ __global__ void __launch_bounds__(2 * kDT) SSM_TWO_WAVES k_delta_fwd(const Delta
       load_k(next);
       load_v(next);
       lds_barrier();
+      bf8 X[NV][2][NM];
+#pragma unroll
+      for (int n = 0; n < NV; ++n) {
+        Xt[n].get(0, lane, X[n][0]);
+        Xt[n].get(1, lane, X[n][1]);
+      }
 #pragma unroll
       for (int s = 0; s < 2; ++s)  // Y = X + (T - I) X
         if (s <= w / 2) {
 #pragma unroll
-          for (int n = 0; n < NV; ++n) {
-            bf8 A[NM];
-            Xt[n].get(s, lane, A);
-            y[n] = mma<NM>(A, T[s], y[n]);
-          }
+          for (int n = 0; n < NV; ++n) y[n] = mma<NM>(X[n][s], T[s], y[n]);
         }
 #pragma unroll
       for (int n = 0; n < NV; ++n) {
@@ -358,6 +361,7 @@ __global__ void __launch_bounds__(2 * kDT) SSM_TWO_WAVES k_delta_fwd(const Delta
 #pragma unroll
           for (int r = 0; r < RT; ++r) S[n][r] = mma<NM>(A, Kt[r][s], S[n][r]);
         }
+      read_ahead<2 * NM * 2 * NV, 2 * products(NM, NM, NK) * RT * NV, 12>();
       load_kt(next);
       if (p.y) {
 #pragma unroll

@@ -109,6 +109,25 @@ template <int N, int R> struct VTile {
   }
 };
 
+// Products formed of NA by NB parts when the first M are kept.
+constexpr int products(int m, int na, int nb) {
+  int n = 0;
+  for (int i = 0; i < na; ++i)
+    for (int j = 0; j < nb; ++j) n += i + j < m;
+  return n;
+}
+// Orders a block of READS LDS reads and MMAS products: AHEAD reads first, then products and reads in turn, so that
+// a product's operands are read AHEAD reads before it.
+template <int READS, int MMAS, int AHEAD>
+__device__ __forceinline__ void read_ahead() {
+  __builtin_amdgcn_sched_group_barrier(0x100, AHEAD, 0);
+#pragma unroll
+  for (int i = 0; i < MMAS; ++i) {
+    __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
+    __builtin_amdgcn_sched_group_barrier(0x100, (READS + MMAS - 1) / MMAS, 0);
+  }
+}
+
 // Fragment `at` (of 64 lanes x 8) of an array of N parts, `part` elements each.
 template <int N>
 __device__ __forceinline__ void load_frag(const __bf16 *m, int64_t part, int at, int lane, bf8 (&f)[N]) {

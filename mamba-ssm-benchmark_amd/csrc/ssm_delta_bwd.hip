@@ -93,6 +93,7 @@ __global__ void __launch_bounds__(2 * kDT) SSM_TWO_WAVES k_delta_bwd(const Delta
           Dt[n].get(s, lane, A);
           x[n] = mma<NM>(A, K[s], x[n]);
         }
+      read_ahead<KS * NM * 2 * NV, KS * products(NM, NM, NK) * NV, 12>();
 #pragma unroll
       for (int n = 0; n < NV; ++n) {
         x[n] = row[2] * x[n] + Gt[n][me];
@@ -101,15 +102,17 @@ __global__ void __launch_bounds__(2 * kDT) SSM_TWO_WAVES k_delta_bwd(const Delta
       const float by = -row[1] * row[0], decay = row[3];
       load_k(next);
       lds_barrier();
+      bf8 X[NV][2][NM];
 #pragma unroll
-      for (int s = 0; s < 2; ++s)  // dR = dU + (T^T - I) dU
+      for (int n = 0; n < NV; ++n) {
+        Xt[n].get(1, lane, X[n][1]);
+        Xt[n].get(0, lane, X[n][0]);
+      }
+#pragma unroll
+      for (int s = 1; s >= 0; --s)  // dR = dU + (T^T - I) dU
         if (s >= w / 2) {
 #pragma unroll
-          for (int n = 0; n < NV; ++n) {
-            bf8 A[NM];
-            Xt[n].get(s, lane, A);
-            x[n] = mma<NM>(A, T[s], x[n]);
-          }
+          for (int n = 0; n < NV; ++n) x[n] = mma<NM>(X[n][s], T[s], x[n]);
         }
 #pragma unroll
       for (int n = 0; n < NV; ++n) {
@@ -131,6 +134,7 @@ __global__ void __launch_bounds__(2 * kDT) SSM_TWO_WAVES k_delta_bwd(const Delta
 #pragma unroll
           for (int r = 0; r < RT; ++r) D[n][r] = mma<NM>(A, Kt[r][s], D[n][r]);
         }
+      read_ahead<2 * NM * 2 * NV, 2 * products(NM, NM, NK) * RT * NV, 12>();
       load_cols(p.fKt, next, Kt);
     }
     if (p.dh0) {
