@@ -239,9 +239,9 @@ __global__ void __launch_bounds__(kDT, 4 - DParts<IT>::in) k_delta_prep(const De
 // The chain from state to state is what bounds the walk (per chunk three products, each split into parts and
 // handed on through LDS), so four wavefronts do nothing else and four more take the outputs (Q S, P U and
 // the stores) from what the chain leaves in LDS, while it goes on.
-// One stream of 16384 tokens, H8 128 x 128 bf16: 360 us, 1.4 us a chunk (all in eight wavefronts alike, reads
-// not ahead: 1214).  B4 L4096 H16, with the states saved: 275 us, 160 of them the chain, the rest 435 MB of
-// stores that all workgroups, walking in step, send at the same time.
+// One stream of 16384 tokens, H8 128 x 128 bf16: 320 us, 1.25 us a chunk (LDS reads not ahead of the products:
+// 360; four wavefronts for everything, nothing read ahead: 1214).  B4 L4096 H16: 197 us, 274 with the states
+// saved: 435 MB of stores, which all workgroups, walking in step, send at the same time.
 // Everything that does not hang on the state is read a chunk ahead, into the registers that the chunk has
 // just used.  All products are of transposes: rows are 16 columns of v, so a lane holds 4 columns of
 // one token or key, and moves them as one word.  A workgroup walks NV tiles of 16 columns.

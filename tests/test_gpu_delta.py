@@ -133,6 +133,21 @@ def test_correlated_keys(dev):
     check(a, do, dl, F32, True)
 
 
+@pytest.mark.parametrize("io", [F32, BF16, F16])
+def test_a_decay_with_nothing_before_it_has_no_gradient(dev, io):
+    """Without h0 the first token's decay scales zeros: exactly 0, not the rest of a cancellation."""
+    for L in (1, 64):
+        a, do, _ = make(dev, 2, L, 1, 2, 64, 48, io, seed=13)
+        a["h0"] = None
+        g = a["g"].requires_grad_()
+        o = ssm_scan.gated_delta_rule(**a, qk_norm=True)
+        d = torch.autograd.grad(o, g, do)[0]
+        _, _, want = delta_ref.delta(**a, qk_norm=True, dout=do)
+        if L == 1:
+            assert d.abs().max().item() == 0.0
+        close("dg", d, want["g"], io, grad=True)
+
+
 def test_no_tokens(dev):
     a, _, _ = make(dev, 2, 3, 1, 2, 16, 8, F32)
     a = {n: t if n == "h0" else t[:, :0] for n, t in a.items()}
