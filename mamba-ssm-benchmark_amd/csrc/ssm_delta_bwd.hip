@@ -16,7 +16,6 @@
 //   dG_i = q_i.(d dO S0^T + J K)_i + k_i.(H K - J^T Q - H^T K - beta a dR S0^T)_i   (J, H below the diagonal; H with its sign)
 //   dg_t = sum over i >= t of dG_i + sum over j < t of k_j.(c U D^T)_j + e^{G_C} <D, S0>
 #include "ssm_delta.hpp"
-#include "ssm_dpp.hpp"
 
 namespace ssm {
 

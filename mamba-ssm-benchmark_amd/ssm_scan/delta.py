@@ -19,8 +19,6 @@ import torch
 
 from . import _abi
 
-MAX_KEY_DIM = 128
-
 
 def gated_delta_rule(q, k, v, g, beta, h0=None, scale=None, qk_norm=False, return_last_state=False):
     """o (B, L, H, Dv) in v's dtype; with return_last_state, (o, last (B, H, Dk, Dv) float32).

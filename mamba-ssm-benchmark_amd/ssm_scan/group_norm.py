@@ -7,7 +7,6 @@ same pass.  Statistics are per row and group, never over positions, so it is cau
 
 from . import _abi
 
-MAX_GROUP = 1024
 _ACTIVATIONS = {None: 0, "silu": 1}
 
 
