@@ -34,7 +34,7 @@ __device__ __forceinline__ void put16(float *m, int lane, f4 c, float sign) {
 // the first version's occupancy (two workgroups, all 16 tiles of L and P computed) took 113.
 template <typename IT, int DK, bool BWD>
 __global__ void __launch_bounds__(kDT, 4 - DParts<IT>::in) k_delta_prep(const DeltaParams p) {
-  constexpr int NK = DParts<IT>::in, NM = DParts<IT>::mid, NP = BWD ? NM : DParts<IT>::out, KS = DK / 32, FP = kC + 4, YP = 32 + 4;
+  constexpr int NK = DParts<IT>::in, NM = DParts<IT>::mid, KS = DK / 32, FP = kC + 4, YP = 32 + 4;
   constexpr int kRowsOf = 4 * KS * 64 * 8;  // elements of one part of K or Q
   __shared__ __align__(16) __bf16 Kf[NK][kRowsOf], Qf[BWD ? NK : 1][BWD ? kRowsOf : 8];  // as in memory
   __shared__ __align__(16) float Lm[kC][FP];
@@ -164,10 +164,10 @@ __global__ void __launch_bounds__(kDT, 4 - DParts<IT>::in) k_delta_prep(const De
 #pragma unroll
     for (int s = 0; s < 2; ++s)
       if (BWD ? s >= w / 2 : s <= w / 2) {  // the walks read no other
-        bf8 q[NP];
-        split_parts<NP>((f8)__builtin_shufflevector(P[2 * s], P[2 * s + 1], 0, 1, 2, 3, 4, 5, 6, 7), q);
+        bf8 q[NM];
+        split_parts<NM>((f8)__builtin_shufflevector(P[2 * s], P[2 * s + 1], 0, 1, 2, 3, 4, 5, 6, 7), q);
 #pragma unroll
-        for (int n = 0; n < NP; ++n) *(bf8 *)((__bf16 *)p.fP + (ch * NP + n) * kFrag + (2 * w + s) * 512 + (unsigned)(lane * 8)) = q[n];
+        for (int n = 0; n < NM; ++n) *(bf8 *)((__bf16 *)p.fP + (ch * NM + n) * kFrag + (2 * w + s) * 512 + (unsigned)(lane * 8)) = q[n];
       }
   }
   if (tid < kC) {
@@ -247,10 +247,9 @@ __global__ void __launch_bounds__(kDT, 4 - DParts<IT>::in) k_delta_prep(const De
 // one token or key, and moves them as one word.  A workgroup walks NV tiles of 16 columns.
 template <typename IT, int DK, int NV>
 __global__ void __launch_bounds__(2 * kDT) SSM_TWO_WAVES k_delta_fwd(const DeltaParams p) {
-  constexpr int NK = DParts<IT>::in, NM = DParts<IT>::mid, NP = DParts<IT>::out, KS = DK / 32, RT = DK / 64;
+  constexpr int NK = DParts<IT>::in, NM = DParts<IT>::mid, KS = DK / 32, RT = DK / 64;
   __shared__ __align__(16) VTile<NM, DK> St[NV];
-  __shared__ __align__(16) VTile<NM, kC> Xt[NV], Wt[NV];  // X, c U
-  __shared__ __align__(16) VTile<NP, kC> Ut[NV];
+  __shared__ __align__(16) VTile<NM, kC> Xt[NV], Wt[NV], Ut[NV];  // X, c U, U
   const int lane = threadIdx.x % 64, w = wave_id() % 4, r16 = lane % 16, kg = lane / 16;
   int bh, vt;
   delta_tile((p.VT + NV - 1) / NV, (int)p.B * p.H, bh, vt);
@@ -382,7 +381,7 @@ __global__ void __launch_bounds__(2 * kDT) SSM_TWO_WAVES k_delta_fwd(const Delta
     }
   } else {
     IT *op = (IT *)p.o.p + b * p.o.s0 + h * p.o.s2 + v0;
-    bf8 Q[KS][NK], P[2][NP];
+    bf8 Q[KS][NK], P[2][NM];
     float fd;
     auto load_q = [&](int c) {
 #pragma unroll
@@ -392,7 +391,7 @@ __global__ void __launch_bounds__(2 * kDT) SSM_TWO_WAVES k_delta_fwd(const Delta
     auto load_p = [&](int c) {
 #pragma unroll
       for (int s = 0; s < 2; ++s)
-        if (s <= w / 2) load_frag<NP>((const __bf16 *)p.fP + at(c) * NP * kFrag, kFrag, 2 * w + s, lane, P[s]);
+        if (s <= w / 2) load_frag<NM>((const __bf16 *)p.fP + at(c) * NM * kFrag, kFrag, 2 * w + s, lane, P[s]);
     };
     load_q(0);
     load_p(0);
@@ -407,9 +406,9 @@ __global__ void __launch_bounds__(2 * kDT) SSM_TWO_WAVES k_delta_fwd(const Delta
       for (int s = 0; s < KS; ++s)
 #pragma unroll
         for (int n = 0; n < NV; ++n) {
-          bf8 A[NP];
+          bf8 A[NM];
           St[n].get(s, lane, A);
-          o[n] = mma<NP>(A, Q[s], o[n]);
+          o[n] = mma<NM>(A, Q[s], o[n]);
         }
 #pragma unroll
       for (int n = 0; n < NV; ++n) o[n] *= fd;
@@ -431,9 +430,9 @@ __global__ void __launch_bounds__(2 * kDT) SSM_TWO_WAVES k_delta_fwd(const Delta
         if (s <= w / 2) {
 #pragma unroll
           for (int n = 0; n < NV; ++n) {
-            bf8 A[NP];
+            bf8 A[NM];
             Ut[n].get(s, lane, A);
-            o[n] = mma<NP>(A, P[s], o[n]);
+            o[n] = mma<NM>(A, P[s], o[n]);
           }
         }
       load_p(next);

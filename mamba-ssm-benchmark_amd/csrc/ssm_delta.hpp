@@ -13,9 +13,9 @@
 // bf16 parts (x = p0 + p1 + ..., each the rounding of what the earlier ones leave: 8 significant bits
 // each, so one part is off by 2^-8 of the operand at most, two by 2^-16, three by 2^-24), and a product
 // of parts i and j is formed where i + j is below the count of parts kept.  bf16 inputs are one part and
-// exact, fp16 inputs two and exact, float32 inputs three.  The state, its gradient and everything on the
-// way to them have three parts, whatever the inputs' type: they are float32 outputs, as dg is.  What
-// only reaches outputs of 16 bits has two (DParts::out).
+// exact, fp16 inputs two and exact, float32 inputs three.  Every intermediate has three, whatever the inputs'
+// type: the state, its gradient and dg are float32 outputs, and where the terms of an output of 16 bits
+// cancel, two parts would leave more than its rounding.
 //
 // Where the contraction index is stored.  A lane's 8 elements of a fragment of 32 are, in this order,
 // 4 kg + 0..3 and 16 + 4 kg + 0..3 (kg = lane / 16): the order in which lanes hold the rows of two
@@ -44,11 +44,11 @@ constexpr int kDT = 256;          // four wavefronts: wavefront w owns tokens 16
 #define SSM_TWO_WAVES __attribute__((amdgpu_waves_per_eu(2, 2)))
 constexpr int kFrag = kC * kC;    // elements of one part of a 64 x 64 matrix stored as operand fragments
 
-// Parts of an input of type IT, of float32 intermediates beside it, and of those that only reach outputs of type IT.
+// Parts of an input of type IT and of the float32 intermediates beside it.
 template <typename IT> struct DParts;
-template <> struct DParts<bf16_t> { static constexpr int in = 1, mid = 3, out = 2; };
-template <> struct DParts<f16_t> { static constexpr int in = 2, mid = 3, out = 2; };
-template <> struct DParts<float> { static constexpr int in = 3, mid = 3, out = 3; };
+template <> struct DParts<bf16_t> { static constexpr int in = 1, mid = 3; };
+template <> struct DParts<f16_t> { static constexpr int in = 2, mid = 3; };
+template <> struct DParts<float> { static constexpr int in = 3, mid = 3; };
 
 template <int N, typename F, typename V>
 __device__ __forceinline__ void split_parts(F x, V (&p)[N]) {
