@@ -83,7 +83,7 @@ __device__ __forceinline__ float g_normalize(float (&x)[K][V], int l, int n, boo
 template <typename IT, int V, int NP, int K>
 __global__ void __launch_bounds__(256) k_gnorm_fwd(const GnormParams p) {
   const int l = threadIdx.x % NP;
-  const int64_t id = (int64_t)blockIdx.x * (256 / NP) + threadIdx.x / NP;
+  const int64_t id = p.first + (int64_t)blockIdx.x * (256 / NP) + threadIdx.x / NP;
   const int64_t at = id < p.R * p.G ? id : p.R * p.G - 1;  // lane groups past the end write nothing
   const int64_t row = at / p.G;
   const int c0 = (int)(at % p.G) * p.n;
@@ -160,7 +160,7 @@ __global__ void __launch_bounds__(256) k_gnorm_bwd(const GnormParams p) {
 __global__ void __launch_bounds__(1024) k_gnorm_fin(const GnormParams p) {
   __shared__ double part[64][17];
   const int64_t C = (int64_t)p.G * p.n;
-  const int col = threadIdx.x % 16, q = threadIdx.x / 16;
+  const int col = threadIdx.x, q = threadIdx.y;
   const int64_t j = (int64_t)blockIdx.x * 16 + col, per = (p.nblk + 63) / 64, s0 = q * per;
   const bool second = blockIdx.y || !p.dw;
   const float *ws = p.ws + (second && p.dw ? p.nblk * C : 0);
@@ -179,12 +179,17 @@ template <typename IT, int V, int NP, int K>
 static hipError_t gnorm_v(const GnormParams &p, bool bwd, hipStream_t s) {
   constexpr int64_t Q = 256 / NP;  // lane groups of a workgroup
   if (!bwd) {
-    hipLaunchKernelGGL((k_gnorm_fwd<IT, V, NP, K>), dim3((unsigned)((p.R * p.G + Q - 1) / Q)), dim3(256), 0, s, p);
+    constexpr int64_t most = kGridThreads / NP;
+    GnormParams part = p;
+    for (; part.first < p.R * p.G; part.first += most) {
+      const int64_t left = p.R * p.G - part.first, n = left < most ? left : most;
+      hipLaunchKernelGGL((k_gnorm_fwd<IT, V, NP, K>), dim3((unsigned)((n + Q - 1) / Q)), dim3(256), 0, s, part);
+    }
     return hipGetLastError();
   }
   hipLaunchKernelGGL((k_gnorm_bwd<IT, V, NP, K>), dim3((unsigned)(((int64_t)p.nblk * p.G + Q - 1) / Q)), dim3(256), 0, s, p);
-  if (p.dw || p.db)
-    hipLaunchKernelGGL(k_gnorm_fin, dim3((unsigned)(((int64_t)p.G * p.n + 15) / 16), p.dw && p.db ? 2 : 1), dim3(1024), 0, s, p);
+  if (p.dw || p.db)  // (16, 64) threads: a grid row counts channels alone
+    hipLaunchKernelGGL(k_gnorm_fin, dim3((unsigned)(((int64_t)p.G * p.n + 15) / 16), p.dw && p.db ? 2 : 1), dim3(16, 64), 0, s, p);
   return hipGetLastError();
 }
 

@@ -326,6 +326,9 @@ struct DeltaStepParams {
 };
 hipError_t launch_delta_step(const DeltaStepParams &p, int dtype, hipStream_t s);
 
+// Threads that one launch puts into a grid row: from 2^32 on it wraps without an error.
+constexpr int64_t kGridThreads = 1LL << 31;
+
 // Grouped norm over the last dimension.
 constexpr int kGnormMaxGroup = 1024;
 constexpr int kGnormLanes = 1 << 18;   // lanes of the backward, about: 4 wavefronts a SIMD hide its loads
@@ -341,6 +344,7 @@ struct GnormParams {
   float *dw, *db;                      // (C,) or null
   float *ws;                           // (1 or 2, nblk, C): partial dw, db
   int nblk;                            // row slots of the backward
+  int64_t first;                       // forward: lane groups of earlier launches
 };
 // Row slots: enough lane groups for kGnormLanes, at most one per row.  A group takes at least n / 8 lanes
 // (8 channels of 16 bits per load), so this is within a factor of 8 of it for every variant.
