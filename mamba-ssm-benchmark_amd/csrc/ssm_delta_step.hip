@@ -25,7 +25,8 @@ template <typename IT, int JR, int V>
 __global__ void __launch_bounds__(256) k_delta_step(const DeltaStepParams p) {
   __shared__ float red[4][2][64];
   const int tid = threadIdx.x, lane = tid % 64, w = tid / 64, c4 = 4 * (lane % 16), kr = 4 * w + lane / 16;
-  const int tiles = (p.Dv + 63) / 64, bh = blockIdx.x / tiles, v0 = 64 * (blockIdx.x % tiles);
+  const unsigned tiles = (p.Dv + 63) / 64, x = (unsigned)p.first + blockIdx.x;
+  const int bh = x / tiles, v0 = 64 * (x % tiles);
   const int b = bh / p.H, h = bh % p.H, hk = h / (p.H / p.Hk), have = p.Dv - v0 - c4;
   float *hp = p.h + (int64_t)bh * p.Dk * p.Dv + v0 + c4;
   float S[JR][4], k[JR], q[JR];
@@ -108,12 +109,16 @@ __global__ void __launch_bounds__(256) k_delta_step(const DeltaStepParams p) {
 
 template <typename IT>
 static hipError_t delta_step(const DeltaStepParams &p, hipStream_t s) {
-  const dim3 grid((unsigned)(p.B * p.H) * (unsigned)((p.Dv + 63) / 64));
+  const int64_t all = (int64_t)p.B * p.H * ((p.Dv + 63) / 64), most = kGridThreads / 256;
   const bool v4 = p.Dv % 4 == 0 && (uintptr_t)p.h % 16 == 0;
-  if (p.Dk <= 64 && v4) hipLaunchKernelGGL((k_delta_step<IT, 4, 4>), grid, dim3(256), 0, s, p);
-  else if (p.Dk <= 64) hipLaunchKernelGGL((k_delta_step<IT, 4, 1>), grid, dim3(256), 0, s, p);
-  else if (v4) hipLaunchKernelGGL((k_delta_step<IT, 8, 4>), grid, dim3(256), 0, s, p);
-  else hipLaunchKernelGGL((k_delta_step<IT, 8, 1>), grid, dim3(256), 0, s, p);
+  DeltaStepParams part = p;
+  for (; part.first < all; part.first += most) {
+    const dim3 grid((unsigned)(all - part.first < most ? all - part.first : most));
+    if (p.Dk <= 64 && v4) hipLaunchKernelGGL((k_delta_step<IT, 4, 4>), grid, dim3(256), 0, s, part);
+    else if (p.Dk <= 64) hipLaunchKernelGGL((k_delta_step<IT, 4, 1>), grid, dim3(256), 0, s, part);
+    else if (v4) hipLaunchKernelGGL((k_delta_step<IT, 8, 4>), grid, dim3(256), 0, s, part);
+    else hipLaunchKernelGGL((k_delta_step<IT, 8, 1>), grid, dim3(256), 0, s, part);
+  }
   return hipGetLastError();
 }
 hipError_t launch_delta_step(const DeltaStepParams &p, int dtype, hipStream_t s) {

@@ -293,6 +293,9 @@ hipError_t launch_dec_scan(const DecScanParams &p, int method, hipStream_t s);
 hipError_t launch_dec_out(const DecOutParams &p, hipStream_t s);
 hipError_t launch_dec_head(const DecInParams &p, hipStream_t s);
 
+// Threads that one launch puts into a grid row: from 2^32 on it wraps without an error.
+constexpr int64_t kGridThreads = 1LL << 31;
+
 // Gated delta rule.  Tensors' last dimension has unit stride; views' strides are batch, token, head.
 constexpr int kDeltaChunk = 64;        // tokens per chunk
 constexpr int kDeltaRows = 9 * 64;     // floats of row factors per chunk
@@ -323,11 +326,9 @@ struct DeltaStepParams {
   float scale;
   KView q, k, v, g, beta, o;           // strides: batch, head
   float *h;                            // (B, H, Dk, Dv), updated in place
+  int64_t first;                       // workgroups of earlier launches
 };
 hipError_t launch_delta_step(const DeltaStepParams &p, int dtype, hipStream_t s);
-
-// Threads that one launch puts into a grid row: from 2^32 on it wraps without an error.
-constexpr int64_t kGridThreads = 1LL << 31;
 
 // Grouped norm over the last dimension.
 constexpr int kGnormMaxGroup = 1024;
