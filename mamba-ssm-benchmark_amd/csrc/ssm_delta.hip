@@ -252,8 +252,7 @@ __global__ void __launch_bounds__(2 * kDT) SSM_TWO_WAVES k_delta_fwd(const Delta
   __shared__ __align__(16) VTile<NM, kC> Xt[NV], Wt[NV], Ut[NV];  // X, c U, U
   const int lane = threadIdx.x % 64, w = wave_id() % 4, r16 = lane % 16, kg = lane / 16;
   int bh, vt;
-  delta_tile((p.VT + NV - 1) / NV, (int)p.B * p.H, bh, vt);
-  vt *= NV;
+  delta_tile(p, NV, bh, vt);
   const int b = bh / p.H, h = bh % p.H, hk = h / (p.H / p.Hk), v0 = 16 * vt + 4 * kg, have = p.Dv - v0;
   const int tok = 16 * w + r16;
   auto at = [&](int c) { return (int64_t)c * p.B * p.H + bh; };
@@ -447,9 +446,9 @@ static hipError_t delta_fwd(const DeltaParams &p, hipStream_t s) {
   const unsigned heads = (unsigned)(p.B * p.H);
   hipLaunchKernelGGL((k_delta_prep<IT, DK, false>), dim3(heads * (unsigned)p.NC), dim3(kDT), 0, s, p);
   if (delta_pairs(p))
-    hipLaunchKernelGGL((k_delta_fwd<IT, DK, 2>), dim3((unsigned)(p.B * p.H) * (unsigned)((p.VT + 1) / 2)), dim3(2 * kDT), 0, s, p);
+    delta_walk(p, 2, [&](const DeltaParams &part, dim3 grid) { hipLaunchKernelGGL((k_delta_fwd<IT, DK, 2>), grid, dim3(2 * kDT), 0, s, part); });
   else
-    hipLaunchKernelGGL((k_delta_fwd<IT, DK, 1>), dim3((unsigned)(p.B * p.H) * (unsigned)p.VT), dim3(2 * kDT), 0, s, p);
+    delta_walk(p, 1, [&](const DeltaParams &part, dim3 grid) { hipLaunchKernelGGL((k_delta_fwd<IT, DK, 1>), grid, dim3(2 * kDT), 0, s, part); });
   return hipGetLastError();
 }
 template <typename IT>

@@ -223,16 +223,17 @@ __device__ __forceinline__ double wave_scan_f64(double v) {
 
 __device__ __forceinline__ float fexp(float x) { return fast_exp2(x * LOG2E); }
 
-// Head, chunk-independent addressing.  Workgroup l runs on XCD l % 8: the NV column tiles of a head
-// read the same keys, queries and factors, so they are placed 8 apart where the heads divide evenly.
-__device__ __forceinline__ void delta_tile(int nv, int heads, int &bh, int &vt) {
-  const int x = blockIdx.x;
+// Head and first column tile of a walk's workgroup, which takes `per` of them.  Workgroup l runs on XCD l % 8: the
+// workgroups of a head read the same keys, queries and factors, so they are placed 8 apart where the heads
+// divide evenly.
+__device__ __forceinline__ void delta_tile(const DeltaParams &p, int per, int &bh, int &vt) {
+  const int x = (int)p.first + (int)blockIdx.x, heads = (int)p.B * p.H, nv = (p.VT + per - 1) / per;
   if (heads % 8 == 0) {
     bh = x % 8 + 8 * (x / 8 / nv);
-    vt = x / 8 % nv;
+    vt = x / 8 % nv * per;
   } else {
     bh = x / nv;
-    vt = x % nv;
+    vt = x % nv * per;
   }
 }
 
@@ -264,5 +265,12 @@ __device__ __forceinline__ float *value_of(float *m, const DeltaParams &p, int64
 // work.  Forward, L4096, 128 x 128 bf16, no gradients, pairs against single tiles: 128 tiles 180 and 122 us,
 // 256 tiles 195 and 143, 384 tiles 224 and 277, 512 tiles 250 and 317.
 inline bool delta_pairs(const DeltaParams &p) { return p.B * p.H * p.VT > 256; }
+// launch(p, grid) over a walk's workgroups of `per` column tiles each, as many at once as a grid row takes.
+template <typename F>
+static void delta_walk(const DeltaParams &p, int per, F launch) {
+  const int64_t all = p.B * p.H * ((p.VT + per - 1) / per), most = kGridThreads / (2 * kDT);
+  DeltaParams part = p;
+  for (; part.first < all; part.first += most) launch(part, dim3((unsigned)(all - part.first < most ? all - part.first : most)));
+}
 
 }  // namespace ssm

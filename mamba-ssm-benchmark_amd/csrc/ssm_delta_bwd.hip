@@ -33,8 +33,7 @@ __global__ void __launch_bounds__(2 * kDT) SSM_TWO_WAVES k_delta_bwd(const Delta
   __shared__ __align__(16) f4 Gt[NV][kDT], Rt[NV][RT][kDT], Zt[NV][kDT];  // P^T dO, Q^T (d dO), dR, by lane
   const int lane = threadIdx.x % 64, w = wave_id() % 4, r16 = lane % 16, kg = lane / 16, me = threadIdx.x % kDT;
   int bh, vt;
-  delta_tile((p.VT + NV - 1) / NV, (int)p.B * p.H, bh, vt);
-  vt *= NV;
+  delta_tile(p, NV, bh, vt);
   const int b = bh / p.H, h = bh % p.H, hk = h / (p.H / p.Hk), v0 = 16 * vt + 4 * kg, have = p.Dv - v0;
   const int tok = 16 * w + r16;
   auto at = [&](int c) { return (int64_t)c * p.B * p.H + bh; };
@@ -588,9 +587,9 @@ __global__ void __launch_bounds__(4 * DK) SSM_TWO_WAVES k_delta_grad(const Delta
 template <typename IT, int DK>
 static hipError_t delta_bwd(const DeltaParams &p, hipStream_t s) {
   if (delta_pairs(p))
-    hipLaunchKernelGGL((k_delta_bwd<IT, DK, 2>), dim3((unsigned)(p.B * p.H) * (unsigned)((p.VT + 1) / 2)), dim3(2 * kDT), 0, s, p);
+    delta_walk(p, 2, [&](const DeltaParams &part, dim3 grid) { hipLaunchKernelGGL((k_delta_bwd<IT, DK, 2>), grid, dim3(2 * kDT), 0, s, part); });
   else
-    hipLaunchKernelGGL((k_delta_bwd<IT, DK, 1>), dim3((unsigned)(p.B * p.H) * (unsigned)p.VT), dim3(2 * kDT), 0, s, p);
+    delta_walk(p, 1, [&](const DeltaParams &part, dim3 grid) { hipLaunchKernelGGL((k_delta_bwd<IT, DK, 1>), grid, dim3(2 * kDT), 0, s, part); });
   const dim3 grid((unsigned)(p.B * p.Hk) * (unsigned)p.NC);
   if (p.H > p.Hk) hipLaunchKernelGGL((k_delta_grad<IT, DK, true>), grid, dim3(4 * DK), 0, s, p);
   else hipLaunchKernelGGL((k_delta_grad<IT, DK, false>), grid, dim3(4 * DK), 0, s, p);

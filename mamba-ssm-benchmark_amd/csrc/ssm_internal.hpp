@@ -315,6 +315,7 @@ struct DeltaParams {
   KView dout, dq, dk, dv, dg, dbeta;
   const float *dlast;
   float *dh0, *dstates, *dr;           // gradients of the leaving states and dR, laid out as states and y
+  int64_t first;                       // walks: workgroups of earlier launches
 };
 constexpr int kDeltaMidParts = 3;      // bf16 parts of a float32 intermediate
 inline int delta_in_parts(int dtype) { return dtype == 0 ? 3 : dtype == 1 ? 1 : 2; }

@@ -27,3 +27,40 @@ def test_step_of_more_workgroups_than_a_grid_row(dev):
         want_o, want_h = delta_ref.delta(*(t[r, None] for t in (q, k, v, decay, beta)), h0=before[r], qk_norm=True)
         close("o", o[r], want_o[:, 0], F32)
         close("h", h[r], want_h, F32)
+
+
+def walk_inputs(dev, B, Dv):
+    g = torch.Generator(device=dev).manual_seed(52)
+
+    def rn(*s):
+        return torch.randn(*s, generator=g, device=dev)
+
+    return dict(q=rn(B, 1, 1, 1), k=rn(B, 1, 1, 1), v=rn(B, 1, 1, Dv), g=-rn(B, 1, 1).abs(), beta=torch.sigmoid(rn(B, 1, 1)))
+
+
+# 2^20 tiles of 16 columns a head, two to a workgroup of 512 threads: 17 heads are more than 2^32 threads
+COLUMNS = [slice(c, c + 40) for c in (0, (1 << 23) - 20, (1 << 24) - 40)]
+
+
+def test_walk_of_more_workgroups_than_a_grid_row(dev):
+    B, Dv = 17, 1 << 24
+    a = walk_inputs(dev, B, Dv)
+    o, last = ssm_scan.gated_delta_rule(**a, qk_norm=True, return_last_state=True)
+    for c in COLUMNS:
+        want_o, want_last = delta_ref.delta(**{**a, "v": a["v"][..., c]}, qk_norm=True)
+        close("o", o[..., c], want_o, F32)
+        close("last", last[..., c], want_last, F32)
+
+
+def test_backward_walk_of_more_workgroups_than_a_grid_row(dev):
+    """dv's columns hang on their own columns of v and the outputs' gradient alone."""
+    if torch.cuda.mem_get_info()[0] < 230e9:
+        pytest.skip("keeps 10 KB for each of 2^24 tiles: 180 GB")
+    B, Dv = 17, 1 << 24
+    a = walk_inputs(dev, B, Dv)
+    do = torch.randn(B, 1, 1, Dv, device=dev)
+    o = ssm_scan.gated_delta_rule(**{**a, "v": a["v"].requires_grad_()}, qk_norm=True)
+    dv = torch.autograd.grad(o, a["v"], do)[0]
+    for c in COLUMNS:
+        _, _, want = delta_ref.delta(**{**a, "v": a["v"][..., c]}, qk_norm=True, dout=do[..., c])
+        close("dv", dv[..., c], want["v"], F32, grad=True)
