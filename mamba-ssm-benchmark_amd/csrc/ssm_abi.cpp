@@ -1170,7 +1170,8 @@ static int delta_common(int64_t B, int64_t Hk, int64_t H, int64_t Dk, int64_t Dv
   if (Dk > kDeltaMaxK) return fail(SSM_EINVAL, "key_dim=%lld > %d is not supported", (long long)Dk, kDeltaMaxK);
   if (H % Hk) return fail(SSM_EINVAL, "heads=%lld is not a multiple of key_heads=%lld", (long long)H, (long long)Hk);
   if (!(scale - scale == 0.0f)) return fail(SSM_EINVAL, "scale must be finite");
-  if (H > (1 << 24) || Dv > (1 << 24) || B > (1LL << 31) || B * H * cdiv(Dv, 16) >= (1LL << 31))
+  constexpr int64_t most = (1LL << 31) - 1;  // of the walks' column tiles
+  if (H > (1 << 24) || Dv > (1 << 24) || B > most / (H * cdiv(Dv, 16)))
     return fail(SSM_EINVAL, "batch * heads * value_dim is too large: %lld x %lld x %lld", (long long)B, (long long)H,
                 (long long)Dv);
   return ok();
@@ -1191,7 +1192,7 @@ int ssm_delta_check(const ssm_delta_args *a) {
   int rc = delta_common(a->batch, a->key_heads, a->heads, a->key_dim, a->value_dim, a->dtype, a->scale);
   if (rc) return rc;
   if (a->seqlen < 1) return fail(SSM_EINVAL, "empty problem: seqlen=%lld", (long long)a->seqlen);
-  if (a->seqlen > (1LL << 31) || a->batch * a->heads * cdiv(a->seqlen, kDeltaChunk) >= (1LL << 31))
+  if (a->seqlen > (1LL << 31) || a->batch * a->heads * cdiv(a->seqlen, kDeltaChunk) >= kDeltaMaxChunks)
     return fail(SSM_EINVAL, "batch * heads * seqlen is too large: %lld x %lld x %lld", (long long)a->batch,
                 (long long)a->heads, (long long)a->seqlen);
   return need({{a->q.data, "q"}, {a->k.data, "k"}, {a->v.data, "v"}, {a->g.data, "g"}, {a->beta.data, "beta"}});

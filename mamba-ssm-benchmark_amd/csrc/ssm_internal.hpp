@@ -317,6 +317,9 @@ struct DeltaParams {
   float *dh0, *dstates, *dr;           // gradients of the leaving states and dR, laid out as states and y
   int64_t first;                       // walks: workgroups of earlier launches
 };
+// Chunks of all heads together: what is taken chunk by chunk is one launch of at most 512 threads each.  More have
+// a workspace of over 400 GB.
+constexpr int64_t kDeltaMaxChunks = 1 << 23;
 constexpr int kDeltaMidParts = 3;      // bf16 parts of a float32 intermediate
 inline int delta_in_parts(int dtype) { return dtype == 0 ? 3 : dtype == 1 ? 1 : 2; }
 inline int delta_width(int64_t Dk) { return Dk <= 64 ? 64 : 128; }  // keys of the kernel variant
