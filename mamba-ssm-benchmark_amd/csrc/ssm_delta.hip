@@ -38,7 +38,7 @@ __global__ void __launch_bounds__(kDT, 4 - DParts<IT>::in) k_delta_prep(const De
   constexpr int kRowsOf = 4 * KS * 64 * 8;  // elements of one part of K or Q
   __shared__ __align__(16) __bf16 Kf[NK][kRowsOf], Qf[BWD ? NK : 1][BWD ? kRowsOf : 8];  // as in memory
   __shared__ __align__(16) float Lm[kC][FP];
-  __shared__ float Gh[kC], Gl[kC], fk[kC], fq[kC], bs[kC];  // G as the sum of two floats
+  __shared__ float Gh[kC], Gl[kC], fk[kC], fq[kC], fu[BWD ? kC : 1], bs[kC];  // G as the sum of two floats
   static_assert(sizeof(Kf) >= sizeof(float) * 32 * YP, "the inversion's scratch");
   float *const Yr = (float *)&Kf[0][0];                     // ... lies where the keys were
   const int tid = threadIdx.x, lane = tid % 64, w = wave_id(), r16 = lane % 16, kg = lane / 16, own = 16 * w + r16;
@@ -94,14 +94,17 @@ __global__ void __launch_bounds__(kDT, 4 - DParts<IT>::in) k_delta_prep(const De
       if (BWD) *(bf8 *)&Qf[n][((w * KS + s) * 64 + lane) * 8] = Q[s][n];
     }
   }
-  float nk = 1.0f, nq = p.scale;
+  float nk = 1.0f, nq = p.scale, uq = 1.0f;
   if (p.qk_norm) {
+    const float len = sqrtf(kg_sum(qq) + 1e-6f);
     nk = 1.0f / sqrtf(kg_sum(kk) + 1e-6f);
-    nq = p.scale / sqrtf(kg_sum(qq) + 1e-6f);
+    nq = p.scale / len;
+    uq = 1.0f / len;
   }
   if (kg == 0) {
     fk[own] = nk;
     fq[own] = nq;
+    if (BWD) fu[own] = uq;
   }
   lds_barrier();
   if (first) {
@@ -179,6 +182,7 @@ __global__ void __launch_bounds__(kDT, 4 - DParts<IT>::in) k_delta_prep(const De
     rows[6 * kC + tid] = gh;
     rows[7 * kC + tid] = gl;
     rows[8 * kC + tid] = fq[tid] * eG;
+    if (BWD) rows[9 * kC + tid] = fu[tid];
   }
   wave_lds_sync();  // the diagonal block is this wavefront's own
   {

@@ -239,7 +239,7 @@ __device__ __forceinline__ void delta_tile(const DeltaParams &p, int per, int &b
 
 // Row factors of a chunk, kDeltaRows floats: per token a = |k|^-1 e^G, beta, c = |k|^-1 e^{G_C - G} and
 // e^{G_C}, which the chain takes in one read; then [4] |k|^-1, [5] scale |q|^-1 (the norms are 1 without
-// qk_norm), [6] + [7] G as the sum of two floats, [8] d = scale |q|^-1 e^G.
+// qk_norm), [6] + [7] G as the sum of two floats, [8] d = scale |q|^-1 e^G; for the backward [9] |q|^-1.
 __device__ __forceinline__ const float *delta_rows(const DeltaParams &p, int64_t ch) { return p.rows + ch * kDeltaRows; }
 __device__ __forceinline__ f4 token_row(const float *rows, int tok) { return *(const f4 *)(rows + (unsigned)(4 * tok)); }
 

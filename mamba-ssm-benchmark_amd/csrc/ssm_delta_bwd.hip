@@ -73,7 +73,6 @@ __global__ void __launch_bounds__(2 * kDT) SSM_TWO_WAVES k_delta_bwd(const Delta
     load_cols(p.fKt, p.NC - 1, Kt);
     lds_barrier();  // the first chunk's dO
     for (int c = p.NC - 1; c >= 0; --c) {
-      const int64_t t = (int64_t)c * kC + tok;
       const int next = c ? c - 1 : 0;
 #pragma unroll
       for (int n = 0; n < NV; ++n)
@@ -575,7 +574,7 @@ __global__ void __launch_bounds__(4 * DK) SSM_TWO_WAVES k_delta_grad(const Delta
         sq += norm[k][0][tok];
         sk += norm[k][1][tok];
       }
-      const float fk = rows[4 * kC + tok], nq = rows[5 * kC + tok] / p.scale;
+      const float fk = rows[4 * kC + tok], nq = rows[9 * kC + tok];
       Y[it] -= (nq * nq * sq) * whole(Qe[it]);
       Z[it] -= (fk * fk * sk) * whole(Ke[it]);
     }

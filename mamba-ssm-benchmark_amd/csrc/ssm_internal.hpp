@@ -298,7 +298,7 @@ constexpr int64_t kGridThreads = 1LL << 31;
 
 // Gated delta rule.  Tensors' last dimension has unit stride; views' strides are batch, token, head.
 constexpr int kDeltaChunk = 64;        // tokens per chunk
-constexpr int kDeltaRows = 9 * 64;     // floats of row factors per chunk
+constexpr int kDeltaRows = 10 * 64;    // floats of row factors per chunk
 constexpr int kDeltaMaxK = 128;        // key width of the chunked kernels and the step
 struct DeltaParams {
   int64_t B, L;

@@ -9,6 +9,7 @@ import torch
 
 from oracle import delta_ref
 import ssm_scan
+from test_gpu_delta import close, make
 
 pytestmark = pytest.mark.gpu
 
@@ -61,3 +62,19 @@ def test_decays_that_cancel(dev, io):
     x, r = torch.rand(2, H, generator=torch.Generator().manual_seed(2))
     g = torch.stack([0 * x, -r * 2.0 ** -12, -x])[None]
     run(dev, io, *orthogonal_tokens(H), g, torch.ones(1, 3, H))
+
+
+@pytest.mark.parametrize("scale", [0.0, 1e-60])
+@pytest.mark.parametrize("io", [torch.float32, BF16, F16])
+def test_a_scale_of_zero(dev, scale, io):
+    """No scale (1e-60 is 0 in float32): outputs and dq are 0, through the norm too; the last state's gradients are
+    what they are."""
+    a, do, dl = make(dev, 2, 70, 1, 2, 40, 24, io, seed=61)
+    a = {n: t.requires_grad_() for n, t in a.items()}
+    o, last = ssm_scan.gated_delta_rule(**a, scale=scale, qk_norm=True, return_last_state=True)
+    grads = dict(zip(a, torch.autograd.grad([o, last], list(a.values()), [do, dl])))
+    _, want_last, want = delta_ref.delta(**a, scale=0.0, qk_norm=True, dlast=dl)
+    assert not o.any() and not grads["q"].any()
+    close("last", last, want_last, io)
+    for n in ("k", "v", "g", "beta", "h0"):
+        close("d" + n, grads[n], want[n], io, grad=True, size=want["size"].get(n, 0.0))
