@@ -17,6 +17,21 @@ __device__ __forceinline__ f4 mma_f32(const float *a, const float *b, int lane, 
                                              b[(4 * k + lane / 16) * PB + lane % 16], c, 0, 0, 0);
   return c;
 }
+// The same where a (la) or b (lb) is a lower triangular block: where a result is not finite, all are formed again
+// without the zeros above the diagonals (not_finite(), ssm_delta.hpp).
+template <int PA, int PB>
+__device__ __forceinline__ f4 mma_lower(const float *a, bool la, const float *b, bool lb, int lane, f4 c) {
+  const f4 r[1] = {mma_f32<PA, PB>(a, b, lane, c)};
+  if (__builtin_expect(!not_finite(r), 1)) return r[0];
+  const int col = lane % 16;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const int row = 4 * (lane / 16) + i;
+#pragma unroll 1
+    for (int k = lb ? col : 0; k <= (la ? row : 15); ++k) c[i] = fmaf(a[row * PA + k], b[k * PB + col], c[i]);
+  }
+  return c;
+}
 template <int PITCH>
 __device__ __forceinline__ void put16(float *m, int lane, f4 c, float sign) {
 #pragma unroll
@@ -204,9 +219,9 @@ __global__ void __launch_bounds__(kDT, 4 - DParts<IT>::in) k_delta_prep(const De
   lds_barrier();
   if (w < 2) {
     float *Y = Yr + 16 * w * YP;
-    put16<YP>(Y, lane, mma_f32<FP, FP>(&Lm[32 * w + 16][32 * w], &Lm[32 * w][32 * w], lane, (f4)0.0f), 1.0f);
+    put16<YP>(Y, lane, mma_lower<FP, FP>(&Lm[32 * w + 16][32 * w], false, &Lm[32 * w][32 * w], true, lane, (f4)0.0f), 1.0f);
     wave_lds_sync();
-    const f4 t10 = mma_f32<FP, YP>(&Lm[32 * w + 16][32 * w + 16], Y, lane, (f4)0.0f);
+    const f4 t10 = mma_lower<FP, YP>(&Lm[32 * w + 16][32 * w + 16], true, Y, false, lane, (f4)0.0f);
     wave_lds_sync();
     put16<FP>(&Lm[32 * w + 16][32 * w], lane, t10, -1.0f);
   }
@@ -214,13 +229,13 @@ __global__ void __launch_bounds__(kDT, 4 - DParts<IT>::in) k_delta_prep(const De
   const int r = w / 2, cc = w % 2;
   {
     f4 y = 0;
-    for (int k = cc; k < 2; ++k) y = mma_f32<FP, FP>(&Lm[32 + 16 * r][16 * k], &Lm[16 * k][16 * cc], lane, y);
+    for (int k = cc; k < 2; ++k) y = mma_lower<FP, FP>(&Lm[32 + 16 * r][16 * k], false, &Lm[16 * k][16 * cc], k == cc, lane, y);
     put16<YP>(Yr + 16 * r * YP + 16 * cc, lane, y, 1.0f);
   }
   lds_barrier();
   {
     f4 y = 0;
-    for (int k = 0; k <= r; ++k) y = mma_f32<FP, YP>(&Lm[32 + 16 * r][32 + 16 * k], Yr + 16 * k * YP + 16 * cc, lane, y);
+    for (int k = 0; k <= r; ++k) y = mma_lower<FP, YP>(&Lm[32 + 16 * r][32 + 16 * k], k == r, Yr + 16 * k * YP + 16 * cc, false, lane, y);
     put16<FP>(&Lm[32 + 16 * r][16 * cc], lane, y, -1.0f);
   }
   lds_barrier();
@@ -343,12 +358,21 @@ __global__ void __launch_bounds__(2 * kDT) SSM_TWO_WAVES k_delta_fwd(const Delta
 #pragma unroll
           for (int n = 0; n < NV; ++n) y[n] = mma<NM>(X[n][s], T[s], y[n]);
         }
+      auto put_u = [&] {
 #pragma unroll
-      for (int n = 0; n < NV; ++n) {
-        Wt[n].put(tok, kg, bc * y[n]);
-        Ut[n].put(tok, kg, bu * y[n]);
-      }
+        for (int n = 0; n < NV; ++n) {
+          Wt[n].put(tok, kg, bc * y[n]);
+          Ut[n].put(tok, kg, bu * y[n]);
+        }
+      };
+      put_u();
       load_t(next);
+      if (__builtin_expect(not_finite(y), 0)) {  // after the writes, which need not wait for it
+#pragma unroll
+        for (int n = 0; n < NV; ++n)
+          y[n] = row_times<NM>((const __bf16 *)p.fT + at(c) * NM * kFrag, tok, 0, tok, Xt[n], kg, Xt[n].value(tok, kg));
+        put_u();
+      }
       lds_barrier();
 #pragma unroll
       for (int n = 0; n < NV; ++n)
@@ -428,6 +452,9 @@ __global__ void __launch_bounds__(2 * kDT) SSM_TWO_WAVES k_delta_fwd(const Delta
       load_q(next);
       lds_barrier();
       lds_barrier();
+      f4 qs[NV];
+#pragma unroll
+      for (int n = 0; n < NV; ++n) qs[n] = o[n];
 #pragma unroll
       for (int s = 0; s < 2; ++s)
         if (s <= w / 2) {
@@ -438,6 +465,11 @@ __global__ void __launch_bounds__(2 * kDT) SSM_TWO_WAVES k_delta_fwd(const Delta
             o[n] = mma<NM>(A, P[s], o[n]);
           }
         }
+      if (__builtin_expect(not_finite(o), 0)) {
+#pragma unroll
+        for (int n = 0; n < NV; ++n)
+          o[n] = row_times<NM>((const __bf16 *)p.fP + at(c) * NM * kFrag, tok, 0, tok + 1, Ut[n], kg, qs[n]);
+      }
       load_p(next);
 #pragma unroll
       for (int n = 0; n < NV; ++n) store4(op + t * p.o.s1 + 16 * n, o[n], t < p.L ? have - 16 * n : 0, p.vo);

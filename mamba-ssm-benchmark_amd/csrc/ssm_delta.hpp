@@ -100,6 +100,14 @@ template <int N, int R> struct VTile {
     for (int n = N - 1; n >= 0; --n) x += __builtin_convertvector(*(const bf4 *)&e[n][row * 16 + ((kg ^ ((row >> 2) & 2)) * 4)], f4);
     return x;
   }
+  // whole(), but infinite where the value is (its other parts are inf - inf)
+  __device__ __forceinline__ f4 value(int row, int kg) const {
+    f4 x = whole(row, kg);
+    const f4 first = __builtin_convertvector(*(const bf4 *)&e[0][row * 16 + ((kg ^ ((row >> 2) & 2)) * 4)], f4);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) x[i] = fabsf(first[i]) < INFINITY ? x[i] : first[i];
+    return x;
+  }
   // operand of rows 32 s .. 32 s + 31: lane = column of v
   template <int M>
   __device__ __forceinline__ void get(int s, int lane, bf8 (&f)[M]) const {  // the first M parts
@@ -133,6 +141,30 @@ template <int N>
 __device__ __forceinline__ void load_frag(const __bf16 *m, int64_t part, int at, int lane, bf8 (&f)[N]) {
 #pragma unroll
   for (int n = 0; n < N; ++n) f[n] = *(const bf8 *)(m + n * part + at * 512 + (unsigned)(lane * 8));
+}
+
+// The products of a chunk's triangular matrices run over steps of 32 tokens, with the zeros beyond the diagonal,
+// and a zero times an infinity or NaN is NaN: it would reach tokens that the recurrence keeps free of it.  It
+// shows in the wavefront's own results, so these are looked at, and only where one is not finite are they formed
+// again from the tokens that belong to them.
+template <int N> __device__ __forceinline__ bool not_finite(const f4 (&x)[N]) {
+  float s = 0;
+#pragma unroll
+  for (int n = 0; n < N; ++n) s += (fabsf(x[n][0]) + fabsf(x[n][1])) + (fabsf(x[n][2]) + fabsf(x[n][3]));
+  return __builtin_amdgcn_ballot_w64(!(s < INFINITY)) != 0;
+}
+// acc + sum over the tokens j, lo <= j < hi, of m[tok][j] x_j (columns 4 kg + i): m as fragments of token rows.
+template <int N, typename TILE>
+__device__ __forceinline__ f4 row_times(const __bf16 *m, int tok, int lo, int hi, const TILE &x, int kg, f4 acc) {
+#pragma unroll 1
+  for (int j = lo; j < hi; ++j) {
+    const __bf16 *e = m + (2 * (tok / 16) + j / 32) * 512 + (j % 16 / 4 * 16 + tok % 16) * 8 + j % 32 / 16 * 4 + j % 4;
+    float c = 0;
+#pragma unroll
+    for (int n = N - 1; n >= 0; --n) c += (float)e[n * kFrag];
+    acc += c * x.value(j, kg);
+  }
+  return acc;
 }
 
 __device__ __forceinline__ int wave_id() { return __builtin_amdgcn_readfirstlane(threadIdx.x / 64); }

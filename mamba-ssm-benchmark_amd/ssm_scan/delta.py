@@ -27,7 +27,9 @@ def gated_delta_rule(q, k, v, g, beta, h0=None, scale=None, qk_norm=False, retur
     (read in place with any strides whose last one is 1).  g (B, L, H): log decays (<= 0; -inf forgets
     the state, as at a document's start); beta (B, L, H).  h0 (B, H, Dk, Dv): the state before the first
     token, zeros if None.  scale: Dk^-0.5 if None.  qk_norm divides q and k by sqrt(sum of squares + 1e-6)
-    over Dk first."""
+    over Dk first.  An infinity or NaN reaches what the recurrence takes it to: outputs from its own token on
+    (in v, those of its column), never those of earlier tokens, so that the end of a padded row may hold anything;
+    an infinity may come out as NaN."""
     scale = float(q.shape[-1] ** -0.5 if scale is None else scale)
     if v.dim() == 4 and v.numel() == 0 and v.shape[2] and v.shape[3]:   # no token: the state passes through
         _abi.host().delta_checks(q, k, v, g, beta, h0)
