@@ -1200,11 +1200,12 @@ int ssm_delta_check(const ssm_delta_args *a) {
 
 namespace {
 struct DeltaLayout {
-  int64_t states, values, square, keys, rows;  // bytes of one array, 256-byte multiples
+  int64_t states, dstates, values, square, keys, rows;  // bytes of one array, 256-byte multiples
 };
 DeltaLayout delta_layout(const ssm_delta_args *a) {
   const int64_t nc = cdiv(a->seqlen, kDeltaChunk), n = a->batch * a->heads * nc, v = cdiv(a->value_dim, 16) * 16;
-  return {align256(n * cdiv(a->key_dim, 16) * 16 * v * 4), align256(n * kDeltaChunk * v * 4),
+  const int64_t state = cdiv(a->key_dim, 16) * 16 * v * 4;
+  return {align256(n * state), align256((n + a->batch * a->heads) * state), align256(n * kDeltaChunk * v * 4),
           align256(n * kDeltaMidParts * kDeltaChunk * kDeltaChunk * 2),
           align256(a->batch * a->key_heads * nc * delta_in_parts(a->dtype) * kDeltaChunk * delta_width(a->key_dim) * 2),
           align256(n * kDeltaRows * 4)};
@@ -1235,7 +1236,7 @@ DeltaParams delta_params(const ssm_delta_args *a, bool bwd) {
   p.rows = (float *)take(l.rows);
   if (bwd) {
     p.fQt = take(l.keys);
-    p.dstates = (float *)take(l.states);
+    p.dstates = (float *)take(l.dstates);
     p.dr = (float *)take(l.values);
   }
   if (a->saved) {
@@ -1259,7 +1260,7 @@ int64_t ssm_delta_fwd_workspace_bytes(const ssm_delta_args *a) {
 int64_t ssm_delta_bwd_workspace_bytes(const ssm_delta_args *a) {
   if (ssm_delta_check(a)) return -1;
   const DeltaLayout l = delta_layout(a);
-  return 2 * l.square + 4 * l.keys + l.rows + l.states + l.values;
+  return 2 * l.square + 4 * l.keys + l.rows + l.dstates + l.values;
 }
 
 int ssm_delta_fwd(const ssm_delta_args *a, void *stream) {

@@ -38,9 +38,24 @@ __device__ __forceinline__ void put16(float *m, int lane, f4 c, float sign) {
   for (int i = 0; i < 4; ++i) m[(4 * (lane / 16) + i) * PITCH + lane % 16] = sign * c[i];
 }
 
+// Whether any of 8 elements is infinite or NaN: an exponent of all ones carries into the sign's place.
+typedef unsigned u4 __attribute__((ext_vector_type(4)));
+__device__ __forceinline__ bool odd_halves(bf8 x) {
+  const u4 t = (__builtin_bit_cast(u4, x) & 0x7f807f80u) + 0x00800080u;
+  return ((t[0] | t[1]) | (t[2] | t[3])) & 0x80008000u;
+}
+__device__ __forceinline__ bf8 without_odd(bf8 x) {
+#pragma unroll
+  for (int i = 0; i < 8; ++i) x[i] = fabsf((float)x[i]) < INFINITY ? x[i] : (__bf16)0.0f;
+  return x;
+}
+
 // Writes T - I and P as operand fragments, the row factors, and, for the first of the value heads that
 // share a key head, the fragments of K and Q.  BWD: the transposes of T = (I + strictly lower(beta_i
 // e^{G_i - G_j} k_i.k_j))^-1, which the gradient takes, and of P.
+// The backward's columns of K and Q have 0 in the place of an infinity or NaN: J K, J^T Q, H K and H^T K take them
+// with zeros beyond the diagonals, and what the tokens concerned get of them is infinite or NaN without it, through
+// U, dR and J's diagonal.
 // T is inverted in float32: the four 16 x 16 diagonal blocks by substitution, one wavefront each, the
 // rest by T10 = -T11 (L10 T00) for blocks of 16, then of 32 rows.
 // Chunks are independent, so everything that does not hang on the state is done here, once for all columns
@@ -136,8 +151,16 @@ __global__ void __launch_bounds__(kDT, 4 - DParts<IT>::in) k_delta_prep(const De
       for (int y = 0; y < DK / 32; ++y) {  // key tile kt, step s of tokens
         const int kt = w + 4 * (y / 2), s = y % 2, row = 4 * kg + r16 / 4;
         const int lo = ((2 * s * KS + kt / 2) * 64 + (lane % 4) * 16 + row) * 8 + 4 * (kt % 2), hi = lo + KS * 64 * 8;
-        *(bf8 *)(gKt + n * kC * DK + (2 * kt + s) * 512 + (unsigned)(lane * 8)) = read_tr(&Kf[n][lo], &Kf[n][hi]);
-        if (BWD) *(bf8 *)(gQt + n * kC * DK + (2 * kt + s) * 512 + (unsigned)(lane * 8)) = read_tr(&Qf[BWD ? n : 0][lo], &Qf[BWD ? n : 0][hi]);
+        bf8 k = read_tr(&Kf[n][lo], &Kf[n][hi]);
+        if (BWD) {
+          bf8 q = read_tr(&Qf[BWD ? n : 0][lo], &Qf[BWD ? n : 0][hi]);
+          if (__builtin_expect(__builtin_amdgcn_ballot_w64(odd_halves(k) | odd_halves(q)) != 0, 0)) {
+            k = without_odd(k);
+            q = without_odd(q);
+          }
+          *(bf8 *)(gQt + n * kC * DK + (2 * kt + s) * 512 + (unsigned)(lane * 8)) = q;
+        }
+        *(bf8 *)(gKt + n * kC * DK + (2 * kt + s) * 512 + (unsigned)(lane * 8)) = k;
       }
     }
   }
@@ -209,6 +232,18 @@ __global__ void __launch_bounds__(kDT, 4 - DParts<IT>::in) k_delta_prep(const De
 #pragma unroll
       for (int j = 0; j < i; ++j) s = fmaf(-D[i * FP + j], x[j], s);
       x[i] = s;
+    }
+    float sum = 0;
+#pragma unroll
+    for (int i = 0; i < 16; ++i) sum += fabsf(x[i]);
+    if (__builtin_expect(__builtin_amdgcn_ballot_w64(!(sum < INFINITY)) != 0, 0)) {  // a column's zeros above the diagonal left out
+#pragma unroll
+      for (int i = 0; i < 16; ++i) {
+        float s = i == r16 ? 1.0f : 0.0f;
+#pragma unroll
+        for (int j = 0; j < i; ++j) s = j < r16 ? s : fmaf(-D[i * FP + j], x[j], s);
+        x[i] = s;
+      }
     }
     wave_lds_sync();
     if (kg == 0) {

@@ -111,12 +111,21 @@ __global__ void __launch_bounds__(2 * kDT) SSM_TWO_WAVES k_delta_bwd(const Delta
 #pragma unroll
           for (int n = 0; n < NV; ++n) x[n] = mma<NM>(X[n][s], T[s], x[n]);
         }
+      auto put_r = [&] {
 #pragma unroll
-      for (int n = 0; n < NV; ++n) {
-        Yt[n].put(tok, kg, by * x[n]);
-        Zt[n][me] = x[n];
-      }
+        for (int n = 0; n < NV; ++n) {
+          Yt[n].put(tok, kg, by * x[n]);
+          Zt[n][me] = x[n];
+        }
+      };
+      put_r();
       load_t(next);
+      if (__builtin_expect(not_finite(x), 0)) {
+#pragma unroll
+        for (int n = 0; n < NV; ++n)
+          x[n] = row_times<NM>((const __bf16 *)p.fT + at(c) * NM * kFrag, tok, tok + 1, kC, Xt[n], kg, Xt[n].value(tok, kg));
+        put_r();
+      }
       lds_barrier();
 #pragma unroll
       for (int n = 0; n < NV; ++n)
@@ -134,17 +143,19 @@ __global__ void __launch_bounds__(2 * kDT) SSM_TWO_WAVES k_delta_bwd(const Delta
       read_ahead<2 * NM * 2 * NV, 2 * products(NM, NM, NK) * RT * NV, 12>();
       load_cols(p.fKt, next, Kt);
     }
-    if (p.dh0) {
 #pragma unroll
-      for (int n = 0; n < NV; ++n)
+    for (int n = 0; n < NV; ++n)
 #pragma unroll
-        for (int r = 0; r < RT; ++r) {
-          const int key = 16 * (RT * w + r) + r16;
+      for (int r = 0; r < RT; ++r) {
+        const int key = 16 * (RT * w + r) + r16;
+        if (key < p.Dkp && vt + n < p.VT)  // behind the chunks' own
+          *(f4 *)(state_of(p.dstates, p, at(p.NC), vt + n) + (unsigned)(16 * key + 4 * kg)) = D[n][r];
+        if (p.dh0) {
 #pragma unroll
           for (int i = 0; i < 4; ++i)
             if (key < p.Dk && 16 * n + i < have) p.dh0[((int64_t)bh * p.Dk + key) * p.Dv + v0 + 16 * n + i] = D[n][r][i];
         }
-    }
+      }
   } else {
     const IT *dop = (const IT *)p.dout.p + b * p.dout.s0 + h * p.dout.s2 + v0;
     IT *dvp = (IT *)p.dv.p + b * p.dv.s0 + h * p.dv.s2 + v0;
@@ -170,7 +181,7 @@ __global__ void __launch_bounds__(2 * kDT) SSM_TWO_WAVES k_delta_bwd(const Delta
         Ot[n].put_parts(tok, kg, o);
       }
     };
-    auto make_g = [&] {
+    auto make_g = [&](int c) {
       f4 g[NV];
 #pragma unroll
       for (int n = 0; n < NV; ++n) g[n] = 0;
@@ -184,6 +195,11 @@ __global__ void __launch_bounds__(2 * kDT) SSM_TWO_WAVES k_delta_bwd(const Delta
             g[n] = mma<NM>(A, P[s], g[n]);
           }
         }
+      if (__builtin_expect(not_finite(g), 0)) {
+#pragma unroll
+        for (int n = 0; n < NV; ++n)
+          g[n] = row_times<NM>((const __bf16 *)p.fP + at(c) * NM * kFrag, tok, tok, kC, Ot[n], kg, (f4)0.0f);
+      }
 #pragma unroll
       for (int n = 0; n < NV; ++n) Gt[n][me] = g[n];
     };
@@ -194,7 +210,7 @@ __global__ void __launch_bounds__(2 * kDT) SSM_TWO_WAVES k_delta_bwd(const Delta
     put_o(p.NC - 1, go);
     load_o(p.NC > 1 ? p.NC - 2 : 0, next_go);
     lds_barrier();
-    make_g();
+    make_g(p.NC - 1);
     load_p(p.NC > 1 ? p.NC - 2 : 0);
     for (int c = p.NC - 1; c >= 0; --c) {
       const int64_t t = (int64_t)c * kC + tok;
@@ -233,7 +249,7 @@ __global__ void __launch_bounds__(2 * kDT) SSM_TWO_WAVES k_delta_bwd(const Delta
       for (int n = 0; n < NV; ++n)
 #pragma unroll
         for (int r = 0; r < RT; ++r) Rt[n][r][me] = R[n][r];
-      make_g();
+      make_g(next);
       load_cols(p.fQt, next, Qt);
       load_p(after);
       lds_barrier();
@@ -543,16 +559,30 @@ __global__ void __launch_bounds__(4 * DK) SSM_TWO_WAVES k_delta_grad(const Delta
     }
     lds_barrier();
     if (w == 0) {  // dbeta and dg of the head
-      double s = 0, k = 0, ss = 0;
+      double s = 0, k = 0, ss = 0;  // s of token 63 - lane, k of token lane - 1
 #pragma unroll
       for (int n = 0; n < NW; ++n) {
-        s += red[n][0][lane];
-        k += red[n][1][lane];
+        s += red[n][0][63 - lane];
+        k += lane ? red[n][1][lane - 1] : 0.0f;
         ss += sdot[n];
       }
-      // the sum from t on is the whole less what is before t
-      const double upto = wave_scan_f64(s), before = wave_scan_f64(k) - k;
-      const double from = (__shfl(upto, 63) - upto) + s + before + (double)rows[3] * ss;
+      double rest = __shfl(wave_scan_f64(s), 63 - lane);  // sum over i >= t of dG_i
+      if (__builtin_expect(__builtin_amdgcn_ballot_w64(!(fabs(rest) < INFINITY)) != 0, 0)) {
+        // A pair after t is in rows and columns of the sum and cancels, but not where it is infinite or NaN.  The sum of
+        // all tokens less those before t is the same from finite terms: in that of all every pair cancels, and what is
+        // left is the entering state's share, <S0, dS0 - e^{G_C} D>.
+        const float *S = state_of(p.states, p, ch, 0), *D = state_of(p.dstates, p, ch, 0);
+        const float *E = state_of(p.dstates, p, c ? ch - p.B * p.H : ch + (int64_t)p.NC * p.B * p.H, 0);
+        double g = 0, all = 0;
+#pragma unroll
+        for (int n = 0; n < NW; ++n) g += lane ? red[n][0][lane - 1] : 0.0f;
+#pragma unroll 1
+        for (int64_t i = lane; i < (int64_t)p.VT * p.Dkp * 16; i += 64) all += S[i] * ((double)E[i] - (double)rows[3] * D[i]);
+        all = __shfl(wave_scan_f64(all), 63);
+        const double less = all - wave_scan_f64(g);
+        if (!(fabs(rest) < INFINITY)) rest = less;
+      }
+      const double from = rest + wave_scan_f64(k) + (double)rows[3] * ss;
       const int64_t t = t0 + lane;
       if (t < p.L) {
         ((float *)p.dg.p)[b * p.dg.s0 + t * p.dg.s1 + h * p.dg.s2] = (float)from;

@@ -314,7 +314,7 @@ struct DeltaParams {
   float *states, *y;                   // saved: (NC, B H, VT, Dkp, 16) entering states, (NC, B H, VT, 64, 16) Y
   KView dout, dq, dk, dv, dg, dbeta;
   const float *dlast;
-  float *dh0, *dstates, *dr;           // gradients of the leaving states and dR, laid out as states and y
+  float *dh0, *dstates, *dr;           // gradients of the leaving states (the first chunk's entering one last) and dR, laid out as states and y
   int64_t first;                       // walks: workgroups of earlier launches
 };
 // Chunks of all heads together: what is taken chunk by chunk is one launch of at most 512 threads each.  More have

@@ -29,7 +29,8 @@ def gated_delta_rule(q, k, v, g, beta, h0=None, scale=None, qk_norm=False, retur
     token, zeros if None.  scale: Dk^-0.5 if None.  qk_norm divides q and k by sqrt(sum of squares + 1e-6)
     over Dk first.  An infinity or NaN reaches what the recurrence takes it to: outputs from its own token on
     (in v, those of its column), never those of earlier tokens, so that the end of a padded row may hold anything;
-    an infinity may come out as NaN."""
+    an infinity may come out as NaN.  Gradients follow the adjoint likewise, but for one in g, which makes all of
+    its 64 tokens' NaN."""
     scale = float(q.shape[-1] ** -0.5 if scale is None else scale)
     if v.dim() == 4 and v.numel() == 0 and v.shape[2] and v.shape[3]:   # no token: the state passes through
         _abi.host().delta_checks(q, k, v, g, beta, h0)

@@ -74,3 +74,38 @@ def test_a_state_that_is_not_finite_stays_in_its_columns(dev):
     want_o, want_last = delta_ref.delta(**a, qk_norm=True)
     same("o", o, want_o, F32)
     same("last", last, want_last, F32)
+
+
+# one element of token t of the first batch row and head in an operand or the outputs' gradient; the first and last
+# tokens of a chunk and of its blocks of 16 and 32, a second chunk, the end
+@pytest.mark.parametrize("t", [0, 5, 31, 40, 63, 64, 107, 149])
+@pytest.mark.parametrize("name,bad", [("q", INF), ("q", NAN), ("k", INF), ("k", NAN), ("v", INF), ("v", NAN), ("beta", NAN), ("do", INF), ("do", NAN)])
+@pytest.mark.parametrize("io", [F32, BF16, F16])
+def test_gradients(dev, io, name, bad, t):
+    for shape, norm in (((2, 150, 1, 2, 128, 20), False), ((2, 150, 2, 2, 40, 48), name in ("v", "do"))):
+        a, do, dl = make(dev, *shape, io, seed=74, norm=norm)
+        if name == "do":
+            do[0, t, 0, 3] = bad
+        else:
+            put(a, name, t, bad)
+        a = {n: x.requires_grad_() for n, x in a.items()}
+        o, last = ssm_scan.gated_delta_rule(**a, qk_norm=norm, return_last_state=True)
+        grads = torch.autograd.grad([o, last], list(a.values()), [do, dl])
+        _, _, want = delta_ref.delta(**a, qk_norm=norm, dout=do, dlast=dl)
+        for n, d in zip(a, grads):
+            same("d" + n, d, want[n], io if d.dtype == io else BF16 if io == BF16 else F16, grad=True)
+
+
+def test_gradients_over_pairs_of_tiles(dev):
+    """Rows of several lengths whose ends hold anything in v and a gradient of zeros: what is before them is right."""
+    B, L, H = 14, 130, 4
+    a, do, dl = make(dev, B, L, 2, H, 64, 72, F32, seed=75)
+    for b, n in enumerate([1, 2, 15, 16, 17, 31, 33, 47, 63, 64, 65, 100, 129, 130]):
+        a["v"][b, n:] = NAN
+        do[b, n:] = 0
+    a = {n: x.requires_grad_() for n, x in a.items()}
+    o = ssm_scan.gated_delta_rule(**a, qk_norm=True)
+    grads = torch.autograd.grad(o, list(a.values()), do)
+    _, _, want = delta_ref.delta(**a, qk_norm=True, dout=do)
+    for n, d in zip(a, grads):
+        same("d" + n, d, want[n], F32, grad=True)
