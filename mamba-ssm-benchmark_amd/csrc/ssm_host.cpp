@@ -501,12 +501,18 @@ bool needs_grad(std::initializer_list<const Tensor *> ts) {
     if (t->defined() && t->requires_grad()) return true;
   return false;
 }
+// A dual tensor need not require a gradient: without this its tangent would be left out where no node is made.
+void no_tangents(std::initializer_list<const Tensor *> ts, const char *what) {
+  for (const Tensor *t : ts)
+    TORCH_CHECK_NOT_IMPLEMENTED(!t->defined() || !t->_fw_grad(0).defined(), what, " has no forward-mode derivative");
+}
 bool delta_type(at::ScalarType t) { return t == at::kFloat || t == at::kBFloat16 || t == at::kHalf; }
 
 // Shapes and types of one call; `lead` = (B, L) of the chunked form, (B,) of the step.
 void delta_checks(const Tensor &q, const Tensor &k, const Tensor &v, const Tensor &g, const Tensor &beta, const Tensor &h,
                   int64_t lead) {
   require_gpu({&q, &k, &v, &g, &beta, &h});
+  no_tangents({&q, &k, &v, &g, &beta, &h}, "the gated delta rule");
   for (const Tensor *t : {&k, &v, &g, &beta, &h})
     TORCH_CHECK_VALUE(!t->defined() || t->device() == q.device(), "tensors on ", q.device().str(), " and ",
                       t->device().str());
@@ -698,6 +704,7 @@ variable_list gnorm_forward(const Tensor &x, const OptTensor &weight, const OptT
                             int64_t groups, int64_t act, bool center, double eps) {
   const Tensor g = get(gate), w_ = get(weight), b_ = get(bias);
   require_gpu({&x, &g, &w_, &b_});
+  no_tangents({&x, &g, &w_, &b_}, "group_norm");
   TORCH_CHECK_VALUE(x.dim() >= 1 && x.size(-1) > 0 && groups > 0 && x.size(-1) % groups == 0, "the last dimension of x, ",
                     shape_str(x.sizes()), ", is not ", groups, " whole groups");
   TORCH_CHECK_TYPE(delta_type(x.scalar_type()), "group_norm takes float32, bfloat16 or float16, got ", x.scalar_type());
