@@ -8,6 +8,8 @@
 // Errors of the C ABI become the exception classes of ssm_scan._abi.check.
 #include <torch/csrc/Exceptions.h>
 #include <torch/csrc/autograd/custom_function.h>
+#include <torch/csrc/autograd/function.h>
+#include <torch/csrc/autograd/functions/utils.h>
 #include <torch/csrc/utils/pybind.h>
 
 #include <ATen/ATen.h>
@@ -506,6 +508,23 @@ void no_tangents(std::initializer_list<const Tensor *> ts, const char *what) {
   for (const Tensor *t : ts)
     TORCH_CHECK_NOT_IMPLEMENTED(!t->defined() || !t->_fw_grad(0).defined(), what, " has no forward-mode derivative");
 }
+// The gradients of a backward that has itself no derivative: under create_graph they carry a node over the inputs and
+// the outputs' gradients that refuses, where without one they would pass for constants.
+struct Twice : torch::autograd::Node {
+  const char *what;
+  Twice(const char *w, torch::autograd::edge_list next) : Node(std::move(next)), what(w) {}
+  variable_list apply(variable_list &&) override {
+    TORCH_CHECK(false, what, " cannot be differentiated twice");
+  }
+};
+void not_twice(variable_list &d, const variable_list &douts, const char *what) {
+  if (!at::GradMode::is_enabled()) return;
+  torch::autograd::edge_list next = torch::autograd::get_current_node()->next_edges();
+  for (const torch::autograd::Edge &e : torch::autograd::collect_next_edges(douts)) next.push_back(e);
+  const auto node = std::make_shared<Twice>(what, std::move(next));
+  for (Tensor &t : d)
+    if (t.defined()) torch::autograd::set_history(t, node);
+}
 bool delta_type(at::ScalarType t) { return t == at::kFloat || t == at::kBFloat16 || t == at::kHalf; }
 
 // Shapes and types of one call; `lead` = (B, L) of the chunked form, (B,) of the step.
@@ -648,6 +667,7 @@ struct DeltaFn : torch::autograd::Function<DeltaFn> {
                                      ctx->saved_data["h0"].toBool() && ctx->needs_input_grad(5));
     const auto types = ctx->saved_data["types"].toIntVector();
     for (size_t i = 0; i < d.size(); ++i) d[i] = cast(d[i], (at::ScalarType)types[i]);
+    not_twice(d, grads, "the gated delta rule");
     d.resize(9);
     return d;
   }
@@ -770,6 +790,7 @@ struct GnormFn : torch::autograd::Function<GnormFn> {
                                      ctx->saved_data["eps"].toDouble(), dw, db);
     const auto types = ctx->saved_data["types"].toIntVector();
     for (size_t i = 0; i < d.size(); ++i) d[i] = cast(d[i], (at::ScalarType)types[i]);
+    not_twice(d, grads, "group_norm");
     d.resize(8);
     return d;
   }

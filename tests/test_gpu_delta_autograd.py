@@ -33,3 +33,54 @@ def test_forward_mode_of_the_norm_is_refused(dev, name):
         a[name] = fwd.make_dual(a[name], torch.ones_like(a[name]))
         with pytest.raises(NotImplementedError, match="forward-mode"):
             ssm_scan.group_norm(groups=2, **a)
+
+
+def test_a_second_derivative_is_refused(dev):
+    """First gradients are the same under create_graph; differentiating them raises, by every way to the leaves."""
+    a, do, dl = make(dev, 1, 70, 1, 2, 16, 8, F32)
+    leaves = [t.requires_grad_() for t in a.values()] + [do.requires_grad_()]
+
+    def grads(create_graph):
+        o, last = ssm_scan.gated_delta_rule(**a, qk_norm=True, return_last_state=True)
+        return torch.autograd.grad([o, last], list(a.values()), [do, dl], create_graph=create_graph)
+
+    once, graph = grads(False), grads(True)
+    assert all(torch.equal(x, y) and not x.requires_grad and y.requires_grad for x, y in zip(once, graph))
+    for g in graph:
+        for leaf in leaves:
+            with pytest.raises(RuntimeError, match="twice"):
+                torch.autograd.grad(g.sum() + 0 * leaf.sum(), leaf, retain_graph=True)
+        with pytest.raises(RuntimeError, match="twice"):
+            g.sum().backward(retain_graph=True)
+
+
+def test_a_second_derivative_through_casts_is_refused(dev):
+    """Operands that the kernels read as copies."""
+    a, do, _ = make(dev, 1, 20, 1, 2, 16, 8, BF16)
+    a["v"], a["g"] = a["v"].float().requires_grad_(), a["g"].double().requires_grad_()
+    o = ssm_scan.gated_delta_rule(**a)
+    dv, dg = torch.autograd.grad(o, [a["v"], a["g"]], do.float(), create_graph=True)
+    for d in (dv, dg):
+        for leaf in (a["v"], a["g"]):
+            with pytest.raises(RuntimeError, match="twice"):
+                torch.autograd.grad(d.sum(), leaf, retain_graph=True)
+
+
+def test_a_second_derivative_of_the_norm_is_refused(dev):
+    x, w, b, gate = (torch.randn(s, device=dev).requires_grad_() for s in ((3, 8), (8,), (8,), (3, 8)))
+    dy = torch.randn(3, 8, device=dev).requires_grad_()
+    leaves = [x, w, b, gate]
+
+    def grads(create_graph):
+        return torch.autograd.grad(ssm_scan.group_norm(x, 2, w, b, gate=gate), leaves, dy, create_graph=create_graph)
+
+    once, graph = grads(False), grads(True)
+    assert all(torch.equal(p, q) and not p.requires_grad and q.requires_grad for p, q in zip(once, graph))
+    for g in graph:
+        for leaf in leaves + [dy]:
+            with pytest.raises(RuntimeError, match="twice"):
+                torch.autograd.grad(g.sum(), leaf, retain_graph=True)
+    # only the weight's: the others have no gradient at all
+    d = torch.autograd.grad(ssm_scan.group_norm(x.detach(), 2, w), w, dy.detach(), create_graph=True)[0]
+    with pytest.raises(RuntimeError, match="twice"):
+        torch.autograd.grad(d.sum(), w)
