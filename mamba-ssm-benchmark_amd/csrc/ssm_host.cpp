@@ -688,6 +688,8 @@ Tensor delta_step(const Tensor &h, const Tensor &q_, const Tensor &k_, const Ten
   delta_checks(q_, k_, v_, g_, beta_, h, 1);
   TORCH_CHECK_VALUE(h.scalar_type() == at::kFloat && h.is_contiguous(), "the state must be contiguous float32, got ",
                     h.scalar_type(), " with strides ", h.strides());
+  TORCH_CHECK(!needs_grad({&h, &q_, &k_, &v_, &g_, &beta_}),
+              "gated_delta_step is not differentiable, as it updates its state in place: call it under torch.no_grad()");
   const DeltaOps t(q_, k_, v_, g_, beta_);
   const Tensor o = at::empty(t.v.sizes(), t.v.options());
   ssm_delta_step_args a;
@@ -696,6 +698,7 @@ Tensor delta_step(const Tensor &h, const Tensor &q_, const Tensor &k_, const Ten
   a.out = lead_view(o, 2);
   const Launch l(o);
   l.run_anywhere("ssm_delta_step", ssm_delta_step, a);
+  if (!h.is_inference()) h.unsafeGetTensorImpl()->bump_version();
   return o.scalar_type() == v_.scalar_type() ? o : o.to(v_.scalar_type());
 }
 

@@ -7,8 +7,8 @@ Per batch row and value head, with S (Dk, Dv):
     S' = e^{g_t} S_{t-1}      u_t = beta_t (v_t - S'^T k_t)      S_t = S' + k_t u_t^T
     o_t = scale S_t^T q_t
 
-``gated_delta_rule`` runs whole sequences (training, prefill; differentiable in every tensor),
-``gated_delta_step`` one token per stream.  Key heads may be fewer than value heads (value head h
+``gated_delta_rule`` runs whole sequences (training, prefill; differentiable once in every tensor, in
+reverse mode), ``gated_delta_step`` one token per stream.  Key heads may be fewer than value heads (value head h
 reads key head h // (H // Hk)); their gradients are summed over the heads that share them.
 Products run on the matrix cores over bf16 parts of the operands (one part for bf16 inputs, two
 for fp16, three for float32 inputs and for the float32 intermediates); states,
@@ -43,6 +43,7 @@ def gated_delta_rule(q, k, v, g, beta, h0=None, scale=None, qk_norm=False, retur
 
 def gated_delta_step(h, q, k, v, g, beta, scale=None, qk_norm=False):
     """One token per stream: o (B, H, Dv) in v's dtype; h (B, H, Dk, Dv), contiguous float32, is updated
-    in place.  q, k (B, Hk, Dk), v (B, H, Dv), g and beta (B, H) as in gated_delta_rule."""
+    in place.  q, k (B, Hk, Dk), v (B, H, Dv), g and beta (B, H) as in gated_delta_rule.  Not differentiable: in
+    grad mode, operands that require a gradient are refused."""
     scale = float(q.shape[-1] ** -0.5 if scale is None else scale)
     return _abi.host().delta_step(h, q, k, v, g, beta, scale, bool(qk_norm))

@@ -84,3 +84,31 @@ def test_a_second_derivative_of_the_norm_is_refused(dev):
     d = torch.autograd.grad(ssm_scan.group_norm(x.detach(), 2, w), w, dy.detach(), create_graph=True)[0]
     with pytest.raises(RuntimeError, match="twice"):
         torch.autograd.grad(d.sum(), w)
+
+
+@pytest.mark.parametrize("name", ["h0", "q", "k", "v", "g", "beta"])
+def test_a_step_that_would_lose_a_gradient_is_refused(dev, name):
+    a, _, _ = make(dev, 2, 1, 1, 2, 16, 8, F32)
+    one = {n: t if n == "h0" else t[:, 0] for n, t in a.items()}
+    h, ops = one["h0"].clone(), ("q", "k", "v", "g", "beta")
+    want = ssm_scan.gated_delta_step(h, *(one[n] for n in ops))
+    one[name] = one[name].detach().requires_grad_()
+    before = one["h0"].detach().clone()
+    with pytest.raises(RuntimeError, match="not differentiable"):
+        ssm_scan.gated_delta_step(one["h0"], *(one[n] for n in ops))
+    assert torch.equal(one["h0"], before)
+    with torch.no_grad():
+        assert torch.equal(ssm_scan.gated_delta_step(one["h0"], *(one[n] for n in ops)), want)
+    assert torch.equal(one["h0"].detach(), h)
+
+
+def test_a_step_counts_as_a_change_of_its_state(dev):
+    """A graph that has kept the state finds it changed, as after any operation in place."""
+    a, _, _ = make(dev, 2, 1, 1, 2, 16, 8, F32)
+    w = torch.ones_like(a["h0"]).requires_grad_()
+    y = (w * a["h0"]).sum()
+    ssm_scan.gated_delta_step(a["h0"], *(a[n][:, 0] for n in ("q", "k", "v", "g", "beta")))
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        y.backward()
+    with torch.inference_mode():
+        ssm_scan.gated_delta_step(torch.zeros_like(a["h0"]), *(a[n][:, 0] for n in ("q", "k", "v", "g", "beta")))
