@@ -28,7 +28,8 @@ from .linear import linear
 class GatedDeltaMixer(nn.Module):
     """(B, L, d_model) -> (B, L, d_model).  heads value heads of value_dim, key_heads (dividing heads; all
     by default) of key_dim <= 128.  With a state (init_state) the call continues the sequence and updates
-    it; one token per call is the decode step, without autograd as the state changes in place."""
+    it, one token per call being the decode step.  The states change in place, so such a call is inference: it
+    runs without autograd whatever the grad mode, and its output has no graph."""
 
     def __init__(self, d_model, heads, key_dim, value_dim=None, key_heads=None, d_conv=4, dt_min=1e-3, dt_max=0.1):
         super().__init__()
@@ -52,6 +53,10 @@ class GatedDeltaMixer(nn.Module):
             delta=torch.zeros(batch, self.heads, self.key_dim, self.value_dim, device=device))
 
     def forward(self, u, state=None):
+        with torch.set_grad_enabled(torch.is_grad_enabled() and state is None):
+            return self._forward(u, state)
+
+    def _forward(self, u, state):
         mixed, z, dt, b = linear(self.in_proj, u).split(
             [2 * self.d_keys + self.d_values, self.d_values, self.heads, self.heads], dim=-1)
         mixed = causal_conv1d(mixed, self.conv.weight, self.conv.bias, state=None if state is None else state.conv)

@@ -1,0 +1,25 @@
+"""GatedDeltaMixer with a state is inference, whatever the grad mode: outputs and states without a graph."""
+
+import pytest
+import torch
+
+from ssm_scan.delta_mixer import GatedDeltaMixer
+
+pytestmark = pytest.mark.gpu
+
+
+@pytest.mark.parametrize("pieces", [(5, 1, 3), (1, 1), (7,)])
+def test_no_graph_with_a_state(dev, pieces):
+    torch.manual_seed(0)
+    m = GatedDeltaMixer(d_model=64, heads=4, key_dim=16, value_dim=24, key_heads=2).to(dev)
+    u = torch.randn(2, sum(pieces), 64, device=dev, requires_grad=True)
+    with torch.no_grad():
+        want = m(u)
+    state, outs, t = m.init_state(2, dev), [], 0
+    for n in pieces:
+        outs.append(m(u[:, t:t + n], state))
+        t += n
+        assert not outs[-1].requires_grad and not state.delta.requires_grad and not state.conv.requires_grad
+    # two float32 GEMMs, the conv, the rule and the norm: 2^-15 of the largest output
+    assert (torch.cat(outs, 1) - want).abs().max().item() <= 2.0 ** -15 * want.abs().max().item()
+    assert torch.is_grad_enabled() and m(u).requires_grad   # without a state it is trained
