@@ -690,6 +690,7 @@ Tensor delta_step(const Tensor &h, const Tensor &q_, const Tensor &k_, const Ten
                     h.scalar_type(), " with strides ", h.strides());
   TORCH_CHECK(!needs_grad({&h, &q_, &k_, &v_, &g_, &beta_}),
               "gated_delta_step is not differentiable, as it updates its state in place: call it under torch.no_grad()");
+  if (h.size(0) == 0) return at::empty(v_.sizes(), v_.options());  // no stream
   const DeltaOps t(q_, k_, v_, g_, beta_);
   const Tensor o = at::empty(t.v.sizes(), t.v.options());
   ssm_delta_step_args a;

@@ -35,8 +35,9 @@ def gated_delta_rule(q, k, v, g, beta, h0=None, scale=None, qk_norm=False, retur
     if v.dim() == 4 and v.numel() == 0 and v.shape[2] and v.shape[3]:   # no token: the state passes through
         _abi.host().delta_checks(q, k, v, g, beta, h0)
         last = v.new_zeros((v.shape[0], v.shape[2], q.shape[-1], v.shape[3]), dtype=torch.float32) if h0 is None \
-            else h0.float()
-        return (v * 1, last) if return_last_state else v * 1
+            else h0.float() * 1
+        o = v * sum((t.sum() for t in (q, k, g, beta)), v.new_ones(())).to(v.dtype)   # in every operand's graph
+        return (o, last) if return_last_state else o
     o, last = _abi.host().delta(q, k, v, g, beta, h0, scale, bool(qk_norm), bool(return_last_state))
     return (o, last) if return_last_state else o
 

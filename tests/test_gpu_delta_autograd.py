@@ -112,3 +112,28 @@ def test_a_step_counts_as_a_change_of_its_state(dev):
         y.backward()
     with torch.inference_mode():
         ssm_scan.gated_delta_step(torch.zeros_like(a["h0"]), *(a[n][:, 0] for n in ("q", "k", "v", "g", "beta")))
+
+
+@pytest.mark.parametrize("empty", ["B", "L"])
+def test_no_tokens_give_new_tensors_in_the_graph(dev, empty):
+    """No batch rows or no tokens: o and last are new tensors, and every operand has its (empty or passed on) gradient."""
+    a, _, _ = make(dev, 2, 3, 1, 2, 16, 8, F32)
+    a = {n: (t[:0] if empty == "B" else t if n == "h0" else t[:, :0]).detach().requires_grad_() for n, t in a.items()}
+    o, last = ssm_scan.gated_delta_rule(**a, return_last_state=True)
+    assert torch.equal(last, a["h0"]) and last.data_ptr() != a["h0"].data_ptr() or not last.numel()
+    assert o.dtype == a["v"].dtype and o.shape == a["v"].shape
+    grads = torch.autograd.grad([o, last], list(a.values()), [torch.ones_like(o), torch.full_like(last, 3.0)])
+    for n, d in zip(a, grads):
+        assert d.shape == a[n].shape and d.dtype == a[n].dtype and bool((d == 3).all())
+    with torch.no_grad():
+        last = ssm_scan.gated_delta_rule(**a, return_last_state=True)[1]
+        last.zero_()
+    assert a["h0"].any() or not a["h0"].numel()
+
+
+def test_no_streams_to_step(dev):
+    a, _, _ = make(dev, 2, 1, 1, 2, 16, 8, BF16)
+    o = ssm_scan.gated_delta_step(a["h0"][:0], *(a[n][:0, 0] for n in ("q", "k", "v", "g", "beta")))
+    assert o.shape == (0, 2, 8) and o.dtype == BF16
+    with pytest.raises(ValueError):   # checked all the same
+        ssm_scan.gated_delta_step(a["h0"][:0], *(a[n][:0, 0] for n in ("q", "k", "v", "g")), a["beta"][:1, 0])
