@@ -723,10 +723,7 @@ ssm_gnorm_args gnorm_args(const Tensor &x2, const Tensor &w, const Tensor &b, co
 }
 Tensor f32(const OptTensor &t) { return t ? cast(*t, at::kFloat).contiguous() : Tensor(); }
 
-// y, x as rows, weight, bias, gate as rows
-variable_list gnorm_forward(const Tensor &x, const OptTensor &weight, const OptTensor &bias, const OptTensor &gate,
-                            int64_t groups, int64_t act, bool center, double eps) {
-  const Tensor g = get(gate), w_ = get(weight), b_ = get(bias);
+void gnorm_checks(const Tensor &x, const Tensor &w_, const Tensor &b_, const Tensor &g, int64_t groups) {
   require_gpu({&x, &g, &w_, &b_});
   no_tangents({&x, &g, &w_, &b_}, "group_norm");
   TORCH_CHECK_VALUE(x.dim() >= 1 && x.size(-1) > 0 && groups > 0 && x.size(-1) % groups == 0, "the last dimension of x, ",
@@ -735,6 +732,11 @@ variable_list gnorm_forward(const Tensor &x, const OptTensor &weight, const OptT
   want("weight", w_, {x.size(-1)});
   want("bias", b_, {x.size(-1)});
   want("gate", g, x.sizes());
+}
+// y, x as rows, weight, bias, gate as rows
+variable_list gnorm_forward(const Tensor &x, const OptTensor &weight, const OptTensor &bias, const OptTensor &gate,
+                            int64_t groups, int64_t act, bool center, double eps) {
+  const Tensor g = get(gate);
   const Tensor x2 = rows(x, x.size(-1)), w = f32(weight), b = f32(bias);
   const Tensor g2 = g.defined() ? rows(cast(g, x.scalar_type()), x.size(-1)) : g;
   const Tensor o = at::empty(x2.sizes(), x2.options());
@@ -802,6 +804,13 @@ struct GnormFn : torch::autograd::Function<GnormFn> {
 Tensor gnorm(const Tensor &x, const OptTensor &weight, const OptTensor &bias, const OptTensor &gate, int64_t groups, int64_t act,
              bool center, double eps) {
   const Tensor w = get(weight), b = get(bias), g = get(gate);
+  gnorm_checks(x, w, b, g, groups);
+  if (x.numel() == 0) {  // no rows: an empty tensor in the graph of what was given
+    Tensor y = x * 1;
+    for (const Tensor *t : {&w, &b, &g})
+      if (t->defined()) y = y * *t;
+    return cast(y, x.scalar_type());
+  }
   if (!needs_grad({&x, &w, &b, &g})) return gnorm_forward(x, weight, bias, gate, groups, act, center, eps)[0];
   return GnormFn::apply(x, weight, bias, gate, groups, act, center, eps);
 }

@@ -137,3 +137,17 @@ def test_no_streams_to_step(dev):
     assert o.shape == (0, 2, 8) and o.dtype == BF16
     with pytest.raises(ValueError):   # checked all the same
         ssm_scan.gated_delta_step(a["h0"][:0], *(a[n][:0, 0] for n in ("q", "k", "v", "g")), a["beta"][:1, 0])
+
+
+def test_a_norm_of_no_rows_is_checked_and_in_the_graph(dev):
+    x, gate = (torch.zeros(0, 5, 32, device=dev, dtype=BF16).requires_grad_() for _ in range(2))
+    w, b = (torch.ones(32, device=dev).requires_grad_() for _ in range(2))
+    y = ssm_scan.group_norm(x, 4, w, b, gate=gate)
+    assert y.shape == x.shape and y.dtype == BF16
+    for t, d in zip((x, w, b, gate), torch.autograd.grad(y, (x, w, b, gate), torch.ones_like(y))):
+        assert d.shape == t.shape and d.dtype == t.dtype and not d.any()
+    for kw in (dict(groups=5), dict(groups=0), dict(groups=4, weight=w[:8]), dict(groups=4, gate=gate[:, :2])):
+        with pytest.raises(ValueError):
+            ssm_scan.group_norm(x, **kw)
+    with pytest.raises(TypeError):
+        ssm_scan.group_norm(x.double(), 4)
