@@ -525,6 +525,10 @@ void not_twice(variable_list &d, const variable_list &douts, const char *what) {
   for (Tensor &t : d)
     if (t.defined()) torch::autograd::set_history(t, node);
 }
+void one_device(const Tensor &x, std::initializer_list<const Tensor *> ts) {
+  for (const Tensor *t : ts)
+    TORCH_CHECK_VALUE(!t->defined() || t->device() == x.device(), "tensors on ", x.device().str(), " and ", t->device().str());
+}
 bool delta_type(at::ScalarType t) { return t == at::kFloat || t == at::kBFloat16 || t == at::kHalf; }
 
 // Shapes and types of one call; `lead` = (B, L) of the chunked form, (B,) of the step.
@@ -532,9 +536,7 @@ void delta_checks(const Tensor &q, const Tensor &k, const Tensor &v, const Tenso
                   int64_t lead) {
   require_gpu({&q, &k, &v, &g, &beta, &h});
   no_tangents({&q, &k, &v, &g, &beta, &h}, "the gated delta rule");
-  for (const Tensor *t : {&k, &v, &g, &beta, &h})
-    TORCH_CHECK_VALUE(!t->defined() || t->device() == q.device(), "tensors on ", q.device().str(), " and ",
-                      t->device().str());
+  one_device(q, {&k, &v, &g, &beta, &h});
   const char *const form = lead == 2 ? "(B, L, H, D)" : "(B, H, D)";
   for (const Tensor *t : {&q, &k, &v})
     TORCH_CHECK_VALUE(t->dim() == lead + 2, "q, k and v must be ", form, ", got ", shape_str(t->sizes()));
@@ -725,6 +727,7 @@ Tensor f32(const OptTensor &t) { return t ? cast(*t, at::kFloat).contiguous() : 
 
 void gnorm_checks(const Tensor &x, const Tensor &w_, const Tensor &b_, const Tensor &g, int64_t groups) {
   require_gpu({&x, &g, &w_, &b_});
+  one_device(x, {&g, &w_, &b_});
   no_tangents({&x, &g, &w_, &b_}, "group_norm");
   TORCH_CHECK_VALUE(x.dim() >= 1 && x.size(-1) > 0 && groups > 0 && x.size(-1) % groups == 0, "the last dimension of x, ",
                     shape_str(x.sizes()), ", is not ", groups, " whole groups");

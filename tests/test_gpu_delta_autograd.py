@@ -151,3 +151,12 @@ def test_a_norm_of_no_rows_is_checked_and_in_the_graph(dev):
             ssm_scan.group_norm(x, **kw)
     with pytest.raises(TypeError):
         ssm_scan.group_norm(x.double(), 4)
+
+
+@pytest.mark.skipif(torch.cuda.device_count() < 2, reason="needs a second GPU")
+@pytest.mark.parametrize("name", ["weight", "bias", "gate"])
+def test_a_norm_over_two_devices_is_refused(dev, name):
+    a = dict(weight=torch.ones(8, device=dev), bias=torch.ones(8, device=dev), gate=torch.ones(3, 8, device=dev))
+    a[name] = a[name].to("cuda:1")
+    with pytest.raises(ValueError, match="tensors on"):
+        ssm_scan.group_norm(torch.ones(3, 8, device=dev), 2, **a)
