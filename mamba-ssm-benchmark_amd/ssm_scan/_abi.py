@@ -255,6 +255,15 @@ def lib():
 
 
 _host = None
+_timers = 0   # profiling.KernelTimers in effect
+
+
+def count_timers(change):
+    """Counts KernelTimers for the binding, which asks for the one in effect only while there are any."""
+    global _timers
+    _timers += change
+    if _host is not None:
+        _host.count_timers(change)
 
 
 def host():
@@ -271,6 +280,7 @@ def host():
         built = getattr(_ssmhost, "ABI_VERSION", None)   # compiled in: lib() has checked the library's own
         if built != ABI_VERSION:
             raise RuntimeError(f"_ssmhost was built for ABI version {built}, expected {ABI_VERSION}")
+        _ssmhost.count_timers(_timers)   # those entered before it was loaded
         _host = _ssmhost
     return _host
 

@@ -22,13 +22,13 @@ class KernelTimer:
         global _active
         self._prev = _active
         _active = self
-        _abi.host().count_timers(1)
+        _abi.count_timers(1)
         return self
 
     def __exit__(self, *exc):
         global _active
         _active = self._prev
-        _abi.host().count_timers(-1)
+        _abi.count_timers(-1)
         return False
 
     def begin(self, name):
