@@ -20,6 +20,12 @@ import torch
 from . import _abi
 
 
+def _scale(q, scale):
+    if scale is None:
+        return max(q.shape[-1], 1) ** -0.5 if q.dim() else 1.0   # no keys: the checks refuse them
+    return float(scale)
+
+
 def gated_delta_rule(q, k, v, g, beta, h0=None, scale=None, qk_norm=False, return_last_state=False):
     """o (B, L, H, Dv) in v's dtype; with return_last_state, (o, last (B, H, Dk, Dv) float32).
 
@@ -31,7 +37,7 @@ def gated_delta_rule(q, k, v, g, beta, h0=None, scale=None, qk_norm=False, retur
     (in v, those of its column), never those of earlier tokens, so that the end of a padded row may hold anything;
     an infinity may come out as NaN.  Gradients follow the adjoint likewise, but for one in g, which makes all of
     its 64 tokens' NaN."""
-    scale = float(q.shape[-1] ** -0.5 if scale is None else scale)
+    scale = _scale(q, scale)
     if v.dim() == 4 and v.numel() == 0 and v.shape[2] and v.shape[3]:   # no token: the state passes through
         _abi.host().delta_checks(q, k, v, g, beta, h0)
         last = v.new_zeros((v.shape[0], v.shape[2], q.shape[-1], v.shape[3]), dtype=torch.float32) if h0 is None \
@@ -46,5 +52,5 @@ def gated_delta_step(h, q, k, v, g, beta, scale=None, qk_norm=False):
     """One token per stream: o (B, H, Dv) in v's dtype; h (B, H, Dk, Dv), contiguous float32, is updated
     in place.  q, k (B, Hk, Dk), v (B, H, Dv), g and beta (B, H) as in gated_delta_rule.  Not differentiable: in
     grad mode, operands that require a gradient are refused."""
-    scale = float(q.shape[-1] ** -0.5 if scale is None else scale)
+    scale = _scale(q, scale)
     return _abi.host().delta_step(h, q, k, v, g, beta, scale, bool(qk_norm))

@@ -3,7 +3,9 @@
 import ctypes
 
 import pytest
+import torch
 
+import ssm_scan
 from ssm_scan import _abi
 from test_delta_cpu import delta_args
 
@@ -21,3 +23,14 @@ def test_chunks_of_all_heads():
     lib = _abi.lib()
     for L, rc in ((64 * (1 << 19), _abi.EINVAL), (64 * ((1 << 19) - 1), 0)):
         assert lib.ssm_delta_check(ctypes.byref(delta_args(batch=1, heads=16, key_heads=16, seqlen=L))) == rc
+
+
+def test_keys_of_no_width_are_refused_as_any_other_shape():
+    """The default scale, Dk^-0.5, is not formed of a width that the checks refuse."""
+    t = torch.zeros
+    with pytest.raises(RuntimeError, match="no CPU path"):
+        ssm_scan.gated_delta_rule(t(1, 2, 1, 0), t(1, 2, 1, 0), t(1, 2, 1, 4), t(1, 2, 1), t(1, 2, 1))
+    with pytest.raises(RuntimeError, match="no CPU path"):
+        ssm_scan.gated_delta_step(t(1, 1, 0, 4), t(1, 1, 0), t(1, 1, 0), t(1, 1, 4), t(1, 1), t(1, 1))
+    with pytest.raises(RuntimeError, match="no CPU path"):
+        ssm_scan.gated_delta_rule(t(()), t(()), t(()), t(()), t(()))
