@@ -52,6 +52,14 @@ class GatedDeltaMixer(nn.Module):
             conv=torch.zeros(batch, 2 * self.d_keys + self.d_values, self.d_conv - 1, device=device, dtype=dtype),
             delta=torch.zeros(batch, self.heads, self.key_dim, self.value_dim, device=device))
 
+    def _conv(self, x, state):
+        if state is None or state.conv.dtype == x.dtype:
+            return causal_conv1d(x, self.conv.weight, self.conv.bias, state=None if state is None else state.conv)
+        previous = state.conv.to(x.dtype)   # a float32 state under autocast
+        out = causal_conv1d(x, self.conv.weight, self.conv.bias, state=previous)
+        state.conv.copy_(previous)
+        return out
+
     def forward(self, u, state=None):
         with torch.set_grad_enabled(torch.is_grad_enabled() and state is None):
             return self._forward(u, state)
@@ -59,7 +67,7 @@ class GatedDeltaMixer(nn.Module):
     def _forward(self, u, state):
         mixed, z, dt, b = linear(self.in_proj, u).split(
             [2 * self.d_keys + self.d_values, self.d_values, self.heads, self.heads], dim=-1)
-        mixed = causal_conv1d(mixed, self.conv.weight, self.conv.bias, state=None if state is None else state.conv)
+        mixed = self._conv(mixed, state)
         q, k, v = mixed.split([self.d_keys, self.d_keys, self.d_values], dim=-1)
         q, k = (t.unflatten(-1, (self.key_heads, self.key_dim)) for t in (q, k))
         v = v.unflatten(-1, (self.heads, self.value_dim))
