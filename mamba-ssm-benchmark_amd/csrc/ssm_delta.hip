@@ -404,9 +404,13 @@ __global__ void __launch_bounds__(2 * kDT) SSM_TWO_WAVES k_delta_fwd(const Delta
       load_t(next);
       if (__builtin_expect(not_finite(y), 0)) {  // after the writes, which need not wait for it
 #pragma unroll
-        for (int n = 0; n < NV; ++n)
-          y[n] = row_times<NM>((const __bf16 *)p.fT + at(c) * NM * kFrag, tok, 0, tok, Xt[n], kg, Xt[n].value(tok, kg));
-        put_u();
+        for (int n = 0; n < NV; ++n) x[n] = Xt[n].value(tok, kg);
+        if (not_finite_of(y, x)) {
+#pragma unroll
+          for (int n = 0; n < NV; ++n)
+            y[n] = row_times<NM>((const __bf16 *)p.fT + at(c) * NM * kFrag, tok, 0, tok, Xt[n], kg, x[n]);
+          put_u();
+        }
       }
       lds_barrier();
 #pragma unroll
@@ -500,7 +504,7 @@ __global__ void __launch_bounds__(2 * kDT) SSM_TWO_WAVES k_delta_fwd(const Delta
             o[n] = mma<NM>(A, P[s], o[n]);
           }
         }
-      if (__builtin_expect(not_finite(o), 0)) {
+      if (__builtin_expect(not_finite(o), 0) && not_finite_of(o, qs)) {
 #pragma unroll
         for (int n = 0; n < NV; ++n)
           o[n] = row_times<NM>((const __bf16 *)p.fP + at(c) * NM * kFrag, tok, 0, tok + 1, Ut[n], kg, qs[n]);

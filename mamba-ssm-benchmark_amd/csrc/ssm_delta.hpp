@@ -145,13 +145,22 @@ __device__ __forceinline__ void load_frag(const __bf16 *m, int64_t part, int at,
 
 // The products of a chunk's triangular matrices run over steps of 32 tokens, with the zeros beyond the diagonal,
 // and a zero times an infinity or NaN is NaN: it would reach tokens that the recurrence keeps free of it.  It
-// shows in the wavefront's own results, so these are looked at, and only where one is not finite are they formed
-// again from the tokens that belong to them.
+// shows in the wavefront's own results, so these are looked at, and only where one is not finite that was before
+// the product (with the state infinite or NaN, all are, from chunk to chunk) are they formed again from the tokens
+// that belong to them.
 template <int N> __device__ __forceinline__ bool not_finite(const f4 (&x)[N]) {
   float s = 0;
 #pragma unroll
   for (int n = 0; n < N; ++n) s += (fabsf(x[n][0]) + fabsf(x[n][1])) + (fabsf(x[n][2]) + fabsf(x[n][3]));
   return __builtin_amdgcn_ballot_w64(!(s < INFINITY)) != 0;
+}
+template <int N> __device__ __forceinline__ bool not_finite_of(const f4 (&x)[N], const f4 (&before)[N]) {
+  bool b = false;
+#pragma unroll
+  for (int n = 0; n < N; ++n)
+#pragma unroll
+    for (int i = 0; i < 4; ++i) b |= fabsf(before[n][i]) < INFINITY && !(fabsf(x[n][i]) < INFINITY);
+  return __builtin_amdgcn_ballot_w64(b) != 0;
 }
 // acc + sum over the tokens j, lo <= j < hi, of m[tok][j] x_j (columns 4 kg + i): m as fragments of token rows.
 template <int N, typename TILE>

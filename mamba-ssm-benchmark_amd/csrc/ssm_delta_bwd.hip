@@ -121,10 +121,15 @@ __global__ void __launch_bounds__(2 * kDT) SSM_TWO_WAVES k_delta_bwd(const Delta
       put_r();
       load_t(next);
       if (__builtin_expect(not_finite(x), 0)) {
+        f4 before[NV];
 #pragma unroll
-        for (int n = 0; n < NV; ++n)
-          x[n] = row_times<NM>((const __bf16 *)p.fT + at(c) * NM * kFrag, tok, tok + 1, kC, Xt[n], kg, Xt[n].value(tok, kg));
-        put_r();
+        for (int n = 0; n < NV; ++n) before[n] = Xt[n].value(tok, kg);
+        if (not_finite_of(x, before)) {
+#pragma unroll
+          for (int n = 0; n < NV; ++n)
+            x[n] = row_times<NM>((const __bf16 *)p.fT + at(c) * NM * kFrag, tok, tok + 1, kC, Xt[n], kg, before[n]);
+          put_r();
+        }
       }
       lds_barrier();
 #pragma unroll
@@ -567,7 +572,7 @@ __global__ void __launch_bounds__(4 * DK) SSM_TWO_WAVES k_delta_grad(const Delta
         ss += sdot[n];
       }
       double rest = __shfl(wave_scan_f64(s), 63 - lane);  // sum over i >= t of dG_i
-      if (__builtin_expect(__builtin_amdgcn_ballot_w64(!(fabs(rest) < INFINITY)) != 0, 0)) {
+      if (__builtin_expect(__builtin_amdgcn_ballot_w64(!(fabs(rest) < INFINITY)) != 0, 0) && fabs(ss) < INFINITY) {
         // A pair after t is in rows and columns of the sum and cancels, but not where it is infinite or NaN.  The sum of
         // all tokens less those before t is the same from finite terms: in that of all every pair cancels, and what is
         // left is the entering state's share, <S0, dS0 - e^{G_C} D>.
