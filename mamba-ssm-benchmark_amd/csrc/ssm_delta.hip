@@ -476,6 +476,7 @@ __global__ void __launch_bounds__(2 * kDT) SSM_TWO_WAVES k_delta_fwd(const Delta
           St[n].get(s, lane, A);
           o[n] = mma<NM>(A, Q[s], o[n]);
         }
+      read_ahead<KS * NM * 2 * NV, KS * products(NM, NM, NK) * NV, 12>();
 #pragma unroll
       for (int n = 0; n < NV; ++n) o[n] *= fd;
       if (p.states) {
