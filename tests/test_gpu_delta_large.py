@@ -64,3 +64,24 @@ def test_backward_walk_of_more_workgroups_than_a_grid_row(dev):
     for c in COLUMNS:
         _, _, want = delta_ref.delta(**{**a, "v": a["v"][..., c]}, qk_norm=True, dout=do[..., c])
         close("dv", dv[..., c], want["v"], F32, grad=True)
+
+
+def test_batch_rows_and_heads_far_apart(dev):
+    """Rows of the operands, and of the outputs' gradient, 2^31 and more elements apart."""
+    B, L, H, D, far = 2, 70, 2, 16, (1 << 31) + 8
+    g = torch.Generator(device=dev).manual_seed(53)
+    buf = torch.empty(far + 4 * L * H * D, device=dev, dtype=torch.bfloat16)
+
+    def spread(i):   # part i of the buffer
+        t = buf.as_strided((B, L, H, D), (far, H * D, D, 1), i * L * H * D)
+        return t.copy_(torch.randn(B, L, H, D, generator=g, device=dev))
+
+    q, k, v, do = (spread(i) for i in range(4))
+    decay, beta = -torch.rand(B, L, H, generator=g, device=dev), torch.rand(B, L, H, generator=g, device=dev)
+    leaves = [t.detach().requires_grad_() for t in (q, k, v, decay, beta)]
+    o = ssm_scan.gated_delta_rule(*leaves, qk_norm=True)
+    grads = torch.autograd.grad(o, leaves, do)
+    want_o, _, want = delta_ref.delta(*leaves, qk_norm=True, dout=do)
+    close("o", o, want_o, torch.bfloat16)
+    for n, d in zip(("q", "k", "v", "g", "beta"), grads):
+        close("d" + n, d, want[n], torch.bfloat16, grad=True, size=want["size"].get(n, 0.0))
