@@ -60,7 +60,7 @@ __device__ __forceinline__ bf8 without_odd(bf8 x) {
 // rest by T10 = -T11 (L10 T00) for blocks of 16, then of 32 rows.
 // Chunks are independent, so everything that does not hang on the state is done here, once for all columns
 // of v.  Latency bounds a workgroup (two waits for memory, a chain of five barriers: 9 us alone), hence three
-// to a compute unit for bf16 rows.  B4 L4096 H16 Hk8 128 x 128 bf16: 83 us for 270 MB written; 512 threads of
+// to a compute unit for bf16 rows.  B4 L4096 H16 Hk8 128 x 128 bf16: 89 us for 261 MB written; 512 threads of
 // the first version's occupancy (two workgroups, all 16 tiles of L and P computed) took 113.
 template <typename IT, int DK, bool BWD>
 __global__ void __launch_bounds__(kDT, 4 - DParts<IT>::in) k_delta_prep(const DeltaParams p) {
@@ -293,9 +293,10 @@ __global__ void __launch_bounds__(kDT, 4 - DParts<IT>::in) k_delta_prep(const De
 // The chain from state to state is what bounds the walk (per chunk three products, each split into parts and
 // handed on through LDS), so four wavefronts do nothing else and four more take the outputs (Q S, P U and
 // the stores) from what the chain leaves in LDS, while it goes on.
-// One stream of 16384 tokens, H8 128 x 128 bf16: 320 us, 1.25 us a chunk (LDS reads not ahead of the products:
-// 360; four wavefronts for everything, nothing read ahead: 1214).  B4 L4096 H16: 197 us, 274 with the states
-// saved: 435 MB of stores, which all workgroups, walking in step, send at the same time.
+// One stream of 16384 tokens, H8 128 x 128 bf16: 350 us, 1.37 us a chunk (320 with two parts of the outputs'
+// operands and no search for results that are not finite; 18 more where the outputs' LDS reads do not run ahead of
+// their products; four wavefronts for everything, nothing read ahead: 1214).  B4 L4096 H16: 202 us, 283 with the
+// states saved: 435 MB of stores, which all workgroups, walking in step, send at the same time.
 // Everything that does not hang on the state is read a chunk ahead, into the registers that the chunk has
 // just used.  All products are of transposes: rows are 16 columns of v, so a lane holds 4 columns of
 // one token or key, and moves them as one word.  A workgroup walks NV tiles of 16 columns.

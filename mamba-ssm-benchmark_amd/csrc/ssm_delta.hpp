@@ -303,8 +303,10 @@ __device__ __forceinline__ float *value_of(float *m, const DeltaParams &p, int64
 // Whether a wavefront of the walks takes two tiles of 16 columns of v.  Every read of memory takes a compute
 // unit's address unit 16 cycles, whatever its width, and the fragments' reads are the most of them; two
 // tiles share them.  While every tile can have a compute unit of its own, the pair only leaves some without
-// work.  Forward, L4096, 128 x 128 bf16, no gradients, pairs against single tiles: 128 tiles 180 and 122 us,
-// 256 tiles 195 and 143, 384 tiles 224 and 277, 512 tiles 250 and 317.
+// work.  Forward + backward of H16 L1024 with values of 64 columns, us, single tiles and pairs at 256 and at 384
+// tiles: bf16 keys of 64 131 153, 214 196; of 128 190 213, 312 292; fp16 143 172, 245 229; 255 285, 450 400;
+// float32 189 212, 331 299; 356 381, 612 534.  Either direction alone decides alike.  With one tile a head the
+// pair is half empty and 0 to 4 % longer.
 inline bool delta_pairs(const DeltaParams &p) { return p.B * p.H * p.VT > 256; }
 // launch(p, grid) over a walk's workgroups of `per` column tiles each, as many at once as a grid row takes.
 template <typename F>

@@ -23,7 +23,7 @@ hipError_t launch_delta_prep_t(const DeltaParams &p, int dtype, hipStream_t s);
 
 // As in the forward, four wavefronts walk the chain and four more prepare what it takes: P^T dO of the chunk
 // to come, d dO and Q^T (d dO), and they store D, dR and dV.  Same bounds as the forward: B4 L4096 H16 Hk8
-// 128 x 128 bf16 280 us (576 in the first version).
+// 128 x 128 bf16 274 us (576 in the first version).
 template <typename IT, int DK, int NV>
 __global__ void __launch_bounds__(2 * kDT) SSM_TWO_WAVES k_delta_bwd(const DeltaParams p) {
   constexpr int NK = DParts<IT>::in, NM = DParts<IT>::mid, KS = DK / 32, RT = DK / 64;
@@ -281,8 +281,8 @@ __global__ void __launch_bounds__(2 * kDT) SSM_TWO_WAVES k_delta_bwd(const Delta
 // the states go from memory to registers, both one slab ahead; what the products of the chunk's end want is
 // read during the last slab.  One workgroup of eight wavefronts fills a compute unit's registers at DK = 128 (F1,
 // F2, F3 alone are 48 of them), so a slab's phases add up: 1.5 us of products, 0.7 of splitting, the rest
-// barriers.  B4 L4096 H16 Hk8 128 x 128 bf16: 366 us for 0.7 GB (779 with 16 keys by two tiles a wavefront of
-// four, which spilled); B16 L512 H8 64 x 64 float32: 56 us.  SHARED: several value heads add to dq', dk', which wait in LDS meanwhile.
+// barriers.  B4 L4096 H16 Hk8 128 x 128 bf16: 365 us for 0.7 GB (779 with 16 keys by two tiles a wavefront of
+// four, which spilled); B16 L512 H8 64 x 64 float32: 58 us.  SHARED: several value heads add to dq', dk', which wait in LDS meanwhile.
 template <typename IT, int DK, bool SHARED>
 __global__ void __launch_bounds__(4 * DK) SSM_TWO_WAVES k_delta_grad(const DeltaParams p) {
   constexpr int NK = DParts<IT>::in, NM = DParts<IT>::mid, NT = 4 * DK, NW = DK / 16;

@@ -4,8 +4,8 @@
 // loads its part of the state before anything else and both products with the old state are taken
 // from the same registers: one pass, one barrier.  A workgroup owns 64 columns of v of one head; lane
 // l holds 4 columns, (l % 16), of the key rows 4 w + l / 16 + 16 j.
-// 64 streams of 8 heads of 128 x 128: 13.8 us, 4.9 TB/s (a copy reaches 5.15); one stream of 8 heads of 64 x 64:
-// 4.4 us, a launch's own time.
+// 64 streams of 8 heads of 128 x 128: 13.9 us, 4.9 TB/s (a copy reaches 5.15); one stream of 8 heads of 64 x 64:
+// 4.5 us, a launch's own time.
 #include "ssm_delta.hpp"
 
 namespace ssm {

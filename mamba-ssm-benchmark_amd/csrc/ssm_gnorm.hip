@@ -8,9 +8,9 @@
 // loads where its rows allow, and its sums are reductions over NP lanes.  Everything is float32 in
 // between.  The backward recomputes mean and r from the x that it needs anyway, so the forward saves
 // nothing; it is persistent, a lane group keeping one group of channels over its rows, with dw and db in
-// registers and one partial row per row slot that a second kernel adds in order, in float64: no float
+// float32 registers and one partial row per row slot that a second kernel adds in order, in float64: no float
 // atomics, bitwise reproducible.  HBM bounds both directions from some 8 MB on:
-// 16384 rows of 16 groups of 128, bf16, gate: forward 38 us (5.3 TB/s), backward 77 us (4.4 TB/s; with 2
+// 16384 rows of 16 groups of 128, bf16, gate: forward 39 us (5.2 TB/s), backward 76 us (4.4 TB/s; with 2
 // wavefronts a SIMD 104, with 8 the same 77 and twice the partial rows; reading a row ahead changed nothing).
 #include "ssm_device.hpp"
 #include "ssm_internal.hpp"

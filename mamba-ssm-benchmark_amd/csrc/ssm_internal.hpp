@@ -351,8 +351,9 @@ struct GnormParams {
   int nblk;                            // row slots of the backward
   int64_t first;                       // forward: lane groups of earlier launches
 };
-// Row slots: enough lane groups for kGnormLanes, at most one per row.  A group takes at least n / 8 lanes
-// (8 channels of 16 bits per load), so this is within a factor of 8 of it for every variant.
+// Row slots, at most one per row: kGnormLanes lanes where a lane has 8 channels, as in groups of 64 and more of 16
+// bits.  Every variant takes as many slots, so the lanes are NP * 8 / n times that: twice for float32, 8 times for
+// groups of 8, 30 times for 17 channels that are read one by one, 128 times for a single one.
 inline int64_t gnorm_slots(int64_t R, int64_t C) {
   const int64_t want = kGnormLanes * 8 / C;
   return want < 1 ? 1 : want < R ? want : R;
