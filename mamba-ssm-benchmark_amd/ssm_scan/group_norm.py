@@ -17,7 +17,7 @@ def group_norm(x, groups, weight=None, bias=None, gate=None, activation=None, ce
         y = z silu(gate) with a gate, silu(z) with activation="silu", else z
 
     x (..., C) float32, bfloat16 or float16; gate like x; weight, bias (C,).  float32 arithmetic;
-    differentiable in x, weight, bias and gate."""
+    differentiable (once, reverse mode) in x, weight, bias and gate."""
     if activation not in _ACTIVATIONS:
         raise ValueError(f"unknown activation {activation!r}")
     if gate is not None and activation is not None:
