@@ -64,6 +64,8 @@ def test_backward_walk_of_more_workgroups_than_a_grid_row(dev):
     for c in COLUMNS:
         _, _, want = delta_ref.delta(**{**a, "v": a["v"][..., c]}, qk_norm=True, dout=do[..., c])
         close("dv", dv[..., c], want["v"], F32, grad=True)
+    del o, dv, do, a
+    torch.cuda.empty_cache()   # for the tests that follow
 
 
 def test_batch_rows_and_heads_far_apart(dev):
