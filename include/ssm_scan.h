@@ -28,7 +28,7 @@
 extern "C" {
 #endif
 
-#define SSM_ABI_VERSION 9
+#define SSM_ABI_VERSION 10
 
 enum { SSM_OK = 0, SSM_EINVAL = 1, SSM_EKEY = 2, SSM_ESPACE = 3, SSM_EHIP = 4 };
 
@@ -448,6 +448,98 @@ typedef struct ssm_gnorm_args {
   int64_t workspace_bytes;
 } ssm_gnorm_args;
 
+/* ------------------------------------------------------------------ norm with the residual's addition
+ * The pre-norm residual stream of models/lm.py:82-83 in one pass (the reference adds, then normalizes,
+ * models/common.py:14-16).  Per row, in float32:
+ *   s = x + residual, rounded to res_dtype;   out = s / sqrt(mean(s^2) + eps) * weight.
+ * With `q` the row is written in 8 bits in place of out: scale = max |out| / 448 (1 for a row of zeros),
+ * q = out / scale in OCP e4m3; a residual is then optional, and without `weight` the rows of x themselves are
+ * written so.  Rows have unit column stride; dim <= SSM_RNORM_MAX_DIM. */
+#define SSM_RNORM_MAX_DIM 16384
+typedef struct ssm_rnorm_args {
+  int64_t rows, dim;
+  int32_t dtype;           /* x, out, dout, dx: SSM_F32, SSM_BF16 or SSM_F16 */
+  int32_t res_dtype;       /* residual, sum, dsum, dresidual: dtype or SSM_F32 */
+  double eps;
+  ssm_tensor x, residual;  /* (rows, dim): stride[0] = row stride, stride[1] = 1 */
+  const float *weight;     /* (dim,) */
+  ssm_tensor sum;          /* s: written by the forward with a residual, read by the backward */
+  ssm_tensor out;          /* forward, 16 or 32 bits */
+  ssm_tensor q;            /* forward, 8 bits: in place of out */
+  float *scale;            /* with q: (rows,) */
+  ssm_tensor dout, dsum;   /* backward; dsum optional */
+  ssm_tensor dx;           /* backward */
+  ssm_tensor dresidual;    /* backward, optional: equals dx but for its type */
+  float *dweight;          /* backward, optional */
+  void *workspace;         /* backward: ssm_rnorm_workspace_bytes() */
+  int64_t workspace_bytes;
+} ssm_rnorm_args;
+
+/* ------------------------------------------------------------------ token embedding
+ * models/lm.py:125 with a scale: out[i] = scale * weight[tokens[i]], zeros for a token outside [0, vocab)
+ * (padding; the reference's nn.Embedding raises).  Backward: dweight[v] = scale * sum of dout[i] over the i with
+ * tokens[i] = v, in their order, every row written. */
+typedef struct ssm_embed_args {
+  int64_t n, vocab, dim;
+  int32_t dtype;           /* weight, out, dout, dweight: SSM_F32, SSM_BF16 or SSM_F16 */
+  int32_t reserved0;
+  double scale;
+  const int64_t *tokens;   /* (n,) */
+  ssm_tensor weight;       /* (vocab, dim): stride[0] = row stride, stride[1] = 1; forward */
+  ssm_tensor out;          /* (n, dim) likewise; forward */
+  ssm_tensor dout;         /* (n, dim) likewise; backward */
+  void *dweight;           /* (vocab, dim) dense; backward */
+  void *workspace;         /* backward: ssm_embed_workspace_bytes() */
+  int64_t workspace_bytes;
+} ssm_embed_args;
+
+/* ------------------------------------------------------------------ linear layer with its epilogue
+ * nn.Linear (models/mamba.py:34-65, models/lm.py:95) with what follows it:
+ *   z = x weight^T [x_scale weight_scale] + bias,   out = act(z) + residual
+ * in 16 bits, or with 8-bit rows (OCP e4m3, a float32 scale per row of x and of weight).  Sums are float32.
+ * Backward (16 bits): dz = dout act'(z) with z as the forward stored it in `pre`, dx = dz weight,
+ * dweight = dz^T x, dbias = sum over rows of dz; the residual's gradient is dout itself. */
+enum { SSM_ACT_NONE = 0, SSM_ACT_SILU = 1, SSM_ACT_GELU = 2 };   /* GELU: z Phi(z) */
+typedef struct ssm_linear_args {
+  int64_t m, n, k;
+  int32_t dtype;           /* out, bias, residual, pre (and x, weight unless in8): SSM_BF16 or SSM_F16 */
+  int32_t in8, activation, reserved0;
+  ssm_tensor x;            /* (m, k): stride[0] = row stride, stride[1] = 1 */
+  ssm_tensor weight;       /* (n, k) likewise */
+  const float *x_scale, *weight_scale;  /* in8: (m,), (n,) */
+  const void *bias;        /* (n,) optional */
+  ssm_tensor residual;     /* (m, n) optional */
+  ssm_tensor out;          /* forward: (m, n) */
+  void *pre;               /* (m, n) dense z: with an activation, written by the forward when given, read by the backward */
+  ssm_tensor dout;         /* backward: (m, n) */
+  ssm_tensor dx, dweight;  /* backward: (m, k), (n, k); each optional */
+  void *dbias;             /* backward: (n,) optional */
+  void *workspace;         /* ssm_linear_workspace_bytes() / ssm_linear_bwd_workspace_bytes() */
+  int64_t workspace_bytes;
+} ssm_linear_args;
+
+/* ------------------------------------------------------------------ next token
+ * The sampling steps of models/lm.py:138-143 with top-p, min-p and the random numbers given.  Per row, with
+ * w_i = exp((l_i - max l) / T): of the order by falling logit (ties: the lower index first) the first top_k are kept,
+ * of those the shortest prefix with top_p of their mass, of those the ones with w_i >= min_p, and always the first;
+ * the token is the first kept index at which the running sum of the kept w, by index, passes u times their sum.
+ * T <= 0 (or NaN) takes the first of the order.  A row with a NaN, or with no logit above -inf, gives -1. */
+typedef struct ssm_sample_args {
+  int64_t rows, vocab;
+  int32_t dtype;           /* logits: SSM_F32, SSM_BF16 or SSM_F16 */
+  int32_t u_f64;           /* u is float64, else float32 */
+  ssm_tensor logits;       /* (rows, vocab): stride[0] = row stride, stride[1] = 1 */
+  const void *u;           /* (rows,) in [0, 1) */
+  double temperature, top_p, min_p;     /* of every row: top_p >= 1 and min_p <= 0 keep all */
+  int64_t top_k;                        /* <= 0: all */
+  const float *temperatures, *top_ps, *min_ps;  /* (rows,) optional, in their place */
+  const int64_t *top_ks;
+  int64_t *token;          /* (rows,) */
+  float *logprob;          /* (rows,): log of the token's share of the kept mass; NaN with -1 */
+  void *workspace;         /* ssm_sample_workspace_bytes() */
+  int64_t workspace_bytes;
+} ssm_sample_args;
+
 /* ------------------------------------------------------------------ entry points */
 int ssm_abi_version(void);
 const char *ssm_last_error(void);
@@ -467,6 +559,10 @@ int ssm_norm_check(const ssm_norm_args *args);
 int ssm_delta_check(const ssm_delta_args *args);
 int ssm_delta_step_check(const ssm_delta_step_args *args);
 int ssm_gnorm_check(const ssm_gnorm_args *args);
+int ssm_rnorm_check(const ssm_rnorm_args *args);
+int ssm_embed_check(const ssm_embed_args *args);
+int ssm_linear_check(const ssm_linear_args *args);
+int ssm_sample_check(const ssm_sample_args *args);
 
 /* Buffer sizes in bytes (host-only). */
 int64_t ssm_fwd_saved_bytes(const ssm_fwd_args *args);
@@ -483,6 +579,11 @@ int64_t ssm_delta_saved_bytes(const ssm_delta_args *args);
 int64_t ssm_delta_fwd_workspace_bytes(const ssm_delta_args *args);
 int64_t ssm_delta_bwd_workspace_bytes(const ssm_delta_args *args);
 int64_t ssm_gnorm_workspace_bytes(const ssm_gnorm_args *args);   /* backward */
+int64_t ssm_rnorm_workspace_bytes(const ssm_rnorm_args *args);   /* backward */
+int64_t ssm_embed_workspace_bytes(const ssm_embed_args *args);   /* backward */
+int64_t ssm_linear_workspace_bytes(const ssm_linear_args *args);
+int64_t ssm_linear_bwd_workspace_bytes(const ssm_linear_args *args);
+int64_t ssm_sample_workspace_bytes(const ssm_sample_args *args);
 int64_t ssm_decode_stack_workspace_bytes(const ssm_decode_stack_args *args);
 /* Byte offset inside the decode-stack workspace of an int32 status word: ssm_decode_stack sets
  * it to 1 when a token id lies outside [0, vocab) (the reference's nn.Embedding,
@@ -513,6 +614,13 @@ int ssm_delta_bwd(const ssm_delta_args *args, void *stream);
 int ssm_delta_step(const ssm_delta_step_args *args, void *stream);
 int ssm_gnorm_fwd(const ssm_gnorm_args *args, void *stream);
 int ssm_gnorm_bwd(const ssm_gnorm_args *args, void *stream);
+int ssm_rnorm_fwd(const ssm_rnorm_args *args, void *stream);
+int ssm_rnorm_bwd(const ssm_rnorm_args *args, void *stream);
+int ssm_embed_fwd(const ssm_embed_args *args, void *stream);
+int ssm_embed_bwd(const ssm_embed_args *args, void *stream);
+int ssm_linear_fwd(const ssm_linear_args *args, void *stream);
+int ssm_linear_bwd(const ssm_linear_args *args, void *stream);
+int ssm_sample(const ssm_sample_args *args, void *stream);
 
 /* ssm_fwd without allocation.  No counterpart in the reference: for callers that cannot
  * allocate device memory (code under HIP graph capture, tight serving loops, harnesses that

@@ -1394,6 +1394,307 @@ int ssm_gnorm_bwd(const ssm_gnorm_args *a, void *stream) {
   return e == hipSuccess ? ok() : hip_fail(e, "ssm_gnorm_bwd");
 }
 
+// ------------------------------------------------------------------ norm with the residual's addition
+static bool io16_32(int dtype) { return dtype == SSM_F32 || dtype == SSM_BF16 || dtype == SSM_F16; }
+static bool lines16(const ssm_tensor &t, int64_t rows, int64_t per) {  // rows of whole 16-byte loads of `per` elements
+  return !has(t) || ((uintptr_t)t.data % 16 == 0 && (rows == 1 || t.stride[0] % per == 0));
+}
+int ssm_rnorm_check(const ssm_rnorm_args *a) {
+  if (!a) return fail(SSM_EINVAL, "null args");
+  if (!io16_32(a->dtype)) return fail(SSM_EINVAL, "the norm takes float32, bfloat16 or float16");
+  if (a->res_dtype != a->dtype && a->res_dtype != SSM_F32) return fail(SSM_EINVAL, "the residual must be of x's type or float32");
+  if (a->rows < 1 || a->dim < 1)
+    return fail(SSM_EINVAL, "empty norm: rows=%lld dim=%lld", (long long)a->rows, (long long)a->dim);
+  if (a->dim > kRnormMaxDim) return fail(SSM_EINVAL, "dim=%lld > %d is not supported", (long long)a->dim, kRnormMaxDim);
+  if (a->rows >= (1LL << 40)) return fail(SSM_EINVAL, "rows=%lld is too large", (long long)a->rows);
+  if (!(a->eps >= 0.0)) return fail(SSM_EINVAL, "eps must be >= 0");
+  return ok();
+}
+int64_t ssm_rnorm_workspace_bytes(const ssm_rnorm_args *a) {
+  if (ssm_rnorm_check(a)) return -1;
+  return a->dweight ? align256(rnorm_blocks(a->rows, 4) * a->dim * 4) : 0;
+}
+static RnormParams rnorm_params(const ssm_rnorm_args *a) {
+  RnormParams p{};
+  p.R = a->rows;
+  p.C = (int)a->dim;
+  p.eps = (float)a->eps;
+  p.w = a->weight;
+  const int64_t e = a->dtype == SSM_F32 ? 4 : 8, er = a->res_dtype == SSM_F32 ? 4 : 8;
+  p.vec = a->dim % e == 0 && (uintptr_t)a->weight % 16 == 0 && lines16(a->x, a->rows, e) && lines16(a->residual, a->rows, er) &&
+          lines16(a->sum, a->rows, er) && lines16(a->out, a->rows, e) && lines16(a->dout, a->rows, e) &&
+          lines16(a->dsum, a->rows, er) && lines16(a->dx, a->rows, e) && lines16(a->dresidual, a->rows, er) &&
+          (!has(a->q) || ((uintptr_t)a->q.data % e == 0 && (a->rows == 1 || a->q.stride[0] % e == 0)));
+  return p;
+}
+int ssm_rnorm_fwd(const ssm_rnorm_args *a, void *stream) {
+  int rc = ssm_rnorm_check(a);
+  if (!rc) rc = gnorm_view(a->x, "x");
+  if (!rc && has(a->residual)) rc = gnorm_view(a->residual, "residual");
+  if (!rc && has(a->residual)) rc = gnorm_view(a->sum, "sum");
+  if (!rc) rc = has(a->q) ? gnorm_view(a->q, "q") : gnorm_view(a->out, "out");
+  if (!rc && has(a->q)) rc = need({{a->scale, "scale"}});
+  if (!rc && !has(a->q)) rc = need({{a->weight, "weight"}});
+  if (rc) return rc;
+  RnormParams p = rnorm_params(a);
+  p.x = a->x.data; p.sx = a->x.stride[0];
+  p.res = a->residual.data; p.sr = a->residual.stride[0];
+  p.s = a->sum.data; p.ss = a->sum.stride[0];
+  p.y = a->out.data; p.sy = a->out.stride[0];
+  p.q = (uint8_t *)a->q.data; p.sq = a->q.stride[0];
+  p.scale = a->scale;
+  hipError_t e = launch_rnorm(p, a->dtype, a->res_dtype, false, (hipStream_t)stream);
+  return e == hipSuccess ? ok() : hip_fail(e, "ssm_rnorm_fwd");
+}
+int ssm_rnorm_bwd(const ssm_rnorm_args *a, void *stream) {
+  int rc = ssm_rnorm_check(a);
+  if (!rc) rc = gnorm_view(a->sum, "sum");
+  if (!rc) rc = gnorm_view(a->dout, "dout");
+  if (!rc && has(a->dsum)) rc = gnorm_view(a->dsum, "dsum");
+  if (!rc) rc = gnorm_view(a->dx, "dx");
+  if (!rc && has(a->dresidual)) rc = gnorm_view(a->dresidual, "dresidual");
+  if (!rc) rc = need({{a->weight, "weight"}});
+  if (rc) return rc;
+  const int64_t bytes = ssm_rnorm_workspace_bytes(a);
+  if (bytes && (!a->workspace || a->workspace_bytes < bytes))
+    return fail(SSM_ESPACE, "workspace of %lld bytes required", (long long)bytes);
+  RnormParams p = rnorm_params(a);
+  p.s = a->sum.data; p.ss = a->sum.stride[0];
+  p.dy = a->dout.data; p.sdy = a->dout.stride[0];
+  p.ds = a->dsum.data; p.sds = a->dsum.stride[0];
+  p.dx = a->dx.data; p.sdx = a->dx.stride[0];
+  p.dres = a->dresidual.data; p.sdr = a->dresidual.stride[0];
+  p.dw = a->dweight;
+  p.ws = (float *)a->workspace;
+  hipError_t e = launch_rnorm(p, a->dtype, a->res_dtype, true, (hipStream_t)stream);
+  return e == hipSuccess ? ok() : hip_fail(e, "ssm_rnorm_bwd");
+}
+
+// ------------------------------------------------------------------ token embedding
+int ssm_embed_check(const ssm_embed_args *a) {
+  if (!a) return fail(SSM_EINVAL, "null args");
+  if (!io16_32(a->dtype)) return fail(SSM_EINVAL, "the embedding takes float32, bfloat16 or float16");
+  if (a->n < 1 || a->vocab < 1 || a->dim < 1)
+    return fail(SSM_EINVAL, "empty embedding: n=%lld vocab=%lld dim=%lld", (long long)a->n, (long long)a->vocab, (long long)a->dim);
+  if (a->n >= (1LL << 40) || a->vocab >= (1LL << 31) - 1 || a->dim >= (1LL << 24))
+    return fail(SSM_EINVAL, "embedding is too large: n=%lld vocab=%lld dim=%lld", (long long)a->n, (long long)a->vocab, (long long)a->dim);
+  if (!isfinite(a->scale)) return fail(SSM_EINVAL, "scale must be finite");
+  return ok();
+}
+namespace {
+// Parts of the gradient's workspace.
+struct EmbedLayout {
+  int64_t per, nw, hist, items, start, pieces, groups;
+  int64_t bytes() const { return hist + 4 * items + start + pieces + groups; }
+};
+EmbedLayout embed_layout(const ssm_embed_args *a) {
+  EmbedLayout l;
+  l.per = cdiv(cdiv(a->n, kEmbedWaves), 64) * 64;
+  l.nw = cdiv(a->n, l.per);
+  l.hist = align256(l.nw * ((int64_t)4 << kEmbedBits));
+  l.items = align256(4 * a->n);
+  l.start = align256(4 * (a->vocab + 1));
+  const int64_t pieces = a->n / kEmbedPiece, groups = pieces / kEmbedGroup;
+  l.pieces = align256(pieces * a->dim * 4);
+  l.groups = groups >= kEmbedGroup ? align256(groups * a->dim * 4) : 0;   // from 2^16 tokens on
+  return l;
+}
+EmbedParams embed_params(const ssm_embed_args *a) {
+  EmbedParams p{};
+  p.n = a->n; p.V = a->vocab; p.D = a->dim;
+  p.scale = (float)a->scale;
+  p.tokens = a->tokens;
+  const int64_t e = a->dtype == SSM_F32 ? 4 : 8;
+  p.vec = a->dim % e == 0 && lines16(a->weight, a->vocab, e) && lines16(a->out, a->n, e) && lines16(a->dout, a->n, e) &&
+          (uintptr_t)a->dweight % 16 == 0;
+  return p;
+}
+}  // namespace
+int64_t ssm_embed_workspace_bytes(const ssm_embed_args *a) {
+  if (ssm_embed_check(a)) return -1;
+  return embed_layout(a).bytes();
+}
+int ssm_embed_fwd(const ssm_embed_args *a, void *stream) {
+  int rc = ssm_embed_check(a);
+  if (!rc) rc = need({{a->tokens, "tokens"}});
+  if (!rc) rc = gnorm_view(a->weight, "weight");
+  if (!rc) rc = gnorm_view(a->out, "out");
+  if (rc) return rc;
+  EmbedParams p = embed_params(a);
+  p.w = a->weight.data; p.sw = a->weight.stride[0];
+  p.out = a->out.data; p.so = a->out.stride[0];
+  hipError_t e = launch_embed(p, a->dtype, false, (hipStream_t)stream);
+  return e == hipSuccess ? ok() : hip_fail(e, "ssm_embed_fwd");
+}
+int ssm_embed_bwd(const ssm_embed_args *a, void *stream) {
+  int rc = ssm_embed_check(a);
+  if (!rc) rc = need({{a->tokens, "tokens"}, {a->dweight, "dweight"}});
+  if (!rc) rc = gnorm_view(a->dout, "dout");
+  if (rc) return rc;
+  if (a->n >= (1LL << 27)) return fail(SSM_EINVAL, "the gradient of %lld tokens is not supported", (long long)a->n);
+  const EmbedLayout l = embed_layout(a);
+  if (!a->workspace || a->workspace_bytes < l.bytes())
+    return fail(SSM_ESPACE, "workspace of %lld bytes required", (long long)l.bytes());
+  EmbedParams p = embed_params(a);
+  p.dout = a->dout.data; p.sd = a->dout.stride[0];
+  p.dw = a->dweight;
+  p.nw = l.nw; p.per = l.per;
+  char *ws = (char *)a->workspace;
+  auto take = [&](int64_t bytes) {
+    char *at = ws;
+    ws += bytes;
+    return at;
+  };
+  p.hist = (uint32_t *)take(l.hist);
+  for (int i = 0; i < 2; ++i) p.key[i] = (uint32_t *)take(l.items);
+  for (int i = 0; i < 2; ++i) p.pos[i] = (uint32_t *)take(l.items);
+  p.start = (uint32_t *)take(l.start);
+  p.piece = (float *)take(l.pieces);
+  p.group = l.groups ? (float *)take(l.groups) : nullptr;
+  hipError_t e = launch_embed(p, a->dtype, true, (hipStream_t)stream);
+  return e == hipSuccess ? ok() : hip_fail(e, "ssm_embed_bwd");
+}
+
+// ------------------------------------------------------------------ linear layer with its epilogue
+int ssm_linear_check(const ssm_linear_args *a) {
+  if (!a) return fail(SSM_EINVAL, "null args");
+  if (a->dtype != SSM_BF16 && a->dtype != SSM_F16) return fail(SSM_EINVAL, "the linear layer takes bfloat16 or float16");
+  if (a->m < 1 || a->n < 1 || a->k < 1)
+    return fail(SSM_EINVAL, "empty product: m=%lld n=%lld k=%lld", (long long)a->m, (long long)a->n, (long long)a->k);
+  const int64_t side = 1LL << 24, area = 1LL << 35;   // tiles of 64 x 64 fit a launch of 256 threads each
+  if (a->m > side || a->n > side || a->k > side || a->m * a->n > area || a->m * a->k > area || a->n * a->k > area)
+    return fail(SSM_EINVAL, "product is too large: m=%lld n=%lld k=%lld (each up to 2^24, each matrix up to 2^35)", (long long)a->m,
+                (long long)a->n, (long long)a->k);
+  if (a->activation < SSM_ACT_NONE || a->activation > SSM_ACT_GELU) return fail(SSM_EINVAL, "unknown activation %d", a->activation);
+  int rc = gnorm_view(a->x, "x");
+  if (!rc) rc = gnorm_view(a->weight, "weight");
+  if (!rc && a->in8) rc = need({{a->x_scale, "x_scale"}, {a->weight_scale, "weight_scale"}});
+  return rc ? rc : ok();
+}
+int64_t ssm_linear_workspace_bytes(const ssm_linear_args *a) {
+  if (ssm_linear_check(a)) return -1;
+  return 0;
+}
+namespace {
+int64_t linear_slots(const ssm_linear_args *a) { return std::min<int64_t>(64, cdiv(a->m, 64)); }
+struct LinearBwdLayout {
+  int64_t dz, partial;
+  int64_t bytes() const { return dz + partial; }
+};
+LinearBwdLayout linear_bwd_layout(const ssm_linear_args *a) {
+  LinearBwdLayout l{};
+  if (a->activation) l.dz = align256(a->m * a->n * 2);
+  if (a->dbias) l.partial = align256(linear_slots(a) * a->n * 4);
+  return l;
+}
+}  // namespace
+int64_t ssm_linear_bwd_workspace_bytes(const ssm_linear_args *a) {
+  if (ssm_linear_check(a)) return -1;
+  return linear_bwd_layout(a).bytes();
+}
+int ssm_linear_fwd(const ssm_linear_args *a, void *stream) {
+  int rc = ssm_linear_check(a);
+  if (!rc) rc = gnorm_view(a->out, "out");
+  if (!rc && has(a->residual)) rc = gnorm_view(a->residual, "residual");
+  if (rc) return rc;
+  GemmParams p{};
+  p.M = a->m; p.N = a->n; p.K = a->k;
+  p.A = a->x.data; p.sa = a->x.stride[0]; p.a_along = 1;
+  p.B = a->weight.data; p.sb = a->weight.stride[0]; p.b_along = 1;
+  p.C = a->out.data; p.sc = a->out.stride[0];
+  p.fp8 = a->in8;
+  p.xs = a->in8 ? a->x_scale : nullptr;
+  p.ws = a->in8 ? a->weight_scale : nullptr;
+  p.act = a->activation;
+  p.bias = a->bias;
+  p.residual = a->residual.data; p.sr = a->residual.stride[0];
+  p.pre = a->activation ? a->pre : nullptr; p.spre = a->n;
+  hipError_t e = launch_gemm(p, a->dtype, (hipStream_t)stream);
+  return e == hipSuccess ? ok() : hip_fail(e, "ssm_linear_fwd");
+}
+int ssm_linear_bwd(const ssm_linear_args *a, void *stream) {
+  int rc = ssm_linear_check(a);
+  if (!rc && a->in8) rc = fail(SSM_EINVAL, "the 8-bit product has no backward");
+  if (!rc) rc = gnorm_view(a->dout, "dout");
+  if (!rc && a->activation) rc = need({{a->pre, "pre"}});
+  if (!rc && has(a->dx)) rc = gnorm_view(a->dx, "dx");
+  if (!rc && has(a->dweight)) rc = gnorm_view(a->dweight, "dweight");
+  if (rc) return rc;
+  const LinearBwdLayout l = linear_bwd_layout(a);
+  if (l.bytes() && (!a->workspace || a->workspace_bytes < l.bytes()))
+    return fail(SSM_ESPACE, "workspace of %lld bytes required", (long long)l.bytes());
+  const void *dz = a->dout.data;
+  int64_t sdz = a->dout.stride[0];
+  hipError_t e = hipSuccess;
+  if (a->activation || a->dbias) {
+    LinearDzParams d{};
+    d.M = a->m; d.N = a->n;
+    d.act = a->activation;
+    d.dy = a->dout.data; d.sdy = a->dout.stride[0];
+    d.pre = a->pre;
+    d.slots = (int)linear_slots(a);
+    d.dbias = a->dbias;
+    if (a->dbias) d.partial = (float *)((char *)a->workspace + l.dz);
+    if (a->activation) {
+      dz = d.dz = a->workspace;
+      sdz = a->n;
+    }
+    e = launch_linear_dz(d, a->dtype, (hipStream_t)stream);
+  }
+  GemmParams p{};
+  if (e == hipSuccess && has(a->dx)) {   // dx[m, k] = sum over n of dz[m, n] weight[n, k]
+    p.M = a->m; p.N = a->k; p.K = a->n;
+    p.A = dz; p.sa = sdz; p.a_along = 1;
+    p.B = a->weight.data; p.sb = a->weight.stride[0]; p.b_along = 0;
+    p.C = a->dx.data; p.sc = a->dx.stride[0];
+    e = launch_gemm(p, a->dtype, (hipStream_t)stream);
+  }
+  if (e == hipSuccess && has(a->dweight)) {   // dweight[n, k] = sum over m of dz[m, n] x[m, k]
+    p.M = a->n; p.N = a->k; p.K = a->m;
+    p.A = dz; p.sa = sdz; p.a_along = 0;
+    p.B = a->x.data; p.sb = a->x.stride[0]; p.b_along = 0;
+    p.C = a->dweight.data; p.sc = a->dweight.stride[0];
+    e = launch_gemm(p, a->dtype, (hipStream_t)stream);
+  }
+  return e == hipSuccess ? ok() : hip_fail(e, "ssm_linear_bwd");
+}
+
+// ------------------------------------------------------------------ next token
+int ssm_sample_check(const ssm_sample_args *a) {
+  if (!a) return fail(SSM_EINVAL, "null args");
+  if (!io16_32(a->dtype)) return fail(SSM_EINVAL, "logits must be float32, bfloat16 or float16");
+  if (a->rows < 1 || a->vocab < 1) return fail(SSM_EINVAL, "empty logits: rows=%lld vocab=%lld", (long long)a->rows, (long long)a->vocab);
+  if (a->rows >= (1LL << 40) || a->vocab > (1LL << 24))
+    return fail(SSM_EINVAL, "logits are too large: rows=%lld vocab=%lld (at most 2^24)", (long long)a->rows, (long long)a->vocab);
+  if (!a->temperatures && !(a->temperature >= 0)) return fail(SSM_EINVAL, "temperature must be >= 0, got %g", a->temperature);
+  if (!a->top_ks && a->top_k < 0) return fail(SSM_EINVAL, "top_k must be >= 0, got %lld", (long long)a->top_k);
+  if (!a->top_ps && !(a->top_p >= 0)) return fail(SSM_EINVAL, "top_p must be >= 0, got %g", a->top_p);
+  if (!a->min_ps && !(a->min_p >= 0)) return fail(SSM_EINVAL, "min_p must be >= 0, got %g", a->min_p);
+  return ok();
+}
+int64_t ssm_sample_workspace_bytes(const ssm_sample_args *a) {
+  if (ssm_sample_check(a)) return -1;
+  return 0;
+}
+int ssm_sample(const ssm_sample_args *a, void *stream) {
+  int rc = ssm_sample_check(a);
+  if (!rc) rc = gnorm_view(a->logits, "logits");
+  if (!rc) rc = need({{a->u, "u"}, {a->token, "token"}, {a->logprob, "logprob"}});
+  if (rc) return rc;
+  SampleParams p{};
+  p.R = a->rows; p.V = a->vocab;
+  p.logits = a->logits.data; p.sl = a->logits.stride[0];
+  p.u = a->u; p.u_f64 = a->u_f64;
+  int bits = 0;
+  while ((a->vocab >> bits) > 0) ++bits;
+  p.shift = std::min(52, 62 - bits);
+  p.temperature = a->temperature; p.top_p = a->top_p; p.min_p = a->min_p; p.top_k = a->top_k;
+  p.temperatures = a->temperatures; p.top_ps = a->top_ps; p.min_ps = a->min_ps; p.top_ks = a->top_ks;
+  p.token = a->token; p.logprob = a->logprob;
+  hipError_t e = launch_sample(p, a->dtype, (hipStream_t)stream);
+  return e == hipSuccess ? ok() : hip_fail(e, "ssm_sample");
+}
+
 // ------------------------------------------------------------------ forward without allocation
 // ssm_fwd with the long-sequence workspace taken from a fixed device array instead of the
 // caller's buffer, for callers that cannot allocate.  Every GPU the library runs on holds its

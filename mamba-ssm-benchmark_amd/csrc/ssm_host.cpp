@@ -10,6 +10,7 @@
 #include <torch/csrc/autograd/custom_function.h>
 #include <torch/csrc/autograd/function.h>
 #include <torch/csrc/autograd/functions/utils.h>
+#include <torch/csrc/autograd/python_variable.h>
 #include <torch/csrc/utils/pybind.h>
 
 #include <ATen/ATen.h>
@@ -818,6 +819,383 @@ Tensor gnorm(const Tensor &x, const OptTensor &weight, const OptTensor &bias, co
   return GnormFn::apply(x, weight, bias, gate, groups, act, center, eps);
 }
 
+// ------------------------------------------------------------------ norm with the residual's addition
+void no_graph(std::initializer_list<const Tensor *> ts, const char *what) {
+  no_tangents(ts, what);
+  TORCH_CHECK(!needs_grad(ts), what, " is not differentiable: call it under torch.no_grad() or on detached tensors");
+}
+ssm_rnorm_args rnorm_args(const Tensor &x2, const Tensor &w, at::ScalarType io, at::ScalarType rt, double eps) {
+  ssm_rnorm_args a;
+  memset(&a, 0, sizeof(a));
+  a.rows = x2.size(0);
+  a.dim = x2.size(1);
+  a.dtype = dtype_code(io);
+  a.res_dtype = dtype_code(rt);
+  a.eps = eps;
+  a.weight = w.defined() ? w.data_ptr<float>() : nullptr;
+  return a;
+}
+void rnorm_checks(const Tensor &x, const Tensor &r, const Tensor &w, const char *what) {
+  require_gpu({&x, &r, &w});
+  one_device(x, {&r, &w});
+  TORCH_CHECK_VALUE(x.dim() >= 1 && x.size(-1) > 0, what, ": x must have channels, got ", shape_str(x.sizes()));
+  TORCH_CHECK_TYPE(delta_type(x.scalar_type()), what, " takes float32, bfloat16 or float16, got ", x.scalar_type());
+  want("residual", r, x.sizes());
+  TORCH_CHECK_TYPE(!r.defined() || r.scalar_type() == x.scalar_type() || r.scalar_type() == at::kFloat,
+                   "the residual must be of x's type or float32, got ", r.scalar_type(), " beside ", x.scalar_type());
+  want("weight", w, {x.size(-1)});
+  TORCH_CHECK_TYPE(!w.defined() || at::isFloatingType(w.scalar_type()), "weight must be floating, got ", w.scalar_type());
+}
+// y, s, weight
+variable_list add_rnorm_forward(const Tensor &x, const Tensor &r, const Tensor &weight, double eps) {
+  const Tensor x2 = rows(x, x.size(-1)), r2 = rows(r, x.size(-1)), w = f32(weight);
+  const Tensor y = at::empty(x2.sizes(), x2.options()), s = at::empty(x2.sizes(), r2.options());
+  ssm_rnorm_args a = rnorm_args(x2, w, x.scalar_type(), r.scalar_type(), eps);
+  a.x = view(x2); a.residual = view(r2); a.sum = view(s); a.out = view(y);
+  const Launch l(x);
+  l.run_anywhere("ssm_rnorm_fwd", ssm_rnorm_fwd, a);
+  return {y.view(x.sizes()), s.view(x.sizes()), w};
+}
+struct AddRnormFn : torch::autograd::Function<AddRnormFn> {
+  static variable_list forward(AutogradContext *ctx, const Tensor &x, const Tensor &r, const Tensor &weight, double eps) {
+    const variable_list o = add_rnorm_forward(x, r, weight, eps);
+    ctx->save_for_backward({o[1], o[2]});
+    ctx->set_materialize_grads(false);
+    ctx->saved_data["eps"] = eps;
+    ctx->saved_data["types"] = std::vector<int64_t>{(int64_t)x.scalar_type(), (int64_t)weight.scalar_type()};
+    return {o[0], o[1]};
+  }
+  static variable_list backward(AutogradContext *ctx, variable_list grads) {
+    const variable_list t = ctx->get_saved_variables();
+    const Tensor &s = t[0], &w = t[1];
+    const auto types = ctx->saved_data["types"].toIntVector();
+    const at::ScalarType io = (at::ScalarType)types[0], rt = s.scalar_type();
+    variable_list d(4);
+    if (!grads[0].defined()) {   // the sum alone was used
+      if (grads[1].defined()) {
+        d[0] = cast(grads[1], io);
+        d[1] = cast(grads[1], rt);
+        if (ctx->needs_input_grad(2)) d[2] = at::zeros(w.sizes(), w.options().dtype((at::ScalarType)types[1]));
+      }
+      not_twice(d, grads, "add_rms_norm");
+      return d;
+    }
+    const int64_t C = s.size(-1);
+    const Tensor s2 = rows(s, C), dy = rows(cast(grads[0], io), C);
+    const Tensor ds = grads[1].defined() ? rows(cast(grads[1], rt), C) : Tensor();
+    const Tensor dx = at::empty(s2.sizes(), dy.options());
+    const Tensor dr = rt == io || !ctx->needs_input_grad(1) ? Tensor() : at::empty(s2.sizes(), s2.options());
+    const Tensor dw = ctx->needs_input_grad(2) ? empty({C}, s, at::kFloat) : Tensor();
+    ssm_rnorm_args a = rnorm_args(s2, w, io, rt, ctx->saved_data["eps"].toDouble());
+    a.sum = view(s2); a.dout = view(dy); a.dsum = view(ds); a.dx = view(dx); a.dresidual = view(dr);
+    a.dweight = dw.defined() ? dw.data_ptr<float>() : nullptr;
+    SSM_BYTES(n, ssm_rnorm_workspace_bytes, ssm_rnorm_check, a, "ssm_rnorm_bwd");
+    Tensor ws;
+    if (n) {
+      ws = bytes(n, s);
+      a.workspace = ws.data_ptr();
+      a.workspace_bytes = n;
+    }
+    const Launch l(s);
+    l.run_anywhere("ssm_rnorm_bwd", ssm_rnorm_bwd, a);
+    d[0] = dx.view(s.sizes());
+    d[1] = rt == io ? d[0] : dr.defined() ? dr.view(s.sizes()) : dr;
+    d[2] = cast(dw, (at::ScalarType)types[1]);
+    not_twice(d, grads, "add_rms_norm");
+    return d;
+  }
+};
+py::tuple add_rnorm(const Tensor &x, const Tensor &r, const Tensor &weight, double eps) {
+  rnorm_checks(x, r, weight, "add_rms_norm");
+  no_tangents({&x, &r, &weight}, "add_rms_norm");
+  if (x.numel() == 0) {  // no rows: empty tensors in the graph of what was given
+    const Tensor s = cast(x + r, r.scalar_type());
+    return py::make_tuple(cast(s * weight, x.scalar_type()), s);
+  }
+  const variable_list o = needs_grad({&x, &r, &weight}) ? AddRnormFn::apply(x, r, weight, eps) : add_rnorm_forward(x, r, weight, eps);
+  return py::make_tuple(o[0], o[1]);
+}
+// q, scale, s (None without a residual); without weight the rows of x as they are
+py::tuple rnorm8(const Tensor &x, const OptTensor &weight, const OptTensor &residual, double eps) {
+  const Tensor r = get(residual), wt = get(weight);
+  const char *const what = wt.defined() ? "rms_norm_8bit" : "quantize_rows";
+  rnorm_checks(x, r, wt, what);
+  no_graph({&x, &r, &wt}, what);
+  const int64_t C = x.size(-1);
+  const auto lead = x.sizes().slice(0, x.dim() - 1);
+  const Tensor q = at::empty(x.sizes(), x.options().dtype(at::kFloat8_e4m3fn)), scale = at::empty(lead, x.options().dtype(at::kFloat));
+  Tensor s;
+  if (r.defined()) s = at::empty(x.sizes(), r.options());
+  if (x.numel() == 0) return py::make_tuple(q, scale, out(s));
+  const Tensor x2 = rows(x, C), r2 = r.defined() ? rows(r, C) : r, w = wt.defined() ? f32(wt) : wt;
+  ssm_rnorm_args a = rnorm_args(x2, w, x.scalar_type(), r.defined() ? r.scalar_type() : x.scalar_type(), eps);
+  a.x = view(x2); a.residual = view(r2);
+  if (s.defined()) a.sum = view(s.view({-1, C}));
+  a.q = view(q.view({-1, C}));
+  a.scale = scale.data_ptr<float>();
+  const Launch l(x);
+  l.run_anywhere("ssm_rnorm_fwd", ssm_rnorm_fwd, a);
+  return py::make_tuple(q, scale, out(s));
+}
+
+// ------------------------------------------------------------------ token embedding
+ssm_embed_args embed_args(const Tensor &tokens, int64_t V, int64_t D, at::ScalarType io, double scale) {
+  ssm_embed_args a;
+  memset(&a, 0, sizeof(a));
+  a.n = tokens.numel();
+  a.vocab = V;
+  a.dim = D;
+  a.dtype = dtype_code(io);
+  a.scale = scale;
+  a.tokens = tokens.data_ptr<int64_t>();
+  return a;
+}
+Tensor embed_forward(const Tensor &tokens, const Tensor &weight, double scale, at::IntArrayRef shape) {
+  const Tensor w = unit_last(weight), o = at::empty(shape, w.options());
+  ssm_embed_args a = embed_args(tokens, w.size(0), w.size(1), w.scalar_type(), scale);
+  a.weight = view(w);
+  a.out = view(o.view({-1, w.size(1)}));
+  const Launch l(w);
+  l.run_anywhere("ssm_embed_fwd", ssm_embed_fwd, a);
+  return o;
+}
+struct EmbedFn : torch::autograd::Function<EmbedFn> {
+  static Tensor forward(AutogradContext *ctx, const Tensor &weight, const Tensor &tokens, double scale, at::IntArrayRef shape) {
+    ctx->save_for_backward({tokens});
+    ctx->saved_data["scale"] = scale;
+    ctx->saved_data["vocab"] = weight.size(0);
+    return embed_forward(tokens, weight, scale, shape);
+  }
+  static variable_list backward(AutogradContext *ctx, variable_list grads) {
+    const Tensor tokens = ctx->get_saved_variables()[0];
+    const int64_t V = ctx->saved_data["vocab"].toInt(), D = grads[0].size(-1);
+    const Tensor dy = rows(grads[0], D), dw = at::empty({V, D}, dy.options());
+    ssm_embed_args a = embed_args(tokens, V, D, dy.scalar_type(), ctx->saved_data["scale"].toDouble());
+    a.dout = view(dy);
+    a.dweight = dw.data_ptr();
+    SSM_BYTES(n, ssm_embed_workspace_bytes, ssm_embed_check, a, "ssm_embed_bwd");
+    const Tensor ws = bytes(n, dy);
+    a.workspace = ws.data_ptr();
+    a.workspace_bytes = n;
+    const Launch l(dy);
+    l.run_anywhere("ssm_embed_bwd", ssm_embed_bwd, a);
+    variable_list d{dw, Tensor(), Tensor(), Tensor()};
+    not_twice(d, grads, "embedding");
+    return d;
+  }
+};
+Tensor embedding(const Tensor &tokens, const Tensor &weight, double scale) {
+  require_gpu({&tokens, &weight});
+  one_device(weight, {&tokens});
+  no_tangents({&weight}, "embedding");
+  TORCH_CHECK_VALUE(weight.dim() == 2 && weight.size(1) > 0, "weight must be (vocabulary, channels), got ", shape_str(weight.sizes()));
+  TORCH_CHECK_TYPE(delta_type(weight.scalar_type()), "embedding takes float32, bfloat16 or float16, got ", weight.scalar_type());
+  TORCH_CHECK_TYPE(at::isIntegralType(tokens.scalar_type(), false), "tokens must be integers, got ", tokens.scalar_type());
+  std::vector<int64_t> shape(tokens.sizes().begin(), tokens.sizes().end());
+  shape.push_back(weight.size(1));
+  if (tokens.numel() == 0) return weight.narrow(0, 0, 0).reshape(shape);   // in weight's graph
+  const Tensor t = tokens.to(at::kLong).contiguous();
+  if (!needs_grad({&weight})) return embed_forward(t, weight, scale, shape);
+  return EmbedFn::apply(weight, t, scale, at::IntArrayRef(shape));
+}
+
+// ------------------------------------------------------------------ linear layer with its epilogue
+ssm_linear_args linear_args(const Tensor &x2, const Tensor &w, at::ScalarType io, bool in8, int64_t act) {
+  ssm_linear_args a;
+  memset(&a, 0, sizeof(a));
+  a.m = x2.size(0); a.n = w.size(0); a.k = w.size(1);
+  a.dtype = dtype_code(io);
+  a.in8 = in8;
+  a.activation = (int32_t)act;
+  a.x = view(x2);
+  a.weight = view(w);
+  return a;
+}
+std::vector<int64_t> linear_checks(const Tensor &x, const Tensor &w, const Tensor &bias, const Tensor &residual, at::ScalarType io,
+                                   const char *what) {
+  require_gpu({&x, &w, &bias, &residual});
+  one_device(x, {&w, &bias, &residual});
+  TORCH_CHECK_VALUE(w.dim() == 2 && w.size(0) > 0 && w.size(1) > 0, "weight must be (out, in), got ", shape_str(w.sizes()));
+  TORCH_CHECK_VALUE(x.dim() >= 1 && x.size(-1) == w.size(1), "the last dimension of x, ", shape_str(x.sizes()), ", must be weight's ",
+                    w.size(1));
+  TORCH_CHECK_TYPE(io == at::kBFloat16 || io == at::kHalf, what, " takes bfloat16 or float16, got ", io);
+  std::vector<int64_t> shape(x.sizes().begin(), x.sizes().end() - 1);
+  shape.push_back(w.size(0));
+  want("bias", bias, {w.size(0)});
+  want("residual", residual, shape);
+  for (const Tensor *t : {&bias, &residual})
+    TORCH_CHECK_TYPE(!t->defined() || t->scalar_type() == io, what, ": bias and residual must be ", io, ", got ",
+                     t->defined() ? t->scalar_type() : io);
+  return shape;
+}
+void linear_call(ssm_linear_args &a, const Tensor &bias, const Tensor &r2, const Tensor &o, const Tensor &pre) {
+  a.bias = bias.defined() ? bias.data_ptr() : nullptr;
+  a.residual = view(r2);
+  a.out = view(o);
+  a.pre = pre.defined() ? pre.data_ptr() : nullptr;
+  SSM_BYTES(n, ssm_linear_workspace_bytes, ssm_linear_check, a, "ssm_linear_fwd");
+  Tensor ws;
+  if (n) {
+    ws = bytes(n, o);
+    a.workspace = ws.data_ptr();
+    a.workspace_bytes = n;
+  }
+  const Launch l(o);
+  l.run_anywhere("ssm_linear_fwd", ssm_linear_fwd, a);
+}
+// y as rows, x as rows, weight, z before the activation (undefined unless asked for)
+variable_list linear_forward(const Tensor &x, const Tensor &weight, const Tensor &bias, const Tensor &residual, int64_t act,
+                             bool keep) {
+  const int64_t N = weight.size(0);
+  const Tensor x2 = rows(x, x.size(-1)), w = unit_last(weight), b = bias.defined() ? bias.contiguous() : bias;
+  const Tensor r2 = residual.defined() ? rows(residual, N) : residual;
+  const Tensor o = at::empty({x2.size(0), N}, x.options());
+  const Tensor pre = keep && act ? at::empty({x2.size(0), N}, x.options()) : Tensor();
+  ssm_linear_args a = linear_args(x2, w, x.scalar_type(), false, act);
+  linear_call(a, b, r2, o, pre);
+  return {o, x2, w, pre};
+}
+struct LinearFn : torch::autograd::Function<LinearFn> {
+  static Tensor forward(AutogradContext *ctx, const Tensor &x, const Tensor &weight, const OptTensor &bias, const OptTensor &residual,
+                        int64_t act, at::IntArrayRef shape) {
+    const variable_list o = linear_forward(x, weight, get(bias), get(residual), act, true);
+    ctx->save_for_backward({o[1], o[2], o[3]});
+    ctx->saved_data["act"] = act;
+    ctx->saved_data["x"] = x.sizes().vec();
+    ctx->saved_data["bias"] = bias.has_value();
+    ctx->saved_data["residual"] = residual.has_value();
+    return o[0].view(shape);
+  }
+  static variable_list backward(AutogradContext *ctx, variable_list grads) {
+    const variable_list t = ctx->get_saved_variables();
+    const Tensor &x2 = t[0], &w = t[1], &pre = t[2];
+    const bool bias = ctx->saved_data["bias"].toBool(), residual = ctx->saved_data["residual"].toBool();
+    // edges are numbered over the tensors that were given
+    const bool need_x = ctx->needs_input_grad(0), need_w = ctx->needs_input_grad(1), need_b = bias && ctx->needs_input_grad(2);
+    const Tensor dy = rows(grads[0], w.size(0));
+    const Tensor dx = need_x ? at::empty(x2.sizes(), x2.options()) : Tensor();
+    const Tensor dw = need_w ? at::empty(w.sizes(), w.options()) : Tensor();
+    const Tensor db = need_b ? at::empty({w.size(0)}, w.options()) : Tensor();
+    if (need_x || need_w || need_b) {
+      ssm_linear_args a = linear_args(x2, w, x2.scalar_type(), false, ctx->saved_data["act"].toInt());
+      a.pre = pre.defined() ? pre.data_ptr() : nullptr;
+      a.dout = view(dy); a.dx = view(dx); a.dweight = view(dw);
+      a.dbias = need_b ? db.data_ptr() : nullptr;
+      SSM_BYTES(n, ssm_linear_bwd_workspace_bytes, ssm_linear_check, a, "ssm_linear_bwd");
+      Tensor ws;
+      if (n) {
+        ws = bytes(n, dy);
+        a.workspace = ws.data_ptr();
+        a.workspace_bytes = n;
+      }
+      const Launch l(dy);
+      l.run_anywhere("ssm_linear_bwd", ssm_linear_bwd, a);
+    }
+    variable_list d{need_x ? dx.view(ctx->saved_data["x"].toIntVector()) : dx, dw, db,
+                    residual && ctx->needs_input_grad(bias ? 3 : 2) ? grads[0] : Tensor(), Tensor(), Tensor()};
+    not_twice(d, grads, "linear_act");
+    return d;
+  }
+};
+Tensor linear_act(const Tensor &x, const Tensor &weight, const OptTensor &bias_, const OptTensor &residual_, int64_t act) {
+  const Tensor bias = get(bias_), residual = get(residual_);
+  const auto shape = linear_checks(x, weight, bias, residual, x.scalar_type(), "linear_act");
+  TORCH_CHECK_TYPE(weight.scalar_type() == x.scalar_type(), "weight must be of x's type, got ", weight.scalar_type(), " beside ",
+                   x.scalar_type());
+  no_tangents({&x, &weight, &bias, &residual}, "linear_act");
+  if (x.numel() == 0) {  // no rows: an empty tensor in the graph of what was given
+    Tensor y = at::matmul(x, weight.t());
+    for (const Tensor *t : {&bias, &residual})
+      if (t->defined()) y = y + *t;
+    return y;
+  }
+  if (!needs_grad({&x, &weight, &bias, &residual})) return linear_forward(x, weight, bias, residual, act, false)[0].view(shape);
+  return LinearFn::apply(x, weight, bias_, residual_, act, at::IntArrayRef(shape));
+}
+Tensor linear_8bit(const Tensor &q, const Tensor &scale, const Tensor &wq, const Tensor &wscale, const OptTensor &bias_,
+                   const OptTensor &residual_, int64_t act, at::ScalarType io) {
+  const Tensor bias = get(bias_), residual = get(residual_);
+  const auto shape = linear_checks(q, wq, bias, residual, io, "linear_8bit");
+  require_gpu({&scale, &wscale});
+  one_device(q, {&scale, &wscale});
+  for (const Tensor *t : {&q, &wq})
+    TORCH_CHECK_TYPE(t->scalar_type() == at::kFloat8_e4m3fn, "8-bit rows must be float8_e4m3fn, got ", t->scalar_type());
+  for (const Tensor *t : {&scale, &wscale})
+    TORCH_CHECK_TYPE(t->scalar_type() == at::kFloat, "scales must be float32, got ", t->scalar_type());
+  want("scale", scale, q.sizes().slice(0, q.dim() - 1));
+  want("weight_scale", wscale, {wq.size(0)});
+  no_graph({&scale, &wscale, &bias, &residual}, "linear_8bit");
+  const Tensor o = at::empty(shape, q.options().dtype(io));
+  if (q.numel() == 0) return o;
+  const int64_t N = wq.size(0);
+  const Tensor x2 = rows(q, q.size(-1)), w = unit_last(wq), b = bias.defined() ? bias.contiguous() : bias;
+  const Tensor r2 = residual.defined() ? rows(residual, N) : residual, s = scale.contiguous(), ws = wscale.contiguous();
+  ssm_linear_args a = linear_args(x2, w, io, true, act);
+  a.x_scale = s.data_ptr<float>();
+  a.weight_scale = ws.data_ptr<float>();
+  linear_call(a, b, r2, o.view({-1, N}), Tensor());
+  return o;
+}
+
+// ------------------------------------------------------------------ next token
+// A setting: a number for all rows, or a tensor with one per row (returned as the kernel reads it).
+Tensor setting(const char *name, const py::object &v, at::ScalarType type, const Tensor &logits, at::IntArrayRef lead) {
+  if (!THPVariable_Check(v.ptr())) return Tensor();
+  const Tensor t = THPVariable_Unpack(v.ptr());
+  require_gpu({&t});
+  one_device(logits, {&t});
+  want(name, t, lead);
+  const bool whole = at::isIntegralType(t.scalar_type(), false);
+  TORCH_CHECK_TYPE(type == at::kLong ? whole : whole || at::isFloatingType(t.scalar_type()), name, " cannot be of type ", t.scalar_type());
+  return t.to(type).contiguous();
+}
+py::tuple sample(const Tensor &logits, const Tensor &u_, const py::object &temperature, const py::object &top_k, const py::object &top_p,
+                 const py::object &min_p) {
+  require_gpu({&logits, &u_});
+  one_device(logits, {&u_});
+  TORCH_CHECK_VALUE(logits.dim() >= 1 && logits.size(-1) > 0, "logits must be (..., vocabulary), got ", shape_str(logits.sizes()));
+  TORCH_CHECK_TYPE(delta_type(logits.scalar_type()), "logits must be float32, bfloat16 or float16, got ", logits.scalar_type());
+  TORCH_CHECK_TYPE(u_.scalar_type() == at::kFloat || u_.scalar_type() == at::kDouble, "u must be float32 or float64, got ", u_.scalar_type());
+  no_graph({&logits}, "sample");
+  const auto lead = logits.sizes().slice(0, logits.dim() - 1);
+  want("u", u_, lead);
+  const Tensor t = setting("temperature", temperature, at::kFloat, logits, lead), k = setting("top_k", top_k, at::kLong, logits, lead),
+               p = setting("top_p", top_p, at::kFloat, logits, lead), m = setting("min_p", min_p, at::kFloat, logits, lead);
+  const Tensor token = at::empty(lead, logits.options().dtype(at::kLong)), logprob = at::empty(lead, logits.options().dtype(at::kFloat));
+  ssm_sample_args a;
+  memset(&a, 0, sizeof(a));
+  a.temperature = t.defined() ? 1.0 : temperature.cast<double>();
+  a.top_k = k.defined() || top_k.is_none() ? 0 : top_k.cast<int64_t>();
+  a.top_p = p.defined() || top_p.is_none() ? 1.0 : top_p.cast<double>();
+  a.min_p = m.defined() || min_p.is_none() ? 0.0 : min_p.cast<double>();
+  a.vocab = logits.size(-1);
+  a.rows = logits.numel() / a.vocab;
+  const bool none = a.rows == 0;
+  if (none) a.rows = 1;   // the settings are checked all the same
+  a.dtype = dtype_code(logits.scalar_type());
+  SSM_BYTES(n, ssm_sample_workspace_bytes, ssm_sample_check, a, "ssm_sample");
+  if (none) return py::make_tuple(token, logprob);
+  const Tensor x2 = rows(logits, a.vocab), u = u_.contiguous();
+  a.logits = view(x2);
+  a.u = u.data_ptr();
+  a.u_f64 = u.scalar_type() == at::kDouble;
+  a.temperatures = t.defined() ? t.data_ptr<float>() : nullptr;
+  a.top_ks = k.defined() ? k.data_ptr<int64_t>() : nullptr;
+  a.top_ps = p.defined() ? p.data_ptr<float>() : nullptr;
+  a.min_ps = m.defined() ? m.data_ptr<float>() : nullptr;
+  a.token = token.data_ptr<int64_t>();
+  a.logprob = logprob.data_ptr<float>();
+  Tensor ws;
+  if (n) {
+    ws = bytes(n, logits);
+    a.workspace = ws.data_ptr();
+    a.workspace_bytes = n;
+  }
+  const Launch l(logits);
+  l.run_anywhere("ssm_sample", ssm_sample, a);
+  return py::make_tuple(token, logprob);
+}
+
 // ------------------------------------------------------------------ decode
 // The weights of a block stack's token step, laid out once; a step brings tokens and states.
 struct DecodePlan {
@@ -942,6 +1320,12 @@ PYBIND11_MODULE(_ssmhost, m) {
   m.def("delta", torch::wrap_pybind_function(delta));
   m.def("delta_step", torch::wrap_pybind_function(delta_step));
   m.def("gnorm", torch::wrap_pybind_function(gnorm));
+  m.def("add_rnorm", torch::wrap_pybind_function(add_rnorm));
+  m.def("rnorm8", torch::wrap_pybind_function(rnorm8));
+  m.def("embedding", torch::wrap_pybind_function(embedding));
+  m.def("linear_act", torch::wrap_pybind_function(linear_act));
+  m.def("linear_8bit", torch::wrap_pybind_function(linear_8bit));
+  m.def("sample", torch::wrap_pybind_function(sample));
   m.attr("ABI_VERSION") = SSM_ABI_VERSION;  // of the header the argument structs above were compiled from
   py::class_<DecodePlan>(m, "DecodePlan")
       .def(py::init<const std::vector<std::pair<std::vector<Tensor>, double>> &, Tensor, int64_t, int64_t, int64_t, int64_t,

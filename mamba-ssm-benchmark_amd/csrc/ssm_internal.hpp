@@ -360,6 +360,98 @@ inline int64_t gnorm_slots(int64_t R, int64_t C) {
 }
 hipError_t launch_gnorm(const GnormParams &p, int dtype, bool bwd, hipStream_t s);
 
+// Root-mean-square norm with the residual's addition, and its 8-bit form.
+constexpr int kRnormMaxDim = 16384;
+struct RnormParams {
+  int64_t R;
+  int C, vec;                          // vec: rows load 16 bytes of x's type at a time
+  float eps;
+  const void *x, *res, *dy, *ds;
+  const float *w;                      // null: rows as they are (8-bit form only)
+  void *s, *y, *dx, *dres;             // s: written by the forward with a residual, read by the backward
+  uint8_t *q;                          // 8-bit rows in y's place, or null
+  float *scale;
+  int64_t sx, sr, sdy, sds, ss, sy, sq, sdx, sdr;  // row strides
+  float *dw, *ws;                      // (C,) or null; partial rows
+  int nblk;
+  int64_t first;                       // forward: rows of earlier launches
+};
+// Wavefronts a row: the fewest that hold it in 4 loads a lane; where there are few rows, more of them.
+inline int rnorm_waves(int64_t R, int64_t C, int V) {
+  const int64_t least = C <= 256 * V ? 1 : C <= 1024 * V ? 4 : 16;
+  if (R < 1024 && least == 1 && C > 64 * V) return 4;
+  return (int)least;
+}
+inline int64_t rnorm_blocks(int64_t R, int W) {
+  const int64_t want = W == 1 ? (R + 3) / 4 : R, most = W == 16 ? 512 : 1024;
+  return want < most ? want : most;
+}
+hipError_t launch_rnorm(const RnormParams &p, int dtype, int rdtype, bool bwd, hipStream_t s);
+
+// Token embedding and its gradient.
+constexpr int kEmbedBits = 9;          // of a sorting pass
+constexpr int64_t kEmbedWaves = 128;   // wavefronts that sort, at most
+constexpr int kEmbedPiece = 64;        // sorted places that are summed at once where they hold one token
+constexpr int kEmbedGroup = 32;        // pieces likewise
+struct EmbedParams {
+  int64_t n, V, D;
+  int vec, lanes;                      // lanes: threads a row
+  float scale;
+  const int64_t *tokens;
+  const void *w, *dout;
+  void *out, *dw;
+  int64_t sw, so, sd;                  // row strides
+  int64_t first;                       // rows of earlier launches
+  // gradient
+  int pass, bits, shift;
+  int64_t nw, per;                     // sorting wavefronts, items of each
+  uint32_t *hist;                      // (nw, 2^bits)
+  const uint32_t *key_in, *pos_in;
+  uint32_t *key_out, *pos_out;
+  uint32_t *key[2], *pos[2];           // (n,) each: the passes' outputs in turn
+  uint32_t *start;                     // (V + 1)
+  float *piece, *group;                // sums of whole pieces, of whole groups (null: not formed)
+  int64_t npiece_blocks;
+};
+hipError_t launch_embed(const EmbedParams &p, int dtype, bool bwd, hipStream_t s);
+
+// The draw of the next token.
+struct SampleParams {
+  int64_t R, V, first;                 // first: rows of earlier launches
+  const void *logits, *u;
+  int64_t sl;
+  int u_f64, shift;                    // weights are integers of 2^-shift
+  double temperature, top_p, min_p;
+  int64_t top_k;                       // 0: all
+  const float *temperatures, *top_ps, *min_ps;  // per row, in the settings' place where given
+  const int64_t *top_ks;
+  int64_t *token;
+  float *logprob;
+};
+hipError_t launch_sample(const SampleParams &p, int dtype, hipStream_t s);
+
+// Products C[m, n] = sum over k of A(m, k) B(n, k) with the linear layer's epilogue.
+enum { kActNone = 0, kActSilu = 1, kActGelu = 2 };
+struct GemmParams {
+  int64_t M, N, K;
+  const void *A, *B;
+  int a_along, b_along;                // stored along k (rows of k), or along m, n
+  int64_t sa, sb, sc, sr, spre;        // row strides
+  int fp8, act;
+  const void *bias, *residual;
+  const float *xs, *ws;                // 8 bits: scales per row of A, of B
+  void *C, *pre;                       // pre: z before the activation, or null
+};
+hipError_t launch_gemm(const GemmParams &p, int dtype, hipStream_t s);
+struct LinearDzParams {
+  int64_t M, N, sdy;
+  int act, slots;                      // slots: ranges of rows
+  const void *dy, *pre;                // pre, dz: (M, N) dense
+  void *dz, *dbias;
+  float *partial;                      // (slots, N)
+};
+hipError_t launch_linear_dz(const LinearDzParams &p, int dtype, hipStream_t s);
+
 // Runs the summary and carry passes first when p.nseg > 1.
 hipError_t launch_fwd(const FwdParams &p, int dtype, int method, int np, hipStream_t s);
 hipError_t launch_bwd(const BwdParams &p, int dtype, int method, int np, hipStream_t s);

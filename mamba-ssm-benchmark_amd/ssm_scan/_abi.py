@@ -11,7 +11,7 @@ import os
 import torch
 
 LIB_PATH = os.path.join(os.path.dirname(os.path.abspath(__file__)), "libssmscan.so")
-ABI_VERSION = 9
+ABI_VERSION = 10
 
 OK, EINVAL, EKEY, ESPACE, EHIP = 0, 1, 2, 3, 4
 ZOH, EULER, BILINEAR = 0, 1, 2
@@ -168,6 +168,33 @@ class GnormArgs(ctypes.Structure):
                 ("workspace", c_vp), ("workspace_bytes", c_i64)]
 
 
+class RnormArgs(ctypes.Structure):
+    _fields_ = [("rows", c_i64), ("dim", c_i64), ("dtype", c_i32), ("res_dtype", c_i32), ("eps", ctypes.c_double),
+                ("x", Tensor), ("residual", Tensor), ("weight", c_vp), ("sum", Tensor), ("out", Tensor), ("q", Tensor),
+                ("scale", c_vp), ("dout", Tensor), ("dsum", Tensor), ("dx", Tensor), ("dresidual", Tensor),
+                ("dweight", c_vp), ("workspace", c_vp), ("workspace_bytes", c_i64)]
+
+
+class EmbedArgs(ctypes.Structure):
+    _fields_ = [("n", c_i64), ("vocab", c_i64), ("dim", c_i64), ("dtype", c_i32), ("reserved0", c_i32),
+                ("scale", ctypes.c_double), ("tokens", c_vp), ("weight", Tensor), ("out", Tensor), ("dout", Tensor),
+                ("dweight", c_vp), ("workspace", c_vp), ("workspace_bytes", c_i64)]
+
+
+class LinearArgs(ctypes.Structure):
+    _fields_ = [("m", c_i64), ("n", c_i64), ("k", c_i64), ("dtype", c_i32), ("in8", c_i32), ("activation", c_i32),
+                ("reserved0", c_i32), ("x", Tensor), ("weight", Tensor), ("x_scale", c_vp), ("weight_scale", c_vp),
+                ("bias", c_vp), ("residual", Tensor), ("out", Tensor), ("pre", c_vp), ("dout", Tensor), ("dx", Tensor),
+                ("dweight", Tensor), ("dbias", c_vp), ("workspace", c_vp), ("workspace_bytes", c_i64)]
+
+
+class SampleArgs(ctypes.Structure):
+    _fields_ = [("rows", c_i64), ("vocab", c_i64), ("dtype", c_i32), ("u_f64", c_i32), ("logits", Tensor), ("u", c_vp),
+                ("temperature", ctypes.c_double), ("top_p", ctypes.c_double), ("min_p", ctypes.c_double), ("top_k", c_i64),
+                ("temperatures", c_vp), ("top_ps", c_vp), ("min_ps", c_vp), ("top_ks", c_vp), ("token", c_vp),
+                ("logprob", c_vp), ("workspace", c_vp), ("workspace_bytes", c_i64)]
+
+
 # name -> (restype, argtypes)
 _SIGS = {
     "ssm_abi_version": (c_i32, []),
@@ -223,6 +250,22 @@ _SIGS = {
     "ssm_delta_step": (c_i32, [ctypes.POINTER(DeltaStepArgs), c_vp]),
     "ssm_gnorm_fwd": (c_i32, [ctypes.POINTER(GnormArgs), c_vp]),
     "ssm_gnorm_bwd": (c_i32, [ctypes.POINTER(GnormArgs), c_vp]),
+    "ssm_rnorm_check": (c_i32, [ctypes.POINTER(RnormArgs)]),
+    "ssm_rnorm_workspace_bytes": (c_i64, [ctypes.POINTER(RnormArgs)]),
+    "ssm_rnorm_fwd": (c_i32, [ctypes.POINTER(RnormArgs), c_vp]),
+    "ssm_rnorm_bwd": (c_i32, [ctypes.POINTER(RnormArgs), c_vp]),
+    "ssm_embed_check": (c_i32, [ctypes.POINTER(EmbedArgs)]),
+    "ssm_embed_workspace_bytes": (c_i64, [ctypes.POINTER(EmbedArgs)]),
+    "ssm_embed_fwd": (c_i32, [ctypes.POINTER(EmbedArgs), c_vp]),
+    "ssm_embed_bwd": (c_i32, [ctypes.POINTER(EmbedArgs), c_vp]),
+    "ssm_linear_check": (c_i32, [ctypes.POINTER(LinearArgs)]),
+    "ssm_linear_workspace_bytes": (c_i64, [ctypes.POINTER(LinearArgs)]),
+    "ssm_linear_fwd": (c_i32, [ctypes.POINTER(LinearArgs), c_vp]),
+    "ssm_linear_bwd": (c_i32, [ctypes.POINTER(LinearArgs), c_vp]),
+    "ssm_sample_check": (c_i32, [ctypes.POINTER(SampleArgs)]),
+    "ssm_sample_workspace_bytes": (c_i64, [ctypes.POINTER(SampleArgs)]),
+    "ssm_sample": (c_i32, [ctypes.POINTER(SampleArgs), c_vp]),
+    "ssm_linear_bwd_workspace_bytes": (c_i64, [ctypes.POINTER(LinearArgs)]),
     "ssm_cscan_tile": (c_i64, [c_i32, c_i32]),
     "ssm_default_chunk": (c_i64, [c_i64]),
     "ssm_scan_blocks": (c_i64, [c_i64, c_i64, c_i64, c_i64, c_i64, ctypes.POINTER(c_i64), c_i64]),

@@ -9,10 +9,15 @@ S independent products in one batched GEMM followed by a fixed-order sum over th
 fills the GPU: on one MI355X (float32) 45 / 26 / 26 / 25 us against 60 / 55 / 45 / 53 us.
 The forward and the input gradient stay the plain GEMMs of F.linear; the parameters are the
 nn.Linear modules' own (models/mamba.py, models/lm.py use nn.Linear).
+
+``linear_act`` (16 bits, trained) and ``linear_8bit`` (8-bit rows with scales, for serving) are products of the engine's
+own on the matrix cores, with bias, activation and residual in their epilogue.
 """
 
 import torch
 import torch.nn.functional as F
+
+from . import _abi
 
 SPLITS = 8          # token slices of the weight gradient
 MIN_TOKENS = 2048   # below this the plain product already fills the GPU as well
@@ -87,6 +92,33 @@ def linear(layer, x):
         return _SplitKLinear.apply(x, w, layer.bias)
     with rocblas():
         return layer(x)
+
+
+_ACTIVATIONS = {None: 0, "silu": 1, "gelu": 2}
+
+
+def _activation(activation):
+    if activation not in _ACTIVATIONS:
+        raise ValueError(f"unknown activation {activation!r}")
+    return _ACTIVATIONS[activation]
+
+
+def linear_act(x, weight, bias=None, activation=None, residual=None):
+    """act(x weight^T + bias) + residual, (..., N) in x's type.
+
+    x (..., K), weight (N, K), bias (N,), residual (..., N), all bfloat16 or all float16 (float32 layers: linear);
+    activation None, "silu" or "gelu" (z Phi(z)).  Sums and the epilogue are float32, the result is rounded once.
+    Differentiable (once, reverse mode) in every tensor; with an activation the forward keeps z, rounded to x's type."""
+    return _abi.host().linear_act(x, weight, bias, residual, _activation(activation))
+
+
+def linear_8bit(q, scale, weight, weight_scale, bias=None, activation=None, residual=None, dtype=torch.bfloat16):
+    """act((q scale) (weight weight_scale)^T + bias) + residual, (..., N) in dtype (bfloat16 or float16).
+
+    q (..., K) with scale (...) as rms_norm_8bit gives them, weight (N, K) with weight_scale (N,) as
+    quantize_rows does: torch.float8_e4m3fn rows with a float32 scale each.  bias (N,) and residual (..., N) of
+    dtype.  Products of 8-bit values are exact, sums and the epilogue float32.  Not differentiable."""
+    return _abi.host().linear_8bit(q, scale, weight, weight_scale, bias, residual, _activation(activation), dtype)
 
 
 MAX_DENSE_VOCAB = 4096  # vocabularies up to this size take the one-hot product
