@@ -1571,45 +1571,88 @@ int ssm_linear_check(const ssm_linear_args *a) {
   if (!rc && a->in8) rc = need({{a->x_scale, "x_scale"}, {a->weight_scale, "weight_scale"}});
   return rc ? rc : ok();
 }
-int64_t ssm_linear_workspace_bytes(const ssm_linear_args *a) {
-  if (ssm_linear_check(a)) return -1;
-  return 0;
-}
 namespace {
-int64_t linear_slots(const ssm_linear_args *a) { return std::min<int64_t>(64, cdiv(a->m, 64)); }
-struct LinearBwdLayout {
-  int64_t dz, partial;
-  int64_t bytes() const { return dz + partial; }
-};
-LinearBwdLayout linear_bwd_layout(const ssm_linear_args *a) {
-  LinearBwdLayout l{};
-  if (a->activation) l.dz = align256(a->m * a->n * 2);
-  if (a->dbias) l.partial = align256(linear_slots(a) * a->n * 4);
-  return l;
-}
-}  // namespace
-int64_t ssm_linear_bwd_workspace_bytes(const ssm_linear_args *a) {
-  if (ssm_linear_check(a)) return -1;
-  return linear_bwd_layout(a).bytes();
-}
-int ssm_linear_fwd(const ssm_linear_args *a, void *stream) {
-  int rc = ssm_linear_check(a);
-  if (!rc) rc = gnorm_view(a->out, "out");
-  if (!rc && has(a->residual)) rc = gnorm_view(a->residual, "residual");
-  if (rc) return rc;
+GemmParams linear_forward_params(const ssm_linear_args *a) {
   GemmParams p{};
   p.M = a->m; p.N = a->n; p.K = a->k;
   p.A = a->x.data; p.sa = a->x.stride[0]; p.a_along = 1;
   p.B = a->weight.data; p.sb = a->weight.stride[0]; p.b_along = 1;
   p.C = a->out.data; p.sc = a->out.stride[0];
-  p.fp8 = a->in8;
+  p.fp8 = a->in8 != 0;
   p.xs = a->in8 ? a->x_scale : nullptr;
   p.ws = a->in8 ? a->weight_scale : nullptr;
   p.act = a->activation;
   p.bias = a->bias;
   p.residual = a->residual.data; p.sr = a->residual.stride[0];
   p.pre = a->activation ? a->pre : nullptr; p.spre = a->n;
-  hipError_t e = launch_gemm(p, a->dtype, (hipStream_t)stream);
+  return p;
+}
+// The backward: dz (formed where there is an activation, or where the products cannot read dout as it lies), the
+// products dx and dweight one after the other in one workspace.
+struct LinearBwd {
+  bool own_dz;
+  int64_t dz, partial, products;
+  LinearDzParams d;
+  GemmParams dx, dw;
+  int64_t bytes() const { return dz + partial + products; }
+};
+LinearBwd linear_backward_plan(const ssm_linear_args *a) {
+  LinearBwd l{};
+  const int64_t wide = (a->n + 7) / 8 * 8;
+  const bool whole = a->n % 8 == 0 && (uintptr_t)a->dout.data % 16 == 0 && a->dout.stride[0] % 8 == 0 && a->dout.stride[0] >= a->n;
+  l.own_dz = a->activation || ((has(a->dx) || has(a->dweight)) && !whole);
+  if (l.own_dz) l.dz = align256(a->m * wide * 2);
+  LinearDzParams &d = l.d;
+  d.M = a->m; d.N = a->n;
+  d.act = a->activation;
+  d.dy = a->dout.data; d.sdy = a->dout.stride[0]; d.sdz = wide;
+  d.pre = a->pre;
+  d.dz = l.own_dz ? a->workspace : nullptr;
+  // ranges of 32 rows and more, as many as make 1024 workgroups
+  d.slots = (int)std::max<int64_t>(1, std::min(cdiv(a->m, 32), cdiv(1024, cdiv(wide, 64))));
+  d.dbias = a->dbias;
+  if (a->dbias) {
+    l.partial = align256(d.slots * a->n * 4);
+    d.partial = (float *)((char *)a->workspace + l.dz);
+  }
+  const void *dz = l.own_dz ? a->workspace : a->dout.data;
+  const int64_t sdz = l.own_dz ? wide : a->dout.stride[0];
+  if (has(a->dx)) {   // dx[m, k] = sum over n of dz[m, n] weight[n, k]
+    GemmParams &p = l.dx;
+    p.M = a->m; p.N = a->k; p.K = a->n;
+    p.A = dz; p.sa = sdz; p.a_along = 1; p.a_padded = 1;
+    p.B = a->weight.data; p.sb = a->weight.stride[0]; p.b_along = 0;
+    p.C = a->dx.data; p.sc = a->dx.stride[0];
+    l.products = linear_plan(p).bytes();
+  }
+  if (has(a->dweight)) {   // dweight[n, k] = sum over m of dz[m, n] x[m, k]
+    GemmParams &p = l.dw;
+    p.M = a->n; p.N = a->k; p.K = a->m;
+    p.A = dz; p.sa = sdz; p.a_along = 0;
+    p.B = a->x.data; p.sb = a->x.stride[0]; p.b_along = 0;
+    p.C = a->dweight.data; p.sc = a->dweight.stride[0];
+    l.products = std::max(l.products, linear_plan(p).bytes());
+  }
+  return l;
+}
+}  // namespace
+int64_t ssm_linear_workspace_bytes(const ssm_linear_args *a) {
+  if (ssm_linear_check(a)) return -1;
+  return linear_plan(linear_forward_params(a)).bytes();
+}
+int64_t ssm_linear_bwd_workspace_bytes(const ssm_linear_args *a) {
+  if (ssm_linear_check(a)) return -1;
+  return linear_backward_plan(a).bytes();
+}
+int ssm_linear_fwd(const ssm_linear_args *a, void *stream) {
+  int rc = ssm_linear_check(a);
+  if (!rc) rc = gnorm_view(a->out, "out");
+  if (!rc && has(a->residual)) rc = gnorm_view(a->residual, "residual");
+  if (rc) return rc;
+  const int64_t bytes = ssm_linear_workspace_bytes(a);
+  if (bytes && (!a->workspace || a->workspace_bytes < bytes))
+    return fail(SSM_ESPACE, "workspace of %lld bytes required", (long long)bytes);
+  hipError_t e = launch_gemm(linear_forward_params(a), a->dtype, a->workspace, (hipStream_t)stream);
   return e == hipSuccess ? ok() : hip_fail(e, "ssm_linear_fwd");
 }
 int ssm_linear_bwd(const ssm_linear_args *a, void *stream) {
@@ -1620,42 +1663,14 @@ int ssm_linear_bwd(const ssm_linear_args *a, void *stream) {
   if (!rc && has(a->dx)) rc = gnorm_view(a->dx, "dx");
   if (!rc && has(a->dweight)) rc = gnorm_view(a->dweight, "dweight");
   if (rc) return rc;
-  const LinearBwdLayout l = linear_bwd_layout(a);
+  const LinearBwd l = linear_backward_plan(a);
   if (l.bytes() && (!a->workspace || a->workspace_bytes < l.bytes()))
     return fail(SSM_ESPACE, "workspace of %lld bytes required", (long long)l.bytes());
-  const void *dz = a->dout.data;
-  int64_t sdz = a->dout.stride[0];
+  void *products = (char *)a->workspace + l.dz + l.partial;
   hipError_t e = hipSuccess;
-  if (a->activation || a->dbias) {
-    LinearDzParams d{};
-    d.M = a->m; d.N = a->n;
-    d.act = a->activation;
-    d.dy = a->dout.data; d.sdy = a->dout.stride[0];
-    d.pre = a->pre;
-    d.slots = (int)linear_slots(a);
-    d.dbias = a->dbias;
-    if (a->dbias) d.partial = (float *)((char *)a->workspace + l.dz);
-    if (a->activation) {
-      dz = d.dz = a->workspace;
-      sdz = a->n;
-    }
-    e = launch_linear_dz(d, a->dtype, (hipStream_t)stream);
-  }
-  GemmParams p{};
-  if (e == hipSuccess && has(a->dx)) {   // dx[m, k] = sum over n of dz[m, n] weight[n, k]
-    p.M = a->m; p.N = a->k; p.K = a->n;
-    p.A = dz; p.sa = sdz; p.a_along = 1;
-    p.B = a->weight.data; p.sb = a->weight.stride[0]; p.b_along = 0;
-    p.C = a->dx.data; p.sc = a->dx.stride[0];
-    e = launch_gemm(p, a->dtype, (hipStream_t)stream);
-  }
-  if (e == hipSuccess && has(a->dweight)) {   // dweight[n, k] = sum over m of dz[m, n] x[m, k]
-    p.M = a->n; p.N = a->k; p.K = a->m;
-    p.A = dz; p.sa = sdz; p.a_along = 0;
-    p.B = a->x.data; p.sb = a->x.stride[0]; p.b_along = 0;
-    p.C = a->dweight.data; p.sc = a->dweight.stride[0];
-    e = launch_gemm(p, a->dtype, (hipStream_t)stream);
-  }
+  if (l.own_dz || a->dbias) e = launch_linear_dz(l.d, a->dtype, (hipStream_t)stream);
+  if (e == hipSuccess && has(a->dx)) e = launch_gemm(l.dx, a->dtype, products, (hipStream_t)stream);
+  if (e == hipSuccess && has(a->dweight)) e = launch_gemm(l.dw, a->dtype, products, (hipStream_t)stream);
   return e == hipSuccess ? ok() : hip_fail(e, "ssm_linear_bwd");
 }
 

@@ -436,17 +436,31 @@ struct GemmParams {
   int64_t M, N, K;
   const void *A, *B;
   int a_along, b_along;                // stored along k (rows of k), or along m, n
+  int a_padded;                        // rows of A end in zeros up to whole 16 bytes
   int64_t sa, sb, sc, sr, spre;        // row strides
-  int fp8, act;
+  int fp8, act, splits;                // splits: ranges of k, whose sums are joined
   const void *bias, *residual;
   const float *xs, *ws;                // 8 bits: scales per row of A, of B
   void *C, *pre;                       // pre: z before the activation, or null
+  float *partial;                      // (splits, M, N)
 };
-hipError_t launch_gemm(const GemmParams &p, int dtype, hipStream_t s);
+struct LinearPlan {
+  int rows, MT, NT;                    // the kernel for few rows, of 16 MT rows and 16 NT columns a workgroup
+  int tile, splits;                    // else tiles of tile x tile
+  int64_t pack_a, pack_b, partial;     // workspace bytes: operands that are copied into whole rows, sums of the splits
+  int64_t bytes() const { return pack_a + pack_b + partial; }
+};
+LinearPlan linear_plan(const GemmParams &p);
+hipError_t launch_gemm(const GemmParams &p, int dtype, void *workspace, hipStream_t s);
+struct LinearPack {
+  const void *from;
+  void *to;
+  int64_t rows, cols, stride, to_stride;
+};
 struct LinearDzParams {
-  int64_t M, N, sdy;
+  int64_t M, N, sdy, sdz;              // sdz: N up to whole 16 bytes
   int act, slots;                      // slots: ranges of rows
-  const void *dy, *pre;                // pre, dz: (M, N) dense
+  const void *dy, *pre;                // pre: (M, N) dense
   void *dz, *dbias;
   float *partial;                      // (slots, N)
 };

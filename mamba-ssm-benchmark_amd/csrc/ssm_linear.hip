@@ -16,18 +16,37 @@ typedef _Float16 lh8 __attribute__((ext_vector_type(8)));
 
 struct fp8_t { uint8_t bits; };
 
+typedef int li4 __attribute__((ext_vector_type(4)));
+typedef int li8 __attribute__((ext_vector_type(8)));
+typedef short ls4 __attribute__((ext_vector_type(4)));
+typedef __attribute__((address_space(3))) void *LdsPtr;
+typedef __attribute__((address_space(3))) ls4 *LdsTr;
+
+// One matrix instruction: lane l holds of the first operand row l % 16 (of the 16 x 16 result row 4 (l / 16) + i), of the
+// second column l % 16, and of both `bytes` bytes of k from bytes * (l / 16) on.
 template <typename T> struct Mma;
 template <> struct Mma<bf16_t> {
-  typedef lbf8 Frag;   // 8 consecutive k of a row
-  __device__ __forceinline__ static lf4 mul(Frag a, Frag b, lf4 c) { return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0); }
+  static constexpr int bytes = 16;
+  typedef li4 Frag;
+  __device__ __forceinline__ static lf4 mul(Frag a, Frag b, lf4 c) {
+    return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(lbf8, a), __builtin_bit_cast(lbf8, b), c, 0, 0, 0);
+  }
 };
 template <> struct Mma<f16_t> {
-  typedef lh8 Frag;
-  __device__ __forceinline__ static lf4 mul(Frag a, Frag b, lf4 c) { return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0); }
+  static constexpr int bytes = 16;
+  typedef li4 Frag;
+  __device__ __forceinline__ static lf4 mul(Frag a, Frag b, lf4 c) {
+    return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(lh8, a), __builtin_bit_cast(lh8, b), c, 0, 0, 0);
+  }
 };
+// 128 k of e4m3, scales of one.  The instruction adds 8 products at a time in steps of 2^-13 of the largest one's power
+// of two: what it loses is far below e4m3's own 2^-4 of each factor.
 template <> struct Mma<fp8_t> {
-  typedef long Frag;
-  __device__ __forceinline__ static lf4 mul(Frag a, Frag b, lf4 c) { return __builtin_amdgcn_mfma_f32_16x16x32_fp8_fp8(a, b, c, 0, 0, 0); }
+  static constexpr int bytes = 32;
+  typedef li8 Frag;
+  __device__ __forceinline__ static lf4 mul(Frag a, Frag b, lf4 c) {
+    return __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(a, b, c, 0, 0, 0, 0x7f7f7f7f, 0, 0x7f7f7f7f);
+  }
 };
 
 __device__ __forceinline__ float lin_act(float z, int act) {
@@ -44,84 +63,357 @@ __device__ __forceinline__ float lin_slope(float z, int act) {
   return 1.0f;
 }
 
-// ------------------------------------------------------------------ any size, stride and alignment
-// A workgroup of four wavefronts takes 64 x 64 of C, a wavefront 32 x 32 of it; both operands' 64 x 32 tiles pass
-// through registers into LDS, [row][k] whatever their storage, zeros past their ends.
-template <typename T> __device__ __forceinline__ T lin_zero() { return T{}; }
-template <typename T, typename OT>
-__global__ void __launch_bounds__(256) k_linear_any(const GemmParams p) {
-  constexpr int BK = 32, LD = BK + 8;
-  __shared__ __attribute__((aligned(16))) T As[64][LD], Bs[64][LD];
-  const int lane = threadIdx.x % 64, wave = threadIdx.x / 64;
-  const int64_t tn = (p.N + 63) / 64, m0 = blockIdx.x / tn * 64, n0 = blockIdx.x % tn * 64;
-  const int wm = (wave / 2) * 32, wn = (wave % 2) * 32;
-  lf4 acc[2][2] = {};
-  for (int64_t k0 = 0; k0 < p.K; k0 += BK) {
-    __syncthreads();
+// ------------------------------------------------------------------ epilogue
+// W consecutive n of row m (those past N are not there); rows may begin anywhere.
+template <typename OT, int W>
+__device__ __forceinline__ void lin_load(const OT *src, int64_t left, float (&v)[W]) {
+  OT e[W];
+  if (left >= W) {
+    __builtin_memcpy(e, src, sizeof(e));
+  } else {
 #pragma unroll
-    for (int e = 0; e < 8; ++e) {
-      const int id = threadIdx.x + 256 * e;
-      {
-        const int row = p.a_along ? id / BK : id % 64, k = p.a_along ? id % BK : id / 64;
-        As[row][k] = m0 + row < p.M && k0 + k < p.K ? ((const T *)p.A)[(m0 + row) * (p.a_along ? p.sa : 1) + (k0 + k) * (p.a_along ? 1 : p.sa)] : lin_zero<T>();
-      }
-      {
-        const int row = p.b_along ? id / BK : id % 64, k = p.b_along ? id % BK : id / 64;
-        Bs[row][k] = n0 + row < p.N && k0 + k < p.K ? ((const T *)p.B)[(n0 + row) * (p.b_along ? p.sb : 1) + (k0 + k) * (p.b_along ? 1 : p.sb)] : lin_zero<T>();
-      }
-    }
-    __syncthreads();
-    typename Mma<T>::Frag a[2], b[2];
-#pragma unroll
-    for (int i = 0; i < 2; ++i) {
-      a[i] = *(const typename Mma<T>::Frag *)&As[wm + 16 * i + lane % 16][8 * (lane / 16)];
-      b[i] = *(const typename Mma<T>::Frag *)&Bs[wn + 16 * i + lane % 16][8 * (lane / 16)];
-    }
-#pragma unroll
-    for (int i = 0; i < 2; ++i)
-#pragma unroll
-      for (int j = 0; j < 2; ++j) acc[i][j] = Mma<T>::mul(b[j], a[i], acc[i][j]);   // rows of the result: n
+    for (int q = 0; q < W; ++q) e[q] = q < left ? src[q] : OT{};
   }
 #pragma unroll
-  for (int i = 0; i < 2; ++i)
+  for (int q = 0; q < W; ++q) v[q] = Conv<OT>::load(&e[q]);
+}
+template <typename OT, int W>
+__device__ __forceinline__ void lin_store(OT *dst, int64_t left, const float (&v)[W]) {
+  OT e[W];
 #pragma unroll
-    for (int j = 0; j < 2; ++j)
+  for (int q = 0; q < W; ++q) Conv<OT>::store(&e[q], v[q]);
+  if (left >= W) {
+    __builtin_memcpy(dst, e, sizeof(e));
+  } else {
 #pragma unroll
-      for (int q = 0; q < 4; ++q) {
-        const int64_t m = m0 + wm + 16 * i + lane % 16, n = n0 + wn + 16 * j + 4 * (lane / 16) + q;
-        if (m >= p.M || n >= p.N) continue;
-        float z = acc[i][j][q];
-        if (p.xs) z *= p.xs[m] * p.ws[n];
-        if (p.bias) z += Conv<OT>::load((const OT *)p.bias + n);
-        if (p.pre) Conv<OT>::store((OT *)p.pre + m * p.spre + n, z);
-        z = lin_act(z, p.act);
-        if (p.residual) z += Conv<OT>::load((const OT *)p.residual + m * p.sr + n);
-        Conv<OT>::store((OT *)p.C + m * p.sc + n, z);
+    for (int q = 0; q < W; ++q)
+      if (q < left) dst[q] = e[q];
+  }
+}
+template <typename OT, int W>
+__device__ __forceinline__ void lin_epilogue(const GemmParams &p, int64_t m, int64_t n, float (&z)[W]) {
+  const int64_t left = p.N - n;
+  if (p.xs) {
+    float ws[W];
+    lin_load<float, W>(p.ws + n, left, ws);
+    const float xs = p.xs[m];
+#pragma unroll
+    for (int q = 0; q < W; ++q) z[q] *= xs * ws[q];
+  }
+  if (p.bias) {
+    float b[W];
+    lin_load<OT, W>((const OT *)p.bias + n, left, b);
+#pragma unroll
+    for (int q = 0; q < W; ++q) z[q] += b[q];
+  }
+  if (p.act) {
+    if (p.pre) lin_store<OT, W>((OT *)p.pre + m * p.spre + n, left, z);
+#pragma unroll
+    for (int q = 0; q < W; ++q) z[q] = lin_act(z[q], p.act);
+  }
+  if (p.residual) {
+    float r[W];
+    lin_load<OT, W>((const OT *)p.residual + m * p.sr + n, left, r);
+#pragma unroll
+    for (int q = 0; q < W; ++q) z[q] += r[q];
+  }
+  lin_store<OT, W>((OT *)p.C + m * p.sc + n, left, z);
+}
+
+// ------------------------------------------------------------------ tiles
+// A workgroup of WM x WN wavefronts takes BM x BN of C in steps of 128 bytes of k (64 in the transposed storage).  Both
+// operands go from HBM straight into LDS, 16 bytes a lane (a buffer load past the matrix's end leaves zeros), a step
+// ahead of the products.  In LDS:
+//   along k       [row][128 bytes]: the 16-byte pieces of a row change places by its number, so that the reads of 8
+//                 rows' equal pieces meet in no bank
+//   along m, n    [k][2 R bytes]: pieces change places in pairs by k; a transposing read gives a lane its column's
+//                 4 values of k
+// B is the first operand of the matrix instructions, so a lane holds consecutive n of a row of C.  B's rows along k are
+// dealt to the instructions such that the NT results a lane has of a row are 4 NT consecutive n.
+template <bool ALONG, int R, int NW, int SPREAD>   // R rows (or columns); the share of one of NW wavefronts
+struct LinTile {
+  static constexpr int bytes = R * 128, loads = bytes / 1024 / NW;
+  static constexpr int line = ALONG ? 128 : 2 * R, pieces = line / 16, rows = 64 / pieces;   // rows: of one load
+  __device__ __forceinline__ static int piece(int row, int c) {   // which piece of the row lies at place c, and back
+    if constexpr (ALONG) return c ^ (((row / SPREAD) & 1) * 4 | (row & 3));
+    else return c ^ ((2 * ((row + 4 * (row >> 3)) & 7)) & (pieces - 1));
+  }
+  uint32_t off[loads];
+  int wave, lane;
+  __device__ __forceinline__ void init(int64_t stride) {
+    wave = threadIdx.x / 64;
+    lane = threadIdx.x % 64;
+#pragma unroll
+    for (int i = 0; i < loads; ++i) {
+      const int row = (i * NW + wave) * rows + lane / pieces;
+      off[i] = (uint32_t)(row * stride) + piece(row, lane % pieces) * 16;
+    }
+  }
+  // base: the tile's first byte of this step; left: bytes from there to the matrix's end; k: bytes of k from there
+  __device__ __forceinline__ void load(char *__restrict lds, const char *base, int64_t left, int64_t k) const {
+    const __amdgpu_buffer_rsrc_t r =
+        __builtin_amdgcn_make_buffer_rsrc((void *)base, (short)0, (int)(left < 0x7fffffff ? left : 0x7fffffff), kBufferFlags);
+    const bool cut = ALONG && k < 128;   // the last step: pieces past the rows' end are left out
+#pragma unroll
+    for (int i = 0; i < loads; ++i) {
+      uint32_t o = off[i];
+      if (cut && piece((i * NW + wave) * rows + lane / pieces, lane % pieces) * 16 >= k) o = 0x80000000u;
+      __builtin_amdgcn_raw_ptr_buffer_load_lds(r, (LdsPtr)(lds + (i * NW + wave) * 1024), 16, o, 0, 0, 0);
+    }
+  }
+  // the operand of 16 rows (along k: `row` is the lane's own; else the first of the lane's group), step kk of the tile
+  template <typename T>
+  __device__ __forceinline__ static typename Mma<T>::Frag get(const char *__restrict lds, int row, int kk) {
+    const int lane = threadIdx.x % 64, g = lane / 16;
+    if constexpr (ALONG && Mma<T>::bytes == 32) {
+      const int at = row * 128 + piece(row, 2 * g) * 16;
+      const li4 lo = *(const li4 *)(lds + at), hi = *(const li4 *)(lds + (at ^ 16));
+      return __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
+    } else if constexpr (ALONG) {
+      return *(const li4 *)(lds + row * 128 + piece(row, 4 * kk + g) * 16);
+    } else {
+      const int k = 32 * kk + 8 * g + (lane % 16) / 4, col = 2 * row + 8 * (lane % 4);   // bytes
+      const char *lo = lds + k * line + piece(k, col / 16) * 16 + col % 16;
+      const char *hi = lds + (k + 4) * line + piece(k + 4, col / 16) * 16 + col % 16;
+      const ls4 a = __builtin_amdgcn_ds_read_tr16_b64_v4i16((LdsTr)lo), b = __builtin_amdgcn_ds_read_tr16_b64_v4i16((LdsTr)hi);
+      return __builtin_bit_cast(li4, __builtin_shufflevector(a, b, 0, 1, 2, 3, 4, 5, 6, 7));
+    }
+  }
+};
+
+template <typename T, typename OT, bool AL, bool BL, int BM, int BN, int WM, int WN>
+__global__ void __launch_bounds__(64 * WM * WN) __attribute__((amdgpu_waves_per_eu(2, 2))) k_linear_tile(const GemmParams p) {
+  constexpr int NW = WM * WN, MT = BM / WM / 16, NT = BN / WN / 16, E = sizeof(T);
+  constexpr int KE = AL || BL ? 128 / E : 64, STEPS = 128 / (4 * Mma<T>::bytes);
+  typedef LinTile<AL, BM, NW, 4> TA;
+  typedef LinTile<BL, BN, NW, 4 * NT> TB;
+  __shared__ __attribute__((aligned(1024))) char As0[TA::bytes], Bs0[TB::bytes], As1[TA::bytes], Bs1[TB::bytes];
+  // Tiles in the order that the 8 dies take workgroups: each die its own run of them, 8 rows of tiles by columns.
+  const int64_t tm = (p.M + BM - 1) / BM, tn = (p.N + BN - 1) / BN, tiles = tm * tn;
+  const int64_t all = tiles * p.splits, q8 = all / 8, r8 = all % 8, die = blockIdx.x % 8;
+  const int64_t id = die * q8 + (die < r8 ? die : r8) + blockIdx.x / 8, split = id / tiles, t = id % tiles;
+  const int64_t band = t / (8 * tn), in_band = t % (8 * tn), high = tm - band * 8 < 8 ? tm - band * 8 : 8;
+  const int64_t m0 = (band * 8 + in_band % high) * BM, n0 = in_band / high * BN;
+  const int64_t ks = (p.K + KE - 1) / KE, s0 = ks * split / p.splits, s1 = ks * (split + 1) / p.splits;
+
+  const int64_t sa = p.sa * E, sb = p.sb * E;
+  const char *a = (const char *)p.A + (AL ? m0 * sa + s0 * KE * E : m0 * E + s0 * KE * sa);
+  const char *b = (const char *)p.B + (BL ? n0 * sb + s0 * KE * E : n0 * E + s0 * KE * sb);
+  const char *const a1 = (const char *)p.A + (AL ? (p.M - 1) * sa + p.K * E + 15 : (p.K - 1) * sa + p.M * E + 15);
+  const char *const b1 = (const char *)p.B + (BL ? (p.N - 1) * sb + p.K * E + 15 : (p.K - 1) * sb + p.N * E + 15);
+  int64_t left = (p.K - s0 * KE) * E;
+  TA ta;
+  TB tb;
+  ta.init(sa);
+  tb.init(sb);
+  auto load = [&](char *__restrict as, char *__restrict bs) {   // one step on
+    ta.load(as, a, (a1 - a) & ~15ll, left);
+    tb.load(bs, b, (b1 - b) & ~15ll, left);
+    a += AL ? KE * E : KE * sa;
+    b += BL ? KE * E : KE * sb;
+    left -= KE * E;
+  };
+  const int lane = threadIdx.x % 64, wave = threadIdx.x / 64, wm = wave / WN * (BM / WM), wn = wave % WN * (BN / WN);
+  const int ra = wm + (AL ? lane % 16 : 0);
+  const int rb = wn + (BL ? 4 * NT * ((lane % 16) / 4) + lane % 4 : 0);
+  lf4 acc[MT][NT] = {};
+  auto multiply = [&](const char *__restrict as, const char *__restrict bs) {
+#pragma unroll
+    for (int kk = 0; kk < STEPS; ++kk) {
+      typename Mma<T>::Frag fa[MT], fb[NT];
+#pragma unroll
+      for (int j = 0; j < NT; ++j) fb[j] = TB::template get<T>(bs, rb + (BL ? 4 : 16) * j, kk);
+#pragma unroll
+      for (int i = 0; i < MT; ++i) fa[i] = TA::template get<T>(as, ra + 16 * i, kk);
+#pragma unroll
+      for (int i = 0; i < MT; ++i)
+#pragma unroll
+        for (int j = 0; j < NT; ++j) acc[i][j] = Mma<T>::mul(fb[j], fa[i], acc[i][j]);
+    }
+  };
+  auto arrived = [&] {
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+    lds_barrier();
+  };
+  load(As0, Bs0);
+  arrived();
+  for (int64_t s = s0; s < s1; s += 2) {
+    if (s + 1 < s1) load(As1, Bs1);
+    multiply(As0, Bs0);
+    arrived();
+    if (s + 1 >= s1) break;
+    if (s + 2 < s1) load(As0, Bs0);
+    multiply(As1, Bs1);
+    arrived();
+  }
+#pragma unroll
+  for (int i = 0; i < MT; ++i) {
+    const int64_t m = m0 + wm + 16 * i + lane % 16;
+    if (m >= p.M) continue;
+    if (p.splits > 1) {
+#pragma unroll
+      for (int j = 0; j < NT; ++j) {
+        const int64_t n = n0 + wn + (BL ? 4 * NT * (lane / 16) + 4 * j : 16 * j + 4 * (lane / 16));
+        const float v[4] = {acc[i][j][0], acc[i][j][1], acc[i][j][2], acc[i][j][3]};
+        if (n < p.N) lin_store<float, 4>(p.partial + (split * p.M + m) * p.N + n, p.N - n, v);
       }
+    } else if constexpr (BL) {
+#pragma unroll
+      for (int j = 0; j < NT; j += 2) {
+        const int64_t n = n0 + wn + 4 * NT * (lane / 16) + 4 * j;
+        float v[8];
+#pragma unroll
+        for (int q = 0; q < 8; ++q) v[q] = acc[i][j + q / 4][q % 4];
+        if (n < p.N) lin_epilogue<OT, 8>(p, m, n, v);
+      }
+    } else {
+#pragma unroll
+      for (int j = 0; j < NT; ++j) {
+        const int64_t n = n0 + wn + 16 * j + 4 * (lane / 16);
+        float v[4] = {acc[i][j][0], acc[i][j][1], acc[i][j][2], acc[i][j][3]};
+        if (n < p.N) lin_epilogue<OT, 4>(p, m, n, v);
+      }
+    }
+  }
+}
+
+// The splits' sums in order, and the epilogue: 8 consecutive n a thread.
+template <typename OT>
+__global__ void __launch_bounds__(256) k_linear_join(const GemmParams p) {
+  const int64_t per = (p.N + 7) / 8, id = (int64_t)blockIdx.x * 256 + threadIdx.x, m = id / per, n = id % per * 8;
+  if (m >= p.M) return;
+  float z[8] = {};
+  for (int s = 0; s < p.splits; ++s) {
+    float v[8];
+    lin_load<float, 8>(p.partial + (s * p.M + m) * p.N + n, p.N - n, v);
+#pragma unroll
+    for (int q = 0; q < 8; ++q) z[q] += v[q];
+  }
+  lin_epilogue<OT, 8>(p, m, n, z);
+}
+
+// ------------------------------------------------------------------ few rows
+// Up to 16 MT rows: the weights are read once, straight into the matrix instructions' operands, 16 NT of their rows a
+// workgroup, whose 8 wavefronts share k and join their sums in LDS in order.  Rows may begin anywhere.
+template <typename T, int F>
+__device__ __forceinline__ void lin_row(const T *row, int64_t k, int64_t K, int (&f)[F]) {   // 4 F bytes from k on
+  constexpr int n = 4 * F / sizeof(T);
+  if (k + n <= K) {
+    __builtin_memcpy(f, row + k, 4 * F);
+  } else {
+    T e[n];
+#pragma unroll
+    for (int i = 0; i < n; ++i) e[i] = k + i < K ? row[k + i] : T{};
+    __builtin_memcpy(f, e, 4 * F);
+  }
+}
+template <typename T, typename OT, int MT, int NT>
+__global__ void __launch_bounds__(512) k_linear_rows(const GemmParams p) {
+  constexpr int F = Mma<T>::bytes / 4, KE = 4 * Mma<T>::bytes / sizeof(T), U = MT * NT >= 8 ? 2 : 4;
+  __shared__ __attribute__((aligned(16))) float red[8][MT * 16][NT * 16 + 4];
+  const int lane = threadIdx.x % 64, wave = threadIdx.x / 64, g = lane / 16;
+  const int64_t nb = (p.N + 16 * NT - 1) / (16 * NT), n0 = blockIdx.x % nb * (16 * NT), split = blockIdx.x / nb;
+  const int64_t ks = (p.K + KE - 1) / KE, parts = 8 * p.splits, part = split * 8 + wave;
+  const int64_t s0 = ks * part / parts, s1 = ks * (part + 1) / parts;
+  const T *w[NT], *x[MT];
+#pragma unroll
+  for (int j = 0; j < NT; ++j) {   // rows past the end repeat the last one, and are not written
+    const int64_t n = n0 + 16 * j + lane % 16;
+    w[j] = (const T *)p.B + (n < p.N ? n : p.N - 1) * p.sb;
+  }
+#pragma unroll
+  for (int i = 0; i < MT; ++i) {
+    const int64_t m = 16 * i + lane % 16;
+    x[i] = (const T *)p.A + (m < p.M ? m : p.M - 1) * p.sa;
+  }
+  lf4 acc[MT][NT] = {};
+  const int64_t at = g * (KE / 4);
+  auto steps = [&](int64_t s, auto count) {
+    constexpr int C = decltype(count)::value;
+    int fw[C][NT][F], fx[C][MT][F];
+#pragma unroll
+    for (int u = 0; u < C; ++u) {
+#pragma unroll
+      for (int j = 0; j < NT; ++j) lin_row<T, F>(w[j], (s + u) * KE + at, p.K, fw[u][j]);
+#pragma unroll
+      for (int i = 0; i < MT; ++i) lin_row<T, F>(x[i], (s + u) * KE + at, p.K, fx[u][i]);
+    }
+#pragma unroll
+    for (int u = 0; u < C; ++u)
+#pragma unroll
+      for (int i = 0; i < MT; ++i)
+#pragma unroll
+        for (int j = 0; j < NT; ++j)
+          acc[i][j] = Mma<T>::mul(__builtin_bit_cast(typename Mma<T>::Frag, fw[u][j]), __builtin_bit_cast(typename Mma<T>::Frag, fx[u][i]),
+                                  acc[i][j]);
+  };
+  int64_t s = s0;
+  for (; s + U <= s1; s += U) steps(s, std::integral_constant<int, U>{});
+  for (; s < s1; ++s) steps(s, std::integral_constant<int, 1>{});
+#pragma unroll
+  for (int i = 0; i < MT; ++i)
+#pragma unroll
+    for (int j = 0; j < NT; ++j) *(lf4 *)&red[wave][16 * i + lane % 16][16 * j + 4 * g] = acc[i][j];
+  __syncthreads();
+  for (int e = threadIdx.x; e < MT * 16 * NT * 2; e += 512) {
+    const int mi = e / (NT * 2), c = e % (NT * 2) * 8;
+    const int64_t m = mi, n = n0 + c;
+    if (m >= p.M || n >= p.N) continue;
+    float z[8] = {};
+#pragma unroll
+    for (int v = 0; v < 8; ++v)
+#pragma unroll
+      for (int q = 0; q < 8; ++q) z[q] += red[v][mi][c + q];
+    if (p.splits > 1) lin_store<float, 8>(p.partial + (split * p.M + m) * p.N + n, p.N - n, z);
+    else lin_epilogue<OT, 8>(p, m, n, z);
+  }
+}
+
+// ------------------------------------------------------------------ packed copies
+// Rows of `cols` elements from anywhere to rows of whole 16 bytes, zeros past their end.
+template <typename T>
+__global__ void __launch_bounds__(256) k_linear_pack(const LinearPack p) {
+  constexpr int n = 16 / sizeof(T);
+  const int64_t per = p.to_stride / n, id = (int64_t)blockIdx.x * 256 + threadIdx.x, row = id / per, c = id % per * n;
+  if (row >= p.rows) return;
+  int f[4];
+  lin_row<T, 4>((const T *)p.from + row * p.stride, c, p.cols, f);
+  __builtin_memcpy(__builtin_assume_aligned((T *)p.to + row * p.to_stride + c, 16), f, 16);
 }
 
 // ------------------------------------------------------------------ dz and dbias
-// dz = dy act'(z), 64 columns by a range of rows per workgroup, and that range's column sums of dz.
+// dz = dy act'(z), 64 columns by a range of rows per workgroup, and that range's column sums of dz.  Rows of dz are
+// whole 16 bytes, zeros past column N.
 template <typename T>
 __global__ void __launch_bounds__(256) k_linear_dz(const LinearDzParams p) {
-  __shared__ float part[4][64];
-  const int col = threadIdx.x % 64, sub = threadIdx.x / 64;
-  const int64_t n = (int64_t)blockIdx.x * 64 + col, per = (p.M + gridDim.y - 1) / gridDim.y, m0 = blockIdx.y * per;
-  const int64_t m1 = m0 + per < p.M ? m0 + per : p.M;
-  float s = 0;
-  if (n < p.N)
-    for (int64_t m = m0 + sub; m < m1; m += 4) {
-      float d = Conv<T>::load((const T *)p.dy + m * p.sdy + n);
+  __shared__ float part[32][65];
+  const int col = threadIdx.x % 8 * 8, sub = threadIdx.x / 8;
+  const int64_t nb = (p.sdz + 63) / 64, n = blockIdx.x % nb * 64 + col, slot = blockIdx.x / nb;
+  const int64_t m0 = p.M * slot / p.slots, m1 = p.M * (slot + 1) / p.slots;
+  float s[8] = {};
+  if (n < p.sdz)
+    for (int64_t m = m0 + sub; m < m1; m += 32) {
+      float d[8], z[8];
+      lin_load<T, 8>((const T *)p.dy + m * p.sdy + n, p.N - n, d);
       if (p.act) {
-        d *= lin_slope(Conv<T>::load((const T *)p.pre + m * p.N + n), p.act);
-        Conv<T>::store((T *)p.dz + m * p.N + n, d);
+        lin_load<T, 8>((const T *)p.pre + m * p.N + n, p.N - n, z);
+#pragma unroll
+        for (int q = 0; q < 8; ++q) d[q] *= lin_slope(z[q], p.act);
       }
-      s += d;
+      if (p.dz) lin_store<T, 8>((T *)p.dz + m * p.sdz + n, 8, d);
+#pragma unroll
+      for (int q = 0; q < 8; ++q) s[q] += d[q];
     }
-  part[sub][col] = s;
+  if (!p.partial) return;
+#pragma unroll
+  for (int q = 0; q < 8; ++q) part[sub][col + q] = s[q];
   __syncthreads();
-  if (p.partial && sub == 0 && n < p.N)
-    p.partial[blockIdx.y * p.N + n] = (part[0][col] + part[1][col]) + (part[2][col] + part[3][col]);
+  if (threadIdx.x >= 64) return;
+  const int64_t c = blockIdx.x % nb * 64 + threadIdx.x;
+  float t = 0;
+#pragma unroll
+  for (int k = 0; k < 32; ++k) t += part[k][threadIdx.x];
+  if (c < p.N) p.partial[slot * p.N + c] = t;
 }
 template <typename T>
 __global__ void __launch_bounds__(256) k_linear_dbias(const LinearDzParams p) {
@@ -129,18 +421,99 @@ __global__ void __launch_bounds__(256) k_linear_dbias(const LinearDzParams p) {
   if (n < p.N) Conv<T>::store((T *)p.dbias + n, (float)ordered_sum<8, float, double>(p.partial + n, p.N, p.slots));
 }
 
+// ------------------------------------------------------------------ plan and launch
+static bool loadable(const void *data, int64_t stride, int64_t row, int e) {   // 16 bytes a lane, 32-bit offsets
+  return (uintptr_t)data % 16 == 0 && stride * e % 16 == 0 && row * e % 16 == 0 && stride >= 0 && stride * e < (1 << 22);
+}
+LinearPlan linear_plan(const GemmParams &p) {
+  LinearPlan l{};
+  const int e = p.fp8 ? 1 : 2;
+  const int64_t unit = 16 / e;
+  auto up = [&](int64_t n) { return (n + unit - 1) / unit * unit; };
+  if (p.a_along && p.b_along && p.M <= 64) {
+    l.rows = 1;
+    l.MT = p.M <= 16 ? 1 : p.M <= 32 ? 2 : 4;
+    l.NT = p.N >= 16 * 4 * 512 && l.MT < 4 ? 4 : p.N >= 16 * 2 * 256 ? 2 : 1;
+    const int64_t nb = (p.N + 16 * l.NT - 1) / (16 * l.NT), steps = p.K * e / 64;
+    l.splits = 1;   // more where few workgroups would each walk a long k: 16 steps a wavefront at least
+    while (nb * l.splits < 128 && steps / (8 * l.splits * 2) >= 16) l.splits *= 2;
+  } else {
+    if (!loadable(p.A, p.sa, p.a_along && !p.a_padded ? p.K : unit, e)) l.pack_a = p.a_along ? p.M * up(p.K) * e : p.K * up(p.M) * e;
+    if (!loadable(p.B, p.sb, p.b_along ? p.K : unit, e)) l.pack_b = p.b_along ? p.N * up(p.K) * e : p.K * up(p.N) * e;
+    const int64_t big = ((p.M + 255) / 256) * ((p.N + 255) / 256);
+    l.tile = big >= 192 ? 256 : 128;
+    const int64_t tiles = l.tile == 256 ? big : ((p.M + 127) / 128) * ((p.N + 127) / 128), steps = (p.K * e + 127) / 128;
+    l.splits = 1;   // two workgroups a compute unit, 4 steps each at least
+    while (l.tile == 128 && tiles * l.splits * 2 <= 512 && steps / (l.splits * 2) >= 4 && l.splits < 16) l.splits *= 2;
+  }
+  l.pack_a = (l.pack_a + 255) / 256 * 256;
+  l.pack_b = (l.pack_b + 255) / 256 * 256;
+  if (l.splits > 1) l.partial = (l.splits * p.M * p.N * 4 + 255) / 256 * 256;
+  return l;
+}
+
+static void pack(const void *from, int64_t stride, void *to, int64_t rows, int64_t cols, int64_t to_stride, int fp8, hipStream_t s) {
+  const LinearPack k{from, to, rows, cols, stride, to_stride};
+  const int64_t items = rows * to_stride * (fp8 ? 1 : 2) / 16;
+  const dim3 grid((unsigned)((items + 255) / 256));
+  if (fp8) hipLaunchKernelGGL((k_linear_pack<fp8_t>), grid, dim3(256), 0, s, k);
+  else hipLaunchKernelGGL((k_linear_pack<bf16_t>), grid, dim3(256), 0, s, k);
+}
+template <typename T, typename OT, bool AL, bool BL>
+static void tile_v(const GemmParams &p, const LinearPlan &l, hipStream_t s) {
+  const int64_t t = l.tile, tiles = ((p.M + t - 1) / t) * ((p.N + t - 1) / t) * l.splits;
+  if (l.tile == 256) hipLaunchKernelGGL((k_linear_tile<T, OT, AL, BL, 256, 256, 2, 4>), dim3((unsigned)tiles), dim3(512), 0, s, p);
+  else hipLaunchKernelGGL((k_linear_tile<T, OT, AL, BL, 128, 128, 2, 2>), dim3((unsigned)tiles), dim3(256), 0, s, p);
+}
+template <typename T, typename OT, int MT>
+static void rows_v(const GemmParams &p, const LinearPlan &l, hipStream_t s) {
+  const dim3 grid((unsigned)((p.N + 16 * l.NT - 1) / (16 * l.NT) * l.splits));
+  if constexpr (MT < 4)
+    if (l.NT == 4) {
+      hipLaunchKernelGGL((k_linear_rows<T, OT, MT, 4>), grid, dim3(512), 0, s, p);
+      return;
+    }
+  if (l.NT == 2) hipLaunchKernelGGL((k_linear_rows<T, OT, MT, 2>), grid, dim3(512), 0, s, p);
+  else hipLaunchKernelGGL((k_linear_rows<T, OT, MT, 1>), grid, dim3(512), 0, s, p);
+}
 template <typename T, typename OT>
-static hipError_t gemm_t(const GemmParams &p, hipStream_t s) {
-  hipLaunchKernelGGL((k_linear_any<T, OT>), dim3((unsigned)(((p.N + 63) / 64) * ((p.M + 63) / 64))), dim3(256), 0, s, p);
+static hipError_t gemm_t(GemmParams p, void *workspace, hipStream_t s) {
+  const LinearPlan l = linear_plan(p);
+  char *ws = (char *)workspace;
+  p.splits = l.splits;
+  p.partial = (float *)(ws + l.pack_a + l.pack_b);
+  if (l.rows) {
+    if (l.MT == 1) rows_v<T, OT, 1>(p, l, s);
+    else if (l.MT == 2) rows_v<T, OT, 2>(p, l, s);
+    else rows_v<T, OT, 4>(p, l, s);
+  } else {
+    constexpr int64_t unit = 16 / sizeof(T);
+    auto packed = [&](const void *&data, int64_t &stride, char *to, int64_t rows, int64_t cols) {
+      const int64_t wide = (cols + unit - 1) / unit * unit;
+      pack(data, stride, to, rows, cols, wide, p.fp8, s);
+      data = to;
+      stride = wide;
+    };
+    if (l.pack_a) packed(p.A, p.sa, ws, p.a_along ? p.M : p.K, p.a_along ? p.K : p.M);
+    if (l.pack_b) packed(p.B, p.sb, ws + l.pack_a, p.b_along ? p.N : p.K, p.b_along ? p.K : p.N);
+    if constexpr (sizeof(T) == 1) {
+      tile_v<T, OT, true, true>(p, l, s);
+    } else {
+      if (p.a_along && p.b_along) tile_v<T, OT, true, true>(p, l, s);
+      else if (p.a_along) tile_v<T, OT, true, false>(p, l, s);
+      else tile_v<T, OT, false, false>(p, l, s);
+    }
+  }
+  if (l.splits > 1) hipLaunchKernelGGL((k_linear_join<OT>), dim3((unsigned)((p.M * ((p.N + 7) / 8) + 255) / 256)), dim3(256), 0, s, p);
   return hipGetLastError();
 }
-hipError_t launch_gemm(const GemmParams &p, int dtype, hipStream_t s) {
-  if (p.fp8) return dtype == 1 ? gemm_t<fp8_t, bf16_t>(p, s) : gemm_t<fp8_t, f16_t>(p, s);
-  return dtype == 1 ? gemm_t<bf16_t, bf16_t>(p, s) : gemm_t<f16_t, f16_t>(p, s);
+hipError_t launch_gemm(const GemmParams &p, int dtype, void *workspace, hipStream_t s) {
+  if (p.fp8) return dtype == 1 ? gemm_t<fp8_t, bf16_t>(p, workspace, s) : gemm_t<fp8_t, f16_t>(p, workspace, s);
+  return dtype == 1 ? gemm_t<bf16_t, bf16_t>(p, workspace, s) : gemm_t<f16_t, f16_t>(p, workspace, s);
 }
 template <typename T>
 static hipError_t dz_t(const LinearDzParams &p, hipStream_t s) {
-  hipLaunchKernelGGL((k_linear_dz<T>), dim3((unsigned)((p.N + 63) / 64), (unsigned)p.slots), dim3(256), 0, s, p);
+  hipLaunchKernelGGL((k_linear_dz<T>), dim3((unsigned)((p.sdz + 63) / 64 * p.slots)), dim3(256), 0, s, p);
   if (p.dbias) hipLaunchKernelGGL((k_linear_dbias<T>), dim3((unsigned)((p.N + 255) / 256)), dim3(256), 0, s, p);
   return hipGetLastError();
 }
