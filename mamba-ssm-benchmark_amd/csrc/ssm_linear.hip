@@ -138,28 +138,26 @@ struct LinTile {
     if constexpr (ALONG) return c ^ (((row / SPREAD) & 1) * 4 | (row & 3));
     else return c ^ ((2 * ((row + 4 * (row >> 3)) & 7)) & (pieces - 1));
   }
-  uint32_t off[loads];
-  int wave, lane;
+  static_assert(ALONG ? NW * rows % (2 * SPREAD) == 0 : NW * rows % 16 == 0, "all of a lane's loads have the same piece");
+  uint32_t off, step, at;   // bytes of the lane's first load, from one load to the next, of the piece within its row
+  int wave;
   __device__ __forceinline__ void init(int64_t stride) {
-    wave = threadIdx.x / 64;
-    lane = threadIdx.x % 64;
-#pragma unroll
-    for (int i = 0; i < loads; ++i) {
-      const int row = (i * NW + wave) * rows + lane / pieces;
-      off[i] = (uint32_t)(row * stride) + piece(row, lane % pieces) * 16;
-    }
+    const int lane = threadIdx.x % 64;
+    wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64);
+    const int row = wave * rows + lane / pieces;
+    at = piece(row, lane % pieces) * 16;
+    off = (uint32_t)(row * stride) + at;
+    step = (uint32_t)(NW * rows * stride);
   }
-  // base: the tile's first byte of this step; left: bytes from there to the matrix's end; k: bytes of k from there
+  // base: the tile's first byte of this step; left: bytes from there to the matrix's end; k: bytes of k from there, past
+  // which pieces are left out (in the transposed storage the matrix's end does that)
   __device__ __forceinline__ void load(char *__restrict lds, const char *base, int64_t left, int64_t k) const {
     const __amdgpu_buffer_rsrc_t r =
-        __builtin_amdgcn_make_buffer_rsrc((void *)base, (short)0, (int)(left < 0x7fffffff ? left : 0x7fffffff), kBufferFlags);
-    const bool cut = ALONG && k < 128;   // the last step: pieces past the rows' end are left out
+        __builtin_amdgcn_make_buffer_rsrc((void *)base, (short)0, (int)(left < 0 ? 0 : left < 0x7fffffff ? left : 0x7fffffff), kBufferFlags);
+    const uint32_t o = ALONG && at >= k ? 0x80000000u : off;
 #pragma unroll
-    for (int i = 0; i < loads; ++i) {
-      uint32_t o = off[i];
-      if (cut && piece((i * NW + wave) * rows + lane / pieces, lane % pieces) * 16 >= k) o = 0x80000000u;
-      __builtin_amdgcn_raw_ptr_buffer_load_lds(r, (LdsPtr)(lds + (i * NW + wave) * 1024), 16, o, 0, 0, 0);
-    }
+    for (int i = 0; i < loads; ++i)
+      __builtin_amdgcn_raw_ptr_buffer_load_lds(r, (LdsPtr)(lds + (i * NW + wave) * 1024), 16, o + i * step, 0, 0, 0);
   }
   // the operand of 16 rows (along k: `row` is the lane's own; else the first of the lane's group), step kk of the tile
   template <typename T>
@@ -189,12 +187,16 @@ __global__ void __launch_bounds__(64 * WM * WN) __attribute__((amdgpu_waves_per_
   typedef LinTile<BL, BN, NW, 4 * NT> TB;
   __shared__ __attribute__((aligned(1024))) char As0[TA::bytes], Bs0[TB::bytes], As1[TA::bytes], Bs1[TB::bytes];
   // Tiles in the order that the 8 dies take workgroups: each die its own run of them, 8 rows of tiles by columns.
-  const int64_t tm = (p.M + BM - 1) / BM, tn = (p.N + BN - 1) / BN, tiles = tm * tn;
-  const int64_t all = tiles * p.splits, q8 = all / 8, r8 = all % 8, die = blockIdx.x % 8;
-  const int64_t id = die * q8 + (die < r8 ? die : r8) + blockIdx.x / 8, split = id / tiles, t = id % tiles;
-  const int64_t band = t / (8 * tn), in_band = t % (8 * tn), high = tm - band * 8 < 8 ? tm - band * 8 : 8;
-  const int64_t m0 = (band * 8 + in_band % high) * BM, n0 = in_band / high * BN;
-  const int64_t ks = (p.K + KE - 1) / KE, s0 = ks * split / p.splits, s1 = ks * (split + 1) / p.splits;
+  const uint32_t tm = (uint32_t)((p.M + BM - 1) / BM), tn = (uint32_t)((p.N + BN - 1) / BN), tiles = tm * tn;
+  const uint32_t all = tiles * p.splits, q8 = all / 8, r8 = all % 8, die = blockIdx.x % 8;
+  const uint32_t id = die * q8 + (die < r8 ? die : r8) + blockIdx.x / 8, t = id % tiles;
+  const uint32_t band = t / (8 * tn), in_band = t % (8 * tn), high = tm - band * 8 < 8 ? tm - band * 8 : 8;
+  // quotients are formed in vector registers: back to scalar ones, as the loads' descriptors need
+  const int64_t split = __builtin_amdgcn_readfirstlane(id / tiles);
+  const int64_t m0 = (int64_t)__builtin_amdgcn_readfirstlane(band * 8 + in_band % high) * BM;
+  const int64_t n0 = (int64_t)__builtin_amdgcn_readfirstlane(in_band / high) * BN;
+  const int ks = (int)((p.K + KE - 1) / KE), s0 = __builtin_amdgcn_readfirstlane(ks * (int)split / p.splits);
+  const int s1 = __builtin_amdgcn_readfirstlane(ks * ((int)split + 1) / p.splits);
 
   const int64_t sa = p.sa * E, sb = p.sb * E;
   const char *a = (const char *)p.A + (AL ? m0 * sa + s0 * KE * E : m0 * E + s0 * KE * sa);
@@ -212,8 +214,9 @@ __global__ void __launch_bounds__(64 * WM * WN) __attribute__((amdgpu_waves_per_
     a += AL ? KE * E : KE * sa;
     b += BL ? KE * E : KE * sb;
     left -= KE * E;
+    __builtin_amdgcn_sched_barrier(0);   // the loads are under way before the products
   };
-  const int lane = threadIdx.x % 64, wave = threadIdx.x / 64, wm = wave / WN * (BM / WM), wn = wave % WN * (BN / WN);
+  const int lane = threadIdx.x % 64, wave = ta.wave, wm = wave / WN * (BM / WM), wn = wave % WN * (BN / WN);
   const int ra = wm + (AL ? lane % 16 : 0);
   const int rb = wn + (BL ? 4 * NT * ((lane % 16) / 4) + lane % 4 : 0);
   lf4 acc[MT][NT] = {};
@@ -230,6 +233,14 @@ __global__ void __launch_bounds__(64 * WM * WN) __attribute__((amdgpu_waves_per_
 #pragma unroll
         for (int j = 0; j < NT; ++j) acc[i][j] = Mma<T>::mul(fb[j], fa[i], acc[i][j]);
     }
+    // the operands of two rows of products ahead of them, then two reads a row
+    constexpr int each = Mma<T>::bytes == 32 || !AL ? 2 : 1;
+    __builtin_amdgcn_sched_group_barrier(0x100, (NT + 2) * each, 0);
+#pragma unroll
+    for (int i = 0; i < MT * STEPS; ++i) {
+      __builtin_amdgcn_sched_group_barrier(0x008, NT, 0);
+      __builtin_amdgcn_sched_group_barrier(0x100, 2 * each, 0);
+    }
   };
   auto arrived = [&] {
     asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
@@ -237,15 +248,16 @@ __global__ void __launch_bounds__(64 * WM * WN) __attribute__((amdgpu_waves_per_
   };
   load(As0, Bs0);
   arrived();
-  for (int64_t s = s0; s < s1; s += 2) {
-    if (s + 1 < s1) load(As1, Bs1);
+  int s = s0;
+  for (; s + 1 < s1; s += 2) {
+    load(As1, Bs1);
     multiply(As0, Bs0);
     arrived();
-    if (s + 1 >= s1) break;
-    if (s + 2 < s1) load(As0, Bs0);
+    load(As0, Bs0);   // past the last step: beyond the split's end, and not used
     multiply(As1, Bs1);
     arrived();
   }
+  if (s < s1) multiply(As0, Bs0);
 #pragma unroll
   for (int i = 0; i < MT; ++i) {
     const int64_t m = m0 + wm + 16 * i + lane % 16;
