@@ -64,11 +64,13 @@ __device__ __forceinline__ float lin_slope(float z, int act) {
 }
 
 // ------------------------------------------------------------------ epilogue
-// W consecutive n of row m (those past N are not there); rows may begin anywhere.
-template <typename OT, int W>
+// W consecutive n of row m (those past N are not there, unless WHOLE); rows may begin anywhere.
+template <typename OT> struct LinOut { typedef OT E; };
+template <> struct LinOut<bf16_t> { typedef __bf16 E; };   // converted by the hardware, to nearest even
+template <typename OT, int W, bool WHOLE = false>
 __device__ __forceinline__ void lin_load(const OT *src, int64_t left, float (&v)[W]) {
   OT e[W];
-  if (left >= W) {
+  if (WHOLE || left >= W) {
     __builtin_memcpy(e, src, sizeof(e));
   } else {
 #pragma unroll
@@ -77,47 +79,50 @@ __device__ __forceinline__ void lin_load(const OT *src, int64_t left, float (&v)
 #pragma unroll
   for (int q = 0; q < W; ++q) v[q] = Conv<OT>::load(&e[q]);
 }
-template <typename OT, int W>
+template <typename OT, int W, bool WHOLE = false>
 __device__ __forceinline__ void lin_store(OT *dst, int64_t left, const float (&v)[W]) {
-  OT e[W];
-#pragma unroll
-  for (int q = 0; q < W; ++q) Conv<OT>::store(&e[q], v[q]);
-  if (left >= W) {
-    __builtin_memcpy(dst, e, sizeof(e));
+  typedef float F __attribute__((ext_vector_type(W)));
+  typedef typename LinOut<OT>::E O __attribute__((ext_vector_type(W)));
+  const O o = __builtin_convertvector(__builtin_bit_cast(F, v), O);
+  if (WHOLE || left >= W) {
+    __builtin_memcpy(dst, &o, W * sizeof(OT));
   } else {
 #pragma unroll
     for (int q = 0; q < W; ++q)
-      if (q < left) dst[q] = e[q];
+      if (q < left) __builtin_memcpy(dst + q, (const OT *)&o + q, sizeof(OT));
   }
 }
-template <typename OT, int W>
+template <typename OT, int W, bool WHOLE>
 __device__ __forceinline__ void lin_epilogue(const GemmParams &p, int64_t m, int64_t n, float (&z)[W]) {
   const int64_t left = p.N - n;
   if (p.xs) {
     float ws[W];
-    lin_load<float, W>(p.ws + n, left, ws);
+    lin_load<float, W, WHOLE>(p.ws + n, left, ws);
     const float xs = p.xs[m];
 #pragma unroll
     for (int q = 0; q < W; ++q) z[q] *= xs * ws[q];
   }
   if (p.bias) {
     float b[W];
-    lin_load<OT, W>((const OT *)p.bias + n, left, b);
+    lin_load<OT, W, WHOLE>((const OT *)p.bias + n, left, b);
 #pragma unroll
     for (int q = 0; q < W; ++q) z[q] += b[q];
   }
-  if (p.act) {
-    if (p.pre) lin_store<OT, W>((OT *)p.pre + m * p.spre + n, left, z);
+  if (p.pre) lin_store<OT, W, WHOLE>((OT *)p.pre + m * p.spre + n, left, z);
+  if (p.act == kActSilu) {
 #pragma unroll
-    for (int q = 0; q < W; ++q) z[q] = lin_act(z[q], p.act);
+    for (int q = 0; q < W; ++q) z[q] = lin_act(z[q], kActSilu);
+  } else if (p.act == kActGelu) {
+#pragma unroll
+    for (int q = 0; q < W; ++q) z[q] = lin_act(z[q], kActGelu);
   }
   if (p.residual) {
     float r[W];
-    lin_load<OT, W>((const OT *)p.residual + m * p.sr + n, left, r);
+    lin_load<OT, W, WHOLE>((const OT *)p.residual + m * p.sr + n, left, r);
 #pragma unroll
     for (int q = 0; q < W; ++q) z[q] += r[q];
   }
-  lin_store<OT, W>((OT *)p.C + m * p.sc + n, left, z);
+  lin_store<OT, W, WHOLE>((OT *)p.C + m * p.sc + n, left, z);
 }
 
 // ------------------------------------------------------------------ tiles
@@ -130,7 +135,7 @@ __device__ __forceinline__ void lin_epilogue(const GemmParams &p, int64_t m, int
 //                 4 values of k
 // B is the first operand of the matrix instructions, so a lane holds consecutive n of a row of C.  B's rows along k are
 // dealt to the instructions such that the NT results a lane has of a row are 4 NT consecutive n.
-template <bool ALONG, int R, int NW, int SPREAD>   // R rows (or columns); the share of one of NW wavefronts
+template <bool ALONG, int R, int NW, int SPREAD, bool TWICE>   // R rows (or columns); the share of one of NW wavefronts; TWICE: 32 bytes a lane and instruction
 struct LinTile {
   static constexpr int bytes = R * 128, loads = bytes / 1024 / NW;
   static constexpr int line = ALONG ? 128 : 2 * R, pieces = line / 16, rows = 64 / pieces;   // rows: of one load
@@ -159,21 +164,32 @@ struct LinTile {
     for (int i = 0; i < loads; ++i)
       __builtin_amdgcn_raw_ptr_buffer_load_lds(r, (LdsPtr)(lds + (i * NW + wave) * 1024), 16, o + i * step, 0, 0, 0);
   }
-  // the operand of 16 rows (along k: `row` is the lane's own; else the first of the lane's group), step kk of the tile
-  template <typename T>
-  __device__ __forceinline__ static typename Mma<T>::Frag get(const char *__restrict lds, int row, int kk) {
+  // Where the lane reads the operand of the 16 rows from `first` on, and from there the operands of the rows 16 i (along k
+  // in B's dealing: 4 i) further on, step kk of the tile.
+  __device__ __forceinline__ static int place(int first) {
     const int lane = threadIdx.x % 64, g = lane / 16;
-    if constexpr (ALONG && Mma<T>::bytes == 32) {
-      const int at = row * 128 + piece(row, 2 * g) * 16;
-      const li4 lo = *(const li4 *)(lds + at), hi = *(const li4 *)(lds + (at ^ 16));
-      return __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
-    } else if constexpr (ALONG) {
-      return *(const li4 *)(lds + row * 128 + piece(row, 4 * kk + g) * 16);
+    if constexpr (ALONG) {
+      const int row = first + (SPREAD == 4 ? lane % 16 : SPREAD * ((lane % 16) / 4) + lane % 4);
+      return row * 128 + piece(row, TWICE ? 2 * g : g) * 16;
     } else {
-      const int k = 32 * kk + 8 * g + (lane % 16) / 4, col = 2 * row + 8 * (lane % 4);   // bytes
-      const char *lo = lds + k * line + piece(k, col / 16) * 16 + col % 16;
-      const char *hi = lds + (k + 4) * line + piece(k + 4, col / 16) * 16 + col % 16;
-      const ls4 a = __builtin_amdgcn_ds_read_tr16_b64_v4i16((LdsTr)lo), b = __builtin_amdgcn_ds_read_tr16_b64_v4i16((LdsTr)hi);
+      const int k = 8 * g + (lane % 16) / 4, col = 2 * first + 8 * (lane % 4);   // bytes
+      return k * line + piece(k, col / 16) * 16 + col % 16;
+    }
+  }
+  template <typename T>
+  __device__ __forceinline__ static typename Mma<T>::Frag get(const char *__restrict lds, int place, int i, int kk) {
+    if constexpr (ALONG) {
+      const char *at = lds + (SPREAD == 4 ? 16 : 4) * 128 * i;
+      if constexpr (Mma<T>::bytes == 32) {
+        const li4 lo = *(const li4 *)(at + place), hi = *(const li4 *)(at + (place ^ 16));
+        return __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
+      } else {
+        return *(const li4 *)(at + (place ^ (64 * kk)));
+      }
+    } else {   // 16 columns on: two pieces; 4 k on: the pairs of pieces are dealt 4 pairs further; 32 k on: as here
+      const char *at = lds + 32 * kk * line;
+      const ls4 a = __builtin_amdgcn_ds_read_tr16_b64_v4i16((LdsTr)(at + (place ^ (32 * i))));
+      const ls4 b = __builtin_amdgcn_ds_read_tr16_b64_v4i16((LdsTr)(at + 4 * line + (place ^ (32 * i) ^ 128)));
       return __builtin_bit_cast(li4, __builtin_shufflevector(a, b, 0, 1, 2, 3, 4, 5, 6, 7));
     }
   }
@@ -183,8 +199,8 @@ template <typename T, typename OT, bool AL, bool BL, int BM, int BN, int WM, int
 __global__ void __launch_bounds__(64 * WM * WN) __attribute__((amdgpu_waves_per_eu(2, 2))) k_linear_tile(const GemmParams p) {
   constexpr int NW = WM * WN, MT = BM / WM / 16, NT = BN / WN / 16, E = sizeof(T);
   constexpr int KE = AL || BL ? 128 / E : 64, STEPS = 128 / (4 * Mma<T>::bytes);
-  typedef LinTile<AL, BM, NW, 4> TA;
-  typedef LinTile<BL, BN, NW, 4 * NT> TB;
+  typedef LinTile<AL, BM, NW, 4, E == 1> TA;
+  typedef LinTile<BL, BN, NW, 4 * NT, E == 1> TB;
   __shared__ __attribute__((aligned(1024))) char As0[TA::bytes], Bs0[TB::bytes], As1[TA::bytes], Bs1[TB::bytes];
   // Tiles in the order that the 8 dies take workgroups: each die its own run of them, 8 rows of tiles by columns.
   const uint32_t tm = (uint32_t)((p.M + BM - 1) / BM), tn = (uint32_t)((p.N + BN - 1) / BN), tiles = tm * tn;
@@ -217,76 +233,125 @@ __global__ void __launch_bounds__(64 * WM * WN) __attribute__((amdgpu_waves_per_
     __builtin_amdgcn_sched_barrier(0);   // the loads are under way before the products
   };
   const int lane = threadIdx.x % 64, wave = ta.wave, wm = wave / WN * (BM / WM), wn = wave % WN * (BN / WN);
-  const int ra = wm + (AL ? lane % 16 : 0);
-  const int rb = wn + (BL ? 4 * NT * ((lane % 16) / 4) + lane % 4 : 0);
+  const int pa = TA::place(wm), pb = TB::place(wn);
   lf4 acc[MT][NT] = {};
-  auto multiply = [&](const char *__restrict as, const char *__restrict bs) {
+  struct Operands {
+    typename Mma<T>::Frag a[MT], b[NT];
+  };
+  auto read = [&](Operands &f, const char *__restrict as, const char *__restrict bs, int kk) {
+    int qa = pa, qb = pb;   // the reads' addresses are formed anew each time: all of them would not fit the registers
+    if (!AL || !BL) asm volatile("" : "+v"(qa), "+v"(qb));
 #pragma unroll
-    for (int kk = 0; kk < STEPS; ++kk) {
-      typename Mma<T>::Frag fa[MT], fb[NT];
+    for (int j = 0; j < NT; ++j) f.b[j] = TB::template get<T>(bs, qb, j, kk);
 #pragma unroll
-      for (int j = 0; j < NT; ++j) fb[j] = TB::template get<T>(bs, rb + (BL ? 4 : 16) * j, kk);
+    for (int i = 0; i < MT; ++i) f.a[i] = TA::template get<T>(as, qa, i, kk);
+  };
+  auto multiply = [&](const Operands &f) {
 #pragma unroll
-      for (int i = 0; i < MT; ++i) fa[i] = TA::template get<T>(as, ra + 16 * i, kk);
+    for (int i = 0; i < MT; ++i)
 #pragma unroll
-      for (int i = 0; i < MT; ++i)
+      for (int j = 0; j < NT; ++j) acc[i][j] = Mma<T>::mul(f.b[j], f.a[i], acc[i][j]);
+  };
+  // spreads a half's reads over the other half's products
+  auto interleave = [&] {
+    constexpr int reads = NT * (BL ? 1 : 2) + MT * (AL ? 1 : 2);
 #pragma unroll
-        for (int j = 0; j < NT; ++j) acc[i][j] = Mma<T>::mul(fb[j], fa[i], acc[i][j]);
-    }
-    // the operands of two rows of products ahead of them, then two reads a row
-    constexpr int each = Mma<T>::bytes == 32 || !AL ? 2 : 1;
-    __builtin_amdgcn_sched_group_barrier(0x100, (NT + 2) * each, 0);
-#pragma unroll
-    for (int i = 0; i < MT * STEPS; ++i) {
+    for (int i = 0; i < MT; ++i) {
       __builtin_amdgcn_sched_group_barrier(0x008, NT, 0);
-      __builtin_amdgcn_sched_group_barrier(0x100, 2 * each, 0);
+      __builtin_amdgcn_sched_group_barrier(0x100, (reads + MT - 1) / MT, 0);
     }
   };
   auto arrived = [&] {
     asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
     lds_barrier();
   };
-  load(As0, Bs0);
-  arrived();
-  int s = s0;
-  for (; s + 1 < s1; s += 2) {
+  if constexpr (STEPS == 2) {
+    // A step in halves: the products of one while the operands of the next are read.  Where the second half has been read,
+    // all wavefronts are done with the step's buffer and the next step's loads, issued a whole step before, have come:
+    // one barrier, behind which the buffer is filled for the step after the next.
+    Operands f0, f1;
+    load(As0, Bs0);
     load(As1, Bs1);
-    multiply(As0, Bs0);
     arrived();
-    load(As0, Bs0);   // past the last step: beyond the split's end, and not used
-    multiply(As1, Bs1);
+    read(f0, As0, Bs0, 0);
+    auto step = [&](char *__restrict a0, char *__restrict b0, char *__restrict a1, char *__restrict b1) {
+      read(f1, a0, b0, 1);
+      multiply(f0);
+      interleave();
+      arrived();
+      load(a0, b0);
+      read(f0, a1, b1, 0);
+      multiply(f1);
+      interleave();
+      __builtin_amdgcn_sched_barrier(0);
+    };
+    int s = s0;
+    for (; s + 1 < s1; s += 2) {   // loads past the split's end bring nothing that is used
+      step(As0, Bs0, As1, Bs1);
+      step(As1, Bs1, As0, Bs0);
+    }
+    if (s < s1) {
+      read(f1, As0, Bs0, 1);
+      multiply(f0);
+      multiply(f1);
+    }
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");   // no load into LDS outlives the workgroup
+  } else {
+    Operands f;
+    load(As0, Bs0);
     arrived();
+    int s = s0;
+    auto step = [&](const char *__restrict as, const char *__restrict bs) {
+      read(f, as, bs, 0);
+      multiply(f);
+      constexpr int each = 2;
+      __builtin_amdgcn_sched_group_barrier(0x100, (NT + 2) * each, 0);
+#pragma unroll
+      for (int i = 0; i < MT; ++i) {
+        __builtin_amdgcn_sched_group_barrier(0x008, NT, 0);
+        __builtin_amdgcn_sched_group_barrier(0x100, 2 * each, 0);
+      }
+    };
+    for (; s + 1 < s1; s += 2) {
+      load(As1, Bs1);
+      step(As0, Bs0);
+      arrived();
+      load(As0, Bs0);   // past the last step: beyond the split's end, and not used
+      step(As1, Bs1);
+      arrived();
+    }
+    if (s < s1) step(As0, Bs0);
   }
-  if (s < s1) multiply(As0, Bs0);
+  auto write = [&](auto whole) {
+    constexpr bool WHOLE = decltype(whole)::value;
 #pragma unroll
-  for (int i = 0; i < MT; ++i) {
-    const int64_t m = m0 + wm + 16 * i + lane % 16;
-    if (m >= p.M) continue;
-    if (p.splits > 1) {
+    for (int i = 0; i < MT; ++i) {
+      const int64_t m = m0 + wm + 16 * i + lane % 16;
+      if (!WHOLE && m >= p.M) continue;
+      if (p.splits > 1) {
 #pragma unroll
-      for (int j = 0; j < NT; ++j) {
-        const int64_t n = n0 + wn + (BL ? 4 * NT * (lane / 16) + 4 * j : 16 * j + 4 * (lane / 16));
-        const float v[4] = {acc[i][j][0], acc[i][j][1], acc[i][j][2], acc[i][j][3]};
-        if (n < p.N) lin_store<float, 4>(p.partial + (split * p.M + m) * p.N + n, p.N - n, v);
-      }
-    } else if constexpr (BL) {
+        for (int j = 0; j < NT; ++j) {
+          const int64_t n = n0 + wn + (BL ? 4 * NT * (lane / 16) + 4 * j : 16 * j + 4 * (lane / 16));
+          const float v[4] = {acc[i][j][0], acc[i][j][1], acc[i][j][2], acc[i][j][3]};
+          if (WHOLE || n < p.N) lin_store<float, 4, WHOLE>(p.partial + (split * p.M + m) * p.N + n, p.N - n, v);
+        }
+      } else {
+        constexpr int W = BL ? 8 : 4;
 #pragma unroll
-      for (int j = 0; j < NT; j += 2) {
-        const int64_t n = n0 + wn + 4 * NT * (lane / 16) + 4 * j;
-        float v[8];
+        for (int j = 0; j < NT; j += W / 4) {
+          const int64_t n = n0 + wn + (BL ? 4 * NT * (lane / 16) + 4 * j : 16 * j + 4 * (lane / 16));
+          float v[W];
 #pragma unroll
-        for (int q = 0; q < 8; ++q) v[q] = acc[i][j + q / 4][q % 4];
-        if (n < p.N) lin_epilogue<OT, 8>(p, m, n, v);
-      }
-    } else {
-#pragma unroll
-      for (int j = 0; j < NT; ++j) {
-        const int64_t n = n0 + wn + 16 * j + 4 * (lane / 16);
-        float v[4] = {acc[i][j][0], acc[i][j][1], acc[i][j][2], acc[i][j][3]};
-        if (n < p.N) lin_epilogue<OT, 4>(p, m, n, v);
+          for (int q = 0; q < W; ++q) v[q] = acc[i][j + q / 4][q % 4];
+          if (!WHOLE && n >= p.N) continue;
+          if constexpr (BL) lin_epilogue<OT, W, WHOLE>(p, m, n, v);
+          else lin_store<OT, W, WHOLE>((OT *)p.C + m * p.sc + n, p.N - n, v);   // the backward's products have no epilogue
+        }
       }
     }
-  }
+  };
+  if (m0 + BM <= p.M && n0 + BN <= p.N) write(std::true_type{});
+  else write(std::false_type{});
 }
 
 // The splits' sums in order, and the epilogue: 8 consecutive n a thread.
@@ -301,7 +366,7 @@ __global__ void __launch_bounds__(256) k_linear_join(const GemmParams p) {
 #pragma unroll
     for (int q = 0; q < 8; ++q) z[q] += v[q];
   }
-  lin_epilogue<OT, 8>(p, m, n, z);
+  lin_epilogue<OT, 8, false>(p, m, n, z);
 }
 
 // ------------------------------------------------------------------ few rows
@@ -377,7 +442,7 @@ __global__ void __launch_bounds__(512) k_linear_rows(const GemmParams p) {
 #pragma unroll
       for (int q = 0; q < 8; ++q) z[q] += red[v][mi][c + q];
     if (p.splits > 1) lin_store<float, 8>(p.partial + (split * p.M + m) * p.N + n, p.N - n, z);
-    else lin_epilogue<OT, 8>(p, m, n, z);
+    else lin_epilogue<OT, 8, false>(p, m, n, z);
   }
 }
 
