@@ -1679,7 +1679,7 @@ int ssm_sample_check(const ssm_sample_args *a) {
   if (!a) return fail(SSM_EINVAL, "null args");
   if (!io16_32(a->dtype)) return fail(SSM_EINVAL, "logits must be float32, bfloat16 or float16");
   if (a->rows < 1 || a->vocab < 1) return fail(SSM_EINVAL, "empty logits: rows=%lld vocab=%lld", (long long)a->rows, (long long)a->vocab);
-  if (a->rows >= (1LL << 40) || a->vocab > (1LL << 24))
+  if (a->rows >= (1LL << 31) || a->vocab > (1LL << 24))
     return fail(SSM_EINVAL, "logits are too large: rows=%lld vocab=%lld (at most 2^24)", (long long)a->rows, (long long)a->vocab);
   if (!a->temperatures && !(a->temperature >= 0)) return fail(SSM_EINVAL, "temperature must be >= 0, got %g", a->temperature);
   if (!a->top_ks && a->top_k < 0) return fail(SSM_EINVAL, "top_k must be >= 0, got %lld", (long long)a->top_k);
@@ -1687,25 +1687,66 @@ int ssm_sample_check(const ssm_sample_args *a) {
   if (!a->min_ps && !(a->min_p >= 0)) return fail(SSM_EINVAL, "min_p must be >= 0, got %g", a->min_p);
   return ok();
 }
+namespace {
+struct SampleLayout {
+  int64_t chunks, chunk, parts, ntiles, filtered, firsts, cuts, tiles, masses, counts;
+  int64_t bytes() const { return firsts + cuts + tiles + masses + counts; }
+};
+SampleLayout sample_layout(const ssm_sample_args *a) {
+  SampleLayout l{};
+  if (a->vocab <= kSampleRow) return l;
+  l.chunk = a->rows * cdiv(a->vocab, kSampleRow) >= 64 ? kSampleRow : kSampleRow / 4;   // small chunks where there are few
+  l.chunks = cdiv(a->vocab, l.chunk);
+  l.parts = cdiv(a->vocab, 8192);
+  l.ntiles = cdiv(a->vocab, 512);
+  const bool greedy = !a->temperatures && a->temperature == 0;
+  l.filtered = greedy || a->top_ks || a->top_k > 0 || a->top_ps || a->top_p < 1 || a->temperatures || a->min_ps || a->min_p > 0;
+  l.firsts = align256(a->rows * l.parts * 8);
+  l.tiles = align256(a->rows * l.ntiles * 8);
+  if (l.filtered) {
+    l.cuts = align256(a->rows * 8);
+    l.masses = align256(a->rows * l.chunks * 2048 * 8);
+    l.counts = align256(a->rows * l.chunks * 2048 * 4);
+  }
+  return l;
+}
+}  // namespace
 int64_t ssm_sample_workspace_bytes(const ssm_sample_args *a) {
   if (ssm_sample_check(a)) return -1;
-  return 0;
+  return sample_layout(a).bytes();
 }
 int ssm_sample(const ssm_sample_args *a, void *stream) {
   int rc = ssm_sample_check(a);
   if (!rc) rc = gnorm_view(a->logits, "logits");
   if (!rc) rc = need({{a->u, "u"}, {a->token, "token"}, {a->logprob, "logprob"}});
   if (rc) return rc;
+  const SampleLayout l = sample_layout(a);
+  if (l.bytes() && (!a->workspace || a->workspace_bytes < l.bytes()))
+    return fail(SSM_ESPACE, "workspace of %lld bytes required", (long long)l.bytes());
   SampleParams p{};
   p.R = a->rows; p.V = a->vocab;
   p.logits = a->logits.data; p.sl = a->logits.stride[0];
   p.u = a->u; p.u_f64 = a->u_f64;
   int bits = 0;
   while ((a->vocab >> bits) > 0) ++bits;
-  p.shift = std::min(52, 62 - bits);
+  p.shift = std::min(51, 62 - bits);
   p.temperature = a->temperature; p.top_p = a->top_p; p.min_p = a->min_p; p.top_k = a->top_k;
   p.temperatures = a->temperatures; p.top_ps = a->top_ps; p.min_ps = a->min_ps; p.top_ks = a->top_ks;
   p.token = a->token; p.logprob = a->logprob;
+  p.chunks = l.chunks; p.parts = l.parts; p.chunk = (int)l.chunk; p.ntiles = l.ntiles; p.filtered = (int)l.filtered;
+  char *ws = (char *)a->workspace;
+  auto take = [&](int64_t bytes) {
+    char *at = ws;
+    ws += bytes;
+    return at;
+  };
+  if (l.chunks) {
+    p.firsts = (uint64_t *)take(l.firsts);
+    p.tiles = (uint64_t *)take(l.tiles);
+    p.cuts = (uint64_t *)take(l.cuts);
+    p.masses = (uint64_t *)take(l.masses);
+    p.counts = (uint32_t *)take(l.counts);
+  }
   hipError_t e = launch_sample(p, a->dtype, (hipStream_t)stream);
   return e == hipSuccess ? ok() : hip_fail(e, "ssm_sample");
 }

@@ -1173,16 +1173,16 @@ py::tuple sample(const Tensor &logits, const Tensor &u_, const py::object &tempe
   const bool none = a.rows == 0;
   if (none) a.rows = 1;   // the settings are checked all the same
   a.dtype = dtype_code(logits.scalar_type());
+  a.temperatures = t.defined() ? t.data_ptr<float>() : nullptr;
+  a.top_ks = k.defined() ? k.data_ptr<int64_t>() : nullptr;
+  a.top_ps = p.defined() ? p.data_ptr<float>() : nullptr;
+  a.min_ps = m.defined() ? m.data_ptr<float>() : nullptr;
   SSM_BYTES(n, ssm_sample_workspace_bytes, ssm_sample_check, a, "ssm_sample");
   if (none) return py::make_tuple(token, logprob);
   const Tensor x2 = rows(logits, a.vocab), u = u_.contiguous();
   a.logits = view(x2);
   a.u = u.data_ptr();
   a.u_f64 = u.scalar_type() == at::kDouble;
-  a.temperatures = t.defined() ? t.data_ptr<float>() : nullptr;
-  a.top_ks = k.defined() ? k.data_ptr<int64_t>() : nullptr;
-  a.top_ps = p.defined() ? p.data_ptr<float>() : nullptr;
-  a.min_ps = m.defined() ? m.data_ptr<float>() : nullptr;
   a.token = token.data_ptr<int64_t>();
   a.logprob = logprob.data_ptr<float>();
   Tensor ws;

@@ -427,7 +427,13 @@ struct SampleParams {
   const int64_t *top_ks;
   int64_t *token;
   float *logprob;
+  // rows that are walked in chunks (chunks = 0: in one workgroup)
+  int64_t chunks, parts, ntiles;       // a row's: chunks of `chunk` logits, parts of 8192, tiles of 512
+  int chunk, filtered;                 // a top_k, top_p, min_p or temperature of 0 may be in effect
+  uint64_t *firsts, *cuts, *tiles, *masses;  // (rows, parts), (rows), (rows, ntiles), (rows, chunks, 2048)
+  uint32_t *counts;                    // (rows, chunks, 2048)
 };
+constexpr int64_t kSampleRow = 32768;  // logits that a workgroup holds in registers
 hipError_t launch_sample(const SampleParams &p, int dtype, hipStream_t s);
 
 // Products C[m, n] = sum over k of A(m, k) B(n, k) with the linear layer's epilogue.

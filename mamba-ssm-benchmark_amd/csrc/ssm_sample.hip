@@ -3,9 +3,19 @@
 // those the shortest prefix that holds top_p of their mass, of those the ones with w_i >= min_p, and always the first;
 // the token is the first kept index at which the running sum of the kept weights, by index, passes u times their sum.
 //
-// Weights are 64-bit integers, w_i 2^S rounded, S as large as the sum of V of them allows (52 at most): their sums
-// are exact in any order, so LDS atomics give the same token every time, and what is rounded is 2^-S of the largest
+// Weights are 64-bit integers, w_i 2^S rounded, S as large as the sum of V of them allows (51 at most): their sums
+// are exact in any order, so atomics in LDS give the same token every time, and what is rounded is 2^-S of the largest
 // weight, below what a float64 sum of as many terms loses for V <= 2^17.
+//
+// The row is not sorted.  What is kept is a prefix of the order, so it ends at one element, the cut (key, index).  A
+// histogram of 2048 bins by falling logit, of counts for top_k and of weights for top_p, gives the bin that the cut is
+// in; the elements of that bin (some hundred) are gathered and sorted in LDS.  A bin of more than kCandidates is cut
+// by digits of (key, index) instead, 11 bits a pass.  What min_p leaves out is a range of keys, so it only moves the cut.
+//
+// A row of up to 32768 logits is one workgroup's from the maximum to the token.  Longer ones
+// are walked by a workgroup a chunk, in five launches: maxima, histograms, cut (a workgroup a row), kept masses, token.
+#include <type_traits>
+
 #include "ssm_device.hpp"
 #include "ssm_internal.hpp"
 #include "ssm_wave.hpp"
@@ -13,320 +23,678 @@
 namespace ssm {
 
 typedef unsigned long long u64;
+constexpr int kE = 8;                  // consecutive logits a lane reads at once
+constexpr int kTile = 64 * kE;         // and a wavefront
+constexpr int kCandidates = 2048;   // and places of the sort
 
-// Keys in the order of the values, -0 and 0 alike.
+// Keys in the order of the values, -0 and 0 alike; a NaN's is above infinity's.
 __device__ __forceinline__ uint32_t sm_key(float l) {
   const uint32_t u = __float_as_uint(l + 0.0f);
-  return u & 0x80000000u ? ~u : u | 0x80000000u;
+  return l == l ? (u & 0x80000000u ? ~u : u | 0x80000000u) : 0xffffffffu;
 }
 __device__ __forceinline__ float sm_value(uint32_t key) {
   return __uint_as_float(key & 0x80000000u ? key & 0x7fffffffu : ~key);
 }
 
-// E consecutive logits from index i (those past the row's end are -inf), read whole whatever their alignment.
-constexpr int kSampleE = 8;
+// kE consecutive logits from index i, read whole whatever their alignment; those past the row's end are not there.
 template <typename IT>
-__device__ __forceinline__ void sm_load(const IT *row, int64_t i, int64_t V, float (&v)[kSampleE]) {
-  if (i + kSampleE <= V) {
-    IT e[kSampleE];
+__device__ __forceinline__ void sm_load(const IT *row, int64_t i, int64_t V, float (&v)[kE]) {
+  if (i + kE <= V) {
+    IT e[kE];
     __builtin_memcpy(e, row + i, sizeof(e));
 #pragma unroll
-    for (int k = 0; k < kSampleE; ++k) v[k] = to_f32(e[k]);
+    for (int k = 0; k < kE; ++k) v[k] = to_f32(e[k]);
   } else {
 #pragma unroll
-    for (int k = 0; k < kSampleE; ++k) v[k] = i + k < V ? to_f32(row[i + k]) : -INFINITY;
+    for (int k = 0; k < kE; ++k) v[k] = i + k < V ? to_f32(row[i + k]) : -INFINITY;
   }
 }
 
+// A row's settings and its weights.  exp2(t / 256) = 2^(i / 256) e^x with i the nearest whole number, |x| <= ln 2 / 512: the
+// first factor from a table in LDS and the exponent, the second as its series to x^4 (the rest is below 4e-17).
+constexpr int kTable = 256;
 struct SampleRow {
-  double inv_t, scale;   // 1 / T; 2^S
-  float top;             // the largest logit
-  double temperature;
-  __device__ __forceinline__ double z(float l) const { return l == top ? 0.0 : ((double)l - (double)top) / temperature; }
-  __device__ __forceinline__ u64 weight(float l) const { return (u64)(exp(z(l)) * scale + 0.5); }
+  double top, step;   // the largest logit; 256 / (T ln 2)
+  double temperature, lowest;
+  float topf, octave64;   // 64 / (T ln 2)
+  int shift;
+  uint32_t top_key;
+  const double *table;
+  __device__ __forceinline__ double z(float l) const { return l == topf ? 0.0 : ((double)l - top) / temperature; }
+  __device__ __forceinline__ u64 weight(float l) const {
+    constexpr double whole = 6755399441055744.0, one = 4503599627370496.0, h = 0.0027076061740622863;   // 1.5 2^52, 2^52, ln 2 / 256
+    const double t = l == topf ? 0.0 : fmax(((double)l - top) * step, -2e5);
+    const double n = t + whole, x = t - (n - whole);
+    const int i = (int)(uint32_t)__builtin_bit_cast(u64, n);
+    double e = fma(x, h * h * h * h / 24, h * h * h / 6);
+    e = fma(x, e, h * h / 2);
+    e = fma(x, e, h);
+    e = fma(x, e, 1.0);
+    // w 2^shift + 2^52, whose low bits are the number: w < 2^52
+    const u64 f = __builtin_bit_cast(u64, table[i & (kTable - 1)]) + ((u64)(uint32_t)(i >> 8) << 52);
+    return __builtin_bit_cast(u64, fma(__builtin_bit_cast(double, f), e, one)) - __builtin_bit_cast(u64, one);
+  }
+  // 1/64 octaves of weight down from the top: 1792 bins of one, then 32 a doubling; falling logits, rising bins.
+  __device__ __forceinline__ int bin(float l) const {
+    if (l == topf) return 0;
+    const float d = (topf - l) * octave64;
+    return d < 1792.0f ? (int)d : d < 458752.0f ? 1792 + (int)((__float_as_uint(d) - __float_as_uint(1792.0f)) >> 18) : 2047;
+  }
 };
+constexpr int kBins = 2048;
+struct SampleSettings {
+  int64_t k;          // 0: all
+  double top_p;       // >= 1: all
+};
+__device__ __forceinline__ SampleSettings sm_settings(const SampleParams &p, int64_t row, SampleRow &r) {
+  SampleSettings s;
+  r.temperature = p.temperatures ? (double)p.temperatures[row] : p.temperature;
+  s.k = p.top_ks ? p.top_ks[row] : p.top_k;
+  s.top_p = p.top_ps ? (double)p.top_ps[row] : p.top_p;
+  const double min_p = p.min_ps ? (double)p.min_ps[row] : p.min_p;
+  if (!(r.temperature > 0)) {
+    r.temperature = 1;
+    s.k = 1;
+  }
+  if (s.k < 0 || s.k >= p.V) s.k = 0;
+  if (!(s.top_p < 1)) s.top_p = 1;
+  r.lowest = min_p > 0 ? log(min_p < 1 ? min_p : 1.0) : -INFINITY;
+  r.step = 369.3299304757465 / r.temperature;   // 256 / ln 2
+  r.octave64 = (float)(r.step / 4);
+  r.shift = p.shift;
+  return s;
+}
+// (key, first index) of the row's largest logit, as a number that is larger the earlier in the order
+__device__ __forceinline__ u64 sm_place(uint32_t key, uint32_t i) { return (u64)key << 32 | (uint32_t)~i; }
+__device__ __forceinline__ bool sm_top(SampleRow &r, u64 best) {   // false: no distribution
+  r.top_key = (uint32_t)(best >> 32);
+  r.topf = sm_value(r.top_key);
+  r.top = r.topf;
+  return r.top_key != 0xffffffffu && r.topf != -INFINITY;
+}
 
 template <int NT, typename T, typename F>
 __device__ __forceinline__ T sm_block(T v, T *lds, F f) {   // f over all threads' values, to all of them
 #pragma unroll
   for (int d = 1; d < 64; d *= 2) v = f(v, (T)__shfl_xor(v, d));
-  __syncthreads();
-  if (threadIdx.x % 64 == 0) lds[threadIdx.x / 64] = v;
-  __syncthreads();
-  v = lds[0];
-  for (int k = 1; k < NT / 64; ++k) v = f(v, lds[k]);
+  if constexpr (NT > 64) {
+    __syncthreads();
+    if (threadIdx.x % 64 == 0) lds[threadIdx.x / 64] = v;
+    __syncthreads();
+    v = lds[0];
+    for (int k = 1; k < NT / 64; ++k) v = f(v, lds[k]);
+  }
+  return v;
+}
+__device__ __forceinline__ u64 sm_scan(u64 v) {   // inclusive, over the wavefront
+#pragma unroll
+  for (int d = 1; d < 64; d *= 2) {
+    const u64 t = __shfl_up(v, d);
+    if ((int)(threadIdx.x % 64) >= d) v += t;
+  }
   return v;
 }
 
-// Walks the NB bins of `hist` from the highest down to the one at which the sum reaches `target` (> 0, at most the
-// whole): its index, and the sum above it.
+template <int NT> struct SampleLds {
+  u64 mass[kBins];
+  uint32_t count[kBins];
+  u64 place[kCandidates];
+  double table[kTable];
+  u64 red[NT / 64];
+  u64 above, cut;
+  int bin, n;
+};
 template <int NT>
-__device__ __forceinline__ void sm_find(const u64 *hist, int nb, u64 target, u64 *lds, int *bin, u64 *above) {
-  const int per = (nb + NT - 1) / NT, hi = nb - (int)threadIdx.x * per;   // bins [hi - per, hi) of this thread
-  u64 mine = 0;
-  for (int b = hi - 1; b >= hi - per; --b)
-    if (b >= 0 && b < nb) mine += hist[b];
-  u64 upto = mine;
+__device__ __forceinline__ void sm_table(double *table, SampleRow &r) {   // before a barrier
+  for (int i = threadIdx.x; i < kTable; i += NT) table[i] = ldexp(exp2((double)i / kTable), r.shift);
+  r.table = table;
+}
+
+// The first of kBins bins at which the running sum reaches `target` (1 .. the whole), into m.bin, and the sum before
+// it, into m.above.
+template <int NT, typename C>
+__device__ __forceinline__ void sm_find(SampleLds<NT> &m, const C *bins, u64 target) {
+  constexpr int per = kBins / NT;
+  u64 v[per], mine = 0;
 #pragma unroll
-  for (int d = 1; d < 64; d *= 2) {
-    const u64 t = __shfl_up(upto, d);
-    if (threadIdx.x % 64 >= d) upto += t;
-  }
+  for (int k = 0; k < per; ++k) mine += v[k] = bins[threadIdx.x * per + k];
+  u64 upto = sm_scan(mine);
   __syncthreads();
-  if (threadIdx.x % 64 == 63) lds[threadIdx.x / 64] = upto;
+  if (threadIdx.x % 64 == 63) m.red[threadIdx.x / 64] = upto;
   __syncthreads();
-  for (int k = 0; k < (int)threadIdx.x / 64; ++k) upto += lds[k];
+  for (int k = 0; k < (int)threadIdx.x / 64; ++k) upto += m.red[k];
   u64 sum = upto - mine;
-  if (sum < target && upto >= target)
-    for (int b = hi - 1; b >= hi - per; --b) {
-      if (b < 0 || b >= nb) continue;
-      if (sum + hist[b] >= target) {
-        *bin = b;
-        *above = sum;
-        break;
+  if (sum < target && upto >= target) {
+#pragma unroll
+    for (int k = 0; k < per; ++k) {
+      if (sum < target && sum + v[k] >= target) {
+        m.bin = threadIdx.x * per + k;
+        m.above = sum;
       }
-      sum += hist[b];
+      sum += v[k];
     }
+  }
   __syncthreads();
 }
 
-template <typename IT, int NT>
-__global__ void __launch_bounds__(NT) k_sample(const SampleParams p) {
-  constexpr int kBits = 11, kBins = 1 << kBits, kSteps = 2048;
-  __shared__ u64 hist[kBins];          // also: masses of the steps
-  __shared__ uint32_t ties[kSteps];
-  __shared__ u64 red[NT / 64];
-  __shared__ int bin;
-  __shared__ u64 above;
+// The smallest key from -inf's to the top's at which in(l) holds, which does from there on.  A wavefront tries 64 at once.
+template <typename F>
+__device__ __forceinline__ uint32_t sm_border(const SampleRow &r, F in) {
+  const uint32_t lane = threadIdx.x % 64;
+  uint32_t from = 0x007fffffu, n = r.top_key - from;   // it is one of from .. from + n
+  while (n) {
+    const uint32_t step = n / 64 + 1, mine = lane * step;
+    const u64 yes = __ballot(mine <= n && in(sm_value(from + mine)));
+    const uint32_t l = yes ? __ffsll((long long)yes) - 1 : n / step + 1;   // the first lane that it holds for, or past the last one tried
+    const uint32_t lower = l ? (l - 1) * step + 1 : 0, upper = yes ? l * step : n;
+    from += lower;
+    n = upper - lower;
+  }
+  return from;
+}
+// The logits of bin `bin`, from hi down to lo: bins rise with falling keys, so each is a range of them.
+__device__ __forceinline__ void sm_range(const SampleRow &r, int bin, float &lo, float &hi) {
+  lo = sm_value(sm_border(r, [&](float l) { return r.bin(l) <= bin; }));
+  hi = bin ? sm_value(sm_border(r, [&](float l) { return r.bin(l) < bin; }) - 1) : r.topf;
+}
+// Gathers the elements of a range of logits; m.n counts them, the first kCandidates are kept.
+template <int NT, typename Each>
+__device__ __forceinline__ int sm_gather(SampleLds<NT> &m, const SampleRow &r, Each each, float lo, float hi) {
+  if (threadIdx.x == 0) m.n = 0;
+  __syncthreads();
+  each([&](uint32_t i, float l) {
+    if (!(l >= lo && l <= hi)) return;
+    const int at = atomicAdd(&m.n, 1);
+    if (at < kCandidates) m.place[at] = sm_place(sm_key(l), i);
+  });
+  __syncthreads();
+  return m.n;
+}
+// Of the elements of a range of logits the one at which the running sum of value(l, place), by falling place, reaches
+// `target` (1 .. the whole), as its place.  n: how many there are, of which up to kCandidates have been gathered; ones:
+// every value is one.
+template <int NT, typename Each, typename Value>
+__device__ __forceinline__ u64 sm_cut(SampleLds<NT> &m, Each each, float lo, float hi, int n, u64 target, bool ones, Value value) {
+  if (n <= kCandidates) {
+    int P = 64;
+    while (P < n) P *= 2;
+    for (int c = n + threadIdx.x; c < P; c += NT) m.place[c] = 0;   // below any element's
+    __syncthreads();
+    for (int k = 2; k <= P; k *= 2)   // falling order, by a bitonic network
+      for (int d = k / 2; d; d /= 2) {
+        for (int e = threadIdx.x; e < P / 2; e += NT) {
+          const int x = 2 * e - (e & (d - 1)), y = x + d;
+          const u64 u = m.place[x], v = m.place[y];
+          if ((u < v) == !(x & k)) {
+            m.place[x] = v;
+            m.place[y] = u;
+          }
+        }
+        __syncthreads();
+      }
+    if (ones) return m.place[target - 1];
+    u64 sum = 0;   // of the elements before this turn's
+    for (int c0 = 0; c0 < n; c0 += NT) {
+      const int c = c0 + threadIdx.x;
+      const u64 at = c < n ? m.place[c] : 0, own = c < n ? value(sm_value((uint32_t)(at >> 32)), at) : 0;
+      u64 upto = sm_scan(own);
+      if (threadIdx.x % 64 == 63) m.red[threadIdx.x / 64] = upto;
+      __syncthreads();
+      u64 all = 0;
+      for (int k = 0; k < NT / 64; ++k) {
+        if (k == (int)threadIdx.x / 64) upto += all;
+        all += m.red[k];
+      }
+      upto += sum;
+      if (upto - own < target && upto >= target) m.cut = at;
+      sum += all;
+      __syncthreads();
+    }
+    return m.cut;
+  }
+  u64 prefix = 0, sum = 0;
+  for (int shift = 53; shift > -11; shift -= 11) {   // digits of 11 bits, the last of 9
+    const int s = shift < 0 ? 0 : shift, bits = shift < 0 ? 11 + shift : 11;
+    for (int b = threadIdx.x; b < kBins; b += NT) m.mass[b] = 0;
+    __syncthreads();
+    each([&](uint32_t i, float l) {
+      if (!(l >= lo && l <= hi)) return;
+      const u64 at = sm_place(sm_key(l), i);
+      if (shift < 53 && at >> (s + bits) != prefix >> (s + bits)) return;
+      atomicAdd(&m.mass[(1 << bits) - 1 - (int)(at >> s & ((1 << bits) - 1))], value(l, at));   // falling
+    });
+    __syncthreads();
+    sm_find<NT>(m, m.mass, target - sum);
+    prefix |= (u64)((1 << bits) - 1 - m.bin) << s;
+    sum += m.above;
+    __syncthreads();
+  }
+  return prefix;
+}
+
+// The cut of a row whose histograms are in m (of counts if k, of weights if top_p): the place of the last kept element,
+// min_p aside.
+template <int NT, typename Each>
+__device__ __forceinline__ u64 sm_select(SampleLds<NT> &m, const SampleRow &r, const SampleSettings &s, Each each) {
+  auto add = [](u64 a, u64 b) { return a + b; };
+  u64 cut = 0, mass = 0;
+  int have = -1, n = 0;   // the bin whose elements are gathered
+  float lo, hi;
+  if (s.k > 1) {
+    sm_find<NT>(m, m.count, (u64)s.k);
+    have = m.bin;
+    const u64 rest = (u64)s.k - m.above;
+    sm_range(r, have, lo, hi);
+    n = sm_gather<NT>(m, r, each, lo, hi);
+    u64 save[kBins / NT];   // cutting by digits takes the histogram's place
+#pragma unroll
+    for (int b = 0; b < kBins / NT; ++b) save[b] = m.mass[b * NT + threadIdx.x];
+    __syncthreads();
+    cut = sm_cut<NT>(m, each, lo, hi, n, rest, true, [](float, u64) { return (u64)1; });
+    __syncthreads();
+    if (s.top_p < 1) {   // what top_k has left of the weights
+      u64 kept = 0;
+      if (n <= kCandidates) {
+        for (int c = threadIdx.x; c < n; c += NT) kept += m.place[c] >= cut ? r.weight(sm_value((uint32_t)(m.place[c] >> 32))) : 0;
+      } else {
+        each([&](uint32_t i, float l) {
+          if (l >= lo && l <= hi && sm_place(sm_key(l), i) >= cut) kept += r.weight(l);
+        });
+      }
+      kept = sm_block<NT>(kept, m.red, add);
+#pragma unroll
+      for (int b = 0; b < kBins / NT; ++b) {
+        const int at = b * NT + threadIdx.x;
+        m.mass[at] = save[b] = at < have ? save[b] : at == have ? kept : 0;
+        mass += save[b];
+      }
+    }
+  } else {
+    for (int b = threadIdx.x; b < kBins; b += NT) mass += m.mass[b];
+  }
+  if (!(s.top_p < 1)) return cut;
+  mass = sm_block<NT>(mass, m.red, add);
+  const double want = s.top_p > 0 ? ceil(s.top_p * (double)mass) : 1.0;   // the first place at which the sum reaches it is the last one kept
+  u64 target = (u64)want;
+  target = target < 1 ? 1 : target > mass ? mass : target;
+  __syncthreads();
+  sm_find<NT>(m, m.mass, target);
+  const int b = m.bin;
+  const u64 rest = target - m.above, kcut = cut;
+  __syncthreads();
+  if (b != have) {
+    sm_range(r, b, lo, hi);
+    n = sm_gather<NT>(m, r, each, lo, hi);
+  }
+  return sm_cut<NT>(m, each, lo, hi, n, rest, false, [&](float l, u64 at) { return at >= kcut ? r.weight(l) : (u64)0; });
+}
+
+// The cut with min_p: the smallest key that it keeps, at any index.
+__device__ __forceinline__ u64 sm_min_p(const SampleRow &r, u64 cut, u64 first) {
+  if (r.lowest == -INFINITY) return cut;
+  const u64 lowest = (u64)sm_border(r, [&](float l) { return r.z(l) >= r.lowest; }) << 32;
+  cut = cut > lowest ? cut : lowest;
+  return cut < first ? cut : first;   // the first stays
+}
+// The weight of element i in the draw.
+struct SampleCut {
+  float l;
+  uint32_t i;
+  __device__ __forceinline__ explicit SampleCut(u64 cut) : l(sm_value((uint32_t)(cut >> 32))), i((uint32_t)~cut) {
+    if (cut == 0) l = -INFINITY;   // all: -inf has no weight
+  }
+  __device__ __forceinline__ u64 weight(const SampleRow &r, uint32_t at, float v) const {
+    return v > l || (v == l && at <= i) ? r.weight(v) : 0;
+  }
+};
+
+// The running sum that the token's is the first to pass.
+__device__ __forceinline__ u64 sm_goal(const SampleParams &p, int64_t row, u64 total) {
+  const double u = p.u_f64 ? ((const double *)p.u)[row] : (double)((const float *)p.u)[row], x = u * (double)total;
+  const u64 goal = x > 0 ? (u64)x : 0;
+  return goal >= total || u != u ? total - 1 : goal;
+}
+// One wavefront: the tile of `tiles` in which the running sum of their masses passes u times the whole, and the sum
+// before it.
+__device__ __forceinline__ void sm_tile(const SampleParams &p, int64_t row, const u64 *masses, int64_t tiles, int64_t &tile, u64 &run,
+                                        u64 &goal, u64 &total) {
+  const int lane = threadIdx.x % 64;
+  total = 0;
+  for (int64_t t = lane; t < tiles; t += 64) total += masses[t];
+#pragma unroll
+  for (int d = 1; d < 64; d *= 2) total += __shfl_xor(total, d);
+  goal = sm_goal(p, row, total);
+  run = 0;
+  for (int64_t t0 = 0; t0 < tiles; t0 += 64) {
+    const u64 m = t0 + lane < tiles ? masses[t0 + lane] : 0, upto = sm_scan(m), past = __ballot(run + upto > goal);
+    if (past) {
+      const int l = __ffsll((long long)past) - 1;
+      tile = t0 + l;
+      run += __shfl(upto - m, l);
+      return;
+    }
+    run += __shfl(upto, 63);
+  }
+  tile = tiles - 1;   // not reached: the sums end at the total
+}
+// One wavefront: the token, in the tile whose logits its lanes hold.
+__device__ __forceinline__ void sm_pick(const SampleParams &p, const SampleRow &r, int64_t row, const SampleCut &cut, int64_t i, const float (&v)[kE],
+                                        u64 run, u64 goal, u64 total) {
+  u64 w[kE], m = 0;
+#pragma unroll
+  for (int q = 0; q < kE; ++q) m += w[q] = i + q < p.V ? cut.weight(r, (uint32_t)(i + q), v[q]) : 0;
+  const u64 upto = sm_scan(m), past = __ballot(run + upto > goal);
+  if ((int)(threadIdx.x % 64) != __ffsll((long long)past) - 1) return;
+  u64 sum = run + upto - m;
+  int at = 0;
+  float l = v[0];
+#pragma unroll
+  for (int q = 0; q < kE - 1; ++q) {   // the first q whose sum passes
+    sum += w[q];
+    if (sum <= goal) {
+      at = q + 1;
+      l = v[q + 1];
+    }
+  }
+  p.token[row] = i + at;
+  p.logprob[row] = (float)(r.z(l) - (log((double)total) - r.shift * 0.6931471805599453));
+}
+
+// ------------------------------------------------------------------ rows of one workgroup
+template <typename IT, int NT, int J>   // J tiles a wavefront: one stays in registers, more are read anew (from L2) each time
+__global__ void __launch_bounds__(NT) k_sample_row(const SampleParams p) {
+  __shared__ SampleLds<NT> m;
+  __shared__ u64 tiles[J * NT / 64];
   const int64_t row = p.first + blockIdx.x, V = p.V;
   const IT *logits = (const IT *)p.logits + row * p.sl;
   const int lane = threadIdx.x % 64, wave = threadIdx.x / 64;
-  constexpr int64_t kStride = (int64_t)NT * kSampleE;
-  auto each = [&](auto f) {   // f(index, logit) over the row
-    for (int64_t i = (int64_t)threadIdx.x * kSampleE; i < V; i += kStride) {
-      float v[kSampleE];
-      sm_load<IT>(logits, i, V, v);
+  float held[kE];
+  if (threadIdx.x * kE < V) sm_load<IT>(logits, threadIdx.x * kE, V, held);
+  auto tile_at = [&](int j, float (&v)[kE]) {   // the lane's first index
+    const int64_t i = (int64_t)(j * (NT / 64) + wave) * kTile + lane * kE;
+    if (j == 0) {
 #pragma unroll
-      for (int k = 0; k < kSampleE; ++k)
-        if (i + k < V) f(i + k, v[k]);
+      for (int q = 0; q < kE; ++q) v[q] = held[q];
+    } else if (i < V) {
+      sm_load<IT>(logits, i, V, v);
+    }
+    return i;
+  };
+  auto each = [&](auto f) {
+#pragma unroll 2
+    for (int j = 0; j < J; ++j) {
+      float v[kE];
+      const int64_t i = tile_at(j, v);
+#pragma unroll
+      for (int q = 0; q < kE; ++q)
+        if (i + q < V) f((uint32_t)(i + q), v[q]);
     }
   };
-
-  uint32_t top = 0;
-  each([&](int64_t, float l) { top = max(top, l == l ? sm_key(l) : 0xffffffffu); });   // above infinity's: a NaN
-  top = (uint32_t)sm_block<NT>((u64)top, red, [](u64 a, u64 b) { return a > b ? a : b; });
+  u64 first = 0;
+  each([&](uint32_t i, float l) {
+    const u64 at = sm_place(sm_key(l), i);
+    first = at > first ? at : first;
+  });
+  first = sm_block<NT>(first, m.red, [](u64 a, u64 b) { return a > b ? a : b; });
   SampleRow r;
-  r.top = sm_value(top);
-  if (top == 0xffffffffu || r.top == -INFINITY) {   // no distribution
+  const SampleSettings s = sm_settings(p, row, r);
+  if (!sm_top(r, first)) {
     if (threadIdx.x == 0) {
       p.token[row] = -1;
       p.logprob[row] = NAN;
     }
     return;
   }
-  r.temperature = p.temperatures ? (double)p.temperatures[row] : p.temperature;
-  int64_t k = p.top_ks ? p.top_ks[row] : p.top_k;
-  double top_p = p.top_ps ? (double)p.top_ps[row] : p.top_p;
-  const double min_p = p.min_ps ? (double)p.min_ps[row] : p.min_p;
-  if (!(r.temperature > 0)) {
-    r.temperature = 1;
-    k = 1;
-  }
-  r.scale = ldexp(1.0, p.shift);
-  const double lowest = min_p > 0 ? log(min_p < 1 ? min_p : 1.0) : -INFINITY;
-
-  uint32_t cut = 0;              // kept: keys above the cut, and the first `at_cut` of it
-  u64 at_cut = ~0ull;
-  auto select = [&](auto value, u64 target) {   // the key at which the values' sum, by falling key, reaches the target
-    uint32_t prefix = 0;
-    u64 sum = 0;
-    for (int pass = 0; pass < 3; ++pass) {
-      const int shift = pass == 0 ? 21 : pass == 1 ? 10 : 0, bits = pass == 2 ? 10 : 11;
-      for (int b = threadIdx.x; b < kBins; b += NT) hist[b] = 0;
-      __syncthreads();
-      each([&](int64_t, float l) {
-        const uint32_t key = sm_key(l);
-        if (pass == 0 || key >> (shift + bits) == prefix >> (shift + bits))
-          atomicAdd(&hist[(key >> shift) & ((1 << bits) - 1)], value(l, key));
-      });
-      __syncthreads();
-      sm_find<NT>(hist, 1 << bits, target - sum, red, &bin, &above);
-      prefix |= (uint32_t)bin << shift;
-      sum += above;
-      __syncthreads();
+  if (s.k == 1) {
+    if (threadIdx.x == 0) {
+      p.token[row] = (uint32_t)~first;
+      p.logprob[row] = 0.0f;
     }
-    cut = prefix;
-    return sum;   // above the cut
-  };
-  if (k == 1) {
-    cut = top;
-    at_cut = 1;
-  } else if (k > 0 && k < V) {
-    at_cut = (u64)k - select([&](float, uint32_t) { return (u64)1; }, (u64)k);
+    return;
   }
-  if (top_p < 1 && k != 1) {
-    // the mass that is kept so far
-    u64 mass = 0, at = 0;
-    each([&](int64_t, float l) {
-      const uint32_t key = sm_key(l);
-      if (key > cut) mass += r.weight(l);
-      at += key == cut;
+  sm_table<NT>(m.table, r);
+  u64 cut = 0;
+  if (s.k > 1 || s.top_p < 1) {
+    for (int b = threadIdx.x; b < kBins; b += NT) m.mass[b] = m.count[b] = 0;
+    __syncthreads();
+    each([&](uint32_t, float l) {
+      const int b = r.bin(l);
+      if (s.k > 1) atomicAdd(&m.count[b], 1u);
+      if (s.top_p < 1) atomicAdd(&m.mass[b], r.weight(l));
     });
-    mass = sm_block<NT>(mass, red, [](u64 a, u64 b) { return a + b; });
-    at = sm_block<NT>(at, red, [](u64 a, u64 b) { return a + b; });
-    const u64 wcut = cut ? r.weight(sm_value(cut)) : 0;
-    mass += (at < at_cut ? at : at_cut) * wcut;
-    const uint32_t kcut = cut;
-    const u64 at_kcut = at_cut;
-    const double want = top_p > 0 ? top_p * (double)mass : 0.0;
-    u64 target = (u64)ceil(want);   // the first place at which the sum reaches it is the last one kept
-    target = target < 1 ? 1 : target > mass ? mass : target;
-    // of the ties at top_k's cut only the first count: the sum may be reached among them, before those that do not
-    const u64 sum = select([&](float l, uint32_t key) { return key >= kcut ? r.weight(l) : (u64)0; }, target);
-    const u64 w = r.weight(sm_value(cut));
-    at_cut = (target - sum + w - 1) / w;
-    if (cut == kcut && at_kcut < at_cut) at_cut = at_kcut;
+    __syncthreads();
+    cut = sm_select<NT>(m, r, s, each);
   }
-
-  // Masses and ties of every step of 64 x E consecutive logits; steps grow with V so that kSteps of them hold a row.
-  const int64_t unit = 64 * kSampleE;
-  const int64_t fold = (V + unit * kSteps - 1) / (unit * kSteps), step = unit * fold;   // logits a step
-  const int steps = (int)((V + step - 1) / step);
-  auto kept = [&](float l, uint32_t key) { return key >= cut && (key == top || r.z(l) >= lowest); };
-  for (int s = wave; s < steps; s += NT / 64) {
-    u64 m = 0, t = 0;
-    for (int64_t f = 0; f < fold; ++f) {
-      const int64_t i = s * step + f * unit + lane * kSampleE;
-      float v[kSampleE];
-      if (i < V) sm_load<IT>(logits, i, V, v);
+  const SampleCut kept(sm_min_p(r, cut, first));
+  __syncthreads();
+#pragma unroll 1
+  for (int j = 0; j < J; ++j) {
+    float v[kE];
+    const int64_t i = tile_at(j, v);
+    u64 sum = 0;
 #pragma unroll
-      for (int q = 0; q < kSampleE; ++q)
-        if (i + q < V) {
-          const uint32_t key = sm_key(v[q]);
-          if (kept(v[q], key)) {
-            t += key == cut;
-            if (key != cut) m += r.weight(v[q]);
-          }
-        }
-    }
+    for (int q = 0; q < kE; ++q) sum += i + q < V ? kept.weight(r, (uint32_t)(i + q), v[q]) : 0;
 #pragma unroll
-    for (int d = 1; d < 64; d *= 2) {
-      m += __shfl_xor(m, d);
-      t += __shfl_xor(t, d);
-    }
-    if (lane == 0) {
-      hist[s] = m;
-      ties[s] = (uint32_t)t;
-    }
+    for (int d = 1; d < 64; d *= 2) sum += __shfl_xor(sum, d);
+    if (lane == 0) tiles[j * (NT / 64) + wave] = sum;
   }
   __syncthreads();
-  if (wave) return;
-  // one wavefront: the total, the step of the token, then the token
-  const float vcut = sm_value(cut);
-  const u64 wcut = cut ? r.weight(vcut) : 0;
-  auto ties_kept = [&](u64 before, u64 n) { return before >= at_cut ? (u64)0 : n < at_cut - before ? n : at_cut - before; };
-  u64 total = 0, tie_run = 0;
-  for (int s0 = 0; s0 < steps; s0 += 64) {   // ties before each step, in place of them; kept masses
-    const int s = s0 + lane;
-    const u64 n = s < steps ? ties[s] : 0;
-    u64 upto = n;
-#pragma unroll
-    for (int d = 1; d < 64; d *= 2) {
-      const u64 t = __shfl_up(upto, d);
-      if (lane >= d) upto += t;
-    }
-    const u64 before = tie_run + upto - n;
-    u64 m = s < steps ? hist[s] + ties_kept(before, n) * wcut : 0;
-    if (s < steps) {
-      hist[s] = m;
-      ties[s] = (uint32_t)before;
-    }
-    tie_run += __shfl(upto, 63);
-#pragma unroll
-    for (int d = 1; d < 64; d *= 2) m += __shfl_xor(m, d);
-    total += m;
-  }
-  wave_lds_sync();
-  const double u = p.u_f64 ? ((const double *)p.u)[row] : (double)((const float *)p.u)[row];
-  const double x = u * (double)total;
-  u64 goal = x > 0 ? (u64)x : 0;   // the first sum above it
-  if (goal >= total || u != u) goal = total - 1;
-  u64 run = 0;
-  int at = 0;
-  for (int s0 = 0; s0 < steps; s0 += 64) {
-    const int s = s0 + lane;
-    const u64 m = s < steps ? hist[s] : 0;
-    u64 upto = m;
-#pragma unroll
-    for (int d = 1; d < 64; d *= 2) {
-      const u64 t = __shfl_up(upto, d);
-      if (lane >= d) upto += t;
-    }
-    const u64 past = __ballot(run + upto > goal);
-    if (past) {
-      const int l = __ffsll((long long)past) - 1;
-      at = s0 + l;
-      run += __shfl(upto - m, l);
-      break;
-    }
-    run += __shfl(upto, 63);
-  }
-  u64 tie_before = ties[at];
-  for (int64_t f = 0; f < fold; ++f) {
-    const int64_t i = at * step + f * unit + lane * kSampleE;
-    float v[kSampleE];
-    u64 w[kSampleE], m = 0, t = 0;
-    if (i < V) sm_load<IT>(logits, i, V, v);
-#pragma unroll
-    for (int q = 0; q < kSampleE; ++q) t += i + q < V && sm_key(v[q]) == cut && kept(v[q], cut);
-    u64 upto = t;
-#pragma unroll
-    for (int d = 1; d < 64; d *= 2) {
-      const u64 a = __shfl_up(upto, d);
-      if (lane >= d) upto += a;
-    }
-    u64 before = tie_before + upto - t;
-    tie_before += __shfl(upto, 63);
-#pragma unroll
-    for (int q = 0; q < kSampleE; ++q) {
-      w[q] = 0;
-      if (i + q < V) {
-        const uint32_t key = sm_key(v[q]);
-        if (kept(v[q], key)) {
-          w[q] = key != cut || before < at_cut ? r.weight(v[q]) : 0;
-          before += key == cut;
-        }
-      }
-      m += w[q];
-    }
-    upto = m;
-#pragma unroll
-    for (int d = 1; d < 64; d *= 2) {
-      const u64 a = __shfl_up(upto, d);
-      if (lane >= d) upto += a;
-    }
-    const u64 past = __ballot(run + upto > goal);
-    if (past) {
-      if (lane == __ffsll((long long)past) - 1) {
-        u64 sum = run + upto - m;
-        int q = 0;
-        for (; q < kSampleE - 1 && sum + w[q] <= goal; ++q) sum += w[q];
-        p.token[row] = i + q;
-        p.logprob[row] = (float)(r.z(v[q]) - log((double)total / r.scale));
-      }
-      return;
-    }
-    run += __shfl(upto, 63);
-  }
+  int64_t tile;
+  u64 run, goal, total;
+  sm_tile(p, row, tiles, J * NT / 64, tile, run, goal, total);
+  if (wave != tile % (NT / 64)) return;   // the wavefront that holds it
+  float v[kE];
+  const int64_t i = tile_at((int)(tile / (NT / 64)), v);
+  sm_pick(p, r, row, kept, i, v, run, goal, total);
 }
 
+// ------------------------------------------------------------------ longer rows
+template <int NT> constexpr int sm_chunk() { return 4 * NT * kE; }   // logits a workgroup
+template <typename IT, int NT>
+struct SampleChunk {
+  float v[4][kE];
+  int64_t row, c, at;   // at: the lane's first index
+  __device__ __forceinline__ SampleChunk(const SampleParams &p, int64_t chunks) {
+    const int64_t b = p.first + blockIdx.x;
+    row = b / chunks;
+    c = b % chunks;
+    const IT *logits = (const IT *)p.logits + row * p.sl;
+    at = c * sm_chunk<NT>() + (threadIdx.x / 64) * kTile + (threadIdx.x % 64) * kE;
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+      if (index(j) < p.V) sm_load<IT>(logits, index(j), p.V, v[j]);
+  }
+  __device__ __forceinline__ int64_t index(int j) const { return at + (int64_t)j * (NT / 64) * kTile; }
+  template <typename F>
+  __device__ __forceinline__ void each(int64_t V, F f) const {
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+#pragma unroll
+      for (int q = 0; q < kE; ++q)
+        if (index(j) + q < V) f((uint32_t)(index(j) + q), v[j][q]);
+  }
+};
+__device__ __forceinline__ u64 sm_first(const SampleParams &p, int64_t row) {   // the row's, of its chunks'; for a whole wavefront
+  u64 best = 0;
+  for (int64_t c = threadIdx.x % 64; c < p.parts; c += 64) best = max(best, (u64)p.firsts[row * p.parts + c]);
+#pragma unroll
+  for (int d = 1; d < 64; d *= 2) best = max(best, (u64)__shfl_xor(best, d));
+  return best;
+}
+template <typename IT>
+__global__ void __launch_bounds__(256) k_sample_first(const SampleParams p) {
+  __shared__ u64 red[4];
+  const SampleChunk<IT, 256> x(p, p.parts);
+  u64 first = 0;
+  x.each(p.V, [&](uint32_t i, float l) {
+    const u64 at = sm_place(sm_key(l), i);
+    first = at > first ? at : first;
+  });
+  first = sm_block<256>(first, red, [](u64 a, u64 b) { return a > b ? a : b; });
+  if (threadIdx.x == 0) p.firsts[x.row * p.parts + x.c] = first;
+}
+template <typename IT, int NT>
+__global__ void __launch_bounds__(NT) k_sample_bins(const SampleParams p) {
+  __shared__ u64 mass[kBins];
+  __shared__ uint32_t count[kBins];
+  __shared__ double table[kTable];
+  const SampleChunk<IT, NT> x(p, p.chunks);
+  SampleRow r;
+  const SampleSettings s = sm_settings(p, x.row, r);
+  if (!sm_top(r, sm_first(p, x.row)) || s.k == 1 || (s.k == 0 && s.top_p >= 1)) return;   // the whole workgroup
+  sm_table<NT>(table, r);
+  for (int b = threadIdx.x; b < kBins; b += NT) mass[b] = count[b] = 0;
+  __syncthreads();
+  x.each(p.V, [&](uint32_t, float l) {
+    const int b = r.bin(l);
+    if (s.k > 1) atomicAdd(&count[b], 1u);
+    if (s.top_p < 1) atomicAdd(&mass[b], r.weight(l));
+  });
+  __syncthreads();
+  const int64_t at = (x.row * p.chunks + x.c) * kBins;
+  for (int b = threadIdx.x; b < kBins; b += NT) {
+    if (s.k > 1) p.counts[at + b] = count[b];
+    if (s.top_p < 1) p.masses[at + b] = mass[b];
+  }
+}
+template <typename IT, int NT>
+__global__ void __launch_bounds__(NT) k_sample_cut(const SampleParams p) {
+  __shared__ SampleLds<NT> m;
+  const int64_t row = p.first + blockIdx.x, V = p.V;
+  const IT *logits = (const IT *)p.logits + row * p.sl;
+  SampleRow r;
+  const SampleSettings s = sm_settings(p, row, r);
+  const u64 first = sm_first(p, row);
+  u64 cut = s.k == 1 ? first : 0;
+  if (sm_top(r, first) && s.k != 1 && (s.k > 1 || s.top_p < 1)) {
+    sm_table<NT>(m.table, r);
+    for (int b = threadIdx.x; b < kBins; b += NT) {
+      uint32_t n = 0;
+      u64 w = 0;
+      const int64_t at = row * p.chunks * kBins + b;
+      if (s.k > 1)
+#pragma unroll 4
+        for (int64_t c = 0; c < p.chunks; ++c) n += p.counts[at + c * kBins];
+      if (s.top_p < 1)
+#pragma unroll 4
+        for (int64_t c = 0; c < p.chunks; ++c) w += p.masses[at + c * kBins];
+      m.count[b] = n;
+      m.mass[b] = w;
+    }
+    __syncthreads();
+    auto each = [&](auto f) {
+      constexpr int64_t stride = NT * kE;
+      for (int64_t i0 = (int64_t)threadIdx.x * kE; i0 < V; i0 += 4 * stride) {   // four loads under way together
+        float v[4][kE];
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+          if (i0 + j * stride < V) sm_load<IT>(logits, i0 + j * stride, V, v[j]);
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+#pragma unroll
+          for (int q = 0; q < kE; ++q)
+            if (i0 + j * stride + q < V) f((uint32_t)(i0 + j * stride + q), v[j][q]);
+      }
+    };
+    cut = sm_select<NT>(m, r, s, each);
+  }
+  if (sm_top(r, first)) cut = sm_min_p(r, cut, first);
+  if (threadIdx.x == 0) p.cuts[row] = cut;
+}
+template <typename IT>
+__global__ void __launch_bounds__(256) k_sample_tiles(const SampleParams p) {
+  __shared__ double table[kTable];
+  const SampleChunk<IT, 256> x(p, p.parts);
+  SampleRow r;
+  sm_settings(p, x.row, r);
+  sm_table<256>(table, r);
+  const SampleCut cut(p.filtered ? p.cuts[x.row] : 0);
+  if (!sm_top(r, sm_first(p, x.row))) return;
+  __syncthreads();
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+    const int64_t i = x.index(j);
+    u64 sum = 0;
+#pragma unroll
+    for (int q = 0; q < kE; ++q) sum += i + q < p.V ? cut.weight(r, (uint32_t)(i + q), x.v[j][q]) : 0;
+#pragma unroll
+    for (int d = 1; d < 64; d *= 2) sum += __shfl_xor(sum, d);
+    if (threadIdx.x % 64 == 0 && i < p.V) p.tiles[x.row * p.ntiles + i / kTile] = sum;
+  }
+}
+template <typename IT>
+__global__ void __launch_bounds__(256) k_sample_token(const SampleParams p) {
+  __shared__ double table[kTable];
+  __shared__ u64 red[4], found[2];
+  const int64_t row = p.first + blockIdx.x;
+  const u64 *masses = (const u64 *)p.tiles + row * p.ntiles;
+  SampleRow r;
+  sm_settings(p, row, r);
+  sm_table<256>(table, r);
+  // consecutive tiles a thread
+  const int64_t per = (p.ntiles + 255) / 256, t0 = threadIdx.x * per, t1 = t0 + per < p.ntiles ? t0 + per : p.ntiles;
+  u64 mine = 0;
+  for (int64_t t = t0; t < t1; ++t) mine += masses[t];
+  const SampleCut cut(p.filtered ? p.cuts[row] : 0);
+  if (!sm_top(r, sm_first(p, row))) {
+    if (threadIdx.x == 0) {
+      p.token[row] = -1;
+      p.logprob[row] = NAN;
+    }
+    return;
+  }
+  u64 upto = sm_scan(mine);
+  if (threadIdx.x % 64 == 63) red[threadIdx.x / 64] = upto;
+  __syncthreads();
+  u64 total = 0;
+  for (int k = 0; k < 4; ++k) {
+    if (k == (int)threadIdx.x / 64) upto += total;
+    total += red[k];
+  }
+  const u64 goal = sm_goal(p, row, total);
+  if (upto > goal && upto - mine <= goal) {   // one thread
+    u64 run = upto - mine;
+    int64_t t = t0;
+    for (; t + 1 < t1 && run + masses[t] <= goal; ++t) run += masses[t];
+    found[0] = t;
+    found[1] = run;
+  }
+  __syncthreads();
+  if (threadIdx.x >= 64) return;
+  const int64_t i = found[0] * kTile + threadIdx.x * kE;
+  float v[kE] = {};
+  if (i < p.V) sm_load<IT>((const IT *)p.logits + row * p.sl, i, p.V, v);
+  sm_pick(p, r, row, cut, i, v, found[1], goal, total);
+}
+
+template <typename IT, int NT>
+static void sample_long(SampleParams p, hipStream_t s) {
+  auto launch = [&](auto kernel, int64_t all, int threads) {
+    const int64_t most = kGridThreads / threads;
+    for (p.first = 0; p.first < all; p.first += most)
+      hipLaunchKernelGGL(kernel, dim3((unsigned)(all - p.first < most ? all - p.first : most)), dim3(threads), 0, s, p);
+  };
+  launch(k_sample_first<IT>, p.R * p.parts, 256);
+  if (p.filtered) {
+    launch(k_sample_bins<IT, NT>, p.R * p.chunks, NT);
+    launch(k_sample_cut<IT, 1024>, p.R, 1024);
+  }
+  launch(k_sample_tiles<IT>, p.R * p.parts, 256);
+  launch(k_sample_token<IT>, p.R, 256);
+}
 template <typename IT>
 static hipError_t sample_t(SampleParams p, hipStream_t s) {
+  if (p.chunks) {
+    if (p.chunk == sm_chunk<256>()) sample_long<IT, 256>(p, s);
+    else sample_long<IT, 1024>(p, s);
+    return hipGetLastError();
+  }
   const int64_t most = kGridThreads / 1024;
   for (; p.first < p.R; p.first += most) {
     const dim3 grid((unsigned)(p.R - p.first < most ? p.R - p.first : most));
-    if (p.V <= 4096) hipLaunchKernelGGL((k_sample<IT, 256>), grid, dim3(256), 0, s, p);
-    else hipLaunchKernelGGL((k_sample<IT, 1024>), grid, dim3(1024), 0, s, p);
+    if (p.V <= 2048) hipLaunchKernelGGL((k_sample_row<IT, 256, 1>), grid, dim3(256), 0, s, p);
+    else if (p.V <= 8192) hipLaunchKernelGGL((k_sample_row<IT, 1024, 1>), grid, dim3(1024), 0, s, p);
+    else hipLaunchKernelGGL((k_sample_row<IT, 1024, 4>), grid, dim3(1024), 0, s, p);
   }
   return hipGetLastError();
 }

@@ -192,3 +192,38 @@ def test_refusals_and_no_rows(dev):
         ssm_scan.sample(logits, u, top_p=torch.ones(4))
     t, p = ssm_scan.sample(logits[:0], u[:0])
     assert t.shape == p.shape == (0,)
+
+
+@pytest.mark.parametrize("B,V", [(70, 33000), (5, 70001)])   # workgroups of large and of small chunks
+def test_settings_per_row_of_long_rows(dev, B, V):
+    logits, u = make(dev, B, V, BF16, seed=12)
+    r = torch.Generator().manual_seed(13)
+
+    def choose(values, dtype=F32):
+        return torch.tensor(values, dtype=dtype)[torch.randint(len(values), (B,), generator=r)].to(dev)
+
+    check(logits, u, temperature=choose([0.0, 0.1, 0.6, 1.0, 2.0]), top_k=choose([0, 1, 7, 300, 5000, 32000], torch.int64),
+          top_p=choose([1.0, 0.9, 0.4, 0.999]), min_p=choose([0.0, 0.05]))
+    for kw in (dict(temperature=choose([0.0, 0.7])), dict(top_k=choose([0, 1, 50], torch.int64)), dict(top_p=choose([1.0, 0.8])),
+               dict(min_p=choose([0.0, 0.1])), dict(temperature=0.0)):
+        check(logits, u, **kw)
+    logits[1] = -math.inf
+    logits[2, 5] = float("nan")
+    logits[3] = 0.0      # a bin of the whole row
+    logits[4, 100:20000] = 1.0
+    check(logits, u)
+    check(logits, u, top_k=10000, top_p=0.8)
+    check(logits, u, top_p=0.7)
+
+
+@pytest.mark.parametrize("V", [2000, 9000, 40000])
+def test_crowded_bins(dev, V):
+    """More logits in one bin of the histogram than are ranked at once, distinct and tied."""
+    g = torch.Generator().manual_seed(14)
+    logits = (1e-4 * torch.rand(6, V, generator=g)).to(dev)
+    logits[2] = torch.round(logits[2] * 3e4) / 3e4
+    logits[3:] -= 50.0
+    logits[3:, 17] = 0.0
+    u = torch.rand(6, generator=g).to(dev)
+    for kw in (dict(top_k=V // 2 + 3), dict(top_p=0.6), dict(top_k=V - 100, top_p=0.5), dict(top_k=1200), dict(top_k=V // 2, temperature=1e3)):
+        check(logits, u, **kw)
