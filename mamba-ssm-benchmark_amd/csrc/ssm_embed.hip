@@ -70,25 +70,29 @@ __global__ void __launch_bounds__(256) k_embed_place(const EmbedParams p) {
   __shared__ uint32_t sums[256];
   const int lane = threadIdx.x % 64, w = threadIdx.x / 64, B = 1 << p.bits;
   const int64_t wave0 = (int64_t)blockIdx.x * 4;
-  // items of the digits below, then of this digit in the wavefronts before
-  constexpr int per = (1 << kEmbedBits) / 256;
-  uint32_t total[per], run = 0;
+  // items of the digits below, then of this digit in the wavefronts before: two digits a thread
+  constexpr int per = 2;
+  static_assert(per * 256 == 1 << kEmbedBits, "digits");
+  uint32_t total[per] = {}, run = 0, mine[per][4] = {};
+  if ((int)threadIdx.x * per < B) {
+    const uint2 *h = (const uint2 *)p.hist + threadIdx.x;
+#pragma unroll 32
+    for (int v = 0; v < (int)p.nw; ++v) {
+      const uint2 c = h[(int64_t)v * (B / 2)];
+      total[0] += c.x;
+      total[1] += c.y;
+#pragma unroll
+      for (int q = 0; q < 4; ++q) {
+        mine[0][q] += v < wave0 + q ? c.x : 0;
+        mine[1][q] += v < wave0 + q ? c.y : 0;
+      }
+    }
+  }
 #pragma unroll
   for (int k = 0; k < per; ++k) {
-    const int b = threadIdx.x * per + k;
-    uint32_t all = 0, mine[4] = {0, 0, 0, 0};
-    if (b < B)
-#pragma unroll 8
-      for (int64_t v = 0; v < p.nw; ++v) {
-        const uint32_t c = p.hist[v * B + b];
-        all += c;
+    run += total[k];
 #pragma unroll
-        for (int q = 0; q < 4; ++q) mine[q] += v < wave0 + q ? c : 0;
-      }
-    total[k] = all;
-    run += all;
-#pragma unroll
-    for (int q = 0; q < 4; ++q) base[q][b] = mine[q];
+    for (int q = 0; q < 4; ++q) base[q][threadIdx.x * per + k] = mine[k][q];
   }
   sums[threadIdx.x] = run;
   __syncthreads();
@@ -107,47 +111,70 @@ __global__ void __launch_bounds__(256) k_embed_place(const EmbedParams p) {
   }
   __syncthreads();
   const int64_t wave = wave0 + w, end = (wave + 1) * p.per < p.n ? (wave + 1) * p.per : p.n;
-  for (int64_t i0 = wave * p.per; i0 < end; i0 += 64) {   // no barrier in here: wavefronts may differ in their steps
-    const int64_t i = i0 + lane;
-    const bool there = i < end;
-    const uint32_t key = there ? em_key(p, i) : 0, pos = there ? (p.pass ? p.pos_in[i] : (uint32_t)i) : 0;
-    const uint32_t digit = (key >> p.shift) & (B - 1);
-    uint64_t same = __ballot(there);
-    for (int b = 0; b < p.bits; ++b) {
-      const uint64_t set = __ballot((digit >> b) & 1);
-      same &= (digit >> b) & 1 ? set : ~set;
+  constexpr int U = 4;   // steps whose items are loaded together
+  for (int64_t i0 = wave * p.per; i0 < end; i0 += 64 * U) {   // no barrier in here: wavefronts may differ in their steps
+    uint32_t keys[U], places[U];
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const int64_t i = i0 + 64 * u + lane;
+      keys[u] = i < end ? em_key(p, i) : 0;
+      places[u] = i < end ? (p.pass ? p.pos_in[i] : (uint32_t)i) : 0;
     }
-    const int before = __popcll(same & ((1ull << lane) - 1));
-    uint32_t at = 0;
-    if (there) at = base[w][digit] + before;
-    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-    __builtin_amdgcn_wave_barrier();
-    if (there && before == 0) base[w][digit] += __popcll(same);
-    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-    __builtin_amdgcn_wave_barrier();
-    if (there) {
-      p.key_out[at] = key;
-      p.pos_out[at] = pos;
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const bool there = i0 + 64 * u + lane < end;
+      const uint32_t digit = (keys[u] >> p.shift) & (B - 1);
+      uint64_t same = __ballot(there);
+      for (int b = 0; b < p.bits; ++b) {
+        const uint64_t set = __ballot((digit >> b) & 1);
+        same &= (digit >> b) & 1 ? set : ~set;
+      }
+      const int before = __popcll(same & ((1ull << lane) - 1));
+      uint32_t at = 0;
+      if (there) at = base[w][digit] + before;
+      __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+      __builtin_amdgcn_wave_barrier();
+      if (there && before == 0) base[w][digit] += __popcll(same);
+      __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+      __builtin_amdgcn_wave_barrier();
+      if (there) {
+        p.key_out[at] = keys[u];
+        p.pos_out[at] = places[u];
+      }
     }
   }
 }
 
 // ------------------------------------------------------------------ sums
-// Sum of dout's rows at sorted places [from, to), columns j .. j + V, in order; 8 rows are read together.
+// Sum of dout's rows at sorted places [from, to), columns j .. j + V, in order; up to 16 rows are read together.
+template <int U, typename IT, int V>
+__device__ __forceinline__ void em_some(const EmbedParams &p, int64_t from, int64_t j, float (&acc)[V]) {
+  struct alignas(V * sizeof(IT)) Pack { IT e[V]; };
+  Pack e[U];
+#pragma unroll
+  for (int u = 0; u < U; ++u) e[u] = *(const Pack *)((const IT *)p.dout + (int64_t)p.pos_in[from + u] * p.sd + j);
+#pragma unroll
+  for (int u = 0; u < U; ++u)
+#pragma unroll
+    for (int i = 0; i < V; ++i) acc[i] += to_f32(e[u].e[i]);
+}
 template <typename IT, int V>
 __device__ __forceinline__ void em_rows(const EmbedParams &p, int64_t from, int64_t to, int64_t j, float (&acc)[V]) {
-  for (int64_t k = from; k < to; k += 8) {
-    float e[8][V];
-#pragma unroll
-    for (int u = 0; u < 8; ++u) {
-      const int64_t at = k + u < to ? k + u : to - 1;
-      em_load<IT, V>((const IT *)p.dout + (int64_t)p.pos_in[at] * p.sd + j, e[u]);
-    }
-#pragma unroll
-    for (int u = 0; u < 8; ++u)
-#pragma unroll
-      for (int i = 0; i < V; ++i) acc[i] += k + u < to ? e[u][i] : 0.0f;
+  int64_t k = from;
+  for (; k + 16 <= to; k += 16) em_some<16, IT, V>(p, k, j, acc);
+  if (k + 8 <= to) {
+    em_some<8, IT, V>(p, k, j, acc);
+    k += 8;
   }
+  if (k + 4 <= to) {
+    em_some<4, IT, V>(p, k, j, acc);
+    k += 4;
+  }
+  if (k + 2 <= to) {
+    em_some<2, IT, V>(p, k, j, acc);
+    k += 2;
+  }
+  if (k < to) em_some<1, IT, V>(p, k, j, acc);
 }
 template <int V>
 __device__ __forceinline__ void em_parts(const float *src, int64_t from, int64_t to, int64_t D, int64_t j, float (&acc)[V]) {
@@ -166,15 +193,22 @@ __device__ __forceinline__ void em_parts(const float *src, int64_t from, int64_t
 template <typename IT, int V>
 __global__ void __launch_bounds__(256) k_embed_pieces(const EmbedParams p) {
   if ((int64_t)blockIdx.x >= p.npiece_blocks) {
-    const int64_t v = ((int64_t)blockIdx.x - p.npiece_blocks) * 256 + threadIdx.x;
-    if (v > p.V) return;
-    int64_t lo = 0, hi = p.n;   // the first place whose key is not below v
-    while (lo < hi) {
-      const int64_t mid = (lo + hi) >> 1;
-      if (p.key_in[mid] < (uint32_t)v) lo = mid + 1;
-      else hi = mid;
+    // place i is the first of the tokens above its forerunner's up to its own: mostly few, else the wavefront's work
+    const int64_t i = ((int64_t)blockIdx.x - p.npiece_blocks) * 256 + threadIdx.x;
+    int64_t v0 = 0, v1 = -1;
+    if (i <= p.n) {
+      v0 = i ? (int64_t)p.key_in[i - 1] + 1 : 0;
+      v1 = i < p.n ? (int64_t)p.key_in[i] : p.V;
     }
-    p.start[v] = (uint32_t)lo;
+    uint64_t wide = __ballot(v1 - v0 >= 16);
+    if (v1 - v0 < 16)
+      for (int64_t v = v0; v <= v1; ++v) p.start[v] = (uint32_t)i;
+    while (wide) {
+      const int l = __ffsll((unsigned long long)wide) - 1;
+      wide &= wide - 1;
+      const int64_t w1 = __shfl(v1, l), at = __shfl(i, l);
+      for (int64_t v = __shfl(v0, l) + threadIdx.x % 64; v <= w1; v += 64) p.start[v] = (uint32_t)at;
+    }
     return;
   }
   const int l = threadIdx.x & (p.lanes - 1);
@@ -203,34 +237,50 @@ __global__ void __launch_bounds__(256) k_embed_groups(const EmbedParams p) {
     em_store<float, V>(p.group + group * p.D + j, acc);
   }
 }
-// Every row of dw: the places of its token, with whole pieces (and groups of them) in their sums' place.
+// Every row of dw: those of the tokens that come, by the first of their places (a lane group looks at each), with
+// whole pieces (and groups of them) in their sums' place; zeros by the first workgroups, which wait for nothing.
 template <typename IT, int V>
 __global__ void __launch_bounds__(256) k_embed_rows(const EmbedParams p) {
-  const int l = threadIdx.x & (p.lanes - 1);
-  const int64_t v = p.first + (int64_t)blockIdx.x * (256 / p.lanes) + threadIdx.x / p.lanes;
-  if (v >= p.V) return;
-  const int64_t s = p.start[v], e = p.start[v + 1];
   constexpr int64_t P = kEmbedPiece, G = kEmbedGroup;
-  int64_t p0 = (s + P - 1) / P, p1 = e / P;         // whole pieces
-  if (p0 >= p1) p0 = p1 = -1;
-  int64_t g0 = (p0 + G - 1) / G, g1 = p1 / G;       // whole groups
-  if (!p.group || p0 < 0 || g0 >= g1) g0 = g1 = -1;
-  for (int64_t j = (int64_t)l * V; j < p.D; j += (int64_t)p.lanes * V) {
-    float acc[V] = {};
-    if (p0 < 0) {
-      em_rows<IT, V>(p, s, e, j, acc);
-    } else {
-      em_rows<IT, V>(p, s, p0 * P, j, acc);
-      em_parts<V>(p.piece, p0, g0 < 0 ? p1 : g0 * G, p.D, j, acc);
-      if (g0 >= 0) {
-        em_parts<V>(p.group, g0, g1, p.D, j, acc);
-        em_parts<V>(p.piece, g1 * G, p1, p.D, j, acc);
+  const int l = threadIdx.x & (p.lanes - 1), group = threadIdx.x / p.lanes, groups = 256 / p.lanes;
+  if ((int64_t)blockIdx.x < p.nzero_blocks) {
+    const int64_t v0 = (int64_t)blockIdx.x * kEmbedRows;
+    __shared__ uint32_t start[kEmbedRows + 1];
+    for (int i = threadIdx.x; i <= kEmbedRows && v0 + i <= p.V; i += 256) start[i] = p.start[v0 + i];
+    __syncthreads();
+    const float zero[V] = {};
+    for (int i = group; i < kEmbedRows && v0 + i < p.V; i += groups)
+      if (start[i] == start[i + 1])
+        for (int64_t j = (int64_t)l * V; j < p.D; j += (int64_t)p.lanes * V) em_store<IT, V>((IT *)p.dw + (v0 + i) * p.D + j, zero);
+    return;
+  }
+  const int64_t i = ((int64_t)blockIdx.x - p.nzero_blocks) * groups + group;
+  if (i >= p.n) return;
+  {
+    const uint32_t v = p.key_in[i], last = i ? p.key_in[i - 1] : v + 1;
+    if (v >= (uint32_t)p.V || last == v) return;
+    const int64_t s = i, e = p.start[v + 1];
+    int64_t p0 = (s + P - 1) / P, p1 = e / P;         // whole pieces
+    if (p0 >= p1) p0 = p1 = -1;
+    int64_t g0 = (p0 + G - 1) / G, g1 = p1 / G;       // whole groups
+    if (!p.group || p0 < 0 || g0 >= g1) g0 = g1 = -1;
+    for (int64_t j = (int64_t)l * V; j < p.D; j += (int64_t)p.lanes * V) {
+      float acc[V] = {};
+      if (p0 < 0) {
+        em_rows<IT, V>(p, s, e, j, acc);
+      } else {
+        em_rows<IT, V>(p, s, p0 * P, j, acc);
+        em_parts<V>(p.piece, p0, g0 < 0 ? p1 : g0 * G, p.D, j, acc);
+        if (g0 >= 0) {
+          em_parts<V>(p.group, g0, g1, p.D, j, acc);
+          em_parts<V>(p.piece, g1 * G, p1, p.D, j, acc);
+        }
+        em_rows<IT, V>(p, p1 * P, e, j, acc);
       }
-      em_rows<IT, V>(p, p1 * P, e, j, acc);
-    }
 #pragma unroll
-    for (int i = 0; i < V; ++i) acc[i] *= p.scale;
-    em_store<IT, V>((IT *)p.dw + v * p.D + j, acc);
+      for (int k = 0; k < V; ++k) acc[k] *= p.scale;
+      em_store<IT, V>((IT *)p.dw + (int64_t)v * p.D + j, acc);
+    }
   }
 }
 
@@ -260,10 +310,10 @@ static hipError_t embed_v(EmbedParams p, bool bwd, hipStream_t s) {
   }
   const int64_t pieces = p.n / kEmbedPiece;
   p.npiece_blocks = (pieces + Q - 1) / Q;
-  hipLaunchKernelGGL((k_embed_pieces<IT, V>), dim3((unsigned)(p.npiece_blocks + (p.V + 256) / 256)), dim3(256), 0, s, p);
+  hipLaunchKernelGGL((k_embed_pieces<IT, V>), dim3((unsigned)(p.npiece_blocks + (p.n + 256) / 256)), dim3(256), 0, s, p);
   if (p.group) hipLaunchKernelGGL((k_embed_groups<V>), blocks(pieces / kEmbedGroup), dim3(256), 0, s, p);
-  for (; p.first < p.V; p.first += most)
-    hipLaunchKernelGGL((k_embed_rows<IT, V>), blocks(p.V - p.first < most ? p.V - p.first : most), dim3(256), 0, s, p);
+  p.nzero_blocks = (p.V + kEmbedRows - 1) / kEmbedRows;
+  hipLaunchKernelGGL((k_embed_rows<IT, V>), dim3((unsigned)(p.nzero_blocks + (p.n + Q - 1) / Q)), dim3(256), 0, s, p);
   return hipGetLastError();
 }
 template <typename IT>

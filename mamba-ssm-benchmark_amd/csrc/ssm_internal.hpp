@@ -390,8 +390,9 @@ hipError_t launch_rnorm(const RnormParams &p, int dtype, int rdtype, bool bwd, h
 
 // Token embedding and its gradient.
 constexpr int kEmbedBits = 9;          // of a sorting pass
-constexpr int64_t kEmbedWaves = 128;   // wavefronts that sort, at most
-constexpr int kEmbedPiece = 64;        // sorted places that are summed at once where they hold one token
+constexpr int64_t kEmbedWaves = 64;   // wavefronts that sort, at most
+constexpr int kEmbedRows = 32;         // rows of the gradient that a workgroup looks at for zeros
+constexpr int kEmbedPiece = 32;        // sorted places that are summed at once where they hold one token
 constexpr int kEmbedGroup = 32;        // pieces likewise
 struct EmbedParams {
   int64_t n, V, D;
@@ -411,7 +412,7 @@ struct EmbedParams {
   uint32_t *key[2], *pos[2];           // (n,) each: the passes' outputs in turn
   uint32_t *start;                     // (V + 1)
   float *piece, *group;                // sums of whole pieces, of whole groups (null: not formed)
-  int64_t npiece_blocks;
+  int64_t npiece_blocks, nzero_blocks;
 };
 hipError_t launch_embed(const EmbedParams &p, int dtype, bool bwd, hipStream_t s);
 

@@ -150,14 +150,14 @@ __device__ __forceinline__ void sm_table(double *table, SampleRow &r) {   // bef
   r.table = table;
 }
 
-// The first of kBins bins at which the running sum reaches `target` (1 .. the whole), into m.bin, and the sum before
-// it, into m.above.
-template <int NT, typename C>
-__device__ __forceinline__ void sm_find(SampleLds<NT> &m, const C *bins, u64 target) {
+// The first of kBins bins of the counts, or of the masses, at which the running sum reaches `target` (1 .. the whole),
+// into m.bin, and the sum before it, into m.above.
+template <int NT>
+__device__ __forceinline__ void sm_find(SampleLds<NT> &m, int by_mass, u64 target) {
   constexpr int per = kBins / NT;
   u64 v[per], mine = 0;
 #pragma unroll
-  for (int k = 0; k < per; ++k) mine += v[k] = bins[threadIdx.x * per + k];
+  for (int k = 0; k < per; ++k) mine += v[k] = by_mass ? m.mass[threadIdx.x * per + k] : m.count[threadIdx.x * per + k];
   u64 upto = sm_scan(mine);
   __syncthreads();
   if (threadIdx.x % 64 == 63) m.red[threadIdx.x / 64] = upto;
@@ -210,47 +210,60 @@ __device__ __forceinline__ int sm_gather(SampleLds<NT> &m, const SampleRow &r, E
   __syncthreads();
   return m.n;
 }
+// The n gathered elements in falling order, by a bitonic network.
+template <int NT>
+__device__ __forceinline__ void sm_sort(u64 *place, int n) {
+  int P = 64;
+  while (P < n) P *= 2;
+  for (int c = n + threadIdx.x; c < P; c += NT) place[c] = 0;   // below any element's
+  __syncthreads();
+  for (int k = 2; k <= P; k *= 2)
+    for (int d = k / 2; d; d /= 2) {
+      for (int e = threadIdx.x; e < P / 2; e += NT) {
+        const int x = 2 * e - (e & (d - 1)), y = x + d;
+        const u64 u = place[x], v = place[y];
+        if ((u < v) == !(x & k)) {
+          place[x] = v;
+          place[y] = u;
+        }
+      }
+      // pairs 64 threads apart and less are the wavefront's own
+      if (d > 64 || (d == 1 && k >= 64)) __syncthreads();
+      else wave_lds_sync();
+    }
+  __syncthreads();
+}
+// Of sorted elements the one at which the running sum of value(l, place) reaches `target` (1 .. the whole).
+template <int NT, typename M, typename Value>
+__device__ __forceinline__ u64 sm_reach(M &m, int n, u64 target, Value value) {
+  u64 sum = 0;   // of the elements before this turn's
+  for (int c0 = 0; c0 < n; c0 += NT) {
+    const int c = c0 + threadIdx.x;
+    const u64 at = c < n ? m.place[c] : 0, own = c < n ? value(sm_value((uint32_t)(at >> 32)), at) : 0;
+    u64 upto = sm_scan(own);
+    if (threadIdx.x % 64 == 63) m.red[threadIdx.x / 64] = upto;
+    __syncthreads();
+    u64 all = 0;
+    for (int k = 0; k < NT / 64; ++k) {
+      if (k == (int)threadIdx.x / 64) upto += all;
+      all += m.red[k];
+    }
+    upto += sum;
+    if (upto - own < target && upto >= target) m.cut = at;
+    sum += all;
+    __syncthreads();
+  }
+  return m.cut;
+}
 // Of the elements of a range of logits the one at which the running sum of value(l, place), by falling place, reaches
 // `target` (1 .. the whole), as its place.  n: how many there are, of which up to kCandidates have been gathered; ones:
 // every value is one.
 template <int NT, typename Each, typename Value>
 __device__ __forceinline__ u64 sm_cut(SampleLds<NT> &m, Each each, float lo, float hi, int n, u64 target, bool ones, Value value) {
   if (n <= kCandidates) {
-    int P = 64;
-    while (P < n) P *= 2;
-    for (int c = n + threadIdx.x; c < P; c += NT) m.place[c] = 0;   // below any element's
-    __syncthreads();
-    for (int k = 2; k <= P; k *= 2)   // falling order, by a bitonic network
-      for (int d = k / 2; d; d /= 2) {
-        for (int e = threadIdx.x; e < P / 2; e += NT) {
-          const int x = 2 * e - (e & (d - 1)), y = x + d;
-          const u64 u = m.place[x], v = m.place[y];
-          if ((u < v) == !(x & k)) {
-            m.place[x] = v;
-            m.place[y] = u;
-          }
-        }
-        __syncthreads();
-      }
+    sm_sort<NT>(m.place, n);
     if (ones) return m.place[target - 1];
-    u64 sum = 0;   // of the elements before this turn's
-    for (int c0 = 0; c0 < n; c0 += NT) {
-      const int c = c0 + threadIdx.x;
-      const u64 at = c < n ? m.place[c] : 0, own = c < n ? value(sm_value((uint32_t)(at >> 32)), at) : 0;
-      u64 upto = sm_scan(own);
-      if (threadIdx.x % 64 == 63) m.red[threadIdx.x / 64] = upto;
-      __syncthreads();
-      u64 all = 0;
-      for (int k = 0; k < NT / 64; ++k) {
-        if (k == (int)threadIdx.x / 64) upto += all;
-        all += m.red[k];
-      }
-      upto += sum;
-      if (upto - own < target && upto >= target) m.cut = at;
-      sum += all;
-      __syncthreads();
-    }
-    return m.cut;
+    return sm_reach<NT>(m, n, target, value);
   }
   u64 prefix = 0, sum = 0;
   for (int shift = 53; shift > -11; shift -= 11) {   // digits of 11 bits, the last of 9
@@ -264,7 +277,7 @@ __device__ __forceinline__ u64 sm_cut(SampleLds<NT> &m, Each each, float lo, flo
       atomicAdd(&m.mass[(1 << bits) - 1 - (int)(at >> s & ((1 << bits) - 1))], value(l, at));   // falling
     });
     __syncthreads();
-    sm_find<NT>(m, m.mass, target - sum);
+    sm_find<NT>(m, 1, target - sum);
     prefix |= (u64)((1 << bits) - 1 - m.bin) << s;
     sum += m.above;
     __syncthreads();
@@ -272,61 +285,63 @@ __device__ __forceinline__ u64 sm_cut(SampleLds<NT> &m, Each each, float lo, flo
   return prefix;
 }
 
+// The sum that the last place kept by top_p is the first to reach.
+__device__ __forceinline__ u64 sm_target(const SampleSettings &s, u64 mass) {
+  const u64 target = s.top_p > 0 ? (u64)ceil(s.top_p * (double)mass) : 1;
+  return target < 1 ? 1 : target > mass ? mass : target;
+}
 // The cut of a row whose histograms are in m (of counts if k, of weights if top_p): the place of the last kept element,
-// min_p aside.
+// min_p aside.  One after the other top_k's cut by counts and top_p's by what that leaves of the weights, in one loop: the
+// code of a walk is long, and a kernel of one workgroup a row waits for every line of it.
 template <int NT, typename Each>
 __device__ __forceinline__ u64 sm_select(SampleLds<NT> &m, const SampleRow &r, const SampleSettings &s, Each each) {
   auto add = [](u64 a, u64 b) { return a + b; };
-  u64 cut = 0, mass = 0;
+  u64 cut = 0, target = (u64)s.k;
   int have = -1, n = 0;   // the bin whose elements are gathered
-  float lo, hi;
-  if (s.k > 1) {
-    sm_find<NT>(m, m.count, (u64)s.k);
-    have = m.bin;
-    const u64 rest = (u64)s.k - m.above;
-    sm_range(r, have, lo, hi);
-    n = sm_gather<NT>(m, r, each, lo, hi);
+  float lo = 0, hi = 0;
+#pragma unroll 1
+  for (int by_mass = s.k > 1 ? 0 : 1; by_mass < (s.top_p < 1 ? 2 : 1); ++by_mass) {
+    if (by_mass) {
+      u64 mass = 0;
+#pragma unroll 1
+      for (int b = threadIdx.x; b < kBins; b += NT) mass += m.mass[b];
+      target = sm_target(s, sm_block<NT>(mass, m.red, add));
+      __syncthreads();
+    }
+    sm_find<NT>(m, by_mass, target);
+    const int bin = m.bin;
+    const u64 rest = target - m.above, kcut = cut;
+    __syncthreads();
+    if (bin != have) {
+      sm_range(r, bin, lo, hi);
+      n = sm_gather<NT>(m, r, each, lo, hi);
+      have = bin;
+    }
     u64 save[kBins / NT];   // cutting by digits takes the histogram's place
 #pragma unroll
     for (int b = 0; b < kBins / NT; ++b) save[b] = m.mass[b * NT + threadIdx.x];
     __syncthreads();
-    cut = sm_cut<NT>(m, each, lo, hi, n, rest, true, [](float, u64) { return (u64)1; });
+    cut = sm_cut<NT>(m, each, lo, hi, n, rest, !by_mass, [&](float l, u64 at) { return !by_mass ? 1 : at >= kcut ? r.weight(l) : (u64)0; });
     __syncthreads();
-    if (s.top_p < 1) {   // what top_k has left of the weights
-      u64 kept = 0;
-      if (n <= kCandidates) {
-        for (int c = threadIdx.x; c < n; c += NT) kept += m.place[c] >= cut ? r.weight(sm_value((uint32_t)(m.place[c] >> 32))) : 0;
-      } else {
-        each([&](uint32_t i, float l) {
-          if (l >= lo && l <= hi && sm_place(sm_key(l), i) >= cut) kept += r.weight(l);
-        });
-      }
-      kept = sm_block<NT>(kept, m.red, add);
-#pragma unroll
-      for (int b = 0; b < kBins / NT; ++b) {
-        const int at = b * NT + threadIdx.x;
-        m.mass[at] = save[b] = at < have ? save[b] : at == have ? kept : 0;
-        mass += save[b];
-      }
+    if (by_mass || !(s.top_p < 1)) continue;
+    u64 kept = 0;   // what top_k has left of the weights
+    if (n <= kCandidates) {
+#pragma unroll 1
+      for (int c = threadIdx.x; c < n; c += NT) kept += m.place[c] >= cut ? r.weight(sm_value((uint32_t)(m.place[c] >> 32))) : 0;
+    } else {
+      each([&](uint32_t i, float l) {
+        if (l >= lo && l <= hi && sm_place(sm_key(l), i) >= cut) kept += r.weight(l);
+      });
     }
-  } else {
-    for (int b = threadIdx.x; b < kBins; b += NT) mass += m.mass[b];
+    kept = sm_block<NT>(kept, m.red, add);
+#pragma unroll
+    for (int b = 0; b < kBins / NT; ++b) {
+      const int at = b * NT + threadIdx.x;
+      m.mass[at] = at < have ? save[b] : at == have ? kept : 0;
+    }
+    __syncthreads();
   }
-  if (!(s.top_p < 1)) return cut;
-  mass = sm_block<NT>(mass, m.red, add);
-  const double want = s.top_p > 0 ? ceil(s.top_p * (double)mass) : 1.0;   // the first place at which the sum reaches it is the last one kept
-  u64 target = (u64)want;
-  target = target < 1 ? 1 : target > mass ? mass : target;
-  __syncthreads();
-  sm_find<NT>(m, m.mass, target);
-  const int b = m.bin;
-  const u64 rest = target - m.above, kcut = cut;
-  __syncthreads();
-  if (b != have) {
-    sm_range(r, b, lo, hi);
-    n = sm_gather<NT>(m, r, each, lo, hi);
-  }
-  return sm_cut<NT>(m, each, lo, hi, n, rest, false, [&](float l, u64 at) { return at >= kcut ? r.weight(l) : (u64)0; });
+  return cut;
 }
 
 // The cut with min_p: the smallest key that it keeps, at any index.
@@ -377,6 +392,9 @@ __device__ __forceinline__ void sm_tile(const SampleParams &p, int64_t row, cons
   }
   tile = tiles - 1;   // not reached: the sums end at the total
 }
+__device__ __forceinline__ float sm_logprob(const SampleRow &r, float l, u64 total) {
+  return (float)(r.z(l) - (log((double)total) - r.shift * 0.6931471805599453));
+}
 // One wavefront: the token, in the tile whose logits its lanes hold.
 __device__ __forceinline__ void sm_pick(const SampleParams &p, const SampleRow &r, int64_t row, const SampleCut &cut, int64_t i, const float (&v)[kE],
                                         u64 run, u64 goal, u64 total) {
@@ -397,7 +415,95 @@ __device__ __forceinline__ void sm_pick(const SampleParams &p, const SampleRow &
     }
   }
   p.token[row] = i + at;
-  p.logprob[row] = (float)(r.z(l) - (log((double)total) - r.shift * 0.6931471805599453));
+  p.logprob[row] = sm_logprob(r, l, total);
+}
+
+// ------------------------------------------------------------------ short rows
+// Up to kShort logits: the whole row is sorted, and nothing is unrolled (see sm_select).
+constexpr int kShort = 1024;
+template <typename IT>
+__global__ void __launch_bounds__(256) k_sample_short(const SampleParams p) {
+  constexpr int NT = 256, per = kShort / NT;
+  __shared__ struct {
+    u64 place[kShort], weight[kShort], red[NT / 64], cut;
+    double table[kTable];
+  } m;
+  const int64_t row = p.first + blockIdx.x;
+  const IT *logits = (const IT *)p.logits + row * p.sl;
+  const int V = (int)p.V, t = threadIdx.x;
+  u64 first = 0;
+#pragma unroll 1
+  for (int c = t; c < V; c += NT) {
+    const u64 at = sm_place(sm_key(to_f32(logits[c])), c);
+    m.place[c] = at;
+    first = at > first ? at : first;
+  }
+  SampleRow r;
+  const SampleSettings s = sm_settings(p, row, r);
+  sm_table<NT>(m.table, r);
+  first = sm_block<NT>(first, m.red, [](u64 a, u64 b) { return a > b ? a : b; });
+  const bool there = sm_top(r, first);
+  if (!there || s.k == 1) {
+    if (t == 0) {
+      p.token[row] = there ? (int64_t)(uint32_t)~first : -1;
+      p.logprob[row] = there ? 0.0f : NAN;
+    }
+    return;
+  }
+  __syncthreads();
+#pragma unroll 1
+  for (int c = t; c < kShort; c += NT) m.weight[c] = c < V ? r.weight(sm_value((uint32_t)(m.place[c] >> 32))) : 0;
+  __syncthreads();
+  u64 w[per];   // of consecutive logits
+#pragma unroll
+  for (int q = 0; q < per; ++q) w[q] = m.weight[t * per + q];
+  u64 cut = 0;
+  if (s.k > 1 || s.top_p < 1 || r.lowest > -INFINITY) {
+    u64 at[per];
+#pragma unroll
+    for (int q = 0; q < per; ++q) at[q] = t * per + q < V ? m.place[t * per + q] : 0;
+    __syncthreads();
+    if (s.k > 1 || s.top_p < 1) {
+      sm_sort<NT>(m.place, V);
+      const int n = s.k > 1 ? (int)s.k : V;
+      cut = m.place[n - 1];
+      if (s.top_p < 1) {
+        u64 mass = 0;
+#pragma unroll
+        for (int q = 0; q < per; ++q) mass += at[q] >= cut ? w[q] : 0;
+        mass = sm_block<NT>(mass, m.red, [](u64 a, u64 b) { return a + b; });
+        __syncthreads();
+        cut = sm_reach<NT>(m, n, sm_target(s, mass), [&](float, u64 at) { return m.weight[(uint32_t)~at]; });
+      }
+    }
+#pragma unroll
+    for (int q = 0; q < per; ++q) {   // without branches: with them the compiler loses the zeros
+      const double z = r.z(sm_value((uint32_t)(at[q] >> 32)));
+      w[q] = (at[q] >= cut) & ((at[q] == first) | (z >= r.lowest)) ? w[q] : 0;
+    }
+  }
+  u64 mine = 0;
+#pragma unroll
+  for (int q = 0; q < per; ++q) mine += w[q];
+  u64 upto = sm_scan(mine), total = 0;
+  __syncthreads();
+  if (t % 64 == 63) m.red[t / 64] = upto;
+  __syncthreads();
+  for (int k = 0; k < NT / 64; ++k) {
+    if (k == t / 64) upto += total;
+    total += m.red[k];
+  }
+  const u64 goal = sm_goal(p, row, total);
+  if (!(upto > goal && upto - mine <= goal)) return;   // one thread has it
+  u64 run = upto - mine;
+  int q = 0;
+#pragma unroll
+  for (int k = 0; k < per - 1; ++k) {
+    run += w[k];
+    if (run <= goal) q = k + 1;
+  }
+  p.token[row] = t * per + q;
+  p.logprob[row] = sm_logprob(r, to_f32(logits[t * per + q]), total);
 }
 
 // ------------------------------------------------------------------ rows of one workgroup
@@ -692,7 +798,8 @@ static hipError_t sample_t(SampleParams p, hipStream_t s) {
   const int64_t most = kGridThreads / 1024;
   for (; p.first < p.R; p.first += most) {
     const dim3 grid((unsigned)(p.R - p.first < most ? p.R - p.first : most));
-    if (p.V <= 2048) hipLaunchKernelGGL((k_sample_row<IT, 256, 1>), grid, dim3(256), 0, s, p);
+    if (p.V <= kShort) hipLaunchKernelGGL((k_sample_short<IT>), grid, dim3(256), 0, s, p);
+    else if (p.V <= 2048) hipLaunchKernelGGL((k_sample_row<IT, 256, 1>), grid, dim3(256), 0, s, p);
     else if (p.V <= 8192) hipLaunchKernelGGL((k_sample_row<IT, 1024, 1>), grid, dim3(1024), 0, s, p);
     else hipLaunchKernelGGL((k_sample_row<IT, 1024, 4>), grid, dim3(1024), 0, s, p);
   }
