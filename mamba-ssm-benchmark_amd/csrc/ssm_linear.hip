@@ -189,14 +189,14 @@ struct LinTile {
     } else {   // 16 columns on: two pieces; 4 k on: the pairs of pieces are dealt 4 pairs further; 32 k on: as here
       const char *at = lds + 32 * kk * line;
       const ls4 a = __builtin_amdgcn_ds_read_tr16_b64_v4i16((LdsTr)(at + (place ^ (32 * i))));
-      const ls4 b = __builtin_amdgcn_ds_read_tr16_b64_v4i16((LdsTr)(at + 4 * line + (place ^ (32 * i) ^ 128)));
+      const ls4 b = __builtin_amdgcn_ds_read_tr16_b64_v4i16((LdsTr)(at + 4 * line + (place ^ (32 * i) ^ (128 & (line - 1)))));
       return __builtin_bit_cast(li4, __builtin_shufflevector(a, b, 0, 1, 2, 3, 4, 5, 6, 7));
     }
   }
 };
 
 template <typename T, typename OT, bool AL, bool BL, int BM, int BN, int WM, int WN>
-__global__ void __launch_bounds__(64 * WM * WN) __attribute__((amdgpu_waves_per_eu(2, 2))) k_linear_tile(const GemmParams p) {
+__global__ void __launch_bounds__(64 * WM * WN) __attribute__((amdgpu_waves_per_eu(BM == 64 ? 4 : 2, BM == 64 ? 4 : 2))) k_linear_tile(const GemmParams p) {
   constexpr int NW = WM * WN, MT = BM / WM / 16, NT = BN / WN / 16, E = sizeof(T);
   constexpr int KE = AL || BL ? 128 / E : 64, STEPS = 128 / (4 * Mma<T>::bytes);
   typedef LinTile<AL, BM, NW, 4, E == 1> TA;
@@ -372,10 +372,10 @@ __global__ void __launch_bounds__(256) k_linear_join(const GemmParams p) {
 // ------------------------------------------------------------------ few rows
 // Up to 16 MT rows: the weights are read once, straight into the matrix instructions' operands, 16 NT of their rows a
 // workgroup, whose 8 wavefronts share k and join their sums in LDS in order.  Rows may begin anywhere.
-template <typename T, int F>
+template <typename T, int F, bool WHOLE = false>
 __device__ __forceinline__ void lin_row(const T *row, int64_t k, int64_t K, int (&f)[F]) {   // 4 F bytes from k on
   constexpr int n = 4 * F / sizeof(T);
-  if (k + n <= K) {
+  if (WHOLE || k + n <= K) {
     __builtin_memcpy(f, row + k, 4 * F);
   } else {
     T e[n];
@@ -385,12 +385,13 @@ __device__ __forceinline__ void lin_row(const T *row, int64_t k, int64_t K, int 
   }
 }
 template <typename T, typename OT, int MT, int NT>
-__global__ void __launch_bounds__(512) k_linear_rows(const GemmParams p) {
-  constexpr int F = Mma<T>::bytes / 4, KE = 4 * Mma<T>::bytes / sizeof(T), U = MT * NT >= 8 ? 2 : 4;
+__global__ void __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2, 2))) k_linear_rows(const GemmParams p) {
+  constexpr int F = Mma<T>::bytes / 4, KE = 4 * Mma<T>::bytes / sizeof(T), U = sizeof(T) == 1 && MT * NT == 8 ? 2 : 4;   // steps whose loads are under way together
   __shared__ __attribute__((aligned(16))) float red[8][MT * 16][NT * 16 + 4];
   const int lane = threadIdx.x % 64, wave = threadIdx.x / 64, g = lane / 16;
-  const int64_t nb = (p.N + 16 * NT - 1) / (16 * NT), n0 = blockIdx.x % nb * (16 * NT), split = blockIdx.x / nb;
-  const int64_t ks = (p.K + KE - 1) / KE, parts = 8 * p.splits, part = split * 8 + wave;
+  const uint32_t nb = (uint32_t)((p.N + 16 * NT - 1) / (16 * NT)), split = blockIdx.x / nb;
+  const int64_t n0 = (int64_t)(blockIdx.x % nb) * (16 * NT);
+  const uint32_t ks = (uint32_t)((p.K + KE - 1) / KE), parts = 8 * p.splits, part = split * 8 + wave;   // ks < 2^20, parts < 2^11
   const int64_t s0 = ks * part / parts, s1 = ks * (part + 1) / parts;
   const T *w[NT], *x[MT];
 #pragma unroll
@@ -404,17 +405,25 @@ __global__ void __launch_bounds__(512) k_linear_rows(const GemmParams p) {
     x[i] = (const T *)p.A + (m < p.M ? m : p.M - 1) * p.sa;
   }
   lf4 acc[MT][NT] = {};
-  const int64_t at = g * (KE / 4);
-  auto steps = [&](int64_t s, auto count) {
+  // A load takes 64 consecutive bytes of a row, so of a step's two in 8 bits a lane holds 16 bytes each: the order of k
+  // within a step is the same for both operands, and no matter.
+  constexpr int PIECES = F / 4, P16 = 16 / sizeof(T);
+  const int64_t at = g * P16;
+  auto steps = [&](int64_t s, auto count, auto whole) {
     constexpr int C = decltype(count)::value;
-    int fw[C][NT][F], fx[C][MT][F];
+    constexpr bool WHOLE = decltype(whole)::value;
+    int fw[C][NT][PIECES][4], fx[C][MT][PIECES][4];
 #pragma unroll
-    for (int u = 0; u < C; ++u) {
+    for (int u = 0; u < C; ++u)
 #pragma unroll
-      for (int j = 0; j < NT; ++j) lin_row<T, F>(w[j], (s + u) * KE + at, p.K, fw[u][j]);
+      for (int h = 0; h < PIECES; ++h) {
+        const int64_t k = (s + u) * KE + at + 4 * P16 * h;
 #pragma unroll
-      for (int i = 0; i < MT; ++i) lin_row<T, F>(x[i], (s + u) * KE + at, p.K, fx[u][i]);
-    }
+        for (int j = 0; j < NT; ++j) lin_row<T, 4, WHOLE>(w[j], k, p.K, fw[u][j][h]);
+#pragma unroll
+        for (int i = 0; i < MT; ++i) lin_row<T, 4, WHOLE>(x[i], k, p.K, fx[u][i][h]);
+      }
+    __builtin_amdgcn_sched_barrier(0);   // all loads are under way before the first product
 #pragma unroll
     for (int u = 0; u < C; ++u)
 #pragma unroll
@@ -424,9 +433,12 @@ __global__ void __launch_bounds__(512) k_linear_rows(const GemmParams p) {
           acc[i][j] = Mma<T>::mul(__builtin_bit_cast(typename Mma<T>::Frag, fw[u][j]), __builtin_bit_cast(typename Mma<T>::Frag, fx[u][i]),
                                   acc[i][j]);
   };
+  const int64_t s2 = s1 < p.K / KE ? s1 : p.K / KE;   // the whole steps' end
   int64_t s = s0;
-  for (; s + U <= s1; s += U) steps(s, std::integral_constant<int, U>{});
-  for (; s < s1; ++s) steps(s, std::integral_constant<int, 1>{});
+  for (; s + U <= s2; s += U) steps(s, std::integral_constant<int, U>{}, std::true_type{});
+#pragma unroll 1
+  for (; s < s2; ++s) steps(s, std::integral_constant<int, 1>{}, std::true_type{});
+  if (s < s1) steps(s, std::integral_constant<int, 1>{}, std::false_type{});
 #pragma unroll
   for (int i = 0; i < MT; ++i)
 #pragma unroll
@@ -517,11 +529,12 @@ LinearPlan linear_plan(const GemmParams &p) {
   } else {
     if (!loadable(p.A, p.sa, p.a_along && !p.a_padded ? p.K : unit, e)) l.pack_a = p.a_along ? p.M * up(p.K) * e : p.K * up(p.M) * e;
     if (!loadable(p.B, p.sb, p.b_along ? p.K : unit, e)) l.pack_b = p.b_along ? p.N * up(p.K) * e : p.K * up(p.N) * e;
-    const int64_t big = ((p.M + 255) / 256) * ((p.N + 255) / 256);
-    l.tile = big >= 192 ? 256 : 128;
-    const int64_t tiles = l.tile == 256 ? big : ((p.M + 127) / 128) * ((p.N + 127) / 128), steps = (p.K * e + 127) / 128;
-    l.splits = 1;   // two workgroups a compute unit, 4 steps each at least
-    while (l.tile == 128 && tiles * l.splits * 2 <= 512 && steps / (l.splits * 2) >= 4 && l.splits < 16) l.splits *= 2;
+    auto tiles = [&](int64_t t) { return ((p.M + t - 1) / t) * ((p.N + t - 1) / t); };
+    const int64_t steps = (p.K * e + 127) / 128;
+    // the largest tiles that occupy three quarters of the compute units
+    l.tile = tiles(256) >= 192 ? 256 : tiles(128) >= 192 ? 128 : 64;
+    l.splits = 1;   // up to two workgroups a compute unit, 8 steps each at least
+    while (l.tile == 64 && tiles(64) * l.splits * 2 <= 512 && steps / (l.splits * 2) >= 8) l.splits *= 2;
   }
   l.pack_a = (l.pack_a + 255) / 256 * 256;
   l.pack_b = (l.pack_b + 255) / 256 * 256;
@@ -540,7 +553,8 @@ template <typename T, typename OT, bool AL, bool BL>
 static void tile_v(const GemmParams &p, const LinearPlan &l, hipStream_t s) {
   const int64_t t = l.tile, tiles = ((p.M + t - 1) / t) * ((p.N + t - 1) / t) * l.splits;
   if (l.tile == 256) hipLaunchKernelGGL((k_linear_tile<T, OT, AL, BL, 256, 256, 2, 4>), dim3((unsigned)tiles), dim3(512), 0, s, p);
-  else hipLaunchKernelGGL((k_linear_tile<T, OT, AL, BL, 128, 128, 2, 2>), dim3((unsigned)tiles), dim3(256), 0, s, p);
+  else if (l.tile == 128) hipLaunchKernelGGL((k_linear_tile<T, OT, AL, BL, 128, 128, 2, 2>), dim3((unsigned)tiles), dim3(256), 0, s, p);
+  else hipLaunchKernelGGL((k_linear_tile<T, OT, AL, BL, 64, 64, 2, 2>), dim3((unsigned)tiles), dim3(256), 0, s, p);
 }
 template <typename T, typename OT, int MT>
 static void rows_v(const GemmParams &p, const LinearPlan &l, hipStream_t s) {

@@ -29,7 +29,8 @@ from .conv import causal_conv1d
 from .hip_scan import selective_scan_fn
 from .linear import embedding, linear
 from .mixer import mixer, mixer_applies
-from .norm import rms_norm
+from .norm import add_rms_norm, rms_norm
+from .sampling import sample
 from .scan import selective_scan
 from .step import ssm_step
 
@@ -166,14 +167,17 @@ class Mamba(nn.Module):
 
 class RMSNorm(nn.Module):
     """models/common.py RMSNorm: x / rms(x) * weight (ssm_scan.norm: one kernel per pass for
-    float32 rows)."""
+    float32 rows).  With a residual the call returns (norm of x + residual, x + residual), in one kernel per
+    pass (ssm_scan.norm.add_rms_norm)."""
 
     def __init__(self, d, eps=1e-5):
         super().__init__()
         self.eps = eps
         self.weight = nn.Parameter(torch.ones(d))
 
-    def forward(self, x):
+    def forward(self, x, residual=None):
+        if residual is not None:
+            return add_rms_norm(x, residual, self.weight, self.eps)
         return rms_norm(x, self.weight, self.eps)
 
 
@@ -253,18 +257,25 @@ class MambaLM(nn.Module):
         return linear(self.head, self.norm_f(x))
 
     @torch.no_grad()
-    def generate(self, prompt, n_new, temperature=1.0, top_k=None, max_len=None):
-        """Autoregressive sampling (models/lm.py:130-147): prefill, then one step per token."""
+    def generate(self, prompt, n_new, temperature=1.0, top_k=None, max_len=None, top_p=None, min_p=None, generator=None):
+        """Autoregressive sampling (models/lm.py:130-147): prefill, then one step per token.  With top_p, min_p or
+        a generator the tokens are drawn by ssm_scan.sample from uniform numbers (the generator's, on the model's
+        device), whose settings may be tensors with one per row; without, by the reference's steps."""
         Bsz, T = prompt.shape
         states = self.init_state(Bsz, max_len or T + n_new, prompt.device)
         logits = self(prompt, states, 0)[:, -1]
         out = [prompt]
+        own = top_p is not None or min_p is not None or generator is not None
         for t in range(n_new):
-            logits = logits.float() / max(temperature, 1e-6)
-            if top_k:
-                v, _ = torch.topk(logits, top_k)
-                logits[logits < v[:, [-1]]] = float("-inf")
-            nxt = torch.multinomial(F.softmax(logits, -1), 1)
+            if own:
+                u = torch.rand(Bsz, generator=generator, device=prompt.device)
+                nxt = sample(logits, u, temperature, top_k, top_p, min_p)[0].unsqueeze(1)
+            else:
+                logits = logits.float() / max(temperature, 1e-6)
+                if top_k:
+                    v, _ = torch.topk(logits, top_k)
+                    logits[logits < v[:, [-1]]] = float("-inf")
+                nxt = torch.multinomial(F.softmax(logits, -1), 1)
             out.append(nxt)
             if t < n_new - 1:
                 logits = self(nxt, states, T + t)[:, -1]

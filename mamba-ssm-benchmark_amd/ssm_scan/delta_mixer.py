@@ -22,13 +22,14 @@ import torch.nn.functional as F
 from .conv import causal_conv1d
 from .delta import gated_delta_rule, gated_delta_step
 from .group_norm import group_norm
-from .linear import linear
+from .linear import linear, linear_act
 
 
 class GatedDeltaMixer(nn.Module):
     """(B, L, d_model) -> (B, L, d_model).  heads value heads of value_dim, key_heads (dividing heads; all
     by default) of key_dim <= 128.  With a state (init_state) the call continues the sequence and updates
-    it, one token per call being the decode step.  The states change in place, so such a call is inference: it
+    it, one token per call being the decode step.  A residual (B, L, d_model) is added to the output: in 16 bits
+    (weights, u and residual of one type, no autocast) in the output projection's epilogue.  The states change in place, so such a call is inference: it
     runs without autograd whatever the grad mode, and its output has no graph."""
 
     def __init__(self, d_model, heads, key_dim, value_dim=None, key_heads=None, d_conv=4, dt_min=1e-3, dt_max=0.1):
@@ -60,11 +61,11 @@ class GatedDeltaMixer(nn.Module):
         state.conv.copy_(previous)
         return out
 
-    def forward(self, u, state=None):
+    def forward(self, u, state=None, residual=None):
         with torch.set_grad_enabled(torch.is_grad_enabled() and state is None):
-            return self._forward(u, state)
+            return self._forward(u, state, residual)
 
-    def _forward(self, u, state):
+    def _forward(self, u, state, residual):
         mixed, z, dt, b = linear(self.in_proj, u).split(
             [2 * self.d_keys + self.d_values, self.d_values, self.heads, self.heads], dim=-1)
         mixed = self._conv(mixed, state)
@@ -81,4 +82,10 @@ class GatedDeltaMixer(nn.Module):
             if state is not None:
                 state.delta.copy_(last)
         y = group_norm(y.flatten(-2), self.heads, self.norm_weight, gate=z, center=False)
-        return linear(self.out_proj, y)
+        if residual is None:
+            return linear(self.out_proj, y)
+        w = self.out_proj.weight
+        if (w.dtype in (torch.bfloat16, torch.float16) and y.dtype == residual.dtype == w.dtype
+                and not torch.is_autocast_enabled(y.device.type)):
+            return linear_act(y, w, residual=residual)
+        return residual + linear(self.out_proj, y)

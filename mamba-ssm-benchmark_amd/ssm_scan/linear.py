@@ -18,6 +18,7 @@ import torch
 import torch.nn.functional as F
 
 from . import _abi
+from .embed import embedding as scaled_embedding
 
 SPLITS = 8          # token slices of the weight gradient
 MIN_TOKENS = 2048   # below this the plain product already fills the GPU as well
@@ -121,6 +122,7 @@ def linear_8bit(q, scale, weight, weight_scale, bias=None, activation=None, resi
     return _abi.host().linear_8bit(q, scale, weight, weight_scale, bias, residual, _activation(activation), dtype)
 
 
+_SORTED_TYPES = (torch.float32, torch.bfloat16, torch.float16)
 MAX_DENSE_VOCAB = 4096  # vocabularies up to this size take the one-hot product
 
 
@@ -146,11 +148,15 @@ def embedding(layer, idx):
     <= MAX_DENSE_VOCAB) the weight gradient is onehot(idx)^T dY, a dense product (split-K over
     the tokens): the same sums as torch's embedding backward, which sorts the indices with
     sizes it reads back on the host -- this one makes no host reads, so a training step that
-    contains it can be captured in a HIP graph, and it runs in a fixed order."""
+    contains it can be captured in a HIP graph, and it runs in a fixed order.  Trained with a larger vocabulary, or in
+    16 bits, it is ssm_scan.embedding, which sorts on the GPU and has the same properties (ids outside the vocabulary,
+    at which nn.Embedding ends the process, give zeros there)."""
     w = layer.weight
     plain = (layer.padding_idx is None and layer.max_norm is None and not layer.scale_grad_by_freq
              and not layer.sparse)
     if (plain and torch.is_grad_enabled() and w.requires_grad and w.dtype == torch.float32
             and w.shape[0] <= MAX_DENSE_VOCAB and not torch.is_autocast_enabled(w.device.type)):
         return _DenseGradEmbedding.apply(idx, w)
+    if plain and torch.is_grad_enabled() and w.requires_grad and w.is_cuda and w.dtype in _SORTED_TYPES:
+        return scaled_embedding(idx, w)
     return layer(idx)
