@@ -1476,7 +1476,7 @@ int ssm_embed_check(const ssm_embed_args *a) {
   if (!io16_32(a->dtype)) return fail(SSM_EINVAL, "the embedding takes float32, bfloat16 or float16");
   if (a->n < 1 || a->vocab < 1 || a->dim < 1)
     return fail(SSM_EINVAL, "empty embedding: n=%lld vocab=%lld dim=%lld", (long long)a->n, (long long)a->vocab, (long long)a->dim);
-  if (a->n >= (1LL << 40) || a->vocab >= (1LL << 31) - 1 || a->dim >= (1LL << 24))
+  if (a->n >= (1LL << 40) || a->vocab > (1LL << 27) || a->dim >= (1LL << 24))
     return fail(SSM_EINVAL, "embedding is too large: n=%lld vocab=%lld dim=%lld", (long long)a->n, (long long)a->vocab, (long long)a->dim);
   if (!isfinite(a->scale)) return fail(SSM_EINVAL, "scale must be finite");
   return ok();
@@ -1561,9 +1561,9 @@ int ssm_linear_check(const ssm_linear_args *a) {
   if (a->dtype != SSM_BF16 && a->dtype != SSM_F16) return fail(SSM_EINVAL, "the linear layer takes bfloat16 or float16");
   if (a->m < 1 || a->n < 1 || a->k < 1)
     return fail(SSM_EINVAL, "empty product: m=%lld n=%lld k=%lld", (long long)a->m, (long long)a->n, (long long)a->k);
-  const int64_t side = 1LL << 24, area = 1LL << 35;   // tiles of 64 x 64 fit a launch of 256 threads each
+  const int64_t side = 1LL << 24, area = 1LL << 34;   // a thread each 16 bytes of a copied matrix fits a launch
   if (a->m > side || a->n > side || a->k > side || a->m * a->n > area || a->m * a->k > area || a->n * a->k > area)
-    return fail(SSM_EINVAL, "product is too large: m=%lld n=%lld k=%lld (each up to 2^24, each matrix up to 2^35)", (long long)a->m,
+    return fail(SSM_EINVAL, "product is too large: m=%lld n=%lld k=%lld (each up to 2^24, each matrix up to 2^34)", (long long)a->m,
                 (long long)a->n, (long long)a->k);
   if (a->activation < SSM_ACT_NONE || a->activation > SSM_ACT_GELU) return fail(SSM_EINVAL, "unknown activation %d", a->activation);
   int rc = gnorm_view(a->x, "x");
@@ -1628,7 +1628,7 @@ LinearBwd linear_backward_plan(const ssm_linear_args *a) {
   if (has(a->dweight)) {   // dweight[n, k] = sum over m of dz[m, n] x[m, k]
     GemmParams &p = l.dw;
     p.M = a->n; p.N = a->k; p.K = a->m;
-    p.A = dz; p.sa = sdz; p.a_along = 0;
+    p.A = dz; p.sa = sdz; p.a_along = 0; p.a_padded = 1;
     p.B = a->x.data; p.sb = a->x.stride[0]; p.b_along = 0;
     p.C = a->dweight.data; p.sc = a->dweight.stride[0];
     l.products = std::max(l.products, linear_plan(p).bytes());

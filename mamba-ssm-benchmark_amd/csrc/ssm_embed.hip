@@ -3,6 +3,8 @@
 // The gradient sorts the tokens (stable radix sort, so equal tokens keep their order), adds the rows of dout that belong
 // to one token in that order and writes every row of dw once, zeros included: no float atomics, bitwise repeatable,
 // nothing is read back on the host.
+#include <algorithm>
+
 #include "ssm_device.hpp"
 #include "ssm_internal.hpp"
 
@@ -145,6 +147,107 @@ __global__ void __launch_bounds__(256) k_embed_place(const EmbedParams p) {
   }
 }
 
+// Place i is the first of the tokens above its forerunner's up to its own: mostly few, else the wavefront's work.
+__device__ __forceinline__ void em_bounds(const EmbedParams &p, int64_t i, bool there, int64_t before, int64_t own) {
+  const int64_t v0 = before + 1, v1 = there ? own : before;
+  uint64_t wide = __ballot(v1 - v0 >= 16);
+  if (v1 - v0 < 16)
+    for (int64_t v = v0; v <= v1; ++v) p.start[v] = (uint32_t)i;
+  while (wide) {
+    const int l = __ffsll((unsigned long long)wide) - 1;
+    wide &= wide - 1;
+    const int64_t w1 = __shfl(v1, l), at = __shfl(i, l);
+    for (int64_t v = __shfl(v0, l) + threadIdx.x % 64; v <= w1; v += 64) p.start[v] = (uint32_t)at;
+  }
+}
+
+// All passes in one workgroup, for up to kEmbedShort tokens: keys and places stay in LDS, a wavefront's items pass through
+// its registers.  The same steps as above, and the first place of every token with them.
+__global__ void __launch_bounds__(1024) k_embed_sort(const EmbedParams p) {
+  constexpr int U = kEmbedShort / 1024, B = 1 << kEmbedBits;
+  __shared__ uint32_t keys[kEmbedShort];
+  __shared__ uint16_t places[kEmbedShort];
+  __shared__ uint32_t base[16][B];
+  __shared__ uint32_t sums[16];
+  const int lane = threadIdx.x % 64, w = threadIdx.x / 64, n = (int)p.n;
+  const int steps = (n + 1023) / 1024, i0 = w * steps * 64;   // of a wavefront
+  for (int pass = 0; pass * p.bits < p.all_bits; ++pass) {
+    const int shift = pass * p.bits;
+    for (int b = threadIdx.x; b < 16 * B; b += 1024) base[b / B][b % B] = 0;
+    uint32_t key[U], place[U];
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const int i = i0 + 64 * u + lane;
+      if (u >= steps || i >= n) continue;
+      if (pass) {
+        key[u] = keys[i];
+        place[u] = places[i];
+      } else {
+        const int64_t v = p.tokens[i];
+        key[u] = v >= 0 && v < p.V ? (uint32_t)v : (uint32_t)p.V;
+        place[u] = i;
+      }
+    }
+    __syncthreads();
+#pragma unroll
+    for (int u = 0; u < U; ++u)
+      if (u < steps && i0 + 64 * u + lane < n) atomicAdd(&base[w][(key[u] >> shift) & (B - 1)], 1u);
+    __syncthreads();
+    uint32_t all = 0, before = 0;
+    if (threadIdx.x < B)
+      for (int v = 0; v < 16; ++v) all += base[v][threadIdx.x];
+    uint32_t upto = all;
+#pragma unroll
+    for (int d = 1; d < 64; d *= 2) {
+      const uint32_t t = __shfl_up(upto, d);
+      if (lane >= d) upto += t;
+    }
+    if (lane == 63) sums[w] = upto;
+    __syncthreads();
+    for (int v = 0; v < w; ++v) before += sums[v];
+    if (threadIdx.x < B) {
+      uint32_t at = before + upto - all;
+      for (int v = 0; v < 16; ++v) {
+        const uint32_t c = base[v][threadIdx.x];
+        base[v][threadIdx.x] = at;
+        at += c;
+      }
+    }
+    __syncthreads();
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      if (u >= steps) continue;
+      const bool there = i0 + 64 * u + lane < n;
+      const uint32_t digit = there ? (key[u] >> shift) & (B - 1) : 0;
+      uint64_t same = __ballot(there);
+      for (int b = 0; b < p.bits; ++b) {
+        const uint64_t set = __ballot((digit >> b) & 1);
+        same &= (digit >> b) & 1 ? set : ~set;
+      }
+      const int ahead = __popcll(same & ((1ull << lane) - 1));
+      uint32_t at = 0;
+      if (there) at = base[w][digit] + ahead;
+      __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+      __builtin_amdgcn_wave_barrier();
+      if (there && ahead == 0) base[w][digit] += __popcll(same);
+      __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+      __builtin_amdgcn_wave_barrier();
+      if (there) {
+        keys[at] = key[u];
+        places[at] = (uint16_t)place[u];
+      }
+    }
+    __syncthreads();
+  }
+  for (int i = threadIdx.x; i - (int)threadIdx.x <= n; i += 1024) {   // whole wavefronts, and place n too
+    if (i < n) {
+      p.key[0][i] = keys[i];
+      p.pos[0][i] = places[i];
+    }
+    em_bounds(p, i, i <= n, i && i <= n ? (int64_t)keys[i - 1] : -1, i < n ? (int64_t)keys[i] : p.V);
+  }
+}
+
 // ------------------------------------------------------------------ sums
 // Sum of dout's rows at sorted places [from, to), columns j .. j + V, in order; up to 16 rows are read together.
 template <int U, typename IT, int V>
@@ -193,22 +296,8 @@ __device__ __forceinline__ void em_parts(const float *src, int64_t from, int64_t
 template <typename IT, int V>
 __global__ void __launch_bounds__(256) k_embed_pieces(const EmbedParams p) {
   if ((int64_t)blockIdx.x >= p.npiece_blocks) {
-    // place i is the first of the tokens above its forerunner's up to its own: mostly few, else the wavefront's work
     const int64_t i = ((int64_t)blockIdx.x - p.npiece_blocks) * 256 + threadIdx.x;
-    int64_t v0 = 0, v1 = -1;
-    if (i <= p.n) {
-      v0 = i ? (int64_t)p.key_in[i - 1] + 1 : 0;
-      v1 = i < p.n ? (int64_t)p.key_in[i] : p.V;
-    }
-    uint64_t wide = __ballot(v1 - v0 >= 16);
-    if (v1 - v0 < 16)
-      for (int64_t v = v0; v <= v1; ++v) p.start[v] = (uint32_t)i;
-    while (wide) {
-      const int l = __ffsll((unsigned long long)wide) - 1;
-      wide &= wide - 1;
-      const int64_t w1 = __shfl(v1, l), at = __shfl(i, l);
-      for (int64_t v = __shfl(v0, l) + threadIdx.x % 64; v <= w1; v += 64) p.start[v] = (uint32_t)at;
-    }
+    em_bounds(p, i, i <= p.n, i && i <= p.n ? (int64_t)p.key_in[i - 1] : -1, i < p.n ? (int64_t)p.key_in[i] : p.V);
     return;
   }
   const int l = threadIdx.x & (p.lanes - 1);
@@ -254,14 +343,14 @@ __global__ void __launch_bounds__(256) k_embed_rows(const EmbedParams p) {
         for (int64_t j = (int64_t)l * V; j < p.D; j += (int64_t)p.lanes * V) em_store<IT, V>((IT *)p.dw + (v0 + i) * p.D + j, zero);
     return;
   }
-  const int64_t i = ((int64_t)blockIdx.x - p.nzero_blocks) * groups + group;
+  const int64_t i = p.first + ((int64_t)blockIdx.x - p.nzero_blocks) * groups + group;
   if (i >= p.n) return;
   {
     const uint32_t v = p.key_in[i], last = i ? p.key_in[i - 1] : v + 1;
     if (v >= (uint32_t)p.V || last == v) return;
     const int64_t s = i, e = p.start[v + 1];
     int64_t p0 = (s + P - 1) / P, p1 = e / P;         // whole pieces
-    if (p0 >= p1) p0 = p1 = -1;
+    if (p0 >= p1 || !p.pieces) p0 = p1 = -1;
     int64_t g0 = (p0 + G - 1) / G, g1 = p1 / G;       // whole groups
     if (!p.group || p0 < 0 || g0 >= g1) g0 = g1 = -1;
     for (int64_t j = (int64_t)l * V; j < p.D; j += (int64_t)p.lanes * V) {
@@ -295,25 +384,37 @@ static hipError_t embed_v(EmbedParams p, bool bwd, hipStream_t s) {
       hipLaunchKernelGGL((k_embed_fwd<IT, V>), blocks(p.n - p.first < most ? p.n - p.first : most), dim3(256), 0, s, p);
     return hipGetLastError();
   }
-  int bits = 0;
-  while ((p.V >> bits) > 0) ++bits;   // keys 0 .. V
-  const int passes = (bits + kEmbedBits - 1) / kEmbedBits;
-  p.bits = (bits + passes - 1) / passes;
-  for (p.pass = 0; p.pass < passes; ++p.pass) {
-    p.shift = p.pass * p.bits;
-    p.key_out = p.key[p.pass & 1];
-    p.pos_out = p.pos[p.pass & 1];
-    hipLaunchKernelGGL(k_embed_count, dim3((unsigned)((p.nw + 3) / 4)), dim3(256), 0, s, p);
-    hipLaunchKernelGGL(k_embed_place, dim3((unsigned)((p.nw + 3) / 4)), dim3(256), 0, s, p);
-    p.key_in = p.key_out;
-    p.pos_in = p.pos_out;
+  while ((p.V >> p.all_bits) > 0) ++p.all_bits;   // keys 0 .. V
+  const int passes = (p.all_bits + kEmbedBits - 1) / kEmbedBits;
+  p.bits = (p.all_bits + passes - 1) / passes;
+  // One launch in place of two a pass and the bounds: 15 us against 17 for 8192 tokens and a pass, at two passes from
+  // 4096 tokens on more (16384: 62 against 36).
+  const bool one = p.n <= (passes == 1 ? kEmbedShort : 2048);
+  if (one) {
+    p.bits = kEmbedBits;
+    hipLaunchKernelGGL(k_embed_sort, dim3(1), dim3(1024), 0, s, p);
+    p.key_in = p.key[0];
+    p.pos_in = p.pos[0];
+  } else {
+    for (p.pass = 0; p.pass < passes; ++p.pass) {
+      p.shift = p.pass * p.bits;
+      p.key_out = p.key[p.pass & 1];
+      p.pos_out = p.pos[p.pass & 1];
+      hipLaunchKernelGGL(k_embed_count, dim3((unsigned)((p.nw + 3) / 4)), dim3(256), 0, s, p);
+      hipLaunchKernelGGL(k_embed_place, dim3((unsigned)((p.nw + 3) / 4)), dim3(256), 0, s, p);
+      p.key_in = p.key_out;
+      p.pos_in = p.pos_out;
+    }
   }
-  const int64_t pieces = p.n / kEmbedPiece;
+  // a few hundred places are summed one by one whatever their tokens
+  const int64_t pieces = p.n <= 512 ? 0 : p.n / kEmbedPiece, bounds = one ? 0 : (p.n + 256) / 256;
+  p.pieces = pieces > 0;
   p.npiece_blocks = (pieces + Q - 1) / Q;
-  hipLaunchKernelGGL((k_embed_pieces<IT, V>), dim3((unsigned)(p.npiece_blocks + (p.n + 256) / 256)), dim3(256), 0, s, p);
+  if (pieces || bounds) hipLaunchKernelGGL((k_embed_pieces<IT, V>), dim3((unsigned)(p.npiece_blocks + bounds)), dim3(256), 0, s, p);
   if (p.group) hipLaunchKernelGGL((k_embed_groups<V>), blocks(pieces / kEmbedGroup), dim3(256), 0, s, p);
   p.nzero_blocks = (p.V + kEmbedRows - 1) / kEmbedRows;
-  hipLaunchKernelGGL((k_embed_rows<IT, V>), dim3((unsigned)(p.nzero_blocks + (p.n + Q - 1) / Q)), dim3(256), 0, s, p);
+  for (; p.first < p.n; p.first += most, p.nzero_blocks = 0)
+    hipLaunchKernelGGL((k_embed_rows<IT, V>), dim3((unsigned)(p.nzero_blocks + (std::min(p.n - p.first, most) + Q - 1) / Q)), dim3(256), 0, s, p);
   return hipGetLastError();
 }
 template <typename IT>

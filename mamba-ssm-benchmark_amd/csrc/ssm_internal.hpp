@@ -391,6 +391,7 @@ hipError_t launch_rnorm(const RnormParams &p, int dtype, int rdtype, bool bwd, h
 // Token embedding and its gradient.
 constexpr int kEmbedBits = 9;          // of a sorting pass
 constexpr int64_t kEmbedWaves = 64;   // wavefronts that sort, at most
+constexpr int kEmbedShort = 8192;      // tokens that one workgroup sorts, at most
 constexpr int kEmbedRows = 32;         // rows of the gradient that a workgroup looks at for zeros
 constexpr int kEmbedPiece = 32;        // sorted places that are summed at once where they hold one token
 constexpr int kEmbedGroup = 32;        // pieces likewise
@@ -404,7 +405,7 @@ struct EmbedParams {
   int64_t sw, so, sd;                  // row strides
   int64_t first;                       // rows of earlier launches
   // gradient
-  int pass, bits, shift;
+  int pass, bits, all_bits, shift, pieces;  // pieces: sums of whole pieces are formed
   int64_t nw, per;                     // sorting wavefronts, items of each
   uint32_t *hist;                      // (nw, 2^bits)
   const uint32_t *key_in, *pos_in;

@@ -527,8 +527,8 @@ LinearPlan linear_plan(const GemmParams &p) {
     l.splits = 1;   // more where few workgroups would each walk a long k: 16 steps a wavefront at least
     while (nb * l.splits < 128 && steps / (8 * l.splits * 2) >= 16) l.splits *= 2;
   } else {
-    if (!loadable(p.A, p.sa, p.a_along && !p.a_padded ? p.K : unit, e)) l.pack_a = p.a_along ? p.M * up(p.K) * e : p.K * up(p.M) * e;
-    if (!loadable(p.B, p.sb, p.b_along ? p.K : unit, e)) l.pack_b = p.b_along ? p.N * up(p.K) * e : p.K * up(p.N) * e;
+    if (!loadable(p.A, p.sa, p.a_padded ? unit : p.a_along ? p.K : p.M, e)) l.pack_a = p.a_along ? p.M * up(p.K) * e : p.K * up(p.M) * e;
+    if (!loadable(p.B, p.sb, p.b_along ? p.K : p.N, e)) l.pack_b = p.b_along ? p.N * up(p.K) * e : p.K * up(p.N) * e;
     auto tiles = [&](int64_t t) { return ((p.M + t - 1) / t) * ((p.N + t - 1) / t); };
     const int64_t steps = (p.K * e + 127) / 128;
     // the largest tiles that occupy three quarters of the compute units

@@ -206,3 +206,35 @@ def test_refusals_and_no_rows(dev):
     g, = torch.autograd.grad(ssm_scan.linear_act(leaf, w).sum(), leaf, create_graph=True)
     with pytest.raises(RuntimeError, match="twice"):
         g.sum().backward()
+
+
+def test_views_that_end_with_their_storage(dev):
+    """Rows of whole loads whose last one ends inside a load, at the end of the memory that is theirs."""
+    for io in (BF16, F16):
+        x, w, b, r, dy = make(dev, (70, 515), 136, io, seed=9)
+        sx, sw = torch.zeros(69 * 520 + 515, dtype=io, device=dev), torch.zeros(135 * 520 + 515, dtype=io, device=dev)
+        vx, vw = sx.as_strided((70, 515), (520, 1)), sw.as_strided((136, 515), (520, 1))
+        vx.copy_(x)
+        vw.copy_(w)
+        sx.as_strided((69, 5), (520, 1), 515).fill_(float("nan"))   # between the rows
+        sw.as_strided((135, 5), (520, 1), 515).fill_(float("nan"))
+        check(vx, vw, b, "silu", r, dy)
+        check(vx[:9], vw, b, "silu", r[:9], dy[:9])
+
+
+@pytest.mark.parametrize("M,N,K", [(70, 65, 4200), (65, 64, 64), (129, 200, 130), (2100, 2050, 72), (3000, 1100, 40), (66, 3000, 1000),
+                                   (3700, 3500, 136)])
+def test_tiles_and_splits(dev, M, N, K):
+    """Every size of tile, ragged in each direction, with one split of k and with several."""
+    x, w, b, r, dy = make(dev, (M, K), N, BF16, seed=M)
+    check(x, w, b, "gelu", r, dy)
+
+
+@pytest.mark.parametrize("M,N,K", [(3700, 3500, 400), (1800, 2000, 272), (700, 130, 4112)])
+def test_8bit_tiles(dev, M, N, K):
+    """Whole numbers (exact sums) through every size of tile."""
+    r = torch.Generator().manual_seed(10)
+    x, w = (torch.randint(-4, 5, s, generator=r).float() for s in ((M, K), (N, K)))
+    ones = torch.ones(max(M, N), device=dev) / 64
+    y = ssm_scan.linear_8bit(x.to(torch.float8_e4m3fn).to(dev), ones[:M], w.to(torch.float8_e4m3fn).to(dev), ones[:N])
+    assert torch.equal(y.cpu(), (x.to(dev) @ w.to(dev).t() / 4096).bfloat16().cpu())

@@ -125,10 +125,10 @@ def sample(**kw):
 @pytest.mark.parametrize("make,check,bad", [
     (rnorm, "ssm_rnorm_check", [dict(rows=0), dict(dim=0), dict(dim=16385), dict(dtype=_abi.F64), dict(res_dtype=_abi.F16), dict(eps=-1.0),
                                 dict(eps=math.nan), dict(rows=1 << 40)]),
-    (embed, "ssm_embed_check", [dict(n=0), dict(vocab=0), dict(dim=0), dict(dtype=_abi.F64), dict(scale=math.inf), dict(vocab=(1 << 31) - 1),
+    (embed, "ssm_embed_check", [dict(n=0), dict(vocab=0), dict(dim=0), dict(dtype=_abi.F64), dict(scale=math.inf), dict(vocab=(1 << 27) + 1),
                                 dict(n=1 << 40), dict(dim=1 << 24)]),
     (linear, "ssm_linear_check", [dict(m=0), dict(n=0), dict(k=0), dict(dtype=_abi.F32), dict(activation=3), dict(activation=-1),
-                                  dict(m=(1 << 24) + 1), dict(m=1 << 20, n=1 << 16), dict(in8=1), dict(x=_abi.Tensor()),
+                                  dict(m=(1 << 24) + 1), dict(m=1 << 20, n=1 << 15), dict(in8=1), dict(x=_abi.Tensor()),
                                   dict(weight=_abi.Tensor(256, (ctypes.c_int64 * 3)(8, 2, 0)))]),
     (sample, "ssm_sample_check", [dict(rows=0), dict(vocab=0), dict(vocab=(1 << 24) + 1), dict(dtype=_abi.F64), dict(temperature=-1.0),
                                   dict(temperature=math.nan), dict(top_k=-1), dict(top_p=-0.1), dict(min_p=-0.1), dict(rows=1 << 31)]),
