@@ -177,29 +177,38 @@ __device__ __forceinline__ void sm_find(SampleLds<NT> &m, int by_mass, u64 targe
   __syncthreads();
 }
 
-// The smallest key from -inf's to the top's at which in(l) holds, which does from there on.  A wavefront tries 64 at once.
+// The smallest keys from -inf's to the top's at which in(l, 0) and in(l, 1) hold, which do from there on.  A wavefront
+// tries 64 keys at once, for both.
 template <typename F>
-__device__ __forceinline__ uint32_t sm_border(const SampleRow &r, F in) {
+__device__ __forceinline__ void sm_borders(const SampleRow &r, F in, uint32_t (&from)[2]) {
   const uint32_t lane = threadIdx.x % 64;
-  uint32_t from = 0x007fffffu, n = r.top_key - from;   // it is one of from .. from + n
-  while (n) {
-    const uint32_t step = n / 64 + 1, mine = lane * step;
-    const u64 yes = __ballot(mine <= n && in(sm_value(from + mine)));
-    const uint32_t l = yes ? __ffsll((long long)yes) - 1 : n / step + 1;   // the first lane that it holds for, or past the last one tried
-    const uint32_t lower = l ? (l - 1) * step + 1 : 0, upper = yes ? l * step : n;
-    from += lower;
-    n = upper - lower;
+  uint32_t n[2];   // it is one of from .. from + n
+#pragma unroll
+  for (int h = 0; h < 2; ++h) {
+    from[h] = 0x007fffffu;
+    n[h] = r.top_key - from[h];
   }
-  return from;
+  while (n[0] | n[1])
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      const uint32_t step = n[h] / 64 + 1, mine = lane * step;
+      const u64 yes = __ballot(mine <= n[h] && in(sm_value(from[h] + mine), h));
+      const uint32_t l = yes ? __ffsll((long long)yes) - 1 : n[h] / step + 1;   // the first lane that it holds for, or past the last one tried
+      const uint32_t lower = l ? (l - 1) * step + 1 : 0, upper = yes ? l * step : n[h];
+      from[h] += lower;
+      n[h] = upper - lower;
+    }
 }
 // The logits of bin `bin`, from hi down to lo: bins rise with falling keys, so each is a range of them.
 __device__ __forceinline__ void sm_range(const SampleRow &r, int bin, float &lo, float &hi) {
-  lo = sm_value(sm_border(r, [&](float l) { return r.bin(l) <= bin; }));
-  hi = bin ? sm_value(sm_border(r, [&](float l) { return r.bin(l) < bin; }) - 1) : r.topf;
+  uint32_t from[2];
+  sm_borders(r, [&](float l, int h) { return r.bin(l) <= bin - (h && bin); }, from);
+  lo = sm_value(from[0]);
+  hi = bin ? sm_value(from[1] - 1) : r.topf;
 }
 // Gathers the elements of a range of logits; m.n counts them, the first kCandidates are kept.
 template <int NT, typename Each>
-__device__ __forceinline__ int sm_gather(SampleLds<NT> &m, const SampleRow &r, Each each, float lo, float hi) {
+__device__ __forceinline__ int sm_gather(SampleLds<NT> &m, Each each, float lo, float hi) {
   if (threadIdx.x == 0) m.n = 0;
   __syncthreads();
   each([&](uint32_t i, float l) {
@@ -210,27 +219,57 @@ __device__ __forceinline__ int sm_gather(SampleLds<NT> &m, const SampleRow &r, E
   __syncthreads();
   return m.n;
 }
-// The n gathered elements in falling order, by a bitonic network.
-template <int NT>
+// The first n of NT E elements in falling order, by a bitonic network: E consecutive ones a thread in registers, pairs of
+// one thread and (by lane exchanges) of one wavefront without LDS, so 1024 elements pass LDS in 3 of 55 steps.
+template <int NT, int E>
 __device__ __forceinline__ void sm_sort(u64 *place, int n) {
-  int P = 64;
+  int P = 64 * E;
   while (P < n) P *= 2;
-  for (int c = n + threadIdx.x; c < P; c += NT) place[c] = 0;   // below any element's
-  __syncthreads();
-  for (int k = 2; k <= P; k *= 2)
-    for (int d = k / 2; d; d /= 2) {
-      for (int e = threadIdx.x; e < P / 2; e += NT) {
-        const int x = 2 * e - (e & (d - 1)), y = x + d;
-        const u64 u = place[x], v = place[y];
-        if ((u < v) == !(x & k)) {
-          place[x] = v;
-          place[y] = u;
-        }
+  const int i0 = threadIdx.x * E;
+  const bool active = i0 < P;   // whole wavefronts
+  u64 v[E];
+#pragma unroll
+  for (int q = 0; q < E; ++q) v[q] = i0 + q < n ? place[i0 + q] : 0;   // 0: below any element
+  auto keep = [](u64 &x, u64 o, bool larger) { x = (x > o) == larger ? x : o; };
+  auto own = [&](int k) {   // the steps between a thread's elements, up to k / 2 apart
+#pragma unroll
+    for (int d = E / 2; d; d /= 2) {
+      if (d >= k) continue;
+#pragma unroll
+      for (int q = 0; q < E; ++q) {
+        if (q & d) continue;
+        const bool falling = !((i0 + q) & k);
+        const u64 x = v[q], y = v[q | d];
+        v[q] = (x > y) == falling ? x : y;
+        v[q | d] = (x > y) == falling ? y : x;
       }
-      // pairs 64 threads apart and less are the wavefront's own
-      if (d > 64 || (d == 1 && k >= 64)) __syncthreads();
-      else wave_lds_sync();
     }
+  };
+#pragma unroll
+  for (int k = 2; k < E; k *= 2) own(k);
+#pragma unroll 1
+  for (int k = E; k <= P; k *= 2) {
+#pragma unroll 1
+    for (int d = k / 2; d >= E; d /= 2) {
+      const bool larger = !(i0 & k) == !(i0 & d);
+      if (d < 64 * E) {
+        if (active)
+#pragma unroll
+          for (int q = 0; q < E; ++q) keep(v[q], __shfl_xor(v[q], d / E), larger);
+      } else {
+        __syncthreads();
+#pragma unroll
+        for (int q = 0; q < E; ++q) place[i0 + q] = v[q];
+        __syncthreads();
+#pragma unroll
+        for (int q = 0; q < E; ++q) keep(v[q], place[(i0 + q) ^ d], larger);
+      }
+    }
+    own(k);
+  }
+  __syncthreads();
+#pragma unroll
+  for (int q = 0; q < E; ++q) place[i0 + q] = v[q];
   __syncthreads();
 }
 // Of sorted elements the one at which the running sum of value(l, place) reaches `target` (1 .. the whole).
@@ -261,7 +300,20 @@ __device__ __forceinline__ u64 sm_reach(M &m, int n, u64 target, Value value) {
 template <int NT, typename Each, typename Value>
 __device__ __forceinline__ u64 sm_cut(SampleLds<NT> &m, Each each, float lo, float hi, int n, u64 target, bool ones, Value value) {
   if (n <= kCandidates) {
-    sm_sort<NT>(m.place, n);
+    if (n <= 256) {   // each element's rank by comparing it with all: 0.7 us for 100 where the network takes 4.6
+      u64 mine = 0;
+      int rank = 0;
+      if ((int)threadIdx.x < n) {
+        mine = m.place[threadIdx.x];
+#pragma unroll 8
+        for (int o = 0; o < n; ++o) rank += m.place[o] > mine;
+      }
+      __syncthreads();
+      if ((int)threadIdx.x < n) m.place[rank] = mine;
+      __syncthreads();
+    } else {
+      sm_sort<NT, kCandidates / NT>(m.place, n);
+    }
     if (ones) return m.place[target - 1];
     return sm_reach<NT>(m, n, target, value);
   }
@@ -314,7 +366,7 @@ __device__ __forceinline__ u64 sm_select(SampleLds<NT> &m, const SampleRow &r, c
     __syncthreads();
     if (bin != have) {
       sm_range(r, bin, lo, hi);
-      n = sm_gather<NT>(m, r, each, lo, hi);
+      n = sm_gather<NT>(m, each, lo, hi);
       have = bin;
     }
     u64 save[kBins / NT];   // cutting by digits takes the histogram's place
@@ -347,7 +399,9 @@ __device__ __forceinline__ u64 sm_select(SampleLds<NT> &m, const SampleRow &r, c
 // The cut with min_p: the smallest key that it keeps, at any index.
 __device__ __forceinline__ u64 sm_min_p(const SampleRow &r, u64 cut, u64 first) {
   if (r.lowest == -INFINITY) return cut;
-  const u64 lowest = (u64)sm_border(r, [&](float l) { return r.z(l) >= r.lowest; }) << 32;
+  uint32_t from[2];
+  sm_borders(r, [&](float l, int) { return r.z(l) >= r.lowest; }, from);
+  const u64 lowest = (u64)from[0] << 32;
   cut = cut > lowest ? cut : lowest;
   return cut < first ? cut : first;   // the first stays
 }
@@ -464,7 +518,7 @@ __global__ void __launch_bounds__(256) k_sample_short(const SampleParams p) {
     for (int q = 0; q < per; ++q) at[q] = t * per + q < V ? m.place[t * per + q] : 0;
     __syncthreads();
     if (s.k > 1 || s.top_p < 1) {
-      sm_sort<NT>(m.place, V);
+      sm_sort<NT, per>(m.place, V);
       const int n = s.k > 1 ? (int)s.k : V;
       cut = m.place[n - 1];
       if (s.top_p < 1) {
@@ -690,16 +744,24 @@ __global__ void __launch_bounds__(NT) k_sample_cut(const SampleParams p) {
     __syncthreads();
     auto each = [&](auto f) {
       constexpr int64_t stride = NT * kE;
-      for (int64_t i0 = (int64_t)threadIdx.x * kE; i0 < V; i0 += 4 * stride) {   // four loads under way together
-        float v[4][kE];
+      constexpr int U = 16 / sizeof(IT);   // loads under way together: 32 registers
+      struct Raw { IT e[kE]; };
+#pragma unroll 1
+      for (int64_t i0 = (int64_t)threadIdx.x * kE; i0 < V; i0 += U * stride) {
+        Raw raw[U];
 #pragma unroll
-        for (int j = 0; j < 4; ++j)
-          if (i0 + j * stride < V) sm_load<IT>(logits, i0 + j * stride, V, v[j]);
+        for (int j = 0; j < U; ++j)
+          if (i0 + j * stride + kE <= V) __builtin_memcpy(&raw[j], logits + i0 + j * stride, sizeof(Raw));
 #pragma unroll
-        for (int j = 0; j < 4; ++j)
+        for (int j = 0; j < U; ++j) {
+          const int64_t i = i0 + j * stride;
+          if (i >= V) break;
+          if (i + kE > V)
+            for (int q = 0; q < kE; ++q) raw[j].e[q] = logits[i + q < V ? i + q : V - 1];
 #pragma unroll
           for (int q = 0; q < kE; ++q)
-            if (i0 + j * stride + q < V) f((uint32_t)(i0 + j * stride + q), v[j][q]);
+            if (i + q < V) f((uint32_t)(i + q), to_f32(raw[j].e[q]));
+        }
       }
     };
     cut = sm_select<NT>(m, r, s, each);
@@ -799,8 +861,6 @@ static hipError_t sample_t(SampleParams p, hipStream_t s) {
   for (; p.first < p.R; p.first += most) {
     const dim3 grid((unsigned)(p.R - p.first < most ? p.R - p.first : most));
     if (p.V <= kShort) hipLaunchKernelGGL((k_sample_short<IT>), grid, dim3(256), 0, s, p);
-    else if (p.V <= 2048) hipLaunchKernelGGL((k_sample_row<IT, 256, 1>), grid, dim3(256), 0, s, p);
-    else if (p.V <= 8192) hipLaunchKernelGGL((k_sample_row<IT, 1024, 1>), grid, dim3(1024), 0, s, p);
     else hipLaunchKernelGGL((k_sample_row<IT, 1024, 4>), grid, dim3(1024), 0, s, p);
   }
   return hipGetLastError();
