@@ -12,8 +12,14 @@
 // in; the elements of that bin (some hundred) are gathered and sorted in LDS.  A bin of more than kCandidates is cut
 // by digits of (key, index) instead, 11 bits a pass.  What min_p leaves out is a range of keys, so it only moves the cut.
 //
-// A row of up to 32768 logits is one workgroup's from the maximum to the token.  Longer ones
-// are walked by a workgroup a chunk, in five launches: maxima, histograms, cut (a workgroup a row), kept masses, token.
+// A row of up to 32768 logits is one workgroup's from the maximum to the token.  Longer ones are walked by a workgroup a
+// chunk, in five launches: maxima, histograms, cut (a workgroup a row), kept masses, token.  One workgroup against five
+// launches, top_p, us: 64 x 8192 34 against 52, 64 x 16384 40 against 56, 64 x 32768 51 against 64 (1 x 32768, all kept, 23
+// against 21).
+//
+// What bounds it is latency: a chain of passes over a row with barriers between them, by few workgroups.  64 rows of 131072
+// in bf16 are 16.8 MB (3.3 us at 5 TB/s); top_k 40 and top_p 0.9 take 104 us, most of it in the cut's kernel, whose
+// workgroup gathers twice from its whole row.  A row of 256 takes 4.8 us with all kept, the launch itself, and 11 with top_p.
 #include <type_traits>
 
 #include "ssm_device.hpp"
@@ -447,7 +453,7 @@ __device__ __forceinline__ void sm_tile(const SampleParams &p, int64_t row, cons
   tile = tiles - 1;   // not reached: the sums end at the total
 }
 __device__ __forceinline__ float sm_logprob(const SampleRow &r, float l, u64 total) {
-  return (float)(r.z(l) - (log((double)total) - r.shift * 0.6931471805599453));
+  return (float)(r.z(l) - log(ldexp((double)total, -r.shift)));   // 0 where the token is all that is kept
 }
 // One wavefront: the token, in the tile whose logits its lanes hold.
 __device__ __forceinline__ void sm_pick(const SampleParams &p, const SampleRow &r, int64_t row, const SampleCut &cut, int64_t i, const float (&v)[kE],
@@ -474,6 +480,7 @@ __device__ __forceinline__ void sm_pick(const SampleParams &p, const SampleRow &
 
 // ------------------------------------------------------------------ short rows
 // Up to kShort logits: the whole row is sorted, and nothing is unrolled (see sm_select).
+// 64 rows of 1000, top_p 19 us against 30 in k_sample_row, which holds more than a short row needs; all kept 5.7 against 17.
 constexpr int kShort = 1024;
 template <typename IT>
 __global__ void __launch_bounds__(256) k_sample_short(const SampleParams p) {

@@ -227,3 +227,10 @@ def test_crowded_bins(dev, V):
     u = torch.rand(6, generator=g).to(dev)
     for kw in (dict(top_k=V // 2 + 3), dict(top_p=0.6), dict(top_k=V - 100, top_p=0.5), dict(top_k=1200), dict(top_k=V // 2, temperature=1e3)):
         check(logits, u, **kw)
+
+
+@pytest.mark.parametrize("V", [30, 1000, 3000, 20000, 33000, 131072])
+def test_a_token_that_is_all_that_is_kept(dev, V):   # its probability is 1, whatever the weights' scale
+    logits, u = make(dev, 3, V, F32, seed=V)
+    for kw in (dict(top_k=1), dict(temperature=0.0), dict(top_k=1, temperature=0.6, top_p=0.5, min_p=0.05)):
+        assert (ssm_scan.sample(logits, u, **kw)[1] == 0).all()
