@@ -376,7 +376,9 @@ struct RnormParams {
   int nblk;
   int64_t first;                       // forward: rows of earlier launches
 };
-// Wavefronts a row: the fewest that hold it in 4 loads a lane; where there are few rows, more of them.
+// Wavefronts a row: the fewest that hold it in 4 loads a lane; where there are few rows, more of them.  Forward in bf16,
+// 1 / 4 / 16 a row, us: 64 x 2048 7.6 / 5.4 / 5.5, 512 x 2048 8.0 / 6.1 / 6.9, 4096 x 2048 15.1 / 15.9 / 23, 16384 x 1024
+// 25 / 28 / 69.
 inline int rnorm_waves(int64_t R, int64_t C, int V) {
   const int64_t least = C <= 256 * V ? 1 : C <= 1024 * V ? 4 : 16;
   if (R < 1024 && least == 1 && C > 64 * V) return 4;

@@ -386,7 +386,7 @@ __device__ __forceinline__ void lin_row(const T *row, int64_t k, int64_t K, int 
 }
 template <typename T, typename OT, int MT, int NT>
 __global__ void __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2, 2))) k_linear_rows(const GemmParams p) {
-  constexpr int F = Mma<T>::bytes / 4, KE = 4 * Mma<T>::bytes / sizeof(T), U = sizeof(T) == 1 && MT * NT == 8 ? 2 : 4;   // steps whose loads are under way together
+  constexpr int F = Mma<T>::bytes / 4, KE = 4 * Mma<T>::bytes / sizeof(T), U = 4;   // steps whose loads are under way together
   __shared__ __attribute__((aligned(16))) float red[8][MT * 16][NT * 16 + 4];
   const int lane = threadIdx.x % 64, wave = threadIdx.x / 64, g = lane / 16;
   const uint32_t nb = (uint32_t)((p.N + 16 * NT - 1) / (16 * NT)), split = blockIdx.x / nb;
@@ -519,22 +519,43 @@ LinearPlan linear_plan(const GemmParams &p) {
   const int e = p.fp8 ? 1 : 2;
   const int64_t unit = 16 / e;
   auto up = [&](int64_t n) { return (n + unit - 1) / unit * unit; };
-  if (p.a_along && p.b_along && p.M <= 64) {
+  // Up to 32 rows go to k_linear_rows: 1 x 8192 x 2048 in bf16 7.6 us against 11.9 in tiles, 16 rows 9.0 against 12.3, 32
+  // 11.0 against 13.1 (64: 14.8 against 14.5).  Tiles are as fast or faster where the weights are more than 48 MB (16 x
+  // 16384 x 4096: 25 us against 30) or of many rows (1 x 32768 x 1024: 14.7 against 17.8, e4m3 9.8 against 13.0), unless
+  // they would have to be copied first.
+  const bool b_loads = loadable(p.B, p.sb, p.b_along ? p.K : p.N, e);
+  if (p.a_along && p.b_along && p.M <= 32 && ((p.N * p.K * e <= 48 << 20 && p.N < 32768) || !b_loads)) {
     l.rows = 1;
-    l.MT = p.M <= 16 ? 1 : p.M <= 32 ? 2 : 4;
-    l.NT = p.N >= 16 * 4 * 512 && l.MT < 4 ? 4 : p.N >= 16 * 2 * 256 ? 2 : 1;
+    l.MT = p.M <= 16 ? 1 : 2;
+    // weight rows of a workgroup: 16 where 32 would leave compute units without one (1 x 2048 x 2048: 5.4 us against 7.1),
+    // 32 beyond (1 x 8192 x 2048: 7.6 against 9.1)
+    l.NT = p.N >= 16 * 2 * 256 ? 2 : 1;
     const int64_t nb = (p.N + 16 * l.NT - 1) / (16 * l.NT), steps = p.K * e / 64;
-    l.splits = 1;   // more where few workgroups would each walk a long k: 16 steps a wavefront at least
+    // k is split where few workgroups would each walk a long one, 16 steps a wavefront at least: 1 x 1024 x 16384 14.5 us
+    // against 20.6, 16 x 1024 x 8192 12.5 against 17.1
+    l.splits = 1;
     while (nb * l.splits < 128 && steps / (8 * l.splits * 2) >= 16) l.splits *= 2;
   } else {
     if (!loadable(p.A, p.sa, p.a_padded ? unit : p.a_along ? p.K : p.M, e)) l.pack_a = p.a_along ? p.M * up(p.K) * e : p.K * up(p.M) * e;
-    if (!loadable(p.B, p.sb, p.b_along ? p.K : p.N, e)) l.pack_b = p.b_along ? p.N * up(p.K) * e : p.K * up(p.N) * e;
+    if (!b_loads) l.pack_b = p.b_along ? p.N * up(p.K) * e : p.K * up(p.N) * e;
     auto tiles = [&](int64_t t) { return ((p.M + t - 1) / t) * ((p.N + t - 1) / t); };
     const int64_t steps = (p.K * e + 127) / 128;
-    // the largest tiles that occupy three quarters of the compute units
+    // The largest tiles that occupy three quarters of the compute units.  In us, tiles of 256 / 128 / 64, bf16:
+    // 8192 x 8192 x 2048 228 / 261 / 367, 3584 x 3584 x 1024 (196 tiles of 256) 31 / 37 / 46, 2048 x 4096 x 1024 (128 of
+    // them) 29 / 23 / 29, 2048 x 2048 x 1024 28 / 15 / 16, 1024 x 1024 x 1024 26 / 13 / 8; e4m3 4096 x 4096 x 4096 61 / 73 / 103.
     l.tile = tiles(256) >= 192 ? 256 : tiles(128) >= 192 ? 128 : 64;
-    l.splits = 1;   // up to two workgroups a compute unit, 8 steps each at least
-    while (l.tile == 64 && tiles(64) * l.splits * 2 <= 512 && steps / (l.splits * 2) >= 8) l.splits *= 2;
+    // Small tiles split k, up to two workgroups a compute unit and 8 steps each at least, by what it saves (0.3 us a step,
+    // 0.5 where no two tiles share a long operand's rows) less what the join costs (4 us and a write and a read of the sums):
+    // 128 x 1024 x 4096 11.3 us against 18.9 whole, 512 x 1024 x 8192 23.4 against 55, 1024 x 1024 x 4096 23.1 against 30.3,
+    // e4m3 64 x 8192 x 4096 13.7 against 20.2, but 1024 x 1024 x 2048 17.4 against 11.8.
+    l.splits = 1;
+    const float step = p.M <= 64 || p.N <= 64 ? 0.5f : 0.3f;
+    float best = 0;
+    if (l.tile == 64)
+      for (int64_t s = 2; tiles(64) * s <= 512 && steps / s >= 8; s *= 2) {
+        const float saved = step * steps * (s - 1) / s - 4 - (float)(p.M * p.N * s) / 6e5f;
+        if (saved > best) best = saved, l.splits = s;
+      }
   }
   l.pack_a = (l.pack_a + 255) / 256 * 256;
   l.pack_b = (l.pack_b + 255) / 256 * 256;
@@ -559,11 +580,6 @@ static void tile_v(const GemmParams &p, const LinearPlan &l, hipStream_t s) {
 template <typename T, typename OT, int MT>
 static void rows_v(const GemmParams &p, const LinearPlan &l, hipStream_t s) {
   const dim3 grid((unsigned)((p.N + 16 * l.NT - 1) / (16 * l.NT) * l.splits));
-  if constexpr (MT < 4)
-    if (l.NT == 4) {
-      hipLaunchKernelGGL((k_linear_rows<T, OT, MT, 4>), grid, dim3(512), 0, s, p);
-      return;
-    }
   if (l.NT == 2) hipLaunchKernelGGL((k_linear_rows<T, OT, MT, 2>), grid, dim3(512), 0, s, p);
   else hipLaunchKernelGGL((k_linear_rows<T, OT, MT, 1>), grid, dim3(512), 0, s, p);
 }
@@ -575,8 +591,7 @@ static hipError_t gemm_t(GemmParams p, void *workspace, hipStream_t s) {
   p.partial = (float *)(ws + l.pack_a + l.pack_b);
   if (l.rows) {
     if (l.MT == 1) rows_v<T, OT, 1>(p, l, s);
-    else if (l.MT == 2) rows_v<T, OT, 2>(p, l, s);
-    else rows_v<T, OT, 4>(p, l, s);
+    else rows_v<T, OT, 2>(p, l, s);
   } else {
     constexpr int64_t unit = 16 / sizeof(T);
     auto packed = [&](const void *&data, int64_t &stride, char *to, int64_t rows, int64_t cols) {
