@@ -959,6 +959,34 @@ Tensor embed_forward(const Tensor &tokens, const Tensor &weight, double scale, a
   l.run_anywhere("ssm_embed_fwd", ssm_embed_fwd, a);
   return o;
 }
+Tensor embed_backward(const Tensor &dout, const Tensor &tokens, double scale, int64_t V) {
+  const int64_t D = dout.size(-1);
+  const Tensor dy = rows(dout, D), dw = at::empty({V, D}, dy.options());
+  ssm_embed_args a = embed_args(tokens, V, D, dy.scalar_type(), scale);
+  a.dout = view(dy);
+  a.dweight = dw.data_ptr();
+  SSM_BYTES(n, ssm_embed_workspace_bytes, ssm_embed_check, a, "ssm_embed_bwd");
+  const Tensor ws = bytes(n, dy);
+  a.workspace = ws.data_ptr();
+  a.workspace_bytes = n;
+  const Launch l(dy);
+  l.run_anywhere("ssm_embed_bwd", ssm_embed_bwd, a);
+  return dw;
+}
+Tensor embed_node(const Tensor &weight, const Tensor &tokens, double scale, at::IntArrayRef shape);
+// The gradient as a node of its own, for derivatives of it: linear in dout, its adjoint is the embedding.
+struct EmbedGradFn : torch::autograd::Function<EmbedGradFn> {
+  static Tensor forward(AutogradContext *ctx, const Tensor &dout, const Tensor &tokens, double scale, int64_t V) {
+    ctx->save_for_backward({tokens});
+    ctx->saved_data["scale"] = scale;
+    ctx->saved_data["shape"] = dout.sizes().vec();
+    return embed_backward(dout, tokens, scale, V);
+  }
+  static variable_list backward(AutogradContext *ctx, variable_list grads) {
+    const std::vector<int64_t> shape = ctx->saved_data["shape"].toIntVector();
+    return {embed_node(grads[0], ctx->get_saved_variables()[0], ctx->saved_data["scale"].toDouble(), shape), Tensor(), Tensor(), Tensor()};
+  }
+};
 struct EmbedFn : torch::autograd::Function<EmbedFn> {
   static Tensor forward(AutogradContext *ctx, const Tensor &weight, const Tensor &tokens, double scale, at::IntArrayRef shape) {
     ctx->save_for_backward({tokens});
@@ -968,22 +996,15 @@ struct EmbedFn : torch::autograd::Function<EmbedFn> {
   }
   static variable_list backward(AutogradContext *ctx, variable_list grads) {
     const Tensor tokens = ctx->get_saved_variables()[0];
-    const int64_t V = ctx->saved_data["vocab"].toInt(), D = grads[0].size(-1);
-    const Tensor dy = rows(grads[0], D), dw = at::empty({V, D}, dy.options());
-    ssm_embed_args a = embed_args(tokens, V, D, dy.scalar_type(), ctx->saved_data["scale"].toDouble());
-    a.dout = view(dy);
-    a.dweight = dw.data_ptr();
-    SSM_BYTES(n, ssm_embed_workspace_bytes, ssm_embed_check, a, "ssm_embed_bwd");
-    const Tensor ws = bytes(n, dy);
-    a.workspace = ws.data_ptr();
-    a.workspace_bytes = n;
-    const Launch l(dy);
-    l.run_anywhere("ssm_embed_bwd", ssm_embed_bwd, a);
-    variable_list d{dw, Tensor(), Tensor(), Tensor()};
-    not_twice(d, grads, "embedding");
-    return d;
+    const int64_t V = ctx->saved_data["vocab"].toInt();
+    const double scale = ctx->saved_data["scale"].toDouble();
+    return {needs_grad({&grads[0]}) ? EmbedGradFn::apply(grads[0], tokens, scale, V) : embed_backward(grads[0], tokens, scale, V),
+            Tensor(), Tensor(), Tensor()};
   }
 };
+Tensor embed_node(const Tensor &weight, const Tensor &tokens, double scale, at::IntArrayRef shape) {
+  return EmbedFn::apply(weight, tokens, scale, shape);
+}
 Tensor embedding(const Tensor &tokens, const Tensor &weight, double scale) {
   require_gpu({&tokens, &weight});
   one_device(weight, {&tokens});

@@ -11,6 +11,6 @@ def embedding(tokens, weight, scale=1.0):
     """scale * weight[tokens], (..., C) in weight's type.
 
     tokens (...): integers; a token outside [0, vocabulary), as -1 for padding, gives a row of zeros and no
-    gradient.  weight (vocabulary, C) float32, bfloat16 or float16.  Differentiable (once, reverse mode) in weight; the gradient is
-    dense, summed in float32."""
+    gradient.  weight (vocabulary, C) float32, bfloat16 or float16.  Differentiable (reverse mode) in weight, any number
+    of times; the gradient is dense, summed in float32, of fewer than 2^27 tokens."""
     return _abi.host().embedding(tokens, weight, float(scale))

@@ -16,6 +16,7 @@ own on the matrix cores, with bias, activation and residual in their epilogue.
 
 import torch
 import torch.nn.functional as F
+from torch.autograd import forward_ad
 
 from . import _abi
 from .embed import embedding as scaled_embedding
@@ -122,6 +123,7 @@ def linear_8bit(q, scale, weight, weight_scale, bias=None, activation=None, resi
     return _abi.host().linear_8bit(q, scale, weight, weight_scale, bias, residual, _activation(activation), dtype)
 
 
+MAX_SORTED = 1 << 27    # rows and tokens of the sorted gradient
 _SORTED_TYPES = (torch.float32, torch.bfloat16, torch.float16)
 MAX_DENSE_VOCAB = 4096  # vocabularies up to this size take the one-hot product
 
@@ -150,13 +152,15 @@ def embedding(layer, idx):
     sizes it reads back on the host -- this one makes no host reads, so a training step that
     contains it can be captured in a HIP graph, and it runs in a fixed order.  Trained with a larger vocabulary, or in
     16 bits, it is ssm_scan.embedding, which sorts on the GPU and has the same properties (ids outside the vocabulary,
-    at which nn.Embedding ends the process, give zeros there)."""
+    at which nn.Embedding ends the process, give zeros there; nn.Embedding itself from 2^27 rows or tokens on and in
+    forward mode)."""
     w = layer.weight
     plain = (layer.padding_idx is None and layer.max_norm is None and not layer.scale_grad_by_freq
              and not layer.sparse)
     if (plain and torch.is_grad_enabled() and w.requires_grad and w.dtype == torch.float32
             and w.shape[0] <= MAX_DENSE_VOCAB and not torch.is_autocast_enabled(w.device.type)):
         return _DenseGradEmbedding.apply(idx, w)
-    if plain and torch.is_grad_enabled() and w.requires_grad and w.is_cuda and w.dtype in _SORTED_TYPES:
+    if (plain and torch.is_grad_enabled() and w.requires_grad and w.is_cuda and w.dtype in _SORTED_TYPES
+            and max(w.shape[0], idx.numel()) < MAX_SORTED and forward_ad._current_level < 0):
         return scaled_embedding(idx, w)
     return layer(idx)

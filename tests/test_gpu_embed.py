@@ -11,6 +11,7 @@ import torch
 
 from oracle import token_ref
 import ssm_scan
+from ssm_scan import linear
 
 pytestmark = pytest.mark.gpu
 
@@ -130,6 +131,37 @@ def test_refusals_and_no_tokens(dev):
     leaf = w.clone().requires_grad_()
     e = ssm_scan.embedding(t[:0].reshape(2, 0), leaf)
     assert e.shape == (2, 0, 16) and not torch.autograd.grad(e.sum(), leaf)[0].any()
-    g, = torch.autograd.grad(ssm_scan.embedding(t, leaf).sum(), leaf, create_graph=True)
-    with pytest.raises(RuntimeError, match="twice"):
-        g.sum().backward()
+
+
+@pytest.mark.parametrize("V,n", [(10, 60), (5000, 300)])
+def test_derivatives_of_the_gradient(dev, V, n):
+    """Of sum of out^3: the terms of a row and channel are alike, so n additions and fewer than 16 other roundings of
+    float32 are off by n + 16 halves of its step, relative to the result."""
+    tokens, w, _ = make(dev, n, V, 24, F32, "uniform", seed=6)
+    tokens, r = tokens.clamp(0, V - 1), torch.randn(V, 24, generator=torch.Generator().manual_seed(7)).to(dev)
+
+    def twice(call, w, r):
+        leaf = w.detach().requires_grad_()
+        g, = torch.autograd.grad((call(leaf) ** 3).sum(), leaf, create_graph=True)
+        return torch.autograd.grad((g * r).sum(), leaf)[0]
+
+    want = twice(lambda leaf: 1.5 * leaf[tokens], w.double(), r.double())
+    layer = torch.nn.Embedding(V, 24).to(dev)
+    layer.weight = torch.nn.Parameter(w.detach())
+    got = twice(lambda leaf: ssm_scan.embedding(tokens, leaf, 1.5), w, r)
+    assert ((got - want).abs() <= (n + 16) * 2.0 ** -24 * want.abs()).all()
+    if V > 4096:   # a layer of a model
+        g, = torch.autograd.grad((linear.embedding(layer, tokens) ** 3).sum(), layer.weight, create_graph=True)
+        got, = torch.autograd.grad((g * r).sum(), layer.weight)
+        assert ((1.5 ** 3 * got - want).abs() <= (n + 18) * 2.0 ** -24 * want.abs()).all()
+
+
+def test_forward_mode_of_a_layer(dev):
+    layer = torch.nn.Embedding(5000, 16).to(dev)
+    tokens, tangent = torch.arange(40, device=dev), torch.randn(5000, 16, device=dev)
+    with torch.autograd.forward_ad.dual_level():
+        w = torch.autograd.forward_ad.make_dual(layer.weight.detach(), tangent).requires_grad_()
+        del layer.weight
+        layer.weight = w
+        out = torch.autograd.forward_ad.unpack_dual(linear.embedding(layer, tokens))
+    assert torch.equal(out.tangent, tangent[:40])
