@@ -1695,7 +1695,8 @@ struct SampleLayout {
 SampleLayout sample_layout(const ssm_sample_args *a) {
   SampleLayout l{};
   if (a->vocab <= kSampleRow) return l;
-  l.chunk = a->rows * cdiv(a->vocab, kSampleRow) >= 64 ? kSampleRow : kSampleRow / 4;   // small chunks where there are few: 8 x 50000 59 us against 63, 64 x 131072 103 against 98
+  // small chunks where there are few: 8 x 50000 59 us against 63, 64 x 131072 103 against 98
+  l.chunk = a->rows * cdiv(a->vocab, kSampleRow) >= 64 ? kSampleRow : kSampleRow / 4;
   l.chunks = cdiv(a->vocab, l.chunk);
   l.parts = cdiv(a->vocab, 8192);
   l.ntiles = cdiv(a->vocab, 512);
