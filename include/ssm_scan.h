@@ -584,6 +584,8 @@ int64_t ssm_embed_workspace_bytes(const ssm_embed_args *args);   /* backward */
 int64_t ssm_linear_workspace_bytes(const ssm_linear_args *args);
 int64_t ssm_linear_bwd_workspace_bytes(const ssm_linear_args *args);
 int64_t ssm_sample_workspace_bytes(const ssm_sample_args *args);
+/* Rows and columns of the tiles that ssm_linear_fwd takes (host-only): 256, 128 or 64; 0 for its kernel for few rows. */
+int64_t ssm_linear_tile(const ssm_linear_args *args);
 int64_t ssm_decode_stack_workspace_bytes(const ssm_decode_stack_args *args);
 /* Byte offset inside the decode-stack workspace of an int32 status word: ssm_decode_stack sets
  * it to 1 when a token id lies outside [0, vocab) (the reference's nn.Embedding,

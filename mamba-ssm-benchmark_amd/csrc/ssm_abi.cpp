@@ -1640,6 +1640,10 @@ int64_t ssm_linear_workspace_bytes(const ssm_linear_args *a) {
   if (ssm_linear_check(a)) return -1;
   return linear_plan(linear_forward_params(a)).bytes();
 }
+int64_t ssm_linear_tile(const ssm_linear_args *a) {
+  if (ssm_linear_check(a)) return -1;
+  return linear_plan(linear_forward_params(a)).tile;
+}
 int64_t ssm_linear_bwd_workspace_bytes(const ssm_linear_args *a) {
   if (ssm_linear_check(a)) return -1;
   return linear_backward_plan(a).bytes();

@@ -456,7 +456,7 @@ struct GemmParams {
 };
 struct LinearPlan {
   int rows, MT, NT;                    // the kernel for few rows, of 16 MT rows and 16 NT columns a workgroup
-  int tile, splits;                    // else tiles of tile x tile
+  int tile, splits;                    // else tiles of tile x tile (0 with rows)
   int64_t pack_a, pack_b, partial;     // workspace bytes: operands that are copied into whole rows, sums of the splits
   int64_t bytes() const { return pack_a + pack_b + partial; }
 };

@@ -523,21 +523,34 @@ __global__ void __launch_bounds__(256) k_linear_dbias(const LinearDzParams p) {
 }
 
 // ------------------------------------------------------------------ plan and launch
-static bool loadable(const void *data, int64_t stride, int64_t row, int e) {   // 16 bytes a lane, 32-bit offsets
-  return (uintptr_t)data % 16 == 0 && stride * e % 16 == 0 && row * e % 16 == 0 && stride >= 0 && stride * e < (1 << 22);
+static bool loadable(const void *data, int64_t stride, int64_t row, int e, int64_t reach) {   // 16 bytes a lane
+  return (uintptr_t)data % 16 == 0 && stride * e % 16 == 0 && row * e % 16 == 0 && stride >= 0 && stride * e <= reach;
 }
+// The longest row in bytes whose `rows` fit the descriptor of a tile's loads, 2^31 - 1 bytes: what lies past that comes as
+// zeros.  The last row's loads end within 512 bytes of its first one's begin.
+static int64_t linear_reach(int64_t rows) { return (0x7fffffff - 512) / (rows - 1); }
 LinearPlan linear_plan(const GemmParams &p) {
   LinearPlan l{};
   const int e = p.fp8 ? 1 : 2;
   const int64_t unit = 16 / e;
   auto up = [&](int64_t n) { return (n + unit - 1) / unit * unit; };
+  auto tiles = [&](int64_t t) { return ((p.M + t - 1) / t) * ((p.N + t - 1) / t); };
+  // The largest tiles that occupy three quarters of the compute units.  In us, tiles of 256 / 128 / 64, bf16:
+  // 8192 x 8192 x 2048 228 / 261 / 367, 3584 x 3584 x 1024 (196 tiles of 256) 31 / 37 / 46, 2048 x 4096 x 1024 (128 of
+  // them) 29 / 23 / 29, 2048 x 2048 x 1024 28 / 15 / 16, 1024 x 1024 x 1024 26 / 13 / 8; e4m3 4096 x 4096 x 4096 61 / 73 / 103.
+  l.tile = tiles(256) >= 192 ? 256 : tiles(128) >= 192 ? 128 : 64;
+  // Smaller ones where whole rows along k (copied ones too) are longer than theirs may be: from 4.2 million channels on in
+  // 16 bits.  Tiles of 64 take the longest there are, 2^24 channels; of a transposed operand every tile has 64 rows.
+  while (l.tile > 64 && (p.a_along || p.b_along) && up(p.K) * e > linear_reach(l.tile)) l.tile /= 2;
+  const int64_t reach_a = linear_reach(p.a_along ? l.tile : 64), reach_b = linear_reach(p.b_along ? l.tile : 64);
   // Up to 32 rows go to k_linear_rows: 1 x 8192 x 2048 in bf16 7.6 us against 11.9 in tiles, 16 rows 9.0 against 12.3, 32
   // 11.0 against 13.1 (64: 14.8 against 14.5).  Tiles are as fast or faster where the weights are more than 48 MB (16 x
   // 16384 x 4096: 25 us against 30) or of many rows (1 x 32768 x 1024: 14.7 against 17.8, e4m3 9.8 against 13.0), unless
   // they would have to be copied first.
-  const bool b_loads = loadable(p.B, p.sb, p.b_along ? p.K : p.N, e);
+  const bool b_loads = loadable(p.B, p.sb, p.b_along ? p.K : p.N, e, reach_b);
   if (p.a_along && p.b_along && p.M <= 32 && ((p.N * p.K * e <= 48 << 20 && p.N < 32768) || !b_loads)) {
     l.rows = 1;
+    l.tile = 0;
     l.MT = p.M <= 16 ? 1 : 2;
     // weight rows of a workgroup: 16 where 32 would leave compute units without one (1 x 2048 x 2048: 5.4 us against 7.1),
     // 32 beyond (1 x 8192 x 2048: 7.6 against 9.1)
@@ -548,14 +561,9 @@ LinearPlan linear_plan(const GemmParams &p) {
     l.splits = 1;
     while (nb * l.splits < 128 && steps / (8 * l.splits * 2) >= 16) l.splits *= 2;
   } else {
-    if (!loadable(p.A, p.sa, p.a_padded ? unit : p.a_along ? p.K : p.M, e)) l.pack_a = p.a_along ? p.M * up(p.K) * e : p.K * up(p.M) * e;
+    if (!loadable(p.A, p.sa, p.a_padded ? unit : p.a_along ? p.K : p.M, e, reach_a)) l.pack_a = p.a_along ? p.M * up(p.K) * e : p.K * up(p.M) * e;
     if (!b_loads) l.pack_b = p.b_along ? p.N * up(p.K) * e : p.K * up(p.N) * e;
-    auto tiles = [&](int64_t t) { return ((p.M + t - 1) / t) * ((p.N + t - 1) / t); };
     const int64_t steps = (p.K * e + 127) / 128;
-    // The largest tiles that occupy three quarters of the compute units.  In us, tiles of 256 / 128 / 64, bf16:
-    // 8192 x 8192 x 2048 228 / 261 / 367, 3584 x 3584 x 1024 (196 tiles of 256) 31 / 37 / 46, 2048 x 4096 x 1024 (128 of
-    // them) 29 / 23 / 29, 2048 x 2048 x 1024 28 / 15 / 16, 1024 x 1024 x 1024 26 / 13 / 8; e4m3 4096 x 4096 x 4096 61 / 73 / 103.
-    l.tile = tiles(256) >= 192 ? 256 : tiles(128) >= 192 ? 128 : 64;
     // Small tiles split k, up to two workgroups a compute unit and 8 steps each at least, by what it saves (0.3 us a step,
     // 0.5 where no two tiles share a long operand's rows) less what the join costs (4 us and a write and a read of the sums):
     // 128 x 1024 x 4096 11.3 us against 18.9 whole, 512 x 1024 x 8192 23.4 against 55, 1024 x 1024 x 4096 23.1 against 30.3,

@@ -265,6 +265,7 @@ _SIGS = {
     "ssm_sample_check": (c_i32, [ctypes.POINTER(SampleArgs)]),
     "ssm_sample_workspace_bytes": (c_i64, [ctypes.POINTER(SampleArgs)]),
     "ssm_sample": (c_i32, [ctypes.POINTER(SampleArgs), c_vp]),
+    "ssm_linear_tile": (c_i64, [ctypes.POINTER(LinearArgs)]),
     "ssm_linear_bwd_workspace_bytes": (c_i64, [ctypes.POINTER(LinearArgs)]),
     "ssm_cscan_tile": (c_i64, [c_i32, c_i32]),
     "ssm_default_chunk": (c_i64, [c_i64]),

@@ -1,0 +1,44 @@
+"""CPU tier of the operators around the mixers at the ends of their ranges: the linear layer's plan where rows are long, the
+checks that come before anything reaches the device."""
+
+import ctypes
+import math
+
+import pytest
+import torch
+import torch.nn as nn
+
+from oracle import token_ref
+from ssm_scan import _abi, linear
+from test_token_cpu import embed, rnorm
+
+
+def product(m, n, k, in8=0, stride=None):
+    t = _abi.Tensor(4096, (ctypes.c_int64 * 3)(stride or k, 1, 0))
+    return _abi.LinearArgs(m=m, n=n, k=k, dtype=_abi.BF16, x=t, weight=t, in8=in8, x_scale=4096, weight_scale=4096)
+
+
+@pytest.mark.parametrize("in8", [0, 1])
+def test_tiles_of_long_rows_stay_within_32_bits(in8):
+    """A tile's loads take offsets below 2^31 from its first row, whether the rows are read in place or copied."""
+    lib, seen, e = _abi.lib(), set(), 1 if in8 else 2
+    for k in [1 << b for b in range(10, 25)] + [4210000, 4210752, 4300000, 5160000, 8454000, 8500000, 16777208]:
+        for m, n in [(40, 1 << 10), (64, 64), (1000, 1000), (1024, 1024), (1800, 1800), (2040, 2040), (3331, 3331), (3584, 3584), (8192, 8192), (3400, 4080)]:
+            if max(m, n) * k > 1 << 34:
+                continue
+            tile = lib.ssm_linear_tile(ctypes.byref(product(m, n, k, in8)))
+            assert tile in (0, 64, 128, 256)
+            if tile:
+                assert (tile - 1) * k * e + 512 < 1 << 31, (m, n, k, tile)
+                seen.add(tile)
+                for stride in (k + 3, 1 << 22, 1 << 23):   # copied, or read where their own stride allows it
+                    assert lib.ssm_linear_tile(ctypes.byref(product(m, n, k, in8, max(stride, k)))) in (0, tile)
+            if k % 16 == 0 and k * e >= 1 << 22:   # as long as a copy would be: nothing is copied, sums of splits at most
+                assert lib.ssm_linear_workspace_bytes(ctypes.byref(product(m, n, k, in8))) <= m * n * 4 * 512, (m, n, k)
+    assert seen == {64, 128, 256}
+    assert lib.ssm_linear_tile(ctypes.byref(product(8192, 8192, 2048, in8))) == 256
+    assert lib.ssm_linear_tile(ctypes.byref(product(1, 4096, 1024, in8))) == 0
+    assert lib.ssm_linear_tile(ctypes.byref(product(0, 8, 8))) == -1
+    # a stride past the reach of the tile is copied
+    far = product(8192, 8192, 2048, in8, stride=1 << 24)
+    assert lib.ssm_linear_workspace_bytes(ctypes.byref(far)) == 2 * 8192 * 2048 * e
