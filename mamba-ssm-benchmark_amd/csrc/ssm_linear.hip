@@ -54,7 +54,10 @@ __device__ __forceinline__ float lin_act(float z, int act) {
   if (act == kActGelu) return 0.5f * z * (1.0f + erff(z * 0.70710678f));
   return z;
 }
+// From |z| = 128 on the slopes are 0 and 1 to float32's last bit (z e^-z is below its smallest number); a z that float16
+// keeps as an infinity has them too, where infinity times zero would be NaN.  NaN stays.
 __device__ __forceinline__ float lin_slope(float z, int act) {
+  z = z < -128.0f ? -128.0f : z > 128.0f ? 128.0f : z;
   if (act == kActSilu) {
     const float s = sigmoidf(z);
     return s * fmaf(z, 1.0f - s, 1.0f);

@@ -29,3 +29,27 @@ def test_long_rows(dev, MN, K):
     assert len(cols) == 128 and torch.equal(y, (small[0] @ small[1].t()).to(BF16))
     del x, w, t
     torch.cuda.empty_cache()
+
+
+@pytest.mark.parametrize("act", ["silu", "gelu"])
+def test_gradient_where_z_leaves_float16(dev, act):
+    """z = -10^5, which float16 keeps as -inf: the activation and its slope are 0.  z = 10^5: the slope is 1."""
+    x = torch.tensor([[1000.0], [-1000.0], [1.0]], device=dev, dtype=F16).requires_grad_()
+    w = torch.tensor([[-100.0], [0.5]], device=dev, dtype=F16).requires_grad_()
+    b = torch.zeros(2, device=dev, dtype=F16).requires_grad_()
+    y = ssm_scan.linear_act(x, w, b, act)
+    assert y[0, 0] == 0 and y[1, 0] == float("inf")
+    dy = torch.tensor([[2.0, 1.0], [4.0, 1.0], [0.0, 0.0]], device=dev, dtype=F16)
+    dx, dw, db = torch.autograd.grad(y, [x, w, b], dy)
+    # slopes: 0 and 1 (z = 500) of the first row, 1 and 0 (z = -500) of the second
+    assert torch.equal(dx.cpu(), torch.tensor([[0.5], [-400.0], [0.0]], dtype=F16))
+    assert torch.equal(dw.cpu(), torch.tensor([[-4000.0], [1000.0]], dtype=F16))
+    assert torch.equal(db.cpu(), torch.tensor([4.0, 1.0], dtype=F16))
+
+
+@pytest.mark.parametrize("act", ["silu", "gelu"])
+def test_gradient_of_not_a_number(dev, act):
+    x = torch.tensor([[float("nan")], [2.0]], device=dev, dtype=BF16).requires_grad_()
+    w = torch.ones(3, 1, device=dev, dtype=BF16)
+    dx, = torch.autograd.grad(ssm_scan.linear_act(x, w, activation=act), x, torch.ones(2, 3, device=dev, dtype=BF16))
+    assert torch.isnan(dx[0]).all() and torch.isfinite(dx[1]).all()
