@@ -526,8 +526,10 @@ __global__ void __launch_bounds__(256) k_linear_dbias(const LinearDzParams p) {
 }
 
 // ------------------------------------------------------------------ plan and launch
-static bool loadable(const void *data, int64_t stride, int64_t row, int e, int64_t reach) {   // 16 bytes a lane
-  return (uintptr_t)data % 16 == 0 && stride * e % 16 == 0 && row * e % 16 == 0 && stride >= 0 && stride * e <= reach;
+// 16 bytes a lane.  Rows of a transposed operand (k) may not share memory: a load past the last of them has to reach past the
+// matrix's end, where it gives zeros, and not an earlier row again, whose infinity the other operand's zeros make NaN.
+static bool loadable(const void *data, int64_t stride, int64_t row, bool along, int e, int64_t reach) {
+  return (uintptr_t)data % 16 == 0 && stride * e % 16 == 0 && row * e % 16 == 0 && stride >= (along ? 0 : row) && stride * e <= reach;
 }
 // The longest row in bytes whose `rows` fit the descriptor of a tile's loads, 2^31 - 1 bytes: what lies past that comes as
 // zeros.  The last row's loads end within 512 bytes of its first one's begin.
@@ -550,7 +552,7 @@ LinearPlan linear_plan(const GemmParams &p) {
   // 11.0 against 13.1 (64: 14.8 against 14.5).  Tiles are as fast or faster where the weights are more than 48 MB (16 x
   // 16384 x 4096: 25 us against 30) or of many rows (1 x 32768 x 1024: 14.7 against 17.8, e4m3 9.8 against 13.0), unless
   // they would have to be copied first.
-  const bool b_loads = loadable(p.B, p.sb, p.b_along ? p.K : p.N, e, reach_b);
+  const bool b_loads = loadable(p.B, p.sb, p.b_along ? p.K : p.N, p.b_along, e, reach_b);
   if (p.a_along && p.b_along && p.M <= 32 && ((p.N * p.K * e <= 48 << 20 && p.N < 32768) || !b_loads)) {
     l.rows = 1;
     l.tile = 0;
@@ -564,7 +566,8 @@ LinearPlan linear_plan(const GemmParams &p) {
     l.splits = 1;
     while (nb * l.splits < 128 && steps / (8 * l.splits * 2) >= 16) l.splits *= 2;
   } else {
-    if (!loadable(p.A, p.sa, p.a_padded ? unit : p.a_along ? p.K : p.M, e, reach_a)) l.pack_a = p.a_along ? p.M * up(p.K) * e : p.K * up(p.M) * e;
+    if (!loadable(p.A, p.sa, p.a_padded ? unit : p.a_along ? p.K : p.M, p.a_along, e, reach_a))
+      l.pack_a = p.a_along ? p.M * up(p.K) * e : p.K * up(p.M) * e;
     if (!b_loads) l.pack_b = p.b_along ? p.N * up(p.K) * e : p.K * up(p.N) * e;
     const int64_t steps = (p.K * e + 127) / 128;
     // Small tiles split k, up to two workgroups a compute unit and 8 steps each at least, by what it saves (0.3 us a step,

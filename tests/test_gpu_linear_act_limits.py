@@ -53,3 +53,34 @@ def test_gradient_of_not_a_number(dev, act):
     w = torch.ones(3, 1, device=dev, dtype=BF16)
     dx, = torch.autograd.grad(ssm_scan.linear_act(x, w, activation=act), x, torch.ones(2, 3, device=dev, dtype=BF16))
     assert torch.isnan(dx[0]).all() and torch.isfinite(dx[1]).all()
+
+
+@pytest.mark.parametrize("M", [70, 200, 300])
+def test_infinities_in_rows_that_share_their_memory(dev, M):
+    """Broadcast rows of x (in dweight) and of weight (in dx): the sum ends with the last row."""
+    row = torch.ones(1, 256, device=dev, dtype=BF16)
+    row[0, 5] = float("inf")
+    other = torch.ones(72, 256, device=dev, dtype=BF16)
+    w = other.clone().requires_grad_()
+    y = ssm_scan.linear_act(row.expand(M, 256), w)
+    g, = torch.autograd.grad(y, w, torch.ones_like(y))
+    want = torch.full((72, 256), float(M), device=dev)
+    want[:, 5] = float("inf")
+    assert torch.equal(g.float(), want.to(BF16).float())
+    x = other.clone().requires_grad_()
+    y = ssm_scan.linear_act(x, row.expand(M, 256))
+    g, = torch.autograd.grad(y, x, torch.ones_like(y))
+    assert torch.equal(g.float(), want.to(BF16).float())
+
+
+def test_overlapping_rows(dev):
+    """Rows that begin 8 elements apart: a window over one signal."""
+    signal = torch.randn(8 * 69 + 256, device=dev).to(BF16)
+    x = signal.as_strided((70, 256), (8, 1))
+    w, dy = torch.randn(40, 256, device=dev).to(BF16), torch.randn(70, 40, device=dev).to(BF16)
+    got = []
+    for t in (x, x.contiguous()):
+        leaf = w.clone().requires_grad_()
+        y = ssm_scan.linear_act(t, leaf)
+        got.append([y.detach(), *torch.autograd.grad(y, leaf, dy)])
+    assert all(torch.equal(a, b) for a, b in zip(*got))
