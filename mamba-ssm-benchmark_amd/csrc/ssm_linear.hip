@@ -98,12 +98,14 @@ __device__ __forceinline__ void lin_store(OT *dst, int64_t left, const float (&v
 template <typename OT, int W, bool WHOLE>
 __device__ __forceinline__ void lin_epilogue(const GemmParams &p, int64_t m, int64_t n, float (&z)[W]) {
   const int64_t left = p.N - n;
-  if (p.xs) {
+  if (p.xs) {   // exponents apart: the scales' product alone may leave float32 where the result does not
     float ws[W];
     lin_load<float, W, WHOLE>(p.ws + n, left, ws);
-    const float xs = p.xs[m];
+    const float xs = p.xs[m], xm = __builtin_amdgcn_frexp_mantf(xs);
+    const int xe = __builtin_amdgcn_frexp_expf(xs);
 #pragma unroll
-    for (int q = 0; q < W; ++q) z[q] *= xs * ws[q];
+    for (int q = 0; q < W; ++q)
+      z[q] = __builtin_amdgcn_ldexpf(z[q] * (xm * __builtin_amdgcn_frexp_mantf(ws[q])), xe + __builtin_amdgcn_frexp_expf(ws[q]));
   }
   if (p.bias) {
     float b[W];

@@ -84,3 +84,22 @@ def test_overlapping_rows(dev):
         y = ssm_scan.linear_act(t, leaf)
         got.append([y.detach(), *torch.autograd.grad(y, leaf, dy)])
     assert all(torch.equal(a, b) for a, b in zip(*got))
+
+
+@pytest.mark.parametrize("M", [3, 70])
+def test_8bit_scales_whose_product_leaves_float32(dev, M):
+    """The product of the scales alone would be of a few bits, 0 or infinite; the result is none of them.  The largest values: sums
+    are 49 2^21 or 0, exactly, two roundings of float32 and half a step of bfloat16 remain."""
+    K = 512
+    q = torch.full((M, K), 448.0, device=dev)
+    wq = torch.full((16, K), 448.0, device=dev)
+    wq[1::4, ::2] = -448.0     # sums of zero
+    for xs, ws in ((1.3e-25, 1.7e-20), (1.1e-30, 1.9e-12), (3e-38, 1.5e-7), (1.3e25, 1.7e-20), (1.3e20, 1.1e16), (5e30, 7e20)):
+        y = ssm_scan.linear_8bit(q.to(torch.float8_e4m3fn), torch.full((M,), xs, device=dev), wq.to(torch.float8_e4m3fn), torch.full((16,), ws, device=dev))
+        z = 448.0 * wq.double().sum(1).cpu() * torch.tensor(xs).double() * torch.tensor(ws).double()
+        z = z.expand(M, 16)
+        got = y.double().cpu()
+        big = z.abs() > torch.finfo(BF16).max
+        assert torch.isinf(got[big]).all() and (got[z == 0] == 0).all(), (xs, ws)
+        tol = 2.0 ** -8 * z.abs().clamp(min=torch.finfo(BF16).tiny) + 3 * 2.0 ** -24 * z.abs()
+        assert ((got - z).abs()[~big] <= tol[~big]).all(), (xs, ws)
