@@ -103,3 +103,22 @@ def test_8bit_scales_whose_product_leaves_float32(dev, M):
         assert torch.isinf(got[big]).all() and (got[z == 0] == 0).all(), (xs, ws)
         tol = 2.0 ** -8 * z.abs().clamp(min=torch.finfo(BF16).tiny) + 3 * 2.0 ** -24 * z.abs()
         assert ((got - z).abs()[~big] <= tol[~big]).all(), (xs, ws)
+
+
+@pytest.mark.parametrize("io", [BF16, F16])
+def test_gelu_tail(dev, io):
+    """z Phi(z) and its slope for z from -12 to 12, z exact.  A relative error e of erfc's argument is one of z^2 e of Phi (and of
+    the density): e is at most three roundings, and as many again follow, so (z^2 + 4) 2^-22 of each term; then half a step of
+    the result, and for the slope, which is rounded as dz and as dx (weights of one), twice."""
+    z = torch.cat([torch.linspace(-12, 12, 2001), torch.tensor([-5.0, -5.5, -0.0, 0.0])]).to(io)[:, None]
+    x = z.to(dev).requires_grad_()
+    y = ssm_scan.linear_act(x, torch.ones(1, 1, device=dev, dtype=io), activation="gelu")
+    g, = torch.autograd.grad(y, x, torch.ones_like(y))
+    v = z.double()
+    half, tiny = torch.finfo(io).eps / 2, torch.finfo(io).tiny
+    phi, density = 0.5 * torch.erfc(-v * 0.5 ** 0.5), torch.exp(-0.5 * v * v) / (2 * torch.pi) ** 0.5
+    want, slope = v * phi, phi + v * density
+    grow = (v * v + 4) * 2.0 ** -22
+    assert ((y.detach().double().cpu() - want).abs() <= half * want.abs().clamp(min=tiny) + grow * want.abs()).all()
+    tol = 2 * half * slope.abs().clamp(min=tiny) * (1 + half) + grow * (phi + (v * density).abs())
+    assert ((g.double().cpu() - slope).abs() <= tol).all()
