@@ -510,7 +510,8 @@ void no_tangents(std::initializer_list<const Tensor *> ts, const char *what) {
     TORCH_CHECK_NOT_IMPLEMENTED(!t->defined() || !t->_fw_grad(0).defined(), what, " has no forward-mode derivative");
 }
 // The gradients of a backward that has itself no derivative: under create_graph they carry a node over the inputs and
-// the outputs' gradients that refuses, where without one they would pass for constants.
+// the outputs' gradients that refuses, where without one they would pass for constants.  Of d, which are the backward's own
+// tensors: a history set on one that was given would be its owner's too.
 struct Twice : torch::autograd::Node {
   const char *what;
   Twice(const char *w, torch::autograd::edge_list next) : Node(std::move(next)), what(w) {}
@@ -871,13 +872,12 @@ struct AddRnormFn : torch::autograd::Function<AddRnormFn> {
     const auto types = ctx->saved_data["types"].toIntVector();
     const at::ScalarType io = (at::ScalarType)types[0], rt = s.scalar_type();
     variable_list d(4);
-    if (!grads[0].defined()) {   // the sum alone was used
+    if (!grads[0].defined()) {   // the sum alone was used: linear, so a gradient of its gradient is the operations' own
       if (grads[1].defined()) {
         d[0] = cast(grads[1], io);
         d[1] = cast(grads[1], rt);
         if (ctx->needs_input_grad(2)) d[2] = at::zeros(w.sizes(), w.options().dtype((at::ScalarType)types[1]));
       }
-      not_twice(d, grads, "add_rms_norm");
       return d;
     }
     const int64_t C = s.size(-1);
@@ -1112,9 +1112,10 @@ struct LinearFn : torch::autograd::Function<LinearFn> {
       const Launch l(dy);
       l.run_anywhere("ssm_linear_bwd", ssm_linear_bwd, a);
     }
-    variable_list d{need_x ? dx.view(ctx->saved_data["x"].toIntVector()) : dx, dw, db,
-                    residual && ctx->needs_input_grad(bias ? 3 : 2) ? grads[0] : Tensor(), Tensor(), Tensor()};
+    variable_list d{need_x ? dx.view(ctx->saved_data["x"].toIntVector()) : dx, dw, db};
     not_twice(d, grads, "linear_act");
+    // the residual's gradient is the caller's tensor, and keeps its own history
+    d.insert(d.end(), {residual && ctx->needs_input_grad(bias ? 3 : 2) ? grads[0] : Tensor(), Tensor(), Tensor()});
     return d;
   }
 };
