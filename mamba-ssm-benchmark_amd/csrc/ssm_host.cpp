@@ -40,6 +40,7 @@ ssm_tensor view(const Tensor &t) {
   TORCH_CHECK_VALUE(t.dim() <= 3, "expected a tensor of at most 3 dims, got ", t.dim());
   v.data = t.data_ptr();
   for (int64_t i = 0; i < t.dim(); ++i) v.stride[i] = t.stride(i);
+  if (t.dim() && t.size(-1) == 1) v.stride[t.dim() - 1] = 1;   // torch's own may be anything, of a contiguous tensor too
   return v;
 }
 Tensor get(const OptTensor &t) { return t.has_value() ? *t : Tensor(); }

@@ -122,3 +122,23 @@ def test_gelu_tail(dev, io):
     assert ((y.detach().double().cpu() - want).abs() <= half * want.abs().clamp(min=tiny) + grow * want.abs()).all()
     tol = 2 * half * slope.abs().clamp(min=tiny) * (1 + half) + grow * (phi + (v * density).abs())
     assert ((g.double().cpu() - slope).abs() <= tol).all()
+
+
+def test_one_channel_with_any_stride(dev):
+    """(n, 1) tensors whose last stride is n: transposed rows, and what autograd makes of them."""
+    x, w, r, dy = (torch.randn(1, n, device=dev).to(BF16).t() for n in (5, 7, 5, 5))
+    assert x.stride() == (1, 5)
+    assert torch.equal(ssm_scan.linear_act(x, w), ssm_scan.linear_act(x.clone(memory_format=torch.contiguous_format).reshape(5).reshape(5, 1), w.reshape(7).reshape(7, 1)))
+    X, W = torch.randn(5, 16, device=dev).to(BF16).requires_grad_(), torch.randn(1, 16, device=dev).to(BF16).requires_grad_()
+    y = ssm_scan.linear_act(X, W, residual=r)
+    assert torch.equal(y, ssm_scan.linear_act(X, W, residual=r.reshape(5).reshape(5, 1)))
+    a = torch.autograd.grad(ssm_scan.linear_act(X, W, residual=r), [X, W], dy)
+    b = torch.autograd.grad(ssm_scan.linear_act(X, W, residual=r), [X, W], dy.reshape(5).reshape(5, 1))
+    assert all(torch.equal(p, q) for p, q in zip(a, b))
+    (ssm_scan.linear_act(X, W).t().float() @ torch.randn(5, 3, device=dev)).sum().backward()
+    assert torch.isfinite(X.grad).all()
+    q, s = ssm_scan.quantize_rows(x.float())
+    wq, ws = ssm_scan.quantize_rows(w.float())
+    flat = lambda t: t.view(torch.uint8).reshape(-1).clone().reshape(-1, 1).view(torch.float8_e4m3fn)
+    turned = lambda t: t.view(torch.uint8).reshape(1, -1).t().view(torch.float8_e4m3fn)
+    assert torch.equal(ssm_scan.linear_8bit(turned(q), s, turned(wq), ws), ssm_scan.linear_8bit(flat(q), s, flat(wq), ws))

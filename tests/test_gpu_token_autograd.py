@@ -56,3 +56,32 @@ def test_norm_leaves_the_given_gradient_of_the_sum_alone(dev, io, rt):
     dx, = torch.autograd.grad([y, s], [x], [torch.ones_like(y), a * 2], create_graph=True)
     with pytest.raises(RuntimeError, match="twice"):
         dx.sum().backward()
+
+
+def test_one_channel_with_any_stride(dev):
+    def turned(n, dtype=BF16):   # (n, 1) with strides (1, n)
+        return torch.randn(1, n, device=dev).to(dtype).t()
+
+    def flat(t):
+        return t.reshape(-1).reshape(-1, 1)
+
+    x, r, dy = turned(5), turned(5), turned(5)
+    w = torch.ones(1, device=dev)
+    assert x.stride() == (1, 5) and flat(x).stride() == (1, 1)
+    got, want = ssm_scan.add_rms_norm(x, r, w), ssm_scan.add_rms_norm(flat(x), flat(r), w)
+    assert all(torch.equal(a, b) for a, b in zip(got, want))
+    X = flat(x).detach().requires_grad_()
+    a, b = (torch.autograd.grad(ssm_scan.add_rms_norm(X, flat(r), w)[0], X, d)[0] for d in (dy, flat(dy)))
+    assert torch.equal(a, b)
+    for f in (lambda t: ssm_scan.rms_norm_8bit(t, w), ssm_scan.quantize_rows):
+        (q, s), (q2, s2) = f(x), f(flat(x))
+        assert torch.equal(q.float(), q2.float()) and torch.equal(s, s2)
+    tokens = torch.tensor([3, 0, 3, 8, 8], device=dev)
+    table = turned(9).requires_grad_()
+    out = ssm_scan.embedding(tokens, table, 2.0)
+    assert torch.equal(out, ssm_scan.embedding(tokens, flat(table), 2.0))
+    a, b = (torch.autograd.grad(ssm_scan.embedding(tokens, table, 2.0), table, d)[0] for d in (dy, flat(dy)))
+    assert torch.equal(a, b)
+    logits, u = turned(4), torch.rand(4, device=dev)
+    assert (ssm_scan.sample(logits, u)[0] == 0).all()
+    assert torch.equal(ssm_scan.group_norm(x, 1, w), ssm_scan.group_norm(flat(x), 1, w))
