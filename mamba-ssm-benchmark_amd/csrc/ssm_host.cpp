@@ -974,7 +974,7 @@ Tensor embed_backward(const Tensor &dout, const Tensor &tokens, double scale, in
   l.run_anywhere("ssm_embed_bwd", ssm_embed_bwd, a);
   return dw;
 }
-Tensor embed_node(const Tensor &weight, const Tensor &tokens, double scale, at::IntArrayRef shape);
+Tensor embed_node(const Tensor &weight, const Tensor &tokens, double scale, at::IntArrayRef shape, bool layer);
 // The gradient as a node of its own, for derivatives of it: linear in dout, its adjoint is the embedding.
 struct EmbedGradFn : torch::autograd::Function<EmbedGradFn> {
   static Tensor forward(AutogradContext *ctx, const Tensor &dout, const Tensor &tokens, double scale, int64_t V) {
@@ -985,27 +985,30 @@ struct EmbedGradFn : torch::autograd::Function<EmbedGradFn> {
   }
   static variable_list backward(AutogradContext *ctx, variable_list grads) {
     const std::vector<int64_t> shape = ctx->saved_data["shape"].toIntVector();
-    return {embed_node(grads[0], ctx->get_saved_variables()[0], ctx->saved_data["scale"].toDouble(), shape), Tensor(), Tensor(), Tensor()};
+    return {embed_node(grads[0], ctx->get_saved_variables()[0], ctx->saved_data["scale"].toDouble(), shape, false), Tensor(), Tensor(),
+            Tensor()};
   }
 };
 struct EmbedFn : torch::autograd::Function<EmbedFn> {
-  static Tensor forward(AutogradContext *ctx, const Tensor &weight, const Tensor &tokens, double scale, at::IntArrayRef shape) {
-    ctx->save_for_backward({tokens});
+  static Tensor forward(AutogradContext *ctx, const Tensor &weight, const Tensor &tokens, double scale, at::IntArrayRef shape, bool layer) {
+    ctx->save_for_backward({tokens.to(at::kLong).contiguous()});
     ctx->saved_data["scale"] = scale;
     ctx->saved_data["vocab"] = weight.size(0);
-    return embed_forward(tokens, weight, scale, shape);
+    return layer ? at::embedding(weight, tokens) : embed_forward(tokens, weight, scale, shape);
   }
   static variable_list backward(AutogradContext *ctx, variable_list grads) {
     const Tensor tokens = ctx->get_saved_variables()[0];
     const int64_t V = ctx->saved_data["vocab"].toInt();
     const double scale = ctx->saved_data["scale"].toDouble();
     return {needs_grad({&grads[0]}) ? EmbedGradFn::apply(grads[0], tokens, scale, V) : embed_backward(grads[0], tokens, scale, V),
-            Tensor(), Tensor(), Tensor()};
+            Tensor(), Tensor(), Tensor(), Tensor()};
   }
 };
-Tensor embed_node(const Tensor &weight, const Tensor &tokens, double scale, at::IntArrayRef shape) {
-  return EmbedFn::apply(weight, tokens, scale, shape);
+Tensor embed_node(const Tensor &weight, const Tensor &tokens, double scale, at::IntArrayRef shape, bool layer) {
+  return EmbedFn::apply(weight, tokens, scale, shape, layer);
 }
+// nn.Embedding's own lookup, with its check of the ids, and the gradient by sorted tokens.
+Tensor embedding_layer(const Tensor &tokens, const Tensor &weight) { return embed_node(weight, tokens, 1.0, {}, true); }
 Tensor embedding(const Tensor &tokens, const Tensor &weight, double scale) {
   require_gpu({&tokens, &weight});
   one_device(weight, {&tokens});
@@ -1018,7 +1021,7 @@ Tensor embedding(const Tensor &tokens, const Tensor &weight, double scale) {
   if (tokens.numel() == 0) return weight.narrow(0, 0, 0).reshape(shape);   // in weight's graph
   const Tensor t = tokens.to(at::kLong).contiguous();
   if (!needs_grad({&weight})) return embed_forward(t, weight, scale, shape);
-  return EmbedFn::apply(weight, t, scale, at::IntArrayRef(shape));
+  return embed_node(weight, t, scale, shape, false);
 }
 
 // ------------------------------------------------------------------ linear layer with its epilogue
@@ -1346,6 +1349,7 @@ PYBIND11_MODULE(_ssmhost, m) {
   m.def("add_rnorm", torch::wrap_pybind_function(add_rnorm));
   m.def("rnorm8", torch::wrap_pybind_function(rnorm8));
   m.def("embedding", torch::wrap_pybind_function(embedding));
+  m.def("embedding_layer", torch::wrap_pybind_function(embedding_layer));
   m.def("linear_act", torch::wrap_pybind_function(linear_act));
   m.def("linear_8bit", torch::wrap_pybind_function(linear_8bit));
   m.def("sample", torch::wrap_pybind_function(sample));

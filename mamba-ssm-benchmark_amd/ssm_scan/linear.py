@@ -19,7 +19,6 @@ import torch.nn.functional as F
 from torch.autograd import forward_ad
 
 from . import _abi
-from .embed import embedding as scaled_embedding
 
 SPLITS = 8          # token slices of the weight gradient
 MIN_TOKENS = 2048   # below this the plain product already fills the GPU as well
@@ -151,9 +150,9 @@ def embedding(layer, idx):
     the tokens): the same sums as torch's embedding backward, which sorts the indices with
     sizes it reads back on the host -- this one makes no host reads, so a training step that
     contains it can be captured in a HIP graph, and it runs in a fixed order.  Trained with a larger vocabulary, or in
-    16 bits, it is ssm_scan.embedding, which sorts on the GPU and has the same properties (ids outside the vocabulary,
-    at which nn.Embedding ends the process, give zeros there; nn.Embedding itself from 2^27 rows or tokens on and in
-    forward mode)."""
+    16 bits, the rows are looked up by the layer's own function, which checks the ids, and the gradient is
+    ssm_scan.embedding's, which sorts on the GPU and has the same properties (nn.Embedding itself from 2^27 rows or
+    tokens on and in forward mode)."""
     w = layer.weight
     plain = (layer.padding_idx is None and layer.max_norm is None and not layer.scale_grad_by_freq
              and not layer.sparse)
@@ -161,6 +160,6 @@ def embedding(layer, idx):
             and w.shape[0] <= MAX_DENSE_VOCAB and not torch.is_autocast_enabled(w.device.type)):
         return _DenseGradEmbedding.apply(idx, w)
     if (plain and torch.is_grad_enabled() and w.requires_grad and w.is_cuda and w.dtype in _SORTED_TYPES
-            and max(w.shape[0], idx.numel()) < MAX_SORTED and forward_ad._current_level < 0):
-        return scaled_embedding(idx, w)
+            and 0 < idx.numel() < MAX_SORTED and w.shape[0] < MAX_SORTED and forward_ad._current_level < 0):
+        return _abi.host().embedding_layer(idx, w)
     return layer(idx)

@@ -1,0 +1,62 @@
+"""linear.embedding(layer, ids): where it stands in for nn.Embedding, the layer's own call keeps what it does: hooks, an
+overridden forward, transforms, autocast, the check of the ids."""
+
+import pytest
+import torch
+import torch.nn as nn
+
+from ssm_scan import _abi, linear
+
+pytestmark = pytest.mark.gpu
+
+
+def layer(dev, V=5000, D=16, cls=nn.Embedding, dtype=torch.float32):
+    torch.manual_seed(0)
+    return cls(V, D).to(dev).to(dtype)
+
+
+class Scaled(nn.Embedding):
+    def forward(self, idx):
+        return super().forward(idx) * 8.0
+
+
+class Wrap(nn.Module):
+    def __init__(self, m):
+        super().__init__()
+        self.m = m
+
+    def forward(self, idx):
+        return linear.embedding(self.m, idx)
+
+
+@pytest.mark.parametrize("idx_dtype", [torch.int32, torch.int64])
+def test_gradient_is_the_sorted_one(dev, idx_dtype):
+    m, idx = layer(dev), torch.randint(0, 5000, (4, 700), device=dev).to(idx_dtype)
+    dout = torch.randn(4, 700, 16, device=dev)
+    import ssm_scan
+    w = m.weight.detach().requires_grad_()
+    want, = torch.autograd.grad(ssm_scan.embedding(idx, w), w, dout)
+    got, = torch.autograd.grad(linear.embedding(m, idx), m.weight, dout)
+    assert torch.equal(got, want)
+    g, = torch.autograd.grad(linear.embedding(m, idx), m.weight, dout.permute(1, 0, 2).contiguous().permute(1, 0, 2))
+    assert torch.equal(g, want)
+
+
+@pytest.mark.parametrize("dtype,V", [(torch.float32, 5000), (torch.bfloat16, 60)])
+def test_lookup_is_the_layers_own(dev, monkeypatch, dtype, V):
+    """It checks the ids as the layer in evaluation does; its result can be changed in place."""
+    m, idx = layer(dev, V=V, dtype=dtype), torch.randint(0, V, (4, 7), device=dev)
+    host, called = _abi.host(), []
+
+    class Spy:
+        def __getattr__(self, name):
+            called.append(name)
+            return getattr(host, name)
+
+    monkeypatch.setattr(_abi, "host", Spy)
+    out = linear.embedding(m, idx)
+    assert called == ["embedding_layer"] and torch.equal(out, m(idx))
+    out += 1
+    out.mul_(2)
+    g, = torch.autograd.grad(out, m.weight, torch.ones_like(out))
+    assert torch.equal(g[:, 0].float(), 2.0 * torch.bincount(idx.reshape(-1), minlength=V))

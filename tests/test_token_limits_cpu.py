@@ -42,3 +42,14 @@ def test_tiles_of_long_rows_stay_within_32_bits(in8):
     # a stride past the reach of the tile is copied
     far = product(8192, 8192, 2048, in8, stride=1 << 24)
     assert lib.ssm_linear_workspace_bytes(ctypes.byref(far)) == 2 * 8192 * 2048 * e
+
+
+def test_a_trained_layers_ids_are_checked_as_the_layer_does():
+    """The node that stands in for a layer looks its rows up with the layer's own function, which refuses other ids."""
+    w = torch.randn(5000, 4, requires_grad=True)
+    for bad in (-1, 5000):
+        with pytest.raises(IndexError):
+            _abi.host().embedding_layer(torch.tensor([3, bad]), w)
+    idx = torch.tensor([[3, 4999], [0, 3]])
+    out = _abi.host().embedding_layer(idx, w)
+    assert torch.equal(out, w[idx]) and out.requires_grad
