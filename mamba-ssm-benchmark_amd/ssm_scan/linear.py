@@ -123,6 +123,9 @@ def linear_8bit(q, scale, weight, weight_scale, bias=None, activation=None, resi
 
 
 MAX_SORTED = 1 << 27    # rows and tokens of the sorted gradient
+# ... and its fewest tokens.  Forward and gradient in us, sorted / nn.Embedding's: 130000 x 2048 in float32, 512 tokens 249 / 207,
+# 1024 250 / 254, 2048 255 / 343; 50000 x 256 in bfloat16 54 / 49, 57 / 63, 56 / 115.
+MIN_SORTED = 1024
 _SORTED_TYPES = (torch.float32, torch.bfloat16, torch.float16)
 MAX_DENSE_VOCAB = 4096  # vocabularies up to this size take the one-hot product
 
@@ -150,8 +153,8 @@ def embedding(layer, idx):
     the tokens): the same sums as torch's embedding backward, which sorts the indices with
     sizes it reads back on the host -- this one makes no host reads, so a training step that
     contains it can be captured in a HIP graph, and it runs in a fixed order.  Trained with a larger vocabulary, or in
-    16 bits, the rows are looked up by the layer's own function, which checks the ids, and the gradient is
-    ssm_scan.embedding's, which sorts on the GPU and has the same properties (nn.Embedding itself from 2^27 rows or
+    16 bits, on MIN_SORTED tokens and more, the rows are looked up by the layer's own function, which checks the ids, and the gradient is
+    ssm_scan.embedding's, which sorts on the GPU and has the same properties (nn.Embedding itself otherwise, from 2^27 rows or
     tokens on and in forward mode)."""
     w = layer.weight
     plain = (layer.padding_idx is None and layer.max_norm is None and not layer.scale_grad_by_freq
@@ -160,6 +163,6 @@ def embedding(layer, idx):
             and w.shape[0] <= MAX_DENSE_VOCAB and not torch.is_autocast_enabled(w.device.type)):
         return _DenseGradEmbedding.apply(idx, w)
     if (plain and torch.is_grad_enabled() and w.requires_grad and w.is_cuda and w.dtype in _SORTED_TYPES
-            and 0 < idx.numel() < MAX_SORTED and w.shape[0] < MAX_SORTED and forward_ad._current_level < 0):
+            and MIN_SORTED <= idx.numel() < MAX_SORTED and w.shape[0] < MAX_SORTED and forward_ad._current_level < 0):
         return _abi.host().embedding_layer(idx, w)
     return layer(idx)

@@ -45,7 +45,7 @@ def test_gradient_is_the_sorted_one(dev, idx_dtype):
 @pytest.mark.parametrize("dtype,V", [(torch.float32, 5000), (torch.bfloat16, 60)])
 def test_lookup_is_the_layers_own(dev, monkeypatch, dtype, V):
     """It checks the ids as the layer in evaluation does; its result can be changed in place."""
-    m, idx = layer(dev, V=V, dtype=dtype), torch.randint(0, V, (4, 7), device=dev)
+    m, idx = layer(dev, V=V, dtype=dtype), torch.randint(0, V, (40, 70), device=dev)
     host, called = _abi.host(), []
 
     class Spy:
@@ -60,3 +60,13 @@ def test_lookup_is_the_layers_own(dev, monkeypatch, dtype, V):
     out.mul_(2)
     g, = torch.autograd.grad(out, m.weight, torch.ones_like(out))
     assert torch.equal(g[:, 0].float(), 2.0 * torch.bincount(idx.reshape(-1), minlength=V))
+
+
+@pytest.mark.parametrize("n", [1, 1023, 1024])
+def test_short_batches_stay_the_layers(dev, n):
+    """Below 1024 tokens nn.Embedding's own gradient is faster."""
+    m, idx = layer(dev), torch.randint(0, 5000, (n,), device=dev)
+    out = linear.embedding(m, idx)
+    assert (out.grad_fn.name() == "EmbeddingBackward0") == (n < 1024)
+    g, = torch.autograd.grad(out.sum(), m.weight)
+    assert torch.equal(g[:, 0], torch.bincount(idx, minlength=5000).float())
