@@ -15,6 +15,7 @@ own on the matrix cores, with bias, activation and residual in their epilogue.
 """
 
 import torch
+import torch.nn as nn
 import torch.nn.functional as F
 from torch.autograd import forward_ad
 
@@ -95,6 +96,14 @@ def linear(layer, x):
         return layer(x)
 
 
+def plain_call(layer, cls):
+    """Whether layer(x) does what cls.forward does and nothing beside: no subclass (of its weight neither), forward or hook
+    of its own, no transform of torch.func around it.  Where this is not so the engine's own may not take its place."""
+    return (type(layer) is cls and type(layer.weight) in (nn.Parameter, torch.Tensor) and "forward" not in layer.__dict__
+            and not (layer._forward_hooks or layer._forward_pre_hooks or layer._backward_hooks or layer._backward_pre_hooks)
+            and not nn.modules.module._has_any_global_hook() and not torch._C._are_functorch_transforms_active())
+
+
 _ACTIVATIONS = {None: 0, "silu": 1, "gelu": 2}
 
 
@@ -155,7 +164,7 @@ def embedding(layer, idx):
     contains it can be captured in a HIP graph, and it runs in a fixed order.  Trained with a larger vocabulary, or in
     16 bits, on MIN_SORTED tokens and more, the rows are looked up by the layer's own function, which checks the ids, and the gradient is
     ssm_scan.embedding's, which sorts on the GPU and has the same properties (nn.Embedding itself otherwise, from 2^27 rows or
-    tokens on and in forward mode)."""
+    tokens on, in forward mode and within torch.func's transforms; layers with hooks or a forward of their own)."""
     w = layer.weight
     plain = (layer.padding_idx is None and layer.max_norm is None and not layer.scale_grad_by_freq
              and not layer.sparse)
@@ -163,6 +172,7 @@ def embedding(layer, idx):
             and w.shape[0] <= MAX_DENSE_VOCAB and not torch.is_autocast_enabled(w.device.type)):
         return _DenseGradEmbedding.apply(idx, w)
     if (plain and torch.is_grad_enabled() and w.requires_grad and w.is_cuda and w.dtype in _SORTED_TYPES
-            and MIN_SORTED <= idx.numel() < MAX_SORTED and w.shape[0] < MAX_SORTED and forward_ad._current_level < 0):
+            and MIN_SORTED <= idx.numel() < MAX_SORTED and w.shape[0] < MAX_SORTED and forward_ad._current_level < 0
+            and plain_call(layer, nn.Embedding)):
         return _abi.host().embedding_layer(idx, w)
     return layer(idx)

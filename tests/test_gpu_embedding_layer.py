@@ -15,9 +15,42 @@ def layer(dev, V=5000, D=16, cls=nn.Embedding, dtype=torch.float32):
     return cls(V, D).to(dev).to(dtype)
 
 
+def test_hooks_run(dev):
+    idx = torch.randint(0, 5000, (40, 30), device=dev)
+    for dtype in (torch.float32, torch.bfloat16):
+        m = layer(dev, dtype=dtype)
+        want = linear.embedding(m, idx)
+        seen = []
+        h = m.register_forward_hook(lambda mod, args, out: out * 2)
+        assert torch.equal(linear.embedding(m, idx), want * 2)
+        h.remove()
+        h = m.register_forward_pre_hook(lambda mod, args: seen.append(1))
+        assert torch.equal(linear.embedding(m, idx), want) and seen == [1]
+        h.remove()
+        h = m.register_full_backward_hook(lambda mod, gi, go: seen.append(2))
+        linear.embedding(m, idx).sum().backward()
+        assert seen == [1, 2]
+        h.remove()
+        assert torch.equal(linear.embedding(m, idx), want)
+    h = nn.modules.module.register_module_forward_hook(lambda mod, args, out: out * 3 if mod is m else None)
+    try:
+        assert torch.equal(linear.embedding(m, idx), want * 3)
+    finally:
+        h.remove()
+
+
 class Scaled(nn.Embedding):
     def forward(self, idx):
         return super().forward(idx) * 8.0
+
+
+def test_a_forward_of_its_own_runs(dev):
+    idx = torch.randint(0, 5000, (1200,), device=dev)
+    m = layer(dev, cls=Scaled)
+    assert torch.equal(linear.embedding(m, idx), m.weight[idx] * 8.0)
+    m = layer(dev)
+    m.forward = lambda i: nn.Embedding.forward(m, i) + 1.0
+    assert torch.equal(linear.embedding(m, idx), m.weight[idx] + 1.0)
 
 
 class Wrap(nn.Module):
@@ -27,6 +60,16 @@ class Wrap(nn.Module):
 
     def forward(self, idx):
         return linear.embedding(self.m, idx)
+
+
+def test_transforms(dev):
+    m, idx = Wrap(layer(dev)), torch.tensor([4, 4, 4999], device=dev).repeat(400)
+    call = lambda w: torch.func.functional_call(m, {"m.weight": w}, (idx,))
+    w = m.m.weight.detach()
+    g = torch.func.grad(lambda w: call(w).sum())(w)
+    assert g[4].eq(800).all() and g[4999].eq(400).all() and g.sum() == 1200 * 16
+    two = torch.stack([w, 2 * w])
+    assert torch.equal(torch.func.vmap(call)(two), two[:, idx])
 
 
 @pytest.mark.parametrize("idx_dtype", [torch.int32, torch.int64])

@@ -44,6 +44,36 @@ def test_tiles_of_long_rows_stay_within_32_bits(in8):
     assert lib.ssm_linear_workspace_bytes(ctypes.byref(far)) == 2 * 8192 * 2048 * e
 
 
+def test_layers_that_may_be_passed_by():
+    layer = nn.Embedding(10, 4)
+    assert linear.plain_call(layer, nn.Embedding)
+    for register in (layer.register_forward_hook, layer.register_forward_pre_hook, layer.register_full_backward_hook,
+                     layer.register_full_backward_pre_hook):
+        h = register(lambda *a: None)
+        assert not linear.plain_call(layer, nn.Embedding)
+        h.remove()
+        assert linear.plain_call(layer, nn.Embedding)
+    h = nn.modules.module.register_module_forward_hook(lambda *a: None)
+    assert not linear.plain_call(layer, nn.Embedding)
+    h.remove()
+
+    class Own(nn.Embedding):
+        pass
+
+    class Weight(nn.Parameter):   # as a distributed tensor's
+        pass
+
+    assert not linear.plain_call(Own(10, 4), nn.Embedding)
+    layer.weight = Weight(torch.zeros(10, 4))
+    assert not linear.plain_call(layer, nn.Embedding)
+    layer = nn.Embedding(10, 4)
+    layer.forward = lambda i: i
+    assert not linear.plain_call(layer, nn.Embedding)
+    seen = []
+    torch.func.grad(lambda w: (seen.append(linear.plain_call(nn.Embedding(10, 4), nn.Embedding)), w.sum())[1])(torch.ones(3))
+    assert seen == [False]
+
+
 def test_a_trained_layers_ids_are_checked_as_the_layer_does():
     """The node that stands in for a layer looks its rows up with the layer's own function, which refuses other ids."""
     w = torch.randn(5000, 4, requires_grad=True)
