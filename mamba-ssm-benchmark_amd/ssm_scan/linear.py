@@ -172,6 +172,7 @@ def embedding(layer, idx):
             and w.shape[0] <= MAX_DENSE_VOCAB and not torch.is_autocast_enabled(w.device.type)):
         return _DenseGradEmbedding.apply(idx, w)
     if (plain and torch.is_grad_enabled() and w.requires_grad and w.is_cuda and w.dtype in _SORTED_TYPES
+            and (w.dtype != torch.float32 or w.shape[0] > MAX_DENSE_VOCAB)
             and MIN_SORTED <= idx.numel() < MAX_SORTED and w.shape[0] < MAX_SORTED and forward_ad._current_level < 0
             and plain_call(layer, nn.Embedding)):
         return _abi.host().embedding_layer(idx, w)

@@ -72,6 +72,17 @@ def test_transforms(dev):
     assert torch.equal(torch.func.vmap(call)(two), two[:, idx])
 
 
+def test_autocast_leaves_small_tables_to_the_layer(dev):
+    m, idx = layer(dev, V=100), torch.randint(0, 100, (1200,), device=dev)
+    with torch.autocast("cuda", torch.bfloat16):
+        out = linear.embedding(m, idx)
+    assert out.grad_fn.name() == "EmbeddingBackward0"
+    big, idx = layer(dev), torch.randint(0, 5000, (1200,), device=dev)
+    with torch.autocast("cuda", torch.bfloat16):
+        out = linear.embedding(big, idx)
+    assert out.dtype == torch.float32 and out.grad_fn.name() != "EmbeddingBackward0"
+
+
 @pytest.mark.parametrize("idx_dtype", [torch.int32, torch.int64])
 def test_gradient_is_the_sorted_one(dev, idx_dtype):
     m, idx = layer(dev), torch.randint(0, 5000, (4, 700), device=dev).to(idx_dtype)
