@@ -102,6 +102,7 @@ __device__ __forceinline__ SampleSettings sm_settings(const SampleParams &p, int
     r.temperature = 1;
     s.k = 1;
   }
+  if (min_p > 1) s.k = 1;   // no weight reaches it: the first alone, of ties too
   if (s.k < 0 || s.k >= p.V) s.k = 0;
   if (!(s.top_p < 1)) s.top_p = 1;
   r.lowest = min_p > 0 ? log(min_p < 1 ? min_p : 1.0) : -INFINITY;

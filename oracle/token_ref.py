@@ -107,7 +107,8 @@ def sample(logits, u, temperature=1.0, top_k=None, top_p=None, min_p=None):
         if p < 1:
             reach = int(np.argmax(np.cumsum(w) >= p * w.sum())) + 1
             order, w = order[:reach], w[:reach]
-        keep = w >= min(m, 1.0)
+        keep = w >= m
+        keep[0] = True
         order, w = order[keep], w[keep]
         back = np.argsort(order)
         order, w = order[back], w[back]

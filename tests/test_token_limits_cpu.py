@@ -44,6 +44,13 @@ def test_tiles_of_long_rows_stay_within_32_bits(in8):
     assert lib.ssm_linear_workspace_bytes(ctypes.byref(far)) == 2 * 8192 * 2048 * e
 
 
+def test_the_oracles_min_p_above_one_keeps_the_first():
+    logits = torch.tensor([[0.0, 1.0, 1.0, 0.5]])
+    for u in (0.0, 0.6, 0.99):
+        assert token_ref.sample(logits, torch.tensor([u]), min_p=1.5)[0][0] == 1
+        assert token_ref.sample(logits, torch.tensor([u]), min_p=1.0)[0][0] == (1 if u < 0.5 else 2)
+
+
 def test_layers_that_may_be_passed_by():
     layer = nn.Embedding(10, 4)
     assert linear.plain_call(layer, nn.Embedding)
