@@ -1478,7 +1478,7 @@ int ssm_embed_check(const ssm_embed_args *a) {
     return fail(SSM_EINVAL, "empty embedding: n=%lld vocab=%lld dim=%lld", (long long)a->n, (long long)a->vocab, (long long)a->dim);
   if (a->n >= (1LL << 40) || a->vocab > (1LL << 27) || a->dim >= (1LL << 24))
     return fail(SSM_EINVAL, "embedding is too large: n=%lld vocab=%lld dim=%lld", (long long)a->n, (long long)a->vocab, (long long)a->dim);
-  if (!isfinite(a->scale)) return fail(SSM_EINVAL, "scale must be finite");
+  if (!isfinite((float)a->scale)) return fail(SSM_EINVAL, "scale must be finite in float32, got %g", a->scale);
   return ok();
 }
 namespace {

@@ -85,3 +85,11 @@ def test_one_channel_with_any_stride(dev):
     logits, u = turned(4), torch.rand(4, device=dev)
     assert (ssm_scan.sample(logits, u)[0] == 0).all()
     assert torch.equal(ssm_scan.group_norm(x, 1, w), ssm_scan.group_norm(flat(x), 1, w))
+
+
+def test_a_scale_beyond_float32_is_refused(dev):
+    t, w = torch.zeros(3, dtype=torch.long, device=dev), torch.zeros(4, 8, device=dev)
+    for scale in (1e39, -1e300):
+        with pytest.raises(ValueError, match="scale"):
+            ssm_scan.embedding(t, w, scale=scale)
+    assert not ssm_scan.embedding(t, w, scale=3e38).any()

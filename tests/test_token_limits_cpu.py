@@ -44,6 +44,13 @@ def test_tiles_of_long_rows_stay_within_32_bits(in8):
     assert lib.ssm_linear_workspace_bytes(ctypes.byref(far)) == 2 * 8192 * 2048 * e
 
 
+def test_embedding_scales_are_finite_in_float32():
+    fn = _abi.lib().ssm_embed_check
+    for scale in (1e39, -1e300, math.nan):
+        assert fn(ctypes.byref(embed(scale=scale))) == _abi.EINVAL
+    assert fn(ctypes.byref(embed(scale=-3e38))) == _abi.OK
+
+
 def test_the_oracles_min_p_above_one_keeps_the_first():
     logits = torch.tensor([[0.0, 1.0, 1.0, 0.5]])
     for u in (0.0, 0.6, 0.99):
