@@ -848,6 +848,16 @@ void rnorm_checks(const Tensor &x, const Tensor &r, const Tensor &w, const char 
   want("weight", w, {x.size(-1)});
   TORCH_CHECK_TYPE(!w.defined() || at::isFloatingType(w.scalar_type()), "weight must be floating, got ", w.scalar_type());
 }
+// What a launch would refuse, for calls that have no rows to launch for.
+void rnorm_check_empty(const Tensor &x, double eps, const char *what) {
+  ssm_rnorm_args a;
+  memset(&a, 0, sizeof(a));
+  a.rows = 1;
+  a.dim = x.size(-1);
+  a.dtype = a.res_dtype = dtype_code(x.scalar_type());
+  a.eps = eps;
+  check(ssm_rnorm_check(&a), what);
+}
 // y, s, weight
 variable_list add_rnorm_forward(const Tensor &x, const Tensor &r, const Tensor &weight, double eps) {
   const Tensor x2 = rows(x, x.size(-1)), r2 = rows(r, x.size(-1)), w = f32(weight);
@@ -910,6 +920,7 @@ py::tuple add_rnorm(const Tensor &x, const Tensor &r, const Tensor &weight, doub
   rnorm_checks(x, r, weight, "add_rms_norm");
   no_tangents({&x, &r, &weight}, "add_rms_norm");
   if (x.numel() == 0) {  // no rows: empty tensors in the graph of what was given
+    rnorm_check_empty(x, eps, "add_rms_norm");
     const Tensor s = cast(x + r, r.scalar_type());
     return py::make_tuple(cast(s * weight, x.scalar_type()), s);
   }
@@ -927,7 +938,10 @@ py::tuple rnorm8(const Tensor &x, const OptTensor &weight, const OptTensor &resi
   const Tensor q = at::empty(x.sizes(), x.options().dtype(at::kFloat8_e4m3fn)), scale = at::empty(lead, x.options().dtype(at::kFloat));
   Tensor s;
   if (r.defined()) s = at::empty(x.sizes(), r.options());
-  if (x.numel() == 0) return py::make_tuple(q, scale, out(s));
+  if (x.numel() == 0) {
+    rnorm_check_empty(x, eps, what);
+    return py::make_tuple(q, scale, out(s));
+  }
   const Tensor x2 = rows(x, C), r2 = r.defined() ? rows(r, C) : r, w = wt.defined() ? f32(wt) : wt;
   ssm_rnorm_args a = rnorm_args(x2, w, x.scalar_type(), r.defined() ? r.scalar_type() : x.scalar_type(), eps);
   a.x = view(x2); a.residual = view(r2);
@@ -1018,7 +1032,15 @@ Tensor embedding(const Tensor &tokens, const Tensor &weight, double scale) {
   TORCH_CHECK_TYPE(at::isIntegralType(tokens.scalar_type(), false), "tokens must be integers, got ", tokens.scalar_type());
   std::vector<int64_t> shape(tokens.sizes().begin(), tokens.sizes().end());
   shape.push_back(weight.size(1));
-  if (tokens.numel() == 0) return weight.narrow(0, 0, 0).reshape(shape);   // in weight's graph
+  if (tokens.numel() == 0) {   // checked all the same; in weight's graph
+    ssm_embed_args a;
+    memset(&a, 0, sizeof(a));
+    a.n = 1; a.vocab = std::max<int64_t>(1, weight.size(0)); a.dim = weight.size(1);
+    a.dtype = dtype_code(weight.scalar_type());
+    a.scale = scale;
+    check(ssm_embed_check(&a), "embedding");
+    return weight.narrow(0, 0, 0).reshape(shape);
+  }
   const Tensor t = tokens.to(at::kLong).contiguous();
   if (!needs_grad({&weight})) return embed_forward(t, weight, scale, shape);
   return embed_node(weight, t, scale, shape, false);

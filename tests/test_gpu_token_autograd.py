@@ -87,6 +87,23 @@ def test_one_channel_with_any_stride(dev):
     assert torch.equal(ssm_scan.group_norm(x, 1, w), ssm_scan.group_norm(flat(x), 1, w))
 
 
+def test_calls_without_rows_are_checked(dev):
+    x, w = torch.zeros(0, 32, device=dev), torch.ones(32, device=dev)
+    for eps in (-1.0, float("nan")):
+        with pytest.raises(ValueError, match="eps"):
+            ssm_scan.add_rms_norm(x, x, w, eps=eps)
+        with pytest.raises(ValueError, match="eps"):
+            ssm_scan.rms_norm_8bit(x, w, eps=eps)
+    wide = torch.zeros(0, 16385, device=dev)
+    with pytest.raises(ValueError, match="16384"):
+        ssm_scan.add_rms_norm(wide, wide, wide.new_ones(16385))
+    with pytest.raises(ValueError, match="16384"):
+        ssm_scan.quantize_rows(wide)
+    with pytest.raises(ValueError, match="scale"):
+        ssm_scan.embedding(torch.zeros(0, dtype=torch.long, device=dev), torch.zeros(4, 8, device=dev), scale=float("nan"))
+    assert ssm_scan.embedding(torch.zeros(0, dtype=torch.long, device=dev), torch.zeros(0, 8, device=dev)).shape == (0, 8)
+
+
 def test_a_scale_beyond_float32_is_refused(dev):
     t, w = torch.zeros(3, dtype=torch.long, device=dev), torch.zeros(4, 8, device=dev)
     for scale in (1e39, -1e300):
