@@ -861,12 +861,13 @@ void rnorm_check_empty(const Tensor &x, double eps, const char *what) {
 // y, s, weight
 variable_list add_rnorm_forward(const Tensor &x, const Tensor &r, const Tensor &weight, double eps) {
   const Tensor x2 = rows(x, x.size(-1)), r2 = rows(r, x.size(-1)), w = f32(weight);
-  const Tensor y = at::empty(x2.sizes(), x2.options()), s = at::empty(x2.sizes(), r2.options());
+  // results of their own shape: a node's result that is a view cannot be changed in place
+  const Tensor y = at::empty(x.sizes(), x.options()), s = at::empty(x.sizes(), r.options());
   ssm_rnorm_args a = rnorm_args(x2, w, x.scalar_type(), r.scalar_type(), eps);
-  a.x = view(x2); a.residual = view(r2); a.sum = view(s); a.out = view(y);
+  a.x = view(x2); a.residual = view(r2); a.sum = view(s.view(x2.sizes())); a.out = view(y.view(x2.sizes()));
   const Launch l(x);
   l.run_anywhere("ssm_rnorm_fwd", ssm_rnorm_fwd, a);
-  return {y.view(x.sizes()), s.view(x.sizes()), w};
+  return {y, s, w};
 }
 struct AddRnormFn : torch::autograd::Function<AddRnormFn> {
   static variable_list forward(AutogradContext *ctx, const Tensor &x, const Tensor &r, const Tensor &weight, double eps) {
@@ -1090,28 +1091,28 @@ void linear_call(ssm_linear_args &a, const Tensor &bias, const Tensor &r2, const
   const Launch l(o);
   l.run_anywhere("ssm_linear_fwd", ssm_linear_fwd, a);
 }
-// y as rows, x as rows, weight, z before the activation (undefined unless asked for)
+// y (of `shape`, no view: see add_rnorm_forward), x as rows, weight, z before the activation (undefined unless asked for)
 variable_list linear_forward(const Tensor &x, const Tensor &weight, const Tensor &bias, const Tensor &residual, int64_t act,
-                             bool keep) {
+                             at::IntArrayRef shape, bool keep) {
   const int64_t N = weight.size(0);
   const Tensor x2 = rows(x, x.size(-1)), w = unit_last(weight), b = bias.defined() ? bias.contiguous() : bias;
   const Tensor r2 = residual.defined() ? rows(residual, N) : residual;
-  const Tensor o = at::empty({x2.size(0), N}, x.options());
+  const Tensor o = at::empty(shape, x.options()), o2 = o.view({x2.size(0), N});
   const Tensor pre = keep && act ? at::empty({x2.size(0), N}, x.options()) : Tensor();
   ssm_linear_args a = linear_args(x2, w, x.scalar_type(), false, act);
-  linear_call(a, b, r2, o, pre);
+  linear_call(a, b, r2, o2, pre);
   return {o, x2, w, pre};
 }
 struct LinearFn : torch::autograd::Function<LinearFn> {
   static Tensor forward(AutogradContext *ctx, const Tensor &x, const Tensor &weight, const OptTensor &bias, const OptTensor &residual,
                         int64_t act, at::IntArrayRef shape) {
-    const variable_list o = linear_forward(x, weight, get(bias), get(residual), act, true);
+    const variable_list o = linear_forward(x, weight, get(bias), get(residual), act, shape, true);
     ctx->save_for_backward({o[1], o[2], o[3]});
     ctx->saved_data["act"] = act;
     ctx->saved_data["x"] = x.sizes().vec();
     ctx->saved_data["bias"] = bias.has_value();
     ctx->saved_data["residual"] = residual.has_value();
-    return o[0].view(shape);
+    return o[0];
   }
   static variable_list backward(AutogradContext *ctx, variable_list grads) {
     const variable_list t = ctx->get_saved_variables();
@@ -1157,7 +1158,7 @@ Tensor linear_act(const Tensor &x, const Tensor &weight, const OptTensor &bias_,
       if (t->defined()) y = y + *t;
     return y;
   }
-  if (!needs_grad({&x, &weight, &bias, &residual})) return linear_forward(x, weight, bias, residual, act, false)[0].view(shape);
+  if (!needs_grad({&x, &weight, &bias, &residual})) return linear_forward(x, weight, bias, residual, act, shape, false)[0];
   return LinearFn::apply(x, weight, bias_, residual_, act, at::IntArrayRef(shape));
 }
 Tensor linear_8bit(const Tensor &q, const Tensor &scale, const Tensor &wq, const Tensor &wscale, const OptTensor &bias_,

@@ -58,6 +58,28 @@ def test_norm_leaves_the_given_gradient_of_the_sum_alone(dev, io, rt):
         dx.sum().backward()
 
 
+def test_results_change_in_place(dev):
+    x, w, r = leaf(dev, 3, 5, 16), leaf(dev, 8, 16, seed=1), leaf(dev, 3, 5, 8, seed=2)
+    dy = torch.randn(3, 5, 8, device=dev).to(BF16)
+    want = torch.autograd.grad(ssm_scan.linear_act(x, w, activation="gelu", residual=r), [x, w, r], dy)
+    y = ssm_scan.linear_act(x, w, activation="gelu", residual=r)
+    y.mul_(2)
+    y += 1
+    for a, b in zip(torch.autograd.grad(y, [x, w, r], dy / 2), want):
+        assert torch.equal(a, b)
+    x, r, w = leaf(dev, 3, 5, 16), leaf(dev, 3, 5, 16, seed=1), leaf(dev, 16, dtype=F32, seed=2)
+    dy = torch.randn(3, 5, 16, device=dev).to(BF16)
+    want = torch.autograd.grad(ssm_scan.add_rms_norm(x, r, w)[0], [x, r, w], dy)
+    y, s = ssm_scan.add_rms_norm(x, r, w)
+    y.mul_(2)
+    for a, b in zip(torch.autograd.grad(y, [x, r, w], dy / 2), want):
+        assert torch.equal(a, b)
+    y, s = ssm_scan.add_rms_norm(x, r, w)
+    s.add_(1)   # the backward reads it
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        torch.autograd.grad(y, [x], dy)
+
+
 def test_one_channel_with_any_stride(dev):
     def turned(n, dtype=BF16):   # (n, 1) with strides (1, n)
         return torch.randn(1, n, device=dev).to(dtype).t()
