@@ -1198,6 +1198,13 @@ Tensor setting(const char *name, const py::object &v, at::ScalarType type, const
   TORCH_CHECK_TYPE(type == at::kLong ? whole : whole || at::isFloatingType(t.scalar_type()), name, " cannot be of type ", t.scalar_type());
   return t.to(type).contiguous();
 }
+template <typename T> T number(const char *name, const py::object &v) {
+  try {
+    return v.cast<T>();
+  } catch (const py::cast_error &) {
+    TORCH_CHECK_TYPE(false, name, " must be a number or a tensor with one per row, got ", std::string(py::repr(v)));
+  }
+}
 py::tuple sample(const Tensor &logits, const Tensor &u_, const py::object &temperature, const py::object &top_k, const py::object &top_p,
                  const py::object &min_p) {
   require_gpu({&logits, &u_});
@@ -1213,10 +1220,10 @@ py::tuple sample(const Tensor &logits, const Tensor &u_, const py::object &tempe
   const Tensor token = at::empty(lead, logits.options().dtype(at::kLong)), logprob = at::empty(lead, logits.options().dtype(at::kFloat));
   ssm_sample_args a;
   memset(&a, 0, sizeof(a));
-  a.temperature = t.defined() ? 1.0 : temperature.cast<double>();
-  a.top_k = k.defined() || top_k.is_none() ? 0 : top_k.cast<int64_t>();
-  a.top_p = p.defined() || top_p.is_none() ? 1.0 : top_p.cast<double>();
-  a.min_p = m.defined() || min_p.is_none() ? 0.0 : min_p.cast<double>();
+  a.temperature = t.defined() ? 1.0 : number<double>("temperature", temperature);
+  a.top_k = k.defined() || top_k.is_none() ? 0 : number<int64_t>("top_k", top_k);
+  a.top_p = p.defined() || top_p.is_none() ? 1.0 : number<double>("top_p", top_p);
+  a.min_p = m.defined() || min_p.is_none() ? 0.0 : number<double>("min_p", min_p);
   a.vocab = logits.size(-1);
   a.rows = logits.numel() / a.vocab;
   const bool none = a.rows == 0;

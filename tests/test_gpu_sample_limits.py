@@ -41,3 +41,10 @@ def test_the_largest_vocabularies(dev, V):
         assert token.tolist() == at.cpu().gather(-1, torch.from_numpy(want)[:, None])[:, 0].tolist()
         # weights of 2^-S steps, S = 37 at 2^24: 50 of them off by half a step each
         assert (lp.double().cpu() - torch.from_numpy(wp)).abs().max() <= 2.0 ** -23 * 8 + 50 * 2.0 ** -37
+
+
+def test_settings_that_are_no_numbers(dev):
+    logits, u = torch.zeros(2, 10, device=dev), torch.rand(2, device=dev)
+    for kw in (dict(temperature=None), dict(temperature="1"), dict(top_k=2.5), dict(top_k="3"), dict(top_p="x"), dict(min_p=[0.1, 0.2])):
+        with pytest.raises(TypeError, match=next(iter(kw))):
+            ssm_scan.sample(logits, u, **kw)
