@@ -22,15 +22,16 @@ import torch.nn.functional as F
 from .conv import causal_conv1d
 from .delta import gated_delta_rule, gated_delta_step
 from .group_norm import group_norm
-from .linear import linear, linear_act
+from .linear import linear, linear_act, plain_call
 
 
 class GatedDeltaMixer(nn.Module):
     """(B, L, d_model) -> (B, L, d_model).  heads value heads of value_dim, key_heads (dividing heads; all
     by default) of key_dim <= 128.  With a state (init_state) the call continues the sequence and updates
     it, one token per call being the decode step.  A residual (B, L, d_model) is added to the output: in 16 bits
-    (weights, u and residual of one type, no autocast) in the output projection's epilogue.  The states change in place, so such a call is inference: it
-    runs without autograd whatever the grad mode, and its output has no graph."""
+    (weights, u and residual of one type, no autocast, an nn.Linear without hooks) in the output projection's
+    epilogue.  The states change in place, so such a call is inference: it runs without autograd whatever the grad
+    mode, and its output has no graph."""
 
     def __init__(self, d_model, heads, key_dim, value_dim=None, key_heads=None, d_conv=4, dt_min=1e-3, dt_max=0.1):
         super().__init__()
@@ -84,8 +85,9 @@ class GatedDeltaMixer(nn.Module):
         y = group_norm(y.flatten(-2), self.heads, self.norm_weight, gate=z, center=False)
         if residual is None:
             return linear(self.out_proj, y)
-        w = self.out_proj.weight
-        if (w.dtype in (torch.bfloat16, torch.float16) and y.dtype == residual.dtype == w.dtype
-                and not torch.is_autocast_enabled(y.device.type)):
-            return linear_act(y, w, residual=residual)
+        if plain_call(self.out_proj, nn.Linear):
+            w, bias = self.out_proj.weight, self.out_proj.bias
+            if (w.dtype in (torch.bfloat16, torch.float16) and y.dtype == residual.dtype == w.dtype
+                    and (bias is None or bias.dtype == w.dtype) and not torch.is_autocast_enabled(y.device.type)):
+                return linear_act(y, w, bias, residual=residual)
         return residual + linear(self.out_proj, y)
