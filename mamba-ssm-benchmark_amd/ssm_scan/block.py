@@ -260,7 +260,8 @@ class MambaLM(nn.Module):
     def generate(self, prompt, n_new, temperature=1.0, top_k=None, max_len=None, top_p=None, min_p=None, generator=None):
         """Autoregressive sampling (models/lm.py:130-147): prefill, then one step per token.  With top_p, min_p or
         a generator the tokens are drawn by ssm_scan.sample from uniform numbers (the generator's, on the model's
-        device), whose settings may be tensors with one per row; without, by the reference's steps."""
+        device), whose settings may be tensors with one per row; without, by the reference's steps.  Where a row has
+        no distribution (a NaN among its logits) sample gives -1, and the model goes on from token 0 in its place."""
         Bsz, T = prompt.shape
         states = self.init_state(Bsz, max_len or T + n_new, prompt.device)
         logits = self(prompt, states, 0)[:, -1]
@@ -278,7 +279,7 @@ class MambaLM(nn.Module):
                 nxt = torch.multinomial(F.softmax(logits, -1), 1)
             out.append(nxt)
             if t < n_new - 1:
-                logits = self(nxt, states, T + t)[:, -1]
+                logits = self(nxt.clamp(min=0) if own else nxt, states, T + t)[:, -1]
         return torch.cat(out, 1)
 
 

@@ -45,3 +45,16 @@ def test_other_output_projections_of_the_mixer(dev):
         m.out_proj = Doubled(m.out_proj.in_features, 64, bias=False).to(dev).to(BF16)
         m.out_proj.weight = w
         assert torch.equal(m(u, residual=r), r + plain * 2)
+
+
+def test_generate_goes_on_where_a_row_has_no_distribution(dev):
+    """Such a row gives -1, and the model is never given that as an id."""
+    lm = block.MambaLM(n_layers=2, d_model=64).to(dev).eval()
+    prompt = torch.randint(0, 256, (3, 12), device=dev)
+    seen = []
+    lm.register_forward_pre_hook(lambda mod, args: seen.append(args[0]))
+    head = lm.head.register_forward_hook(lambda mod, args, out: out.index_fill(0, torch.tensor([1], device=dev), float("nan")))
+    out = lm.generate(prompt, 5, top_p=0.9)
+    head.remove()
+    assert (out[1, 12:] == -1).all() and (out[[0, 2]] >= 0).all()
+    assert len(seen) == 5 and all(int(s.min()) >= 0 for s in seen)
