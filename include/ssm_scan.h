@@ -471,7 +471,7 @@ typedef struct ssm_rnorm_args {
   ssm_tensor dx;           /* backward */
   ssm_tensor dresidual;    /* backward, optional: equals dx but for its type */
   float *dweight;          /* backward, optional */
-  void *workspace;         /* backward: ssm_rnorm_workspace_bytes() */
+  void *workspace;         /* backward: ssm_rnorm_workspace_bytes(), 16-byte aligned */
   int64_t workspace_bytes;
 } ssm_rnorm_args;
 
@@ -489,14 +489,15 @@ typedef struct ssm_embed_args {
   ssm_tensor out;          /* (n, dim) likewise; forward */
   ssm_tensor dout;         /* (n, dim) likewise; backward */
   void *dweight;           /* (vocab, dim) dense; backward */
-  void *workspace;         /* backward: ssm_embed_workspace_bytes() */
+  void *workspace;         /* backward: ssm_embed_workspace_bytes(), 16-byte aligned */
   int64_t workspace_bytes;
 } ssm_embed_args;
 
 /* ------------------------------------------------------------------ linear layer with its epilogue
  * nn.Linear (models/mamba.py:34-65, models/lm.py:95) with what follows it:
  *   z = x weight^T [x_scale weight_scale] + bias,   out = act(z) + residual
- * in 16 bits, or with 8-bit rows (OCP e4m3, a float32 scale per row of x and of weight).  Sums are float32.
+ * in 16 bits, or with 8-bit rows (OCP e4m3, a float32 scale per row of x and of weight).  Sums are float32; of 8-bit
+ * products 8 at a time are first added in steps of 2^-13 of the largest one's power of two.
  * Backward (16 bits): dz = dout act'(z) with z as the forward stored it in `pre`, dx = dz weight,
  * dweight = dz^T x, dbias = sum over rows of dz; the residual's gradient is dout itself. */
 enum { SSM_ACT_NONE = 0, SSM_ACT_SILU = 1, SSM_ACT_GELU = 2 };   /* GELU: z Phi(z) */
@@ -514,7 +515,7 @@ typedef struct ssm_linear_args {
   ssm_tensor dout;         /* backward: (m, n) */
   ssm_tensor dx, dweight;  /* backward: (m, k), (n, k); each optional */
   void *dbias;             /* backward: (n,) optional */
-  void *workspace;         /* ssm_linear_workspace_bytes() / ssm_linear_bwd_workspace_bytes() */
+  void *workspace;         /* ssm_linear_workspace_bytes() / ssm_linear_bwd_workspace_bytes(), 16-byte aligned */
   int64_t workspace_bytes;
 } ssm_linear_args;
 
@@ -536,7 +537,7 @@ typedef struct ssm_sample_args {
   const int64_t *top_ks;
   int64_t *token;          /* (rows,) */
   float *logprob;          /* (rows,): log of the token's share of the kept mass; NaN with -1 */
-  void *workspace;         /* ssm_sample_workspace_bytes() */
+  void *workspace;         /* ssm_sample_workspace_bytes(), 16-byte aligned */
   int64_t workspace_bytes;
 } ssm_sample_args;
 

@@ -1395,6 +1395,12 @@ int ssm_gnorm_bwd(const ssm_gnorm_args *a, void *stream) {
 }
 
 // ------------------------------------------------------------------ norm with the residual's addition
+// A workspace of the operators below: its parts are read 16 bytes at a time.
+static int space(const void *workspace, int64_t have, int64_t bytes) {
+  if (bytes && (!workspace || have < bytes)) return fail(SSM_ESPACE, "workspace of %lld bytes required", (long long)bytes);
+  if (bytes && (uintptr_t)workspace % 16) return fail(SSM_EINVAL, "the workspace must be 16-byte aligned");
+  return ok();
+}
 static bool io16_32(int dtype) { return dtype == SSM_F32 || dtype == SSM_BF16 || dtype == SSM_F16; }
 static bool lines16(const ssm_tensor &t, int64_t rows, int64_t per) {  // rows of whole 16-byte loads of `per` elements
   return !has(t) || ((uintptr_t)t.data % 16 == 0 && (rows == 1 || t.stride[0] % per == 0));
@@ -1456,8 +1462,7 @@ int ssm_rnorm_bwd(const ssm_rnorm_args *a, void *stream) {
   if (!rc) rc = need({{a->weight, "weight"}});
   if (rc) return rc;
   const int64_t bytes = ssm_rnorm_workspace_bytes(a);
-  if (bytes && (!a->workspace || a->workspace_bytes < bytes))
-    return fail(SSM_ESPACE, "workspace of %lld bytes required", (long long)bytes);
+  if ((rc = space(a->workspace, a->workspace_bytes, bytes))) return rc;
   RnormParams p = rnorm_params(a);
   p.s = a->sum.data; p.ss = a->sum.stride[0];
   p.dy = a->dout.data; p.sdy = a->dout.stride[0];
@@ -1533,8 +1538,7 @@ int ssm_embed_bwd(const ssm_embed_args *a, void *stream) {
   if (rc) return rc;
   if (a->n >= (1LL << 27)) return fail(SSM_EINVAL, "the gradient of %lld tokens is not supported", (long long)a->n);
   const EmbedLayout l = embed_layout(a);
-  if (!a->workspace || a->workspace_bytes < l.bytes())
-    return fail(SSM_ESPACE, "workspace of %lld bytes required", (long long)l.bytes());
+  if ((rc = space(a->workspace, a->workspace_bytes, l.bytes()))) return rc;
   EmbedParams p = embed_params(a);
   p.dout = a->dout.data; p.sd = a->dout.stride[0];
   p.dw = a->dweight;
@@ -1654,8 +1658,7 @@ int ssm_linear_fwd(const ssm_linear_args *a, void *stream) {
   if (!rc && has(a->residual)) rc = gnorm_view(a->residual, "residual");
   if (rc) return rc;
   const int64_t bytes = ssm_linear_workspace_bytes(a);
-  if (bytes && (!a->workspace || a->workspace_bytes < bytes))
-    return fail(SSM_ESPACE, "workspace of %lld bytes required", (long long)bytes);
+  if ((rc = space(a->workspace, a->workspace_bytes, bytes))) return rc;
   hipError_t e = launch_gemm(linear_forward_params(a), a->dtype, a->workspace, (hipStream_t)stream);
   return e == hipSuccess ? ok() : hip_fail(e, "ssm_linear_fwd");
 }
@@ -1668,8 +1671,7 @@ int ssm_linear_bwd(const ssm_linear_args *a, void *stream) {
   if (!rc && has(a->dweight)) rc = gnorm_view(a->dweight, "dweight");
   if (rc) return rc;
   const LinearBwd l = linear_backward_plan(a);
-  if (l.bytes() && (!a->workspace || a->workspace_bytes < l.bytes()))
-    return fail(SSM_ESPACE, "workspace of %lld bytes required", (long long)l.bytes());
+  if ((rc = space(a->workspace, a->workspace_bytes, l.bytes()))) return rc;
   void *products = (char *)a->workspace + l.dz + l.partial;
   hipError_t e = hipSuccess;
   if (l.own_dz || a->dbias) e = launch_linear_dz(l.d, a->dtype, (hipStream_t)stream);
@@ -1726,8 +1728,7 @@ int ssm_sample(const ssm_sample_args *a, void *stream) {
   if (!rc) rc = need({{a->u, "u"}, {a->token, "token"}, {a->logprob, "logprob"}});
   if (rc) return rc;
   const SampleLayout l = sample_layout(a);
-  if (l.bytes() && (!a->workspace || a->workspace_bytes < l.bytes()))
-    return fail(SSM_ESPACE, "workspace of %lld bytes required", (long long)l.bytes());
+  if ((rc = space(a->workspace, a->workspace_bytes, l.bytes()))) return rc;
   SampleParams p{};
   p.R = a->rows; p.V = a->vocab;
   p.logits = a->logits.data; p.sl = a->logits.stride[0];

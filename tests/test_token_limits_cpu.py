@@ -10,7 +10,7 @@ import torch.nn as nn
 
 from oracle import token_ref
 from ssm_scan import _abi, linear
-from test_token_cpu import embed, rnorm
+from test_token_cpu import embed, linear as linear_args, rnorm, sample
 
 
 def product(m, n, k, in8=0, stride=None):
@@ -97,3 +97,20 @@ def test_a_trained_layers_ids_are_checked_as_the_layer_does():
     idx = torch.tensor([[3, 4999], [0, 3]])
     out = _abi.host().embedding_layer(idx, w)
     assert torch.equal(out, w[idx]) and out.requires_grad
+
+
+def test_workspaces_are_aligned():
+    """Refused before anything reaches the device."""
+    lib, t = _abi.lib(), _abi.Tensor(256, (ctypes.c_int64 * 3)(8, 1, 0))
+    big = 1 << 40
+    for call, args in ((lib.ssm_rnorm_bwd, rnorm(sum=t, dout=t, dx=t, weight=256, dweight=256)),
+                       (lib.ssm_embed_bwd, embed(tokens=256, dout=t, dweight=256)),
+                       (lib.ssm_linear_fwd, linear_args(m=100, n=4096, k=4096, out=t)),
+                       (lib.ssm_linear_bwd, linear_args(dout=t, activation=1, pre=256, dx=t)),
+                       (lib.ssm_sample, sample(logits=t, u=256, token=256, logprob=256, vocab=100000))):
+        args.workspace_bytes = big
+        for at in (257, 260, 264):
+            args.workspace = at
+            assert call(ctypes.byref(args), None) == _abi.EINVAL and b"aligned" in lib.ssm_last_error()
+        args.workspace, args.workspace_bytes = 256, 16
+        assert call(ctypes.byref(args), None) == _abi.ESPACE
