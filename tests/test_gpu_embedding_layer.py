@@ -124,3 +124,18 @@ def test_short_batches_stay_the_layers(dev, n):
     assert (out.grad_fn.name() == "EmbeddingBackward0") == (n < 1024)
     g, = torch.autograd.grad(out.sum(), m.weight)
     assert torch.equal(g[:, 0], torch.bincount(idx, minlength=5000).float())
+
+
+def test_derivatives_of_the_layers_gradient(dev):
+    """Of sum of out^3 over 1500 tokens: a token's terms are alike, so c of them are off by c + 16 halves of float32's step at most,
+    relative to the result; c is below 16 here."""
+    m, idx = layer(dev), torch.randint(0, 5000, (1500,), device=dev, generator=torch.Generator(dev).manual_seed(1))
+    r = torch.randn(5000, 16, device=dev)
+    count = torch.bincount(idx, minlength=5000)
+    assert count.max() < 16
+    out = linear.embedding(m, idx)
+    assert out.grad_fn.name() != "EmbeddingBackward0"
+    g, = torch.autograd.grad((out ** 3).sum(), m.weight, create_graph=True)
+    got, = torch.autograd.grad((g * r).sum(), m.weight)
+    want = 6 * count[:, None].double() * m.weight.detach().double() * r.double()
+    assert ((got - want).abs() <= 32 * 2.0 ** -24 * want.abs()).all()
