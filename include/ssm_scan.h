@@ -524,7 +524,8 @@ typedef struct ssm_linear_args {
  * w_i = exp((l_i - max l) / T): of the order by falling logit (ties: the lower index first) the first top_k are kept,
  * of those the shortest prefix with top_p of their mass, of those the ones with w_i >= min_p, and always the first;
  * the token is the first kept index at which the running sum of the kept w, by index, passes u times their sum.
- * T <= 0 (or NaN) takes the first of the order.  A row with a NaN, or with no logit above -inf, gives -1. */
+ * T <= 0 (or NaN) takes the first of the order.  A row with a NaN, or with no logit above -inf, gives -1.
+ * The w are rounded to 2^-S of the largest, S = min(51, 62 - bits of vocab); their sums are exact. */
 typedef struct ssm_sample_args {
   int64_t rows, vocab;
   int32_t dtype;           /* logits: SSM_F32, SSM_BF16 or SSM_F16 */

@@ -2,7 +2,8 @@
 //   z = (x W^T) [xs ws] + bias,   y = act(z) + residual          (8 bits: rows of x and W are q scale)
 //   backward: dz = dy act'(z), dx = dz W, dW = dz^T x, dbias = sum over rows of dz.
 // All products are of the form C[m, n] = sum over k of A(m, k) B(n, k) with each operand stored along k or along its
-// rows; sums are float32 in the matrix cores, z meets bias, activation and residual in float32 and is rounded once.
+// rows; sums are float32 in the matrix cores (e4m3: see Mma<fp8_t>), z meets bias, activation and residual in float32 and is
+// rounded once.
 #include "ssm_device.hpp"
 #include "ssm_internal.hpp"
 #include "ssm_tiles.hpp"
@@ -39,8 +40,9 @@ template <> struct Mma<f16_t> {
     return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(lh8, a), __builtin_bit_cast(lh8, b), c, 0, 0, 0);
   }
 };
-// 128 k of e4m3, scales of one.  The instruction adds 8 products at a time in steps of 2^-13 of the largest one's power
-// of two: what it loses is far below e4m3's own 2^-4 of each factor.
+// 128 k of e4m3, scales of one.  The instruction adds 8 products of consecutive k at a time in steps of 2^-13 of the largest
+// one's power of two (2^3 beside 2^16 is kept, 2^2 lost, in places 0..7 of 128 and no others), and these sums in float32: what
+// is lost is far below e4m3's own 2^-4 of each factor.
 template <> struct Mma<fp8_t> {
   static constexpr int bytes = 32;
   typedef li8 Frag;
@@ -206,11 +208,12 @@ struct LinTile {
 // straight into LDS, of which there are two sets: a step's loads are issued a whole step before they are waited for, one
 // barrier a step, and each matrix instruction's operands are read an instruction group ahead.  An operand that is stored
 // along its rows (both of dw's, dx's weights) is turned by LDS's transposing reads.  Pieces of 16 bytes are dealt over the
-// banks by row (no conflicts counted); a tile's rows and columns come from one die's L2 by the order of the tiles.
+// banks by row (16 bits: no conflicts counted; e4m3, whose operand is two pieces: 4 cycles an LDS instruction); a tile's rows
+// and columns come from one die's L2 by the order of the tiles.
 //
-// Bound by the matrix cores' feed: 8192 x 8192 x 2048 in bf16 226-244 us for dx and dw each (1.13-1.22 PF/s, a library
-// product 1.38), 271-292 us forward, whose 134 MB of z, residual and result are not hidden behind the next tile's product;
-// e4m3 with bias and activation 116-120 us (2.3 PF/s of 2.9).  64 x 64 tiles of 1000-odd rows 9-11 us, latency.
+// 8192 x 8192 x 2048 in bf16 222-244 us for dx and dw each (1.13-1.24 PF/s, a library product 1.38), matrix cores busy 63 % of
+// the cycles; 271-292 us forward, 49 %, whose 268 MB of z and result are not hidden behind the next tile's product; e4m3 4096 x
+// 4096 x 8192 with a residual 116-120 us (2.3 PF/s of 2.9), 53 %.  64 x 64 tiles of 1000-odd rows 9-11 us, latency.
 template <typename T, typename OT, bool AL, bool BL, int BM, int BN, int WM, int WN>
 __global__ void __launch_bounds__(64 * WM * WN) __attribute__((amdgpu_waves_per_eu(BM == 64 ? 4 : 2, BM == 64 ? 4 : 2))) k_linear_tile(const GemmParams p) {
   constexpr int NW = WM * WN, MT = BM / WM / 16, NT = BN / WN / 16, E = sizeof(T);

@@ -118,7 +118,8 @@ def linear_act(x, weight, bias=None, activation=None, residual=None):
 
     x (..., K), weight (N, K), bias (N,), residual (..., N), all bfloat16 or all float16 (float32 layers: linear);
     activation None, "silu" or "gelu" (z Phi(z)).  Sums and the epilogue are float32, the result is rounded once.
-    Differentiable (once, reverse mode) in every tensor; with an activation the forward keeps z, rounded to x's type."""
+    Differentiable (once, reverse mode) in every tensor; with an activation the forward keeps z, rounded to x's type,
+    and the gradient of z is rounded to it on the way to the products."""
     return _abi.host().linear_act(x, weight, bias, residual, _activation(activation))
 
 
@@ -127,7 +128,8 @@ def linear_8bit(q, scale, weight, weight_scale, bias=None, activation=None, resi
 
     q (..., K) with scale (...) as rms_norm_8bit gives them, weight (N, K) with weight_scale (N,) as
     quantize_rows does: torch.float8_e4m3fn rows with a float32 scale each.  bias (N,) and residual (..., N) of
-    dtype.  Products of 8-bit values are exact, sums and the epilogue float32.  Not differentiable."""
+    dtype.  Products of 8-bit values are exact; 8 of consecutive channels are added in steps of 2^-13 of the largest one's
+    power of two, those sums and the epilogue in float32.  Not differentiable."""
     return _abi.host().linear_8bit(q, scale, weight, weight_scale, bias, residual, _activation(activation), dtype)
 
 
@@ -162,9 +164,10 @@ def embedding(layer, idx):
     the tokens): the same sums as torch's embedding backward, which sorts the indices with
     sizes it reads back on the host -- this one makes no host reads, so a training step that
     contains it can be captured in a HIP graph, and it runs in a fixed order.  Trained with a larger vocabulary, or in
-    16 bits, on MIN_SORTED tokens and more, the rows are looked up by the layer's own function, which checks the ids, and the gradient is
-    ssm_scan.embedding's, which sorts on the GPU and has the same properties (nn.Embedding itself otherwise, from 2^27 rows or
-    tokens on, in forward mode and within torch.func's transforms; layers with hooks or a forward of their own)."""
+    16 bits, on MIN_SORTED tokens and more, the rows are looked up by the layer's own function, which checks the
+    ids, and the gradient is ssm_scan.embedding's, which sorts on the GPU and has the same properties.  nn.Embedding
+    itself otherwise: from 2^27 rows or tokens on, in forward mode, within torch.func's transforms, and where the
+    layer has hooks or a forward of its own."""
     w = layer.weight
     plain = (layer.padding_idx is None and layer.max_norm is None and not layer.scale_grad_by_freq
              and not layer.sparse)

@@ -65,13 +65,15 @@ def add_rms_norm(x, residual, weight, eps=1e-5):
 def rms_norm_8bit(x, weight, residual=None, eps=1e-5):
     """(q, scale), with a residual (q, scale, s): add_rms_norm (without a residual: the norm of x) whose rows y are
     written in 8 bits, scale (...,) = max |y| / 448 in float32 (1 for a row of zeros) and q (..., C) = y / scale in
-    torch.float8_e4m3fn.  A NaN stays at its place and does not count for the maximum; a row with an infinity
-    has no other finite values.  Not differentiable: in grad mode, operands that require a gradient are refused."""
+    torch.float8_e4m3fn.  A NaN in a row makes all of it NaN, with a scale of 1; beside an infinity, itself NaN, the row is
+    zeros, with a scale of 1.  Not differentiable: in grad mode, operands that require a gradient are refused."""
     q, scale, s = _abi.host().rnorm8(x, weight, residual, float(eps))
     return (q, scale) if residual is None else (q, scale, s)
 
 
 def quantize_rows(x):
-    """(q, scale): the rows of x (..., C) in 8 bits as rms_norm_8bit writes them, as for the weights of linear_8bit."""
+    """(q, scale): the rows of x (..., C) in 8 bits as rms_norm_8bit writes them, as for the weights of linear_8bit.  A NaN
+    stays at its place and does not count for the maximum; beside an infinity, itself NaN, the row is zeros, with an
+    infinite scale.  Not differentiable, as rms_norm_8bit."""
     q, scale, _ = _abi.host().rnorm8(x, None, None, 0.0)
     return q, scale

@@ -13,8 +13,12 @@ def sample(logits, u, temperature=1.0, top_k=None, top_p=None, min_p=None):
     passes u times their sum; logprob (...) float32 the log of its share of that sum.
 
     u (...) float32 or float64 in [0, 1), as torch.rand gives it.  Each setting is a number or a tensor with one per
-    row: temperature 0 takes the first of the order; top_k None or 0, top_p None or 1, min_p None or 0 keep all.  In a
-    tensor, a temperature below 0 or NaN counts as 0, a top_k below 0 as 0.  A row with a NaN, or with no logit above
-    -inf, gives token -1 and logprob NaN.  Sums are exact or float64, so the same inputs give the same tokens.  Not
-    differentiable: in grad mode, logits that require a gradient are refused."""
+    row, read in float32 (top_k in int64): temperature 0 takes the first of the order; top_k None or 0, top_p None or 1,
+    min_p None or 0 keep all.  In a tensor, a temperature below 0 or NaN counts as 0, a top_k below 0 as 0.  A row with a
+    NaN, or with no logit above -inf, gives token -1 and logprob NaN.  Not differentiable: in grad mode, logits that
+    require a gradient are refused.
+
+    Weights are rounded to 2^-S of the largest, S = min(51, 62 - the bits of V), and their sums are exact, so the same
+    inputs give the same tokens.  V of them may lose V 2^-(S+1) of the largest: 4e-9 at V = 131072, 2.4e-7 at 2^20, 6e-5
+    at 2^24; one below 2^-(S+1) is not drawn."""
     return _abi.host().sample(logits, u, temperature, top_k, top_p, min_p)
